@@ -267,6 +267,110 @@ int rune_engine_set_wait_polls(rune_engine* engine, uint32_t polls);
 int rune_tc_selftest(int32_t M, int32_t N, int32_t K, const float* a_host, const float* b_host,
                      float* c_host, int32_t device);
 
+/* ------------------------------------------------------------------------------------------
+ * Network operators in mixed precision: normalisation, linear layer, gated layer, with their
+ * gradients (the layers of rune/mobius/layers.py:26-67 as differentiable GPU operators).
+ *
+ * They need no engine. All pointers are device memory of CUDA device `device`; matrices are
+ * row-major with unit column stride and the given row stride in elements; outputs and gradients
+ * are contiguous and must not overlap the inputs. The calls only enqueue work on `stream`: they
+ * neither synchronise it nor allocate device memory; scratch is the caller's (`workspace`,
+ * 256-byte aligned, at least the bytes that the *_workspace query writes for the same
+ * arguments; it holds nothing between calls). Sums, statistics and products are accumulated in
+ * float32, in an order that depends on the sizes alone, so equal inputs give equal bits.
+ *
+ * The linear kernels wait for copies with a bounded number of polls. A wait that gives up leaves
+ * the outputs of that call undefined and is reported as RUNE_ERR_CUDA by the next operator call
+ * on the device. */
+#define RUNE_F32 0
+#define RUNE_F16 1
+#define RUNE_BF16 2
+#define RUNE_E4M3 3       /* float8 e4m3 (finite): 448 largest */
+#define RUNE_ACT_NONE -1
+
+typedef struct {
+    int64_t rows, width;
+    int64_t x_stride, residual_stride;
+    int32_t device;
+    int32_t dtype;          /* of x, residual, h: RUNE_F32, RUNE_F16 or RUNE_BF16 */
+    int32_t weight_dtype;   /* dtype or RUNE_F32 */
+    int32_t out_dtype;      /* of y: dtype, or RUNE_E4M3 with `scale` */
+    float eps;
+    int32_t reserved;
+    const void* x;
+    const void* residual;   /* [rows, width] or NULL */
+    const void* weight;     /* [width]; NULL: no normalisation, y = h */
+    void* y;                /* [rows, width] */
+    void* h;                /* [rows, width] x + residual, or NULL */
+    float* scale;           /* [rows], RUNE_E4M3 only: y stands for y * scale */
+    float* rstd;            /* [rows] 1 / sqrt(mean h^2 + eps) for the backward, or NULL */
+} rune_norm_args;
+
+/* h = x + residual; y = h / sqrt(mean(h^2) + eps) * weight over the last axis. */
+int rune_rms_norm(const rune_norm_args* args, void* stream);
+
+typedef struct {
+    int64_t rows, width;
+    int64_t h_stride, dy_stride, dh_stride;
+    int32_t device, dtype, weight_dtype, reserved;
+    const void* h;          /* the forward's x + residual */
+    const void* weight;
+    const float* rstd;
+    const void* dy;
+    const void* dh;         /* gradient that reached h directly, or NULL */
+    void* dx;               /* [rows, width]: of x and of the residual */
+    void* dweight;          /* [width] (weight_dtype), or NULL */
+    void* workspace;
+    int64_t workspace_bytes;
+} rune_norm_grad_args;
+
+int rune_rms_norm_backward(const rune_norm_grad_args* args, void* stream);
+int rune_rms_norm_backward_workspace(const rune_norm_grad_args* args, int64_t* bytes);
+
+typedef struct {
+    int64_t rows, inputs, outputs;
+    int64_t x_stride, weight_stride, residual_stride;
+    int32_t device;
+    int32_t dtype;          /* of x and weight: RUNE_F16, RUNE_BF16 or RUNE_E4M3 */
+    int32_t out_dtype;      /* of y, bias, residual: dtype, or 16-bit for RUNE_E4M3 */
+    int32_t activation;     /* RUNE_ACT_* */
+    int32_t gated;          /* 0: weight [outputs, inputs]; 1: [2 outputs, inputs], gate rows first */
+    int32_t reserved;
+    const void* x;          /* [rows, inputs] */
+    const void* weight;
+    const void* bias;       /* [outputs] or [2 outputs], or NULL */
+    const void* residual;   /* [rows, outputs] or NULL (not with gated) */
+    const float* x_scale;   /* [rows], RUNE_E4M3 only */
+    const float* weight_scale; /* [outputs] or [2 outputs], RUNE_E4M3 only */
+    void* y;                /* [rows, outputs] */
+    float* saved;           /* [rows, outputs] or [rows, 2 outputs]: z for the backward, or NULL */
+    void* workspace;
+    int64_t workspace_bytes;
+} rune_linear_args;
+
+/* z = x weight^T (scaled) + bias; y = act(z) + residual, or gated: y = act(z_gate) z_up. */
+int rune_linear(const rune_linear_args* args, void* stream);
+int rune_linear_workspace(const rune_linear_args* args, int64_t* bytes);
+
+typedef struct {
+    int64_t rows, inputs, outputs;
+    int64_t x_stride, weight_stride, dy_stride;
+    int32_t device, dtype, activation, gated;
+    const void* x;
+    const void* weight;
+    const void* bias;
+    const void* dy;         /* [rows, outputs] */
+    const float* saved;     /* the forward's z; NULL: recomputed from x, weight and bias */
+    void* dx;               /* [rows, inputs], or NULL */
+    void* dweight;          /* as weight, or NULL */
+    void* dbias;            /* as bias, or NULL */
+    void* workspace;
+    int64_t workspace_bytes;
+} rune_linear_grad_args;
+
+int rune_linear_backward(const rune_linear_grad_args* args, void* stream);
+int rune_linear_backward_workspace(const rune_linear_grad_args* args, int64_t* bytes);
+
 /* Release the engine and its device memory. */
 void rune_engine_destroy(rune_engine* engine);
 

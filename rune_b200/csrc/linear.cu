@@ -1,0 +1,1161 @@
+// Linear layers on the tensor cores (tcgen05): the matrix product with scales, bias, activation
+// and residual in its epilogue, the gated pair act(x Wg^T) * (x Wu^T), and their gradients
+// (rune/mobius/layers.py:47-67 trains the same layer by automatic differentiation).
+//
+// One persistent kernel serves every product D[m, n] = sum_k A[m, k] B[n, k]:
+//   forward      A = x   [rows, inputs]  (K-major)    B = W  [outputs, inputs] (K-major)
+//   dx = dz W    A = dz  [rows, outputs] (K-major)    B = W  read MN-major
+//   dW = dz^T x  A = dz  read MN-major                B = x  read MN-major
+// so no operand is ever transposed in memory: the tensor core reads either order from the
+// swizzled tiles that TMA writes. Tails of every size are zeros that TMA fills in.
+//
+// A block works on tiles of 128 rows x bn accumulator columns (bn = 64, 128 or 256):
+//   warp 4    one thread streams tiles of A and B (64 values of k; 128 for e4m3) by TMA into a
+//             ring of as many stages as fit;
+//   warp 5    one thread issues the products into one of two TMEM accumulators;
+//   warps 0-3 the epilogue of the other accumulator: a lane holds a row, so that tiles pass
+//             through shared memory on their way to and from global memory, 128 bytes a row.
+// Every wait is bounded; one that gives up raises the device's wait flag and ends the block.
+
+#include <algorithm>
+#include <atomic>
+#include <mutex>
+
+#include "linear.cuh"
+
+namespace rune {
+namespace ops {
+
+namespace {
+
+enum Mode {
+    kForward,    // y = act(acc + bias) + residual, z saved on request
+    kGated,      // y = act(gate) * up; the tile's columns are half gate, half up
+    kGrad,       // dz = dy act'(acc + bias), column sums of dz
+    kGatedGrad,  // d gate = dy up act'(gate), d up = dy act(gate), column sums
+    kPartial     // float32 sums of one range of k
+};
+
+constexpr int kBM = 128;
+constexpr int kThreads = 192;
+constexpr uint32_t kAStage = kBM * kLineBytes;  // 16 KB
+constexpr uint32_t kWarpBuf = 32 * kLineBytes;  // 4 KB: 32 rows of 64 16-bit or 32 float values
+constexpr int kMaxStages = 8;
+constexpr uint32_t kSmemMax = 227 * 1024;
+
+struct TileParams {
+    int64_t m, n;           // rows and columns of the output (gated: columns of y)
+    int64_t ld_out, ld_in, ld_z;
+    int kblocks, kb_per_split, splits;
+    int tiles_m, tiles_n, bn, stages;
+    int a_mn, b_mn, fp8, act;
+    int vec_out, vec_in, vec_z;  // 16-byte accesses allowed
+    uint32_t idesc;
+    void* out;
+    const void* in;         // residual, or dy
+    const void* bias;
+    const float* x_scale;
+    const float* w_scale;
+    float* z;               // saved z, or the partial sums
+    float* colsum;          // [tiles_m * 4][n or 2n]
+    unsigned* flag;
+};
+
+struct TileShared {
+    unsigned long long full[kMaxStages], empty[kMaxStages];
+    unsigned long long acc_full[2], acc_empty[2], drained;
+    uint32_t tmem;
+    int fail;
+    int issued;             // stages whose copies were issued
+    float bias[2][256], w_scale[2][256];
+};
+
+// buffers of kWarpBuf per epilogue warp, and all shared memory beside the ring
+template <int MODE>
+constexpr uint32_t kWarpBufs = MODE == kGatedGrad ? 2 : 1;
+template <int MODE>
+constexpr uint32_t kFixedSmem =
+    4 * kWarpBufs<MODE> * kWarpBuf + (uint32_t)((sizeof(TileShared) + 127) / 128 * 128);
+
+struct Tile {
+    int mt, nt, split;
+};
+
+// Tiles in groups of 16 tile rows, column by column, so that the blocks at work share a few
+// lines of both operands in L2; the ranges of k of one tile come last.
+__device__ __forceinline__ Tile tile_of(const TileParams& p, int64_t w) {
+    constexpr int G = 16;
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+    Tile t;
+    t.split = (int)(w / tiles);
+    int64_t id = w % tiles;
+    int64_t per = (int64_t)G * p.tiles_n, g = id / per, in = id % per;
+    int gm = (int)min((int64_t)G, p.tiles_m - g * G);
+    t.mt = (int)(g * G + in % gm);
+    t.nt = (int)(in / gm);
+    return t;
+}
+
+// ---- a warp's 32 rows x 64 columns of 16-bit values between global memory and its buffer.
+// Rows are 128-byte lines of eight 16-byte pieces, piece c of row r at c ^ (r & 7), so that both
+// the row-wise accesses of the lanes and the coalesced ones spread over the banks.
+__device__ __forceinline__ uint4* piece(unsigned char* buf, int r, int c) {
+    return reinterpret_cast<uint4*>(buf + r * kLineBytes + ((c ^ (r & 7)) << 4));
+}
+
+template <typename T>
+__device__ __forceinline__ void load_rows(unsigned char* buf, const T* src, int64_t ld,
+                                          int rows, int64_t cols, bool vec, int lane) {
+    if (vec) {
+        const int c = lane & 7;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + (lane >> 3);
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (r < rows && c * 8 < cols)
+                v = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)r * ld + c * 8));
+            *piece(buf, r, c) = v;
+        }
+    } else {
+        for (int r = 0; r < 32; ++r) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int c = lane + 32 * half;
+                T v = from_float<T>(0.0f);
+                if (r < rows && c < cols) v = src[(int64_t)r * ld + c];
+                reinterpret_cast<T*>(piece(buf, r, c >> 3))[c & 7] = v;
+            }
+        }
+    }
+}
+
+// buffer -> global, and on request the sums of the 32 rows of each column
+template <typename T, bool SUMS>
+__device__ __forceinline__ void store_rows(unsigned char* buf, T* dst, int64_t ld, int rows,
+                                           int64_t cols, bool vec, int lane, float* sums) {
+    if (vec) {
+        const int c = lane & 7;
+        float s[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + (lane >> 3);
+            uint4 v = *piece(buf, r, c);
+            if (r < rows && c * 8 < cols)
+                *reinterpret_cast<uint4*>(dst + (int64_t)r * ld + c * 8) = v;
+            if constexpr (SUMS) {
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float2 f = unpack2<T>(w[j]);
+                    s[2 * j] += f.x, s[2 * j + 1] += f.y;
+                }
+            }
+        }
+        if constexpr (SUMS) {
+            if (sums) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    s[j] += __shfl_xor_sync(0xffffffffu, s[j], 8);
+                    s[j] += __shfl_xor_sync(0xffffffffu, s[j], 16);
+                    if (lane < 8 && c * 8 + j < cols) sums[c * 8 + j] = s[j];
+                }
+            }
+        }
+    } else {
+        float s[2] = {0.0f, 0.0f};
+        for (int r = 0; r < 32; ++r) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int c = lane + 32 * half;
+                T v = reinterpret_cast<T*>(piece(buf, r, c >> 3))[c & 7];
+                if (r < rows && c < cols) dst[(int64_t)r * ld + c] = v;
+                if constexpr (SUMS) s[half] += to_float(v);
+            }
+        }
+        if constexpr (SUMS) {
+            if (sums) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+                    if (lane + 32 * half < cols) sums[lane + 32 * half] = s[half];
+            }
+        }
+    }
+}
+
+// a warp's 32 rows x 32 columns of float32, each lane its row, through the buffer to memory
+__device__ __forceinline__ void store_rows32(unsigned char* buf, const float (&v)[32], float* dst,
+                                             int64_t ld, int rows, int64_t cols, bool vec,
+                                             int lane) {
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+        *reinterpret_cast<float4*>(piece(buf, lane, c)) =
+            make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+    __syncwarp();
+    if (vec) {
+        const int c = lane & 7;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + (lane >> 3);
+            if (r < rows && c * 4 < cols)
+                *reinterpret_cast<uint4*>(dst + (int64_t)r * ld + c * 4) = *piece(buf, r, c);
+        }
+    } else {
+        for (int r = 0; r < 32; ++r)
+            if (r < rows && lane < cols)
+                dst[(int64_t)r * ld + lane] =
+                    reinterpret_cast<float*>(piece(buf, r, lane >> 2))[lane & 3];
+    }
+    __syncwarp();
+}
+
+// acc -> z: scales of e4m3 operands and bias of 32 columns
+template <int MODE>
+__device__ __forceinline__ void finish_z(float (&v)[32], const float* bias, const float* w_scale,
+                                         float x_scale, bool scaled) {
+    if (scaled) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = v[j] * (x_scale * w_scale[j]) + bias[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] += bias[j];
+    }
+}
+
+// 32 values of a lane's row to pieces 4 half .. 4 half + 3 of its line
+template <typename T>
+__device__ __forceinline__ void put_row(unsigned char* buf, int lane, int half,
+                                        const float (&v)[32]) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        *piece(buf, lane, half * 4 + c) =
+            make_uint4(pack2<T>(v[8 * c], v[8 * c + 1]), pack2<T>(v[8 * c + 2], v[8 * c + 3]),
+                       pack2<T>(v[8 * c + 4], v[8 * c + 5]), pack2<T>(v[8 * c + 6], v[8 * c + 7]));
+}
+
+template <typename T>
+__device__ __forceinline__ void get_row(unsigned char* buf, int lane, int half, float (&v)[32]) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        uint4 q = *piece(buf, lane, half * 4 + c);
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float2 f = unpack2<T>(w[j]);
+            v[8 * c + 2 * j] = f.x, v[8 * c + 2 * j + 1] = f.y;
+        }
+    }
+}
+
+// One warp's part (32 rows) of a finished tile.
+template <int MODE, typename T>
+__device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uint32_t acc,
+                                         unsigned char* buf, const float* bias,
+                                         const float* w_scale, int warp, int lane) {
+    const int row0 = t.mt * kBM + warp * 32;
+    const int rows = (int)max((int64_t)0, min((int64_t)32, p.m - row0));
+    constexpr bool kPair = MODE == kGated || MODE == kGatedGrad;
+    const int width = kPair ? p.bn / 2 : p.bn;  // output columns of the tile
+    const int64_t col0 = (int64_t)t.nt * width;
+    if constexpr (MODE == kPartial) {
+        for (int c = 0; c < width && col0 + c < p.n; c += 32) {
+            float v[32];
+            tc::tmem_ld32(acc + c, v);
+            store_rows32(buf, v, p.z + ((int64_t)t.split * p.m + row0) * p.ld_z + col0 + c,
+                         p.ld_z, rows, p.n - (col0 + c), true, lane);
+        }
+        return;
+    }
+    const bool scaled = p.x_scale != nullptr;
+    const float xs = scaled && lane < rows ? p.x_scale[row0 + lane] : 0.0f;
+    for (int c = 0; c < width && col0 + c < p.n; c += 64) {
+        const int64_t col = col0 + c, left = p.n - col;
+        if constexpr (MODE == kForward || MODE == kGated) {
+            if (p.z) {  // the pre-activations, in float32
+                for (int part = 0; part < (kPair ? 2 : 1); ++part) {
+                    for (int half = 0; half < 2 && half * 32 < left; ++half) {
+                        const int at = c + part * width + half * 32;
+                        float v[32];
+                        tc::tmem_ld32(acc + at, v);
+                        finish_z<MODE>(v, bias + at, w_scale + at, xs, scaled);
+                        store_rows32(buf, v,
+                                     p.z + (int64_t)row0 * p.ld_z + part * p.n + col + half * 32,
+                                     p.ld_z, rows, left - half * 32, p.vec_z, lane);
+                    }
+                }
+            }
+        }
+        if (MODE == kGrad || MODE == kGatedGrad || (MODE == kForward && p.in)) {
+            load_rows(buf, static_cast<const T*>(p.in) + (int64_t)row0 * p.ld_in + col, p.ld_in,
+                      rows, left, p.vec_in, lane);
+            __syncwarp();
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            float v[32];
+            tc::tmem_ld32(acc + c + half * 32, v);
+            finish_z<MODE>(v, bias + c + half * 32, w_scale + c + half * 32, xs, scaled);
+            if constexpr (MODE == kForward) {
+                with_activation(p.act, [&](auto a) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = act_value<decltype(a)::value>(v[j]);
+                });
+                if (p.in) {
+                    float r[32];
+                    get_row<T>(buf, lane, half, r);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] += r[j];
+                }
+            } else if constexpr (MODE == kGrad) {
+                float d[32];
+                get_row<T>(buf, lane, half, d);
+                with_activation(p.act, [&](auto a) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        float y, da;
+                        act_both<decltype(a)::value>(v[j], y, da);
+                        v[j] = d[j] * da;
+                    }
+                });
+            } else {
+                float u[32];
+                const int at = width + c + half * 32;
+                tc::tmem_ld32(acc + at, u);
+                finish_z<MODE>(u, bias + at, w_scale + at, xs, scaled);
+                if constexpr (MODE == kGated) {
+                    with_activation(p.act, [&](auto a) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            v[j] = act_value<decltype(a)::value>(v[j]) * u[j];
+                    });
+                } else {
+                    float d[32];
+                    get_row<T>(buf, lane, half, d);
+                    with_activation(p.act, [&](auto a) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            float y, da;
+                            act_both<decltype(a)::value>(v[j], y, da);
+                            v[j] = d[j] * u[j] * da;
+                            u[j] = d[j] * y;
+                        }
+                    });
+                    put_row<T>(buf + kWarpBuf, lane, half, u);
+                }
+            }
+            put_row<T>(buf, lane, half, v);
+        }
+        __syncwarp();
+        constexpr bool kSums = MODE == kGrad || MODE == kGatedGrad;
+        const int64_t ncols = kPair ? 2 * p.n : p.n;
+        float* sums = kSums && p.colsum
+                          ? p.colsum + ((int64_t)t.mt * 4 + warp) * ncols + col
+                          : nullptr;
+        T* out = static_cast<T*>(p.out) + (int64_t)row0 * p.ld_out + col;
+        store_rows<T, kSums>(buf, out, p.ld_out, rows, left, p.vec_out, lane, sums);
+        if constexpr (MODE == kGatedGrad)
+            store_rows<T, true>(buf + kWarpBuf, out + p.n, p.ld_out, rows, left, p.vec_out, lane,
+                                sums ? sums + p.n : nullptr);
+        __syncwarp();
+    }
+}
+
+template <int MODE, typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+       const TileParams p) {
+    using namespace tc;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    const uint32_t stage_bytes = kAStage + (uint32_t)p.bn * kLineBytes;
+    unsigned char* bufs = smem + (size_t)p.stages * stage_bytes;
+    auto* sh = reinterpret_cast<TileShared*>(bufs + 4 * kWarpBufs<MODE> * kWarpBuf);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    constexpr bool kPair = MODE == kGated || MODE == kGatedGrad;
+    const int64_t work = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+
+    if (tid == 0) {
+        for (int s = 0; s < p.stages; ++s) {
+            mbar_init(smem_u32(&sh->full[s]), 1);
+            mbar_init(smem_u32(&sh->empty[s]), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(smem_u32(&sh->acc_full[b]), 1);
+            mbar_init(smem_u32(&sh->acc_empty[b]), 128);
+        }
+        mbar_init(smem_u32(&sh->drained), 1);
+        sh->fail = 0;
+        sh->issued = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;");
+    }
+    if (tid == 128) {
+        prefetch_map(&map_a);
+        prefetch_map(&map_b);
+    }
+    if (warp == 5) tmem_alloc(&sh->tmem, 512);
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const uint32_t tmem = sh->tmem;
+    volatile int* fail = &sh->fail;
+
+    if (tid == 128) {
+        // ---- TMA producer
+        int it = 0;
+        for (int64_t w = blockIdx.x; w < work && !*fail; w += gridDim.x) {
+            const Tile t = tile_of(p, w);
+            const int kb0 = t.split * p.kb_per_split;
+            const int kb1 = min(p.kblocks, kb0 + p.kb_per_split);
+            const int m0 = t.mt * kBM, bw = kPair ? p.bn / 2 : p.bn, n0 = t.nt * bw;
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const int st = it % p.stages, use = it / p.stages;
+                if (use > 0 && !mbar_wait(smem_u32(&sh->empty[st]), (use - 1) & 1)) {
+                    *fail = 1;
+                    break;
+                }
+                if (*fail) break;
+                const uint32_t bar = smem_u32(&sh->full[st]);
+                const uint32_t a = smem_u32(smem + (size_t)st * stage_bytes), b = a + kAStage;
+                mbar_expect_tx(bar, stage_bytes);
+                if (p.a_mn) {
+                    tma_load(a, &map_a, m0, kb * 64, bar);
+                    tma_load(a + kMnChunk, &map_a, m0 + 64, kb * 64, bar);
+                } else {
+                    tma_load(a, &map_a, kb * (p.fp8 ? 128 : 64), m0, bar);
+                }
+                if (p.b_mn) {
+                    for (int i = 0; i < p.bn / 64; ++i)
+                        tma_load(b + i * kMnChunk, &map_b, n0 + i * 64, kb * 64, bar);
+                } else {
+                    const int x = kb * (p.fp8 ? 128 : 64);
+                    tma_load(b, &map_b, x, n0, bar);
+                    if (kPair) tma_load(b + bw * kLineBytes, &map_b, x, (int)p.n + n0, bar);
+                }
+                sh->issued = it + 1;
+            }
+        }
+    } else if (tid == 160) {
+        // ---- MMA issuer
+        int it = 0, n_tile = 0;
+        const uint64_t step_a = p.a_mn ? 2048 >> 4 : 32 >> 4;
+        const uint64_t step_b = p.b_mn ? 2048 >> 4 : 32 >> 4;
+        for (int64_t w = blockIdx.x; w < work && !*fail; w += gridDim.x, ++n_tile) {
+            const Tile t = tile_of(p, w);
+            const int kb0 = t.split * p.kb_per_split;
+            const int kb1 = min(p.kblocks, kb0 + p.kb_per_split);
+            const int buf = n_tile & 1, round = n_tile >> 1;
+            if (round > 0 && !mbar_wait(smem_u32(&sh->acc_empty[buf]), (round - 1) & 1)) {
+                *fail = 1;
+                break;
+            }
+            fence_after_sync();
+            const uint32_t acc = tmem + buf * 256;
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const int st = it % p.stages, use = it / p.stages;
+                if (!mbar_wait(smem_u32(&sh->full[st]), use & 1) || *fail) {
+                    *fail = 1;
+                    break;
+                }
+                fence_after_sync();
+                const uint32_t a = smem_u32(smem + (size_t)st * stage_bytes);
+                const uint64_t da = operand_desc(a, p.a_mn);
+                const uint64_t db = operand_desc(a + kAStage, p.b_mn);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const bool more = kb > kb0 || k > 0;
+                    if (p.fp8) mma_f8(acc, da + k * step_a, db + k * step_b, p.idesc, more);
+                    else mma_f16(acc, da + k * step_a, db + k * step_b, p.idesc, more);
+                }
+                mma_commit(smem_u32(&sh->empty[st]));
+            }
+            mma_commit(smem_u32(&sh->acc_full[buf]));
+        }
+    } else if (warp < 4) {
+        // ---- epilogue
+        int n_tile = 0;
+        unsigned char* buf = bufs + warp * kWarpBufs<MODE> * kWarpBuf;
+        for (int64_t w = blockIdx.x; w < work; w += gridDim.x, ++n_tile) {
+            const Tile t = tile_of(p, w);
+            const int b = n_tile & 1, round = n_tile >> 1;
+            if constexpr (MODE != kPartial) {
+                // bias and weight scales of the tile's columns, one set per accumulator
+                const int width = kPair ? p.bn / 2 : p.bn;
+                for (int c = tid; c < p.bn; c += 128) {
+                    const int part = c / width;
+                    const int64_t col = (int64_t)t.nt * width + c % width;
+                    const bool in = col < p.n;
+                    sh->bias[b][c] =
+                        in && p.bias
+                            ? to_float(static_cast<const T*>(p.bias)[part * p.n + col])
+                            : 0.0f;
+                    sh->w_scale[b][c] = in && p.w_scale ? p.w_scale[part * p.n + col] : 0.0f;
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+            }
+            // after a failure the warps still meet at the barrier above for every tile
+            bool ok = !*fail && mbar_wait(smem_u32(&sh->acc_full[b]), round & 1) && !*fail;
+            if (!__all_sync(0xffffffffu, ok)) {
+                *fail = 1;
+                continue;
+            }
+            fence_after_sync();
+            epilogue<MODE, T>(p, t, tmem + b * 256 + ((uint32_t)(warp * 32) << 16), buf,
+                              sh->bias[b], sh->w_scale[b], warp, lane);
+            fence_before_sync();
+            mbar_arrive(smem_u32(&sh->acc_empty[b]));
+        }
+    }
+    __syncthreads();
+    if (*fail) {
+        // let what is in flight land (bounded) before the block's memory goes
+        if (tid == 0) {
+            atomicExch_system(p.flag, 1u);
+            const int issued = sh->issued;
+            for (int i = max(0, issued - p.stages); i < issued; ++i)
+                mbar_wait(smem_u32(&sh->full[i % p.stages]), (i / p.stages) & 1);
+        }
+        if (tid == 160) {
+            mma_commit(smem_u32(&sh->drained));
+            mbar_wait(smem_u32(&sh->drained), 0);
+        }
+        __syncthreads();
+    }
+    fence_before_sync();
+    __syncthreads();
+    if (warp == 5) {
+        fence_after_sync();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// ----------------------------------------------------------------------------- joins
+// y (and z) from the float32 sums of `splits` ranges of k, added in order. Four columns a
+// thread; the sums' lines are padded to four values.
+template <int MODE, typename T>
+__global__ void __launch_bounds__(256) k_join(const TileParams p, const float* __restrict__ part) {
+    constexpr bool kPair = MODE == kGated;
+    const int64_t groups = (p.n + 3) / 4, total = p.m * groups;
+    const int64_t lds = ((kPair ? 2 * p.n : p.n) + 3) / 4 * 4;
+    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
+         i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t row = i / groups, col = (i % groups) * 4;
+        const float xs = p.x_scale ? p.x_scale[row] : 1.0f;
+        auto sum = [&](int64_t c0, float (&v)[4]) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = 0.0f;
+            for (int s = 0; s < p.splits; ++s) {
+                const float* at = part + ((int64_t)s * p.m + row) * lds + c0;
+                if (!kPair || p.n % 4 == 0) {
+                    float4 q = *reinterpret_cast<const float4*>(at);
+                    v[0] += q.x, v[1] += q.y, v[2] += q.z, v[3] += q.w;
+                } else {
+                    for (int j = 0; j < 4 && col + j < p.n; ++j) v[j] += at[j];
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (col + j >= p.n) continue;
+                if (p.w_scale) v[j] *= xs * p.w_scale[c0 + j];
+                if (p.bias) v[j] += to_float(static_cast<const T*>(p.bias)[c0 + j]);
+                if (p.z) p.z[row * p.ld_z + c0 + j] = v[j];
+            }
+        };
+        float v[4], u[4];
+        sum(col, v);
+        if constexpr (kPair) sum(p.n + col, u);
+        with_activation(p.act, [&](auto a) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = act_value<decltype(a)::value>(v[j]);
+        });
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (col + j >= p.n) continue;
+            if constexpr (kPair) v[j] *= u[j];
+            else if (p.in) v[j] += to_float(static_cast<const T*>(p.in)[row * p.ld_in + col + j]);
+        }
+        T* out = static_cast<T*>(p.out) + row * p.ld_out + col;
+        if (p.vec_out && col + 4 <= p.n)
+            *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+        else
+            for (int j = 0; j < 4 && col + j < p.n; ++j) out[j] = from_float<T>(v[j]);
+    }
+}
+
+// ----------------------------------------------------------------------------- elementwise
+// dz from a saved float32 z and dy, and the sums of kGradRows rows of each column. A thread owns
+// one column of a strip; consecutive lanes read consecutive columns.
+constexpr int kGradRows = 64;
+
+template <bool GATED, typename T>
+__global__ void __launch_bounds__(256)
+k_act_grad(int64_t m, int64_t n, const float* __restrict__ z, const T* __restrict__ dy,
+           int64_t ld_dy, T* __restrict__ dz, int64_t ld_dz, int act, float* __restrict__ sums) {
+    const int64_t col = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (col >= n) return;
+    const int64_t nz = GATED ? 2 * n : n;
+    const int64_t strips = (m + kGradRows - 1) / kGradRows;
+    for (int64_t strip = blockIdx.y; strip < strips; strip += gridDim.y) {
+        const int64_t r0 = strip * kGradRows, r1 = min(m, r0 + kGradRows);
+        float s0 = 0.0f, s1 = 0.0f;
+        with_activation(act, [&](auto a) {
+#pragma unroll 8
+            for (int64_t r = r0; r < r1; ++r) {
+                float y, da, d = to_float(dy[r * ld_dy + col]);
+                act_both<decltype(a)::value>(z[r * nz + col], y, da);
+                if constexpr (GATED) {
+                    float g = d * z[r * nz + n + col] * da, u = d * y;
+                    dz[r * ld_dz + col] = from_float<T>(g);
+                    dz[r * ld_dz + n + col] = from_float<T>(u);
+                    s0 += g, s1 += u;
+                } else {
+                    float g = d * da;
+                    dz[r * ld_dz + col] = from_float<T>(g);
+                    s0 += g;
+                }
+            }
+        });
+        if (sums) {
+            sums[strip * nz + col] = s0;
+            if (GATED) sums[strip * nz + n + col] = s1;
+        }
+    }
+}
+
+// sums of kGradRows rows of each column
+template <typename T>
+__global__ void __launch_bounds__(256)
+k_column_sums(int64_t m, int64_t n, const T* __restrict__ x, int64_t ld, float* __restrict__ sums) {
+    const int64_t col = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (col >= n) return;
+    const int64_t strips = (m + kGradRows - 1) / kGradRows;
+    for (int64_t strip = blockIdx.y; strip < strips; strip += gridDim.y) {
+        const int64_t r0 = strip * kGradRows, r1 = min(m, r0 + kGradRows);
+        float s = 0.0f;
+#pragma unroll 8
+        for (int64_t r = r0; r < r1; ++r) s += to_float(x[r * ld + col]);
+        sums[strip * n + col] = s;
+    }
+}
+
+// Copies lines of `cols` values to lines padded to 16 bytes, for operands that TMA cannot read
+// in place. A thread writes 16 bytes; the padding is never read.
+template <typename W>
+__global__ void __launch_bounds__(256)
+k_pack(const W* __restrict__ src, int64_t rows, int64_t cols, int64_t ld, W* __restrict__ dst,
+       int64_t ld_dst) {
+    constexpr int V = 16 / sizeof(W);
+    const int64_t groups = ld_dst / V, total = rows * groups;
+    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
+         i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t r = i / groups, c = (i % groups) * V;
+        __align__(16) W v[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = c + j < cols ? src[r * ld + c + j] : W(0);
+        *reinterpret_cast<uint4*>(dst + r * ld_dst + c) = *reinterpret_cast<uint4*>(v);
+    }
+}
+
+// ----------------------------------------------------------------------------- host
+// Scratch carved from the caller's workspace; with a null base it only adds up the bytes.
+struct Scratch {
+    char* base;
+    int64_t off = 0;
+    template <typename T>
+    T* take(int64_t n) {
+        char* p = base ? base + off : nullptr;
+        off += (n * (int64_t)sizeof(T) + 255) / 256 * 256;
+        return reinterpret_cast<T*>(p);
+    }
+    bool sizing() const { return base == nullptr; }
+};
+
+struct Plan {
+    int bn, splits, kb_per_split, stages;
+};
+
+// Tile width and ranges of k of one product, by a model of its time in cycles: a k-block of 64
+// costs bn * 2 cycles of the tensor core (never less than the 128 + bn lines of shared memory
+// that it reads), an epilogue 10 cycles a column, hidden behind the next tile's products, and a
+// join of splits a launch and its traffic.
+Plan plan_product(int64_t m, int64_t n_cols, int kblocks, bool can_split, bool pair, int sms,
+                  uint32_t fixed) {
+    Plan best{};
+    double best_cost = 0.0;
+    for (int bn : {256, 128, 64}) {
+        if (pair && bn == 64) continue;  // the epilogue takes 64 output columns at a time
+        const int64_t tiles = ((m + kBM - 1) / kBM) * ((n_cols + bn - 1) / bn);
+        const int most = can_split ? (int)std::min<int64_t>(std::max(1, kblocks / 4),
+                                                            std::max<int64_t>(1, sms / tiles))
+                                   : 1;
+        for (int s = 1; s <= most; ++s) {
+            const int per = (kblocks + s - 1) / s;
+            const int splits = (kblocks + per - 1) / per;
+            const double waves = (double)((tiles * splits + sms - 1) / sms);
+            const double main = per * std::max(2.0 * bn, (128.0 + bn) * 1.0);
+            const double epi = 10.0 * bn;
+            double cost = 2000.0 + waves * std::max(main, epi) + std::min(main, epi);
+            if (splits > 1)
+                cost += 5000.0 + (double)m * n_cols * (splits + 1) * 4.0 / 3000.0;
+            if (best.bn == 0 || cost < best_cost) {
+                best_cost = cost;
+                best = {bn, splits, per, 0};
+            }
+        }
+    }
+    const uint32_t stage = kAStage + (uint32_t)best.bn * kLineBytes;
+    best.stages = (int)std::min<uint32_t>(kMaxStages, (kSmemMax - fixed) / stage);
+    return best;
+}
+
+template <int MODE, typename T>
+void launch_tile(const CUtensorMap& a, const CUtensorMap& b, const TileParams& p, int sms,
+                 int device, cudaStream_t stream) {
+    const size_t smem = (size_t)p.stages * (kAStage + (size_t)p.bn * kLineBytes) +
+                        kFixedSmem<MODE>;
+    static std::atomic<uint64_t> allowed{0};  // devices whose limit is raised
+    if (device >= 64 || !(allowed.load(std::memory_order_relaxed) >> device & 1)) {
+        RUNE_CUDA_TRY(cudaFuncSetAttribute(k_tile<MODE, T>,
+                                           cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           (int)kSmemMax));
+        if (device < 64) allowed.fetch_or(uint64_t(1) << device, std::memory_order_relaxed);
+    }
+    const int64_t work = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+    const int grid = (int)std::min<int64_t>(work, sms);
+    k_tile<MODE, T><<<grid, kThreads, smem, stream>>>(a, b, p);
+    RUNE_LAUNCH_CHECK();
+}
+
+// One product D[m, n] = A B^T: operands, epilogue (in p) and scratch for a split.
+struct Product {
+    Matrix a, b;             // K-major: [m, k], [n, k]; MN-major: [k, m], [k, n]
+    bool a_mn = false, b_mn = false;
+    int mode = kForward;
+    int dtype = RUNE_BF16;   // of the operands
+    int out_type = RUNE_BF16;
+    int64_t k = 0;
+};
+
+template <int MODE, typename T>
+void run_mode(const Product& g, TileParams p, Scratch& ws, int device, cudaStream_t stream) {
+    const int sms = sm_count(device);
+    const bool fp8 = g.dtype == RUNE_E4M3, pair = MODE == kGated || MODE == kGatedGrad;
+    const int eb = fp8 ? 1 : 2, line = (int)kLineBytes / eb;
+    const int64_t n_cols = pair ? 2 * p.n : p.n;
+    p.kblocks = (int)((g.k + line - 1) / line);
+    const bool can_split = MODE == kForward || MODE == kGated;
+    Plan plan = plan_product(p.m, n_cols, p.kblocks, can_split, pair, sms, kFixedSmem<MODE>);
+    float* part = nullptr;
+    const int64_t ld_part = (n_cols + 3) / 4 * 4;
+    if (plan.splits > 1) part = ws.take<float>(plan.splits * p.m * ld_part);
+    if (ws.sizing()) return;
+    p.bn = plan.bn;
+    p.splits = plan.splits;
+    p.kb_per_split = plan.kb_per_split;
+    p.stages = plan.stages;
+    p.tiles_m = (int)((p.m + kBM - 1) / kBM);
+    p.a_mn = g.a_mn, p.b_mn = g.b_mn, p.fp8 = fp8;
+    p.idesc = operand_idesc(fp8 ? 0 : g.dtype == RUNE_BF16 ? 1 : 0, g.a_mn, g.b_mn, kBM, p.bn);
+    p.flag = wait_flag(device);
+    const CUtensorMap ma = make_map(g.a, eb, g.a_mn ? 64 : kBM);
+    if (plan.splits == 1) {
+        const int width = pair ? p.bn / 2 : p.bn;
+        p.tiles_n = (int)((p.n + width - 1) / width);
+        const CUtensorMap mb = make_map(g.b, eb, g.b_mn ? 64 : width);
+        launch_tile<MODE, T>(ma, mb, p, sms, device, stream);
+        return;
+    }
+    if constexpr (MODE == kForward || MODE == kGated) {
+        TileParams q = p;  // plain sums over all rows of B, gate and up alike
+        q.n = n_cols;
+        q.tiles_n = (int)((n_cols + p.bn - 1) / p.bn);
+        q.z = part;
+        q.ld_z = ld_part;
+        const CUtensorMap mb = make_map(g.b, eb, g.b_mn ? 64 : p.bn);
+        launch_tile<kPartial, __half>(ma, mb, q, sms, device, stream);
+        const int64_t items = p.m * ((p.n + 3) / 4);
+        const int grid = (int)std::min<int64_t>((items + 255) / 256, (int64_t)sms * 16);
+        k_join<MODE, T><<<grid, 256, 0, stream>>>(p, part);
+        RUNE_LAUNCH_CHECK();
+    }
+}
+
+void run_product(const Product& g, const TileParams& p, Scratch& ws, int device,
+                 cudaStream_t stream) {
+    auto typed = [&](auto t) {
+        using T = decltype(t);
+        switch (g.mode) {
+            case kForward: run_mode<kForward, T>(g, p, ws, device, stream); break;
+            case kGated: run_mode<kGated, T>(g, p, ws, device, stream); break;
+            case kGrad: run_mode<kGrad, T>(g, p, ws, device, stream); break;
+            default: run_mode<kGatedGrad, T>(g, p, ws, device, stream); break;
+        }
+    };
+    if (g.out_type == RUNE_F16) typed(__half());
+    else typed(__nv_bfloat16());
+}
+
+int64_t pad16(int64_t cols, int elem_bytes) {
+    const int64_t v = 16 / elem_bytes;
+    return (cols + v - 1) / v * v;
+}
+
+// the operand itself, or its padded copy in the scratch
+Matrix readable(Matrix m, int elem_bytes, Scratch& ws, cudaStream_t stream) {
+    if (m.rows == 1) m.ld = pad16(m.cols, elem_bytes);  // no second line to reach
+    if (tma_ready(m, elem_bytes)) return m;
+    Matrix d = m;
+    d.ld = pad16(m.cols, elem_bytes);
+    void* to = ws.take<char>(m.rows * d.ld * elem_bytes);
+    d.p = to;
+    if (ws.sizing()) {
+        d.p = reinterpret_cast<const void*>(256);  // any aligned address: only sizes are asked
+        return d;
+    }
+    const int64_t total = m.rows * d.ld * elem_bytes / 16;
+    const int grid = (int)std::min<int64_t>((total + 255) / 256, 1 << 16);
+    if (elem_bytes == 1)
+        k_pack<<<grid, 256, 0, stream>>>(static_cast<const uint8_t*>(m.p), m.rows, m.cols, m.ld,
+                                         static_cast<uint8_t*>(to), d.ld);
+    else
+        k_pack<<<grid, 256, 0, stream>>>(static_cast<const uint16_t*>(m.p), m.rows, m.cols, m.ld,
+                                         static_cast<uint16_t*>(to), d.ld);
+    RUNE_LAUNCH_CHECK();
+    return d;
+}
+
+bool wide16(const void* p, int64_t ld, int64_t cols) {
+    return aligned(p, 16) && ld % 8 == 0 && cols % 8 == 0;
+}
+
+void forward(const rune_linear_args& a, Scratch& ws, cudaStream_t stream) {
+    const int eb = dtype_bytes(a.dtype);
+    const int64_t n_all = a.gated ? 2 * a.outputs : a.outputs;
+    Product g;
+    g.a = readable({a.x, a.rows, a.inputs, a.x_stride}, eb, ws, stream);
+    g.b = readable({a.weight, n_all, a.inputs, a.weight_stride}, eb, ws, stream);
+    g.mode = a.gated ? kGated : kForward;
+    g.dtype = a.dtype;
+    g.out_type = a.out_dtype;
+    g.k = a.inputs;
+    TileParams p{};
+    p.m = a.rows, p.n = a.outputs;
+    p.act = a.activation;
+    p.out = a.y, p.ld_out = a.outputs;
+    p.vec_out = wide16(a.y, a.outputs, a.outputs);
+    p.in = a.residual, p.ld_in = a.residual_stride;
+    p.vec_in = a.residual && wide16(a.residual, a.residual_stride, a.outputs);
+    p.bias = a.bias;
+    p.x_scale = a.x_scale, p.w_scale = a.weight_scale;
+    p.z = a.saved, p.ld_z = n_all;
+    p.vec_z = aligned(a.saved, 16) && a.outputs % 4 == 0;
+    run_product(g, p, ws, a.device, stream);
+}
+
+void backward(const rune_linear_grad_args& a, Scratch& ws, cudaStream_t stream) {
+    const int64_t n_all = a.gated ? 2 * a.outputs : a.outputs;
+    const bool plain = !a.gated && a.activation == RUNE_ACT_NONE;
+    const bool half = a.dtype == RUNE_F16, want_dz = a.dx || a.dweight;
+    // the operands that more than one product reads, readable by TMA
+    Matrix x{a.x, a.rows, a.inputs, a.x_stride}, w{a.weight, n_all, a.inputs, a.weight_stride};
+    const bool recompute = !plain && !a.saved;
+    if (recompute || a.dweight) x = readable(x, 2, ws, stream);
+    if (recompute || a.dx) w = readable(w, 2, ws, stream);
+    // dz and the parts of dbias
+    Matrix dz{a.dy, a.rows, n_all, a.dy_stride};
+    float* sums = nullptr;
+    int64_t parts = 0;
+    const int64_t strips = (a.rows + kGradRows - 1) / kGradRows;
+    if (plain) {
+        if (want_dz) dz = readable(dz, 2, ws, stream);
+        if (a.dbias) {
+            parts = strips;
+            sums = ws.take<float>(parts * n_all);
+            if (!ws.sizing()) {
+                dim3 grid((unsigned)((n_all + 255) / 256),
+                          (unsigned)std::min<int64_t>(strips, 65535));
+                if (half)
+                    k_column_sums<<<grid, 256, 0, stream>>>(
+                        a.rows, n_all, static_cast<const __half*>(a.dy), a.dy_stride, sums);
+                else
+                    k_column_sums<<<grid, 256, 0, stream>>>(
+                        a.rows, n_all, static_cast<const __nv_bfloat16*>(a.dy), a.dy_stride,
+                        sums);
+                RUNE_LAUNCH_CHECK();
+            }
+        }
+    } else {
+        dz.ld = pad16(n_all, 2);
+        uint16_t* to = ws.take<uint16_t>(a.rows * dz.ld);
+        dz.p = to;
+        if (a.saved) {
+            parts = strips;
+            if (a.dbias) sums = ws.take<float>(parts * n_all);
+            if (!ws.sizing()) {
+                dim3 grid((unsigned)((a.outputs + 255) / 256),
+                          (unsigned)std::min<int64_t>(strips, 65535));
+                auto go = [&](auto t) {
+                    using T = decltype(t);
+                    auto* dy = static_cast<const T*>(a.dy);
+                    auto* out = reinterpret_cast<T*>(to);
+                    if (a.gated)
+                        k_act_grad<true, T><<<grid, 256, 0, stream>>>(
+                            a.rows, a.outputs, a.saved, dy, a.dy_stride, out, dz.ld,
+                            a.activation, sums);
+                    else
+                        k_act_grad<false, T><<<grid, 256, 0, stream>>>(
+                            a.rows, a.outputs, a.saved, dy, a.dy_stride, out, dz.ld,
+                            a.activation, sums);
+                };
+                if (half) go(__half());
+                else go(__nv_bfloat16());
+                RUNE_LAUNCH_CHECK();
+            }
+        } else {
+            const int64_t tiles_m = (a.rows + kBM - 1) / kBM;
+            parts = tiles_m * 4;
+            if (a.dbias) sums = ws.take<float>(parts * n_all);
+            Product g;
+            g.a = x, g.b = w;
+            g.mode = a.gated ? kGatedGrad : kGrad;
+            g.dtype = g.out_type = a.dtype;
+            g.k = a.inputs;
+            TileParams p{};
+            p.m = a.rows, p.n = a.outputs;
+            p.act = a.activation;
+            p.out = to, p.ld_out = dz.ld;
+            p.vec_out = !a.gated || a.outputs % 8 == 0;
+            p.in = a.dy, p.ld_in = a.dy_stride;
+            p.vec_in = wide16(a.dy, a.dy_stride, a.outputs);
+            p.bias = a.bias;
+            p.colsum = sums;
+            run_product(g, p, ws, a.device, stream);
+        }
+        if (ws.sizing()) dz.p = reinterpret_cast<const void*>(256);
+    }
+    if (a.dbias && !ws.sizing())
+        sum_partials(sums, parts, n_all, a.dbias, a.dtype, stream);
+    if (a.dx) {
+        Product g;
+        g.a = dz, g.b = w;
+        g.b_mn = true;
+        g.dtype = g.out_type = a.dtype;
+        g.k = n_all;
+        TileParams p{};
+        p.m = a.rows, p.n = a.inputs;
+        p.act = RUNE_ACT_NONE;
+        p.out = a.dx, p.ld_out = a.inputs;
+        p.vec_out = wide16(a.dx, a.inputs, a.inputs);
+        run_product(g, p, ws, a.device, stream);
+    }
+    if (a.dweight) {
+        Product g;
+        g.a = dz, g.b = x;
+        g.a_mn = g.b_mn = true;
+        g.dtype = g.out_type = a.dtype;
+        g.k = a.rows;
+        TileParams p{};
+        p.m = n_all, p.n = a.inputs;
+        p.act = RUNE_ACT_NONE;
+        p.out = a.dweight, p.ld_out = a.inputs;
+        p.vec_out = wide16(a.dweight, a.inputs, a.inputs);
+        run_product(g, p, ws, a.device, stream);
+    }
+}
+
+constexpr int64_t kMaxSize = INT32_MAX - 512;  // tile coordinates are 32-bit
+
+void check_sizes(int64_t rows, int64_t inputs, int64_t outputs, int gated, int act) {
+    require(rows >= 0 && rows <= kMaxSize, "rows out of range");
+    require(inputs >= 1 && inputs <= kMaxSize && outputs >= 1 && outputs <= kMaxSize / 2,
+            "inputs or outputs out of range");
+    require(act == RUNE_ACT_NONE || act == RUNE_ACT_TANH || act == RUNE_ACT_SILU ||
+                act == RUNE_ACT_GELU,
+            "unknown activation");
+    require(!gated || act != RUNE_ACT_NONE, "a gated layer needs an activation");
+}
+
+void check_linear(const rune_linear_args& a) {
+    check_sizes(a.rows, a.inputs, a.outputs, a.gated, a.activation);
+    const bool fp8 = a.dtype == RUNE_E4M3;
+    require(fp8 || a.dtype == RUNE_F16 || a.dtype == RUNE_BF16,
+            "a linear layer takes float16, bfloat16 or e4m3 operands");
+    require(fp8 ? a.out_dtype == RUNE_F16 || a.out_dtype == RUNE_BF16 : a.out_dtype == a.dtype,
+            "the output has the operands' 16-bit type, or is 16-bit for e4m3");
+    require(!!a.x_scale == fp8 && !!a.weight_scale == fp8,
+            "x_scale and weight_scale go with e4m3 operands, both of them");
+    require(!(a.gated && a.residual), "a gated layer takes no residual");
+    require(a.rows == 0 || (a.x && a.weight && a.y), "null argument");
+}
+
+void check_grad(const rune_linear_grad_args& a) {
+    check_sizes(a.rows, a.inputs, a.outputs, a.gated, a.activation);
+    require(a.dtype == RUNE_F16 || a.dtype == RUNE_BF16,
+            "gradients take float16 or bfloat16 operands");
+    require(a.rows == 0 || (a.x && a.weight && a.dy), "null argument");
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                 const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+    static EncodeTiled fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found{};
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000,
+                                             cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    if (!fn) throw Error(RUNE_ERR_CUDA, "the CUDA driver has no cuTensorMapEncodeTiled");
+    return fn;
+}
+
+std::mutex g_flag_mutex;
+constexpr int kMaxDevices = 64;
+std::atomic<unsigned*> g_flag_host[kMaxDevices];
+unsigned* g_flag_dev[kMaxDevices];
+
+}  // namespace
+
+CUtensorMap make_map(const Matrix& m, int elem_bytes, int box_rows) {
+    CUtensorMap map;
+    const cuuint64_t dims[2] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)(m.ld * elem_bytes)};
+    const cuuint32_t box[2] = {kLineBytes / (cuuint32_t)elem_bytes, (cuuint32_t)box_rows};
+    const cuuint32_t step[2] = {1, 1};
+    CUresult r = encode_tiled()(
+        &map, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2,
+        const_cast<void*>(m.p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        throw Error(RUNE_ERR_INVALID,
+                    "an operand cannot be described to TMA (status " + std::to_string(r) + ")");
+    return map;
+}
+
+unsigned* wait_flag(int device) {
+    if (device < 0 || device >= kMaxDevices)
+        throw Error(RUNE_ERR_INVALID, "device index out of range");
+    if (!g_flag_host[device].load(std::memory_order_acquire)) {
+        std::lock_guard<std::mutex> lock(g_flag_mutex);
+        if (!g_flag_host[device].load(std::memory_order_relaxed)) {
+            // allowed while another thread, or this one, captures a graph
+            cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+            RUNE_CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode));
+            unsigned* host = nullptr;
+            cudaError_t e = cudaHostAlloc(&host, sizeof(unsigned),
+                                          cudaHostAllocMapped | cudaHostAllocPortable);
+            if (e == cudaSuccess) {
+                *host = 0;
+                e = cudaHostGetDevicePointer(&g_flag_dev[device], host, 0);
+            }
+            cudaThreadExchangeStreamCaptureMode(&mode);
+            RUNE_CUDA_TRY(e);
+            g_flag_host[device].store(host, std::memory_order_release);
+        }
+    }
+    return g_flag_dev[device];
+}
+
+void check_waits(int device) {
+    if (device < 0 || device >= kMaxDevices) return;
+    volatile unsigned* host = g_flag_host[device].load(std::memory_order_acquire);
+    if (host && *host) {
+        *host = 0;
+        throw Error(RUNE_ERR_CUDA, "A device-side copy of an earlier linear operator did not "
+                                   "complete in time; the results of that call are invalid.");
+    }
+}
+
+}  // namespace ops
+}  // namespace rune
+
+using namespace rune;
+using namespace rune::ops;
+
+extern "C" {
+
+int rune_linear_workspace(const rune_linear_args* args, int64_t* bytes) {
+    if (!args || !bytes) {
+        set_error("null argument");
+        return RUNE_ERR_INVALID;
+    }
+    const rune_linear_args a = *args;
+    return guarded(a.device, [&] {
+        check_linear(a);
+        Scratch ws{nullptr};
+        if (a.rows > 0) forward(a, ws, nullptr);
+        *bytes = ws.off;
+    });
+}
+
+int rune_linear(const rune_linear_args* args, void* stream_) {
+    if (!args) {
+        set_error("null argument");
+        return RUNE_ERR_INVALID;
+    }
+    const rune_linear_args a = *args;
+    auto stream = static_cast<cudaStream_t>(stream_);
+    return guarded(a.device, [&] {
+        check_linear(a);
+        if (a.rows == 0) return;
+        check_waits(a.device);
+        Scratch need{nullptr};
+        forward(a, need, stream);
+        require(need.off == 0 || (a.workspace && aligned(a.workspace, 256) &&
+                                  a.workspace_bytes >= need.off),
+                "the workspace is too small or not 256-byte aligned");
+        Scratch ws{need.off ? static_cast<char*>(a.workspace) : reinterpret_cast<char*>(256)};
+        forward(a, ws, stream);
+    });
+}
+
+int rune_linear_backward_workspace(const rune_linear_grad_args* args, int64_t* bytes) {
+    if (!args || !bytes) {
+        set_error("null argument");
+        return RUNE_ERR_INVALID;
+    }
+    const rune_linear_grad_args a = *args;
+    return guarded(a.device, [&] {
+        check_grad(a);
+        Scratch ws{nullptr};
+        if (a.rows > 0) backward(a, ws, nullptr);
+        *bytes = ws.off;
+    });
+}
+
+int rune_linear_backward(const rune_linear_grad_args* args, void* stream_) {
+    if (!args) {
+        set_error("null argument");
+        return RUNE_ERR_INVALID;
+    }
+    const rune_linear_grad_args a = *args;
+    auto stream = static_cast<cudaStream_t>(stream_);
+    return guarded(a.device, [&] {
+        check_grad(a);
+        const int64_t n_all = a.gated ? 2 * a.outputs : a.outputs;
+        if (a.rows == 0) {
+            if (a.dweight)
+                RUNE_CUDA_TRY(cudaMemsetAsync(a.dweight, 0, (size_t)(n_all * a.inputs * 2),
+                                              stream));
+            if (a.dbias)
+                RUNE_CUDA_TRY(cudaMemsetAsync(a.dbias, 0, (size_t)(n_all * 2), stream));
+            return;
+        }
+        check_waits(a.device);
+        Scratch need{nullptr};
+        backward(a, need, stream);
+        require(need.off == 0 || (a.workspace && aligned(a.workspace, 256) &&
+                                  a.workspace_bytes >= need.off),
+                "the workspace is too small or not 256-byte aligned");
+        Scratch ws{need.off ? static_cast<char*>(a.workspace) : reinterpret_cast<char*>(256)};
+        backward(a, ws, stream);
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,223 @@
+// Shared pieces of the mixed-precision network operators (norm.cu, linear.cu): typed vector
+// access, activations for 16-bit results, host-side argument checks.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <new>
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace rune {
+namespace ops {
+
+constexpr float kE4m3Max = 448.0f;
+
+// ----------------------------------------------------------------------------- host side
+// Runs fn on device `device` and maps every exception to a status; the caller's current device
+// is restored. Nothing throws through the C boundary.
+template <typename Fn>
+int guarded(int device, Fn&& fn) {
+    int before = -1;
+    int code = RUNE_OK;
+    try {
+        RUNE_CUDA_TRY(cudaGetDevice(&before));
+        // also where it is current already: a new thread has no context before this call, and the
+        // driver's tensor-map encoder needs one
+        RUNE_CUDA_TRY(cudaSetDevice(device));
+        fn();
+    } catch (const Error& e) {
+        set_error(e.message);
+        code = e.code;
+        if (code == RUNE_ERR_CUDA) cudaGetLastError();  // reported here: not again by a later call
+    } catch (const std::bad_alloc&) {
+        set_error("out of host memory");
+        code = RUNE_ERR_OOM;
+    } catch (const std::exception& e) {
+        set_error(e.what());
+        code = RUNE_ERR_INVALID;
+    } catch (...) {
+        set_error("unknown failure");
+        code = RUNE_ERR_INVALID;
+    }
+    if (before >= 0 && before != device) cudaSetDevice(before);
+    return code;
+}
+
+inline void require(bool ok, const char* message) {
+    if (!ok) throw Error(RUNE_ERR_INVALID, message);
+}
+
+inline int dtype_bytes(int dtype) { return dtype == RUNE_F32 ? 4 : dtype == RUNE_E4M3 ? 1 : 2; }
+
+inline bool aligned(const void* p, size_t bytes) { return (uintptr_t)p % bytes == 0; }
+
+int sm_count(int device);
+
+// Sums the float32 partials [parts][width] over parts into out[width] of type dtype.
+void sum_partials(const float* partials, int64_t parts, int64_t width, void* out, int dtype,
+                  cudaStream_t stream);
+
+// ----------------------------------------------------------------------------- typed access
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
+    return __float2bfloat16_rn(v);
+}
+
+// two floats rounded to a packed pair (a in the low half)
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&v);
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+    return __half22float2(*reinterpret_cast<__half2*>(&w));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+// VEC consecutive values at p as floats: one 16-byte access where VEC fills it, else one value
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const T* p, float* v) {
+    if constexpr (VEC == 1) {
+        v[0] = to_float(*p);
+    } else if constexpr (sizeof(T) == 4) {
+        float4 q = *reinterpret_cast<const float4*>(p);
+        v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+    } else {
+        uint4 q = *reinterpret_cast<const uint4*>(p);
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float2 f = unpack2<T>(w[i]);
+            v[2 * i] = f.x, v[2 * i + 1] = f.y;
+        }
+    }
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void store_vec(T* p, const float* v) {
+    if constexpr (VEC == 1) {
+        *p = from_float<T>(v[0]);
+    } else if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+        *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]),
+                                                  pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+    }
+}
+
+// maximum that keeps a NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// ----------------------------------------------------------------------------- activations
+// For results that are rounded to 16 bits (2^-9 or 2^-12 relative): few instructions without a
+// branch, errors of some 1e-6 of the value.
+__device__ __forceinline__ float exp_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.44269504088896f));
+    return r;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// tanh x = 1 - 2 / (1 + e^2x); near zero, where that cancels, its Taylor series to x^7
+// (next term 62/2835 x^9: 3e-7 of the value at 1/4).
+__device__ __forceinline__ float tanh_fast(float x) {
+    float t = 1.0f - 2.0f * rcp_fast(1.0f + exp_fast(2.0f * x));
+    float q = x * x;
+    float s = x + x * q * (-1.0f / 3.0f + q * (2.0f / 15.0f - q * (17.0f / 315.0f)));
+    return q < 0.0625f ? s : t;
+}
+
+// Upper tail Q(|x|) = 1 - Phi(|x|) of the normal distribution and e^(-x^2 / 2). erfc by the
+// rational approximation of Abramowitz and Stegun 7.1.26 (absolute error 1.5e-7 of erf), whose
+// factor e^(-x^2 / 2) is the density's as well.
+__device__ __forceinline__ float normal_tail(float x, float& e) {
+    float a = fabsf(x) * 0.70710678118654752f;
+    e = exp_fast(-0.5f * x * x);
+    float t = rcp_fast(1.0f + 0.3275911f * a);
+    float p = t * (0.254829592f +
+                   t * (-0.284496736f +
+                        t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    return 0.5f * p * e;
+}
+
+template <int ACT>
+__device__ __forceinline__ float act_value(float x) {
+    if constexpr (ACT == RUNE_ACT_TANH) {
+        return tanh_fast(x);
+    } else if constexpr (ACT == RUNE_ACT_SILU) {
+        return x * rcp_fast(1.0f + exp_fast(-x));
+    } else if constexpr (ACT == RUNE_ACT_GELU) {
+        float e, q = normal_tail(x, e);
+        return x * (x < 0.0f ? q : 1.0f - q);
+    } else {
+        return x;
+    }
+}
+
+template <int ACT>
+__device__ __forceinline__ void act_both(float x, float& y, float& dy) {
+    if constexpr (ACT == RUNE_ACT_TANH) {
+        y = tanh_fast(x);
+        dy = 1.0f - y * y;
+    } else if constexpr (ACT == RUNE_ACT_SILU) {
+        float s = rcp_fast(1.0f + exp_fast(-x));
+        y = x * s;
+        dy = s * (1.0f + x * (1.0f - s));
+    } else if constexpr (ACT == RUNE_ACT_GELU) {
+        float e, q = normal_tail(x, e);
+        float cdf = x < 0.0f ? q : 1.0f - q;
+        y = x * cdf;
+        dy = cdf + x * e * 0.39894228040143268f;
+    } else {
+        y = x;
+        dy = 1.0f;
+    }
+}
+
+// fn(std::integral_constant<int, ACT>) for the activation code `act`
+template <typename Fn>
+__host__ __device__ __forceinline__ void with_activation(int act, Fn&& fn) {
+    switch (act) {
+        case RUNE_ACT_TANH: fn(std::integral_constant<int, RUNE_ACT_TANH>()); break;
+        case RUNE_ACT_SILU: fn(std::integral_constant<int, RUNE_ACT_SILU>()); break;
+        case RUNE_ACT_GELU: fn(std::integral_constant<int, RUNE_ACT_GELU>()); break;
+        default: fn(std::integral_constant<int, RUNE_ACT_NONE>()); break;
+    }
+}
+
+}  // namespace ops
+}  // namespace rune

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import (POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_uint8,
                     c_uint32, c_void_p)
 from pathlib import Path
@@ -31,6 +32,8 @@ HALO_FN = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_int32, ctypes
 
 RUNE_NEP, RUNE_MOBIUS_LOCAL, RUNE_MOBIUS_MP, RUNE_MOBIUS_EQ = 0, 1, 2, 3
 RUNE_ACT = {"tanh": 0, "silu": 1, "swish": 1, "gelu": 2}
+RUNE_ACT_NONE = -1
+RUNE_F32, RUNE_F16, RUNE_BF16, RUNE_E4M3 = 0, 1, 2, 3
 RUNE_ZBL_NONE, RUNE_ZBL_UNIVERSAL, RUNE_ZBL_FLEXIBLE = 0, 1, 2
 RUNE_FORCES, RUNE_VIRIAL = 1, 2
 
@@ -43,6 +46,9 @@ EXPORTED = [
     "rune_engine_reset_kernel_stats", "rune_engine_destroy", "rune_last_error",
     "rune_md_nve", "rune_engine_compute_domain", "rune_engine_compute_halo",
     "rune_tc_selftest",
+    "rune_rms_norm", "rune_rms_norm_backward", "rune_rms_norm_backward_workspace",
+    "rune_linear", "rune_linear_workspace", "rune_linear_backward",
+    "rune_linear_backward_workspace",
 ]
 
 
@@ -85,6 +91,13 @@ class Stats(ctypes.Structure):
         ("kernel_launches", c_int64), ("tensor_core_layers", c_int64),
     ]
 
+
+# The operators' argument structs (field order of include/rune_b200.h) as struct formats:
+# 64-bit sizes, 32-bit codes, pointers as integers.
+NORM_ARGS = struct.Struct("=4q4ifi7Q")
+NORM_GRAD_ARGS = struct.Struct("=5q4i8Qq")
+LINEAR_ARGS = struct.Struct("=6q6i9Qq")
+LINEAR_GRAD_ARGS = struct.Struct("=6q4i9Qq")
 
 _LIB = None
 
@@ -139,6 +152,13 @@ def load_library(path: Path | None = None):
         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
     lib.rune_tc_selftest.argtypes = [c_int32, c_int32, c_int32, POINTER(c_float),
                                      POINTER(c_float), POINTER(c_float), c_int32]
+    # operator arguments travel as packed bytes of the C structs (NORM_ARGS and the others)
+    for name in ("rune_rms_norm", "rune_rms_norm_backward", "rune_linear",
+                 "rune_linear_backward"):
+        getattr(lib, name).argtypes = [c_char_p, c_void_p]
+    for name in ("rune_rms_norm_backward_workspace", "rune_linear_workspace",
+                 "rune_linear_backward_workspace"):
+        getattr(lib, name).argtypes = [c_char_p, POINTER(c_int64)]
     for name in EXPORTED:
         if name not in ("rune_engine_destroy", "rune_last_error"):
             getattr(lib, name).restype = c_int
