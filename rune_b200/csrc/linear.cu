@@ -48,7 +48,7 @@ struct TileParams {
     int64_t ld_out, ld_in, ld_z;
     int kblocks, kb_per_split, splits;
     int tiles_m, tiles_n, bn, stages;
-    int a_mn, b_mn, fp8, act;
+    int a_mn, b_mn, act;
     int vec_out, vec_in, vec_z;  // 16-byte accesses allowed
     uint32_t idesc;
     void* out;
@@ -362,7 +362,7 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
     }
 }
 
-template <int MODE, typename T>
+template <int MODE, typename T, bool FP8>
 __global__ void __launch_bounds__(kThreads, 1)
 k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
        const TileParams p) {
@@ -371,9 +371,10 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
     const uint32_t stage_bytes = kAStage + (uint32_t)p.bn * kLineBytes;
     unsigned char* bufs = smem + (size_t)p.stages * stage_bytes;
     auto* sh = reinterpret_cast<TileShared*>(bufs + 4 * kWarpBufs<MODE> * kWarpBuf);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform, and known to be
     constexpr bool kPair = MODE == kGated || MODE == kGatedGrad;
-    const int64_t work = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, work = tiles * p.splits;
 
     if (tid == 0) {
         for (int s = 0; s < p.stages; ++s) {
@@ -397,80 +398,105 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
-    const uint32_t tmem = sh->tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sh->tmem, 0);
     volatile int* fail = &sh->fail;
 
-    if (tid == 128) {
+    if (warp == 4) {
         // ---- TMA producer
-        int it = 0;
-        for (int64_t w = blockIdx.x; w < work && !*fail; w += gridDim.x) {
+        const bool one = elect_one();
+        const int bw = kPair ? p.bn / 2 : p.bn;
+        int st = 0, issued = 0;
+        uint32_t parity = 1;  // of the stage's last release; a fresh barrier passes for 1
+        bool ok = true;
+        for (int64_t w = blockIdx.x; w < work && ok; w += gridDim.x) {
             const Tile t = tile_of(p, w);
             const int kb0 = t.split * p.kb_per_split;
             const int kb1 = min(p.kblocks, kb0 + p.kb_per_split);
-            const int m0 = t.mt * kBM, bw = kPair ? p.bn / 2 : p.bn, n0 = t.nt * bw;
-            for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                const int st = it % p.stages, use = it / p.stages;
-                if (use > 0 && !mbar_wait(smem_u32(&sh->empty[st]), (use - 1) & 1)) {
-                    *fail = 1;
+            const int m0 = t.mt * kBM, n0 = t.nt * bw;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                ok = mbar_wait(smem_u32(&sh->empty[st]), parity) && !*fail;
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
                     break;
                 }
-                if (*fail) break;
                 const uint32_t bar = smem_u32(&sh->full[st]);
-                const uint32_t a = smem_u32(smem + (size_t)st * stage_bytes), b = a + kAStage;
-                mbar_expect_tx(bar, stage_bytes);
-                if (p.a_mn) {
-                    tma_load(a, &map_a, m0, kb * 64, bar);
-                    tma_load(a + kMnChunk, &map_a, m0 + 64, kb * 64, bar);
-                } else {
-                    tma_load(a, &map_a, kb * (p.fp8 ? 128 : 64), m0, bar);
+                const uint32_t a = smem_u32(smem) + (uint32_t)st * stage_bytes, b = a + kAStage;
+                if (one) {
+                    mbar_expect_tx(bar, stage_bytes);
+                    if (p.a_mn) {
+                        tma_load(a, &map_a, m0, kb * 64, bar);
+                        tma_load(a + kMnChunk, &map_a, m0 + 64, kb * 64, bar);
+                    } else {
+                        tma_load(a, &map_a, kb * (FP8 ? 128 : 64), m0, bar);
+                    }
+                    if (p.b_mn) {
+                        for (int i = 0; i < p.bn / 64; ++i)
+                            tma_load(b + i * kMnChunk, &map_b, n0 + i * 64, kb * 64, bar);
+                    } else {
+                        const int x = kb * (FP8 ? 128 : 64);
+                        tma_load(b, &map_b, x, n0, bar);
+                        if (kPair) tma_load(b + bw * kLineBytes, &map_b, x, (int)p.n + n0, bar);
+                    }
                 }
-                if (p.b_mn) {
-                    for (int i = 0; i < p.bn / 64; ++i)
-                        tma_load(b + i * kMnChunk, &map_b, n0 + i * 64, kb * 64, bar);
-                } else {
-                    const int x = kb * (p.fp8 ? 128 : 64);
-                    tma_load(b, &map_b, x, n0, bar);
-                    if (kPair) tma_load(b + bw * kLineBytes, &map_b, x, (int)p.n + n0, bar);
-                }
-                sh->issued = it + 1;
+                ++issued;
+                if (++st == p.stages) st = 0, parity ^= 1;
             }
         }
-    } else if (tid == 160) {
-        // ---- MMA issuer
-        int it = 0, n_tile = 0;
+        if (!ok) *fail = 1;
+        if (one) sh->issued = issued;
+    } else if (warp == 5) {
+        // ---- MMA issuer. The whole warp runs the loop and one elected lane issues: control flow
+        // and descriptors are uniform then, and stay in the uniform registers that the tensor
+        // core instructions take (issued from a divergent thread they came too slowly).
+        const bool one = elect_one();
         const uint64_t step_a = p.a_mn ? 2048 >> 4 : 32 >> 4;
         const uint64_t step_b = p.b_mn ? 2048 >> 4 : 32 >> 4;
-        for (int64_t w = blockIdx.x; w < work && !*fail; w += gridDim.x, ++n_tile) {
-            const Tile t = tile_of(p, w);
-            const int kb0 = t.split * p.kb_per_split;
+        const uint64_t desc_a = operand_desc(smem_u32(smem), p.a_mn);
+        const uint64_t desc_b = operand_desc(smem_u32(smem) + kAStage, p.b_mn);
+        int st = 0, buf = 0;
+        uint32_t parity = 0, acc_parity = 1;
+        bool ok = true;
+        for (int64_t w = blockIdx.x; w < work && ok; w += gridDim.x) {
+            const int split = (int)(w / tiles);
+            const int kb0 = split * p.kb_per_split;
             const int kb1 = min(p.kblocks, kb0 + p.kb_per_split);
-            const int buf = n_tile & 1, round = n_tile >> 1;
-            if (round > 0 && !mbar_wait(smem_u32(&sh->acc_empty[buf]), (round - 1) & 1)) {
-                *fail = 1;
+            ok = mbar_wait(smem_u32(&sh->acc_empty[buf]), acc_parity) && !*fail;
+            if (!__all_sync(0xffffffffu, ok)) {
+                ok = false;
                 break;
             }
             fence_after_sync();
             const uint32_t acc = tmem + buf * 256;
-            for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                const int st = it % p.stages, use = it / p.stages;
-                if (!mbar_wait(smem_u32(&sh->full[st]), use & 1) || *fail) {
-                    *fail = 1;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                ok = mbar_wait(smem_u32(&sh->full[st]), parity) && !*fail;
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
                     break;
                 }
                 fence_after_sync();
-                const uint32_t a = smem_u32(smem + (size_t)st * stage_bytes);
-                const uint64_t da = operand_desc(a, p.a_mn);
-                const uint64_t db = operand_desc(a + kAStage, p.b_mn);
+                const uint64_t at = (uint64_t)((uint32_t)st * (stage_bytes >> 4));
+                if (one) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const bool more = kb > kb0 || k > 0;
-                    if (p.fp8) mma_f8(acc, da + k * step_a, db + k * step_b, p.idesc, more);
-                    else mma_f16(acc, da + k * step_a, db + k * step_b, p.idesc, more);
+                    for (int k = 0; k < 4; ++k) {
+                        const bool more = kb > kb0 || k > 0;
+                        if constexpr (FP8)
+                            mma_f8(acc, desc_a + at + k * step_a, desc_b + at + k * step_b,
+                                   p.idesc, more);
+                        else
+                            mma_f16(acc, desc_a + at + k * step_a, desc_b + at + k * step_b,
+                                    p.idesc, more);
+                    }
+                    mma_commit(smem_u32(&sh->empty[st]));
                 }
-                mma_commit(smem_u32(&sh->empty[st]));
+                __syncwarp();
+                if (++st == p.stages) st = 0, parity ^= 1;
             }
-            mma_commit(smem_u32(&sh->acc_full[buf]));
+            if (one) mma_commit(smem_u32(&sh->acc_full[buf]));
+            __syncwarp();
+            buf ^= 1;
+            if (buf == 0) acc_parity ^= 1;
         }
+        if (!ok) *fail = 1;
     } else if (warp < 4) {
         // ---- epilogue
         int n_tile = 0;
@@ -515,8 +541,8 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
             for (int i = max(0, issued - p.stages); i < issued; ++i)
                 mbar_wait(smem_u32(&sh->full[i % p.stages]), (i / p.stages) & 1);
         }
-        if (tid == 160) {
-            mma_commit(smem_u32(&sh->drained));
+        if (warp == 5) {
+            if (elect_one()) mma_commit(smem_u32(&sh->drained));
             mbar_wait(smem_u32(&sh->drained), 0);
         }
         __syncthreads();
@@ -708,21 +734,21 @@ Plan plan_product(int64_t m, int64_t n_cols, int kblocks, bool can_split, bool p
     return best;
 }
 
-template <int MODE, typename T>
+template <int MODE, typename T, bool FP8>
 void launch_tile(const CUtensorMap& a, const CUtensorMap& b, const TileParams& p, int sms,
                  int device, cudaStream_t stream) {
     const size_t smem = (size_t)p.stages * (kAStage + (size_t)p.bn * kLineBytes) +
                         kFixedSmem<MODE>;
     static std::atomic<uint64_t> allowed{0};  // devices whose limit is raised
     if (device >= 64 || !(allowed.load(std::memory_order_relaxed) >> device & 1)) {
-        RUNE_CUDA_TRY(cudaFuncSetAttribute(k_tile<MODE, T>,
+        RUNE_CUDA_TRY(cudaFuncSetAttribute(k_tile<MODE, T, FP8>,
                                            cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            (int)kSmemMax));
         if (device < 64) allowed.fetch_or(uint64_t(1) << device, std::memory_order_relaxed);
     }
     const int64_t work = (int64_t)p.tiles_m * p.tiles_n * p.splits;
     const int grid = (int)std::min<int64_t>(work, sms);
-    k_tile<MODE, T><<<grid, kThreads, smem, stream>>>(a, b, p);
+    k_tile<MODE, T, FP8><<<grid, kThreads, smem, stream>>>(a, b, p);
     RUNE_LAUNCH_CHECK();
 }
 
@@ -754,7 +780,7 @@ void run_mode(const Product& g, TileParams p, Scratch& ws, int device, cudaStrea
     p.kb_per_split = plan.kb_per_split;
     p.stages = plan.stages;
     p.tiles_m = (int)((p.m + kBM - 1) / kBM);
-    p.a_mn = g.a_mn, p.b_mn = g.b_mn, p.fp8 = fp8;
+    p.a_mn = g.a_mn, p.b_mn = g.b_mn;
     p.idesc = operand_idesc(fp8 ? 0 : g.dtype == RUNE_BF16 ? 1 : 0, g.a_mn, g.b_mn, kBM, p.bn);
     p.flag = wait_flag(device);
     const CUtensorMap ma = make_map(g.a, eb, g.a_mn ? 64 : kBM);
@@ -762,7 +788,13 @@ void run_mode(const Product& g, TileParams p, Scratch& ws, int device, cudaStrea
         const int width = pair ? p.bn / 2 : p.bn;
         p.tiles_n = (int)((p.n + width - 1) / width);
         const CUtensorMap mb = make_map(g.b, eb, g.b_mn ? 64 : width);
-        launch_tile<MODE, T>(ma, mb, p, sms, device, stream);
+        if constexpr (MODE == kForward || MODE == kGated) {
+            if (fp8) {
+                launch_tile<MODE, T, true>(ma, mb, p, sms, device, stream);
+                return;
+            }
+        }
+        launch_tile<MODE, T, false>(ma, mb, p, sms, device, stream);
         return;
     }
     if constexpr (MODE == kForward || MODE == kGated) {
@@ -772,7 +804,8 @@ void run_mode(const Product& g, TileParams p, Scratch& ws, int device, cudaStrea
         q.z = part;
         q.ld_z = ld_part;
         const CUtensorMap mb = make_map(g.b, eb, g.b_mn ? 64 : p.bn);
-        launch_tile<kPartial, __half>(ma, mb, q, sms, device, stream);
+        if (fp8) launch_tile<kPartial, __half, true>(ma, mb, q, sms, device, stream);
+        else launch_tile<kPartial, __half, false>(ma, mb, q, sms, device, stream);
         const int64_t items = p.m * ((p.n + 3) / 4);
         const int grid = (int)std::min<int64_t>((items + 255) / 256, (int64_t)sms * 16);
         k_join<MODE, T><<<grid, 256, 0, stream>>>(p, part);
