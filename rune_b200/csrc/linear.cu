@@ -867,6 +867,10 @@ void forward(const rune_linear_args& a, Scratch& ws, cudaStream_t stream) {
     Product g;
     g.a = readable({a.x, a.rows, a.inputs, a.x_stride}, eb, ws, stream);
     g.b = readable({a.weight, n_all, a.inputs, a.weight_stride}, eb, ws, stream);
+    if (a.rows <= kFewRows) {
+        if (!ws.sizing()) linear_few(a, g.a, g.b, stream);
+        return;
+    }
     g.mode = a.gated ? kGated : kForward;
     g.dtype = a.dtype;
     g.out_type = a.out_dtype;

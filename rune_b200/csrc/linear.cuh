@@ -100,6 +100,12 @@ inline bool tma_ready(const Matrix& m, int elem_bytes) {
 // Tensor map of `m` with boxes of one 128-byte line x box_rows lines, zeros outside.
 CUtensorMap make_map(const Matrix& m, int elem_bytes, int box_rows);
 
+// Largest number of rows of x that linear_few takes. Measured on B200, bf16, against the 128-row
+// tiles: 16 rows x 4096 -> 8192 15.8 against 19.3 us, x 1024 -> 1024 5.3 against 8.0; 64 rows
+// 19.2 against 19.3 and 6.5 against 8.0, but x 256 -> 512 10.9 against 5.8.
+constexpr int kFewRows = 48;
+void linear_few(const rune_linear_args& a, const Matrix& x, const Matrix& w, cudaStream_t stream);
+
 // Host-mapped word that a kernel sets when a wait gave up; check_waits throws if it is set.
 unsigned* wait_flag(int device);
 void check_waits(int device);
