@@ -32,7 +32,8 @@ extern "C" {
 #define RUNE_ERR_TYPE 4               /* atom type outside the model       -> ValueError   */
 #define RUNE_ERR_OOM 5                /* device allocation failed          -> MemoryError  */
 #define RUNE_ERR_STATE 6              /* call order (e.g. compute before finalize)         */
-#define RUNE_ERR_RETRY 7              /* halo call: repeat it on every rank (rows regrown)  */
+#define RUNE_ERR_RETRY 7              /* halo call: repeat it on every rank (rows regrown);
+                                         rune_linear: repeat it with a workspace          */
 
 /* Model families (rune/mobius/model.py:47 message_mode / message_layers; rune/nep/model.py:48) */
 #define RUNE_NEP 0
@@ -348,7 +349,9 @@ typedef struct {
     int64_t workspace_bytes;
 } rune_linear_args;
 
-/* z = x weight^T (scaled) + bias; y = act(z) + residual, or gated: y = act(z_gate) z_up. */
+/* z = x weight^T (scaled) + bias; y = act(z) + residual, or gated: y = act(z_gate) z_up. With a
+ * NULL workspace a call that needs none runs, and one that needs some returns RUNE_ERR_RETRY
+ * without having done anything. */
 int rune_linear(const rune_linear_args* args, void* stream);
 int rune_linear_workspace(const rune_linear_args* args, int64_t* bytes);
 

@@ -1144,6 +1144,8 @@ int rune_linear(const rune_linear_args* args, void* stream_) {
         check_waits(a.device);
         Scratch need{nullptr};
         forward(a, need, stream);
+        if (need.off > 0 && !a.workspace)
+            throw Error(RUNE_ERR_RETRY, "the call needs a workspace");
         require(need.off == 0 || (a.workspace && aligned(a.workspace, 256) &&
                                   a.workspace_bytes >= need.off),
                 "the workspace is too small or not 256-byte aligned");

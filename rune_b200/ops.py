@@ -20,7 +20,6 @@ from __future__ import annotations
 from ctypes import byref, c_int64
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .runtime import library as L
 
@@ -52,25 +51,30 @@ def _activation(name):
 
 
 def _rows(t, name):
-    """`t` as [rows, width] with unit column stride (copied only where no view has one)."""
+    """(`t`, rows, stride): `t` as rows of its last axis with unit column stride, copied only
+    where no view has one."""
     shape = t.shape
     if not shape or shape[-1] == 0:
         raise ValueError(f"{name} needs at least one axis, and its last one cannot be empty.")
+    width = shape[-1]
+    if t.is_contiguous():
+        return t, t.numel() // width, width
     if len(shape) != 2:
-        t = t.reshape(-1, shape[-1])
+        t = t.reshape(-1, width)
     step, unit = t.stride()
-    if (unit != 1 and shape[-1] > 1) or (step < shape[-1] and t.shape[0] > 1):
+    if (unit != 1 and width > 1) or (step < width and t.shape[0] > 1):
         t = t.contiguous()
-    return t
+        step = width
+    return t, t.shape[0], step
 
 
-def _check(t, name, dtype, shape, device):
+def _check(t, name, dtype, shape, x):
     if t.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, not {t.dtype}.")
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}.")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}, not {t.device}.")
+    if t.get_device() != x.get_device():
+        raise ValueError(f"{name} must be on {x.device}, not {t.device}.")
 
 
 def _cuda(t, name):
@@ -82,71 +86,81 @@ def _ptr(t):
     return 0 if t is None else t.data_ptr()
 
 
-def _workspace(lib, query, args, device):
+def _workspace(lib, query, args, like):
     """Scratch of the bytes that `query` asks for (None where it needs none)."""
     need = c_int64(0)
     L.check(lib, query(args, byref(need)))
     n = need.value
-    return (torch.empty(n, dtype=torch.uint8, device=device), n) if n else (None, 0)
+    return (like.new_empty(n, dtype=torch.uint8), n) if n else (None, 0)
+
+
+def _first_order_only():
+    if torch.is_grad_enabled():  # create_graph=True
+        raise RuntimeError("the operators of rune_b200.ops have no second derivative.")
 
 
 # ------------------------------------------------------------------------------------ norm
 def _norm_call(x, weight, residual, eps, out_dtype, want_rstd):
-    """(y, h, scale, rstd) of rows x; h is x itself without a residual."""
+    """(y, h, scale, rstd) of the rows of x; h is None without a residual."""
     lib = L.load_library()
-    rows, width = x.shape
-    dev = x.device
-    y = torch.empty((rows, width), dtype=out_dtype, device=dev)
+    shape, dtype, index = x.shape, x.dtype, x.get_device()
+    x, rows, ld = _rows(x, "x")
     h = scale = rstd = None
+    res_ptr = ld_res = h_ptr = 0
     if residual is not None:
-        h = torch.empty((rows, width), dtype=x.dtype, device=dev)
+        res, _, ld_res = _rows(residual, "residual")
+        res_ptr = res.data_ptr()
+        h = x.new_empty(shape)
+        h_ptr = h.data_ptr()
+    y = x.new_empty(shape, dtype=out_dtype)
     if out_dtype is torch.float8_e4m3fn:
-        scale = torch.empty(rows, dtype=torch.float32, device=dev)
+        scale = x.new_empty(shape[:-1], dtype=torch.float32)
     if want_rstd:
-        rstd = torch.empty(rows, dtype=torch.float32, device=dev)
-    code = _CODES[x.dtype]
-    args = L.NORM_ARGS.pack(
-        rows, width, x.stride(0), 0 if residual is None else residual.stride(0), dev.index, code,
+        rstd = x.new_empty(rows, dtype=torch.float32)
+    code = _CODES[dtype]
+    status = lib.rune_rms_norm(L.NORM_ARGS.pack(
+        rows, shape[-1], ld, ld_res, index, code,
         code if weight is None else _CODES[weight.dtype], _CODES[out_dtype], eps, 0,
-        x.data_ptr(), _ptr(residual), _ptr(weight), y.data_ptr(), _ptr(h), _ptr(scale),
-        _ptr(rstd))
-    L.check(lib, lib.rune_rms_norm(args, _stream(dev.index)))
-    return y, x if h is None else h, scale, rstd
+        x.data_ptr(), res_ptr, _ptr(weight), y.data_ptr(), h_ptr, _ptr(scale), _ptr(rstd)),
+        _stream(index))
+    if status:
+        L.check(lib, status)
+    return y, h, scale, rstd
 
 
 class _RMSNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
         y, h, _, rstd = _norm_call(x, weight, residual, eps, x.dtype, True)
-        ctx.save_for_backward(h, weight, rstd)
+        ctx.save_for_backward(x if h is None else h, weight, rstd)
         ctx.set_materialize_grads(False)
         return y if residual is None else (y, h)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dh=None):
+        _first_order_only()
         h, weight, rstd = ctx.saved_tensors
-        with_res = ctx.needs_input_grad[2]
+        _, need_w, with_res, _ = ctx.needs_input_grad
         if dy is None:  # only the residual stream has a gradient
-            return dh, None, dh, None
+            return dh, None, dh if with_res else None, None
         lib = L.load_library()
-        rows, width = h.shape
-        dev = h.device
-        dy = _rows(dy, "dy")
+        width, index = h.shape[-1], h.get_device()
+        dx = h.new_empty(h.shape)
+        h, rows, ld_h = _rows(h, "h")
+        dy, _, ld_dy = _rows(dy, "dy")
+        ld_dh = 0
         if dh is not None:
-            dh = _rows(dh, "dh")
-        dx = torch.empty((rows, width), dtype=h.dtype, device=dev)
-        dw = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
+            dh, _, ld_dh = _rows(dh, "dh")
+        dw = torch.empty_like(weight) if need_w else None
 
         def args(ws, size):
             return L.NORM_GRAD_ARGS.pack(
-                rows, width, h.stride(0), dy.stride(0), 0 if dh is None else dh.stride(0),
-                dev.index, _CODES[h.dtype], _CODES[weight.dtype], 0, h.data_ptr(),
-                weight.data_ptr(), rstd.data_ptr(), dy.data_ptr(), _ptr(dh), dx.data_ptr(),
-                _ptr(dw), _ptr(ws), size)
+                rows, width, ld_h, ld_dy, ld_dh, index, _CODES[h.dtype], _CODES[weight.dtype], 0,
+                h.data_ptr(), weight.data_ptr(), rstd.data_ptr(), dy.data_ptr(), _ptr(dh),
+                dx.data_ptr(), _ptr(dw), _ptr(ws), size)
 
-        ws = _workspace(lib, lib.rune_rms_norm_backward_workspace, args(None, 0), dev)
-        L.check(lib, lib.rune_rms_norm_backward(args(*ws), _stream(dev.index)))
+        ws = _workspace(lib, lib.rune_rms_norm_backward_workspace, args(None, 0), h)
+        L.check(lib, lib.rune_rms_norm_backward(args(*ws), _stream(index)))
         return dx, dw, dx if with_res else None, None
 
 
@@ -155,15 +169,16 @@ def _norm_inputs(x, weight, residual):
     dtype = x.dtype
     if dtype not in _CODES or dtype is torch.float8_e4m3fn:
         raise ValueError(f"rms_norm takes float32, float16 or bfloat16 rows, not {dtype}.")
-    width = x.shape[-1:]
+    shape = x.shape
+    if not shape or shape[-1] == 0:
+        raise ValueError("x needs at least one axis, and its last one cannot be empty.")
     if weight is not None:
-        _check(weight, "weight", dtype if weight.dtype is dtype else torch.float32, width,
-               x.device)
+        _check(weight, "weight", dtype if weight.dtype is dtype else torch.float32, shape[-1:],
+               x)
         weight = weight.contiguous()
     if residual is not None:
-        _check(residual, "residual", dtype, x.shape, x.device)
-        residual = _rows(residual, "residual")
-    return _rows(x, "x"), weight, residual
+        _check(residual, "residual", dtype, shape, x)
+    return weight
 
 
 def rms_norm(x, weight, residual=None, eps=1.0e-8):
@@ -173,29 +188,21 @@ def rms_norm(x, weight, residual=None, eps=1.0e-8):
     float32. Returns y, and with a residual ``(y, h)``: h is the residual stream for what
     follows. Differentiable in x, weight and residual.
     """
-    shape = x.shape
-    rows, weight, res = _norm_inputs(x, weight, residual)
-    if torch.is_grad_enabled() and (
-            x.requires_grad or weight.requires_grad
-            or (residual is not None and residual.requires_grad)):
-        got = _RMSNorm.apply(rows, weight, res, float(eps))
-        y, h = got if residual is not None else (got, None)
-    else:
-        y, h, _, _ = _norm_call(rows, weight, res, float(eps), x.dtype, False)
-    if residual is None:
-        return y.view(shape)
-    return y.view(shape), h.view(shape)
+    weight = _norm_inputs(x, weight, residual)
+    if (x.requires_grad or weight.requires_grad
+            or (residual is not None and residual.requires_grad)) and torch.is_grad_enabled():
+        return _RMSNorm.apply(x, weight, residual, float(eps))
+    y, h, _, _ = _norm_call(x, weight, residual, eps, x.dtype, False)
+    return y if residual is None else (y, h)
 
 
 def _to_fp8(x, weight, residual, eps):
     for t in (x, weight, residual):
         if t is not None and t.requires_grad and torch.is_grad_enabled():
             raise ValueError("8-bit outputs have no gradient; call under torch.no_grad().")
-    shape = x.shape
-    rows, weight, res = _norm_inputs(x, weight, residual)
-    q, h, scale, _ = _norm_call(rows, weight, res, float(eps), torch.float8_e4m3fn, False)
-    got = q.view(shape), scale.view(shape[:-1])
-    return got if residual is None else (*got, h.view(shape))
+    weight = _norm_inputs(x, weight, residual)
+    q, h, scale, _ = _norm_call(x, weight, residual, eps, torch.float8_e4m3fn, False)
+    return (q, scale) if residual is None else (q, scale, h)
 
 
 def rms_norm_fp8(x, weight, residual=None, eps=1.0e-8):
@@ -217,25 +224,30 @@ def quantize_fp8(x):
 
 # ---------------------------------------------------------------------------------- linear
 def _linear_call(x, weight, bias, residual, x_scale, w_scale, act, gated, out_dtype, want_z):
-    """(y, z) of rows x; z is the float32 pre-activation where it is asked for."""
+    """(y, z) of the rows of x; z is the float32 pre-activation where it is asked for."""
     lib = L.load_library()
-    rows, inputs = x.shape
-    outputs = weight.shape[0] // 2 if gated else weight.shape[0]
-    dev = x.device
-    y = torch.empty((rows, outputs), dtype=out_dtype, device=dev)
-    z = None
-    if want_z:
-        z = torch.empty((rows, weight.shape[0]), dtype=torch.float32, device=dev)
-
-    def args(ws, size):
-        return L.LINEAR_ARGS.pack(
-            rows, inputs, outputs, x.stride(0), weight.stride(0),
-            0 if residual is None else residual.stride(0), dev.index, _CODES[x.dtype],
-            _CODES[out_dtype], act, gated, 0, x.data_ptr(), weight.data_ptr(), _ptr(bias),
-            _ptr(residual), _ptr(x_scale), _ptr(w_scale), y.data_ptr(), _ptr(z), _ptr(ws), size)
-
-    ws = _workspace(lib, lib.rune_linear_workspace, args(None, 0), dev)
-    L.check(lib, lib.rune_linear(args(*ws), _stream(dev.index)))
+    shape, index = x.shape, x.get_device()
+    inputs, n_all = shape[-1], weight.shape[0]
+    outputs = n_all // 2 if gated else n_all
+    x, rows, ld = _rows(x, "x")
+    w, _, ld_w = _rows(weight, "weight")
+    res_ptr = ld_res = 0
+    if residual is not None:
+        residual, _, ld_res = _rows(residual, "residual")
+        res_ptr = residual.data_ptr()
+    y = x.new_empty((*shape[:-1], outputs), dtype=out_dtype)
+    z = x.new_empty((rows, n_all), dtype=torch.float32) if want_z else None
+    pack, stream = L.LINEAR_ARGS.pack, _stream(index)
+    head = (rows, inputs, outputs, ld, ld_w, ld_res, index, _CODES[x.dtype], _CODES[out_dtype],
+            act, gated, 0, x.data_ptr(), w.data_ptr(), _ptr(bias), res_ptr, _ptr(x_scale),
+            _ptr(w_scale), y.data_ptr(), _ptr(z))
+    args = pack(*head, 0, 0)
+    status = lib.rune_linear(args, stream)
+    if status == L.RUNE_ERR_RETRY:  # this call needs scratch
+        ws, size = _workspace(lib, lib.rune_linear_workspace, args, x)
+        status = lib.rune_linear(pack(*head, ws.data_ptr(), size), stream)
+    if status:
+        L.check(lib, status)
     return y, z
 
 
@@ -243,45 +255,45 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, gated):
         needs = ctx.needs_input_grad
-        save = act != L.RUNE_ACT_NONE and x.shape[1] > RECOMPUTE_INPUTS and any(needs[:3])
+        save = act != L.RUNE_ACT_NONE and x.shape[-1] > RECOMPUTE_INPUTS and any(needs[:3])
         y, z = _linear_call(x, weight, bias, residual, None, None, act, gated, x.dtype, save)
         ctx.save_for_backward(x, weight, bias, z)
         ctx.act, ctx.gated = act, gated
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        _first_order_only()
         x, weight, bias, z = ctx.saved_tensors
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         dx = dw = db = None
         if need_x or need_w or need_b:
             lib = L.load_library()
-            dev = x.device
-            rows, inputs = x.shape
-            g = _rows(dy, "dy")
+            index, outputs = x.get_device(), dy.shape[-1]
             if need_x:
-                dx = torch.empty((rows, inputs), dtype=x.dtype, device=dev)
+                dx = x.new_empty(x.shape)
             if need_w:
-                dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev)
+                dw = weight.new_empty(weight.shape)
             if need_b:
-                db = torch.empty(bias.shape, dtype=bias.dtype, device=dev)
+                db = bias.new_empty(bias.shape)
+            x, rows, ld = _rows(x, "x")
+            w, _, ld_w = _rows(weight, "weight")
+            g, _, ld_g = _rows(dy, "dy")
 
             def args(ws, size):
                 return L.LINEAR_GRAD_ARGS.pack(
-                    rows, inputs, dy.shape[1], x.stride(0), weight.stride(0), g.stride(0),
-                    dev.index, _CODES[x.dtype], ctx.act, ctx.gated, x.data_ptr(),
-                    weight.data_ptr(), _ptr(bias), g.data_ptr(), _ptr(z), _ptr(dx), _ptr(dw),
-                    _ptr(db), _ptr(ws), size)
+                    rows, x.shape[-1], outputs, ld, ld_w, ld_g, index, _CODES[x.dtype], ctx.act,
+                    ctx.gated, x.data_ptr(), w.data_ptr(), _ptr(bias), g.data_ptr(), _ptr(z),
+                    _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), size)
 
-            ws = _workspace(lib, lib.rune_linear_backward_workspace, args(None, 0), dev)
-            L.check(lib, lib.rune_linear_backward(args(*ws), _stream(dev.index)))
+            ws = _workspace(lib, lib.rune_linear_backward_workspace, args(None, 0), x)
+            L.check(lib, lib.rune_linear_backward(args(*ws), _stream(index)))
         return dx, dw, db, dy if need_r else None, None, None
 
 
 def _layer(x, weight, bias, residual, x_scale, w_scale, act, gated, out_dtype):
     _cuda(x, "x")
-    dtype, dev, shape = x.dtype, x.device, x.shape
+    dtype, shape = x.dtype, x.shape
     fp8 = dtype is torch.float8_e4m3fn
     if not fp8 and dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise ValueError(f"x must be float16, bfloat16 or float8_e4m3fn, not {dtype}.")
@@ -291,7 +303,7 @@ def _layer(x, weight, bias, residual, x_scale, w_scale, act, gated, out_dtype):
     if gated and n_all % 2:
         raise ValueError("weight of a gated layer has the gate's rows, then as many for the "
                          f"other factor; {n_all} rows are odd.")
-    _check(weight, "weight", dtype, (n_all, shape[-1]), dev)
+    _check(weight, "weight", dtype, (n_all, shape[-1]), x)
     outputs = n_all // 2 if gated else n_all
     if fp8:
         out = torch.bfloat16 if out_dtype is None else out_dtype
@@ -299,8 +311,8 @@ def _layer(x, weight, bias, residual, x_scale, w_scale, act, gated, out_dtype):
             raise ValueError(f"out_dtype must be float16 or bfloat16, not {out}.")
         if x_scale is None or w_scale is None:
             raise ValueError("float8_e4m3fn operands need x_scale and weight_scale.")
-        _check(x_scale, "x_scale", torch.float32, shape[:-1], dev)
-        _check(w_scale, "weight_scale", torch.float32, (n_all,), dev)
+        _check(x_scale, "x_scale", torch.float32, shape[:-1], x)
+        _check(w_scale, "weight_scale", torch.float32, (n_all,), x)
         x_scale, w_scale = x_scale.contiguous(), w_scale.contiguous()
     else:
         out = dtype
@@ -309,23 +321,19 @@ def _layer(x, weight, bias, residual, x_scale, w_scale, act, gated, out_dtype):
         if x_scale is not None or w_scale is not None:
             raise ValueError("x_scale and weight_scale go with float8_e4m3fn operands.")
     if bias is not None:
-        _check(bias, "bias", out, (n_all,), dev)
+        _check(bias, "bias", out, (n_all,), x)
         bias = bias.contiguous()
-    rows, wmat, res = _rows(x, "x"), _rows(weight, "weight"), None
     if residual is not None:
-        _check(residual, "residual", out, (*shape[:-1], outputs), dev)
-        res = _rows(residual, "residual")
-    if torch.is_grad_enabled() and (
-            x.requires_grad or weight.requires_grad
+        _check(residual, "residual", out, (*shape[:-1], outputs), x)
+    if (x.requires_grad or weight.requires_grad
             or (bias is not None and bias.requires_grad)
-            or (residual is not None and residual.requires_grad)):
+            or (residual is not None and residual.requires_grad)) and torch.is_grad_enabled():
         if fp8:
             raise ValueError("float8_e4m3fn operands have no gradient; call under "
                              "torch.no_grad().")
-        y = _Linear.apply(rows, wmat, bias, res, act, int(gated))
-    else:
-        y, _ = _linear_call(rows, wmat, bias, res, x_scale, w_scale, act, int(gated), out, False)
-    return y if len(shape) == 2 else y.view(*shape[:-1], outputs)
+        return _Linear.apply(x, weight, bias, residual, act, int(gated))
+    return _linear_call(x, weight, bias, residual, x_scale, w_scale, act, int(gated), out,
+                        False)[0]
 
 
 def linear(x, weight, bias=None, activation=None, residual=None, *, x_scale=None,
