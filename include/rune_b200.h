@@ -312,9 +312,10 @@ int rune_rms_norm(const rune_norm_args* args, void* stream);
 
 typedef struct {
     int64_t rows, width;
-    int64_t h_stride, dy_stride, dh_stride;
+    int64_t x_stride, residual_stride, dy_stride, dh_stride;
     int32_t device, dtype, weight_dtype, reserved;
-    const void* h;          /* the forward's x + residual */
+    const void* x;          /* the forward's operands: their sum unrounded, as it was there */
+    const void* residual;   /* or NULL */
     const void* weight;
     const float* rstd;
     const void* dy;

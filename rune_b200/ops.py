@@ -132,21 +132,25 @@ class _RMSNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
         y, h, _, rstd = _norm_call(x, weight, residual, eps, x.dtype, True)
-        ctx.save_for_backward(x if h is None else h, weight, rstd)
+        # both addends and not their rounded sum, whose error would reach dweight
+        ctx.save_for_backward(x, residual, weight, rstd)
         ctx.set_materialize_grads(False)
         return y if residual is None else (y, h)
 
     @staticmethod
     def backward(ctx, dy, dh=None):
         _first_order_only()
-        h, weight, rstd = ctx.saved_tensors
+        x, residual, weight, rstd = ctx.saved_tensors
         _, need_w, with_res, _ = ctx.needs_input_grad
         if dy is None:  # only the residual stream has a gradient
             return dh, None, dh if with_res else None, None
         lib = L.load_library()
-        width, index = h.shape[-1], h.get_device()
-        dx = h.new_empty(h.shape)
-        h, rows, ld_h = _rows(h, "h")
+        width, index = x.shape[-1], x.get_device()
+        dx = x.new_empty(x.shape)
+        x, rows, ld = _rows(x, "x")
+        ld_res = 0
+        if residual is not None:
+            residual, _, ld_res = _rows(residual, "residual")
         dy, _, ld_dy = _rows(dy, "dy")
         ld_dh = 0
         if dh is not None:
@@ -155,11 +159,11 @@ class _RMSNorm(torch.autograd.Function):
 
         def args(ws, size):
             return L.NORM_GRAD_ARGS.pack(
-                rows, width, ld_h, ld_dy, ld_dh, index, _CODES[h.dtype], _CODES[weight.dtype], 0,
-                h.data_ptr(), weight.data_ptr(), rstd.data_ptr(), dy.data_ptr(), _ptr(dh),
-                dx.data_ptr(), _ptr(dw), _ptr(ws), size)
+                rows, width, ld, ld_res, ld_dy, ld_dh, index, _CODES[x.dtype],
+                _CODES[weight.dtype], 0, x.data_ptr(), _ptr(residual), weight.data_ptr(),
+                rstd.data_ptr(), dy.data_ptr(), _ptr(dh), dx.data_ptr(), _ptr(dw), _ptr(ws), size)
 
-        ws = _workspace(lib, lib.rune_rms_norm_backward_workspace, args(None, 0), h)
+        ws = _workspace(lib, lib.rune_rms_norm_backward_workspace, args(None, 0), x)
         L.check(lib, lib.rune_rms_norm_backward(args(*ws), _stream(index)))
         return dx, dw, dx if with_res else None, None
 

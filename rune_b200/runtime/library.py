@@ -95,7 +95,7 @@ class Stats(ctypes.Structure):
 # The operators' argument structs (field order of include/rune_b200.h) as struct formats:
 # 64-bit sizes, 32-bit codes, pointers as integers.
 NORM_ARGS = struct.Struct("=4q4ifi7Q")
-NORM_GRAD_ARGS = struct.Struct("=5q4i8Qq")
+NORM_GRAD_ARGS = struct.Struct("=6q4i9Qq")
 LINEAR_ARGS = struct.Struct("=6q6i9Qq")
 LINEAR_GRAD_ARGS = struct.Struct("=6q4i9Qq")
 
