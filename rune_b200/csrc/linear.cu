@@ -10,10 +10,10 @@
 // swizzled tiles that TMA writes. Tails of every size are zeros that TMA fills in.
 //
 // A block works on tiles of 128 rows x bn accumulator columns (bn = 64, 128 or 256):
-//   warp 4    one thread streams tiles of A and B (64 values of k; 128 for e4m3) by TMA into a
+//   warp 8    one thread streams tiles of A and B (64 values of k; 128 for e4m3) by TMA into a
 //             ring of as many stages as fit;
-//   warp 5    one thread issues the products into one of two TMEM accumulators;
-//   warps 0-3 the epilogue of the other accumulator: a lane holds a row, so that tiles pass
+//   warp 9    one thread issues the products into one of two TMEM accumulators;
+//   warps 0-7 the epilogue of the other accumulator: a lane holds a row, so that tiles pass
 //             through shared memory on their way to and from global memory, 128 bytes a row.
 // Every wait is bounded; one that gives up raises the device's wait flag and ends the block.
 
@@ -37,7 +37,8 @@ enum Mode {
 };
 
 constexpr int kBM = 128;
-constexpr int kThreads = 192;
+constexpr int kEpiWarps = 8, kTmaWarp = 8, kMmaWarp = 9;
+constexpr int kThreads = 320;
 constexpr uint32_t kAStage = kBM * kLineBytes;  // 16 KB
 constexpr uint32_t kWarpBuf = 32 * kLineBytes;  // 4 KB: 32 rows of 64 16-bit or 32 float values
 constexpr int kMaxStages = 8;
@@ -67,7 +68,7 @@ struct TileShared {
     uint32_t tmem;
     int fail;
     int issued;             // stages whose copies were issued
-    float bias[2][256], w_scale[2][256];
+    float bias[256], w_scale[256];
 };
 
 // buffers of kWarpBuf per epilogue warp, and all shared memory beside the ring
@@ -75,7 +76,7 @@ template <int MODE>
 constexpr uint32_t kWarpBufs = MODE == kGatedGrad ? 2 : 1;
 template <int MODE>
 constexpr uint32_t kFixedSmem =
-    4 * kWarpBufs<MODE> * kWarpBuf + (uint32_t)((sizeof(TileShared) + 127) / 128 * 128);
+    kEpiWarps * kWarpBufs<MODE> * kWarpBuf + (uint32_t)((sizeof(TileShared) + 127) / 128 * 128);
 
 struct Tile {
     int mt, nt, split;
@@ -249,18 +250,20 @@ __device__ __forceinline__ void get_row(unsigned char* buf, int lane, int half, 
     }
 }
 
-// One warp's part (32 rows) of a finished tile.
+// One warp's part of a finished tile: 32 rows (a warp reads the quarter of TMEM's lanes that its
+// number gives) and every other group of columns, the rest being its partner's.
 template <int MODE, typename T>
 __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uint32_t acc,
                                          unsigned char* buf, const float* bias,
                                          const float* w_scale, int warp, int lane) {
-    const int row0 = t.mt * kBM + warp * 32;
+    const int quarter = warp & 3, half_of = warp >> 2;
+    const int row0 = t.mt * kBM + quarter * 32;
     const int rows = (int)max((int64_t)0, min((int64_t)32, p.m - row0));
     constexpr bool kPair = MODE == kGated || MODE == kGatedGrad;
     const int width = kPair ? p.bn / 2 : p.bn;  // output columns of the tile
     const int64_t col0 = (int64_t)t.nt * width;
     if constexpr (MODE == kPartial) {
-        for (int c = 0; c < width && col0 + c < p.n; c += 32) {
+        for (int c = half_of * 32; c < width && col0 + c < p.n; c += 64) {
             float v[32];
             tc::tmem_ld32(acc + c, v);
             store_rows32(buf, v, p.z + ((int64_t)t.split * p.m + row0) * p.ld_z + col0 + c,
@@ -270,7 +273,7 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
     }
     const bool scaled = p.x_scale != nullptr;
     const float xs = scaled && lane < rows ? p.x_scale[row0 + lane] : 0.0f;
-    for (int c = 0; c < width && col0 + c < p.n; c += 64) {
+    for (int c = half_of * 64; c < width && col0 + c < p.n; c += 128) {
         const int64_t col = col0 + c, left = p.n - col;
         if constexpr (MODE == kForward || MODE == kGated) {
             if (p.z) {  // the pre-activations, in float32
@@ -351,7 +354,7 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
         constexpr bool kSums = MODE == kGrad || MODE == kGatedGrad;
         const int64_t ncols = kPair ? 2 * p.n : p.n;
         float* sums = kSums && p.colsum
-                          ? p.colsum + ((int64_t)t.mt * 4 + warp) * ncols + col
+                          ? p.colsum + ((int64_t)t.mt * 4 + quarter) * ncols + col
                           : nullptr;
         T* out = static_cast<T*>(p.out) + (int64_t)row0 * p.ld_out + col;
         store_rows<T, kSums>(buf, out, p.ld_out, rows, left, p.vec_out, lane, sums);
@@ -362,19 +365,27 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
     }
 }
 
-template <int MODE, typename T, bool FP8>
+// PAIR: two blocks of a cluster (the two SMs of a TPC) work on one tile of 256 rows. Each holds its
+// 128 rows of A and of the accumulator and half of the tile's B, which the tensor cores of both
+// read: half the shared-memory traffic and half the copies for B. The even block issues the
+// products; copies of both count on its barriers, completed products on both blocks'.
+template <int MODE, typename T, bool FP8, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
        const TileParams p) {
     using namespace tc;
     extern __shared__ __align__(1024) unsigned char smem[];
-    const uint32_t stage_bytes = kAStage + (uint32_t)p.bn * kLineBytes;
+    const int b_rows = PAIR ? p.bn / 2 : p.bn;  // of B in this block's stages
+    const uint32_t stage_bytes = kAStage + (uint32_t)b_rows * kLineBytes;
     unsigned char* bufs = smem + (size_t)p.stages * stage_bytes;
-    auto* sh = reinterpret_cast<TileShared*>(bufs + 4 * kWarpBufs<MODE> * kWarpBuf);
+    auto* sh = reinterpret_cast<TileShared*>(bufs + kEpiWarps * kWarpBufs<MODE> * kWarpBuf);
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform, and known to be
-    constexpr bool kPair = MODE == kGated || MODE == kGatedGrad;
+    constexpr bool kGate = MODE == kGated || MODE == kGatedGrad;
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, work = tiles * p.splits;
+    const int rank = PAIR ? (int)cluster_rank() : 0;
+    const int first = PAIR ? blockIdx.x >> 1 : blockIdx.x;
+    const int stride = PAIR ? gridDim.x >> 1 : gridDim.x;
 
     if (tid == 0) {
         for (int s = 0; s < p.stages; ++s) {
@@ -383,59 +394,75 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(smem_u32(&sh->acc_full[b]), 1);
-            mbar_init(smem_u32(&sh->acc_empty[b]), 128);
+            mbar_init(smem_u32(&sh->acc_empty[b]), kEpiWarps * (PAIR ? 2 : 1));
         }
         mbar_init(smem_u32(&sh->drained), 1);
         sh->fail = 0;
         sh->issued = 0;
         asm volatile("fence.mbarrier_init.release.cluster;");
     }
-    if (tid == 128) {
+    if (warp == kTmaWarp && elect_one()) {
         prefetch_map(&map_a);
         prefetch_map(&map_b);
     }
-    if (warp == 5) tmem_alloc(&sh->tmem, 512);
+    if (warp == kMmaWarp) {
+        if constexpr (PAIR) tmem_alloc_pair(&sh->tmem, 512);
+        else tmem_alloc(&sh->tmem, 512);
+    }
     fence_before_sync();
-    __syncthreads();
+    __syncwarp();
+    if constexpr (PAIR) cluster_sync();
+    else __syncthreads();
     fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, sh->tmem, 0);
     volatile int* fail = &sh->fail;
 
-    if (warp == 4) {
+    if (warp == kTmaWarp) {
         // ---- TMA producer
         const bool one = elect_one();
-        const int bw = kPair ? p.bn / 2 : p.bn;
+        const int bw = kGate ? p.bn / 2 : p.bn;
+        // barriers of the pair: the even block's
+        const uint32_t full0 = PAIR ? peer_address(smem_u32(sh->full), 0) : smem_u32(sh->full);
+        auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+            if constexpr (PAIR) tma_load_pair(dst, map, x, y, bar);
+            else tma_load(dst, map, x, y, bar);
+        };
         int st = 0, issued = 0;
         uint32_t parity = 1;  // of the stage's last release; a fresh barrier passes for 1
         bool ok = true;
-        for (int64_t w = blockIdx.x; w < work && ok; w += gridDim.x) {
+        for (int64_t w = first; w < work && ok; w += stride) {
             const Tile t = tile_of(p, w);
             const int kb0 = t.split * p.kb_per_split;
             const int kb1 = min(p.kblocks, kb0 + p.kb_per_split);
-            const int m0 = t.mt * kBM, n0 = t.nt * bw;
+            const int m0 = (PAIR ? t.mt * 2 + rank : t.mt) * kBM;
+            // first row of B here: a pair's blocks take halves of the tile, gate and up or not
+            int n0 = t.nt * bw;
+            if (PAIR && rank) n0 += kGate ? (int)p.n : b_rows;
             for (int kb = kb0; kb < kb1; ++kb) {
                 ok = mbar_wait(smem_u32(&sh->empty[st]), parity) && !*fail;
                 if (!__all_sync(0xffffffffu, ok)) {
                     ok = false;
                     break;
                 }
-                const uint32_t bar = smem_u32(&sh->full[st]);
+                const uint32_t bar = full0 + (uint32_t)st * 8;
                 const uint32_t a = smem_u32(smem) + (uint32_t)st * stage_bytes, b = a + kAStage;
                 if (one) {
-                    mbar_expect_tx(bar, stage_bytes);
+                    if (!PAIR || rank == 0)
+                        mbar_expect_tx(smem_u32(&sh->full[st]), (PAIR ? 2 : 1) * stage_bytes);
+                    const int x = kb * (FP8 ? 128 : 64);
                     if (p.a_mn) {
-                        tma_load(a, &map_a, m0, kb * 64, bar);
-                        tma_load(a + kMnChunk, &map_a, m0 + 64, kb * 64, bar);
+                        load(a, &map_a, m0, kb * 64, bar);
+                        load(a + kMnChunk, &map_a, m0 + 64, kb * 64, bar);
                     } else {
-                        tma_load(a, &map_a, kb * (FP8 ? 128 : 64), m0, bar);
+                        load(a, &map_a, x, m0, bar);
                     }
                     if (p.b_mn) {
-                        for (int i = 0; i < p.bn / 64; ++i)
-                            tma_load(b + i * kMnChunk, &map_b, n0 + i * 64, kb * 64, bar);
+                        for (int i = 0; i < b_rows / 64; ++i)
+                            load(b + i * kMnChunk, &map_b, n0 + i * 64, kb * 64, bar);
                     } else {
-                        const int x = kb * (FP8 ? 128 : 64);
-                        tma_load(b, &map_b, x, n0, bar);
-                        if (kPair) tma_load(b + bw * kLineBytes, &map_b, x, (int)p.n + n0, bar);
+                        load(b, &map_b, x, n0, bar);
+                        if (kGate && !PAIR)
+                            load(b + bw * kLineBytes, &map_b, x, (int)p.n + n0, bar);
                     }
                 }
                 ++issued;
@@ -444,7 +471,7 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
         }
         if (!ok) *fail = 1;
         if (one) sh->issued = issued;
-    } else if (warp == 5) {
+    } else if (warp == kMmaWarp && rank == 0) {
         // ---- MMA issuer. The whole warp runs the loop and one elected lane issues: control flow
         // and descriptors are uniform then, and stay in the uniform registers that the tensor
         // core instructions take (issued from a divergent thread they came too slowly).
@@ -453,10 +480,14 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
         const uint64_t step_b = p.b_mn ? 2048 >> 4 : 32 >> 4;
         const uint64_t desc_a = operand_desc(smem_u32(smem), p.a_mn);
         const uint64_t desc_b = operand_desc(smem_u32(smem) + kAStage, p.b_mn);
+        auto commit = [&](unsigned long long* bar) {
+            if constexpr (PAIR) mma_commit_pair(smem_u32(bar));
+            else mma_commit(smem_u32(bar));
+        };
         int st = 0, buf = 0;
         uint32_t parity = 0, acc_parity = 1;
         bool ok = true;
-        for (int64_t w = blockIdx.x; w < work && ok; w += gridDim.x) {
+        for (int64_t w = first; w < work && ok; w += stride) {
             const int split = (int)(w / tiles);
             const int kb0 = split * p.kb_per_split;
             const int kb1 = min(p.kblocks, kb0 + p.kb_per_split);
@@ -479,79 +510,93 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const bool more = kb > kb0 || k > 0;
-                        if constexpr (FP8)
-                            mma_f8(acc, desc_a + at + k * step_a, desc_b + at + k * step_b,
-                                   p.idesc, more);
-                        else
-                            mma_f16(acc, desc_a + at + k * step_a, desc_b + at + k * step_b,
-                                    p.idesc, more);
+                        mma<FP8, PAIR>(acc, desc_a + at + k * step_a, desc_b + at + k * step_b,
+                                       p.idesc, more);
                     }
-                    mma_commit(smem_u32(&sh->empty[st]));
+                    commit(&sh->empty[st]);
                 }
                 __syncwarp();
                 if (++st == p.stages) st = 0, parity ^= 1;
             }
-            if (one) mma_commit(smem_u32(&sh->acc_full[buf]));
+            if (one) commit(&sh->acc_full[buf]);
             __syncwarp();
             buf ^= 1;
             if (buf == 0) acc_parity ^= 1;
         }
         if (!ok) *fail = 1;
-    } else if (warp < 4) {
+    } else if (warp < kEpiWarps) {
         // ---- epilogue
         int n_tile = 0;
         unsigned char* buf = bufs + warp * kWarpBufs<MODE> * kWarpBuf;
-        for (int64_t w = blockIdx.x; w < work; w += gridDim.x, ++n_tile) {
-            const Tile t = tile_of(p, w);
+        for (int64_t w = first; w < work; w += stride, ++n_tile) {
+            Tile t = tile_of(p, w);
+            if (PAIR) t.mt = t.mt * 2 + rank;
             const int b = n_tile & 1, round = n_tile >> 1;
             if constexpr (MODE != kPartial) {
-                // bias and weight scales of the tile's columns, one set per accumulator
-                const int width = kPair ? p.bn / 2 : p.bn;
-                for (int c = tid; c < p.bn; c += 128) {
-                    const int part = c / width;
-                    const int64_t col = (int64_t)t.nt * width + c % width;
+                // bias and weight scales of the tile's columns
+                const int width = kGate ? p.bn / 2 : p.bn;
+                if (n_tile > 0) asm volatile("bar.sync 1, 256;" ::: "memory");
+                if (tid < p.bn) {
+                    const int part = tid / width;
+                    const int64_t col = (int64_t)t.nt * width + tid % width;
                     const bool in = col < p.n;
-                    sh->bias[b][c] =
-                        in && p.bias
-                            ? to_float(static_cast<const T*>(p.bias)[part * p.n + col])
-                            : 0.0f;
-                    sh->w_scale[b][c] = in && p.w_scale ? p.w_scale[part * p.n + col] : 0.0f;
+                    sh->bias[tid] = in && p.bias ? to_float(static_cast<const T*>(
+                                                       p.bias)[part * p.n + col])
+                                                 : 0.0f;
+                    sh->w_scale[tid] = in && p.w_scale ? p.w_scale[part * p.n + col] : 0.0f;
                 }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
+                asm volatile("bar.sync 1, 256;" ::: "memory");
             }
-            // after a failure the warps still meet at the barrier above for every tile
+            // after a failure the warps still meet at the barriers above for every tile
             bool ok = !*fail && mbar_wait(smem_u32(&sh->acc_full[b]), round & 1) && !*fail;
             if (!__all_sync(0xffffffffu, ok)) {
                 *fail = 1;
                 continue;
             }
             fence_after_sync();
-            epilogue<MODE, T>(p, t, tmem + b * 256 + ((uint32_t)(warp * 32) << 16), buf,
-                              sh->bias[b], sh->w_scale[b], warp, lane);
+            epilogue<MODE, T>(p, t, tmem + b * 256 + ((uint32_t)((warp & 3) * 32) << 16), buf,
+                              sh->bias, sh->w_scale, warp, lane);
             fence_before_sync();
-            mbar_arrive(smem_u32(&sh->acc_empty[b]));
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (PAIR)
+                    mbar_arrive_peer(peer_address(smem_u32(&sh->acc_empty[b]), 0));
+                else
+                    mbar_arrive(smem_u32(&sh->acc_empty[b]));
+            }
         }
     }
-    __syncthreads();
-    if (*fail) {
-        // let what is in flight land (bounded) before the block's memory goes
-        if (tid == 0) {
-            atomicExch_system(p.flag, 1u);
+    __syncwarp();
+    if constexpr (PAIR) cluster_sync();
+    else __syncthreads();
+    bool failed = *fail;
+    if constexpr (PAIR)
+        failed = failed || peer_word(peer_address(smem_u32(&sh->fail), rank ^ 1)) != 0;
+    if (failed) {
+        // let what is in flight land (bounded) before the blocks' memory goes: the copies of both
+        // blocks count on the even one's barriers
+        if (tid == 0) atomicExch_system(p.flag, 1u);
+        if (tid == 0 && rank == 0) {
             const int issued = sh->issued;
             for (int i = max(0, issued - p.stages); i < issued; ++i)
                 mbar_wait(smem_u32(&sh->full[i % p.stages]), (i / p.stages) & 1);
         }
-        if (warp == 5) {
-            if (elect_one()) mma_commit(smem_u32(&sh->drained));
+        if (warp == kMmaWarp && rank == 0) {
+            if (elect_one()) {
+                if constexpr (PAIR) mma_commit_pair(smem_u32(&sh->drained));
+                else mma_commit(smem_u32(&sh->drained));
+            }
             mbar_wait(smem_u32(&sh->drained), 0);
         }
-        __syncthreads();
+        __syncwarp();
     }
     fence_before_sync();
-    __syncthreads();
-    if (warp == 5) {
+    if constexpr (PAIR) cluster_sync();
+    else __syncthreads();
+    if (warp == kMmaWarp) {
         fence_after_sync();
-        tmem_dealloc(tmem, 512);
+        if constexpr (PAIR) tmem_dealloc_pair(tmem, 512);
+        else tmem_dealloc(tmem, 512);
     }
 }
 
@@ -698,58 +743,73 @@ struct Scratch {
 
 struct Plan {
     int bn, splits, kb_per_split, stages;
+    bool pair;
 };
 
-// Tile width and ranges of k of one product, by a model of its time in cycles: a k-block of 64
-// costs bn * 2 cycles of the tensor core (never less than the 128 + bn lines of shared memory
-// that it reads), an epilogue 10 cycles a column, hidden behind the next tile's products, and a
-// join of splits a launch and its traffic.
-Plan plan_product(int64_t m, int64_t n_cols, int kblocks, bool can_split, bool pair, int sms,
+// Tile, range of k and pairing of one product, by a model of its time in cycles: a k-block of 64
+// costs bn * 2 cycles of the tensor core (never less than the lines of shared memory that it
+// reads), an epilogue 10 cycles a column, hidden behind the next tile's products, and a join of
+// splits a launch and its traffic.
+Plan plan_product(int64_t m, int64_t n_cols, int kblocks, bool can_split, bool gate, int sms,
                   uint32_t fixed) {
     Plan best{};
     double best_cost = 0.0;
-    for (int bn : {256, 128, 64}) {
-        if (pair && bn == 64) continue;  // the epilogue takes 64 output columns at a time
-        const int64_t tiles = ((m + kBM - 1) / kBM) * ((n_cols + bn - 1) / bn);
-        const int most = can_split ? (int)std::min<int64_t>(std::max(1, kblocks / 4),
-                                                            std::max<int64_t>(1, sms / tiles))
-                                   : 1;
-        for (int s = 1; s <= most; ++s) {
-            const int per = (kblocks + s - 1) / s;
-            const int splits = (kblocks + per - 1) / per;
-            const double waves = (double)((tiles * splits + sms - 1) / sms);
-            const double main = per * std::max(2.0 * bn, (128.0 + bn) * 1.0);
-            const double epi = 10.0 * bn;
-            double cost = 2000.0 + waves * std::max(main, epi) + std::min(main, epi);
-            if (splits > 1)
-                cost += 5000.0 + (double)m * n_cols * (splits + 1) * 4.0 / 3000.0;
-            if (best.bn == 0 || cost < best_cost) {
-                best_cost = cost;
-                best = {bn, splits, per, 0};
+    for (int pair = 1; pair >= 0; --pair) {
+        for (int bn : {256, 128, 64}) {
+            if ((gate || pair) && bn == 64) continue;  // halves of at least 64 columns
+            const int rows = pair ? 2 * kBM : kBM, units = pair ? sms / 2 : sms;
+            const int64_t tiles = ((m + rows - 1) / rows) * ((n_cols + bn - 1) / bn);
+            const int most = can_split ? (int)std::min<int64_t>(std::max(1, kblocks / 4),
+                                                                std::max<int64_t>(1, units / tiles))
+                                       : 1;
+            for (int s = 1; s <= most; ++s) {
+                const int per = (kblocks + s - 1) / s;
+                const int splits = (kblocks + per - 1) / per;
+                const double waves = (double)((tiles * splits + units - 1) / units);
+                const double lines = 1.0 * (kBM + (pair ? bn / 2 : bn));
+                const double main = per * std::max(2.0 * bn, lines * 1.5);
+                const double epi = 10.0 * bn;
+                double cost = 2000.0 + waves * std::max(main, epi) + std::min(main, epi);
+                if (splits > 1)
+                    cost += 5000.0 + (double)m * n_cols * (splits + 1) * 4.0 / 3000.0;
+                if (best.bn == 0 || cost < best_cost) {
+                    best_cost = cost;
+                    best = {bn, splits, per, 0, pair == 1};
+                }
             }
         }
     }
-    const uint32_t stage = kAStage + (uint32_t)best.bn * kLineBytes;
+    const uint32_t stage =
+        kAStage + (uint32_t)(best.pair ? best.bn / 2 : best.bn) * kLineBytes;
     best.stages = (int)std::min<uint32_t>(kMaxStages, (kSmemMax - fixed) / stage);
     return best;
 }
 
-template <int MODE, typename T, bool FP8>
+template <int MODE, typename T, bool FP8, bool PAIR>
 void launch_tile(const CUtensorMap& a, const CUtensorMap& b, const TileParams& p, int sms,
                  int device, cudaStream_t stream) {
-    const size_t smem = (size_t)p.stages * (kAStage + (size_t)p.bn * kLineBytes) +
-                        kFixedSmem<MODE>;
     static std::atomic<uint64_t> allowed{0};  // devices whose limit is raised
     if (device >= 64 || !(allowed.load(std::memory_order_relaxed) >> device & 1)) {
-        RUNE_CUDA_TRY(cudaFuncSetAttribute(k_tile<MODE, T, FP8>,
+        RUNE_CUDA_TRY(cudaFuncSetAttribute(k_tile<MODE, T, FP8, PAIR>,
                                            cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            (int)kSmemMax));
         if (device < 64) allowed.fetch_or(uint64_t(1) << device, std::memory_order_relaxed);
     }
     const int64_t work = (int64_t)p.tiles_m * p.tiles_n * p.splits;
-    const int grid = (int)std::min<int64_t>(work, sms);
-    k_tile<MODE, T, FP8><<<grid, kThreads, smem, stream>>>(a, b, p);
-    RUNE_LAUNCH_CHECK();
+    const int b_rows = PAIR ? p.bn / 2 : p.bn;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = PAIR ? 2 * (unsigned)std::min<int64_t>(work, sms / 2)
+                       : (unsigned)std::min<int64_t>(work, sms);
+    cfg.blockDim = kThreads;
+    cfg.dynamicSmemBytes =
+        (size_t)p.stages * (kAStage + (size_t)b_rows * kLineBytes) + kFixedSmem<MODE>;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim = {2, 1, 1};
+    cfg.attrs = at;
+    cfg.numAttrs = PAIR ? 1 : 0;
+    RUNE_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_tile<MODE, T, FP8, PAIR>, a, b, p));
 }
 
 // One product D[m, n] = A B^T: operands, epilogue (in p) and scratch for a split.
@@ -779,22 +839,30 @@ void run_mode(const Product& g, TileParams p, Scratch& ws, int device, cudaStrea
     p.splits = plan.splits;
     p.kb_per_split = plan.kb_per_split;
     p.stages = plan.stages;
-    p.tiles_m = (int)((p.m + kBM - 1) / kBM);
+    const int tile_rows = plan.pair ? 2 * kBM : kBM;
+    p.tiles_m = (int)((p.m + tile_rows - 1) / tile_rows);
     p.a_mn = g.a_mn, p.b_mn = g.b_mn;
-    p.idesc = operand_idesc(fp8 ? 0 : g.dtype == RUNE_BF16 ? 1 : 0, g.a_mn, g.b_mn, kBM, p.bn);
+    p.idesc = operand_idesc(fp8 ? 0 : g.dtype == RUNE_BF16 ? 1 : 0, g.a_mn, g.b_mn, tile_rows,
+                            p.bn);
+    const int b_box = plan.pair || pair ? p.bn / 2 : p.bn;  // lines of B in one copy
     p.flag = wait_flag(device);
     const CUtensorMap ma = make_map(g.a, eb, g.a_mn ? 64 : kBM);
     if (plan.splits == 1) {
         const int width = pair ? p.bn / 2 : p.bn;
         p.tiles_n = (int)((p.n + width - 1) / width);
-        const CUtensorMap mb = make_map(g.b, eb, g.b_mn ? 64 : width);
+        const CUtensorMap mb = make_map(g.b, eb, g.b_mn ? 64 : b_box);
+        auto go = [&](auto fp8_c) {
+            constexpr bool FP8 = decltype(fp8_c)::value;
+            if (plan.pair) launch_tile<MODE, T, FP8, true>(ma, mb, p, sms, device, stream);
+            else launch_tile<MODE, T, FP8, false>(ma, mb, p, sms, device, stream);
+        };
         if constexpr (MODE == kForward || MODE == kGated) {
             if (fp8) {
-                launch_tile<MODE, T, true>(ma, mb, p, sms, device, stream);
+                go(std::true_type());
                 return;
             }
         }
-        launch_tile<MODE, T, false>(ma, mb, p, sms, device, stream);
+        go(std::false_type());
         return;
     }
     if constexpr (MODE == kForward || MODE == kGated) {
@@ -803,9 +871,16 @@ void run_mode(const Product& g, TileParams p, Scratch& ws, int device, cudaStrea
         q.tiles_n = (int)((n_cols + p.bn - 1) / p.bn);
         q.z = part;
         q.ld_z = ld_part;
-        const CUtensorMap mb = make_map(g.b, eb, g.b_mn ? 64 : p.bn);
-        if (fp8) launch_tile<kPartial, __half, true>(ma, mb, q, sms, device, stream);
-        else launch_tile<kPartial, __half, false>(ma, mb, q, sms, device, stream);
+        const CUtensorMap mb = make_map(g.b, eb, g.b_mn ? 64 : plan.pair ? p.bn / 2 : p.bn);
+        auto go = [&](auto fp8_c) {
+            constexpr bool FP8 = decltype(fp8_c)::value;
+            if (plan.pair)
+                launch_tile<kPartial, __half, FP8, true>(ma, mb, q, sms, device, stream);
+            else
+                launch_tile<kPartial, __half, FP8, false>(ma, mb, q, sms, device, stream);
+        };
+        if (fp8) go(std::true_type());
+        else go(std::false_type());
         const int64_t items = p.m * ((p.n + 3) / 4);
         const int grid = (int)std::min<int64_t>((items + 255) / 256, (int64_t)sms * 16);
         k_join<MODE, T><<<grid, 256, 0, stream>>>(p, part);
@@ -949,9 +1024,8 @@ void backward(const rune_linear_grad_args& a, Scratch& ws, cudaStream_t stream) 
                 RUNE_LAUNCH_CHECK();
             }
         } else {
-            const int64_t tiles_m = (a.rows + kBM - 1) / kBM;
-            parts = tiles_m * 4;
-            if (a.dbias) sums = ws.take<float>(parts * n_all);
+            parts = (a.rows + 31) / 32;  // one a warp; the last tile (of a pair) has more warps
+            if (a.dbias) sums = ws.take<float>((parts + 7) / 8 * 8 * n_all);
             Product g;
             g.a = x, g.b = w;
             g.mode = a.gated ? kGatedGrad : kGrad;

@@ -41,21 +41,87 @@ __host__ __device__ constexpr uint32_t operand_idesc(int type, bool a_mn, bool b
            ((uint32_t)(m >> 4) << 24);
 }
 
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                        bool accumulate) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-        : "memory");
+// D[tmem] (+)= A B^T on f16 / bf16 or e4m3 operands; PAIR: by the tensor cores of two blocks,
+// issued by the even one. One thread issues.
+template <bool FP8, bool PAIR>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                    bool accumulate) {
+    const uint32_t acc = accumulate;
+#define RUNE_MMA(group, kind)                                                       \
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"                      \
+                 " tcgen05.mma.cta_group::" group ".kind::" kind                    \
+                 " [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), \
+                 "r"(acc)                                                           \
+                 : "memory")
+    if constexpr (FP8 && PAIR) RUNE_MMA("2", "f8f6f4");
+    else if constexpr (FP8) RUNE_MMA("1", "f8f6f4");
+    else if constexpr (PAIR) RUNE_MMA("2", "f16");
+    else RUNE_MMA("1", "f16");
+#undef RUNE_MMA
 }
 
-__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                       bool accumulate) {
+// ---- clusters
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+// every thread of every block of the cluster (converged warps)
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;"
+                 ::: "memory");
+}
+// this block's shared address `addr` in the cluster's block `rank`
+__device__ __forceinline__ uint32_t peer_address(uint32_t addr, uint32_t rank) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+    return a;
+}
+// loads from a peer's shared memory; volatile keeps them between the cluster's barriers
+__device__ __forceinline__ float peer_float(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ uint32_t peer_word(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ void mbar_arrive_peer(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
+                 : "memory");
+}
+
+// ---- pairs of blocks on one tile
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(tc::smem_u32(dst)), "r"(cols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols));
+}
+// the barrier at `bar` in both blocks receives an arrival when every product issued so far by
+// this thread is complete
+__device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], %1;" ::"r"(bar), "h"((uint16_t)3)
+        : "memory");
+}
+// a tile into this block's memory, counted on barrier `bar` (cluster address) of the even block
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y,
+                                              uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        ".cta_group::2 [%0], [%1, {%2, %3}], [%4];"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar)
         : "memory");
 }
 

@@ -47,30 +47,6 @@ struct FewShared {
     int issued;
 };
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;"
-                 ::: "memory");
-}
-// float at shared address `addr` of the cluster's block `rank`
-__device__ __forceinline__ float peer_float(uint32_t addr, uint32_t rank) {
-    uint32_t a;
-    float v;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-    // volatile keeps it between the cluster's barriers
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a));
-    return v;
-}
-
 template <typename T, bool FP8>
 __global__ void __launch_bounds__(kThreads)
 k_few(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
@@ -153,10 +129,7 @@ k_few(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtenso
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const bool more = kb > kb0 || k > 0;
-                    if constexpr (FP8)
-                        mma_f8(tmem, desc_w + at + 2 * k, desc_x + at + 2 * k, p.idesc, more);
-                    else
-                        mma_f16(tmem, desc_w + at + 2 * k, desc_x + at + 2 * k, p.idesc, more);
+                    mma<FP8, false>(tmem, desc_w + at + 2 * k, desc_x + at + 2 * k, p.idesc, more);
                 }
                 mma_commit(smem_u32(&sh.empty[st]));
             }
@@ -221,7 +194,7 @@ k_few(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtenso
                 } else {
 #pragma unroll
                     for (int r = 0; r < 8; ++r)
-                        if (r < (int)splits) v[i][r] = peer_float(base + at * 4, r);
+                        if (r < (int)splits) v[i][r] = peer_float(peer_address(base + at * 4, r));
                 }
             }
 #pragma unroll
