@@ -50,7 +50,7 @@ struct TileParams {
     int kblocks, kb_per_split, splits;
     int tiles_m, tiles_n, bn, stages;
     int a_mn, b_mn, act;
-    int vec_out, vec_in, vec_z;  // 16-byte accesses allowed
+    int vec_out, vec_in, vec_z, vec_bias;  // 16-byte accesses allowed
     uint32_t idesc;
     void* out;
     const void* in;         // residual, or dy
@@ -68,7 +68,6 @@ struct TileShared {
     uint32_t tmem;
     int fail;
     int issued;             // stages whose copies were issued
-    float bias[256], w_scale[256];
 };
 
 // buffers of kWarpBuf per epilogue warp, and all shared memory beside the ring
@@ -212,16 +211,35 @@ __device__ __forceinline__ void store_rows32(unsigned char* buf, const float (&v
     __syncwarp();
 }
 
-// acc -> z: scales of e4m3 operands and bias of 32 columns
-template <int MODE>
-__device__ __forceinline__ void finish_z(float (&v)[32], const float* bias, const float* w_scale,
-                                         float x_scale, bool scaled) {
-    if (scaled) {
+// acc -> z for 32 columns from `col` (left of them inside): scales of e4m3 operands and bias,
+// read by all lanes at once
+template <typename T, bool FP8>
+__device__ __forceinline__ void finish_z(float (&v)[32], const TileParams& p, int64_t col,
+                                         int64_t left, float x_scale) {
+    if constexpr (FP8) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = v[j] * (x_scale * w_scale[j]) + bias[j];
-    } else {
+        for (int j = 0; j < 32; ++j)
+            v[j] *= x_scale * (j < left ? __ldg(p.w_scale + col + j) : 0.0f);
+    }
+    if (p.bias) {
+        const T* bias = static_cast<const T*>(p.bias) + col;
+        if (p.vec_bias) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] += bias[j];
+            for (int g = 0; g < 4; ++g) {
+                if (g * 8 >= left) continue;
+                const uint4 q = __ldg(reinterpret_cast<const uint4*>(bias) + g);
+                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 f = unpack2<T>(w[j]);
+                    v[g * 8 + 2 * j] += f.x, v[g * 8 + 2 * j + 1] += f.y;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (j < left) v[j] += to_float(bias[j]);
+        }
     }
 }
 
@@ -251,41 +269,42 @@ __device__ __forceinline__ void get_row(unsigned char* buf, int lane, int half, 
 }
 
 // One warp's part of a finished tile: 32 rows (a warp reads the quarter of TMEM's lanes that its
-// number gives) and every other group of columns, the rest being its partner's.
-template <int MODE, typename T>
+// number gives) and every other group of columns, the rest being its partner's. `release` is
+// called when the accumulator has been read.
+template <int MODE, typename T, bool FP8, typename Release>
 __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uint32_t acc,
-                                         unsigned char* buf, const float* bias,
-                                         const float* w_scale, int warp, int lane) {
+                                         unsigned char* buf, int warp, int lane,
+                                         Release&& release) {
     const int quarter = warp & 3, half_of = warp >> 2;
     const int row0 = t.mt * kBM + quarter * 32;
     const int rows = (int)max((int64_t)0, min((int64_t)32, p.m - row0));
-    constexpr bool kPair = MODE == kGated || MODE == kGatedGrad;
-    const int width = kPair ? p.bn / 2 : p.bn;  // output columns of the tile
+    constexpr bool kGate = MODE == kGated || MODE == kGatedGrad;
+    const int width = kGate ? p.bn / 2 : p.bn;  // output columns of the tile
     const int64_t col0 = (int64_t)t.nt * width;
+    const int end = (int)min((int64_t)width, p.n - col0);
     if constexpr (MODE == kPartial) {
-        for (int c = half_of * 32; c < width && col0 + c < p.n; c += 64) {
+        for (int c = half_of * 32; c < end; c += 64) {
             float v[32];
             tc::tmem_ld32(acc + c, v);
             store_rows32(buf, v, p.z + ((int64_t)t.split * p.m + row0) * p.ld_z + col0 + c,
-                         p.ld_z, rows, p.n - (col0 + c), true, lane);
+                         p.ld_z, rows, end - c, true, lane);
         }
+        release();
         return;
     }
-    const bool scaled = p.x_scale != nullptr;
-    const float xs = scaled && lane < rows ? p.x_scale[row0 + lane] : 0.0f;
-    for (int c = half_of * 64; c < width && col0 + c < p.n; c += 128) {
+    const float xs = FP8 && lane < rows ? p.x_scale[row0 + lane] : 0.0f;
+    for (int c = half_of * 64; c < end; c += 128) {
         const int64_t col = col0 + c, left = p.n - col;
         if constexpr (MODE == kForward || MODE == kGated) {
             if (p.z) {  // the pre-activations, in float32
-                for (int part = 0; part < (kPair ? 2 : 1); ++part) {
+                for (int part = 0; part < (kGate ? 2 : 1); ++part) {
                     for (int half = 0; half < 2 && half * 32 < left; ++half) {
-                        const int at = c + part * width + half * 32;
+                        const int64_t at = part * p.n + col + half * 32;
                         float v[32];
-                        tc::tmem_ld32(acc + at, v);
-                        finish_z<MODE>(v, bias + at, w_scale + at, xs, scaled);
-                        store_rows32(buf, v,
-                                     p.z + (int64_t)row0 * p.ld_z + part * p.n + col + half * 32,
-                                     p.ld_z, rows, left - half * 32, p.vec_z, lane);
+                        tc::tmem_ld32(acc + c + part * width + half * 32, v);
+                        finish_z<T, FP8>(v, p, at, left - half * 32, xs);
+                        store_rows32(buf, v, p.z + (int64_t)row0 * p.ld_z + at, p.ld_z, rows,
+                                     left - half * 32, p.vec_z, lane);
                     }
                 }
             }
@@ -295,23 +314,43 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
                       rows, left, p.vec_in, lane);
             __syncwarp();
         }
-#pragma unroll
+#pragma unroll 1
         for (int half = 0; half < 2; ++half) {
-            float v[32];
-            tc::tmem_ld32(acc + c + half * 32, v);
-            finish_z<MODE>(v, bias + c + half * 32, w_scale + c + half * 32, xs, scaled);
+            float v[32], u[32];
+            const int at = c + half * 32;
+            const int64_t zcol = col + half * 32, zleft = left - half * 32;
+            if constexpr (kGate) tmem_ld32x2(acc + at, acc + at + width, v, u);
+            else tc::tmem_ld32(acc + at, v);
+            if (half == 1 && c + 128 >= end) release();
+            finish_z<T, FP8>(v, p, zcol, zleft, xs);
+            if constexpr (kGate) finish_z<T, FP8>(u, p, p.n + zcol, zleft, xs);
             if constexpr (MODE == kForward) {
                 with_activation(p.act, [&](auto a) {
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] = act_value<decltype(a)::value>(v[j]);
                 });
                 if (p.in) {
-                    float r[32];
-                    get_row<T>(buf, lane, half, r);
+                    get_row<T>(buf, lane, half, u);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] += r[j];
+                    for (int j = 0; j < 32; ++j) v[j] += u[j];
                 }
             } else if constexpr (MODE == kGrad) {
+                get_row<T>(buf, lane, half, u);
+                with_activation(p.act, [&](auto a) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        float y, da;
+                        act_both<decltype(a)::value>(v[j], y, da);
+                        v[j] = u[j] * da;
+                    }
+                });
+            } else if constexpr (MODE == kGated) {
+                with_activation(p.act, [&](auto a) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        v[j] = act_value<decltype(a)::value>(v[j]) * u[j];
+                });
+            } else {
                 float d[32];
                 get_row<T>(buf, lane, half, d);
                 with_activation(p.act, [&](auto a) {
@@ -319,40 +358,17 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
                     for (int j = 0; j < 32; ++j) {
                         float y, da;
                         act_both<decltype(a)::value>(v[j], y, da);
-                        v[j] = d[j] * da;
+                        v[j] = d[j] * u[j] * da;
+                        u[j] = d[j] * y;
                     }
                 });
-            } else {
-                float u[32];
-                const int at = width + c + half * 32;
-                tc::tmem_ld32(acc + at, u);
-                finish_z<MODE>(u, bias + at, w_scale + at, xs, scaled);
-                if constexpr (MODE == kGated) {
-                    with_activation(p.act, [&](auto a) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            v[j] = act_value<decltype(a)::value>(v[j]) * u[j];
-                    });
-                } else {
-                    float d[32];
-                    get_row<T>(buf, lane, half, d);
-                    with_activation(p.act, [&](auto a) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            float y, da;
-                            act_both<decltype(a)::value>(v[j], y, da);
-                            v[j] = d[j] * u[j] * da;
-                            u[j] = d[j] * y;
-                        }
-                    });
-                    put_row<T>(buf + kWarpBuf, lane, half, u);
-                }
+                put_row<T>(buf + kWarpBuf, lane, half, u);
             }
             put_row<T>(buf, lane, half, v);
         }
         __syncwarp();
         constexpr bool kSums = MODE == kGrad || MODE == kGatedGrad;
-        const int64_t ncols = kPair ? 2 * p.n : p.n;
+        const int64_t ncols = kGate ? 2 * p.n : p.n;
         float* sums = kSums && p.colsum
                           ? p.colsum + ((int64_t)t.mt * 4 + quarter) * ncols + col
                           : nullptr;
@@ -363,6 +379,7 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
                                 sums ? sums + p.n : nullptr);
         __syncwarp();
     }
+    if (half_of * 64 >= end) release();  // no columns here
 }
 
 // PAIR: two blocks of a cluster (the two SMs of a TPC) work on one tile of 256 rows. Each holds its
@@ -532,38 +549,23 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
             Tile t = tile_of(p, w);
             if (PAIR) t.mt = t.mt * 2 + rank;
             const int b = n_tile & 1, round = n_tile >> 1;
-            if constexpr (MODE != kPartial) {
-                // bias and weight scales of the tile's columns
-                const int width = kGate ? p.bn / 2 : p.bn;
-                if (n_tile > 0) asm volatile("bar.sync 1, 256;" ::: "memory");
-                if (tid < p.bn) {
-                    const int part = tid / width;
-                    const int64_t col = (int64_t)t.nt * width + tid % width;
-                    const bool in = col < p.n;
-                    sh->bias[tid] = in && p.bias ? to_float(static_cast<const T*>(
-                                                       p.bias)[part * p.n + col])
-                                                 : 0.0f;
-                    sh->w_scale[tid] = in && p.w_scale ? p.w_scale[part * p.n + col] : 0.0f;
-                }
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-            }
-            // after a failure the warps still meet at the barriers above for every tile
-            bool ok = !*fail && mbar_wait(smem_u32(&sh->acc_full[b]), round & 1) && !*fail;
+            const bool ok = mbar_wait(smem_u32(&sh->acc_full[b]), round & 1) && !*fail;
             if (!__all_sync(0xffffffffu, ok)) {
                 *fail = 1;
-                continue;
+                break;
             }
             fence_after_sync();
-            epilogue<MODE, T>(p, t, tmem + b * 256 + ((uint32_t)((warp & 3) * 32) << 16), buf,
-                              sh->bias, sh->w_scale, warp, lane);
-            fence_before_sync();
-            __syncwarp();
-            if (lane == 0) {
-                if constexpr (PAIR)
-                    mbar_arrive_peer(peer_address(smem_u32(&sh->acc_empty[b]), 0));
-                else
-                    mbar_arrive(smem_u32(&sh->acc_empty[b]));
-            }
+            epilogue<MODE, T, FP8>(
+                p, t, tmem + b * 256 + ((uint32_t)((warp & 3) * 32) << 16), buf, warp, lane, [&] {
+                    fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if constexpr (PAIR)
+                            mbar_arrive_peer(peer_address(smem_u32(&sh->acc_empty[b]), 0));
+                        else
+                            mbar_arrive(smem_u32(&sh->acc_empty[b]));
+                    }
+                });
         }
     }
     __syncwarp();
@@ -746,10 +748,16 @@ struct Plan {
     bool pair;
 };
 
-// Tile, range of k and pairing of one product, by a model of its time in cycles: a k-block of 64
-// costs bn * 2 cycles of the tensor core (never less than the lines of shared memory that it
-// reads), an epilogue 10 cycles a column, hidden behind the next tile's products, and a join of
-// splits a launch and its traffic.
+// Cycles that a k-block of 64 takes (measured on B200 at sizes that fill it): the tensor cores'
+// 2 cycles a column for the widest tile of a pair, more for the others, which read more shared
+// memory for a product.
+double block_cycles(bool pair, int bn) {
+    return pair ? (bn == 256 ? 520.0 : 370.0) : bn == 256 ? 660.0 : bn == 128 ? 400.0 : 300.0;
+}
+
+// Tile, range of k and pairing of one product, by a model of its time in cycles: the k-blocks, an
+// epilogue of 10 cycles a column, hidden behind the next tile's products, and for ranges of k the
+// launch and the traffic of their join.
 Plan plan_product(int64_t m, int64_t n_cols, int kblocks, bool can_split, bool gate, int sms,
                   uint32_t fixed) {
     Plan best{};
@@ -766,8 +774,7 @@ Plan plan_product(int64_t m, int64_t n_cols, int kblocks, bool can_split, bool g
                 const int per = (kblocks + s - 1) / s;
                 const int splits = (kblocks + per - 1) / per;
                 const double waves = (double)((tiles * splits + units - 1) / units);
-                const double lines = 1.0 * (kBM + (pair ? bn / 2 : bn));
-                const double main = per * std::max(2.0 * bn, lines * 1.5);
+                const double main = per * block_cycles(pair, bn);
                 const double epi = 10.0 * bn;
                 double cost = 2000.0 + waves * std::max(main, epi) + std::min(main, epi);
                 if (splits > 1)
@@ -958,6 +965,7 @@ void forward(const rune_linear_args& a, Scratch& ws, cudaStream_t stream) {
     p.in = a.residual, p.ld_in = a.residual_stride;
     p.vec_in = a.residual && wide16(a.residual, a.residual_stride, a.outputs);
     p.bias = a.bias;
+    p.vec_bias = aligned(a.bias, 16) && a.outputs % 8 == 0;
     p.x_scale = a.x_scale, p.w_scale = a.weight_scale;
     p.z = a.saved, p.ld_z = n_all;
     p.vec_z = aligned(a.saved, 16) && a.outputs % 4 == 0;
@@ -1039,6 +1047,7 @@ void backward(const rune_linear_grad_args& a, Scratch& ws, cudaStream_t stream) 
             p.in = a.dy, p.ld_in = a.dy_stride;
             p.vec_in = wide16(a.dy, a.dy_stride, a.outputs);
             p.bias = a.bias;
+            p.vec_bias = aligned(a.bias, 16) && a.outputs % 8 == 0;
             p.colsum = sums;
             run_product(g, p, ws, a.device, stream);
         }
