@@ -10,11 +10,13 @@
 // swizzled tiles that TMA writes. Tails of every size are zeros that TMA fills in.
 //
 // A block works on tiles of 128 rows x bn accumulator columns (bn = 64, 128 or 256):
-//   warp 8    one thread streams tiles of A and B (64 values of k; 128 for e4m3) by TMA into a
-//             ring of as many stages as fit;
-//   warp 9    one thread issues the products into one of two TMEM accumulators;
-//   warps 0-7 the epilogue of the other accumulator: a lane holds a row, so that tiles pass
-//             through shared memory on their way to and from global memory, 128 bytes a row.
+//   warp 16    one thread streams tiles of A and B (64 values of k; 128 for e4m3) by TMA into a
+//              ring of as many stages as fit;
+//   warp 17    one thread issues the products into one of two TMEM accumulators;
+//   warps 0-15 the epilogue of the other accumulator: a lane holds a row, so that tiles pass
+//              through shared memory on their way to and from global memory, 64 bytes a row. Four
+//              warps a scheduler, since every instruction waits some cycles for the one before
+//              (gated 110592 x 256 -> 512 forward: 8 warps 101 us).
 // Every wait is bounded; one that gives up raises the device's wait flag and ends the block.
 
 #include <algorithm>
@@ -37,10 +39,11 @@ enum Mode {
 };
 
 constexpr int kBM = 128;
-constexpr int kEpiWarps = 8, kTmaWarp = 8, kMmaWarp = 9;
-constexpr int kThreads = 320;
+constexpr int kEpiWarps = 16, kTmaWarp = 16, kMmaWarp = 17;
+constexpr int kThreads = 32 * 18;
 constexpr uint32_t kAStage = kBM * kLineBytes;  // 16 KB
-constexpr uint32_t kWarpBuf = 32 * kLineBytes;  // 4 KB: 32 rows of 64 16-bit or 32 float values
+constexpr uint32_t kRowBytes = 64;               // of a warp's buffer: 32 16-bit or 16 float values
+constexpr uint32_t kWarpBuf = 32 * kRowBytes;    // 2 KB
 constexpr int kMaxStages = 8;
 constexpr uint32_t kSmemMax = 227 * 1024;
 
@@ -83,48 +86,47 @@ struct Tile {
 
 // Tiles in groups of 16 tile rows, column by column, so that the blocks at work share a few
 // lines of both operands in L2; the ranges of k of one tile come last.
-__device__ __forceinline__ Tile tile_of(const TileParams& p, int64_t w) {
-    constexpr int G = 16;
-    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-    Tile t;
-    t.split = (int)(w / tiles);
-    int64_t id = w % tiles;
-    int64_t per = (int64_t)G * p.tiles_n, g = id / per, in = id % per;
-    int gm = (int)min((int64_t)G, p.tiles_m - g * G);
-    t.mt = (int)(g * G + in % gm);
-    t.nt = (int)(in / gm);
+__device__ __forceinline__ Tile tile_of(const TileParams& p, unsigned w) {
+    constexpr unsigned G = 16;
+    Tile t{0, 0, 0};
+    if (p.splits > 1) {
+        const unsigned tiles = (unsigned)p.tiles_m * p.tiles_n;
+        t.split = w / tiles;
+        w -= t.split * tiles;
+    }
+    const unsigned per = G * p.tiles_n, g = w / per, in = w - g * per;
+    const unsigned gm = min(G, p.tiles_m - g * G);
+    t.nt = gm == G ? in / G : in / gm;
+    t.mt = g * G + (in - t.nt * gm);
     return t;
 }
 
-// ---- a warp's 32 rows x 64 columns of 16-bit values between global memory and its buffer.
-// Rows are 128-byte lines of eight 16-byte pieces, piece c of row r at c ^ (r & 7), so that both
-// the row-wise accesses of the lanes and the coalesced ones spread over the banks.
+// ---- a warp's 32 rows x 32 columns of 16-bit values between global memory and its buffer.
+// Rows are four pieces of 16 bytes, piece c of row r at c ^ (r / 2 & 3), so that both the row-wise
+// accesses of the lanes and the coalesced ones spread over the banks.
 __device__ __forceinline__ uint4* piece(unsigned char* buf, int r, int c) {
-    return reinterpret_cast<uint4*>(buf + r * kLineBytes + ((c ^ (r & 7)) << 4));
+    return reinterpret_cast<uint4*>(buf + r * kRowBytes + ((c ^ ((r >> 1) & 3)) << 4));
 }
 
 template <typename T>
 __device__ __forceinline__ void load_rows(unsigned char* buf, const T* src, int64_t ld,
                                           int rows, int64_t cols, bool vec, int lane) {
     if (vec) {
-        const int c = lane & 7;
+        const int c = lane & 3;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int r = i * 4 + (lane >> 3);
+        for (int i = 0; i < 4; ++i) {
+            const int r = i * 8 + (lane >> 2);
             uint4 v = make_uint4(0, 0, 0, 0);
             if (r < rows && c * 8 < cols)
                 v = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)r * ld + c * 8));
             *piece(buf, r, c) = v;
         }
     } else {
+#pragma unroll 8
         for (int r = 0; r < 32; ++r) {
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int c = lane + 32 * half;
-                T v = from_float<T>(0.0f);
-                if (r < rows && c < cols) v = src[(int64_t)r * ld + c];
-                reinterpret_cast<T*>(piece(buf, r, c >> 3))[c & 7] = v;
-            }
+            T v = from_float<T>(0.0f);
+            if (r < rows && lane < cols) v = src[(int64_t)r * ld + lane];
+            reinterpret_cast<T*>(piece(buf, r, lane >> 3))[lane & 7] = v;
         }
     }
 }
@@ -134,13 +136,13 @@ template <typename T, bool SUMS>
 __device__ __forceinline__ void store_rows(unsigned char* buf, T* dst, int64_t ld, int rows,
                                            int64_t cols, bool vec, int lane, float* sums) {
     if (vec) {
-        const int c = lane & 7;
+        const int c = lane & 3;
         float s[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) s[j] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int r = i * 4 + (lane >> 3);
+        for (int i = 0; i < 4; ++i) {
+            const int r = i * 8 + (lane >> 2);
             uint4 v = *piece(buf, r, c);
             if (r < rows && c * 8 < cols)
                 *reinterpret_cast<uint4*>(dst + (int64_t)r * ld + c * 8) = v;
@@ -157,125 +159,139 @@ __device__ __forceinline__ void store_rows(unsigned char* buf, T* dst, int64_t l
             if (sums) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    s[j] += __shfl_xor_sync(0xffffffffu, s[j], 8);
-                    s[j] += __shfl_xor_sync(0xffffffffu, s[j], 16);
-                    if (lane < 8 && c * 8 + j < cols) sums[c * 8 + j] = s[j];
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) s[j] += __shfl_xor_sync(0xffffffffu, s[j], o);
+                    if (lane < 4 && c * 8 + j < cols) sums[c * 8 + j] = s[j];
                 }
             }
         }
     } else {
-        float s[2] = {0.0f, 0.0f};
+        float s = 0.0f;
+#pragma unroll 8
         for (int r = 0; r < 32; ++r) {
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int c = lane + 32 * half;
-                T v = reinterpret_cast<T*>(piece(buf, r, c >> 3))[c & 7];
-                if (r < rows && c < cols) dst[(int64_t)r * ld + c] = v;
-                if constexpr (SUMS) s[half] += to_float(v);
-            }
+            T v = reinterpret_cast<T*>(piece(buf, r, lane >> 3))[lane & 7];
+            if (r < rows && lane < cols) dst[(int64_t)r * ld + lane] = v;
+            if constexpr (SUMS) s += to_float(v);
         }
         if constexpr (SUMS) {
-            if (sums) {
-#pragma unroll
-                for (int half = 0; half < 2; ++half)
-                    if (lane + 32 * half < cols) sums[lane + 32 * half] = s[half];
-            }
+            if (sums && lane < cols) sums[lane] = s;
         }
     }
 }
 
-// a warp's 32 rows x 32 columns of float32, each lane its row, through the buffer to memory
-__device__ __forceinline__ void store_rows32(unsigned char* buf, const float (&v)[32], float* dst,
+// a warp's 32 rows x 16 columns of float32, each lane its row, through the buffer to memory
+__device__ __forceinline__ void store_rows32(unsigned char* buf, const float (&v)[16], float* dst,
                                              int64_t ld, int rows, int64_t cols, bool vec,
                                              int lane) {
     __syncwarp();
 #pragma unroll
-    for (int c = 0; c < 8; ++c)
+    for (int c = 0; c < 4; ++c)
         *reinterpret_cast<float4*>(piece(buf, lane, c)) =
             make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
     __syncwarp();
     if (vec) {
-        const int c = lane & 7;
+        const int c = lane & 3;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int r = i * 4 + (lane >> 3);
+        for (int i = 0; i < 4; ++i) {
+            const int r = i * 8 + (lane >> 2);
             if (r < rows && c * 4 < cols)
                 *reinterpret_cast<uint4*>(dst + (int64_t)r * ld + c * 4) = *piece(buf, r, c);
         }
     } else {
-        for (int r = 0; r < 32; ++r)
-            if (r < rows && lane < cols)
-                dst[(int64_t)r * ld + lane] =
-                    reinterpret_cast<float*>(piece(buf, r, lane >> 2))[lane & 3];
+        const int c = lane & 15;
+#pragma unroll 8
+        for (int i = 0; i < 16; ++i) {
+            const int r = 2 * i + (lane >> 4);
+            if (r < rows && c < cols)
+                dst[(int64_t)r * ld + c] = reinterpret_cast<float*>(piece(buf, r, c >> 2))[c & 3];
+        }
     }
     __syncwarp();
 }
 
-// acc -> z for 32 columns from `col` (left of them inside): scales of e4m3 operands and bias,
-// read by all lanes at once
-template <typename T, bool FP8>
-__device__ __forceinline__ void finish_z(float (&v)[32], const TileParams& p, int64_t col,
-                                         int64_t left, float x_scale) {
-    if constexpr (FP8) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            v[j] *= x_scale * (j < left ? __ldg(p.w_scale + col + j) : 0.0f);
-    }
-    if (p.bias) {
+// Bias of 16 columns from `col` (left of them inside), read by all lanes at once and before the
+// accumulator, so that the two waits overlap.
+template <typename T>
+struct Bias {
+    uint32_t w[8];
+    __device__ __forceinline__ void load(const TileParams& p, int64_t col, int64_t left) {
         const T* bias = static_cast<const T*>(p.bias) + col;
+        if (!p.bias) return;
         if (p.vec_bias) {
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                if (g * 8 >= left) continue;
-                const uint4 q = __ldg(reinterpret_cast<const uint4*>(bias) + g);
-                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 f = unpack2<T>(w[j]);
-                    v[g * 8 + 2 * j] += f.x, v[g * 8 + 2 * j + 1] += f.y;
-                }
+            for (int g = 0; g < 2; ++g) {
+                uint4 q = make_uint4(0, 0, 0, 0);
+                if (g * 8 < left) q = __ldg(reinterpret_cast<const uint4*>(bias) + g);
+                w[4 * g] = q.x, w[4 * g + 1] = q.y, w[4 * g + 2] = q.z, w[4 * g + 3] = q.w;
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (j < left) v[j] += to_float(bias[j]);
+            for (int j = 0; j < 8; ++j)
+                w[j] = pack2<T>(2 * j < left ? to_float(bias[2 * j]) : 0.0f,
+                                2 * j + 1 < left ? to_float(bias[2 * j + 1]) : 0.0f);
+        }
+    }
+};
+
+// acc -> z: scales of e4m3 operands and bias
+template <typename T, bool FP8>
+__device__ __forceinline__ void finish_z(const float (&v)[16], Two (&z)[8], const Bias<T>& bias,
+                                         const TileParams& p, int64_t col, int64_t left,
+                                         float x_scale) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        z[j] = two(v[2 * j], v[2 * j + 1]);
+        if constexpr (FP8) {
+            const float s0 = 2 * j < left ? __ldg(p.w_scale + col + 2 * j) : 0.0f;
+            const float s1 = 2 * j + 1 < left ? __ldg(p.w_scale + col + 2 * j + 1) : 0.0f;
+            z[j] = z[j] * (two(x_scale) * two(s0, s1));
+        }
+        if (p.bias) {
+            const float2 f = unpack2<T>(bias.w[j]);
+            z[j] = z[j] + two(f.x, f.y);
         }
     }
 }
 
-// 32 values of a lane's row to pieces 4 half .. 4 half + 3 of its line
+// 16 values of a lane's row to and from pieces 2 half, 2 half + 1 of its line
 template <typename T>
 __device__ __forceinline__ void put_row(unsigned char* buf, int lane, int half,
-                                        const float (&v)[32]) {
+                                        const Two (&v)[8]) {
+    uint32_t w[8];
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-        *piece(buf, lane, half * 4 + c) =
-            make_uint4(pack2<T>(v[8 * c], v[8 * c + 1]), pack2<T>(v[8 * c + 2], v[8 * c + 3]),
-                       pack2<T>(v[8 * c + 4], v[8 * c + 5]), pack2<T>(v[8 * c + 6], v[8 * c + 7]));
+    for (int j = 0; j < 8; ++j) {
+        float a, b;
+        split(v[j], a, b);
+        w[j] = pack2<T>(a, b);
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+        *piece(buf, lane, half * 2 + c) =
+            make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
 }
 
 template <typename T>
-__device__ __forceinline__ void get_row(unsigned char* buf, int lane, int half, float (&v)[32]) {
+__device__ __forceinline__ void get_row(unsigned char* buf, int lane, int half, Two (&v)[8]) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        uint4 q = *piece(buf, lane, half * 4 + c);
+    for (int c = 0; c < 2; ++c) {
+        uint4 q = *piece(buf, lane, half * 2 + c);
         const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             float2 f = unpack2<T>(w[j]);
-            v[8 * c + 2 * j] = f.x, v[8 * c + 2 * j + 1] = f.y;
+            v[4 * c + j] = two(f.x, f.y);
         }
     }
 }
 
 // One warp's part of a finished tile: 32 rows (a warp reads the quarter of TMEM's lanes that its
-// number gives) and every other group of columns, the rest being its partner's. `release` is
+// number gives) and every fourth group of 32 columns, the rest being its three partners'. `release` is
 // called when the accumulator has been read.
 template <int MODE, typename T, bool FP8, typename Release>
 __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uint32_t acc,
                                          unsigned char* buf, int warp, int lane,
                                          Release&& release) {
-    const int quarter = warp & 3, half_of = warp >> 2;
+    const int quarter = warp & 3, share = warp >> 2;
     const int row0 = t.mt * kBM + quarter * 32;
     const int rows = (int)max((int64_t)0, min((int64_t)32, p.m - row0));
     constexpr bool kGate = MODE == kGated || MODE == kGatedGrad;
@@ -283,9 +299,9 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
     const int64_t col0 = (int64_t)t.nt * width;
     const int end = (int)min((int64_t)width, p.n - col0);
     if constexpr (MODE == kPartial) {
-        for (int c = half_of * 32; c < end; c += 64) {
-            float v[32];
-            tc::tmem_ld32(acc + c, v);
+        for (int c = share * 16; c < end; c += 64) {
+            float v[16];
+            tc::tmem_ld16(acc + c, v);
             store_rows32(buf, v, p.z + ((int64_t)t.split * p.m + row0) * p.ld_z + col0 + c,
                          p.ld_z, rows, end - c, true, lane);
         }
@@ -293,18 +309,23 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
         return;
     }
     const float xs = FP8 && lane < rows ? p.x_scale[row0 + lane] : 0.0f;
-    for (int c = half_of * 64; c < end; c += 128) {
+    for (int c = share * 32; c < end; c += 128) {
         const int64_t col = col0 + c, left = p.n - col;
         if constexpr (MODE == kForward || MODE == kGated) {
             if (p.z) {  // the pre-activations, in float32
                 for (int part = 0; part < (kGate ? 2 : 1); ++part) {
-                    for (int half = 0; half < 2 && half * 32 < left; ++half) {
-                        const int64_t at = part * p.n + col + half * 32;
-                        float v[32];
-                        tc::tmem_ld32(acc + c + part * width + half * 32, v);
-                        finish_z<T, FP8>(v, p, at, left - half * 32, xs);
+                    for (int half = 0; half < 2 && half * 16 < left; ++half) {
+                        const int64_t at = part * p.n + col + half * 16;
+                        float v[16];
+                        Two z[8];
+                        Bias<T> bias;
+                        bias.load(p, at, left - half * 16);
+                        tc::tmem_ld16(acc + c + part * width + half * 16, v);
+                        finish_z<T, FP8>(v, z, bias, p, at, left - half * 16, xs);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) split(z[j], v[2 * j], v[2 * j + 1]);
                         store_rows32(buf, v, p.z + (int64_t)row0 * p.ld_z + at, p.ld_z, rows,
-                                     left - half * 32, p.vec_z, lane);
+                                     left - half * 16, p.vec_z, lane);
                     }
                 }
             }
@@ -316,55 +337,64 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
         }
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
-            float v[32], u[32];
-            const int at = c + half * 32;
-            const int64_t zcol = col + half * 32, zleft = left - half * 32;
-            if constexpr (kGate) tmem_ld32x2(acc + at, acc + at + width, v, u);
-            else tc::tmem_ld32(acc + at, v);
-            if (half == 1 && c + 128 >= end) release();
-            finish_z<T, FP8>(v, p, zcol, zleft, xs);
-            if constexpr (kGate) finish_z<T, FP8>(u, p, p.n + zcol, zleft, xs);
+            const int at = c + half * 16;
+            const int64_t zcol = col + half * 16, zleft = left - half * 16;
+            Two z[8], u[8];
+            {
+                float v[16], w[16];
+                Bias<T> bias, bias_up;
+                bias.load(p, zcol, zleft);
+                if constexpr (kGate) {
+                    bias_up.load(p, p.n + zcol, zleft);
+                    tmem_ld16x2(acc + at, acc + at + width, v, w);
+                } else {
+                    tc::tmem_ld16(acc + at, v);
+                }
+                if (half == 1 && c + 128 >= end) release();
+                finish_z<T, FP8>(v, z, bias, p, zcol, zleft, xs);
+                if constexpr (kGate) finish_z<T, FP8>(w, u, bias_up, p, p.n + zcol, zleft, xs);
+            }
             if constexpr (MODE == kForward) {
                 with_activation(p.act, [&](auto a) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = act_value<decltype(a)::value>(v[j]);
+                    for (int j = 0; j < 8; ++j) z[j] = act_value<decltype(a)::value>(z[j]);
                 });
                 if (p.in) {
                     get_row<T>(buf, lane, half, u);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] += u[j];
+                    for (int j = 0; j < 8; ++j) z[j] = z[j] + u[j];
                 }
             } else if constexpr (MODE == kGrad) {
                 get_row<T>(buf, lane, half, u);
                 with_activation(p.act, [&](auto a) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        float y, da;
-                        act_both<decltype(a)::value>(v[j], y, da);
-                        v[j] = u[j] * da;
+                    for (int j = 0; j < 8; ++j) {
+                        Two y, da;
+                        act_both<decltype(a)::value>(z[j], y, da);
+                        z[j] = u[j] * da;
                     }
                 });
             } else if constexpr (MODE == kGated) {
                 with_activation(p.act, [&](auto a) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        v[j] = act_value<decltype(a)::value>(v[j]) * u[j];
+                    for (int j = 0; j < 8; ++j)
+                        z[j] = act_value<decltype(a)::value>(z[j]) * u[j];
                 });
             } else {
-                float d[32];
+                Two d[8];
                 get_row<T>(buf, lane, half, d);
                 with_activation(p.act, [&](auto a) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        float y, da;
-                        act_both<decltype(a)::value>(v[j], y, da);
-                        v[j] = d[j] * u[j] * da;
+                    for (int j = 0; j < 8; ++j) {
+                        Two y, da;
+                        act_both<decltype(a)::value>(z[j], y, da);
+                        z[j] = d[j] * u[j] * da;
                         u[j] = d[j] * y;
                     }
                 });
                 put_row<T>(buf + kWarpBuf, lane, half, u);
             }
-            put_row<T>(buf, lane, half, v);
+            put_row<T>(buf, lane, half, z);
         }
         __syncwarp();
         constexpr bool kSums = MODE == kGrad || MODE == kGatedGrad;
@@ -379,7 +409,7 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
                                 sums ? sums + p.n : nullptr);
         __syncwarp();
     }
-    if (half_of * 64 >= end) release();  // no columns here
+    if (share * 32 >= end) release();  // no columns here
 }
 
 // PAIR: two blocks of a cluster (the two SMs of a TPC) work on one tile of 256 rows. Each holds its
@@ -399,10 +429,10 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform, and known to be
     constexpr bool kGate = MODE == kGated || MODE == kGatedGrad;
-    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, work = tiles * p.splits;
+    const unsigned tiles = (unsigned)p.tiles_m * p.tiles_n, work = tiles * p.splits;
     const int rank = PAIR ? (int)cluster_rank() : 0;
-    const int first = PAIR ? blockIdx.x >> 1 : blockIdx.x;
-    const int stride = PAIR ? gridDim.x >> 1 : gridDim.x;
+    const unsigned first = PAIR ? blockIdx.x >> 1 : blockIdx.x;
+    const unsigned stride = PAIR ? gridDim.x >> 1 : gridDim.x;
 
     if (tid == 0) {
         for (int s = 0; s < p.stages; ++s) {
@@ -447,7 +477,7 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
         int st = 0, issued = 0;
         uint32_t parity = 1;  // of the stage's last release; a fresh barrier passes for 1
         bool ok = true;
-        for (int64_t w = first; w < work && ok; w += stride) {
+        for (unsigned w = first; w < work && ok; w += stride) {
             const Tile t = tile_of(p, w);
             const int kb0 = t.split * p.kb_per_split;
             const int kb1 = min(p.kblocks, kb0 + p.kb_per_split);
@@ -504,8 +534,8 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
         int st = 0, buf = 0;
         uint32_t parity = 0, acc_parity = 1;
         bool ok = true;
-        for (int64_t w = first; w < work && ok; w += stride) {
-            const int split = (int)(w / tiles);
+        for (unsigned w = first; w < work && ok; w += stride) {
+            const int split = p.splits > 1 ? (int)(w / tiles) : 0;
             const int kb0 = split * p.kb_per_split;
             const int kb1 = min(p.kblocks, kb0 + p.kb_per_split);
             ok = mbar_wait(smem_u32(&sh->acc_empty[buf]), acc_parity) && !*fail;
@@ -545,7 +575,7 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
         // ---- epilogue
         int n_tile = 0;
         unsigned char* buf = bufs + warp * kWarpBufs<MODE> * kWarpBuf;
-        for (int64_t w = first; w < work; w += stride, ++n_tile) {
+        for (unsigned w = first; w < work; w += stride, ++n_tile) {
             Tile t = tile_of(p, w);
             if (PAIR) t.mt = t.mt * 2 + rank;
             const int b = n_tile & 1, round = n_tile >> 1;
@@ -675,7 +705,7 @@ k_act_grad(int64_t m, int64_t n, const float* __restrict__ z, const T* __restric
 #pragma unroll 8
             for (int64_t r = r0; r < r1; ++r) {
                 float y, da, d = to_float(dy[r * ld_dy + col]);
-                act_both<decltype(a)::value>(z[r * nz + col], y, da);
+                act_both1<decltype(a)::value>(z[r * nz + col], y, da);
                 if constexpr (GATED) {
                     float g = d * z[r * nz + n + col] * da, u = d * y;
                     dz[r * ld_dz + col] = from_float<T>(g);
@@ -803,6 +833,7 @@ void launch_tile(const CUtensorMap& a, const CUtensorMap& b, const TileParams& p
         if (device < 64) allowed.fetch_or(uint64_t(1) << device, std::memory_order_relaxed);
     }
     const int64_t work = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+    require(work < (1LL << 31) - 1024, "too many tiles");
     const int b_rows = PAIR ? p.bn / 2 : p.bn;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = PAIR ? 2 * (unsigned)std::min<int64_t>(work, sms / 2)

@@ -141,71 +141,146 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // ----------------------------------------------------------------------------- activations
 // For results that are rounded to 16 bits (2^-9 or 2^-12 relative): few instructions without a
 // branch, errors of some 1e-6 of the value.
-__device__ __forceinline__ float exp_fast(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.44269504088896f));
-    return r;
-}
 __device__ __forceinline__ float rcp_fast(float x) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 
+// Two float32 values in one 64-bit register: Blackwell adds, multiplies and fuses them in one
+// instruction, which halves the arithmetic of the epilogues.
+struct Two {
+    uint64_t v;
+};
+__device__ __forceinline__ Two two(float a, float b) {
+    Two t;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(t.v) : "f"(a), "f"(b));
+    return t;
+}
+__device__ __forceinline__ Two two(float a) { return two(a, a); }
+__device__ __forceinline__ void split(Two t, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(t.v));
+}
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+    Two t;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(t.v) : "l"(a.v), "l"(b.v));
+    return t;
+}
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+    Two t;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(t.v) : "l"(a.v), "l"(b.v));
+    return t;
+}
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
+    Two t;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(t.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return t;
+}
+template <typename Fn>
+__device__ __forceinline__ Two each(Two t, Fn&& fn) {
+    float a, b;
+    split(t, a, b);
+    return two(fn(a), fn(b));
+}
+__device__ __forceinline__ Two ex2(Two t) {  // 2^t
+    return each(t, [](float x) {
+        float r;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+        return r;
+    });
+}
+__device__ __forceinline__ Two rcp(Two t) {
+    return each(t, [](float x) { return rcp_fast(x); });
+}
+// a where the sign of s is clear, b where it is set
+__device__ __forceinline__ Two by_sign(Two s, Two a, Two b) {
+    float s0, s1, a0, a1, b0, b1;
+    split(s, s0, s1);
+    split(a, a0, a1);
+    split(b, b0, b1);
+    return two(s0 < 0.0f ? b0 : a0, s1 < 0.0f ? b1 : a1);
+}
+
+constexpr float kLog2E = 1.44269504088896f;
+
 // tanh x = 1 - 2 / (1 + e^2x); near zero, where that cancels, its Taylor series to x^7
 // (next term 62/2835 x^9: 3e-7 of the value at 1/4).
-__device__ __forceinline__ float tanh_fast(float x) {
-    float t = 1.0f - 2.0f * rcp_fast(1.0f + exp_fast(2.0f * x));
-    float q = x * x;
-    float s = x + x * q * (-1.0f / 3.0f + q * (2.0f / 15.0f - q * (17.0f / 315.0f)));
-    return q < 0.0625f ? s : t;
+__device__ __forceinline__ Two tanh_two(Two x) {
+    Two t = fma(two(-2.0f), rcp(ex2(x * two(2.0f * kLog2E)) + two(1.0f)), two(1.0f));
+    Two q = x * x;
+    Two s = fma(fma(fma(q, two(-17.0f / 315.0f), two(2.0f / 15.0f)), q, two(-1.0f / 3.0f)) * q, x,
+                x);
+    float q0, q1, t0, t1, s0, s1;
+    split(q, q0, q1);
+    split(t, t0, t1);
+    split(s, s0, s1);
+    return two(q0 < 0.0625f ? s0 : t0, q1 < 0.0625f ? s1 : t1);
 }
 
 // Upper tail Q(|x|) = 1 - Phi(|x|) of the normal distribution and e^(-x^2 / 2). erfc by the
 // rational approximation of Abramowitz and Stegun 7.1.26 (absolute error 1.5e-7 of erf), whose
 // factor e^(-x^2 / 2) is the density's as well.
-__device__ __forceinline__ float normal_tail(float x, float& e) {
-    float a = fabsf(x) * 0.70710678118654752f;
-    e = exp_fast(-0.5f * x * x);
-    float t = rcp_fast(1.0f + 0.3275911f * a);
-    float p = t * (0.254829592f +
-                   t * (-0.284496736f +
-                        t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-    return 0.5f * p * e;
+__device__ __forceinline__ Two normal_tail(Two x, Two& e) {
+    Two a = each(x, [](float v) { return fabsf(v); });
+    e = ex2(x * x * two(-0.5f * kLog2E));
+    Two t = rcp(fma(a, two(0.3275911f * 0.70710678118654752f), two(1.0f)));
+    Two p = fma(t, two(1.061405429f), two(-1.453152027f));
+    p = fma(t, p, two(1.421413741f));
+    p = fma(t, p, two(-0.284496736f));
+    p = fma(t, p, two(0.254829592f));
+    return p * t * e * two(0.5f);
 }
 
 template <int ACT>
-__device__ __forceinline__ float act_value(float x) {
+__device__ __forceinline__ Two act_value(Two x) {
     if constexpr (ACT == RUNE_ACT_TANH) {
-        return tanh_fast(x);
+        return tanh_two(x);
     } else if constexpr (ACT == RUNE_ACT_SILU) {
-        return x * rcp_fast(1.0f + exp_fast(-x));
+        return x * rcp(ex2(x * two(-kLog2E)) + two(1.0f));
     } else if constexpr (ACT == RUNE_ACT_GELU) {
-        float e, q = normal_tail(x, e);
-        return x * (x < 0.0f ? q : 1.0f - q);
+        Two e, q = normal_tail(x, e);
+        return x * by_sign(x, fma(q, two(-1.0f), two(1.0f)), q);
     } else {
         return x;
     }
 }
 
+// value y and derivative dy of the activation
 template <int ACT>
-__device__ __forceinline__ void act_both(float x, float& y, float& dy) {
+__device__ __forceinline__ void act_both(Two x, Two& y, Two& dy) {
     if constexpr (ACT == RUNE_ACT_TANH) {
-        y = tanh_fast(x);
-        dy = 1.0f - y * y;
+        y = tanh_two(x);
+        dy = fma(y * two(-1.0f), y, two(1.0f));
     } else if constexpr (ACT == RUNE_ACT_SILU) {
-        float s = rcp_fast(1.0f + exp_fast(-x));
+        Two s = rcp(ex2(x * two(-kLog2E)) + two(1.0f));
         y = x * s;
-        dy = s * (1.0f + x * (1.0f - s));
+        // s (1 + x (1 - s)), as a product: where s is 0 and x is infinite both forms are NaN
+        dy = s * fma(x, fma(s, two(-1.0f), two(1.0f)), two(1.0f));
     } else if constexpr (ACT == RUNE_ACT_GELU) {
-        float e, q = normal_tail(x, e);
-        float cdf = x < 0.0f ? q : 1.0f - q;
+        Two e, q = normal_tail(x, e);
+        Two cdf = by_sign(x, fma(q, two(-1.0f), two(1.0f)), q);
         y = x * cdf;
-        dy = cdf + x * e * 0.39894228040143268f;
+        dy = fma(x * e, two(0.39894228040143268f), cdf);
     } else {
         y = x;
-        dy = 1.0f;
+        dy = two(1.0f);
     }
+}
+
+template <int ACT>
+__device__ __forceinline__ float act_value(float x) {
+    float a, b;
+    split(act_value<ACT>(two(x)), a, b);
+    return a;
+}
+
+template <int ACT>
+__device__ __forceinline__ void act_both1(float x, float& y, float& dy) {
+    Two a, b;
+    float unused;
+    act_both<ACT>(two(x), a, b);
+    split(a, y, unused);
+    split(b, dy, unused);
 }
 
 // fn(std::integral_constant<int, ACT>) for the activation code `act`
