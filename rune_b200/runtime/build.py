@@ -1,7 +1,8 @@
-"""Build recipe for the engine's shared library (sm_100a).
+"""Build recipe for the engine's shared library (sm_100a) and the operators' Python binding.
 
 ``python -m rune_b200.runtime.build`` compiles every ``rune_b200/csrc/*.cu`` with nvcc into
-``rune_b200/_lib/librune_b200.so`` (in-tree, so it travels with the source tree).
+``rune_b200/_lib/librune_b200.so`` and ``rune_b200/csrc/torch_ops.cpp`` with g++ into
+``rune_b200/_lib/_ops.so`` (in-tree, so they travel with the source tree).
 """
 
 from __future__ import annotations
@@ -15,6 +16,8 @@ PKG = Path(__file__).resolve().parents[1]
 CSRC = PKG / "csrc"
 LIB_DIR = PKG / "_lib"
 LIB = LIB_DIR / "librune_b200.so"
+BINDING = LIB_DIR / "_ops.so"
+BINDING_SOURCE = CSRC / "torch_ops.cpp"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -56,7 +59,43 @@ def needs_build() -> bool:
     return any(p.stat().st_mtime > stamp for p in deps)
 
 
+def _binding_command(out: Path) -> list[str]:
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).parent
+    home = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
+    abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    return ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={abi}", str(BINDING_SOURCE), "-o", str(out),
+            *(f"-I{p}" for p in (root / "include", root / "include/torch/csrc/api/include",
+                                 home / "include",
+                                 sysconfig.get_paths()["include"])),
+            f"-L{root / 'lib'}",
+            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> Path:
+    """The operators' binding to torch (CPython module ``_ops``, host code only)."""
+    header = PKG.parent / "include" / "rune_b200.h"
+    if not force and BINDING.exists() and BINDING.stat().st_mtime >= max(
+            p.stat().st_mtime for p in (BINDING_SOURCE, header)):
+        return BINDING
+    LIB_DIR.mkdir(parents=True, exist_ok=True)
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = _binding_command(tmp)
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed: {res.stdout}{res.stderr}")
+    os.replace(tmp, BINDING)
+    return BINDING
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
+    build_binding(force, verbose)
     if not force and not needs_build():
         return LIB
     LIB_DIR.mkdir(parents=True, exist_ok=True)

@@ -9,7 +9,6 @@ from __future__ import annotations
 
 import ctypes
 import os
-import struct
 from ctypes import (POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_uint8,
                     c_uint32, c_void_p)
 from pathlib import Path
@@ -92,12 +91,49 @@ class Stats(ctypes.Structure):
     ]
 
 
-# The operators' argument structs (field order of include/rune_b200.h) as struct formats:
-# 64-bit sizes, 32-bit codes, pointers as integers.
-NORM_ARGS = struct.Struct("=4q4ifi7Q")
-NORM_GRAD_ARGS = struct.Struct("=6q4i9Qq")
-LINEAR_ARGS = struct.Struct("=6q6i9Qq")
-LINEAR_GRAD_ARGS = struct.Struct("=6q4i9Qq")
+class NormArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_int64), ("width", c_int64), ("x_stride", c_int64),
+        ("residual_stride", c_int64), ("device", c_int32), ("dtype", c_int32),
+        ("weight_dtype", c_int32), ("out_dtype", c_int32), ("eps", c_float),
+        ("reserved", c_int32), ("x", c_void_p), ("residual", c_void_p), ("weight", c_void_p),
+        ("y", c_void_p), ("h", c_void_p), ("scale", c_void_p), ("rstd", c_void_p),
+    ]
+
+
+class NormGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_int64), ("width", c_int64), ("x_stride", c_int64),
+        ("residual_stride", c_int64), ("dy_stride", c_int64), ("dh_stride", c_int64),
+        ("device", c_int32), ("dtype", c_int32), ("weight_dtype", c_int32),
+        ("reserved", c_int32), ("x", c_void_p), ("residual", c_void_p), ("weight", c_void_p),
+        ("rstd", c_void_p), ("dy", c_void_p), ("dh", c_void_p), ("dx", c_void_p),
+        ("dweight", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_int64),
+    ]
+
+
+class LinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_int64), ("inputs", c_int64), ("outputs", c_int64), ("x_stride", c_int64),
+        ("weight_stride", c_int64), ("residual_stride", c_int64), ("device", c_int32),
+        ("dtype", c_int32), ("out_dtype", c_int32), ("activation", c_int32),
+        ("gated", c_int32), ("reserved", c_int32), ("x", c_void_p), ("weight", c_void_p),
+        ("bias", c_void_p), ("residual", c_void_p), ("x_scale", c_void_p),
+        ("weight_scale", c_void_p), ("y", c_void_p), ("saved", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_int64),
+    ]
+
+
+class LinearGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_int64), ("inputs", c_int64), ("outputs", c_int64), ("x_stride", c_int64),
+        ("weight_stride", c_int64), ("dy_stride", c_int64), ("device", c_int32),
+        ("dtype", c_int32), ("activation", c_int32), ("gated", c_int32), ("x", c_void_p),
+        ("weight", c_void_p), ("bias", c_void_p), ("dy", c_void_p), ("saved", c_void_p),
+        ("dx", c_void_p), ("dweight", c_void_p), ("dbias", c_void_p), ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+    ]
+
 
 _LIB = None
 
@@ -152,13 +188,11 @@ def load_library(path: Path | None = None):
         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
     lib.rune_tc_selftest.argtypes = [c_int32, c_int32, c_int32, POINTER(c_float),
                                      POINTER(c_float), POINTER(c_float), c_int32]
-    # operator arguments travel as packed bytes of the C structs (NORM_ARGS and the others)
-    for name in ("rune_rms_norm", "rune_rms_norm_backward", "rune_linear",
-                 "rune_linear_backward"):
-        getattr(lib, name).argtypes = [c_char_p, c_void_p]
-    for name in ("rune_rms_norm_backward_workspace", "rune_linear_workspace",
-                 "rune_linear_backward_workspace"):
-        getattr(lib, name).argtypes = [c_char_p, POINTER(c_int64)]
+    for name, args in (("rune_rms_norm", NormArgs), ("rune_rms_norm_backward", NormGradArgs),
+                       ("rune_linear", LinearArgs), ("rune_linear_backward", LinearGradArgs)):
+        getattr(lib, name).argtypes = [POINTER(args), c_void_p]
+        if name != "rune_rms_norm":
+            getattr(lib, name + "_workspace").argtypes = [POINTER(args), POINTER(c_int64)]
     for name in EXPORTED:
         if name not in ("rune_engine_destroy", "rune_last_error"):
             getattr(lib, name).restype = c_int
@@ -170,7 +204,11 @@ def load_library(path: Path | None = None):
 def check(lib, status: int):
     if status == RUNE_OK:
         return
-    message = (lib.rune_last_error() or b"").decode(errors="replace")
+    fail(status, (lib.rune_last_error() or b"").decode(errors="replace"))
+
+
+def fail(status: int, message: str):
+    """Raise the exception of a status other than RUNE_OK."""
     if status in (RUNE_ERR_INVALID, RUNE_ERR_NEIGHBOR_OVERFLOW, RUNE_ERR_TYPE):
         raise ValueError(message)
     if status == RUNE_ERR_OOM:

@@ -75,7 +75,8 @@ def test_argument_structs_match_the_header(tmp_path):
     subprocess.run(["gcc", str(src), "-o", str(exe)], check=True)
     got = [int(v) for v in subprocess.run([str(exe)], capture_output=True, text=True,
                                           check=True).stdout.split()]
-    sizes = [s.size for s in (L.NORM_ARGS, L.NORM_GRAD_ARGS, L.LINEAR_ARGS, L.LINEAR_GRAD_ARGS)]
+    structs = (L.NormArgs, L.NormGradArgs, L.LinearArgs, L.LinearGradArgs)
+    sizes = [ctypes.sizeof(s) for s in structs]
     assert got == sizes + [sizes[0] - 8, sizes[1] - 8, sizes[2] - 8, sizes[3] - 8]
 
 
@@ -596,10 +597,11 @@ def test_refusals():
         ops.linear(q, p, x_scale=s, weight_scale=t,
                    bias=w[:, 0].contiguous().requires_grad_(True))
     lib = L.load_library()
-    bad = L.LINEAR_ARGS.pack(4, 16, 8, 16, 16, 0, 0, L.RUNE_F32, L.RUNE_F32, -1, 0, 0,
-                             x.data_ptr(), w.data_ptr(), 0, 0, 0, 0, x.data_ptr(), 0, 0, 0)
-    assert lib.rune_linear(bad, None) == L.RUNE_ERR_INVALID
-    dev = L.LINEAR_ARGS.pack(4, 16, 8, 16, 16, 0, 99, L.RUNE_BF16, L.RUNE_BF16, -1, 0, 0,
-                             x.data_ptr(), w.data_ptr(), 0, 0, 0, 0, x.data_ptr(), 0, 0, 0)
-    assert lib.rune_linear(dev, None) == L.RUNE_ERR_CUDA
+    raw = L.LinearArgs(rows=4, inputs=16, outputs=8, x_stride=16, weight_stride=16,
+                       dtype=L.RUNE_F32, out_dtype=L.RUNE_F32, activation=L.RUNE_ACT_NONE,
+                       x=x.data_ptr(), weight=w.data_ptr(), y=x.data_ptr())
+    assert lib.rune_linear(ctypes.byref(raw), None) == L.RUNE_ERR_INVALID
+    raw.dtype = raw.out_dtype = L.RUNE_BF16
+    raw.device = 99
+    assert lib.rune_linear(ctypes.byref(raw), None) == L.RUNE_ERR_CUDA
     assert torch.equal(ops.linear(x, w), ops.linear(x, w))  # the context is as before
