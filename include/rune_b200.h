@@ -345,7 +345,8 @@ typedef struct {
     const float* x_scale;   /* [rows], RUNE_E4M3 only */
     const float* weight_scale; /* [outputs] or [2 outputs], RUNE_E4M3 only */
     void* y;                /* [rows, outputs] */
-    float* saved;           /* [rows, outputs] or [rows, 2 outputs]: z for the backward, or NULL */
+    float* saved;           /* z for the backward, or NULL: [rows, line] or [rows, 2, line] with
+                               line = outputs rounded up to 4; 16-byte aligned */
     void* workspace;
     int64_t workspace_bytes;
 } rune_linear_args;

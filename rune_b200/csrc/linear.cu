@@ -47,13 +47,29 @@ constexpr uint32_t kWarpBuf = 32 * kRowBytes;    // 2 KB
 constexpr int kMaxStages = 8;
 constexpr uint32_t kSmemMax = 227 * 1024;
 
+// Exact quotient of n < 2^31 by a divisor fixed for the launch: n * mul >> shift.
+struct Divisor {
+    unsigned by, mul, shift;
+    __device__ __forceinline__ unsigned quotient(unsigned n) const {
+        return (unsigned)(((uint64_t)n * mul) >> shift);
+    }
+};
+Divisor make_divisor(unsigned by) {
+    // with 2^L >= by, mul = ceil(2^(31 + L) / by) < 2^32 errs by less than n / 2^31 of a unit
+    unsigned l = 0;
+    while ((1ull << l) < by) ++l;
+    return {by, (unsigned)(((1ull << (31 + l)) + by - 1) / by), 31 + l};
+}
+
 struct TileParams {
     int64_t m, n;           // rows and columns of the output (gated: columns of y)
-    int64_t ld_out, ld_in, ld_z;
+    int64_t ld_out, ld_in;
+    int64_t ld_z, ld_part;  // of z: rows, and within a row the parts (gate, up)
     int kblocks, kb_per_split, splits;
     int tiles_m, tiles_n, bn, stages;
+    Divisor by_tiles, by_group, by_last;  // tile_of's: all tiles, a group's, the last group's rows
     int a_mn, b_mn, act;
-    int vec_out, vec_in, vec_z, vec_bias;  // 16-byte accesses allowed
+    int vec_out, vec_in, vec_bias;  // 16-byte accesses allowed
     uint32_t idesc;
     void* out;
     const void* in;         // residual, or dy
@@ -86,92 +102,152 @@ struct Tile {
 
 // Tiles in groups of 16 tile rows, column by column, so that the blocks at work share a few
 // lines of both operands in L2; the ranges of k of one tile come last.
+constexpr unsigned kGroup = 16;
 __device__ __forceinline__ Tile tile_of(const TileParams& p, unsigned w) {
-    constexpr unsigned G = 16;
     Tile t{0, 0, 0};
     if (p.splits > 1) {
-        const unsigned tiles = (unsigned)p.tiles_m * p.tiles_n;
-        t.split = w / tiles;
-        w -= t.split * tiles;
+        t.split = p.by_tiles.quotient(w);
+        w -= t.split * p.by_tiles.by;
     }
-    const unsigned per = G * p.tiles_n, g = w / per, in = w - g * per;
-    const unsigned gm = min(G, p.tiles_m - g * G);
-    t.nt = gm == G ? in / G : in / gm;
-    t.mt = g * G + (in - t.nt * gm);
+    const unsigned g = p.by_group.quotient(w), in = w - g * p.by_group.by;
+    const unsigned left = p.tiles_m - g * kGroup, rows = min(kGroup, left);
+    t.nt = left >= kGroup ? in / kGroup : p.by_last.quotient(in);
+    t.mt = g * kGroup + (in - t.nt * rows);
     return t;
 }
 
 // ---- a warp's 32 rows x 32 columns of 16-bit values between global memory and its buffer.
 // Rows are four pieces of 16 bytes, piece c of row r at c ^ (r / 2 & 3), so that both the row-wise
-// accesses of the lanes and the coalesced ones spread over the banks.
-__device__ __forceinline__ uint4* piece(unsigned char* buf, int r, int c) {
-    return reinterpret_cast<uint4*>(buf + r * kRowBytes + ((c ^ ((r >> 1) & 3)) << 4));
+// accesses of the lanes and the coalesced ones (lane l: piece l & 3 of row 8 i + l / 4) spread
+// over the banks.
+struct Stage {
+    uint32_t row, swizzle;  // of the lane's own row
+    uint32_t coalesced;     // the lane's piece of rows 0 .. 7
+    uint32_t base;
+    int lane;
+    __device__ __forceinline__ Stage(uint32_t buf, int l) : base(buf), lane(l) {
+        row = buf + l * kRowBytes;
+        swizzle = ((l >> 1) & 3) << 4;
+        coalesced = buf + (l >> 2) * kRowBytes + (((l & 3) ^ ((l >> 3) & 3)) << 4);
+    }
+    __device__ __forceinline__ uint32_t own(int c) const {  // piece c of the lane's row
+        return row + (uint32_t(c << 4) ^ swizzle);
+    }
+    __device__ __forceinline__ uint32_t turn(int i) const {  // coalesced, row 8 i + lane / 4
+        return coalesced + i * 8 * kRowBytes;
+    }
+    __device__ __forceinline__ uint32_t at(int r, int byte) const {
+        return base + r * kRowBytes + ((byte & ~15) ^ (((r >> 1) & 3) << 4)) + (byte & 15);
+    }
+};
+__device__ __forceinline__ void put16(uint32_t addr, uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y),
+                 "r"(v.z), "r"(v.w)
+                 : "memory");
+}
+__device__ __forceinline__ uint4 get16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+__device__ __forceinline__ void put_half(uint32_t addr, uint16_t v) {
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(v) : "memory");
+}
+__device__ __forceinline__ uint16_t get_half(uint32_t addr) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t get_word(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
 }
 
+// rows x cols (of 32 x 32, zeros beyond) from src into the buffer
 template <typename T>
-__device__ __forceinline__ void load_rows(unsigned char* buf, const T* src, int64_t ld,
-                                          int rows, int64_t cols, bool vec, int lane) {
+__device__ __forceinline__ void load_rows(const Stage& st, const T* src, int64_t ld, int rows,
+                                          int64_t cols, bool vec) {
     if (vec) {
-        const int c = lane & 3;
+        const int r0 = st.lane >> 2, c = (st.lane & 3) * 8;
+        const T* p = src + r0 * ld + c;
+        const bool in = c < cols;
+        uint4 v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int r = i * 8 + (lane >> 2);
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (r < rows && c * 8 < cols)
-                v = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)r * ld + c * 8));
-            *piece(buf, r, c) = v;
+            v[i] = make_uint4(0, 0, 0, 0);
+            if (in && r0 + 8 * i < rows)
+                v[i] = __ldg(reinterpret_cast<const uint4*>(p + i * 8 * ld));
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) put16(st.turn(i), v[i]);
     } else {
 #pragma unroll 8
         for (int r = 0; r < 32; ++r) {
-            T v = from_float<T>(0.0f);
-            if (r < rows && lane < cols) v = src[(int64_t)r * ld + lane];
-            reinterpret_cast<T*>(piece(buf, r, lane >> 3))[lane & 7] = v;
+            uint16_t v = 0;
+            if (r < rows && st.lane < cols)
+                v = reinterpret_cast<const uint16_t*>(src)[(int64_t)r * ld + st.lane];
+            put_half(st.at(r, st.lane * 2), v);
         }
     }
 }
 
-// buffer -> global, and on request the sums of the 32 rows of each column
+// buffer -> dst, and on request the sums of the 32 rows of each column
 template <typename T, bool SUMS>
-__device__ __forceinline__ void store_rows(unsigned char* buf, T* dst, int64_t ld, int rows,
-                                           int64_t cols, bool vec, int lane, float* sums) {
+__device__ __forceinline__ void store_rows(const Stage& st, T* dst, int64_t ld, int rows,
+                                           int64_t cols, bool vec, float* sums) {
+    const int lane = st.lane;
     if (vec) {
-        const int c = lane & 3;
-        float s[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] = 0.0f;
+        const int r0 = lane >> 2, c = (lane & 3) * 8;
+        T* p = dst + r0 * ld + c;
+        const bool in = c < cols;
+        Two s[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int r = i * 8 + (lane >> 2);
-            uint4 v = *piece(buf, r, c);
-            if (r < rows && c * 8 < cols)
-                *reinterpret_cast<uint4*>(dst + (int64_t)r * ld + c * 8) = v;
+            const uint4 v = get16(st.turn(i));
+            if (in && r0 + 8 * i < rows) *reinterpret_cast<uint4*>(p + i * 8 * ld) = v;
             if constexpr (SUMS) {
                 const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    float2 f = unpack2<T>(w[j]);
-                    s[2 * j] += f.x, s[2 * j + 1] += f.y;
+                    const float2 f = unpack2<T>(w[j]);
+                    s[j] = i == 0 ? two(f.x, f.y) : s[j] + two(f.x, f.y);
                 }
             }
         }
         if constexpr (SUMS) {
             if (sums) {
+                // eight columns in each of the lanes that share lane & 3: every step halves the
+                // columns a lane keeps, and at the end each lane has the sum of one
+                float a[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
+                for (int j = 0; j < 4; ++j) split(s[j], a[2 * j], a[2 * j + 1]);
+                int column = 0;
 #pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) s[j] += __shfl_xor_sync(0xffffffffu, s[j], o);
-                    if (lane < 4 && c * 8 + j < cols) sums[c * 8 + j] = s[j];
+                for (int n = 4; n > 0; n >>= 1) {
+                    const bool upper = lane & (4 * n);
+#pragma unroll
+                    for (int j = 0; j < n; ++j) {
+                        const float give = upper ? a[j] : a[n + j];
+                        a[j] = (upper ? a[n + j] : a[j]) +
+                               __shfl_xor_sync(0xffffffffu, give, 4 * n);
+                    }
+                    column += upper ? n : 0;
                 }
+                if (c + column < cols) sums[c + column] = a[0];
             }
         }
     } else {
         float s = 0.0f;
 #pragma unroll 8
         for (int r = 0; r < 32; ++r) {
-            T v = reinterpret_cast<T*>(piece(buf, r, lane >> 3))[lane & 7];
-            if (r < rows && lane < cols) dst[(int64_t)r * ld + lane] = v;
-            if constexpr (SUMS) s += to_float(v);
+            const uint16_t h = get_half(st.at(r, lane * 2));
+            if (r < rows && lane < cols)
+                reinterpret_cast<uint16_t*>(dst)[(int64_t)r * ld + lane] = h;
+            if constexpr (SUMS) s += unpack2<T>(h).x;
         }
         if constexpr (SUMS) {
             if (sums && lane < cols) sums[lane] = s;
@@ -179,33 +255,22 @@ __device__ __forceinline__ void store_rows(unsigned char* buf, T* dst, int64_t l
     }
 }
 
-// a warp's 32 rows x 16 columns of float32, each lane its row, through the buffer to memory
-__device__ __forceinline__ void store_rows32(unsigned char* buf, const float (&v)[16], float* dst,
-                                             int64_t ld, int rows, int64_t cols, bool vec,
-                                             int lane) {
+// a warp's 32 rows x 16 columns of float32, each lane its row, through the buffer to memory whose
+// rows are padded to 16 bytes
+__device__ __forceinline__ void store_rows32(const Stage& st, const float (&v)[16], float* dst,
+                                             int64_t ld, int rows, int64_t cols) {
     __syncwarp();
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-        *reinterpret_cast<float4*>(piece(buf, lane, c)) =
-            make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+        put16(st.own(c), make_uint4(__float_as_uint(v[4 * c]), __float_as_uint(v[4 * c + 1]),
+                                    __float_as_uint(v[4 * c + 2]), __float_as_uint(v[4 * c + 3])));
     __syncwarp();
-    if (vec) {
-        const int c = lane & 3;
+    const int r0 = st.lane >> 2, c = (st.lane & 3) * 4;
+    float* p = dst + r0 * ld + c;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = i * 8 + (lane >> 2);
-            if (r < rows && c * 4 < cols)
-                *reinterpret_cast<uint4*>(dst + (int64_t)r * ld + c * 4) = *piece(buf, r, c);
-        }
-    } else {
-        const int c = lane & 15;
-#pragma unroll 8
-        for (int i = 0; i < 16; ++i) {
-            const int r = 2 * i + (lane >> 4);
-            if (r < rows && c < cols)
-                dst[(int64_t)r * ld + c] = reinterpret_cast<float*>(piece(buf, r, c >> 2))[c & 3];
-        }
-    }
+    for (int i = 0; i < 4; ++i)
+        if (c < cols && r0 + 8 * i < rows)
+            *reinterpret_cast<uint4*>(p + i * 8 * ld) = get16(st.turn(i));
     __syncwarp();
 }
 
@@ -255,8 +320,7 @@ __device__ __forceinline__ void finish_z(const float (&v)[16], Two (&z)[8], cons
 
 // 16 values of a lane's row to and from pieces 2 half, 2 half + 1 of its line
 template <typename T>
-__device__ __forceinline__ void put_row(unsigned char* buf, int lane, int half,
-                                        const Two (&v)[8]) {
+__device__ __forceinline__ void put_row(const Stage& st, int half, const Two (&v)[8]) {
     uint32_t w[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -266,19 +330,18 @@ __device__ __forceinline__ void put_row(unsigned char* buf, int lane, int half,
     }
 #pragma unroll
     for (int c = 0; c < 2; ++c)
-        *piece(buf, lane, half * 2 + c) =
-            make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+        put16(st.own(half * 2 + c), make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]));
 }
 
 template <typename T>
-__device__ __forceinline__ void get_row(unsigned char* buf, int lane, int half, Two (&v)[8]) {
+__device__ __forceinline__ void get_row(const Stage& st, int half, Two (&v)[8]) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-        uint4 q = *piece(buf, lane, half * 2 + c);
+        const uint4 q = get16(st.own(half * 2 + c));
         const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            float2 f = unpack2<T>(w[j]);
+            const float2 f = unpack2<T>(w[j]);
             v[4 * c + j] = two(f.x, f.y);
         }
     }
@@ -286,11 +349,12 @@ __device__ __forceinline__ void get_row(unsigned char* buf, int lane, int half, 
 
 // One warp's part of a finished tile: 32 rows (a warp reads the quarter of TMEM's lanes that its
 // number gives) and every fourth group of 32 columns, the rest being its three partners'. `release` is
-// called when the accumulator has been read.
-template <int MODE, typename T, bool FP8, typename Release>
+// called when the accumulator has been read. `wait` comes back when the accumulator is complete;
+// what the first group reads from memory is asked for before.
+template <int MODE, typename T, bool FP8, typename Wait, typename Release>
 __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uint32_t acc,
-                                         unsigned char* buf, int warp, int lane,
-                                         Release&& release) {
+                                         const Stage& st, const Stage& st2, int warp,
+                                         Wait&& wait, Release&& release) {
     const int quarter = warp & 3, share = warp >> 2;
     const int row0 = t.mt * kBM + quarter * 32;
     const int rows = (int)max((int64_t)0, min((int64_t)32, p.m - row0));
@@ -298,12 +362,22 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
     const int width = kGate ? p.bn / 2 : p.bn;  // output columns of the tile
     const int64_t col0 = (int64_t)t.nt * width;
     const int end = (int)min((int64_t)width, p.n - col0);
+    const int lane = st.lane;
+    constexpr bool kReads = MODE == kGrad || MODE == kGatedGrad;
+    const bool reads = kReads || (MODE == kForward && p.in);
+    auto read_in = [&](int c) {  // residual or dy of the group
+        load_rows(st, static_cast<const T*>(p.in) + (int64_t)row0 * p.ld_in + col0 + c, p.ld_in,
+                  rows, end - c, p.vec_in);
+    };
+    const bool ahead = reads && !(MODE == kForward && p.z) && share * 32 < end;
+    if (ahead) read_in(share * 32);
+    if (!wait()) return;
     if constexpr (MODE == kPartial) {
         for (int c = share * 16; c < end; c += 64) {
             float v[16];
             tc::tmem_ld16(acc + c, v);
-            store_rows32(buf, v, p.z + ((int64_t)t.split * p.m + row0) * p.ld_z + col0 + c,
-                         p.ld_z, rows, end - c, true, lane);
+            store_rows32(st, v, p.z + ((int64_t)t.split * p.m + row0) * p.ld_z + col0 + c,
+                         p.ld_z, rows, end - c);
         }
         release();
         return;
@@ -324,15 +398,16 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
                         finish_z<T, FP8>(v, z, bias, p, at, left - half * 16, xs);
 #pragma unroll
                         for (int j = 0; j < 8; ++j) split(z[j], v[2 * j], v[2 * j + 1]);
-                        store_rows32(buf, v, p.z + (int64_t)row0 * p.ld_z + at, p.ld_z, rows,
-                                     left - half * 16, p.vec_z, lane);
+                        store_rows32(st, v,
+                                     p.z + (int64_t)row0 * p.ld_z + part * p.ld_part + col +
+                                         half * 16,
+                                     p.ld_z, rows, left - half * 16);
                     }
                 }
             }
         }
-        if (MODE == kGrad || MODE == kGatedGrad || (MODE == kForward && p.in)) {
-            load_rows(buf, static_cast<const T*>(p.in) + (int64_t)row0 * p.ld_in + col, p.ld_in,
-                      rows, left, p.vec_in, lane);
+        if (reads) {
+            if (!ahead || c != share * 32) read_in(c);
             __syncwarp();
         }
 #pragma unroll 1
@@ -360,12 +435,12 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
                     for (int j = 0; j < 8; ++j) z[j] = act_value<decltype(a)::value>(z[j]);
                 });
                 if (p.in) {
-                    get_row<T>(buf, lane, half, u);
+                    get_row<T>(st, half, u);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) z[j] = z[j] + u[j];
                 }
             } else if constexpr (MODE == kGrad) {
-                get_row<T>(buf, lane, half, u);
+                get_row<T>(st, half, u);
                 with_activation(p.act, [&](auto a) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
@@ -382,7 +457,7 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
                 });
             } else {
                 Two d[8];
-                get_row<T>(buf, lane, half, d);
+                get_row<T>(st, half, d);
                 with_activation(p.act, [&](auto a) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
@@ -392,9 +467,9 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
                         u[j] = d[j] * y;
                     }
                 });
-                put_row<T>(buf + kWarpBuf, lane, half, u);
+                put_row<T>(st2, half, u);
             }
-            put_row<T>(buf, lane, half, z);
+            put_row<T>(st, half, z);
         }
         __syncwarp();
         constexpr bool kSums = MODE == kGrad || MODE == kGatedGrad;
@@ -403,9 +478,9 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
                           ? p.colsum + ((int64_t)t.mt * 4 + quarter) * ncols + col
                           : nullptr;
         T* out = static_cast<T*>(p.out) + (int64_t)row0 * p.ld_out + col;
-        store_rows<T, kSums>(buf, out, p.ld_out, rows, left, p.vec_out, lane, sums);
+        store_rows<T, kSums>(st, out, p.ld_out, rows, left, p.vec_out, sums);
         if constexpr (MODE == kGatedGrad)
-            store_rows<T, true>(buf + kWarpBuf, out + p.n, p.ld_out, rows, left, p.vec_out, lane,
+            store_rows<T, true>(st2, out + p.n, p.ld_out, rows, left, p.vec_out,
                                 sums ? sums + p.n : nullptr);
         __syncwarp();
     }
@@ -512,11 +587,18 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
                             load(b + bw * kLineBytes, &map_b, x, (int)p.n + n0, bar);
                     }
                 }
+                __syncwarp();  // the other lanes' polling must not hold up the copies' issue
                 ++issued;
                 if (++st == p.stages) st = 0, parity ^= 1;
             }
         }
-        if (!ok) *fail = 1;
+        // the last releases of every stage arrive here (a pair's from the even block) before this
+        // block's memory may go
+        for (int i = max(0, issued - p.stages); i < issued && ok; ++i) {
+            ok = mbar_wait(smem_u32(&sh->empty[i % p.stages]), (i / p.stages) & 1) && !*fail;
+            ok = __all_sync(0xffffffffu, ok);
+        }
+        if (!ok && !*fail) *fail = 1;
         if (one) sh->issued = issued;
     } else if (warp == kMmaWarp && rank == 0) {
         // ---- MMA issuer. The whole warp runs the loop and one elected lane issues: control flow
@@ -535,11 +617,12 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
         uint32_t parity = 0, acc_parity = 1;
         bool ok = true;
         for (unsigned w = first; w < work && ok; w += stride) {
-            const int split = p.splits > 1 ? (int)(w / tiles) : 0;
+            const int split = p.splits > 1 ? (int)p.by_tiles.quotient(w) : 0;
             const int kb0 = split * p.kb_per_split;
             const int kb1 = min(p.kblocks, kb0 + p.kb_per_split);
             ok = mbar_wait(smem_u32(&sh->acc_empty[buf]), acc_parity) && !*fail;
             if (!__all_sync(0xffffffffu, ok)) {
+                if (!*fail) *fail = 2;
                 ok = false;
                 break;
             }
@@ -570,23 +653,35 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
             buf ^= 1;
             if (buf == 0) acc_parity ^= 1;
         }
-        if (!ok) *fail = 1;
+        if (!ok && !*fail) *fail = 3;
+        // and the last arrivals of the epilogues (both blocks')
+        for (int i = 0; i < 2 && ok; ++i) {
+            ok = mbar_wait(smem_u32(&sh->acc_empty[buf]), acc_parity) && !*fail;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok && !*fail) *fail = 2;
+            buf ^= 1;
+            if (buf == 0) acc_parity ^= 1;
+        }
     } else if (warp < kEpiWarps) {
         // ---- epilogue
         int n_tile = 0;
-        unsigned char* buf = bufs + warp * kWarpBufs<MODE> * kWarpBuf;
-        for (unsigned w = first; w < work; w += stride, ++n_tile) {
+        const uint32_t buf = smem_u32(bufs) + warp * kWarpBufs<MODE> * kWarpBuf;
+        const Stage st(buf, lane), st2(buf + (kWarpBufs<MODE> - 1) * kWarpBuf, lane);
+        const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
+        bool ok = true;
+        for (unsigned w = first; w < work && ok; w += stride, ++n_tile) {
             Tile t = tile_of(p, w);
             if (PAIR) t.mt = t.mt * 2 + rank;
             const int b = n_tile & 1, round = n_tile >> 1;
-            const bool ok = mbar_wait(smem_u32(&sh->acc_full[b]), round & 1) && !*fail;
-            if (!__all_sync(0xffffffffu, ok)) {
-                *fail = 1;
-                break;
-            }
-            fence_after_sync();
             epilogue<MODE, T, FP8>(
-                p, t, tmem + b * 256 + ((uint32_t)((warp & 3) * 32) << 16), buf, warp, lane, [&] {
+                p, t, tmem + b * 256 + quarter, st, st2, warp,
+                [&] {
+                    ok = mbar_wait(smem_u32(&sh->acc_full[b]), round & 1) && !*fail;
+                    ok = __all_sync(0xffffffffu, ok);
+                    fence_after_sync();
+                    return ok;
+                },
+                [&] {
                     fence_before_sync();
                     __syncwarp();
                     if (lane == 0) {
@@ -595,8 +690,10 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
                         else
                             mbar_arrive(smem_u32(&sh->acc_empty[b]));
                     }
+                    __syncwarp();
                 });
         }
+        if (!ok && !*fail) *fail = 4;
     }
     __syncwarp();
     if constexpr (PAIR) cluster_sync();
@@ -607,7 +704,7 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
     if (failed) {
         // let what is in flight land (bounded) before the blocks' memory goes: the copies of both
         // blocks count on the even one's barriers
-        if (tid == 0) atomicExch_system(p.flag, 1u);
+        if (tid == 0 && *fail) atomicExch_system(p.flag, (unsigned)*fail);
         if (tid == 0 && rank == 0) {
             const int issued = sh->issued;
             for (int i = max(0, issued - p.stages); i < issued; ++i)
@@ -661,7 +758,7 @@ __global__ void __launch_bounds__(256) k_join(const TileParams p, const float* _
                 if (col + j >= p.n) continue;
                 if (p.w_scale) v[j] *= xs * p.w_scale[c0 + j];
                 if (p.bias) v[j] += to_float(static_cast<const T*>(p.bias)[c0 + j]);
-                if (p.z) p.z[row * p.ld_z + c0 + j] = v[j];
+                if (p.z) p.z[row * p.ld_z + (c0 >= p.n ? p.ld_part + c0 - p.n : c0) + j] = v[j];
             }
         };
         float v[4], u[4];
@@ -692,11 +789,11 @@ constexpr int kGradRows = 64;
 
 template <bool GATED, typename T>
 __global__ void __launch_bounds__(256)
-k_act_grad(int64_t m, int64_t n, const float* __restrict__ z, const T* __restrict__ dy,
-           int64_t ld_dy, T* __restrict__ dz, int64_t ld_dz, int act, float* __restrict__ sums) {
+k_act_grad(int64_t m, int64_t n, const float* __restrict__ z, int64_t ld_part,
+           const T* __restrict__ dy, int64_t ld_dy, T* __restrict__ dz, int64_t ld_dz, int act, float* __restrict__ sums) {
     const int64_t col = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (col >= n) return;
-    const int64_t nz = GATED ? 2 * n : n;
+    const int64_t nz = GATED ? 2 * n : n, ld_z = GATED ? 2 * ld_part : ld_part;
     const int64_t strips = (m + kGradRows - 1) / kGradRows;
     for (int64_t strip = blockIdx.y; strip < strips; strip += gridDim.y) {
         const int64_t r0 = strip * kGradRows, r1 = min(m, r0 + kGradRows);
@@ -705,9 +802,9 @@ k_act_grad(int64_t m, int64_t n, const float* __restrict__ z, const T* __restric
 #pragma unroll 8
             for (int64_t r = r0; r < r1; ++r) {
                 float y, da, d = to_float(dy[r * ld_dy + col]);
-                act_both1<decltype(a)::value>(z[r * nz + col], y, da);
+                act_both1<decltype(a)::value>(z[r * ld_z + col], y, da);
                 if constexpr (GATED) {
-                    float g = d * z[r * nz + n + col] * da, u = d * y;
+                    float g = d * z[r * ld_z + ld_part + col] * da, u = d * y;
                     dz[r * ld_dz + col] = from_float<T>(g);
                     dz[r * ld_dz + n + col] = from_float<T>(u);
                     s0 += g, s1 += u;
@@ -823,8 +920,8 @@ Plan plan_product(int64_t m, int64_t n_cols, int kblocks, bool can_split, bool g
 }
 
 template <int MODE, typename T, bool FP8, bool PAIR>
-void launch_tile(const CUtensorMap& a, const CUtensorMap& b, const TileParams& p, int sms,
-                 int device, cudaStream_t stream) {
+void launch_tile(const CUtensorMap& a, const CUtensorMap& b, TileParams p, int sms, int device,
+                 cudaStream_t stream) {
     static std::atomic<uint64_t> allowed{0};  // devices whose limit is raised
     if (device >= 64 || !(allowed.load(std::memory_order_relaxed) >> device & 1)) {
         RUNE_CUDA_TRY(cudaFuncSetAttribute(k_tile<MODE, T, FP8, PAIR>,
@@ -834,6 +931,9 @@ void launch_tile(const CUtensorMap& a, const CUtensorMap& b, const TileParams& p
     }
     const int64_t work = (int64_t)p.tiles_m * p.tiles_n * p.splits;
     require(work < (1LL << 31) - 1024, "too many tiles");
+    p.by_tiles = make_divisor((unsigned)p.tiles_m * p.tiles_n);
+    p.by_group = make_divisor(kGroup * p.tiles_n);
+    p.by_last = make_divisor(std::max(1u, (unsigned)p.tiles_m % kGroup));
     const int b_rows = PAIR ? p.bn / 2 : p.bn;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = PAIR ? 2 * (unsigned)std::min<int64_t>(work, sms / 2)
@@ -974,6 +1074,9 @@ bool wide16(const void* p, int64_t ld, int64_t cols) {
     return aligned(p, 16) && ld % 8 == 0 && cols % 8 == 0;
 }
 
+// values of a row of the saved z for `outputs` columns (each of gate and up)
+int64_t saved_line(int64_t outputs) { return (outputs + 3) / 4 * 4; }
+
 void forward(const rune_linear_args& a, Scratch& ws, cudaStream_t stream) {
     const int eb = dtype_bytes(a.dtype);
     const int64_t n_all = a.gated ? 2 * a.outputs : a.outputs;
@@ -998,8 +1101,8 @@ void forward(const rune_linear_args& a, Scratch& ws, cudaStream_t stream) {
     p.bias = a.bias;
     p.vec_bias = aligned(a.bias, 16) && a.outputs % 8 == 0;
     p.x_scale = a.x_scale, p.w_scale = a.weight_scale;
-    p.z = a.saved, p.ld_z = n_all;
-    p.vec_z = aligned(a.saved, 16) && a.outputs % 4 == 0;
+    p.z = a.saved, p.ld_part = saved_line(a.outputs);
+    p.ld_z = (a.gated ? 2 : 1) * p.ld_part;
     run_product(g, p, ws, a.device, stream);
 }
 
@@ -1051,11 +1154,11 @@ void backward(const rune_linear_grad_args& a, Scratch& ws, cudaStream_t stream) 
                     auto* out = reinterpret_cast<T*>(to);
                     if (a.gated)
                         k_act_grad<true, T><<<grid, 256, 0, stream>>>(
-                            a.rows, a.outputs, a.saved, dy, a.dy_stride, out, dz.ld,
+                            a.rows, a.outputs, a.saved, saved_line(a.outputs), dy, a.dy_stride, out, dz.ld,
                             a.activation, sums);
                     else
                         k_act_grad<false, T><<<grid, 256, 0, stream>>>(
-                            a.rows, a.outputs, a.saved, dy, a.dy_stride, out, dz.ld,
+                            a.rows, a.outputs, a.saved, saved_line(a.outputs), dy, a.dy_stride, out, dz.ld,
                             a.activation, sums);
                 };
                 if (half) go(__half());
@@ -1217,9 +1320,11 @@ void check_waits(int device) {
     if (device < 0 || device >= kMaxDevices) return;
     volatile unsigned* host = g_flag_host[device].load(std::memory_order_acquire);
     if (host && *host) {
+        const unsigned where = *host;
         *host = 0;
-        throw Error(RUNE_ERR_CUDA, "A device-side copy of an earlier linear operator did not "
-                                   "complete in time; the results of that call are invalid.");
+        throw Error(RUNE_ERR_CUDA,
+                    "A device-side copy of an earlier linear operator did not complete in time "
+                    "(wait " + std::to_string(where) + "); the results of that call are invalid.");
     }
 }
 

@@ -105,6 +105,7 @@ k_few(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtenso
                     tma_load(a + kWStage / 2, &map_w, x, (int)(p.n + f0), bar);
                 tma_load(a + kWStage, &map_x, x, 0, bar);
             }
+            __syncwarp();  // the other lanes' polling must not hold up the copies' issue
             ++issued;
             if (++st == p.stages) st = 0, parity ^= 1;
         }
@@ -217,9 +218,10 @@ k_few(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtenso
                     z[i] = z[i] * (xs * scale[0]) + bias[0];
                     if (p.gated) u[i] = u[i] * (xs * scale[1]) + bias[1];
                     if (p.z) {
-                        float* at = p.z + (int64_t)row * (p.gated ? 2 * p.n : p.n);
-                        at[col] = z[i];
-                        if (p.gated) at[up] = u[i];
+                        const int64_t line = (p.n + 3) / 4 * 4;
+                        float* at = p.z + row * (p.gated ? 2 * line : line) + col;
+                        at[0] = z[i];
+                        if (p.gated) at[line] = u[i];
                     }
                     float v = act_value<decltype(a)::value>(z[i]);
                     if (p.gated) v *= u[i];

@@ -240,7 +240,8 @@ LinearOut linear_call(const Tensor& x, const Tensor& weight, const Tensor& bias,
     c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
     shape.back() = a.outputs;
     o.y = empty_like_type(x, shape, out);
-    if (want_z) o.z = empty_like_type(x, {rx.n, n_all}, ScalarType::Float);
+    if (want_z)
+        o.z = empty_like_type(x, {rx.n, gated ? 2 : 1, (a.outputs + 3) / 4 * 4}, ScalarType::Float);
     a.x = rx.p(), a.weight = rw.p(), a.bias = ptr(bias), a.residual = rr.p();
     a.x_scale = (const float*)ptr(x_scale), a.weight_scale = (const float*)ptr(w_scale);
     a.y = ptr(o.y), a.saved = (float*)ptr(o.z);
