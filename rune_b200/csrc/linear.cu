@@ -69,7 +69,7 @@ struct TileParams {
     int tiles_m, tiles_n, bn, stages;
     Divisor by_tiles, by_group, by_last;  // tile_of's: all tiles, a group's, the last group's rows
     int a_mn, b_mn, act;
-    int vec_out, vec_in, vec_bias;  // 16-byte accesses allowed
+    int tma_out, vec_in, vec_bias;  // rows on 16 bytes: copies by TMA, 16-byte accesses
     uint32_t idesc;
     void* out;
     const void* in;         // residual, or dy
@@ -161,12 +161,6 @@ __device__ __forceinline__ uint16_t get_half(uint32_t addr) {
     asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
     return v;
 }
-__device__ __forceinline__ uint32_t get_word(uint32_t addr) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-    return v;
-}
-
 // rows x cols (of 32 x 32, zeros beyond) from src into the buffer
 template <typename T>
 __device__ __forceinline__ void load_rows(const Stage& st, const T* src, int64_t ld, int rows,
@@ -195,63 +189,49 @@ __device__ __forceinline__ void load_rows(const Stage& st, const T* src, int64_t
     }
 }
 
-// buffer -> dst, and on request the sums of the 32 rows of each column
-template <typename T, bool SUMS>
+// sums of the buffer's 32 rows in each column, with the roundings that the values have there
+template <typename T>
+__device__ __forceinline__ void column_sums(const Stage& st, int64_t cols, float* sums) {
+    const int lane = st.lane, c = (lane & 3) * 8;
+    Two s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint4 v = get16(st.turn(i));
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 f = unpack2<T>(w[j]);
+            s[j] = i == 0 ? two(f.x, f.y) : s[j] + two(f.x, f.y);
+        }
+    }
+    // eight columns in each of the lanes that share lane & 3: every step halves the columns a lane
+    // keeps, and at the end each lane has the sum of one
+    float a[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) split(s[j], a[2 * j], a[2 * j + 1]);
+    int column = 0;
+#pragma unroll
+    for (int n = 4; n > 0; n >>= 1) {
+        const bool upper = lane & (4 * n);
+#pragma unroll
+        for (int j = 0; j < n; ++j) {
+            const float give = upper ? a[j] : a[n + j];
+            a[j] = (upper ? a[n + j] : a[j]) + __shfl_xor_sync(0xffffffffu, give, 4 * n);
+        }
+        column += upper ? n : 0;
+    }
+    if (c + column < cols) sums[c + column] = a[0];
+}
+
+// the buffer's rows x cols to dst, value by value: outputs whose rows are off 16 bytes
+template <typename T>
 __device__ __forceinline__ void store_rows(const Stage& st, T* dst, int64_t ld, int rows,
-                                           int64_t cols, bool vec, float* sums) {
-    const int lane = st.lane;
-    if (vec) {
-        const int r0 = lane >> 2, c = (lane & 3) * 8;
-        T* p = dst + r0 * ld + c;
-        const bool in = c < cols;
-        Two s[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint4 v = get16(st.turn(i));
-            if (in && r0 + 8 * i < rows) *reinterpret_cast<uint4*>(p + i * 8 * ld) = v;
-            if constexpr (SUMS) {
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 f = unpack2<T>(w[j]);
-                    s[j] = i == 0 ? two(f.x, f.y) : s[j] + two(f.x, f.y);
-                }
-            }
-        }
-        if constexpr (SUMS) {
-            if (sums) {
-                // eight columns in each of the lanes that share lane & 3: every step halves the
-                // columns a lane keeps, and at the end each lane has the sum of one
-                float a[8];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) split(s[j], a[2 * j], a[2 * j + 1]);
-                int column = 0;
-#pragma unroll
-                for (int n = 4; n > 0; n >>= 1) {
-                    const bool upper = lane & (4 * n);
-#pragma unroll
-                    for (int j = 0; j < n; ++j) {
-                        const float give = upper ? a[j] : a[n + j];
-                        a[j] = (upper ? a[n + j] : a[j]) +
-                               __shfl_xor_sync(0xffffffffu, give, 4 * n);
-                    }
-                    column += upper ? n : 0;
-                }
-                if (c + column < cols) sums[c + column] = a[0];
-            }
-        }
-    } else {
-        float s = 0.0f;
+                                           int64_t cols) {
 #pragma unroll 8
-        for (int r = 0; r < 32; ++r) {
-            const uint16_t h = get_half(st.at(r, lane * 2));
-            if (r < rows && lane < cols)
-                reinterpret_cast<uint16_t*>(dst)[(int64_t)r * ld + lane] = h;
-            if constexpr (SUMS) s += unpack2<T>(h).x;
-        }
-        if constexpr (SUMS) {
-            if (sums && lane < cols) sums[lane] = s;
-        }
+    for (int r = 0; r < 32; ++r) {
+        const uint16_t h = get_half(st.at(r, st.lane * 2));
+        if (r < rows && st.lane < cols)
+            reinterpret_cast<uint16_t*>(dst)[(int64_t)r * ld + st.lane] = h;
     }
 }
 
@@ -354,6 +334,7 @@ __device__ __forceinline__ void get_row(const Stage& st, int half, Two (&v)[8]) 
 template <int MODE, typename T, bool FP8, typename Wait, typename Release>
 __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uint32_t acc,
                                          const Stage& st, const Stage& st2, int warp,
+                                         const CUtensorMap* out_map, const CUtensorMap* out2_map,
                                          Wait&& wait, Release&& release) {
     const int quarter = warp & 3, share = warp >> 2;
     const int row0 = t.mt * kBM + quarter * 32;
@@ -369,8 +350,16 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
         load_rows(st, static_cast<const T*>(p.in) + (int64_t)row0 * p.ld_in + col0 + c, p.ld_in,
                   rows, end - c, p.vec_in);
     };
+    // the buffers are free again when the last copy out has read them
+    auto reuse = [&] {
+        if (lane == 0) bulk_store_read();
+        __syncwarp();
+    };
     const bool ahead = reads && !(MODE == kForward && p.z) && share * 32 < end;
-    if (ahead) read_in(share * 32);
+    if (ahead) {
+        reuse();
+        read_in(share * 32);
+    }
     if (!wait()) return;
     if constexpr (MODE == kPartial) {
         for (int c = share * 16; c < end; c += 64) {
@@ -387,6 +376,7 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
         const int64_t col = col0 + c, left = p.n - col;
         if constexpr (MODE == kForward || MODE == kGated) {
             if (p.z) {  // the pre-activations, in float32
+                reuse();
                 for (int part = 0; part < (kGate ? 2 : 1); ++part) {
                     for (int half = 0; half < 2 && half * 16 < left; ++half) {
                         const int64_t at = part * p.n + col + half * 16;
@@ -406,10 +396,11 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
                 }
             }
         }
-        if (reads) {
-            if (!ahead || c != share * 32) read_in(c);
-            __syncwarp();
+        if (!ahead || c != share * 32) {
+            reuse();
+            if (reads) read_in(c);
         }
+        __syncwarp();
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
             const int at = c + half * 16;
@@ -471,17 +462,28 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
             }
             put_row<T>(st, half, z);
         }
+        if (p.tma_out) tc::fence_async_smem();
         __syncwarp();
-        constexpr bool kSums = MODE == kGrad || MODE == kGatedGrad;
-        const int64_t ncols = kGate ? 2 * p.n : p.n;
-        float* sums = kSums && p.colsum
-                          ? p.colsum + ((int64_t)t.mt * 4 + quarter) * ncols + col
-                          : nullptr;
-        T* out = static_cast<T*>(p.out) + (int64_t)row0 * p.ld_out + col;
-        store_rows<T, kSums>(st, out, p.ld_out, rows, left, p.vec_out, sums);
-        if constexpr (MODE == kGatedGrad)
-            store_rows<T, true>(st2, out + p.n, p.ld_out, rows, left, p.vec_out,
-                                sums ? sums + p.n : nullptr);
+        if constexpr (kReads) {
+            if (p.colsum) {
+                const int64_t ncols = kGate ? 2 * p.n : p.n;
+                float* sums = p.colsum + ((int64_t)t.mt * 4 + quarter) * ncols + col;
+                column_sums<T>(st, left, sums);
+                if constexpr (kGate) column_sums<T>(st2, left, sums + p.n);
+            }
+        }
+        if (p.tma_out) {
+            if (lane == 0 && rows > 0) {
+                bulk_store(out_map, st.base, (int)col, row0);
+                if constexpr (MODE == kGatedGrad) bulk_store(out2_map, st2.base, (int)col, row0);
+                bulk_store_commit();
+            }
+        } else {
+            T* out = static_cast<T*>(p.out) + (int64_t)row0 * p.ld_out + col;
+            store_rows<T>(st, out, p.ld_out, rows, left);
+            if constexpr (MODE == kGatedGrad)
+                store_rows<T>(st2, out + p.n, p.ld_out, rows, left);
+        }
         __syncwarp();
     }
     if (share * 32 >= end) release();  // no columns here
@@ -494,6 +496,7 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
 template <int MODE, typename T, bool FP8, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+       const __grid_constant__ CUtensorMap map_o, const __grid_constant__ CUtensorMap map_o2,
        const TileParams p) {
     using namespace tc;
     extern __shared__ __align__(1024) unsigned char smem[];
@@ -674,7 +677,7 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
             if (PAIR) t.mt = t.mt * 2 + rank;
             const int b = n_tile & 1, round = n_tile >> 1;
             epilogue<MODE, T, FP8>(
-                p, t, tmem + b * 256 + quarter, st, st2, warp,
+                p, t, tmem + b * 256 + quarter, st, st2, warp, &map_o, &map_o2,
                 [&] {
                     ok = mbar_wait(smem_u32(&sh->acc_full[b]), round & 1) && !*fail;
                     ok = __all_sync(0xffffffffu, ok);
@@ -693,6 +696,7 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
                     __syncwarp();
                 });
         }
+        if (lane == 0) bulk_store_read();  // the copies out have read the buffers
         if (!ok && !*fail) *fail = 4;
     }
     __syncwarp();
@@ -775,7 +779,7 @@ __global__ void __launch_bounds__(256) k_join(const TileParams p, const float* _
             else if (p.in) v[j] += to_float(static_cast<const T*>(p.in)[row * p.ld_in + col + j]);
         }
         T* out = static_cast<T*>(p.out) + row * p.ld_out + col;
-        if (p.vec_out && col + 4 <= p.n)
+        if (p.tma_out && col + 4 <= p.n)
             *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
         else
             for (int j = 0; j < 4 && col + j < p.n; ++j) out[j] = from_float<T>(v[j]);
@@ -919,9 +923,17 @@ Plan plan_product(int64_t m, int64_t n_cols, int kblocks, bool can_split, bool g
     return best;
 }
 
+CUtensorMap make_out_map(const void* p, int64_t rows, int64_t cols, int64_t ld);
+
 template <int MODE, typename T, bool FP8, bool PAIR>
 void launch_tile(const CUtensorMap& a, const CUtensorMap& b, TileParams p, int sms, int device,
                  cudaStream_t stream) {
+    CUtensorMap o = a, o2 = a;  // unused unless the output goes by TMA
+    if (MODE != kPartial && p.tma_out) {
+        o = make_out_map(p.out, p.m, p.n, p.ld_out);
+        if (MODE == kGatedGrad)
+            o2 = make_out_map(static_cast<T*>(p.out) + p.n, p.m, p.n, p.ld_out);
+    }
     static std::atomic<uint64_t> allowed{0};  // devices whose limit is raised
     if (device >= 64 || !(allowed.load(std::memory_order_relaxed) >> device & 1)) {
         RUNE_CUDA_TRY(cudaFuncSetAttribute(k_tile<MODE, T, FP8, PAIR>,
@@ -947,7 +959,7 @@ void launch_tile(const CUtensorMap& a, const CUtensorMap& b, TileParams p, int s
     at[0].val.clusterDim = {2, 1, 1};
     cfg.attrs = at;
     cfg.numAttrs = PAIR ? 1 : 0;
-    RUNE_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_tile<MODE, T, FP8, PAIR>, a, b, p));
+    RUNE_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_tile<MODE, T, FP8, PAIR>, a, b, o, o2, p));
 }
 
 // One product D[m, n] = A B^T: operands, epilogue (in p) and scratch for a split.
@@ -1095,7 +1107,7 @@ void forward(const rune_linear_args& a, Scratch& ws, cudaStream_t stream) {
     p.m = a.rows, p.n = a.outputs;
     p.act = a.activation;
     p.out = a.y, p.ld_out = a.outputs;
-    p.vec_out = wide16(a.y, a.outputs, a.outputs);
+    p.tma_out = wide16(a.y, a.outputs, a.outputs);
     p.in = a.residual, p.ld_in = a.residual_stride;
     p.vec_in = a.residual && wide16(a.residual, a.residual_stride, a.outputs);
     p.bias = a.bias;
@@ -1177,7 +1189,7 @@ void backward(const rune_linear_grad_args& a, Scratch& ws, cudaStream_t stream) 
             p.m = a.rows, p.n = a.outputs;
             p.act = a.activation;
             p.out = to, p.ld_out = dz.ld;
-            p.vec_out = !a.gated || a.outputs % 8 == 0;
+            p.tma_out = !a.gated || a.outputs % 8 == 0;
             p.in = a.dy, p.ld_in = a.dy_stride;
             p.vec_in = wide16(a.dy, a.dy_stride, a.outputs);
             p.bias = a.bias;
@@ -1199,7 +1211,7 @@ void backward(const rune_linear_grad_args& a, Scratch& ws, cudaStream_t stream) 
         p.m = a.rows, p.n = a.inputs;
         p.act = RUNE_ACT_NONE;
         p.out = a.dx, p.ld_out = a.inputs;
-        p.vec_out = wide16(a.dx, a.inputs, a.inputs);
+        p.tma_out = wide16(a.dx, a.inputs, a.inputs);
         run_product(g, p, ws, a.device, stream);
     }
     if (a.dweight) {
@@ -1212,7 +1224,7 @@ void backward(const rune_linear_grad_args& a, Scratch& ws, cudaStream_t stream) 
         p.m = n_all, p.n = a.inputs;
         p.act = RUNE_ACT_NONE;
         p.out = a.dweight, p.ld_out = a.inputs;
-        p.vec_out = wide16(a.dweight, a.inputs, a.inputs);
+        p.tma_out = wide16(a.dweight, a.inputs, a.inputs);
         run_product(g, p, ws, a.device, stream);
     }
 }
@@ -1291,6 +1303,26 @@ CUtensorMap make_map(const Matrix& m, int elem_bytes, int box_rows) {
                     "an operand cannot be described to TMA (status " + std::to_string(r) + ")");
     return map;
 }
+
+namespace {
+
+// 32 x 32 boxes of a 16-bit output with the 64-byte swizzle, which is the buffers' own
+CUtensorMap make_out_map(const void* p, int64_t rows, int64_t cols, int64_t ld) {
+    CUtensorMap map;
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)(ld * 2)};
+    const cuuint32_t box[2] = {32, 32}, step[2] = {1, 1};
+    CUresult r = encode_tiled()(&map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(p),
+                                dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        throw Error(RUNE_ERR_INVALID,
+                    "an output cannot be described to TMA (status " + std::to_string(r) + ")");
+    return map;
+}
+
+}  // namespace
 
 unsigned* wait_flag(int device) {
     if (device < 0 || device >= kMaxDevices)
