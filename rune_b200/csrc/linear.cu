@@ -787,76 +787,180 @@ __global__ void __launch_bounds__(256) k_join(const TileParams p, const float* _
 }
 
 // ----------------------------------------------------------------------------- elementwise
-// dz from a saved float32 z and dy, and the sums of kGradRows rows of each column. A thread owns
-// one column of a strip; consecutive lanes read consecutive columns.
-constexpr int kGradRows = 64;
+// A block works on strips of rows x kColumns columns: a thread has four columns and every fourth
+// row of the strip, and the four threads of a column join their sums in order.
+constexpr int kColumns = 256;
 
-template <bool GATED, typename T>
-__global__ void __launch_bounds__(256)
-k_act_grad(int64_t m, int64_t n, const float* __restrict__ z, int64_t ld_part,
-           const T* __restrict__ dy, int64_t ld_dy, T* __restrict__ dz, int64_t ld_dz, int act, float* __restrict__ sums) {
-    const int64_t col = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (col >= n) return;
-    const int64_t nz = GATED ? 2 * n : n, ld_z = GATED ? 2 * ld_part : ld_part;
-    const int64_t strips = (m + kGradRows - 1) / kGradRows;
-    for (int64_t strip = blockIdx.y; strip < strips; strip += gridDim.y) {
-        const int64_t r0 = strip * kGradRows, r1 = min(m, r0 + kGradRows);
-        float s0 = 0.0f, s1 = 0.0f;
-        with_activation(act, [&](auto a) {
-#pragma unroll 8
-            for (int64_t r = r0; r < r1; ++r) {
-                float y, da, d = to_float(dy[r * ld_dy + col]);
-                act_both1<decltype(a)::value>(z[r * ld_z + col], y, da);
-                if constexpr (GATED) {
-                    float g = d * z[r * ld_z + ld_part + col] * da, u = d * y;
-                    dz[r * ld_dz + col] = from_float<T>(g);
-                    dz[r * ld_dz + n + col] = from_float<T>(u);
-                    s0 += g, s1 += u;
-                } else {
-                    float g = d * da;
-                    dz[r * ld_dz + col] = from_float<T>(g);
-                    s0 += g;
-                }
-            }
-        });
-        if (sums) {
-            sums[strip * nz + col] = s0;
-            if (GATED) sums[strip * nz + n + col] = s1;
+// rows of a strip: fewer where 64 would leave the GPU short of blocks
+int strip_rows(int64_t m, int64_t n, int sms) {
+    const int64_t across = (n + kColumns - 1) / kColumns;
+    int rows = 64;
+    while (rows > 8 && (m + rows - 1) / rows * across < 4 * sms) rows /= 2;
+    return rows;
+}
+
+// four values at p: by one access, or the `count` of them that are inside
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void get4(const T* p, int count, float (&v)[4]) {
+    if constexpr (WHOLE) {
+        const uint2 q = *reinterpret_cast<const uint2*>(p);
+        const float2 a = unpack2<T>(q.x), b = unpack2<T>(q.y);
+        v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = j < count ? to_float(p[j]) : 0.0f;
+    }
+}
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void set4(T* p, int count, const float (&v)[4]) {
+    if constexpr (WHOLE) {
+        *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < count) p[j] = from_float<T>(v[j]);
+    }
+}
+// joins the four threads' sums of a column and writes them
+__device__ __forceinline__ void join4(const float (&s)[4], float* sums, int count) {
+    __shared__ float joined[4][kColumns];
+    const int quad = threadIdx.x & 63, part = threadIdx.x >> 6;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) joined[part][quad * 4 + j] = s[j];
+    __syncthreads();
+    if (part == 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int c = quad * 4 + j;
+            if (j < count) sums[j] = joined[0][c] + joined[1][c] + joined[2][c] + joined[3][c];
         }
     }
 }
 
-// sums of kGradRows rows of each column
-template <typename T>
-__global__ void __launch_bounds__(256)
-k_column_sums(int64_t m, int64_t n, const T* __restrict__ x, int64_t ld, float* __restrict__ sums) {
-    const int64_t col = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (col >= n) return;
-    const int64_t strips = (m + kGradRows - 1) / kGradRows;
-    for (int64_t strip = blockIdx.y; strip < strips; strip += gridDim.y) {
-        const int64_t r0 = strip * kGradRows, r1 = min(m, r0 + kGradRows);
-        float s = 0.0f;
-#pragma unroll 8
-        for (int64_t r = r0; r < r1; ++r) s += to_float(x[r * ld + col]);
-        sums[strip * n + col] = s;
+// dz from a saved float32 z and dy, and the sums of each strip's columns
+template <bool GATED, typename T>
+__global__ void __launch_bounds__(256, 5)
+k_act_grad(int64_t m, int64_t n, const float* __restrict__ z, int64_t ld_part,
+           const T* __restrict__ dy, int64_t ld_dy, bool wide_dy, T* __restrict__ dz,
+           int64_t ld_dz, int act, int strip, float* __restrict__ sums) {
+    const int64_t col = (int64_t)blockIdx.x * kColumns + (threadIdx.x & 63) * 4;
+    const int count = (int)max((int64_t)0, min((int64_t)4, n - col)), part = threadIdx.x >> 6;
+    const int64_t nz = GATED ? 2 * n : n, ld_z = GATED ? 2 * ld_part : ld_part;
+    const int64_t strips = (m + strip - 1) / strip;
+    const bool whole = wide_dy && count == 4 && (!GATED || n % 4 == 0);
+    for (int64_t k = blockIdx.y; k < strips; k += gridDim.y) {
+        const int64_t r1 = min(m, (k + 1) * strip);
+        float s0[4] = {}, s1[4] = {};
+        auto rows = [&](auto a, auto whole_c) {
+            constexpr int ACT = decltype(a)::value;
+            constexpr bool WHOLE = decltype(whole_c)::value;  // no branch among the loads
+#pragma unroll 2
+            for (int64_t r = k * strip + part; r < r1; r += 4) {
+                const float4 q = *reinterpret_cast<const float4*>(z + r * ld_z + col);
+                float4 up = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (GATED) up = *reinterpret_cast<const float4*>(z + r * ld_z + ld_part + col);
+                float d[4], g[4];
+                get4<T, WHOLE>(dy + r * ld_dy + col, count, d);
+                Two y0, y1, a0, a1;
+                act_both<ACT>(two(q.x, q.y), y0, a0);
+                act_both<ACT>(two(q.z, q.w), y1, a1);
+                Two g0 = two(d[0], d[1]) * a0, g1 = two(d[2], d[3]) * a1;
+                if constexpr (GATED) {
+                    float u[4];
+                    g0 = g0 * two(up.x, up.y), g1 = g1 * two(up.z, up.w);
+                    split(two(d[0], d[1]) * y0, u[0], u[1]);
+                    split(two(d[2], d[3]) * y1, u[2], u[3]);
+                    set4<T, WHOLE>(dz + r * ld_dz + n + col, count, u);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s1[j] += u[j];
+                }
+                split(g0, g[0], g[1]);
+                split(g1, g[2], g[3]);
+                set4<T, WHOLE>(dz + r * ld_dz + col, count, g);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s0[j] += g[j];
+            }
+        };
+        if (count > 0)
+            with_activation(act, [&](auto a) {
+                if (whole) rows(a, std::true_type());
+                else rows(a, std::false_type());
+            });
+        if (sums) {
+            join4(s0, sums + k * nz + col, count);
+            if (GATED) join4(s1, sums + k * nz + n + col, count);
+        }
     }
 }
 
-// Copies lines of `cols` values to lines padded to 16 bytes, for operands that TMA cannot read
-// in place. A thread writes 16 bytes; the padding is never read.
-template <typename W>
+// the sums of each strip's columns
+template <typename T>
 __global__ void __launch_bounds__(256)
-k_pack(const W* __restrict__ src, int64_t rows, int64_t cols, int64_t ld, W* __restrict__ dst,
-       int64_t ld_dst) {
-    constexpr int V = 16 / sizeof(W);
-    const int64_t groups = ld_dst / V, total = rows * groups;
-    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
-         i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t r = i / groups, c = (i % groups) * V;
-        __align__(16) W v[V];
+k_column_sums(int64_t m, int64_t n, const T* __restrict__ x, int64_t ld, bool wide, int strip,
+              float* __restrict__ sums) {
+    const int64_t col = (int64_t)blockIdx.x * kColumns + (threadIdx.x & 63) * 4;
+    const int count = (int)max((int64_t)0, min((int64_t)4, n - col)), part = threadIdx.x >> 6;
+    const int64_t strips = (m + strip - 1) / strip;
+    for (int64_t k = blockIdx.y; k < strips; k += gridDim.y) {
+        const int64_t r1 = min(m, (k + 1) * strip);
+        float s[4] = {};
+        auto rows = [&](auto whole_c) {
+#pragma unroll 8
+            for (int64_t r = k * strip + part; r < r1; r += 4) {
+                float v[4];
+                get4<T, decltype(whole_c)::value>(x + r * ld + col, count, v);
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = c + j < cols ? src[r * ld + c + j] : W(0);
-        *reinterpret_cast<uint4*>(dst + r * ld_dst + c) = *reinterpret_cast<uint4*>(v);
+                for (int j = 0; j < 4; ++j) s[j] += v[j];
+            }
+        };
+        if (wide && count == 4) rows(std::true_type());
+        else if (count > 0) rows(std::false_type());
+        join4(s, sums + k * n + col, count);
+    }
+}
+
+// Copies lines of `bytes` bytes, `ld` apart, to lines padded to 16 bytes (ld_dst), for operands
+// that TMA cannot read in place; the padding is never read. A thread writes 16 bytes from the two
+// aligned 16-byte words that hold them, shifted together; where such a word is not inside the
+// matrix (its first and last lines), byte by byte.
+__global__ void __launch_bounds__(256)
+k_pack(const uint8_t* __restrict__ src, int64_t rows, int64_t bytes, int64_t ld,
+       uint8_t* __restrict__ dst, int64_t ld_dst) {
+    const int64_t pieces = ld_dst / 16;
+    const uint8_t* const end = src + (rows - 1) * ld + bytes;
+    const int64_t piece = (int64_t)blockIdx.x * 32 + threadIdx.x, at = piece * 16;
+    if (piece >= pieces) return;
+    for (int64_t r = (int64_t)blockIdx.y * 8 + threadIdx.y; r < rows; r += (int64_t)gridDim.y * 8) {
+        const uint8_t* from = src + r * ld + at;
+        const unsigned off = (unsigned)((uintptr_t)from & 15);
+        const uint8_t* word = from - off;
+        uint4 out;
+        if (word >= src && word + (off ? 32 : 16) <= end) {
+            const uint4 a = __ldg(reinterpret_cast<const uint4*>(word));
+            const uint4 b = off ? __ldg(reinterpret_cast<const uint4*>(word) + 1) : a;
+            uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            // by whole words in two steps, then by the bits that are left
+            if (off & 8) {
+#pragma unroll
+                for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+            }
+            if (off & 4) {
+#pragma unroll
+                for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+            }
+            const unsigned bits = (off & 3) * 8;
+            out.x = __funnelshift_r(w[0], w[1], bits);
+            out.y = __funnelshift_r(w[1], w[2], bits);
+            out.z = __funnelshift_r(w[2], w[3], bits);
+            out.w = __funnelshift_r(w[3], w[4], bits);
+        } else {
+            uint32_t w[4] = {};
+            for (int i = 0; i < 16; ++i)
+                if (at + i < bytes) w[i / 4] |= (uint32_t)from[i] << (i % 4 * 8);
+            out = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        *reinterpret_cast<uint4*>(dst + r * ld_dst + at) = out;
     }
 }
 
@@ -887,10 +991,11 @@ double block_cycles(bool pair, int bn) {
 }
 
 // Tile, range of k and pairing of one product, by a model of its time in cycles: the k-blocks, an
-// epilogue of 10 cycles a column, hidden behind the next tile's products, and for ranges of k the
-// launch and the traffic of their join.
-Plan plan_product(int64_t m, int64_t n_cols, int kblocks, bool can_split, bool gate, int sms,
-                  uint32_t fixed) {
+// epilogue (16 cycles a column, 25 with an activation: measured at 110592 x 256 -> 512, 35 and
+// 51 us), hidden behind the next tile's products, and for ranges of k the launch and the traffic of
+// their join.
+Plan plan_product(int64_t m, int64_t n_cols, int kblocks, bool can_split, bool gate, bool act,
+                  int sms, uint32_t fixed) {
     Plan best{};
     double best_cost = 0.0;
     for (int pair = 1; pair >= 0; --pair) {
@@ -906,7 +1011,7 @@ Plan plan_product(int64_t m, int64_t n_cols, int kblocks, bool can_split, bool g
                 const int splits = (kblocks + per - 1) / per;
                 const double waves = (double)((tiles * splits + units - 1) / units);
                 const double main = per * block_cycles(pair, bn);
-                const double epi = 10.0 * bn;
+                const double epi = 1000.0 + (act ? (gate ? 15.0 : 25.0) : 16.0) * bn;
                 double cost = 2000.0 + waves * std::max(main, epi) + std::min(main, epi);
                 if (splits > 1)
                     cost += 5000.0 + (double)m * n_cols * (splits + 1) * 4.0 / 3000.0;
@@ -980,7 +1085,8 @@ void run_mode(const Product& g, TileParams p, Scratch& ws, int device, cudaStrea
     const int64_t n_cols = pair ? 2 * p.n : p.n;
     p.kblocks = (int)((g.k + line - 1) / line);
     const bool can_split = MODE == kForward || MODE == kGated;
-    Plan plan = plan_product(p.m, n_cols, p.kblocks, can_split, pair, sms, kFixedSmem<MODE>);
+    Plan plan = plan_product(p.m, n_cols, p.kblocks, can_split, pair,
+                             p.act != RUNE_ACT_NONE, sms, kFixedSmem<MODE>);
     float* part = nullptr;
     const int64_t ld_part = (n_cols + 3) / 4 * 4;
     if (plan.splits > 1) part = ws.take<float>(plan.splits * p.m * ld_part);
@@ -1070,14 +1176,12 @@ Matrix readable(Matrix m, int elem_bytes, Scratch& ws, cudaStream_t stream) {
         d.p = reinterpret_cast<const void*>(256);  // any aligned address: only sizes are asked
         return d;
     }
-    const int64_t total = m.rows * d.ld * elem_bytes / 16;
-    const int grid = (int)std::min<int64_t>((total + 255) / 256, 1 << 16);
-    if (elem_bytes == 1)
-        k_pack<<<grid, 256, 0, stream>>>(static_cast<const uint8_t*>(m.p), m.rows, m.cols, m.ld,
-                                         static_cast<uint8_t*>(to), d.ld);
-    else
-        k_pack<<<grid, 256, 0, stream>>>(static_cast<const uint16_t*>(m.p), m.rows, m.cols, m.ld,
-                                         static_cast<uint16_t*>(to), d.ld);
+    const int64_t pieces = d.ld * elem_bytes / 16;
+    const dim3 grid((unsigned)((pieces + 31) / 32),
+                    (unsigned)std::min<int64_t>((m.rows + 7) / 8, 65535));
+    k_pack<<<grid, dim3(32, 8), 0, stream>>>(static_cast<const uint8_t*>(m.p), m.rows,
+                                         m.cols * elem_bytes, m.ld * elem_bytes,
+                                         static_cast<uint8_t*>(to), d.ld * elem_bytes);
     RUNE_LAUNCH_CHECK();
     return d;
 }
@@ -1131,22 +1235,25 @@ void backward(const rune_linear_grad_args& a, Scratch& ws, cudaStream_t stream) 
     Matrix dz{a.dy, a.rows, n_all, a.dy_stride};
     float* sums = nullptr;
     int64_t parts = 0;
-    const int64_t strips = (a.rows + kGradRows - 1) / kGradRows;
+    const int strip = strip_rows(a.rows, a.outputs, sm_count(a.device));
+    const int64_t strips = (a.rows + strip - 1) / strip;
+    const bool wide_dy = aligned(a.dy, 8) && a.dy_stride % 4 == 0;
     if (plain) {
         if (want_dz) dz = readable(dz, 2, ws, stream);
         if (a.dbias) {
             parts = strips;
             sums = ws.take<float>(parts * n_all);
             if (!ws.sizing()) {
-                dim3 grid((unsigned)((n_all + 255) / 256),
+                dim3 grid((unsigned)((n_all + kColumns - 1) / kColumns),
                           (unsigned)std::min<int64_t>(strips, 65535));
                 if (half)
                     k_column_sums<<<grid, 256, 0, stream>>>(
-                        a.rows, n_all, static_cast<const __half*>(a.dy), a.dy_stride, sums);
+                        a.rows, n_all, static_cast<const __half*>(a.dy), a.dy_stride, wide_dy, strip,
+                        sums);
                 else
                     k_column_sums<<<grid, 256, 0, stream>>>(
-                        a.rows, n_all, static_cast<const __nv_bfloat16*>(a.dy), a.dy_stride,
-                        sums);
+                        a.rows, n_all, static_cast<const __nv_bfloat16*>(a.dy), a.dy_stride, wide_dy,
+                        strip, sums);
                 RUNE_LAUNCH_CHECK();
             }
         }
@@ -1158,7 +1265,7 @@ void backward(const rune_linear_grad_args& a, Scratch& ws, cudaStream_t stream) 
             parts = strips;
             if (a.dbias) sums = ws.take<float>(parts * n_all);
             if (!ws.sizing()) {
-                dim3 grid((unsigned)((a.outputs + 255) / 256),
+                dim3 grid((unsigned)((a.outputs + kColumns - 1) / kColumns),
                           (unsigned)std::min<int64_t>(strips, 65535));
                 auto go = [&](auto t) {
                     using T = decltype(t);
@@ -1166,12 +1273,12 @@ void backward(const rune_linear_grad_args& a, Scratch& ws, cudaStream_t stream) 
                     auto* out = reinterpret_cast<T*>(to);
                     if (a.gated)
                         k_act_grad<true, T><<<grid, 256, 0, stream>>>(
-                            a.rows, a.outputs, a.saved, saved_line(a.outputs), dy, a.dy_stride, out, dz.ld,
-                            a.activation, sums);
+                            a.rows, a.outputs, a.saved, saved_line(a.outputs), dy, a.dy_stride, wide_dy,
+                            out, dz.ld, a.activation, strip, sums);
                     else
                         k_act_grad<false, T><<<grid, 256, 0, stream>>>(
-                            a.rows, a.outputs, a.saved, saved_line(a.outputs), dy, a.dy_stride, out, dz.ld,
-                            a.activation, sums);
+                            a.rows, a.outputs, a.saved, saved_line(a.outputs), dy, a.dy_stride, wide_dy,
+                            out, dz.ld, a.activation, strip, sums);
                 };
                 if (half) go(__half());
                 else go(__nv_bfloat16());

@@ -492,28 +492,28 @@ k_norm_bwd_long(const rune_norm_grad_args p, float* __restrict__ partials) {
     }
 }
 
-// Columns of float32 partials [parts][width]: a block sums 16 columns with 64 threads each, then
+// Columns of float32 partials [parts][width]: a block sums 8 columns with 128 threads each, then
 // joins their sums in order.
 template <typename T>
 __global__ void __launch_bounds__(1024)
 k_sum_partials(const float* __restrict__ partials, int64_t parts, int64_t width, T* out) {
-    __shared__ float s[64][17];
-    const int64_t col = (int64_t)blockIdx.x * 16 + threadIdx.x;
+    __shared__ float s[128][9];
+    const int64_t col = (int64_t)blockIdx.x * 8 + threadIdx.x;
     float v = 0.0f;
     if (col < width) {
-#pragma unroll 8
-        for (int64_t r = threadIdx.y; r < parts; r += 64) v += partials[r * width + col];
+#pragma unroll 16
+        for (int64_t r = threadIdx.y; r < parts; r += 128) v += partials[r * width + col];
     }
     s[threadIdx.y][threadIdx.x] = v;
     __syncthreads();
-    if (threadIdx.y < 8) {
-        for (int k = threadIdx.y + 8; k < 64; k += 8) v += s[k][threadIdx.x];
+    if (threadIdx.y < 16) {
+        for (int k = threadIdx.y + 16; k < 128; k += 16) v += s[k][threadIdx.x];
         s[threadIdx.y][threadIdx.x] = v;
     }
     __syncthreads();
     if (threadIdx.y == 0 && col < width) {
         float sum = 0.0f;
-        for (int k = 0; k < 8; ++k) sum += s[k][threadIdx.x];
+        for (int k = 0; k < 16; ++k) sum += s[k][threadIdx.x];
         out[col] = from_float<T>(sum);
     }
 }
@@ -680,8 +680,8 @@ int sm_count(int device) {
 
 void sum_partials(const float* partials, int64_t parts, int64_t width, void* out, int dtype,
                   cudaStream_t stream) {
-    dim3 block(16, 64);
-    int grid = (int)((width + 15) / 16);
+    dim3 block(8, 128);
+    int grid = (int)((width + 7) / 8);
     if (dtype == RUNE_F32)
         k_sum_partials<<<grid, block, 0, stream>>>(partials, parts, width, (float*)out);
     else if (dtype == RUNE_F16)

@@ -274,15 +274,6 @@ __device__ __forceinline__ float act_value(float x) {
     return a;
 }
 
-template <int ACT>
-__device__ __forceinline__ void act_both1(float x, float& y, float& dy) {
-    Two a, b;
-    float unused;
-    act_both<ACT>(two(x), a, b);
-    split(a, y, unused);
-    split(b, dy, unused);
-}
-
 // fn(std::integral_constant<int, ACT>) for the activation code `act`
 template <typename Fn>
 __host__ __device__ __forceinline__ void with_activation(int act, Fn&& fn) {
