@@ -1,0 +1,129 @@
+"""The Möbius scalar network in mixed precision, trainable: projection, residual blocks, head.
+
+The engine evaluates Möbius models in float32 without parameter gradients. ``ScalarNetwork`` is
+the same per-atom network (rune/mobius/model.py:256-305 without messages, layers.py:26-89) on the
+operators of ``rune_b200.ops``: float32 parameters under the reference's names, 16-bit products
+with float32 accumulation, gradients for all of them. For adapting a checkpoint's network,
+distilling a model into it, or serving many atoms' energies from descriptors; ``quantized`` gives
+an 8-bit copy for serving.
+
+A block adds its output to the residual stream in the next block's normalisation, so the stream
+is read and written once per block.
+"""
+
+from __future__ import annotations
+
+import torch
+import torch.nn as nn
+
+from . import ops
+from .mobius.model import ElementwiseLinearHead, ResidualBlock, RMSNorm
+
+
+class ScalarNetwork(nn.Module):
+    """Per-atom energies [N] (float32) of descriptors [N, inputs] and element indices [N].
+
+    gated: the blocks' first layer is ``act(x Wg^T + bg) * (x Wu^T + bu)``; ``ffn.0`` then holds
+    2 * ffn rows, the gate's first. dtype: torch.bfloat16 or torch.float16, of the states.
+    """
+
+    def __init__(self, n_elements, inputs, hidden, ffn, blocks, activation="silu", gated=False,
+                 norm_eps=1.0e-8, dtype=torch.bfloat16):
+        super().__init__()
+        if min(n_elements, inputs, hidden, ffn) <= 0 or blocks < 0:
+            raise ValueError("ScalarNetwork dimensions must be positive.")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"dtype must be float16 or bfloat16, not {dtype}.")
+        self.activation, self.gated, self.dtype = str(activation).strip().lower(), bool(gated), dtype
+        self.norm_eps = float(norm_eps)
+        self.register_buffer("q_scaler", torch.ones(inputs))
+        self.input_projection = nn.Linear(inputs, hidden)
+        self.element_embedding = nn.Embedding(n_elements, hidden)
+        self.residual_blocks = nn.ModuleList(
+            ResidualBlock(hidden, ffn, activation, norm_eps=norm_eps) for _ in range(blocks))
+        if gated:
+            for block in self.residual_blocks:
+                block.ffn[0] = nn.Linear(hidden, 2 * ffn)
+        self.output_norm = RMSNorm(hidden, eps=norm_eps)
+        self.energy_heads = ElementwiseLinearHead(n_elements, hidden)
+
+    @classmethod
+    def from_mobius(cls, model, dtype=torch.bfloat16):
+        """The network of a Möbius Local model (``rune_b200.mobius.plugin``), its weights copied."""
+        if model.message_layers:
+            raise ValueError("ScalarNetwork has no messages: a Mobius model with "
+                             "message_layers = 0 is needed.")
+        net = cls(model.n_elements, model.input_dim, model.hidden_dim, model.ffn_dim,
+                  model.blocks, model.activation, norm_eps=model.norm_eps, dtype=dtype)
+        own = net.state_dict()
+        net.load_state_dict({k: v for k, v in model.state_dict().items() if k in own})
+        return net.to(model.q_scaler.device)
+
+    def _cast(self, module):
+        return module.weight.to(self.dtype), module.bias.to(self.dtype)
+
+    def _start(self, descriptors, types):
+        q = (descriptors * self.q_scaler).to(self.dtype)
+        weight, bias = self._cast(self.input_projection)
+        embedding = self.element_embedding.weight.to(self.dtype)[types]
+        return ops.linear(q, weight, bias=bias, residual=embedding)
+
+    def _finish(self, stream, delta, types):
+        eps, weight = self.norm_eps, self.output_norm.weight
+        h = (ops.rms_norm(stream, weight, eps=eps) if delta is None
+             else ops.rms_norm(delta, weight, residual=stream, eps=eps)[0])
+        head = self.energy_heads
+        return (h.float() * head.weight[types]).sum(-1) + head.bias[types]
+
+    def forward(self, descriptors, types):
+        stream, delta = self._start(descriptors, types), None
+        for block in self.residual_blocks:
+            if delta is None:
+                x = ops.rms_norm(stream, block.norm.weight, eps=self.norm_eps)
+            else:
+                x, stream = ops.rms_norm(delta, block.norm.weight, residual=stream,
+                                         eps=self.norm_eps)
+            weight, bias = self._cast(block.ffn[0])
+            if self.gated:
+                x = ops.gated_linear(x, weight, bias=bias, activation=self.activation)
+            else:
+                x = ops.linear(x, weight, bias=bias, activation=self.activation)
+            weight, bias = self._cast(block.ffn[2])
+            delta = ops.linear(x, weight, bias=bias)
+        return self._finish(stream, delta, types)
+
+    def quantized(self):
+        """A function like ``forward`` with the blocks' products in 8 bits, weights laid out now."""
+        with torch.no_grad():
+            layers = []
+            for block in self.residual_blocks:
+                pair = []
+                for layer in (block.ffn[0], block.ffn[2]):
+                    w, scale = ops.quantize_fp8(layer.weight)
+                    pair.append((w, scale, layer.bias.to(self.dtype)))
+                layers.append((block.norm.weight.detach().clone(), *pair))
+        return _Quantized(self, layers)
+
+
+class _Quantized:
+    """Forward of a ``ScalarNetwork`` whose blocks read e4m3 weights and activations."""
+
+    def __init__(self, net, layers):
+        self.net, self.layers = net, layers
+
+    @torch.no_grad()
+    def __call__(self, descriptors, types):
+        net, delta = self.net, None
+        first = ops.gated_linear if net.gated else ops.linear
+        more = {"out_dtype": net.dtype}
+        stream = net._start(descriptors, types)
+        for norm, (w0, s0, b0), (w1, s1, b1) in self.layers:
+            if delta is None:
+                x, sx = ops.rms_norm_fp8(stream, norm, eps=net.norm_eps)
+            else:
+                x, sx, stream = ops.rms_norm_fp8(delta, norm, residual=stream, eps=net.norm_eps)
+            x = first(x, w0, bias=b0, activation=net.activation, x_scale=sx, weight_scale=s0,
+                      **more)
+            x, sx = ops.quantize_fp8(x)
+            delta = ops.linear(x, w1, bias=b1, x_scale=sx, weight_scale=s1, **more)
+        return net._finish(stream, delta, types)
