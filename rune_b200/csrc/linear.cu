@@ -189,38 +189,26 @@ __device__ __forceinline__ void load_rows(const Stage& st, const T* src, int64_t
     }
 }
 
-// sums of the buffer's 32 rows in each column, with the roundings that the values have there
-template <typename T>
-__device__ __forceinline__ void column_sums(const Stage& st, int64_t cols, float* sums) {
-    const int lane = st.lane, c = (lane & 3) * 8;
-    Two s[4];
+// sums over the warp's rows of 16 columns that each lane holds of its own row, before they are
+// rounded. Every step halves the columns that a lane keeps; then two lanes have one column.
+__device__ __forceinline__ void column_sums(const Two (&z)[8], int lane, int64_t cols,
+                                            float* sums) {
+    float a[16];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint4 v = get16(st.turn(i));
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 f = unpack2<T>(w[j]);
-            s[j] = i == 0 ? two(f.x, f.y) : s[j] + two(f.x, f.y);
-        }
-    }
-    // eight columns in each of the lanes that share lane & 3: every step halves the columns a lane
-    // keeps, and at the end each lane has the sum of one
-    float a[8];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) split(s[j], a[2 * j], a[2 * j + 1]);
+    for (int j = 0; j < 8; ++j) split(z[j], a[2 * j], a[2 * j + 1]);
     int column = 0;
 #pragma unroll
-    for (int n = 4; n > 0; n >>= 1) {
-        const bool upper = lane & (4 * n);
+    for (int n = 8; n > 0; n >>= 1) {
+        const bool upper = lane & (2 * n);
 #pragma unroll
         for (int j = 0; j < n; ++j) {
             const float give = upper ? a[j] : a[n + j];
-            a[j] = (upper ? a[n + j] : a[j]) + __shfl_xor_sync(0xffffffffu, give, 4 * n);
+            a[j] = (upper ? a[n + j] : a[j]) + __shfl_xor_sync(0xffffffffu, give, 2 * n);
         }
         column += upper ? n : 0;
     }
-    if (c + column < cols) sums[c + column] = a[0];
+    a[0] += __shfl_xor_sync(0xffffffffu, a[0], 1);
+    if (!(lane & 1) && column < cols) sums[column] = a[0];
 }
 
 // the buffer's rows x cols to dst, value by value: outputs whose rows are off 16 bytes
@@ -371,6 +359,9 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
         release();
         return;
     }
+    float* sums = nullptr;  // this warp's row of the parts of dbias
+    if (kReads && p.colsum)
+        sums = p.colsum + ((int64_t)t.mt * 4 + quarter) * (kGate ? 2 * p.n : p.n);
     const float xs = FP8 && lane < rows ? p.x_scale[row0 + lane] : 0.0f;
     for (int c = share * 32; c < end; c += 128) {
         const int64_t col = col0 + c, left = p.n - col;
@@ -460,18 +451,16 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
                 });
                 put_row<T>(st2, half, u);
             }
+            if constexpr (kReads) {
+                if (sums) {
+                    column_sums(z, lane, zleft, sums + zcol);
+                    if constexpr (kGate) column_sums(u, lane, zleft, sums + p.n + zcol);
+                }
+            }
             put_row<T>(st, half, z);
         }
         if (p.tma_out) tc::fence_async_smem();
         __syncwarp();
-        if constexpr (kReads) {
-            if (p.colsum) {
-                const int64_t ncols = kGate ? 2 * p.n : p.n;
-                float* sums = p.colsum + ((int64_t)t.mt * 4 + quarter) * ncols + col;
-                column_sums<T>(st, left, sums);
-                if constexpr (kGate) column_sums<T>(st2, left, sums + p.n);
-            }
-        }
         if (p.tma_out) {
             if (lane == 0 && rows > 0) {
                 bulk_store(out_map, st.base, (int)col, row0);
