@@ -530,6 +530,7 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
     fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, sh->tmem, 0);
     volatile int* fail = &sh->fail;
+    follow_on();
 
     if (warp == kTmaWarp) {
         // ---- TMA producer
@@ -727,6 +728,7 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
 // thread; the sums' lines are padded to four values.
 template <int MODE, typename T>
 __global__ void __launch_bounds__(256) k_join(const TileParams p, const float* __restrict__ part) {
+    follow_on();
     constexpr bool kPair = MODE == kGated;
     const int64_t groups = (p.n + 3) / 4, total = p.m * groups;
     const int64_t lds = ((kPair ? 2 * p.n : p.n) + 3) / 4 * 4;
@@ -833,6 +835,7 @@ __global__ void __launch_bounds__(256, 5)
 k_act_grad(int64_t m, int64_t n, const float* __restrict__ z, int64_t ld_part,
            const T* __restrict__ dy, int64_t ld_dy, bool wide_dy, T* __restrict__ dz,
            int64_t ld_dz, int act, int strip, float* __restrict__ sums) {
+    follow_on();
     const int64_t col = (int64_t)blockIdx.x * kColumns + (threadIdx.x & 63) * 4;
     const int count = (int)max((int64_t)0, min((int64_t)4, n - col)), part = threadIdx.x >> 6;
     const int64_t nz = GATED ? 2 * n : n, ld_z = GATED ? 2 * ld_part : ld_part;
@@ -888,6 +891,7 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 k_column_sums(int64_t m, int64_t n, const T* __restrict__ x, int64_t ld, bool wide, int strip,
               float* __restrict__ sums) {
+    follow_on();
     const int64_t col = (int64_t)blockIdx.x * kColumns + (threadIdx.x & 63) * 4;
     const int count = (int)max((int64_t)0, min((int64_t)4, n - col)), part = threadIdx.x >> 6;
     const int64_t strips = (m + strip - 1) / strip;
@@ -916,6 +920,7 @@ k_column_sums(int64_t m, int64_t n, const T* __restrict__ x, int64_t ld, bool wi
 __global__ void __launch_bounds__(256)
 k_pack(const uint8_t* __restrict__ src, int64_t rows, int64_t bytes, int64_t ld,
        uint8_t* __restrict__ dst, int64_t ld_dst) {
+    follow_on();
     const int64_t pieces = ld_dst / 16;
     const uint8_t* const end = src + (rows - 1) * ld + bytes;
     const int64_t piece = (int64_t)blockIdx.x * 32 + threadIdx.x, at = piece * 16;
@@ -1041,19 +1046,10 @@ void launch_tile(const CUtensorMap& a, const CUtensorMap& b, TileParams p, int s
     p.by_group = make_divisor(kGroup * p.tiles_n);
     p.by_last = make_divisor(std::max(1u, (unsigned)p.tiles_m % kGroup));
     const int b_rows = PAIR ? p.bn / 2 : p.bn;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = PAIR ? 2 * (unsigned)std::min<int64_t>(work, sms / 2)
-                       : (unsigned)std::min<int64_t>(work, sms);
-    cfg.blockDim = kThreads;
-    cfg.dynamicSmemBytes =
-        (size_t)p.stages * (kAStage + (size_t)b_rows * kLineBytes) + kFixedSmem<MODE>;
-    cfg.stream = stream;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim = {2, 1, 1};
-    cfg.attrs = at;
-    cfg.numAttrs = PAIR ? 1 : 0;
-    RUNE_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_tile<MODE, T, FP8, PAIR>, a, b, o, o2, p));
+    const unsigned grid = PAIR ? 2 * (unsigned)std::min<int64_t>(work, sms / 2)
+                               : (unsigned)std::min<int64_t>(work, sms);
+    const size_t smem = (size_t)p.stages * (kAStage + (size_t)b_rows * kLineBytes) + kFixedSmem<MODE>;
+    launch(k_tile<MODE, T, FP8, PAIR>, grid, kThreads, smem, PAIR ? 2 : 0, stream, a, b, o, o2, p);
 }
 
 // One product D[m, n] = A B^T: operands, epilogue (in p) and scratch for a split.
@@ -1128,7 +1124,7 @@ void run_mode(const Product& g, TileParams p, Scratch& ws, int device, cudaStrea
         else go(std::false_type());
         const int64_t items = p.m * ((p.n + 3) / 4);
         const int grid = (int)std::min<int64_t>((items + 255) / 256, (int64_t)sms * 16);
-        k_join<MODE, T><<<grid, 256, 0, stream>>>(p, part);
+        launch(k_join<MODE, T>, grid, 256, 0, 0, stream, p, part);
         RUNE_LAUNCH_CHECK();
     }
 }
@@ -1168,7 +1164,7 @@ Matrix readable(Matrix m, int elem_bytes, Scratch& ws, cudaStream_t stream) {
     const int64_t pieces = d.ld * elem_bytes / 16;
     const dim3 grid((unsigned)((pieces + 31) / 32),
                     (unsigned)std::min<int64_t>((m.rows + 7) / 8, 65535));
-    k_pack<<<grid, dim3(32, 8), 0, stream>>>(static_cast<const uint8_t*>(m.p), m.rows,
+    launch(k_pack, grid, dim3(32, 8), 0, 0, stream, static_cast<const uint8_t*>(m.p), m.rows,
                                          m.cols * elem_bytes, m.ld * elem_bytes,
                                          static_cast<uint8_t*>(to), d.ld * elem_bytes);
     RUNE_LAUNCH_CHECK();
@@ -1236,12 +1232,14 @@ void backward(const rune_linear_grad_args& a, Scratch& ws, cudaStream_t stream) 
                 dim3 grid((unsigned)((n_all + kColumns - 1) / kColumns),
                           (unsigned)std::min<int64_t>(strips, 65535));
                 if (half)
-                    k_column_sums<<<grid, 256, 0, stream>>>(
-                        a.rows, n_all, static_cast<const __half*>(a.dy), a.dy_stride, wide_dy, strip,
+                    launch(
+                        k_column_sums<__half>, grid, 256, 0, 0, stream, a.rows, n_all,
+                        static_cast<const __half*>(a.dy), a.dy_stride, wide_dy, strip,
                         sums);
                 else
-                    k_column_sums<<<grid, 256, 0, stream>>>(
-                        a.rows, n_all, static_cast<const __nv_bfloat16*>(a.dy), a.dy_stride, wide_dy,
+                    launch(
+                        k_column_sums<__nv_bfloat16>, grid, 256, 0, 0, stream, a.rows, n_all,
+                        static_cast<const __nv_bfloat16*>(a.dy), a.dy_stride, wide_dy,
                         strip, sums);
                 RUNE_LAUNCH_CHECK();
             }
@@ -1261,12 +1259,12 @@ void backward(const rune_linear_grad_args& a, Scratch& ws, cudaStream_t stream) 
                     auto* dy = static_cast<const T*>(a.dy);
                     auto* out = reinterpret_cast<T*>(to);
                     if (a.gated)
-                        k_act_grad<true, T><<<grid, 256, 0, stream>>>(
-                            a.rows, a.outputs, a.saved, saved_line(a.outputs), dy, a.dy_stride, wide_dy,
+                        launch(
+                            k_act_grad<true, T>, grid, 256, 0, 0, stream, a.rows, a.outputs, a.saved, saved_line(a.outputs), dy, a.dy_stride, wide_dy,
                             out, dz.ld, a.activation, strip, sums);
                     else
-                        k_act_grad<false, T><<<grid, 256, 0, stream>>>(
-                            a.rows, a.outputs, a.saved, saved_line(a.outputs), dy, a.dy_stride, wide_dy,
+                        launch(
+                            k_act_grad<false, T>, grid, 256, 0, 0, stream, a.rows, a.outputs, a.saved, saved_line(a.outputs), dy, a.dy_stride, wide_dy,
                             out, dz.ld, a.activation, strip, sums);
                 };
                 if (half) go(__half());

@@ -83,6 +83,7 @@ k_few(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtenso
     __syncthreads();
     fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
+    follow_on();
 
     if (warp == 4) {
         const bool one = elect_one();
@@ -252,17 +253,8 @@ void launch_few(const CUtensorMap& mw, const CUtensorMap& mx, const FewParams& p
                                            (int)kSmemMax));
         if (device < 64) allowed.fetch_or(uint64_t(1) << device, std::memory_order_relaxed);
     }
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(tiles * splits));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = p.ring_bytes + sizeof(FewShared);
-    cfg.stream = stream;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim = {(unsigned)splits, 1, 1};
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    RUNE_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_few<T, FP8>, mw, mx, p));
+    launch(k_few<T, FP8>, (unsigned)(tiles * splits), kThreads, p.ring_bytes + sizeof(FewShared),
+           splits, stream, mw, mx, p);
 }
 
 }  // namespace

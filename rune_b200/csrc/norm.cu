@@ -181,6 +181,7 @@ __global__ void
 __launch_bounds__(THREADS, ACC == kWhole && sizeof(T) == 2 && BLOCK ? 1536 / THREADS : 1) k_norm(const rune_norm_args p) {
     using P = Piece<T, ACC>;
     constexpr int N = P::N, NC = EPT / N;
+    follow_on();
     __shared__ float2 shared[32];
     const int width = (int)p.width;
     const int t = BLOCK ? threadIdx.x : threadIdx.x & 31, tpr = BLOCK ? blockDim.x : 32;
@@ -259,6 +260,7 @@ __launch_bounds__(THREADS, ACC == kWhole && sizeof(T) == 2 && BLOCK ? 1536 / THR
 // largest magnitude (8 bits only) and again for the output; the repeats come from L2.
 template <typename T, bool Q8>
 __global__ void __launch_bounds__(kLongThreads) k_norm_long(const rune_norm_args p) {
+    follow_on();
     __shared__ float shared[32];
     const bool w32 = p.weight_dtype == RUNE_F32;
     const int t = threadIdx.x;
@@ -321,6 +323,7 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256, BLOCK || ACC != kWhole ? 1
 k_norm_bwd(const rune_norm_grad_args p, float* __restrict__ partials) {
     using P = Piece<T, ACC>;
     constexpr int N = P::N, NC = kEpt / N;
+    follow_on();
     __shared__ float shared[32];
     extern __shared__ __align__(16) unsigned char dynamic[];
     const int width = (int)p.width;
@@ -457,6 +460,7 @@ k_norm_bwd(const rune_norm_grad_args p, float* __restrict__ partials) {
 template <typename T>
 __global__ void __launch_bounds__(kLongThreads)
 k_norm_bwd_long(const rune_norm_grad_args p, float* __restrict__ partials) {
+    follow_on();
     __shared__ float shared[32];
     const bool w32 = p.weight_dtype == RUNE_F32;
     const int t = threadIdx.x;
@@ -497,6 +501,7 @@ k_norm_bwd_long(const rune_norm_grad_args p, float* __restrict__ partials) {
 template <typename T>
 __global__ void __launch_bounds__(1024)
 k_sum_partials(const float* __restrict__ partials, int64_t parts, int64_t width, T* out) {
+    follow_on();
     __shared__ float s[128][9];
     const int64_t col = (int64_t)blockIdx.x * 8 + threadIdx.x;
     float v = 0.0f;
@@ -584,8 +589,8 @@ void launch_norm(const rune_norm_args& a, cudaStream_t stream) {
         const int wide = threads_for(a.width, 2 * kEpt, ACC, N);
         if (wide > 1024) {
             const int grid = (int)std::min<int64_t>(a.rows, 1 << 20);
-            if (q8) k_norm_long<T, true><<<grid, kLongThreads, 0, stream>>>(a);
-            else k_norm_long<T, false><<<grid, kLongThreads, 0, stream>>>(a);
+            if (q8) launch(k_norm_long<T, true>, grid, kLongThreads, 0, 0, stream, a);
+            else launch(k_norm_long<T, false>, grid, kLongThreads, 0, 0, stream, a);
             return;
         }
         auto go = [&](auto ept_c, auto threads_c, auto block_c) {
@@ -594,8 +599,11 @@ void launch_norm(const rune_norm_args& a, cudaStream_t stream) {
             const int threads = BLOCK ? wide : THREADS;
             const int64_t grid = BLOCK ? a.rows : (a.rows + 7) / 8;
             require(grid <= INT32_MAX, "too many rows");
-            if (q8) k_norm<T, ACC, EPT, THREADS, BLOCK, true><<<(int)grid, threads, 0, stream>>>(a);
-            else k_norm<T, ACC, EPT, THREADS, BLOCK, false><<<(int)grid, threads, 0, stream>>>(a);
+            if (q8)
+                launch(k_norm<T, ACC, EPT, THREADS, BLOCK, true>, (int)grid, threads, 0, 0, stream, a);
+            else
+                launch(k_norm<T, ACC, EPT, THREADS, BLOCK, false>, (int)grid, threads, 0, 0, stream,
+                       a);
         };
         using std::integral_constant;
         if (threads_for(a.width, kEpt, ACC, N) == 32)
@@ -632,7 +640,7 @@ int64_t launch_norm_bwd(const rune_norm_grad_args& a, float* partials, cudaStrea
         const int threads = threads_for(a.width, kEpt, ACC, Piece<T, ACC>::N);
         blocks = backward_blocks(a, threads > 1024);
         if (threads > 1024) {
-            k_norm_bwd_long<T><<<(int)blocks, kLongThreads, 0, stream>>>(a, partials);
+            launch(k_norm_bwd_long<T>, (int)blocks, kLongThreads, 0, 0, stream, a, partials);
         } else {
             const bool block = a.width > kWarpMax || threads > 32;
             const int n = block ? threads : 256;
@@ -642,7 +650,7 @@ int64_t launch_norm_bwd(const rune_norm_grad_args& a, float* partials, cudaStrea
                 if (smem > 48 * 1024)
                     RUNE_CUDA_TRY(cudaFuncSetAttribute(
                         kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-                kernel<<<(int)blocks, n, smem, stream>>>(a, partials);
+                launch(kernel, (int)blocks, n, smem, 0, stream, a, partials);
             };
             if constexpr (ACC == kWhole) {
                 // at most half an SM's shared memory, so that two blocks overlap
@@ -683,11 +691,13 @@ void sum_partials(const float* partials, int64_t parts, int64_t width, void* out
     dim3 block(8, 128);
     int grid = (int)((width + 7) / 8);
     if (dtype == RUNE_F32)
-        k_sum_partials<<<grid, block, 0, stream>>>(partials, parts, width, (float*)out);
+        launch(k_sum_partials<float>, grid, block, 0, 0, stream, partials, parts, width, (float*)out);
     else if (dtype == RUNE_F16)
-        k_sum_partials<<<grid, block, 0, stream>>>(partials, parts, width, (__half*)out);
+        launch(k_sum_partials<__half>, grid, block, 0, 0, stream, partials, parts, width,
+               (__half*)out);
     else
-        k_sum_partials<<<grid, block, 0, stream>>>(partials, parts, width, (__nv_bfloat16*)out);
+        launch(k_sum_partials<__nv_bfloat16>, grid, block, 0, 0, stream, partials, parts, width,
+               (__nv_bfloat16*)out);
     RUNE_LAUNCH_CHECK();
 }
 

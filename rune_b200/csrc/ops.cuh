@@ -57,9 +57,41 @@ inline bool aligned(const void* p, size_t bytes) { return (uintptr_t)p % bytes =
 
 int sm_count(int device);
 
+// Launches an operator's kernel so that it may begin while the one before it in the stream ends
+// (programmatic dependent launch): its prologue and the launch itself are hidden, and follow_on()
+// in the kernel holds back everything that touches memory. cluster: blocks of one, or 0.
+template <typename... Params, typename... Args>
+void launch(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, int cluster,
+            cudaStream_t stream, Args&&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim = {(unsigned)cluster, 1, 1};
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 0 ? 2 : 1;
+    RUNE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
+}
+
 // Sums the float32 partials [parts][width] over parts into out[width] of type dtype.
 void sum_partials(const float* partials, int64_t parts, int64_t width, void* out, int dtype,
                   cudaStream_t stream);
+
+// ----------------------------------------------------------------------------- launches
+// Every thread calls it before its first access to global memory and, in kernels that hold TMEM,
+// after the block has its TMEM: waits until the kernel before in the stream is complete and its
+// writes are visible, and lets the next one begin its own prologue. A kernel whose blocks wait
+// here needs nothing of the next one, and all its blocks are resident by then, so the next one's
+// waiting for shared memory or TMEM ends.
+__device__ __forceinline__ void follow_on() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
 
 // ----------------------------------------------------------------------------- typed access
 __device__ __forceinline__ float to_float(float v) { return v; }
