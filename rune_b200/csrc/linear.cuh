@@ -155,6 +155,13 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
         : "memory");
 }
 
+// the same tile as far as L2
+__device__ __forceinline__ void prefetch_tile(const CUtensorMap* map, int x, int y) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];"
+                 ::"l"(map), "r"(x), "r"(y)
+                 : "memory");
+}
+
 // one lane of a converged warp
 __device__ __forceinline__ bool elect_one() {
     uint32_t r;

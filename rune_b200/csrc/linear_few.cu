@@ -19,8 +19,12 @@ namespace ops {
 namespace {
 
 constexpr int kThreads = 192;
+constexpr int kPrefetchWarp = 4;  // the TMA warp
 constexpr int kFeatures = 128;
-constexpr uint32_t kWStage = kFeatures * kLineBytes;  // 16 KB
+constexpr uint32_t kWLine = kFeatures * kLineBytes;  // 16 KB
+// 128-byte lines of k in a stage: the loop over stages costs some 0.3 us a turn, which the four
+// small products of one line do not fill (1 x 8192 -> 1024 with one line 8.5 us)
+constexpr int kLines = 2;
 constexpr int kMaxStages = 12;
 constexpr uint32_t kRingBytes = 108 * 1024;           // two blocks an SM
 constexpr uint32_t kSmemMax = kRingBytes + 1024;
@@ -28,7 +32,8 @@ constexpr uint32_t kSmemMax = kRingBytes + 1024;
 struct FewParams {
     int rows, rows_pad;      // rows of x, and rounded up to the tensor core's 16
     int64_t n;               // outputs
-    int kblocks, stages, act, gated;
+    int kblocks;             // stages of k
+    int stages, act, gated;
     uint32_t idesc, tmem_cols, ring_bytes;
     int64_t ld_res;
     const void* bias;
@@ -55,7 +60,9 @@ k_few(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtenso
     extern __shared__ __align__(1024) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-    const uint32_t stage_bytes = kWStage + (uint32_t)p.rows_pad * kLineBytes;
+    constexpr int kLine = FP8 ? 128 : 64;  // values
+    const uint32_t x_line = (uint32_t)p.rows_pad * kLineBytes;
+    const uint32_t stage_bytes = kLines * (kWLine + x_line);
     FewShared& sh = *reinterpret_cast<FewShared*>(smem + p.ring_bytes);
     const uint32_t splits = cluster_size(), rank = cluster_rank();
     const int width = p.gated ? kFeatures / 2 : kFeatures;  // features of y in this tile
@@ -83,6 +90,17 @@ k_few(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtenso
     __syncthreads();
     fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
+    if (warp == kPrefetchWarp && kb1 - kb0 > p.stages) {
+        // the first weights on their way to L2, where a write by the kernel before would still be
+        // seen, while that kernel ends (5 x 4096 -> 2 x 8192 25.0 -> 24.4 us); not where the ring
+        // takes them all at once (1 x 1024 -> 1024 4.1 -> 4.4)
+        const int kb = kb0 * kLines + lane;
+        if (lane < p.stages * kLines && kb < kb1 * kLines) {
+            prefetch_tile(&map_w, kb * kLine, (int)f0);
+            if (p.gated) prefetch_tile(&map_w, kb * kLine, (int)(p.n + f0));
+        }
+        __syncwarp();
+    }
     follow_on();
 
     if (warp == 4) {
@@ -98,13 +116,16 @@ k_few(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtenso
             }
             const uint32_t bar = smem_u32(&sh.full[st]);
             const uint32_t a = smem_u32(smem) + (uint32_t)st * stage_bytes;
-            const int x = kb * (FP8 ? 128 : 64);
             if (one) {
                 mbar_expect_tx(bar, stage_bytes);
-                tma_load(a, &map_w, x, (int)f0, bar);
-                if (p.gated)
-                    tma_load(a + kWStage / 2, &map_w, x, (int)(p.n + f0), bar);
-                tma_load(a + kWStage, &map_x, x, 0, bar);
+#pragma unroll
+                for (int l = 0; l < kLines; ++l) {
+                    const int x = (kb * kLines + l) * kLine;
+                    tma_load(a + l * kWLine, &map_w, x, (int)f0, bar);
+                    if (p.gated)
+                        tma_load(a + l * kWLine + kWLine / 2, &map_w, x, (int)(p.n + f0), bar);
+                    tma_load(a + kLines * kWLine + l * x_line, &map_x, x, 0, bar);
+                }
             }
             __syncwarp();  // the other lanes' polling must not hold up the copies' issue
             ++issued;
@@ -115,7 +136,7 @@ k_few(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtenso
     } else if (warp == 5) {
         const bool one = elect_one();
         const uint64_t desc_w = operand_desc(smem_u32(smem), false);
-        const uint64_t desc_x = operand_desc(smem_u32(smem) + kWStage, false);
+        const uint64_t desc_x = operand_desc(smem_u32(smem) + kLines * kWLine, false);
         int st = 0;
         uint32_t parity = 0;
         bool ok = true;
@@ -129,10 +150,12 @@ k_few(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtenso
             const uint64_t at = (uint64_t)((uint32_t)st * (stage_bytes >> 4));
             if (one) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const bool more = kb > kb0 || k > 0;
-                    mma<FP8, false>(tmem, desc_w + at + 2 * k, desc_x + at + 2 * k, p.idesc, more);
-                }
+                for (int l = 0; l < kLines; ++l)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        mma<FP8, false>(tmem, desc_w + at + l * (kWLine >> 4) + 2 * k,
+                                        desc_x + at + l * (x_line >> 4) + 2 * k, p.idesc,
+                                        kb > kb0 || l > 0 || k > 0);
                 mma_commit(smem_u32(&sh.empty[st]));
             }
             __syncwarp();
@@ -262,7 +285,7 @@ void launch_few(const CUtensorMap& mw, const CUtensorMap& mx, const FewParams& p
 // The layer of `a` with operands x and w that TMA can read; a.rows at most kFewRows.
 void linear_few(const rune_linear_args& a, const Matrix& x, const Matrix& w, cudaStream_t stream) {
     const bool fp8 = a.dtype == RUNE_E4M3;
-    const int eb = fp8 ? 1 : 2, line = (int)kLineBytes / eb, sms = sm_count(a.device);
+    const int eb = fp8 ? 1 : 2, line = kLines * (int)kLineBytes / eb, sms = sm_count(a.device);
     FewParams p{};
     p.rows = (int)a.rows;
     p.rows_pad = (p.rows + 15) / 16 * 16;
@@ -272,12 +295,11 @@ void linear_few(const rune_linear_args& a, const Matrix& x, const Matrix& w, cud
     p.kblocks = (int)((a.inputs + line - 1) / line);
     const int width = a.gated ? kFeatures / 2 : kFeatures;
     const int64_t tiles = (a.outputs + width - 1) / width;
-    // as many blocks as two an SM, with kMinBlocks k-blocks each at least
-    constexpr int kMinBlocks = 2;
+    // as many blocks as two an SM, with a stage of k each at least
     int splits = 1;
-    while (splits < 8 && tiles * splits * 2 <= 2 * sms && p.kblocks / (splits * 2) >= kMinBlocks)
+    while (splits < 8 && tiles * splits * 2 <= 2 * sms && p.kblocks >= splits * 2)
         splits *= 2;
-    const uint32_t stage = kWStage + (uint32_t)p.rows_pad * kLineBytes;
+    const uint32_t stage = kLines * (kWLine + (uint32_t)p.rows_pad * kLineBytes);
     p.stages = (int)std::min<uint32_t>(kMaxStages, kRingBytes / stage);
     p.ring_bytes = std::max(p.stages * stage, p.rows_pad * kFeatures * (uint32_t)sizeof(float));
     p.tmem_cols = p.rows_pad <= 32 ? 32 : p.rows_pad <= 64 ? 64 : 128;
