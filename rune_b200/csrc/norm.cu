@@ -5,8 +5,8 @@
 //
 // A row stays in registers between the sum of its squares and its output, so every value is read
 // once and written once: memory bandwidth bounds the kernels, launch latency the shortest calls.
-// A warp takes a row of up to kWarpMax values, a block of width / 8 or / 16 threads one of up
-// to kBlockMax or twice that; longer rows are read twice (the second time from L2).
+// A warp takes a row of up to 256 values (forward 512), a block of width / 8 threads (forward
+// width / 16) one of up to 8192 (16384); longer rows are read twice, the second time from L2.
 //
 // Accesses are 16 bytes. Rows whose width or stride leaves them off 16 bytes, but all arrays by
 // the same amount (contiguous arrays of an odd width), are taken from the 16-byte boundary before
@@ -24,8 +24,6 @@ namespace ops {
 namespace {
 
 constexpr int kEpt = 8;              // values of a row per thread (forward, block: twice that)
-constexpr int kWarpMax = 32 * kEpt;  // 256
-constexpr int kBlockMax = 1024 * kEpt;      // backward; forward twice that
 constexpr int kLongThreads = 1024;
 
 enum Access { kWhole, kShifted, kSingle };
@@ -256,7 +254,7 @@ __launch_bounds__(THREADS, ACC == kWhole && sizeof(T) == 2 && BLOCK ? 1536 / THR
     }
 }
 
-// Rows longer than kBlockMax: a block reads the row for the sum (writing h), again for the
+// Rows longer than a block's registers: a block reads the row for the sum (writing h), again for the
 // largest magnitude (8 bits only) and again for the output; the repeats come from L2.
 template <typename T, bool Q8>
 __global__ void __launch_bounds__(kLongThreads) k_norm_long(const rune_norm_args p) {
@@ -455,7 +453,7 @@ k_norm_bwd(const rune_norm_grad_args p, float* __restrict__ partials) {
     }
 }
 
-// Rows longer than kBlockMax: the row is read twice and the block's partials are accumulated in
+// Rows longer than a block's registers: the row is read twice and the block's partials are accumulated in
 // its own row of the workspace (each column always by the same thread).
 template <typename T>
 __global__ void __launch_bounds__(kLongThreads)
@@ -530,18 +528,19 @@ int threads_for(int64_t width, int ept, Access acc, int n) {
     return (int)((need + ept * 32 - 1) / (ept * 32)) * 32;
 }
 
-// Blocks of the backward: enough to fill the GPU; each leaves one row of partials. A multiple of
-// eight, except where a row is read twice (every block has a row there).
-int64_t backward_blocks(const rune_norm_grad_args& a, bool twice) {
+// Blocks of the backward: as many as are resident at once (a second wave would double the time:
+// 373248 x 256 with four blocks too many 317 against 282 us), each leaving one row of partials. A
+// multiple of eight, except where a row is read twice (every block has a row there). kWarpBlocks
+// and kBlockThreads an SM are what registers and slots allow, kWarpBlocks - 1 without slots.
+constexpr int kWarpBlocks = 3, kBlockThreads = 1024;
+
+int64_t backward_blocks(const rune_norm_grad_args& a, Access acc, int threads) {
     const int64_t sms = sm_count(a.device);
-    if (twice) return std::min(a.rows, sms * 2);
-    int64_t most = std::max<int64_t>(8, sms * 3), rows = (a.rows + 7) / 8;
-    if (a.width > kWarpMax) {
-        most = std::max<int64_t>(
-            8, sms * std::max<int64_t>(1, 1024 / threads_for(a.width, kEpt, kSingle, 1)));
-        rows = a.rows;
-    }
-    return rows < most ? (rows + 7) / 8 * 8 : most / 8 * 8;  // never a second wave
+    if (threads > 1024) return std::min(a.rows, sms * 2);
+    int64_t most = sms * (acc == kWhole ? kWarpBlocks : kWarpBlocks - 1), rows = (a.rows + 7) / 8;
+    if (threads > 32) most = sms * std::max(1, kBlockThreads / threads), rows = a.rows;
+    most = std::max<int64_t>(8, most);
+    return rows < most ? (rows + 7) / 8 * 8 : most / 8 * 8;
 }
 
 // Arrays of type-`es` rows: how all of them can be accessed.
@@ -638,12 +637,14 @@ int64_t launch_norm_bwd(const rune_norm_grad_args& a, float* partials, cudaStrea
     with_access(l.access(), [&](auto acc_c) {
         constexpr Access ACC = decltype(acc_c)::value;
         const int threads = threads_for(a.width, kEpt, ACC, Piece<T, ACC>::N);
-        blocks = backward_blocks(a, threads > 1024);
+        blocks = backward_blocks(a, ACC, threads);
         if (threads > 1024) {
             launch(k_norm_bwd_long<T>, (int)blocks, kLongThreads, 0, 0, stream, a, partials);
         } else {
-            const bool block = a.width > kWarpMax || threads > 32;
+            const bool block = threads > 32;
             const int n = block ? threads : 256;
+            // rows ahead: kBlockThreads threads' slots have to fit an SM
+            constexpr int kAheadBlock = sizeof(T) == 2 ? 3 : 1;
             auto go = [&](auto kernel, int ahead) {
                 const size_t smem =
                     std::max(ahead * slots_bytes<T>(n), block ? 0 : 8 * a.width * sizeof(float));
@@ -653,14 +654,11 @@ int64_t launch_norm_bwd(const rune_norm_grad_args& a, float* partials, cudaStrea
                 launch(kernel, (int)blocks, n, smem, 0, stream, a, partials);
             };
             if constexpr (ACC == kWhole) {
-                // at most half an SM's shared memory, so that two blocks overlap
-                if (!block) go(k_norm_bwd<T, ACC, false, 4>, 4);
-                else if (4 * slots_bytes<T>(n) <= 110 * 1024) go(k_norm_bwd<T, ACC, true, 4>, 4);
-                else if (2 * slots_bytes<T>(n) <= 130 * 1024) go(k_norm_bwd<T, ACC, true, 2>, 2);
-                else go(k_norm_bwd<T, ACC, true, 1>, 1);
+                if (block) go(k_norm_bwd<T, ACC, true, kAheadBlock>, kAheadBlock);
+                else go(k_norm_bwd<T, ACC, false, sizeof(T) == 2 ? 4 : 2>, sizeof(T) == 2 ? 4 : 2);
             } else {
-                if (!block) go(k_norm_bwd<T, ACC, false, 0>, 0);
-                else go(k_norm_bwd<T, ACC, true, 0>, 0);
+                if (block) go(k_norm_bwd<T, ACC, true, 0>, 0);
+                else go(k_norm_bwd<T, ACC, false, 0>, 0);
             }
         }
     });
@@ -669,7 +667,11 @@ int64_t launch_norm_bwd(const rune_norm_grad_args& a, float* partials, cudaStrea
 
 int64_t norm_grad_workspace(const rune_norm_grad_args& a) {
     if (!a.dweight || a.rows <= 0) return 0;
-    const int64_t blocks = std::max(backward_blocks(a, true), backward_blocks(a, false));
+    // enough for every way that the arrays can lie
+    int64_t blocks = 0;
+    for (Access acc : {kWhole, kShifted, kSingle})
+        for (int n : {1, 4, 8})
+            blocks = std::max(blocks, backward_blocks(a, acc, threads_for(a.width, kEpt, acc, n)));
     return blocks * a.width * (int64_t)sizeof(float);
 }
 
