@@ -33,8 +33,10 @@ _OUT = {None: -1, torch.float16: L.RUNE_F16, torch.bfloat16: L.RUNE_BF16}
 
 # Largest input width at which the backward pass of an activated layer recomputes z = x W^T + b
 # instead of reading a float32 copy that the forward saved. Per value of z the copy costs 8 bytes
-# of traffic, the product 2 * inputs operations.
-RECOMPUTE_INPUTS = 512
+# of traffic and its memory, the product 2 * inputs operations. B200, training step of 32768 rows
+# and 1024 outputs, recomputed / saved: 512 inputs 177 / 191 us (gated 257 / 323), 1024 inputs
+# 248 / 243 (424 / 432), 2048 inputs 428 / 379 (770 / 682).
+RECOMPUTE_INPUTS = 1024
 
 _BINDING = None
 
