@@ -329,6 +329,12 @@ typedef struct {
 int rune_rms_norm_backward(const rune_norm_grad_args* args, void* stream);
 int rune_rms_norm_backward_workspace(const rune_norm_grad_args* args, int64_t* bytes);
 
+/* Copies `rows` lines of `bytes` bytes, `stride` bytes apart, to lines `padded_stride` bytes apart
+ * (a multiple of 16, at least `bytes`; `dst` 16-byte aligned): the layout in which the linear calls
+ * read operands in place. The padding is written with whatever; nothing reads it. */
+int rune_pad_rows(int32_t device, int64_t rows, int64_t bytes, int64_t stride, const void* src,
+                  int64_t padded_stride, void* dst, void* stream);
+
 typedef struct {
     int64_t rows, inputs, outputs;
     int64_t x_stride, weight_stride, residual_stride;

@@ -1149,6 +1149,14 @@ int64_t pad16(int64_t cols, int elem_bytes) {
     return (cols + v - 1) / v * v;
 }
 
+void pad_rows(const void* src, int64_t rows, int64_t bytes, int64_t ld, void* dst, int64_t ld_dst,
+              cudaStream_t stream) {
+    const dim3 grid((unsigned)((ld_dst / 16 + 31) / 32),
+                    (unsigned)std::min<int64_t>((rows + 7) / 8, 65535));
+    launch(k_pack, grid, dim3(32, 8), 0, 0, stream, static_cast<const uint8_t*>(src), rows, bytes,
+           ld, static_cast<uint8_t*>(dst), ld_dst);
+}
+
 // the operand itself, or its padded copy in the scratch
 Matrix readable(Matrix m, int elem_bytes, Scratch& ws, cudaStream_t stream) {
     if (m.rows == 1) m.ld = pad16(m.cols, elem_bytes);  // no second line to reach
@@ -1161,13 +1169,7 @@ Matrix readable(Matrix m, int elem_bytes, Scratch& ws, cudaStream_t stream) {
         d.p = reinterpret_cast<const void*>(256);  // any aligned address: only sizes are asked
         return d;
     }
-    const int64_t pieces = d.ld * elem_bytes / 16;
-    const dim3 grid((unsigned)((pieces + 31) / 32),
-                    (unsigned)std::min<int64_t>((m.rows + 7) / 8, 65535));
-    launch(k_pack, grid, dim3(32, 8), 0, 0, stream, static_cast<const uint8_t*>(m.p), m.rows,
-                                         m.cols * elem_bytes, m.ld * elem_bytes,
-                                         static_cast<uint8_t*>(to), d.ld * elem_bytes);
-    RUNE_LAUNCH_CHECK();
+    pad_rows(m.p, m.rows, m.cols * elem_bytes, m.ld * elem_bytes, to, d.ld * elem_bytes, stream);
     return d;
 }
 
@@ -1461,6 +1463,18 @@ using namespace rune;
 using namespace rune::ops;
 
 extern "C" {
+
+int rune_pad_rows(int32_t device, int64_t rows, int64_t bytes, int64_t stride, const void* src,
+                  int64_t padded_stride, void* dst, void* stream) {
+    return guarded(device, [&] {
+        require(rows >= 0 && bytes >= 1 && padded_stride >= bytes && padded_stride % 16 == 0 &&
+                    padded_stride / 16 <= INT32_MAX,
+                "rows, bytes or padded_stride out of range");
+        if (rows == 0) return;
+        require(src && dst && aligned(dst, 16), "null argument, or dst not 16-byte aligned");
+        pad_rows(src, rows, bytes, stride, dst, padded_stride, static_cast<cudaStream_t>(stream));
+    });
+}
 
 int rune_linear_workspace(const rune_linear_args* args, int64_t* bytes) {
     if (!args || !bytes) {

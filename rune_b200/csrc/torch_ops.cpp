@@ -34,6 +34,7 @@ struct Api {
     decltype(&rune_linear_workspace) linear_ws;
     decltype(&rune_linear_backward) linear_bwd;
     decltype(&rune_linear_backward_workspace) linear_bwd_ws;
+    decltype(&rune_pad_rows) pad_rows;
     decltype(&rune_last_error) last_error;
 } api;
 PyObject* g_raise = nullptr;        // runtime.library.check's exceptions by status
@@ -221,6 +222,26 @@ void check_norm(const Tensor& x, Tensor& weight, const Tensor& residual) {
 }
 
 // ---------------------------------------------------------------------------------- linear
+// A copy of the rows of t that start on 16 bytes each: a view of a padded buffer.
+Tensor padded(const Tensor& t) {
+    const Rows r(t);
+    const int64_t width = t.size(-1), eb = t.element_size();
+    const int64_t line = (width * eb + 15) / 16 * 16;
+    Tensor buffer = empty_like_type(t, {r.n, line / eb}, t.scalar_type());
+    check(api.pad_rows(t.get_device(), r.n, width * eb, r.ld * eb, r.p(), line, ptr(buffer),
+                       stream_of(t)));
+    return buffer.narrow(1, 0, width);
+}
+
+// t, or its padded copy where the products could not read it in place (for both passes at once)
+Tensor in_place(const Tensor& t) {
+    if (t.dim() != 2 || t.stride(1) != 1 || t.size(0) < 2) return t;
+    const int64_t eb = t.element_size();
+    const bool ready = t.stride(0) * eb % 16 == 0 && t.stride(0) >= t.size(1) &&
+                       reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+    return ready ? t : padded(t);
+}
+
 struct LinearOut {
     Tensor y, z;
 };
@@ -255,12 +276,13 @@ LinearOut linear_call(const Tensor& x, const Tensor& weight, const Tensor& bias,
 }
 
 struct LinearFn : torch::autograd::Function<LinearFn> {
-    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight,
+    static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& weight_,
                           const std::optional<Tensor>& bias_,
                           const std::optional<Tensor>& residual, int64_t act, bool gated) {
         const Tensor bias = bias_.value_or(Tensor());
-        const bool save = act != RUNE_ACT_NONE && x.size(-1) > g_recompute_inputs &&
-                          (wants_grad(x) || wants_grad(weight) || wants_grad(bias));
+        const bool again = wants_grad(x_) || wants_grad(weight_) || wants_grad(bias);
+        const bool save = act != RUNE_ACT_NONE && x_.size(-1) > g_recompute_inputs && again;
+        const Tensor x = again ? in_place(x_) : x_, weight = again ? in_place(weight_) : weight_;
         LinearOut o = linear_call(x, weight, bias, residual.value_or(Tensor()), Tensor(), Tensor(),
                                   act, gated, x.scalar_type(), save);
         ctx->save_for_backward({x, weight, bias, o.z});
@@ -437,6 +459,19 @@ PyObject* py_to_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
+// padded(t): a copy of its rows, padded to 16 bytes each
+PyObject* py_padded(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (!count_is(n, 1)) return nullptr;
+    return guarded([&] {
+        const Tensor t = tensor_arg(args[0], "t");
+        if (!t.defined() || !t.is_cuda()) bad("t must be a CUDA tensor; there is no CPU path.");
+        if (t.dim() != 2 || t.size(1) == 0) bad("t needs two axes, the last one not empty.");
+        if (at::GradMode::is_enabled() && t.requires_grad())
+            bad("a padded copy has no gradient; call under torch.no_grad().");
+        return THPVariable_Wrap(padded(t));
+    });
+}
+
 // layer(x, weight, bias, residual, x_scale, weight_scale, activation, gated, out code): y
 PyObject* py_layer(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!count_is(n, 9)) return nullptr;
@@ -483,6 +518,7 @@ PyMethodDef methods[] = {
     {"bind", py_bind, METH_VARARGS, "Take the library's entry points."},
     {"rms_norm", reinterpret_cast<PyCFunction>(py_rms_norm), METH_FASTCALL, nullptr},
     {"to_fp8", reinterpret_cast<PyCFunction>(py_to_fp8), METH_FASTCALL, nullptr},
+    {"padded", reinterpret_cast<PyCFunction>(py_padded), METH_FASTCALL, nullptr},
     {"layer", reinterpret_cast<PyCFunction>(py_layer), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ops", nullptr, -1, methods};

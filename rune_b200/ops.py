@@ -7,6 +7,7 @@ CUDA tensors, for training, distilling or serving networks beside the engine's f
   second leaves its rows in 8 bits (e4m3) with a scale per row.
 * ``linear``: ``act(x W^T + b) + residual`` in one kernel; 16-bit operands, or e4m3 with scales.
 * ``gated_linear``: ``act(x Wg^T + bg) * (x Wu^T + bu)`` in one kernel.
+* ``padded``: a copy of a matrix whose rows start on 16 bytes each, for weights of odd widths.
 * ``quantize_fp8``: rows to e4m3 with a scale per row (weights once, activations per call).
 
 Every function works on the last axis of its input, takes row-strided views, runs on the current
@@ -26,7 +27,7 @@ import torch
 from .runtime import library as L
 from .runtime.build import BINDING
 
-__all__ = ["gated_linear", "linear", "quantize_fp8", "rms_norm", "rms_norm_fp8"]
+__all__ = ["gated_linear", "linear", "padded", "quantize_fp8", "rms_norm", "rms_norm_fp8"]
 
 _ACTS = {None: L.RUNE_ACT_NONE, **L.RUNE_ACT}
 _OUT = {None: -1, torch.float16: L.RUNE_F16, torch.bfloat16: L.RUNE_BF16}
@@ -56,7 +57,7 @@ def _native():
         entries = (lib.rune_rms_norm, lib.rune_rms_norm_backward,
                    lib.rune_rms_norm_backward_workspace, lib.rune_linear,
                    lib.rune_linear_workspace, lib.rune_linear_backward,
-                   lib.rune_linear_backward_workspace, lib.rune_last_error)
+                   lib.rune_linear_backward_workspace, lib.rune_pad_rows, lib.rune_last_error)
         module.bind(tuple(ctypes.cast(f, ctypes.c_void_p).value for f in entries), L.fail,
                     RECOMPUTE_INPUTS)
         _BINDING = module
@@ -107,6 +108,16 @@ def quantize_fp8(x):
     ``rms_norm_fp8`` precedes. Not differentiable.
     """
     return (_BINDING or _native()).to_fp8(x, None, None, 0.0)
+
+
+def padded(t):
+    """A copy of the matrix t as a view of a buffer whose rows start on 16 bytes each.
+
+    ``linear`` and ``gated_linear`` read such operands in place; others they copy in every call,
+    which with few rows of x takes longer than the product. For weights of widths that are no
+    multiple of 8 (e4m3: 16), once. Not differentiable.
+    """
+    return (_BINDING or _native()).padded(t)
 
 
 def linear(x, weight, bias=None, activation=None, residual=None, *, x_scale=None,

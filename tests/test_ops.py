@@ -558,6 +558,22 @@ def test_offsets_beyond_32_bits():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [*NARROW, torch.float8_e4m3fn], ids=str)
+@pytest.mark.parametrize("rows,width", [(1, 1), (3, 7), (65, 513), (70, 24), (2000, 130)])
+def test_padded_rows_are_copies_on_16_bytes(rows, width, dtype):
+    base = normal(85, rows, width + 5, dtype=torch.float32).to(dtype)
+    for t in (base, base[:, 3:3 + width], base[:, 1:1 + width]):
+        p = ops.padded(t)
+        raw, want = p.view(torch.uint8), t.contiguous().view(torch.uint8)
+        assert p.shape == t.shape and torch.equal(raw, want)
+        assert p.data_ptr() % 16 == 0 and p.stride(0) * p.element_size() % 16 == 0
+    if dtype is not torch.float8_e4m3fn:
+        x = normal(86, 9, width, dtype=dtype)
+        w = base[:, 3:3 + width]
+        assert torch.equal(ops.linear(x, w), ops.linear(x, ops.padded(w)))
+
+
+@gpu
 def test_refusals():
     x, w = normal(91, 4, 16), normal(92, 8, 16)
     f32 = x.float()
@@ -582,6 +598,7 @@ def test_refusals():
         (lambda: ops.rms_norm(x, w[0], residual=x.half()), "residual must be"),
         (lambda: ops.rms_norm_fp8(x.requires_grad_(True), w[0]), "no gradient"),
         (lambda: ops.quantize_fp8(x[:, :0].detach()), "cannot be empty"),
+        (lambda: ops.padded(w[0]), "two axes"),
     ]
     for call, message in cases:
         with pytest.raises(ValueError, match=message):
