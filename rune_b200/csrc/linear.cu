@@ -1229,7 +1229,7 @@ void backward(const rune_linear_grad_args& a, Scratch& ws, cudaStream_t stream) 
         if (want_dz) dz = readable(dz, 2, ws, stream);
         if (a.dbias) {
             parts = strips;
-            sums = ws.take<float>(parts * n_all);
+            sums = ws.take<float>(((parts + 7) / 8 * 8 + partial_scratch(parts)) * n_all);
             if (!ws.sizing()) {
                 dim3 grid((unsigned)((n_all + kColumns - 1) / kColumns),
                           (unsigned)std::min<int64_t>(strips, 65535));
@@ -1252,7 +1252,7 @@ void backward(const rune_linear_grad_args& a, Scratch& ws, cudaStream_t stream) 
         dz.p = to;
         if (a.saved) {
             parts = strips;
-            if (a.dbias) sums = ws.take<float>(parts * n_all);
+            if (a.dbias) sums = ws.take<float>(((parts + 7) / 8 * 8 + partial_scratch(parts)) * n_all);
             if (!ws.sizing()) {
                 dim3 grid((unsigned)((a.outputs + kColumns - 1) / kColumns),
                           (unsigned)std::min<int64_t>(strips, 65535));
@@ -1275,7 +1275,8 @@ void backward(const rune_linear_grad_args& a, Scratch& ws, cudaStream_t stream) 
             }
         } else {
             parts = (a.rows + 31) / 32;  // one a warp; the last tile (of a pair) has more warps
-            if (a.dbias) sums = ws.take<float>((parts + 7) / 8 * 8 * n_all);
+            if (a.dbias)
+                sums = ws.take<float>(((parts + 7) / 8 * 8 + partial_scratch(parts)) * n_all);
             Product g;
             g.a = x, g.b = w;
             g.mode = a.gated ? kGatedGrad : kGrad;
@@ -1296,7 +1297,8 @@ void backward(const rune_linear_grad_args& a, Scratch& ws, cudaStream_t stream) 
         if (ws.sizing()) dz.p = reinterpret_cast<const void*>(256);
     }
     if (a.dbias && !ws.sizing())
-        sum_partials(sums, parts, n_all, a.dbias, a.dtype, stream);
+        sum_partials(sums, parts, n_all, a.dbias, a.dtype, sums + (parts + 7) / 8 * 8 * n_all,
+                     stream);
     if (a.dx) {
         Product g;
         g.a = dz, g.b = w;

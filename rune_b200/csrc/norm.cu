@@ -494,30 +494,34 @@ k_norm_bwd_long(const rune_norm_grad_args p, float* __restrict__ partials) {
     }
 }
 
-// Columns of float32 partials [parts][width]: a block sums 8 columns with 128 threads each, then
-// joins their sums in order.
+// Columns of float32 partials [parts][width]: a block sums 32 columns of kPartRows parts with 32
+// threads each, then joins their sums in order; block row y writes row y of out.
+constexpr int kPartRows = 512;
+
 template <typename T>
 __global__ void __launch_bounds__(1024)
 k_sum_partials(const float* __restrict__ partials, int64_t parts, int64_t width, T* out) {
     follow_on();
-    __shared__ float s[128][9];
-    const int64_t col = (int64_t)blockIdx.x * 8 + threadIdx.x;
+    __shared__ float s[32][33];
+    const int64_t col = (int64_t)blockIdx.x * 32 + threadIdx.x;
+    const int64_t end = min(parts, ((int64_t)blockIdx.y + 1) * kPartRows);
     float v = 0.0f;
     if (col < width) {
-#pragma unroll 16
-        for (int64_t r = threadIdx.y; r < parts; r += 128) v += partials[r * width + col];
+#pragma unroll 8
+        for (int64_t r = (int64_t)blockIdx.y * kPartRows + threadIdx.y; r < end; r += 32)
+            v += partials[r * width + col];
     }
     s[threadIdx.y][threadIdx.x] = v;
     __syncthreads();
-    if (threadIdx.y < 16) {
-        for (int k = threadIdx.y + 16; k < 128; k += 16) v += s[k][threadIdx.x];
+    if (threadIdx.y < 8) {
+        for (int k = threadIdx.y + 8; k < 32; k += 8) v += s[k][threadIdx.x];
         s[threadIdx.y][threadIdx.x] = v;
     }
     __syncthreads();
     if (threadIdx.y == 0 && col < width) {
         float sum = 0.0f;
-        for (int k = 0; k < 16; ++k) sum += s[k][threadIdx.x];
-        out[col] = from_float<T>(sum);
+        for (int k = 0; k < 8; ++k) sum += s[k][threadIdx.x];
+        out[blockIdx.y * width + col] = from_float<T>(sum);
     }
 }
 
@@ -672,7 +676,7 @@ int64_t norm_grad_workspace(const rune_norm_grad_args& a) {
     for (Access acc : {kWhole, kShifted, kSingle})
         for (int n : {1, 4, 8})
             blocks = std::max(blocks, backward_blocks(a, acc, threads_for(a.width, kEpt, acc, n)));
-    return blocks * a.width * (int64_t)sizeof(float);
+    return (blocks + partial_scratch(blocks)) * a.width * (int64_t)sizeof(float);
 }
 
 }  // namespace
@@ -688,10 +692,24 @@ int sm_count(int device) {
     return n;
 }
 
+int64_t partial_scratch(int64_t parts) {
+    int64_t rows = 0;
+    while (parts > kPartRows) rows += parts = (parts + kPartRows - 1) / kPartRows;
+    return rows;
+}
+
 void sum_partials(const float* partials, int64_t parts, int64_t width, void* out, int dtype,
-                  cudaStream_t stream) {
-    dim3 block(8, 128);
-    int grid = (int)((width + 7) / 8);
+                  float* scratch, cudaStream_t stream) {
+    const dim3 block(32, 32);
+    dim3 grid((unsigned)((width + 31) / 32));
+    while (parts > kPartRows) {
+        const int64_t sets = (parts + kPartRows - 1) / kPartRows;
+        require(sets <= 65535, "too many rows");
+        grid.y = (unsigned)sets;
+        launch(k_sum_partials<float>, grid, block, 0, 0, stream, partials, parts, width, scratch);
+        partials = scratch, parts = sets, grid.y = 1;
+        scratch += sets * width;
+    }
     if (dtype == RUNE_F32)
         launch(k_sum_partials<float>, grid, block, 0, 0, stream, partials, parts, width, (float*)out);
     else if (dtype == RUNE_F16)
@@ -700,7 +718,6 @@ void sum_partials(const float* partials, int64_t parts, int64_t width, void* out
     else
         launch(k_sum_partials<__nv_bfloat16>, grid, block, 0, 0, stream, partials, parts, width,
                (__nv_bfloat16*)out);
-    RUNE_LAUNCH_CHECK();
 }
 
 }  // namespace ops
@@ -779,7 +796,8 @@ int rune_rms_norm_backward(const rune_norm_grad_args* args, void* stream_) {
         else parts = launch_norm_bwd<__nv_bfloat16>(a, partials, stream);
         RUNE_LAUNCH_CHECK();
         if (partials)
-            sum_partials(partials, parts, a.width, a.dweight, a.weight_dtype, stream);
+            sum_partials(partials, parts, a.width, a.dweight, a.weight_dtype,
+                         partials + parts * a.width, stream);
     });
 }
 

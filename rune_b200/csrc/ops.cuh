@@ -78,9 +78,11 @@ void launch(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, int c
     RUNE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
 }
 
-// Sums the float32 partials [parts][width] over parts into out[width] of type dtype.
+// Sums the float32 partials [parts][width] over parts into out[width] of type dtype. Many parts
+// are summed in two steps, through partial_scratch(parts) further rows of `width` floats.
+int64_t partial_scratch(int64_t parts);
 void sum_partials(const float* partials, int64_t parts, int64_t width, void* out, int dtype,
-                  cudaStream_t stream);
+                  float* scratch, cudaStream_t stream);
 
 // ----------------------------------------------------------------------------- launches
 // Every thread calls it before its first access to global memory and, in kernels that hold TMEM,
