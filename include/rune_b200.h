@@ -329,6 +329,11 @@ typedef struct {
 int rune_rms_norm_backward(const rune_norm_grad_args* args, void* stream);
 int rune_rms_norm_backward_workspace(const rune_norm_grad_args* args, int64_t* bytes);
 
+/* Bound of the linear kernels' in-kernel waits, in polls of the mbarrier, for the calls that follow
+ * on any device (default RUNE_DEFAULT_WAIT_POLLS). 0 makes every wait give up at once, so that a
+ * host can exercise the failure path on healthy copies. */
+int rune_linear_set_wait_polls(uint32_t polls);
+
 /* Copies `rows` lines of `bytes` bytes, `stride` bytes apart, to lines `padded_stride` bytes apart
  * (a multiple of 16, at least `bytes`; `dst` 16-byte aligned): the layout in which the linear calls
  * read operands in place. The padding is written with whatever; nothing reads it. */

@@ -79,6 +79,7 @@ struct TileParams {
     float* z;               // saved z, or the partial sums
     float* colsum;          // [tiles_m * 4][n or 2n]
     unsigned* flag;
+    unsigned polls;         // bound of every wait
 };
 
 struct TileShared {
@@ -174,7 +175,7 @@ __device__ __forceinline__ void load_rows(const Stage& st, const T* src, int64_t
         for (int i = 0; i < 4; ++i) {
             v[i] = make_uint4(0, 0, 0, 0);
             if (in && r0 + 8 * i < rows)
-                v[i] = __ldg(reinterpret_cast<const uint4*>(p + i * 8 * ld));
+                v[i] = *reinterpret_cast<const uint4*>(p + i * 8 * ld);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) put16(st.turn(i), v[i]);
@@ -254,7 +255,7 @@ struct Bias {
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 uint4 q = make_uint4(0, 0, 0, 0);
-                if (g * 8 < left) q = __ldg(reinterpret_cast<const uint4*>(bias) + g);
+                if (g * 8 < left) q = reinterpret_cast<const uint4*>(bias)[g];
                 w[4 * g] = q.x, w[4 * g + 1] = q.y, w[4 * g + 2] = q.z, w[4 * g + 3] = q.w;
             }
         } else {
@@ -275,8 +276,8 @@ __device__ __forceinline__ void finish_z(const float (&v)[16], Two (&z)[8], cons
     for (int j = 0; j < 8; ++j) {
         z[j] = two(v[2 * j], v[2 * j + 1]);
         if constexpr (FP8) {
-            const float s0 = 2 * j < left ? __ldg(p.w_scale + col + 2 * j) : 0.0f;
-            const float s1 = 2 * j + 1 < left ? __ldg(p.w_scale + col + 2 * j + 1) : 0.0f;
+            const float s0 = 2 * j < left ? p.w_scale[col + 2 * j] : 0.0f;
+            const float s1 = 2 * j + 1 < left ? p.w_scale[col + 2 * j + 1] : 0.0f;
             z[j] = z[j] * (two(x_scale) * two(s0, s1));
         }
         if (p.bias) {
@@ -453,6 +454,10 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
             }
             if constexpr (kReads) {
                 if (sums) {
+                    if (lane >= rows) {  // beyond the last row: nothing, whatever the bias is
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) z[j] = u[j] = two(0.0f);
+                    }
                     column_sums(z, lane, zleft, sums + zcol);
                     if constexpr (kGate) column_sums(u, lane, zleft, sums + p.n + zcol);
                 }
@@ -554,7 +559,7 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
             int n0 = t.nt * bw;
             if (PAIR && rank) n0 += kGate ? (int)p.n : b_rows;
             for (int kb = kb0; kb < kb1; ++kb) {
-                ok = mbar_wait(smem_u32(&sh->empty[st]), parity) && !*fail;
+                ok = mbar_wait(smem_u32(&sh->empty[st]), parity, p.polls) && !*fail;
                 if (!__all_sync(0xffffffffu, ok)) {
                     ok = false;
                     break;
@@ -588,7 +593,7 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
         // the last releases of every stage arrive here (a pair's from the even block) before this
         // block's memory may go
         for (int i = max(0, issued - p.stages); i < issued && ok; ++i) {
-            ok = mbar_wait(smem_u32(&sh->empty[i % p.stages]), (i / p.stages) & 1) && !*fail;
+            ok = mbar_wait(smem_u32(&sh->empty[i % p.stages]), (i / p.stages) & 1, p.polls) && !*fail;
             ok = __all_sync(0xffffffffu, ok);
         }
         if (!ok && !*fail) *fail = 1;
@@ -613,7 +618,7 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
             const int split = p.splits > 1 ? (int)p.by_tiles.quotient(w) : 0;
             const int kb0 = split * p.kb_per_split;
             const int kb1 = min(p.kblocks, kb0 + p.kb_per_split);
-            ok = mbar_wait(smem_u32(&sh->acc_empty[buf]), acc_parity) && !*fail;
+            ok = mbar_wait(smem_u32(&sh->acc_empty[buf]), acc_parity, p.polls) && !*fail;
             if (!__all_sync(0xffffffffu, ok)) {
                 if (!*fail) *fail = 2;
                 ok = false;
@@ -622,7 +627,7 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
             fence_after_sync();
             const uint32_t acc = tmem + buf * 256;
             for (int kb = kb0; kb < kb1; ++kb) {
-                ok = mbar_wait(smem_u32(&sh->full[st]), parity) && !*fail;
+                ok = mbar_wait(smem_u32(&sh->full[st]), parity, p.polls) && !*fail;
                 if (!__all_sync(0xffffffffu, ok)) {
                     ok = false;
                     break;
@@ -649,7 +654,7 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
         if (!ok && !*fail) *fail = 3;
         // and the last arrivals of the epilogues (both blocks')
         for (int i = 0; i < 2 && ok; ++i) {
-            ok = mbar_wait(smem_u32(&sh->acc_empty[buf]), acc_parity) && !*fail;
+            ok = mbar_wait(smem_u32(&sh->acc_empty[buf]), acc_parity, p.polls) && !*fail;
             ok = __all_sync(0xffffffffu, ok);
             if (!ok && !*fail) *fail = 2;
             buf ^= 1;
@@ -669,7 +674,7 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
             epilogue<MODE, T, FP8>(
                 p, t, tmem + b * 256 + quarter, st, st2, warp, &map_o, &map_o2,
                 [&] {
-                    ok = mbar_wait(smem_u32(&sh->acc_full[b]), round & 1) && !*fail;
+                    ok = mbar_wait(smem_u32(&sh->acc_full[b]), round & 1, p.polls) && !*fail;
                     ok = __all_sync(0xffffffffu, ok);
                     fence_after_sync();
                     return ok;
@@ -727,7 +732,7 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
 // y (and z) from the float32 sums of `splits` ranges of k, added in order. Four columns a
 // thread; the sums' lines are padded to four values.
 template <int MODE, typename T>
-__global__ void __launch_bounds__(256) k_join(const TileParams p, const float* __restrict__ part) {
+__global__ void __launch_bounds__(256) k_join(const TileParams p, const float* part) {
     follow_on();
     constexpr bool kPair = MODE == kGated;
     const int64_t groups = (p.n + 3) / 4, total = p.m * groups;
@@ -832,9 +837,9 @@ __device__ __forceinline__ void join4(const float (&s)[4], float* sums, int coun
 // dz from a saved float32 z and dy, and the sums of each strip's columns
 template <bool GATED, typename T>
 __global__ void __launch_bounds__(256, 5)
-k_act_grad(int64_t m, int64_t n, const float* __restrict__ z, int64_t ld_part,
-           const T* __restrict__ dy, int64_t ld_dy, bool wide_dy, T* __restrict__ dz,
-           int64_t ld_dz, int act, int strip, float* __restrict__ sums) {
+k_act_grad(int64_t m, int64_t n, const float* z, int64_t ld_part,
+           const T* dy, int64_t ld_dy, bool wide_dy, T* dz,
+           int64_t ld_dz, int act, int strip, float* sums) {
     follow_on();
     const int64_t col = (int64_t)blockIdx.x * kColumns + (threadIdx.x & 63) * 4;
     const int count = (int)max((int64_t)0, min((int64_t)4, n - col)), part = threadIdx.x >> 6;
@@ -889,8 +894,8 @@ k_act_grad(int64_t m, int64_t n, const float* __restrict__ z, int64_t ld_part,
 // the sums of each strip's columns
 template <typename T>
 __global__ void __launch_bounds__(256)
-k_column_sums(int64_t m, int64_t n, const T* __restrict__ x, int64_t ld, bool wide, int strip,
-              float* __restrict__ sums) {
+k_column_sums(int64_t m, int64_t n, const T* x, int64_t ld, bool wide, int strip,
+              float* sums) {
     follow_on();
     const int64_t col = (int64_t)blockIdx.x * kColumns + (threadIdx.x & 63) * 4;
     const int count = (int)max((int64_t)0, min((int64_t)4, n - col)), part = threadIdx.x >> 6;
@@ -918,8 +923,8 @@ k_column_sums(int64_t m, int64_t n, const T* __restrict__ x, int64_t ld, bool wi
 // aligned 16-byte words that hold them, shifted together; where such a word is not inside the
 // matrix (its first and last lines), byte by byte.
 __global__ void __launch_bounds__(256)
-k_pack(const uint8_t* __restrict__ src, int64_t rows, int64_t bytes, int64_t ld,
-       uint8_t* __restrict__ dst, int64_t ld_dst) {
+k_pack(const uint8_t* src, int64_t rows, int64_t bytes, int64_t ld,
+       uint8_t* dst, int64_t ld_dst) {
     follow_on();
     const int64_t pieces = ld_dst / 16;
     const uint8_t* const end = src + (rows - 1) * ld + bytes;
@@ -931,8 +936,8 @@ k_pack(const uint8_t* __restrict__ src, int64_t rows, int64_t bytes, int64_t ld,
         const uint8_t* word = from - off;
         uint4 out;
         if (word >= src && word + (off ? 32 : 16) <= end) {
-            const uint4 a = __ldg(reinterpret_cast<const uint4*>(word));
-            const uint4 b = off ? __ldg(reinterpret_cast<const uint4*>(word) + 1) : a;
+            const uint4 a = *reinterpret_cast<const uint4*>(word);
+            const uint4 b = off ? reinterpret_cast<const uint4*>(word)[1] : a;
             uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
             // by whole words in two steps, then by the bits that are left
             if (off & 8) {
@@ -1087,6 +1092,7 @@ void run_mode(const Product& g, TileParams p, Scratch& ws, int device, cudaStrea
                             p.bn);
     const int b_box = plan.pair || pair ? p.bn / 2 : p.bn;  // lines of B in one copy
     p.flag = wait_flag(device);
+    p.polls = wait_polls();
     const CUtensorMap ma = make_map(g.a, eb, g.a_mn ? 64 : kBM);
     if (plan.splits == 1) {
         const int width = pair ? p.bn / 2 : p.bn;
@@ -1209,6 +1215,10 @@ void forward(const rune_linear_args& a, Scratch& ws, cudaStream_t stream) {
     run_product(g, p, ws, a.device, stream);
 }
 
+// rows of float32 for the parts of dbias (the tiles of a pair write whole eights) and their sums
+int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
+int64_t sum_rows(int64_t parts) { return round8(parts) + partial_scratch(parts); }
+
 void backward(const rune_linear_grad_args& a, Scratch& ws, cudaStream_t stream) {
     const int64_t n_all = a.gated ? 2 * a.outputs : a.outputs;
     const bool plain = !a.gated && a.activation == RUNE_ACT_NONE;
@@ -1229,20 +1239,17 @@ void backward(const rune_linear_grad_args& a, Scratch& ws, cudaStream_t stream) 
         if (want_dz) dz = readable(dz, 2, ws, stream);
         if (a.dbias) {
             parts = strips;
-            sums = ws.take<float>(((parts + 7) / 8 * 8 + partial_scratch(parts)) * n_all);
+            sums = ws.take<float>(sum_rows(parts) * n_all);
             if (!ws.sizing()) {
                 dim3 grid((unsigned)((n_all + kColumns - 1) / kColumns),
                           (unsigned)std::min<int64_t>(strips, 65535));
                 if (half)
-                    launch(
-                        k_column_sums<__half>, grid, 256, 0, 0, stream, a.rows, n_all,
-                        static_cast<const __half*>(a.dy), a.dy_stride, wide_dy, strip,
-                        sums);
+                    launch(k_column_sums<__half>, grid, 256, 0, 0, stream, a.rows, n_all,
+                           static_cast<const __half*>(a.dy), a.dy_stride, wide_dy, strip, sums);
                 else
-                    launch(
-                        k_column_sums<__nv_bfloat16>, grid, 256, 0, 0, stream, a.rows, n_all,
-                        static_cast<const __nv_bfloat16*>(a.dy), a.dy_stride, wide_dy,
-                        strip, sums);
+                    launch(k_column_sums<__nv_bfloat16>, grid, 256, 0, 0, stream, a.rows, n_all,
+                           static_cast<const __nv_bfloat16*>(a.dy), a.dy_stride, wide_dy, strip,
+                           sums);
                 RUNE_LAUNCH_CHECK();
             }
         }
@@ -1252,7 +1259,7 @@ void backward(const rune_linear_grad_args& a, Scratch& ws, cudaStream_t stream) 
         dz.p = to;
         if (a.saved) {
             parts = strips;
-            if (a.dbias) sums = ws.take<float>(((parts + 7) / 8 * 8 + partial_scratch(parts)) * n_all);
+            if (a.dbias) sums = ws.take<float>(sum_rows(parts) * n_all);
             if (!ws.sizing()) {
                 dim3 grid((unsigned)((a.outputs + kColumns - 1) / kColumns),
                           (unsigned)std::min<int64_t>(strips, 65535));
@@ -1261,13 +1268,13 @@ void backward(const rune_linear_grad_args& a, Scratch& ws, cudaStream_t stream) 
                     auto* dy = static_cast<const T*>(a.dy);
                     auto* out = reinterpret_cast<T*>(to);
                     if (a.gated)
-                        launch(
-                            k_act_grad<true, T>, grid, 256, 0, 0, stream, a.rows, a.outputs, a.saved, saved_line(a.outputs), dy, a.dy_stride, wide_dy,
-                            out, dz.ld, a.activation, strip, sums);
+                        launch(k_act_grad<true, T>, grid, 256, 0, 0, stream, a.rows, a.outputs,
+                               a.saved, saved_line(a.outputs), dy, a.dy_stride, wide_dy, out,
+                               dz.ld, a.activation, strip, sums);
                     else
-                        launch(
-                            k_act_grad<false, T>, grid, 256, 0, 0, stream, a.rows, a.outputs, a.saved, saved_line(a.outputs), dy, a.dy_stride, wide_dy,
-                            out, dz.ld, a.activation, strip, sums);
+                        launch(k_act_grad<false, T>, grid, 256, 0, 0, stream, a.rows, a.outputs,
+                               a.saved, saved_line(a.outputs), dy, a.dy_stride, wide_dy, out,
+                               dz.ld, a.activation, strip, sums);
                 };
                 if (half) go(__half());
                 else go(__nv_bfloat16());
@@ -1275,8 +1282,7 @@ void backward(const rune_linear_grad_args& a, Scratch& ws, cudaStream_t stream) 
             }
         } else {
             parts = (a.rows + 31) / 32;  // one a warp; the last tile (of a pair) has more warps
-            if (a.dbias)
-                sums = ws.take<float>(((parts + 7) / 8 * 8 + partial_scratch(parts)) * n_all);
+            if (a.dbias) sums = ws.take<float>(sum_rows(parts) * n_all);
             Product g;
             g.a = x, g.b = w;
             g.mode = a.gated ? kGatedGrad : kGrad;
@@ -1297,7 +1303,7 @@ void backward(const rune_linear_grad_args& a, Scratch& ws, cudaStream_t stream) 
         if (ws.sizing()) dz.p = reinterpret_cast<const void*>(256);
     }
     if (a.dbias && !ws.sizing())
-        sum_partials(sums, parts, n_all, a.dbias, a.dtype, sums + (parts + 7) / 8 * 8 * n_all,
+        sum_partials(sums, parts, n_all, a.dbias, a.dtype, sums + round8(parts) * n_all,
                      stream);
     if (a.dx) {
         Product g;
@@ -1378,6 +1384,7 @@ EncodeTiled encode_tiled() {
     return fn;
 }
 
+std::atomic<unsigned> g_polls{RUNE_DEFAULT_WAIT_POLLS};
 std::mutex g_flag_mutex;
 constexpr int kMaxDevices = 64;
 std::atomic<unsigned*> g_flag_host[kMaxDevices];
@@ -1422,6 +1429,8 @@ CUtensorMap make_out_map(const void* p, int64_t rows, int64_t cols, int64_t ld) 
 
 }  // namespace
 
+unsigned wait_polls() { return g_polls.load(std::memory_order_relaxed); }
+
 unsigned* wait_flag(int device) {
     if (device < 0 || device >= kMaxDevices)
         throw Error(RUNE_ERR_INVALID, "device index out of range");
@@ -1465,6 +1474,11 @@ using namespace rune;
 using namespace rune::ops;
 
 extern "C" {
+
+int rune_linear_set_wait_polls(uint32_t polls) {
+    g_polls.store(polls, std::memory_order_relaxed);
+    return RUNE_OK;
+}
 
 int rune_pad_rows(int32_t device, int64_t rows, int64_t bytes, int64_t stride, const void* src,
                   int64_t padded_stride, void* dst, void* stream) {

@@ -215,6 +215,7 @@ void linear_few(const rune_linear_args& a, const Matrix& x, const Matrix& w, cud
 
 // Host-mapped word that a kernel sets when a wait gave up; check_waits throws if it is set.
 unsigned* wait_flag(int device);
+unsigned wait_polls();
 void check_waits(int device);
 
 }  // namespace ops

@@ -43,6 +43,7 @@ struct FewParams {
     void* out;
     float* z;
     unsigned* flag;
+    unsigned polls;          // bound of every wait
 };
 
 struct FewShared {
@@ -109,7 +110,7 @@ k_few(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtenso
         uint32_t parity = 1;
         bool ok = true;
         for (int kb = kb0; kb < kb1; ++kb) {
-            ok = mbar_wait(smem_u32(&sh.empty[st]), parity) && !*fail;
+            ok = mbar_wait(smem_u32(&sh.empty[st]), parity, p.polls) && !*fail;
             if (!__all_sync(0xffffffffu, ok)) {
                 ok = false;
                 break;
@@ -141,7 +142,7 @@ k_few(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtenso
         uint32_t parity = 0;
         bool ok = true;
         for (int kb = kb0; kb < kb1; ++kb) {
-            ok = mbar_wait(smem_u32(&sh.full[st]), parity) && !*fail;
+            ok = mbar_wait(smem_u32(&sh.full[st]), parity, p.polls) && !*fail;
             if (!__all_sync(0xffffffffu, ok)) {
                 ok = false;
                 break;
@@ -167,7 +168,7 @@ k_few(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtenso
     }
     // every warp meets here, also after a failure; the products are done before the ring is reused
     __syncthreads();
-    bool ok = mbar_wait(smem_u32(&sh.done), 0) && !*fail;
+    bool ok = mbar_wait(smem_u32(&sh.done), 0, p.polls) && !*fail;
     if (!ok) *fail = 1;
     __syncthreads();
     if (*fail && tid == 0) {
@@ -311,6 +312,7 @@ void linear_few(const rune_linear_args& a, const Matrix& x, const Matrix& w, cud
     p.out = a.y;
     p.z = a.saved;
     p.flag = wait_flag(a.device);
+    p.polls = wait_polls();
     const CUtensorMap mw = make_map(w, eb, width), mx = make_map(x, eb, p.rows_pad);
     const bool half = a.out_dtype == RUNE_F16;
     auto go = [&](auto t) {

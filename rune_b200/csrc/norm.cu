@@ -318,7 +318,7 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
 
 template <typename T, Access ACC, bool BLOCK, int AHEAD>
 __global__ void __launch_bounds__(BLOCK ? 1024 : 256, BLOCK || ACC != kWhole ? 1 : 3)
-k_norm_bwd(const rune_norm_grad_args p, float* __restrict__ partials) {
+k_norm_bwd(const rune_norm_grad_args p, float* partials) {
     using P = Piece<T, ACC>;
     constexpr int N = P::N, NC = kEpt / N;
     follow_on();
@@ -457,7 +457,7 @@ k_norm_bwd(const rune_norm_grad_args p, float* __restrict__ partials) {
 // its own row of the workspace (each column always by the same thread).
 template <typename T>
 __global__ void __launch_bounds__(kLongThreads)
-k_norm_bwd_long(const rune_norm_grad_args p, float* __restrict__ partials) {
+k_norm_bwd_long(const rune_norm_grad_args p, float* partials) {
     follow_on();
     __shared__ float shared[32];
     const bool w32 = p.weight_dtype == RUNE_F32;
@@ -500,7 +500,7 @@ constexpr int kPartRows = 512;
 
 template <typename T>
 __global__ void __launch_bounds__(1024)
-k_sum_partials(const float* __restrict__ partials, int64_t parts, int64_t width, T* out) {
+k_sum_partials(const float* partials, int64_t parts, int64_t width, T* out) {
     follow_on();
     __shared__ float s[32][33];
     const int64_t col = (int64_t)blockIdx.x * 32 + threadIdx.x;

@@ -89,7 +89,8 @@ void sum_partials(const float* partials, int64_t parts, int64_t width, void* out
 // after the block has its TMEM: waits until the kernel before in the stream is complete and its
 // writes are visible, and lets the next one begin its own prologue. A kernel whose blocks wait
 // here needs nothing of the next one, and all its blocks are resident by then, so the next one's
-// waiting for shared memory or TMEM ends.
+// waiting for shared memory or TMEM ends. What the kernel before wrote is not constant for the
+// life of this one: no read-only (non-coherent) loads of it, which could be moved ahead of here.
 __device__ __forceinline__ void follow_on() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

@@ -520,6 +520,54 @@ def test_operators_run_on_the_current_stream_and_repeat_their_bits():
 
 
 @gpu
+def test_operators_see_what_the_kernels_before_them_wrote():
+    """Launches overlap the kernel before them; every result is that of one launch at a time."""
+    dt = torch.bfloat16
+
+    def chain(pause):
+        x, w = normal(87, 40, 256, dtype=dt), normal(88, 264, 256, dtype=dt, scale=0.05)
+        big, nw = normal(89, 3000, 256, dtype=dt), normal(90, 256, dtype=dt)
+        w2 = normal(91, 256, 264, dtype=dt, scale=0.05)
+        out = []
+        for i in range(30):
+            w.mul_(-1.01)
+            pause()
+            y = ops.linear(x, w, activation="gelu")  # few rows: reads the new w
+            pause()
+            x = ops.linear(y, w2, residual=x)
+            pause()
+            z = ops.linear(big, w)
+            pause()
+            big, _ = ops.rms_norm(ops.linear(z, w2), nw, residual=big)
+            pause()
+            nw.add_(0.01)
+            pause()
+            out.append(x.float().sum() + big.float().sum())
+        return [x, big, torch.stack(out)]
+
+    for got, want in zip(chain(lambda: None), chain(torch.cuda.synchronize)):
+        assert torch.equal(got, want)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [3, 300])
+def test_a_wait_that_gives_up_is_reported_and_leaves_the_context_usable(rows):
+    lib = L.load_library()
+    x, w = normal(95, rows, 640), normal(96, 512, 640, scale=0.1)
+    want = ops.linear(x, w)
+    torch.cuda.synchronize()
+    assert lib.rune_linear_set_wait_polls(0) == L.RUNE_OK
+    try:
+        ops.linear(x, w)  # undefined result
+        torch.cuda.synchronize()
+    finally:
+        lib.rune_linear_set_wait_polls(L.DEFAULT_WAIT_POLLS)
+    with pytest.raises(L.RuneError, match="did not complete in time"):
+        ops.linear(x, w)
+    assert torch.equal(ops.linear(x, w), want)
+
+
+@gpu
 def test_operators_in_a_cuda_graph():
     dt = torch.float16
     x, w = normal(75, 20, 200, dtype=dt), normal(76, 96, 200, dtype=dt, scale=0.1)
