@@ -6,8 +6,8 @@
 // A row stays in registers between the sum of its squares and its output, so every value is read
 // once and written once: memory bandwidth bounds the kernels, launch latency the shortest calls.
 // B200, of the measured copy's 6.5 TB/s: 373248 x 256 bf16 with residual 123 us, 6.2 TB/s;
-// 16384 x 4096 to e4m3 80 us, 5.9; their backward passes 155 us (6.1, five arrays) and 114 us
-// (5.9); one row of 4096 2.2 us.
+// 16384 x 4096 to e4m3 80 us, 5.9; backward 143 us (6.7, five arrays) and 16384 x 4096 112 us
+// (6.0); one row of 4096 2.2 us.
 //
 // A warp takes a row of up to 256 values (forward 512), a block of width / 8 threads (forward
 // width / 16) one of up to 8192 (16384); longer rows are read twice, the second time from L2.
