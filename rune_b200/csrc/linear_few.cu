@@ -172,17 +172,23 @@ k_few(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtenso
     }
     // every warp meets here, also after a failure; the products are done before the ring is reused
     __syncthreads();
-    bool ok = mbar_wait(smem_u32(&sh.done), 0, p.polls) && !*fail;
-    if (!ok) *fail = 1;
+    if (!mbar_wait(smem_u32(&sh.done), 0, p.polls)) *fail = 1;
     __syncthreads();
-    if (*fail && tid == 0) {
-        atomicExch_system(p.flag, 1u);
-        for (int i = max(0, sh.issued - p.stages); i < sh.issued; ++i)
-            mbar_wait(smem_u32(&sh.full[i % p.stages]), (i / p.stages) & 1);
+    const bool failed = *fail;
+    if (failed) {
+        // what is in flight lands, by waits of the full bound, before the ring takes the sums and
+        // TMEM goes: the copies first, then the products (warp 5 commits `done` in any case)
+        if (tid == 0) {
+            atomicExch_system(p.flag, 1u);
+            for (int i = max(0, sh.issued - p.stages); i < sh.issued; ++i)
+                mbar_wait(smem_u32(&sh.full[i % p.stages]), (i / p.stages) & 1);
+        }
+        mbar_wait(smem_u32(&sh.done), 0);
+        __syncthreads();
     }
     fence_after_sync();
     float* sums = reinterpret_cast<float*>(smem);  // [rows_pad][128]
-    if (warp < 4) {
+    if (warp < 4 && !failed) {
         for (int c = 0; c < p.rows; c += 16) {
             float v[16];
             tmem_ld16(tmem + ((uint32_t)(warp * 32) << 16) + c, v);
@@ -199,7 +205,7 @@ k_few(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtenso
     // write neighbouring outputs.
     const int per = width / (int)splits, f = (int)rank * per + tid % per;
     const int64_t col = f0 + f;
-    if (warp < 4 && col < p.n) {
+    if (warp < 4 && col < p.n && !failed) {
         const uint32_t base = smem_u32(sums);
         const int step = 128 / per;
         const int64_t up = p.n + col;

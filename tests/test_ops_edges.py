@@ -1,0 +1,46 @@
+"""The network operators where their inputs, their environment or their waits are unusual: waits
+that give up half way, values at the ends of the number range, transforms, several threads.
+Bounds are derived from the roundings, as in test_ops.py."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from rune_b200 import ops
+from rune_b200.runtime import library as L
+from tests.test_ops import normal
+
+gpu = pytest.mark.gpu
+
+
+# -------------------------------------------------------------------------------- bounded waits
+def give_up_after(polls, call):
+    """call() with the in-kernel waits bounded by `polls`, to its end on the GPU"""
+    lib = L.load_library()
+    torch.cuda.synchronize()
+    assert lib.rune_linear_set_wait_polls(polls) == L.RUNE_OK
+    try:
+        call()
+        torch.cuda.synchronize()
+    finally:
+        lib.rune_linear_set_wait_polls(L.DEFAULT_WAIT_POLLS)
+
+
+@gpu
+@pytest.mark.parametrize("rows,inputs,outputs", [(3, 640, 512), (48, 8192, 256), (16, 96, 8)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_few_rows_give_up_with_copies_and_products_in_flight(rows, inputs, outputs, gated):
+    """A block whose waits run out part way lets its copies and products land and leaves its
+    shared memory and TMEM in order: later launches on the same SMs give the same bits."""
+    x, w = normal(1, rows, inputs), normal(2, 2 * outputs, inputs, scale=inputs ** -0.5)
+    layer = ops.gated_linear if gated else ops.linear
+    want = layer(x, w)
+    for polls in (0, 1, 2, 3, 5, 8, 16):
+        give_up_after(polls, lambda: layer(x, w))  # undefined, or whole if no wait was that long
+        try:
+            layer(x, w)
+        except L.RuneError as e:
+            assert "did not complete in time" in str(e)
+        for _ in range(3):
+            assert torch.equal(layer(x, w), want), polls
