@@ -712,19 +712,29 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
     if constexpr (PAIR)
         failed = failed || peer_word(peer_address(smem_u32(&sh->fail), rank ^ 1)) != 0;
     if (failed) {
-        // let what is in flight land (bounded) before the blocks' memory goes: the copies of both
-        // blocks count on the even one's barriers
+        // Let what is in flight land (bounded) before the blocks' memory goes. The copies of both
+        // blocks count on the even one's barriers; a stage that only one of them had filled when
+        // the other gave up gets the other's part from here.
         if (tid == 0 && *fail) atomicExch_system(p.flag, (unsigned)*fail);
         if (tid == 0 && rank == 0) {
-            const int issued = sh->issued;
-            for (int i = max(0, issued - p.stages); i < issued; ++i)
-                mbar_wait(smem_u32(&sh->full[i % p.stages]), (i / p.stages) & 1);
+            const int mine = sh->issued;
+            const int theirs =
+                PAIR ? (int)peer_word(peer_address(smem_u32(&sh->issued), 1)) : mine;
+            const int issued = max(mine, theirs);
+            for (int i = max(0, issued - p.stages); i < issued; ++i) {
+                const uint32_t bar = smem_u32(&sh->full[i % p.stages]);
+                if (i >= theirs) mbar_complete_tx(bar, stage_bytes);
+                if (i >= mine) mbar_expect_tx(bar, stage_bytes);
+                mbar_wait(bar, (i / p.stages) & 1);
+            }
         }
-        if (warp == kMmaWarp && rank == 0) {
-            if (elect_one()) {
+        // the products, and on the odd block the arrivals that their completion sends there
+        if (warp == kMmaWarp) {
+            if (rank == 0 && elect_one()) {
                 if constexpr (PAIR) mma_commit_pair(smem_u32(&sh->drained));
                 else mma_commit(smem_u32(&sh->drained));
             }
+            __syncwarp();
             mbar_wait(smem_u32(&sh->drained), 0);
         }
         __syncwarp();

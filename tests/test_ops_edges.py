@@ -44,3 +44,32 @@ def test_few_rows_give_up_with_copies_and_products_in_flight(rows, inputs, outpu
             assert "did not complete in time" in str(e)
         for _ in range(3):
             assert torch.equal(layer(x, w), want), polls
+
+
+@gpu
+@pytest.mark.parametrize("rows,inputs,outputs", [(300, 640, 512), (2000, 1024, 1024),
+                                                 (130, 4096, 264), (9000, 256, 520)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_tiles_give_up_with_copies_and_products_in_flight(rows, inputs, outputs, gated):
+    """As above for the tiles, where the blocks of a pair may give up at different stages."""
+    x, w = normal(1, rows, inputs), normal(2, 2 * outputs, inputs, scale=inputs ** -0.5)
+    leaves = [x.requires_grad_(True), w.requires_grad_(True)]
+    layer = ((lambda: ops.gated_linear(x, w, activation="tanh")) if gated
+             else (lambda: ops.linear(x, w, activation="tanh")))
+    y = layer()
+    dy = normal(3, *y.shape)
+
+    def backward():
+        return torch.autograd.grad(y, leaves, dy, retain_graph=True)
+
+    want = [y, *backward()]
+    for polls in (0, 1, 2, 3, 5, 8, 16, 64):
+        for call in (layer, backward):
+            give_up_after(polls, call)
+            try:
+                layer()
+            except L.RuneError as e:
+                assert "did not complete in time" in str(e)
+        for _ in range(3):
+            for a, b in zip([layer(), *backward()], want):
+                assert torch.equal(a, b), polls
