@@ -274,7 +274,8 @@ int rune_tc_selftest(int32_t M, int32_t N, int32_t K, const float* a_host, const
  *
  * They need no engine. All pointers are device memory of CUDA device `device`; matrices are
  * row-major with unit column stride and the given row stride in elements; outputs and gradients
- * are contiguous and must not overlap the inputs. The calls only enqueue work on `stream`: they
+ * are contiguous and must not overlap the inputs. An array that does not start on a multiple of its
+ * values' size is refused (RUNE_ERR_INVALID). The calls only enqueue work on `stream`: they
  * neither synchronise it nor allocate device memory; scratch is the caller's (`workspace`,
  * 256-byte aligned, at least the bytes that the *_workspace query writes for the same
  * arguments; it holds nothing between calls). Sums, statistics and products are accumulated in

@@ -1377,6 +1377,10 @@ void check_linear(const rune_linear_args& a) {
             "x_scale and weight_scale go with e4m3 operands, both of them");
     require(!(a.gated && a.residual), "a gated layer takes no residual");
     require(a.rows == 0 || (a.x && a.weight && a.y), "null argument");
+    require_aligned({a.x, a.weight}, dtype_bytes(a.dtype));
+    require_aligned({a.bias, a.residual, a.y}, dtype_bytes(a.out_dtype));
+    require_aligned({a.x_scale, a.weight_scale}, sizeof(float));
+    require(aligned(a.saved, 16), "saved is not 16-byte aligned");
 }
 
 void check_grad(const rune_linear_grad_args& a) {
@@ -1384,6 +1388,9 @@ void check_grad(const rune_linear_grad_args& a) {
     require(a.dtype == RUNE_F16 || a.dtype == RUNE_BF16,
             "gradients take float16 or bfloat16 operands");
     require(a.rows == 0 || (a.x && a.weight && a.dy), "null argument");
+    require_aligned({a.x, a.weight, a.bias, a.dy, a.dx, a.dweight, a.dbias},
+                    dtype_bytes(a.dtype));
+    require(aligned(a.saved, 16), "saved is not 16-byte aligned");
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,

@@ -748,6 +748,10 @@ int rune_rms_norm(const rune_norm_args* args, void* stream_) {
                 "the output has the rows' type, or is e4m3 with a scale array");
         if (a.rows == 0) return;
         require(a.x && a.y, "null argument");
+        require_aligned({a.x, a.residual, a.h}, dtype_bytes(a.dtype));
+        require_aligned({a.y}, dtype_bytes(a.out_dtype));
+        require_aligned({a.weight}, dtype_bytes(a.weight_dtype));
+        require_aligned({a.scale, a.rstd}, sizeof(float));
         if (a.dtype == RUNE_F32) launch_norm<float>(a, stream);
         else if (a.dtype == RUNE_F16) launch_norm<__half>(a, stream);
         else launch_norm<__nv_bfloat16>(a, stream);
@@ -760,6 +764,9 @@ static void check_norm_grad(const rune_norm_grad_args& a) {
     require(known_norm_type(a.dtype), "rms_norm takes float32, float16 or bfloat16 rows");
     require(a.weight_dtype == a.dtype || a.weight_dtype == RUNE_F32,
             "the weight has the rows' type or float32");
+    require_aligned({a.x, a.residual, a.dy, a.dh, a.dx}, dtype_bytes(a.dtype));
+    require_aligned({a.weight, a.dweight}, dtype_bytes(a.weight_dtype));
+    require_aligned({a.rstd}, sizeof(float));
 }
 
 int rune_rms_norm_backward_workspace(const rune_norm_grad_args* args, int64_t* bytes) {

@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <initializer_list>
 #include <new>
 #include <type_traits>
 
@@ -54,6 +55,12 @@ inline void require(bool ok, const char* message) {
 inline int dtype_bytes(int dtype) { return dtype == RUNE_F32 ? 4 : dtype == RUNE_E4M3 ? 1 : 2; }
 
 inline bool aligned(const void* p, size_t bytes) { return (uintptr_t)p % bytes == 0; }
+
+// every array starts on a multiple of `bytes`, its values' size (or more, where the header asks)
+inline void require_aligned(std::initializer_list<const void*> arrays, size_t bytes) {
+    for (const void* p : arrays)
+        require(aligned(p, bytes), "an array does not start on a multiple of its values' size");
+}
 
 int sm_count(int device);
 

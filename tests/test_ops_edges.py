@@ -4,6 +4,8 @@ Bounds are derived from the roundings, as in test_ops.py."""
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
@@ -73,3 +75,45 @@ def test_tiles_give_up_with_copies_and_products_in_flight(rows, inputs, outputs,
         for _ in range(3):
             for a, b in zip([layer(), *backward()], want):
                 assert torch.equal(a, b), polls
+
+
+# ------------------------------------------------------------------------------------ refusals
+def refused_at(name, args, fields, step):
+    """rune_<name> refuses each field at an address `step` bytes off, and launches nothing"""
+    call = getattr(L.load_library(), name)
+    for field in fields:
+        raw = type(args)()
+        ctypes.pointer(raw)[0] = args
+        setattr(raw, field, getattr(raw, field) + step)
+        assert call(ctypes.byref(raw), None) == L.RUNE_ERR_INVALID, (name, field)
+
+
+@gpu
+def test_misaligned_arrays_are_refused():
+    """An address inside a value, or a saved z off 16 bytes, would fault in the kernels."""
+    buf = torch.zeros(1 << 16, dtype=torch.uint8, device="cuda")
+    at = [buf.data_ptr() + 4096 * i for i in range(12)]
+    size = dict(rows=4, width=16, x_stride=16, residual_stride=16, dtype=L.RUNE_F32,
+                weight_dtype=L.RUNE_F32)
+    norm = L.NormArgs(**size, out_dtype=L.RUNE_F32, x=at[0], residual=at[1], weight=at[2],
+                      y=at[3], h=at[4], scale=at[5], rstd=at[6])
+    refused_at("rune_rms_norm", norm, ("x", "residual", "weight", "y", "h", "scale", "rstd"), 2)
+    grad = L.NormGradArgs(**size, dy_stride=16, dh_stride=16, x=at[0], residual=at[1],
+                          weight=at[2], rstd=at[3], dy=at[4], dh=at[5], dx=at[6], dweight=at[7],
+                          workspace=at[8], workspace_bytes=16384)
+    refused_at("rune_rms_norm_backward", grad,
+               ("x", "residual", "weight", "rstd", "dy", "dh", "dx", "dweight"), 2)
+    size = dict(rows=4, inputs=16, outputs=8, x_stride=16, weight_stride=16, dtype=L.RUNE_BF16,
+                activation=L.RUNE_ACT["silu"])
+    linear = L.LinearArgs(**size, out_dtype=L.RUNE_BF16, residual_stride=8, x=at[0], weight=at[1],
+                          bias=at[2], residual=at[3], y=at[4], saved=at[5])
+    refused_at("rune_linear", linear, ("x", "weight", "bias", "residual", "y"), 1)
+    refused_at("rune_linear", linear, ("saved",), 8)
+    linear.dtype, linear.x_scale, linear.weight_scale = L.RUNE_E4M3, at[6], at[7]
+    refused_at("rune_linear", linear, ("x_scale", "weight_scale"), 2)
+    grad = L.LinearGradArgs(**size, dy_stride=8, x=at[0], weight=at[1], bias=at[2], dy=at[3],
+                            saved=at[4], dx=at[5], dweight=at[6], dbias=at[7], workspace=at[8],
+                            workspace_bytes=16384)
+    refused_at("rune_linear_backward", grad,
+               ("x", "weight", "bias", "dy", "dx", "dweight", "dbias"), 1)
+    refused_at("rune_linear_backward", grad, ("saved",), 8)
