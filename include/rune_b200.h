@@ -304,7 +304,8 @@ typedef struct {
     const void* weight;     /* [width]; NULL: no normalisation, y = h */
     void* y;                /* [rows, width] */
     void* h;                /* [rows, width] x + residual, or NULL */
-    float* scale;           /* [rows], RUNE_E4M3 only: y stands for y * scale */
+    float* scale;           /* [rows], RUNE_E4M3 only: y stands for y * scale. The row's largest
+                               magnitude / 448 but at least 2^-126; 1 for a row of zeros */
     float* rstd;            /* [rows] 1 / sqrt(mean h^2 + eps) for the backward, or NULL */
 } rune_norm_args;
 

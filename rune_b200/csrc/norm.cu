@@ -170,9 +170,10 @@ __device__ __forceinline__ void store_e4m3(void* row, int col, int width, const 
     }
 }
 
-// scale of a row whose largest magnitude is amax: 448 stands for amax; an all-zero row takes 1
+// Scale of a row whose largest magnitude is amax: 448 stands for amax; an all-zero row takes 1.
+// Never below the smallest normal float, whose reciprocal is finite.
 __device__ __forceinline__ float row_scale(float amax) {
-    return amax == 0.0f ? 1.0f : amax * (1.0f / kE4m3Max);
+    return amax == 0.0f ? 1.0f : max_nan(amax * (1.0f / kE4m3Max), 0x1p-126f);
 }
 
 // ----------------------------------------------------------------------------- forward
@@ -237,14 +238,15 @@ __launch_bounds__(THREADS, ACC == kWhole && sizeof(T) == 2 && BLOCK ? 1536 / THR
     row_join<BLOCK, Q8>(sum, amax, shared);
     const float r = p.weight ? 1.0f / sqrtf(sum / (float)width + p.eps) : 1.0f;
     if (t == 0 && p.rstd) p.rstd[row] = r;
-    float f = r;
-    if constexpr (Q8) {
-        const float scale = row_scale(r * amax);
-        if (t == 0) p.scale[row] = scale;
-        f = r * (1.0f / scale);
-    }
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) h[i] *= f;
+    for (int i = 0; i < EPT; ++i) h[i] *= r;
+    if constexpr (Q8) {
+        const float scale = row_scale(r * amax), inv = 1.0f / scale;
+        if (t == 0) p.scale[row] = scale;
+        // after r and not with it: r / scale of a row of tiny values can pass float32's range
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) h[i] *= inv;
+    }
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         if constexpr (Q8) {

@@ -94,7 +94,8 @@ def rms_norm(x, weight, residual=None, eps=1.0e-8):
 def rms_norm_fp8(x, weight, residual=None, eps=1.0e-8):
     """``rms_norm`` with its rows in 8 bits: ``(q, scale)``, and with a residual
     ``(q, scale, h)``. q (float8_e4m3fn) stands for ``q * scale``; a row's scale maps its largest
-    magnitude to 448 and is 1 for a row of zeros. Not differentiable.
+    magnitude to 448, is 1 for a row of zeros and otherwise at least 2^-126 (float32's smallest
+    normal number). Not differentiable.
     """
     if weight is None:
         raise ValueError("rms_norm_fp8 needs a weight.")

@@ -77,6 +77,59 @@ def test_tiles_give_up_with_copies_and_products_in_flight(rows, inputs, outputs,
                 assert torch.equal(a, b), polls
 
 
+# ---------------------------------------------------------------------------------- tiny values
+def check_rows_in_8_bits(q, scale, y, slack):
+    """q * scale against y (float64): scale within `slack` of its definition, each value within
+    e4m3's rounding (2^-4 of the value, 2^-10 below the smallest normal)"""
+    amax = y.abs().amax(-1)
+    want = torch.where(amax > 0, (amax / 448.0).clamp(min=2.0 ** -126), torch.ones_like(amax))
+    assert bool(((scale.double() - want).abs() <= slack * want).all())
+    v = y / scale.double()[:, None]
+    off = (q.double() - v).abs()  # NaN where q is
+    assert bool((off <= 2.0 ** -4 * (1 + 1e-3) * v.abs() + 2.0 ** -10 + 448 * slack).all())
+
+
+def tiny_rows(width, tops, dtype):
+    """rows of random values whose largest magnitudes are `tops`, every third value zero"""
+    pattern = normal(11, len(tops), width, dtype=torch.float32).double()
+    pattern[:, ::3] = 0.0
+    pattern /= pattern.abs().amax(-1, keepdim=True)
+    return (pattern * torch.tensor(tops, dtype=torch.float64, device="cuda")[:, None]).to(dtype)
+
+
+TINY_TOPS = [1.0, 1e-28, 1e-30, 1e-32, 1e-34, 1e-35, 1e-36, 1e-37, 1e-38, 1e-40, 1e-42, 1e-44]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("width", [5, 64, 264, 1001, 5000, 20001])
+def test_rows_of_tiny_values_to_8_bits(width, dtype):
+    tops = TINY_TOPS if dtype is not torch.float16 else [1.0, 1e-4, 1e-6, 6e-8]
+    x = tiny_rows(width, tops, dtype)
+    check_rows_in_8_bits(*ops.quantize_fp8(x), x.double(), 4 * 2.0 ** -24)
+
+
+@gpu
+@pytest.mark.parametrize("width", [64, 1001, 20001])
+@pytest.mark.parametrize("tiny_weight", [False, True])
+def test_norm_of_tiny_values_to_8_bits(width, tiny_weight):
+    """With h^2 below eps the norm multiplies by 1 / sqrt(eps); with a tiny weight only y is tiny.
+    h w may be subnormal in float32: 2^-149 of it is 2^-149 / sqrt(eps) of y."""
+    eps = 1e-8
+    if tiny_weight:
+        x = normal(12, 9, width, dtype=torch.float32)
+        w = tiny_rows(width, [3e-38], torch.float32)[0]
+    else:
+        x = tiny_rows(width, [1e-22, 1e-28, 1e-32, 1e-34, 1e-36, 1e-37, 2e-38], torch.float32)
+        w = normal(13, width, dtype=torch.float32, scale=0.2) + 1
+    h = x.double()
+    y = h / torch.sqrt((h * h).mean(-1, keepdim=True) + eps) * w.double()
+    slack = (width + 16) * 2.0 ** -24
+    if not tiny_weight:  # of a row's largest value
+        slack += float((2.0 ** -149 * eps ** -0.5 / y.abs().amax(-1)).max())
+    check_rows_in_8_bits(*ops.rms_norm_fp8(x, w, eps=eps), y, slack)
+
+
 # ------------------------------------------------------------------------------------ refusals
 def refused_at(name, args, fields, step):
     """rune_<name> refuses each field at an address `step` bytes off, and launches nothing"""
