@@ -65,7 +65,8 @@ class ScalarNetwork(nn.Module):
     def _start(self, descriptors, types):
         q = (descriptors * self.q_scaler).to(self.dtype)
         weight, bias = self._cast(self.input_projection)
-        embedding = self.element_embedding.weight.to(self.dtype)[types]
+        # rows first, then 16 bits: a table's gradient sums over all atoms of an element, in float32
+        embedding = self.element_embedding(types).to(self.dtype)
         return ops.linear(q, weight, bias=bias, residual=embedding)
 
     def _finish(self, stream, delta, types):

@@ -111,6 +111,47 @@ def test_gradients_reach_every_parameter(gated):
         assert float((g - w).norm()) <= 20 * 2.0 ** -8 * float(w.norm()), name
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,unit", [(torch.bfloat16, 2.0 ** -8), (torch.float16, 2.0 ** -11)])
+def test_embedding_gradient_of_many_atoms(dtype, unit):
+    """33333 atoms an element whose gradients have one sign. The network is projection, norm and
+    head: an atom's gradient is the norm's, with 16-bit operands h, w and dy and a result of 16
+    bits, each off by one rounding of its two terms; then float32 sums of all atoms (n 2^-24)."""
+    torch.manual_seed(0)
+    net = ScalarNetwork(3, 8, 64, 96, 0, dtype=dtype).cuda()
+    with torch.no_grad():
+        net.energy_heads.weight.copy_(torch.randn(3, 64, device="cuda"))
+        net.output_norm.weight.copy_(1 + 0.2 * torch.randn(64, device="cuda"))
+    n = 99999
+    q = 0.05 * torch.randn(n, 8, device="cuda")
+    types = torch.arange(n, device="cuda") % 3
+    (100.0 * net(q, types)).sum().backward()
+    p = {k: v.detach().double() for k, v in net.state_dict().items()}
+    # h as the projection rounds it: one rounding of the operands' products and of the sum
+    h = (q.double() * p["q_scaler"]) @ p["input_projection.weight"].t()
+    h = h + p["input_projection.bias"] + p["element_embedding.weight"][types]
+    r = 1.0 / torch.sqrt((h * h).mean(-1, keepdim=True) + net.norm_eps)
+    gw = 100.0 * p["energy_heads.weight"][types] * p["output_norm.weight"]
+    normed = h * r
+    dot = (gw * normed).mean(-1, keepdim=True)
+    dh = r * (gw - normed * dot)
+    # roundings: dy, dx and h (q, weights, bias, embedding and the sum, of the terms' magnitudes)
+    terms = (q.double().abs() @ p["input_projection.weight"].abs().t()
+             + p["input_projection.bias"].abs() + p["element_embedding.weight"][types].abs())
+    eh = 4 * unit * terms
+    en = r * (eh + normed.abs() * (normed.abs() * eh * r).mean(-1, keepdim=True))
+    edot = (gw.abs() * (2 * unit * normed.abs() + en)).mean(-1, keepdim=True)
+    er = (normed.abs() * eh * r).mean(-1, keepdim=True)  # of r, relative
+    bound = r * (2 * unit * gw.abs() + en * dot.abs() + normed.abs() * edot)
+    bound = bound + (unit + er + n * 2.0 ** -24) * r * (gw.abs() + (normed * dot).abs())
+    want, room = (torch.zeros(3, 64, dtype=torch.float64, device="cuda").index_add_(0, types, t)
+                  for t in (dh, bound))
+    got = net.element_embedding.weight.grad.double()
+    assert bool(((got - want).abs() <= 1.01 * room).all())
+    # and 5 roundings of bfloat16 of the largest sum: the gradients of an element are alike
+    assert float((got - want).abs().max()) <= 0.02 * float(want.abs().max())
+
+
 class _Live:
     """detach().double() of a float64 leaf that is to keep its gradient."""
 
