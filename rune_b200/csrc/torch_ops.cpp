@@ -9,10 +9,14 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
+#include <c10/core/AutogradState.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <initializer_list>
 #include <sstream>
 #include <stdexcept>
 #include <string>
@@ -134,9 +138,27 @@ Tensor scratch(Query query, Args& args, const Tensor& x) {
     return ws;
 }
 
-void first_order_only() {
+// What follows tensors through torch's own operators does not see these: a tangent would be
+// lost, and a trace would keep the empty output and no kernel that fills it.
+void no_transforms(std::initializer_list<const Tensor*> inputs) {
+    using c10::impl::TorchDispatchModeKey;
+    using c10::impl::TorchDispatchModeTLS;
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode())
+        for (const Tensor* t : inputs)
+            if (t->defined() && t->_fw_grad(/*level=*/0).defined())
+                throw std::runtime_error(
+                    "the operators of rune_b200.ops have no forward-mode derivative.");
+    if (at::tracer::impl::is_dispatch_enabled() ||
+        (TorchDispatchModeTLS::any_modes_set() &&
+         (TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY) ||
+          TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FAKE))))
+        throw std::runtime_error("the operators of rune_b200.ops cannot be traced.");
+}
+
+void first_order_only(const variable_list& grads) {
     if (at::GradMode::is_enabled())  // create_graph=True
         throw std::runtime_error("the operators of rune_b200.ops have no second derivative.");
+    for (const Tensor& g : grads) no_transforms({&g});
 }
 
 // ------------------------------------------------------------------------------------ norm
@@ -180,7 +202,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
         return {o.y};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        first_order_only();
+        first_order_only(grads);
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &weight = saved[1], &residual = saved[2];
         const Tensor dh_in = grads.size() > 1 ? grads[1] : Tensor();
@@ -292,7 +314,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
         return o.y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        first_order_only();
+        first_order_only(grads);
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2];
         const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
@@ -323,6 +345,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
 
 Tensor layer(const Tensor& x, const Tensor& weight, Tensor bias, const Tensor& residual,
              Tensor x_scale, Tensor w_scale, int64_t act, bool gated, int out_code) {
+    no_transforms({&x, &weight, &bias, &residual, &x_scale, &w_scale});
     check_cuda(x);
     const ScalarType t = x.scalar_type();
     const bool fp8 = t == ScalarType::Float8_e4m3fn;
@@ -431,6 +454,7 @@ PyObject* py_rms_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
         Tensor w = tensor_arg(args[1], "weight");
         const double eps = PyFloat_AsDouble(args[3]);
         if (PyErr_Occurred()) throw 0;
+        no_transforms({&x, &w, &res});
         if (!w.defined()) bad("rms_norm needs a weight.");
         check_norm(x, w, res);
         if (at::GradMode::is_enabled() &&
@@ -451,6 +475,7 @@ PyObject* py_to_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
         Tensor w = tensor_arg(args[1], "weight");
         const double eps = PyFloat_AsDouble(args[3]);
         if (PyErr_Occurred()) throw 0;
+        no_transforms({&x, &w, &res});
         check_norm(x, w, res);
         if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(w) || wants_grad(res)))
             bad("8-bit outputs have no gradient; call under torch.no_grad().");
@@ -464,6 +489,7 @@ PyObject* py_padded(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!count_is(n, 1)) return nullptr;
     return guarded([&] {
         const Tensor t = tensor_arg(args[0], "t");
+        no_transforms({&t});
         if (!t.defined() || !t.is_cuda()) bad("t must be a CUDA tensor; there is no CPU path.");
         if (t.dim() != 2 || t.size(1) == 0) bad("t needs two axes, the last one not empty.");
         if (at::GradMode::is_enabled() && t.requires_grad())

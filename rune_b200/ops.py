@@ -12,8 +12,9 @@ CUDA tensors, for training, distilling or serving networks beside the engine's f
 
 Every function works on the last axis of its input, takes row-strided views, runs on the current
 stream of the tensors' device without synchronising it, and returns new tensors. Wrong types,
-shapes or devices raise ``ValueError``; failures of the GPU raise ``RuneError``. Sums and
-statistics are float32; results are rounded once. Equal inputs give equal bits.
+shapes or devices raise ``ValueError``; failures of the GPU raise ``RuneError``. Gradients are
+reverse-mode and of first order; forward-mode tangents, function transforms and traces are refused
+(``RuntimeError``). Sums and statistics are float32; results are rounded once. Equal inputs give equal bits.
 """
 
 from __future__ import annotations

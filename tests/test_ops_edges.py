@@ -130,6 +130,59 @@ def test_norm_of_tiny_values_to_8_bits(width, tiny_weight):
     check_rows_in_8_bits(*ops.rms_norm_fp8(x, w, eps=eps), y, slack)
 
 
+# ---------------------------------------------------------------------------------- transforms
+def every_operator(x, w):
+    """calls of square x and w, one an operator, with x and with w as the input"""
+    for f in (lambda a, b: ops.linear(a, b), lambda a, b: ops.gated_linear(a, b),
+              lambda a, b: ops.linear(b, b, bias=b[0], residual=a),
+              lambda a, b: ops.rms_norm(a, b[0]), lambda a, b: ops.rms_norm_fp8(a, b[0])):
+        yield lambda a, f=f: f(a, w)
+        yield lambda a, f=f: f(x, a)
+    yield lambda a: ops.quantize_fp8(a)
+    yield lambda a: ops.padded(a)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_forward_mode_and_traces_are_refused(device):
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x = torch.ones(16, 16, dtype=torch.bfloat16, device=device)
+    for f in every_operator(x, torch.ones_like(x)):
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            f(forward_ad.make_dual(x, torch.ones_like(x)))
+        with forward_ad.dual_level(), torch.no_grad(), pytest.raises(RuntimeError,
+                                                                     match="forward-mode"):
+            f(forward_ad.make_dual(x, torch.ones_like(x)))
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(lambda a: f(a + 1), x, check_trace=False)
+        with pytest.raises(RuntimeError, match="traced"):
+            make_fx(lambda a: f(a + 1))(x)
+        for transform in (lambda: torch.func.vmap(f)(x[None]), lambda: torch.func.jvp(f, (x,), (x,))):
+            with pytest.raises((RuntimeError, ValueError)):
+                transform()
+
+
+@gpu
+def test_transforms_of_a_backward_are_refused():
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x = normal(21, 60, 64).requires_grad_(True)
+    w = normal(22, 64, 64).requires_grad_(True)
+    for y in (ops.linear(x, w, activation="tanh"), ops.rms_norm(x, w[0])):
+        dy = torch.ones_like(y)
+
+        def backward(g):
+            return torch.autograd.grad(y, x, g, retain_graph=True)[0]
+
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            backward(forward_ad.make_dual(dy, dy))
+        with pytest.raises(RuntimeError, match="traced"):
+            make_fx(backward)(dy)
+        assert bool(backward(dy).isfinite().all())
+
+
 # ------------------------------------------------------------------------------------ refusals
 def refused_at(name, args, fields, step):
     """rune_<name> refuses each field at an address `step` bytes off, and launches nothing"""
