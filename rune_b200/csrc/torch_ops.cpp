@@ -385,7 +385,8 @@ Tensor layer(const Tensor& x, const Tensor& weight, Tensor bias, const Tensor& r
         check_tensor(residual, "residual", out, shape, x);
     }
     if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() ||
-                                       wants_grad(bias) || wants_grad(residual))) {
+                                       wants_grad(bias) || wants_grad(residual) ||
+                                       wants_grad(x_scale) || wants_grad(w_scale))) {
         if (fp8)
             bad("float8_e4m3fn operands have no gradient; call under torch.no_grad().");
         return LinearFn::apply(x, weight, given(bias), given(residual), act, gated);

@@ -223,3 +223,16 @@ def test_misaligned_arrays_are_refused():
     refused_at("rune_linear_backward", grad,
                ("x", "weight", "bias", "dy", "dx", "dweight", "dbias"), 1)
     refused_at("rune_linear_backward", grad, ("saved",), 8)
+
+
+@gpu
+@pytest.mark.parametrize("layer", [ops.linear, ops.gated_linear])
+def test_scales_that_require_a_gradient_are_refused(layer):
+    """as the 8-bit operands and their bias are: the call has no gradient to give"""
+    (x, xs), (w, ws) = ops.quantize_fp8(normal(31, 60, 64)), ops.quantize_fp8(normal(32, 48, 64))
+    want = layer(x, w, x_scale=xs, weight_scale=ws)
+    for scales in ((xs.clone().requires_grad_(True), ws), (xs, ws.clone().requires_grad_(True))):
+        with pytest.raises(ValueError, match="no gradient"):
+            layer(x, w, x_scale=scales[0], weight_scale=scales[1])
+        with torch.no_grad():
+            assert torch.equal(layer(x, w, x_scale=scales[0], weight_scale=scales[1]), want)
