@@ -282,8 +282,8 @@ int rune_tc_selftest(int32_t M, int32_t N, int32_t K, const float* a_host, const
  * float32, in an order that depends on the sizes alone, so equal inputs give equal bits.
  *
  * The linear kernels wait for copies with a bounded number of polls. A wait that gives up leaves
- * the outputs of that call undefined and is reported as RUNE_ERR_CUDA by the next operator call
- * on the device. */
+ * the outputs of that call undefined and is reported, once, as RUNE_ERR_CUDA by the next operator
+ * call on the device or by rune_linear_check_waits. */
 #define RUNE_F32 0
 #define RUNE_F16 1
 #define RUNE_BF16 2
@@ -335,6 +335,10 @@ int rune_rms_norm_backward_workspace(const rune_norm_grad_args* args, int64_t* b
  * on any device (default RUNE_DEFAULT_WAIT_POLLS). 0 makes every wait give up at once, so that a
  * host can exercise the failure path on healthy copies. */
 int rune_linear_set_wait_polls(uint32_t polls);
+
+/* RUNE_ERR_CUDA if a wait on the device gave up since the last report. For the last call before a
+ * result is used, and for replayed graphs, which make no operator call: synchronise first. */
+int rune_linear_check_waits(int32_t device);
 
 /* Copies `rows` lines of `bytes` bytes, `stride` bytes apart, to lines `padded_stride` bytes apart
  * (a multiple of 16, at least `bytes`; `dst` 16-byte aligned): the layout in which the linear calls

@@ -1485,14 +1485,12 @@ unsigned* wait_flag(int device) {
 
 void check_waits(int device) {
     if (device < 0 || device >= kMaxDevices) return;
-    volatile unsigned* host = g_flag_host[device].load(std::memory_order_acquire);
-    if (host && *host) {
-        const unsigned where = *host;
-        *host = 0;
+    unsigned* host = g_flag_host[device].load(std::memory_order_acquire);
+    if (!host || !*static_cast<volatile unsigned*>(host)) return;
+    if (const unsigned where = __atomic_exchange_n(host, 0u, __ATOMIC_ACQ_REL))
         throw Error(RUNE_ERR_CUDA,
                     "A device-side copy of an earlier linear operator did not complete in time "
                     "(wait " + std::to_string(where) + "); the results of that call are invalid.");
-    }
 }
 
 }  // namespace ops
@@ -1508,12 +1506,17 @@ int rune_linear_set_wait_polls(uint32_t polls) {
     return RUNE_OK;
 }
 
+int rune_linear_check_waits(int32_t device) {
+    return guarded(device, [&] { check_waits(device); });
+}
+
 int rune_pad_rows(int32_t device, int64_t rows, int64_t bytes, int64_t stride, const void* src,
                   int64_t padded_stride, void* dst, void* stream) {
     return guarded(device, [&] {
         require(rows >= 0 && bytes >= 1 && padded_stride >= bytes && padded_stride % 16 == 0 &&
                     padded_stride / 16 <= INT32_MAX,
                 "rows, bytes or padded_stride out of range");
+        check_waits(device);
         if (rows == 0) return;
         require(src && dst && aligned(dst, 16), "null argument, or dst not 16-byte aligned");
         pad_rows(src, rows, bytes, stride, dst, padded_stride, static_cast<cudaStream_t>(stream));
@@ -1543,8 +1546,8 @@ int rune_linear(const rune_linear_args* args, void* stream_) {
     auto stream = static_cast<cudaStream_t>(stream_);
     return guarded(a.device, [&] {
         check_linear(a);
-        if (a.rows == 0) return;
         check_waits(a.device);
+        if (a.rows == 0) return;
         Scratch need{nullptr};
         forward(a, need, stream);
         if (need.off > 0 && !a.workspace)
@@ -1580,6 +1583,7 @@ int rune_linear_backward(const rune_linear_grad_args* args, void* stream_) {
     auto stream = static_cast<cudaStream_t>(stream_);
     return guarded(a.device, [&] {
         check_grad(a);
+        check_waits(a.device);
         const int64_t n_all = a.gated ? 2 * a.outputs : a.outputs;
         if (a.rows == 0) {
             if (a.dweight)
@@ -1589,7 +1593,6 @@ int rune_linear_backward(const rune_linear_grad_args* args, void* stream_) {
                 RUNE_CUDA_TRY(cudaMemsetAsync(a.dbias, 0, (size_t)(n_all * 2), stream));
             return;
         }
-        check_waits(a.device);
         Scratch need{nullptr};
         backward(a, need, stream);
         require(need.off == 0 || (a.workspace && aligned(a.workspace, 256) &&

@@ -220,10 +220,9 @@ CUtensorMap make_map(const Matrix& m, int elem_bytes, int box_rows);
 constexpr int kFewRows = 48;
 void linear_few(const rune_linear_args& a, const Matrix& x, const Matrix& w, cudaStream_t stream);
 
-// Host-mapped word that a kernel sets when a wait gave up; check_waits throws if it is set.
+// Host-mapped word that a kernel sets when a wait gave up (ops::check_waits reads it).
 unsigned* wait_flag(int device);
 unsigned wait_polls();
-void check_waits(int device);
 
 }  // namespace ops
 }  // namespace rune

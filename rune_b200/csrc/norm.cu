@@ -748,6 +748,7 @@ int rune_rms_norm(const rune_norm_args* args, void* stream_) {
                 "the weight has the rows' type or float32");
         require(a.out_dtype == a.dtype || (a.out_dtype == RUNE_E4M3 && a.scale),
                 "the output has the rows' type, or is e4m3 with a scale array");
+        check_waits(a.device);
         if (a.rows == 0) return;
         require(a.x && a.y, "null argument");
         require_aligned({a.x, a.residual, a.h}, dtype_bytes(a.dtype));
@@ -792,6 +793,7 @@ int rune_rms_norm_backward(const rune_norm_grad_args* args, void* stream_) {
     auto stream = static_cast<cudaStream_t>(stream_);
     return guarded(a.device, [&] {
         check_norm_grad(a);
+        check_waits(a.device);
         const int64_t need = norm_grad_workspace(a);
         require(a.workspace_bytes >= need && (need == 0 || aligned(a.workspace, 256)),
                 "the workspace is too small or not 256-byte aligned");

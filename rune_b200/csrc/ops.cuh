@@ -64,6 +64,9 @@ inline void require_aligned(std::initializer_list<const void*> arrays, size_t by
 
 int sm_count(int device);
 
+// Throws, once, if a wait of an operator's kernel on the device gave up. Every entry calls it.
+void check_waits(int device);
+
 // Launches an operator's kernel so that it may begin while the one before it in the stream ends
 // (programmatic dependent launch): its prologue and the launch itself are hidden, and follow_on()
 // in the kernel holds back everything that touches memory. cluster: blocks of one, or 0.

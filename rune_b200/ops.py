@@ -9,6 +9,7 @@ CUDA tensors, for training, distilling or serving networks beside the engine's f
 * ``gated_linear``: ``act(x Wg^T + bg) * (x Wu^T + bu)`` in one kernel.
 * ``padded``: a copy of a matrix whose rows start on 16 bytes each, for weights of odd widths.
 * ``quantize_fp8``: rows to e4m3 with a scale per row (weights once, activations per call).
+* ``check_waits``: whether a kernel of these gave up waiting, where no operator call follows.
 
 Every function works on the last axis of its input, takes row-strided views, runs on the current
 stream of the tensors' device without synchronising it, and returns new tensors. Wrong types,
@@ -28,7 +29,7 @@ import torch
 from .runtime import library as L
 from .runtime.build import BINDING
 
-__all__ = ["gated_linear", "linear", "padded", "quantize_fp8", "rms_norm", "rms_norm_fp8"]
+__all__ = ["check_waits", "gated_linear", "linear", "padded", "quantize_fp8", "rms_norm", "rms_norm_fp8"]
 
 _ACTS = {None: L.RUNE_ACT_NONE, **L.RUNE_ACT}
 _OUT = {None: -1, torch.float16: L.RUNE_F16, torch.bfloat16: L.RUNE_BF16}
@@ -63,6 +64,20 @@ def _native():
                     RECOMPUTE_INPUTS)
         _BINDING = module
     return _BINDING
+
+
+def check_waits(device=None):
+    """Raise ``RuneError`` if a linear kernel's bounded wait gave up on the CUDA device (default:
+    the current one) since the last report; the results of that call are invalid.
+
+    Every operator call reports it too. This is for results that no call follows and for replayed
+    CUDA graphs, after a synchronisation.
+    """
+    index = torch.cuda.current_device() if device is None else torch.device(device).index
+    if index is None:
+        index = torch.cuda.current_device()
+    lib = L.load_library()
+    L.check(lib, lib.rune_linear_check_waits(index))
 
 
 def _activation(name):

@@ -48,6 +48,7 @@ EXPORTED = [
     "rune_rms_norm", "rune_rms_norm_backward", "rune_rms_norm_backward_workspace",
     "rune_linear", "rune_linear_workspace", "rune_linear_backward",
     "rune_linear_backward_workspace", "rune_pad_rows", "rune_linear_set_wait_polls",
+    "rune_linear_check_waits",
 ]
 
 
@@ -189,6 +190,7 @@ def load_library(path: Path | None = None):
     lib.rune_tc_selftest.argtypes = [c_int32, c_int32, c_int32, POINTER(c_float),
                                      POINTER(c_float), POINTER(c_float), c_int32]
     lib.rune_linear_set_wait_polls.argtypes = [c_uint32]
+    lib.rune_linear_check_waits.argtypes = [c_int32]
     lib.rune_pad_rows.argtypes = [c_int32, c_int64, c_int64, c_int64, c_void_p, c_int64,
                                   c_void_p, c_void_p]
     for name, args in (("rune_rms_norm", NormArgs), ("rune_rms_norm_backward", NormGradArgs),

@@ -77,6 +77,44 @@ def test_tiles_give_up_with_copies_and_products_in_flight(rows, inputs, outputs,
                 assert torch.equal(a, b), polls
 
 
+@gpu
+def test_every_operator_reports_a_wait_that_gave_up():
+    x, w = normal(41, 300, 640), normal(42, 512, 640, scale=0.1)
+    want = ops.linear(x, w)
+    leaf = x.clone().requires_grad_(True)
+    y, z = ops.rms_norm(leaf, w[0]), ops.linear(leaf, w)
+    for call in (lambda: ops.rms_norm(x, w[0]), lambda: ops.rms_norm_fp8(x, w[0]),
+                 lambda: ops.quantize_fp8(x), lambda: ops.padded(x), lambda: ops.linear(x, w),
+                 lambda: ops.rms_norm(x[:0], w[0]), lambda: ops.linear(x[:0], w),
+                 lambda: torch.autograd.grad(y.sum(), leaf, retain_graph=True),
+                 lambda: torch.autograd.grad(z.sum(), leaf, retain_graph=True),
+                 ops.check_waits, lambda: ops.check_waits("cuda"), lambda: ops.check_waits("cuda:0")):
+        give_up_after(0, lambda: ops.linear(x, w))
+        with pytest.raises(RuntimeError, match="did not complete in time"):
+            call()
+        call()  # reported once
+        assert torch.equal(ops.linear(x, w), want)
+
+
+@gpu
+def test_a_replayed_graph_reports_a_wait_that_gave_up():
+    x, w = normal(43, 300, 640), normal(44, 512, 640, scale=0.1)
+    ops.linear(x, w)
+    graph = torch.cuda.CUDAGraph()
+
+    def capture():
+        with torch.cuda.graph(graph):
+            ops.linear(x, w)
+
+    give_up_after(0, capture)  # the bound is the launch's
+    ops.check_waits()
+    graph.replay()
+    torch.cuda.synchronize()
+    with pytest.raises(L.RuneError, match="did not complete in time"):
+        ops.check_waits()
+    ops.check_waits()
+
+
 # ---------------------------------------------------------------------------------- tiny values
 def check_rows_in_8_bits(q, scale, y, slack):
     """q * scale against y (float64): scale within `slack` of its definition, each value within
