@@ -70,11 +70,9 @@ class ScalarNetwork(nn.Module):
         return ops.linear(q, weight, bias=bias, residual=embedding)
 
     def _finish(self, stream, delta, types):
-        eps, weight = self.norm_eps, self.output_norm.weight
-        h = (ops.rms_norm(stream, weight, eps=eps) if delta is None
-             else ops.rms_norm(delta, weight, residual=stream, eps=eps)[0])
         head = self.energy_heads
-        return (h.float() * head.weight[types]).sum(-1) + head.bias[types]
+        return _energies(stream, delta, types, self.norm_eps, self.output_norm.weight,
+                         head.weight, head.bias)
 
     def forward(self, descriptors, types):
         stream, delta = self._start(descriptors, types), None
@@ -94,37 +92,54 @@ class ScalarNetwork(nn.Module):
         return self._finish(stream, delta, types)
 
     def quantized(self):
-        """A function like ``forward`` with the blocks' products in 8 bits, weights laid out now."""
-        with torch.no_grad():
-            layers = []
-            for block in self.residual_blocks:
-                pair = []
-                for layer in (block.ffn[0], block.ffn[2]):
-                    w, scale = ops.quantize_fp8(layer.weight)
-                    pair.append((w, scale, layer.bias.to(self.dtype)))
-                layers.append((block.norm.weight.detach().clone(), *pair))
-        return _Quantized(self, layers)
+        """A function like ``forward`` with the blocks' products in 8 bits: a copy of the network
+        as it is now, its weights laid out; later changes of the network do not reach it."""
+        return _Quantized(self)
+
+
+def _energies(stream, delta, types, eps, norm_weight, head_weight, head_bias):
+    """Output normalisation of stream (+ delta) and the elements' head."""
+    h = (ops.rms_norm(stream, norm_weight, eps=eps) if delta is None
+         else ops.rms_norm(delta, norm_weight, residual=stream, eps=eps)[0])
+    return (h.float() * head_weight[types]).sum(-1) + head_bias[types]
 
 
 class _Quantized:
     """Forward of a ``ScalarNetwork`` whose blocks read e4m3 weights and activations."""
 
-    def __init__(self, net, layers):
-        self.net, self.layers = net, layers
+    @torch.no_grad()
+    def __init__(self, net):
+        def copy(t, dtype=None):
+            return t.detach().to(dtype or t.dtype, copy=True)
+
+        self.activation, self.gated, self.dtype = net.activation, net.gated, net.dtype
+        self.norm_eps = net.norm_eps
+        self.q_scaler = copy(net.q_scaler)
+        self.projection = [copy(t, net.dtype) for t in (net.input_projection.weight,
+                                                        net.input_projection.bias)]
+        self.embedding = copy(net.element_embedding.weight, net.dtype)
+        self.ends = [copy(t) for t in (net.output_norm.weight, net.energy_heads.weight,
+                                       net.energy_heads.bias)]
+        self.layers = [(copy(block.norm.weight),
+                        *((*ops.quantize_fp8(layer.weight), copy(layer.bias, net.dtype))
+                          for layer in (block.ffn[0], block.ffn[2])))
+                       for block in net.residual_blocks]
 
     @torch.no_grad()
     def __call__(self, descriptors, types):
-        net, delta = self.net, None
-        first = ops.gated_linear if net.gated else ops.linear
-        more = {"out_dtype": net.dtype}
-        stream = net._start(descriptors, types)
+        delta = None
+        first = ops.gated_linear if self.gated else ops.linear
+        more = {"out_dtype": self.dtype}
+        weight, bias = self.projection
+        stream = ops.linear((descriptors * self.q_scaler).to(self.dtype), weight, bias=bias,
+                            residual=self.embedding[types])
         for norm, (w0, s0, b0), (w1, s1, b1) in self.layers:
             if delta is None:
-                x, sx = ops.rms_norm_fp8(stream, norm, eps=net.norm_eps)
+                x, sx = ops.rms_norm_fp8(stream, norm, eps=self.norm_eps)
             else:
-                x, sx, stream = ops.rms_norm_fp8(delta, norm, residual=stream, eps=net.norm_eps)
-            x = first(x, w0, bias=b0, activation=net.activation, x_scale=sx, weight_scale=s0,
+                x, sx, stream = ops.rms_norm_fp8(delta, norm, residual=stream, eps=self.norm_eps)
+            x = first(x, w0, bias=b0, activation=self.activation, x_scale=sx, weight_scale=s0,
                       **more)
             x, sx = ops.quantize_fp8(x)
             delta = ops.linear(x, w1, bias=b1, x_scale=sx, weight_scale=s1, **more)
-        return net._finish(stream, delta, types)
+        return _energies(stream, delta, types, self.norm_eps, *self.ends)

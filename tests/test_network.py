@@ -152,6 +152,24 @@ def test_embedding_gradient_of_many_atoms(dtype, unit):
     assert float((got - want).abs().max()) <= 0.02 * float(want.abs().max())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("stored", [torch.float32, torch.bfloat16])
+def test_the_8_bit_network_is_a_copy(gated, stored):
+    """of every parameter and buffer, also where their type is the states' already"""
+    torch.manual_seed(6)
+    net = ScalarNetwork(3, 40, 64, 96, 2, activation="gelu", gated=gated).cuda().to(stored)
+    q = torch.randn(100, 40, device="cuda")
+    types = torch.randint(0, 3, (100,), device="cuda")
+    serve = net.quantized()
+    before = serve(q, types)
+    with torch.no_grad():
+        for t in (*net.parameters(), *net.buffers()):
+            t.mul_(1.5).add_(0.25)
+    assert torch.equal(serve(q, types), before)
+    assert not torch.equal(net.quantized()(q, types), before)
+
+
 class _Live:
     """detach().double() of a float64 leaf that is to keep its gradient."""
 
