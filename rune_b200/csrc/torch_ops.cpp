@@ -13,6 +13,7 @@
 #include <c10/core/AutogradState.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -51,6 +52,31 @@ struct Failure : std::runtime_error {
 };
 void check(int status) {
     if (status != RUNE_OK) throw Failure(status, api.last_error());
+}
+
+// Sets Python's exception for e. With the interpreter's lock.
+void set_python_error(const Failure& e) {
+    if (g_raise) {
+        PyObject* r = PyObject_CallFunction(g_raise, "is", e.status, e.what());
+        Py_XDECREF(r);
+    }
+    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
+}
+
+// A node's backward on one of autograd's threads: its Failure goes to the caller of backward() as
+// the same Python exception, which torch carries over, instead of a plain RuntimeError.
+template <typename Fn>
+variable_list in_backward(Fn&& fn) {
+    try {
+        return fn();
+    } catch (const Failure& e) {
+        const PyGILState_STATE lock = PyGILState_Ensure();
+        set_python_error(e);
+        python_error carried;
+        carried.persist();
+        PyGILState_Release(lock);
+        throw carried;
+    }
 }
 
 template <typename... Parts>
@@ -202,6 +228,9 @@ struct NormFn : torch::autograd::Function<NormFn> {
         return {o.y};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        return in_backward([&] { return gradients(ctx, grads); });
+    }
+    static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
         first_order_only(grads);
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &weight = saved[1], &residual = saved[2];
@@ -314,6 +343,9 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
         return o.y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        return in_backward([&] { return gradients(ctx, grads); });
+    }
+    static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
         first_order_only(grads);
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2];
@@ -411,11 +443,7 @@ PyObject* guarded(Fn&& fn) {
     try {
         return fn();
     } catch (const Failure& e) {
-        if (g_raise) {
-            PyObject* r = PyObject_CallFunction(g_raise, "is", e.status, e.what());
-            Py_XDECREF(r);
-        }
-        if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
+        set_python_error(e);
     } catch (const std::invalid_argument& e) {
         PyErr_SetString(PyExc_ValueError, e.what());
     } catch (const c10::OutOfMemoryError& e) {

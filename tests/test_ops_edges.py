@@ -115,6 +115,21 @@ def test_a_replayed_graph_reports_a_wait_that_gave_up():
     ops.check_waits()
 
 
+@gpu
+@pytest.mark.parametrize("layer", ["norm", "linear", "gated"])
+def test_a_failure_inside_a_backward_keeps_its_exception(layer):
+    x, w = normal(45, 300, 640).requires_grad_(True), normal(46, 512, 640, scale=0.1)
+    y = {"norm": lambda: ops.rms_norm(x, w[0]), "linear": lambda: ops.linear(x, w),
+         "gated": lambda: ops.gated_linear(x, w)}[layer]()
+    for run in (lambda: torch.autograd.grad(y.sum(), x, retain_graph=True),
+                lambda: y.sum().backward(retain_graph=True)):
+        give_up_after(0, lambda: ops.linear(x.detach(), w))
+        with pytest.raises(L.RuneError, match="did not complete in time"):
+            run()
+        run()
+    assert bool(x.grad.isfinite().all())
+
+
 # ---------------------------------------------------------------------------------- tiny values
 def check_rows_in_8_bits(q, scale, y, slack):
     """q * scale against y (float64): scale within `slack` of its definition, each value within
