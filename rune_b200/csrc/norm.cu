@@ -631,7 +631,7 @@ void launch_norm(const rune_norm_args& a, cudaStream_t stream) {
 
 // shared memory of the backward's slots for one row ahead
 template <typename T>
-size_t slots_bytes(int threads) { return (size_t)threads * 4 * kEpt * sizeof(T); }
+constexpr size_t slots_bytes(int threads) { return (size_t)threads * 4 * kEpt * sizeof(T); }
 
 // rows of partials for dweight
 template <typename T>
@@ -655,21 +655,34 @@ int64_t launch_norm_bwd(const rune_norm_grad_args& a, float* partials, cudaStrea
             const int n = block ? threads : 256;
             // rows ahead: kBlockThreads threads' slots have to fit an SM
             constexpr int kAheadBlock = sizeof(T) == 2 ? 3 : 1;
-            auto go = [&](auto kernel, int ahead) {
-                const size_t smem =
-                    std::max(ahead * slots_bytes<T>(n), block ? 0 : 8 * a.width * sizeof(float));
-                if (smem > 48 * 1024)
-                    RUNE_CUDA_TRY(cudaFuncSetAttribute(
-                        kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            constexpr int kAheadWarp = sizeof(T) == 2 ? 4 : 2;
+            auto go = [&](auto block_c, auto ahead_c) {
+                constexpr bool BLOCK = decltype(block_c)::value;
+                constexpr int AHEAD = decltype(ahead_c)::value;
+                constexpr auto kernel = k_norm_bwd<T, ACC, BLOCK, AHEAD>;
+                const size_t smem = std::max(AHEAD * slots_bytes<T>(n),
+                                             BLOCK ? 0 : 8 * a.width * sizeof(float));
+                constexpr size_t kMost = AHEAD * slots_bytes<T>(BLOCK ? 1024 : 256);
+                if constexpr (kMost > 48 * 1024) {
+                    // the largest that any width takes, once: a limit of this call's own size could
+                    // be lowered by another thread's narrower call before this one's launch
+                    static std::atomic<uint64_t> allowed{0};  // devices whose limit is raised
+                    if (a.device >= 64 ||
+                        !(allowed.load(std::memory_order_relaxed) >> a.device & 1)) {
+                        RUNE_CUDA_TRY(cudaFuncSetAttribute(
+                            kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMost));
+                        if (a.device < 64)
+                            allowed.fetch_or(uint64_t(1) << a.device, std::memory_order_relaxed);
+                    }
+                }
                 launch(kernel, (int)blocks, n, smem, 0, stream, a, partials);
             };
-            if constexpr (ACC == kWhole) {
-                if (block) go(k_norm_bwd<T, ACC, true, kAheadBlock>, kAheadBlock);
-                else go(k_norm_bwd<T, ACC, false, sizeof(T) == 2 ? 4 : 2>, sizeof(T) == 2 ? 4 : 2);
-            } else {
-                if (block) go(k_norm_bwd<T, ACC, true, 0>, 0);
-                else go(k_norm_bwd<T, ACC, false, 0>, 0);
-            }
+            using std::integral_constant;
+            constexpr bool kSlots = ACC == kWhole;
+            if (block)
+                go(std::true_type(), integral_constant<int, kSlots ? kAheadBlock : 0>());
+            else
+                go(std::false_type(), integral_constant<int, kSlots ? kAheadWarp : 0>());
         }
     });
     return blocks;

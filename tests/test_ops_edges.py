@@ -5,6 +5,7 @@ Bounds are derived from the roundings, as in test_ops.py."""
 from __future__ import annotations
 
 import ctypes
+import threading
 
 import pytest
 import torch
@@ -289,3 +290,39 @@ def test_scales_that_require_a_gradient_are_refused(layer):
             layer(x, w, x_scale=scales[0], weight_scale=scales[1])
         with torch.no_grad():
             assert torch.equal(layer(x, w, x_scale=scales[0], weight_scale=scales[1]), want)
+
+
+# ------------------------------------------------------------------------------------- threads
+@gpu
+@pytest.mark.parametrize("dtype,code", [(torch.bfloat16, L.RUNE_BF16), (torch.float32, L.RUNE_F32)])
+def test_two_threads_with_different_widths(dtype, code):
+    """The norm's backward through the C entry, which holds no lock: each call's shared memory is
+    allowed whatever the other thread's calls need."""
+    lib = L.load_library()
+    failures, results = [], {}
+
+    def work(width, stream):
+        x, dy = normal(51, 64, width, dtype=dtype), normal(52, 64, width, dtype=dtype)
+        w, rstd = normal(53, width, dtype=dtype), torch.ones(64, device="cuda")
+        dx, first = torch.empty_like(x), None
+        args = L.NormGradArgs(rows=64, width=width, x_stride=width, dy_stride=width, dtype=code,
+                              weight_dtype=code, x=x.data_ptr(), weight=w.data_ptr(),
+                              rstd=rstd.data_ptr(), dy=dy.data_ptr(), dx=dx.data_ptr())
+        torch.cuda.synchronize()
+        for i in range(2000):
+            status = lib.rune_rms_norm_backward(ctypes.byref(args), stream.cuda_stream)
+            if status:
+                failures.append((width, status, lib.rune_last_error()))
+            if i == 0:
+                stream.synchronize()
+                first = dx.clone()
+        stream.synchronize()
+        results[width] = torch.equal(first, dx)
+
+    threads = [threading.Thread(target=work, args=(width, torch.cuda.Stream()))
+               for width in (4096, 8192)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures and results == {4096: True, 8192: True}, failures[:2]
