@@ -248,18 +248,23 @@ __device__ __forceinline__ Two by_sign(Two s, Two a, Two b) {
 
 constexpr float kLog2E = 1.44269504088896f;
 
-// tanh x = 1 - 2 / (1 + e^2x); near zero, where that cancels, its Taylor series to x^7
-// (next term 62/2835 x^9: 3e-7 of the value at 1/4).
-__device__ __forceinline__ Two tanh_two(Two x) {
-    Two t = fma(two(-2.0f), rcp(ex2(x * two(2.0f * kLog2E)) + two(1.0f)), two(1.0f));
+// tanh |x| = 1 - 2 E / (1 + E) with E = e^(-2 |x|); near zero, where that cancels, its Taylor series
+// to x^7 (next term 62/2835 x^9: 3e-7 of the value at 1/4). Its derivative is 4 E / (1 + E)^2, which
+// keeps its digits where 1 - tanh^2 cancels.
+__device__ __forceinline__ Two tanh_two(Two x, Two& d) {
+    Two e = ex2(each(x, [](float v) { return fabsf(v); }) * two(-2.0f * kLog2E));
+    Two r = rcp(e + two(1.0f)), er = e * r;
+    Two t = fma(er, two(-2.0f), two(1.0f));
+    d = er * r * two(4.0f);
     Two q = x * x;
     Two s = fma(fma(fma(q, two(-17.0f / 315.0f), two(2.0f / 15.0f)), q, two(-1.0f / 3.0f)) * q, x,
                 x);
-    float q0, q1, t0, t1, s0, s1;
+    float x0, x1, q0, q1, t0, t1, s0, s1;
+    split(x, x0, x1);
     split(q, q0, q1);
     split(t, t0, t1);
     split(s, s0, s1);
-    return two(q0 < 0.0625f ? s0 : t0, q1 < 0.0625f ? s1 : t1);
+    return two(q0 < 0.0625f ? s0 : copysignf(t0, x0), q1 < 0.0625f ? s1 : copysignf(t1, x1));
 }
 
 // Upper tail Q(|x|) = 1 - Phi(|x|) of the normal distribution and e^(-x^2 / 2). erfc by the
@@ -279,7 +284,8 @@ __device__ __forceinline__ Two normal_tail(Two x, Two& e) {
 template <int ACT>
 __device__ __forceinline__ Two act_value(Two x) {
     if constexpr (ACT == RUNE_ACT_TANH) {
-        return tanh_two(x);
+        Two d;
+        return tanh_two(x, d);
     } else if constexpr (ACT == RUNE_ACT_SILU) {
         return x * rcp(ex2(x * two(-kLog2E)) + two(1.0f));
     } else if constexpr (ACT == RUNE_ACT_GELU) {
@@ -294,8 +300,7 @@ __device__ __forceinline__ Two act_value(Two x) {
 template <int ACT>
 __device__ __forceinline__ void act_both(Two x, Two& y, Two& dy) {
     if constexpr (ACT == RUNE_ACT_TANH) {
-        y = tanh_two(x);
-        dy = fma(y * two(-1.0f), y, two(1.0f));
+        y = tanh_two(x, dy);
     } else if constexpr (ACT == RUNE_ACT_SILU) {
         Two s = rcp(ex2(x * two(-kLog2E)) + two(1.0f));
         y = x * s;

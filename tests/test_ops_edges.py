@@ -5,6 +5,7 @@ Bounds are derived from the roundings, as in test_ops.py."""
 from __future__ import annotations
 
 import ctypes
+import math
 import threading
 
 import pytest
@@ -12,7 +13,7 @@ import torch
 
 from rune_b200 import ops
 from rune_b200.runtime import library as L
-from tests.test_ops import normal
+from tests.test_ops import FUNC, U, normal, within
 
 gpu = pytest.mark.gpu
 
@@ -182,6 +183,53 @@ def test_norm_of_tiny_values_to_8_bits(width, tiny_weight):
     if not tiny_weight:  # of a row's largest value
         slack += float((2.0 ** -149 * eps ** -0.5 / y.abs().amax(-1)).max())
     check_rows_in_8_bits(*ops.rms_norm_fp8(x, w, eps=eps), y, slack)
+
+
+# --------------------------------------------------------------------------------- activations
+def activation64(kind, z):
+    """value, derivative and the sum of the derivative's terms' magnitudes, without cancellation"""
+    if kind == "tanh":
+        d = torch.cosh(z) ** -2
+        return torch.tanh(z), d, d
+    if kind == "silu":
+        s = torch.sigmoid(z)
+        rest = torch.sigmoid(-z)
+        return z * s, s * (1 + z * rest), s * (1 + z.abs() * rest)
+    cdf = 0.5 * torch.special.erfc(-z / math.sqrt(2.0))
+    density = torch.exp(-0.5 * z * z) / math.sqrt(2.0 * math.pi)
+    return z * cdf, cdf + z * density, cdf + z.abs() * density
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("act", ["tanh", "silu"])
+@pytest.mark.parametrize("inputs", [8, 1032])  # z recomputed, z saved
+@pytest.mark.parametrize("rows", [48, 4001])   # few rows, tiles
+@pytest.mark.parametrize("gated", [False, True])
+def test_activations_to_their_tails(act, dtype, inputs, rows, gated):
+    """Each output is the activation of one exact z in -10 .. 10 (times 1 in the gated layer): off by
+    its rounding and 4e-6, and z^2 2^-23 for the argument of an exponential, of itself; its
+    derivative by as much of its terms."""
+    z = torch.linspace(-10.0, 10.0, rows, device="cuda").to(dtype)
+    x = torch.zeros(rows, inputs, dtype=dtype, device="cuda")
+    x[:, 0] = z
+    x.requires_grad_(True)
+    w = torch.zeros(16, inputs, dtype=dtype, device="cuda")
+    w[:8, 0] = 1.0
+    if gated:
+        b = torch.zeros(16, dtype=dtype, device="cuda")
+        b[8:] = 1.0
+        y = ops.gated_linear(x, w, bias=b, activation=act)
+    else:
+        y = ops.linear(x, w, activation=act)
+    dy = torch.zeros_like(y)
+    dy[:, 3] = 1.0
+    (dx,) = torch.autograd.grad(y, x, dy)
+    z = z.double()
+    value, slope, terms = activation64(act, z)
+    func = FUNC + 2.0 ** -23 * z * z
+    within(y[:, 3].detach(), value, (U[dtype] + func) * value.abs(), "value")
+    within(dx[:, 0], slope, U[dtype] * slope.abs() + (1 + U[dtype]) * func * terms, "derivative")
 
 
 # ---------------------------------------------------------------------------------- transforms
