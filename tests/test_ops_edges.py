@@ -202,7 +202,7 @@ def activation64(kind, z):
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
-@pytest.mark.parametrize("act", ["tanh", "silu"])
+@pytest.mark.parametrize("act", ["tanh", "silu", "gelu"])
 @pytest.mark.parametrize("inputs", [8, 1032])  # z recomputed, z saved
 @pytest.mark.parametrize("rows", [48, 4001])   # few rows, tiles
 @pytest.mark.parametrize("gated", [False, True])
