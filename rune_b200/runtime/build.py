@@ -18,6 +18,7 @@ LIB_DIR = PKG / "_lib"
 LIB = LIB_DIR / "librune_b200.so"
 BINDING = LIB_DIR / "_ops.so"
 BINDING_SOURCE = CSRC / "torch_ops.cpp"
+BINDING_STAMP = LIB_DIR / "obj" / "_ops.txt"  # what BINDING was built with
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -76,13 +77,27 @@ def _binding_command(out: Path) -> list[str]:
             "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
 
 
+def _binding_stamp() -> str:
+    """The versions and the command that a binding depends on beside its sources."""
+    import torch
+
+    return "\n".join([f"torch {torch.__version__}", f"python {sys.version}",
+                      *_binding_command(BINDING)])
+
+
+def binding_stale() -> bool:
+    if not BINDING.exists() or not BINDING_STAMP.exists():
+        return True
+    header = PKG.parent / "include" / "rune_b200.h"
+    newest = max(p.stat().st_mtime for p in (BINDING_SOURCE, header))
+    return BINDING.stat().st_mtime < newest or BINDING_STAMP.read_text() != _binding_stamp()
+
+
 def build_binding(force: bool = False, verbose: bool = False) -> Path:
     """The operators' binding to torch (CPython module ``_ops``, host code only)."""
-    header = PKG.parent / "include" / "rune_b200.h"
-    if not force and BINDING.exists() and BINDING.stat().st_mtime >= max(
-            p.stat().st_mtime for p in (BINDING_SOURCE, header)):
+    if not force and not binding_stale():
         return BINDING
-    LIB_DIR.mkdir(parents=True, exist_ok=True)
+    BINDING_STAMP.parent.mkdir(parents=True, exist_ok=True)
     tmp = BINDING.with_suffix(".so.tmp")
     cmd = _binding_command(tmp)
     if verbose:
@@ -91,6 +106,7 @@ def build_binding(force: bool = False, verbose: bool = False) -> Path:
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed: {res.stdout}{res.stderr}")
     os.replace(tmp, BINDING)
+    BINDING_STAMP.write_text(_binding_stamp())
     return BINDING
 
 

@@ -374,3 +374,27 @@ def test_two_threads_with_different_widths(dtype, code):
     for t in threads:
         t.join()
     assert not failures and results == {4096: True, 8192: True}, failures[:2]
+
+
+# --------------------------------------------------------------------------------------- build
+def test_the_binding_is_stale_under_another_torch(tmp_path, monkeypatch):
+    """Its ABI is torch's and Python's; the sources' times alone do not show a new one."""
+    from rune_b200.runtime import build
+
+    binding, stamp = tmp_path / "_ops.so", tmp_path / "obj" / "_ops.txt"
+    monkeypatch.setattr(build, "BINDING", binding)
+    monkeypatch.setattr(build, "BINDING_STAMP", stamp)
+    commands = []
+
+    def compile_(cmd, **_):
+        commands.append(cmd)
+        open(cmd[cmd.index("-o") + 1], "w").close()
+        return type("Done", (), {"returncode": 0})
+
+    monkeypatch.setattr(build.subprocess, "run", compile_)
+    assert build.build_binding() == binding and len(commands) == 1
+    assert build.build_binding() == binding and len(commands) == 1
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    assert build.binding_stale()
+    assert build.build_binding() == binding and len(commands) == 2
+    assert not build.binding_stale()
