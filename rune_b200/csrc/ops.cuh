@@ -1,4 +1,4 @@
-// Shared pieces of the mixed-precision network operators (norm.cu, linear.cu): typed vector
+// Shared pieces of the mixed-precision network operators (norm.cu, linear.cu): typed
 // access, activations for 16-bit results, host-side argument checks.
 #pragma once
 
@@ -143,37 +143,6 @@ __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
 template <>
 __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-}
-
-// VEC consecutive values at p as floats: one 16-byte access where VEC fills it, else one value
-template <typename T, int VEC>
-__device__ __forceinline__ void load_vec(const T* p, float* v) {
-    if constexpr (VEC == 1) {
-        v[0] = to_float(*p);
-    } else if constexpr (sizeof(T) == 4) {
-        float4 q = *reinterpret_cast<const float4*>(p);
-        v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
-    } else {
-        uint4 q = *reinterpret_cast<const uint4*>(p);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float2 f = unpack2<T>(w[i]);
-            v[2 * i] = f.x, v[2 * i + 1] = f.y;
-        }
-    }
-}
-
-template <typename T, int VEC>
-__device__ __forceinline__ void store_vec(T* p, const float* v) {
-    if constexpr (VEC == 1) {
-        *p = from_float<T>(v[0]);
-    } else if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    } else {
-        *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]),
-                                                  pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
-    }
 }
 
 // maximum that keeps a NaN
