@@ -13,7 +13,8 @@ import torch
 
 from rune_b200 import ops
 from rune_b200.runtime import library as L
-from tests.test_ops import FUNC, U, normal, within
+from tests.test_ops import (FUNC, U, act64, act_err, normal, products64, rounded, within,
+                            z64)
 
 gpu = pytest.mark.gpu
 
@@ -398,3 +399,105 @@ def test_the_binding_is_stale_under_another_torch(tmp_path, monkeypatch):
     assert build.binding_stale()
     assert build.build_binding() == binding and len(commands) == 2
     assert not build.binding_stale()
+
+
+# ------------------------------------------------------------- sums that keep their digits
+def cancelling(dy, first, second):
+    """dy for even rows, and for odd ones the 16-bit values that cancel dy * first in a sum with
+    second to a rounding of them: what is left is gone if a factor of a term is rounded again"""
+    return torch.stack([dy, -(dy.double() * first / second).to(dy.dtype)])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("width", [64, 264, 1001])
+def test_norm_gradients_use_both_addends_unrounded(width, dtype):
+    """h = x + residual has more digits than 16 bits. dweight: two kinds of rows whose terms cancel
+    to a rounding's size; off by float32's errors of r, n and the sums, and its own rounding. dx:
+    dy along n, which the projection cancels to a rounding's size likewise."""
+    rows, eps = 512, 1e-6
+    f = (width + 16) * 2.0 ** -23
+    base = [normal(61 + i, 2, width, dtype=dtype, scale=s) for i, s in enumerate((1.0, 0.3))]
+    base = [t + torch.sign(t) * (0.5 if i == 0 else 0.0) for i, t in enumerate(base)]
+    pair = base[0].double() + base[1].double()
+    n2 = pair / torch.sqrt((pair * pair).mean(-1, keepdim=True) + eps)
+    x, res = (t.repeat(rows // 2, 1).requires_grad_(True) for t in base)
+    w = torch.ones(width, dtype=dtype, device="cuda", requires_grad=True)
+    dy = cancelling(normal(64, width, dtype=dtype), n2[0], n2[1]).repeat(rows // 2, 1)
+    y, _ = ops.rms_norm(x, w, residual=res, eps=eps)
+    (dw,) = torch.autograd.grad(y, w, dy, retain_graph=True)
+    term = dy.double() * n2.repeat(rows // 2, 1)
+    ok = term.abs().amax(0).isfinite()
+    want, size = term.sum(0), term.abs().sum(0)
+    within(dw[ok], want[ok], ((f + rows * 2.0 ** -24) * size + U[dtype] * want.abs())[ok], "dweight")
+    n = n2.repeat(rows // 2, 1)
+    dy = n.to(dtype)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    r = 1.0 / torch.sqrt((pair * pair).mean(-1, keepdim=True) + eps).repeat(rows // 2, 1)
+    dot = (dy.double() * n).mean(-1, keepdim=True)
+    want = r * (dy.double() - n * dot)
+    within(dx, want, U[dtype] * want.abs() + 4 * f * r * (dy.double().abs() + (n * dot).abs()), "dx")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("inputs", [8, 1032])  # z recomputed, z saved
+@pytest.mark.parametrize("act", ["tanh", "silu", "gelu"])
+@pytest.mark.parametrize("gated", [False, True])
+def test_dbias_sums_unrounded_dz(inputs, act, dtype, gated):
+    """Two kinds of rows whose dz cancel to a rounding's size in every column; z is exact. Off by
+    the activation's error of each term, float32 sums in a tree of fewer than 40 additions, and
+    the sum's own rounding."""
+    rows, outputs = 2000, 24
+    x = torch.zeros(rows, inputs, dtype=dtype, device="cuda")
+    x[0::2, 0], x[1::2, 0] = 0.75, 0.34375
+    w = torch.zeros(2 * outputs if gated else outputs, inputs, dtype=dtype, device="cuda")
+    w[:outputs, 0] = 0.5 + torch.rand(outputs, generator=torch.Generator().manual_seed(5)).cuda()
+    b = torch.zeros(len(w), dtype=dtype, device="cuda", requires_grad=True)
+    z = x[:2, :1].double() * w[:outputs, 0].double()
+    value, slope, terms = activation64(act, z)
+    up = 1.0
+    if gated:
+        w[outputs:, 0], up = 1.25, 1.25 * x[:2, :1].double()
+    dy = cancelling(normal(65, outputs, dtype=dtype), (slope * up)[0], (slope * up)[1])
+    y = (ops.gated_linear(x.requires_grad_(True), w, bias=b, activation=act) if gated
+         else ops.linear(x.requires_grad_(True), w, bias=b, activation=act))
+    (db,) = torch.autograd.grad(y, b, dy.repeat(rows // 2, 1))
+    dz = (dy.double() * up * slope).sum(0) * (rows // 2)
+    size = (dy.double().abs() * up * terms).sum(0) * (rows // 2)
+    func = FUNC + 2.0 ** -23 * float(z.abs().max()) ** 2 + 42 * 2.0 ** -24
+    within(db[:outputs], dz, U[dtype] * dz.abs() + func * size, "dbias")
+
+
+# ------------------------------------------------------------------------------- many tiles
+@gpu
+@pytest.mark.parametrize("rows,inputs,outputs", [(10000, 264, 600), (300, 4200, 5000),
+                                                 (6003, 1100, 1000)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_more_tiles_than_blocks_and_more_than_one_group(rows, inputs, outputs, gated):
+    """Every value of results and gradients whose products have more rows of tiles than a group and
+    more tiles than blocks at once."""
+    dtype, u = torch.bfloat16, U[torch.bfloat16]
+    x = normal(71, rows, inputs, dtype=dtype).requires_grad_(True)
+    w = normal(72, outputs, inputs, dtype=dtype, scale=inputs ** -0.5).requires_grad_(True)
+    b = normal(73, outputs, dtype=dtype, scale=0.5).requires_grad_(True)
+    half = outputs // 2 if gated else outputs
+    dy = normal(74, rows, half, dtype=dtype)
+    y = (ops.gated_linear(x, w, bias=b, activation="gelu") if gated
+         else ops.linear(x, w, bias=b, activation="gelu"))
+    grads = torch.autograd.grad(y, [x, w, b], dy)
+    z, ez = z64(x.detach(), w.detach(), b.detach())
+    g = dy.double()
+    gate, eg = z[:, :half], ez[:, :half]
+    a, da, _ = act64("gelu", gate)
+    ea, eda = act_err("gelu", gate, eg)
+    want, ey, dz, ddz = a, ea, g * da, g.abs() * eda
+    if gated:
+        up, eu = z[:, half:], ez[:, half:]
+        want, ey = a * up, ea * (up.abs() + eu) + a.abs() * eu
+        dz = torch.cat([g * up * da, g * a], 1)
+        ddz = torch.cat([g.abs() * (eda * (up.abs() + eu) + da.abs() * eu), g.abs() * ea], 1)
+    within(y.detach(), *rounded((want, ey + 2.0 ** -23 * want.abs()), u), "y")
+    pairs = products64(dz, ddz + 2.0 ** -22 * dz.abs(), x.detach(), w.detach(), u, rows)
+    for name, got, pair in zip(("dx", "dweight", "dbias"), grads, pairs):
+        within(got, *rounded(pair, u), name)
