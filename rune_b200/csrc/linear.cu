@@ -22,7 +22,7 @@
 // TFLOP/s; gated 4096 x 4096 -> 2 x 8192 338 us, 1624 TFLOP/s, the rate of a library product, and
 // under long load the power limit (390 us). Narrow layers of many rows are bound by the epilogue:
 // 110592 x 256 -> 512 35 us without activation (4.9 TB/s), 51 with silu, whose two special
-// functions a value take 27; gated 63. What it took to get there, each at the size named:
+// functions a value take 27; gated 64. What it took to get there, each at the size named:
 //   tensor-core instructions issued by a converged warp, one kind a kernel   8192 x 4096 -> 4096
 //     518 -> 232 us (from a divergent thread with both kinds they came at a third of the rate)
 //   pairs of blocks, half of B's shared-memory traffic                        232 -> 182 us

@@ -214,9 +214,15 @@ inline bool tma_ready(const Matrix& m, int elem_bytes) {
 // Tensor map of `m` with boxes of one 128-byte line x box_rows lines, zeros outside.
 CUtensorMap make_map(const Matrix& m, int elem_bytes, int box_rows);
 
-// Largest number of rows of x that linear_few takes. Measured on B200, bf16, against the 128-row
-// tiles: 16 rows x 4096 -> 8192 15.8 against 19.3 us, x 1024 -> 1024 5.3 against 8.0; 64 rows
-// 19.2 against 19.3 and 6.5 against 8.0, but x 256 -> 512 10.9 against 5.8.
+// Largest number of rows of x that linear_few takes. B200, bf16, us on the GPU with the weights in
+// L2, few rows / tiles at 1, 16, 32 and 48 rows:
+//   4096 -> 8192   9.6 / 31.2    9.3 / 16.3   10.6 / 16.4   11.8 / 16.4
+//   1024 -> 1024   4.0 / 6.5     4.2 / 6.6     4.3 / 6.6     5.4 / 6.6
+//    512 -> 256    3.8 / 4.9     3.8 / 5.0     4.8 / 5.0     5.7 / 5.0
+//    256 -> 512    3.6 / 3.9     4.8 / 4.0     6.4 / 4.0     8.1 / 4.0
+//   gated 4096 -> 2 x 8192  23.3 / 36.6  23.8 / 26.2  26.2 / 26.3  27.9 / 26.3
+//   gated  256 -> 2 x 512    4.6 / 4.7    4.7 / 4.8    6.4 / 4.9    8.0 / 4.9
+// The rule looks at rows alone: narrow layers of 16 to 48 rows lose by it, up to half.
 constexpr int kFewRows = 48;
 void linear_few(const rune_linear_args& a, const Matrix& x, const Matrix& w, cudaStream_t stream);
 

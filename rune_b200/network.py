@@ -3,9 +3,10 @@
 The engine evaluates Möbius models in float32 without parameter gradients. ``ScalarNetwork`` is
 the same per-atom network (rune/mobius/model.py:256-305 without messages, layers.py:26-89) on the
 operators of ``rune_b200.ops``: float32 parameters under the reference's names, 16-bit products
-with float32 accumulation, gradients for all of them. For adapting a checkpoint's network,
-distilling a model into it, or serving many atoms' energies from descriptors; ``quantized`` gives
-an 8-bit copy for serving.
+with float32 accumulation, gradients for all of them. For distilling a model into it, or for
+adapting a checkpoint's network and serving many atoms' energies where the caller has their
+descriptors (the engine computes its own inside the kernels and returns none); no forces.
+``quantized`` gives an 8-bit copy for serving.
 
 A block adds its output to the residual stream in the next block's normalisation, so the stream
 is read and written once per block.

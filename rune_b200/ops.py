@@ -15,7 +15,8 @@ Every function works on the last axis of its input, takes row-strided views, run
 stream of the tensors' device without synchronising it, and returns new tensors. Wrong types,
 shapes or devices raise ``ValueError``; failures of the GPU raise ``RuneError``. Gradients are
 reverse-mode and of first order; forward-mode tangents, function transforms and traces are refused
-(``RuntimeError``). Sums and statistics are float32; results are rounded once. Equal inputs give equal bits.
+(``RuntimeError``). Sums and statistics are float32. Results are rounded once, but dx and dweight of
+the layers are products of a dz that is rounded to 16 bits first. Equal inputs give equal bits.
 """
 
 from __future__ import annotations
