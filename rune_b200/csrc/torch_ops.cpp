@@ -444,6 +444,8 @@ PyObject* guarded(Fn&& fn) {
         return fn();
     } catch (const Failure& e) {
         set_python_error(e);
+    } catch (python_error& e) {  // raised in Python, by a hook on what a node saves
+        e.restore();
     } catch (const std::invalid_argument& e) {
         PyErr_SetString(PyExc_ValueError, e.what());
     } catch (const c10::OutOfMemoryError& e) {

@@ -286,6 +286,32 @@ def test_transforms_of_a_backward_are_refused():
         assert bool(backward(dy).isfinite().all())
 
 
+@gpu
+def test_hooks_on_saved_tensors_keep_their_exceptions():
+    """Activation checkpointing ends its recomputation by an exception in such a hook."""
+    from torch.utils.checkpoint import checkpoint
+
+    class Stop(Exception):
+        pass
+
+    def stop(_):
+        raise Stop("here")
+
+    w = normal(25, 64, 64)
+    for f in (lambda t: ops.linear(t, w, activation="gelu"), lambda t: ops.gated_linear(t, w),
+              lambda t: ops.rms_norm(t, w[0]),
+              lambda t: ops.linear(ops.rms_norm(t, w[0], residual=t)[1], w, residual=t)):
+        x = normal(24, 60, 64).requires_grad_(True)
+        with torch.autograd.graph.saved_tensors_hooks(stop, lambda t: t), pytest.raises(
+                Stop, match="here"):
+            f(x)
+        (want,) = torch.autograd.grad(f(x).sum(), x)
+        (got,) = torch.autograd.grad(checkpoint(f, x, use_reentrant=False).sum(), x)
+        assert torch.equal(got, want)
+        checkpoint(f, x, use_reentrant=True).sum().backward()
+        assert torch.equal(x.grad, want)
+
+
 # ------------------------------------------------------------------------------------ refusals
 def refused_at(name, args, fields, step):
     """rune_<name> refuses each field at an address `step` bytes off, and launches nothing"""
