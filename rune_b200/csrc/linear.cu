@@ -34,730 +34,12 @@
 #include <atomic>
 #include <mutex>
 
-#include "linear.cuh"
+#include "tile.cuh"
 
 namespace rune {
 namespace ops {
 
 namespace {
-
-enum Mode {
-    kForward,    // y = act(acc + bias) + residual, z saved on request
-    kGated,      // y = act(gate) * up; the tile's columns are half gate, half up
-    kGrad,       // dz = dy act'(acc + bias), column sums of dz
-    kGatedGrad,  // d gate = dy up act'(gate), d up = dy act(gate), column sums
-    kPartial     // float32 sums of one range of k
-};
-
-constexpr int kBM = 128;
-constexpr int kEpiWarps = 16, kTmaWarp = 16, kMmaWarp = 17;
-constexpr int kThreads = 32 * 18;
-constexpr uint32_t kAStage = kBM * kLineBytes;  // 16 KB
-constexpr uint32_t kRowBytes = 64;               // of a warp's buffer: 32 16-bit or 16 float values
-constexpr uint32_t kWarpBuf = 32 * kRowBytes;    // 2 KB
-constexpr int kMaxStages = 8;
-constexpr uint32_t kSmemMax = 227 * 1024;
-
-// Exact quotient of n < 2^31 by a divisor fixed for the launch: n * mul >> shift.
-struct Divisor {
-    unsigned by, mul, shift;
-    __device__ __forceinline__ unsigned quotient(unsigned n) const {
-        return (unsigned)(((uint64_t)n * mul) >> shift);
-    }
-};
-Divisor make_divisor(unsigned by) {
-    // with 2^L >= by, mul = ceil(2^(31 + L) / by) < 2^32 errs by less than n / 2^31 of a unit
-    unsigned l = 0;
-    while ((1ull << l) < by) ++l;
-    return {by, (unsigned)(((1ull << (31 + l)) + by - 1) / by), 31 + l};
-}
-
-struct TileParams {
-    int64_t m, n;           // rows and columns of the output (gated: columns of y)
-    int64_t ld_out, ld_in;
-    int64_t ld_z, ld_part;  // of z: rows, and within a row the parts (gate, up)
-    int kblocks, kb_per_split, splits;
-    int tiles_m, tiles_n, bn, stages;
-    Divisor by_tiles, by_group, by_last;  // tile_of's: all tiles, a group's, the last group's rows
-    int a_mn, b_mn, act;
-    int tma_out, vec_in, vec_bias;  // rows on 16 bytes: copies by TMA, 16-byte accesses
-    uint32_t idesc;
-    void* out;
-    const void* in;         // residual, or dy
-    const void* bias;
-    const float* x_scale;
-    const float* w_scale;
-    float* z;               // saved z, or the partial sums
-    float* colsum;          // [tiles_m * 4][n or 2n]
-    unsigned* flag;
-    unsigned polls;         // bound of every wait
-};
-
-struct TileShared {
-    unsigned long long full[kMaxStages], empty[kMaxStages];
-    unsigned long long acc_full[2], acc_empty[2], drained;
-    uint32_t tmem;
-    int fail;
-    int issued;             // stages whose copies were issued
-};
-
-// buffers of kWarpBuf per epilogue warp, and all shared memory beside the ring
-template <int MODE>
-constexpr uint32_t kWarpBufs = MODE == kGatedGrad ? 2 : 1;
-template <int MODE>
-constexpr uint32_t kFixedSmem =
-    kEpiWarps * kWarpBufs<MODE> * kWarpBuf + (uint32_t)((sizeof(TileShared) + 127) / 128 * 128);
-
-struct Tile {
-    int mt, nt, split;
-};
-
-// Tiles in groups of 16 tile rows, column by column, so that the blocks at work share a few
-// lines of both operands in L2; the ranges of k of one tile come last.
-constexpr unsigned kGroup = 16;
-__device__ __forceinline__ Tile tile_of(const TileParams& p, unsigned w) {
-    Tile t{0, 0, 0};
-    if (p.splits > 1) {
-        t.split = p.by_tiles.quotient(w);
-        w -= t.split * p.by_tiles.by;
-    }
-    const unsigned g = p.by_group.quotient(w), in = w - g * p.by_group.by;
-    const unsigned left = p.tiles_m - g * kGroup, rows = min(kGroup, left);
-    t.nt = left >= kGroup ? in / kGroup : p.by_last.quotient(in);
-    t.mt = g * kGroup + (in - t.nt * rows);
-    return t;
-}
-
-// ---- a warp's 32 rows x 32 columns of 16-bit values between global memory and its buffer.
-// Rows are four pieces of 16 bytes, piece c of row r at c ^ (r / 2 & 3), so that both the row-wise
-// accesses of the lanes and the coalesced ones (lane l: piece l & 3 of row 8 i + l / 4) spread
-// over the banks.
-struct Stage {
-    uint32_t row, swizzle;  // of the lane's own row
-    uint32_t coalesced;     // the lane's piece of rows 0 .. 7
-    uint32_t base;
-    int lane;
-    __device__ __forceinline__ Stage(uint32_t buf, int l) : base(buf), lane(l) {
-        row = buf + l * kRowBytes;
-        swizzle = ((l >> 1) & 3) << 4;
-        coalesced = buf + (l >> 2) * kRowBytes + (((l & 3) ^ ((l >> 3) & 3)) << 4);
-    }
-    __device__ __forceinline__ uint32_t own(int c) const {  // piece c of the lane's row
-        return row + (uint32_t(c << 4) ^ swizzle);
-    }
-    __device__ __forceinline__ uint32_t turn(int i) const {  // coalesced, row 8 i + lane / 4
-        return coalesced + i * 8 * kRowBytes;
-    }
-    __device__ __forceinline__ uint32_t at(int r, int byte) const {
-        return base + r * kRowBytes + ((byte & ~15) ^ (((r >> 1) & 3) << 4)) + (byte & 15);
-    }
-};
-__device__ __forceinline__ void put16(uint32_t addr, uint4 v) {
-    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y),
-                 "r"(v.z), "r"(v.w)
-                 : "memory");
-}
-__device__ __forceinline__ uint4 get16(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "r"(addr)
-                 : "memory");
-    return v;
-}
-__device__ __forceinline__ void put_half(uint32_t addr, uint16_t v) {
-    asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(v) : "memory");
-}
-__device__ __forceinline__ uint16_t get_half(uint32_t addr) {
-    uint16_t v;
-    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
-    return v;
-}
-// rows x cols (of 32 x 32, zeros beyond) from src into the buffer
-template <typename T>
-__device__ __forceinline__ void load_rows(const Stage& st, const T* src, int64_t ld, int rows,
-                                          int64_t cols, bool vec) {
-    if (vec) {
-        const int r0 = st.lane >> 2, c = (st.lane & 3) * 8;
-        const T* p = src + r0 * ld + c;
-        const bool in = c < cols;
-        uint4 v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[i] = make_uint4(0, 0, 0, 0);
-            if (in && r0 + 8 * i < rows)
-                v[i] = *reinterpret_cast<const uint4*>(p + i * 8 * ld);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) put16(st.turn(i), v[i]);
-    } else {
-#pragma unroll 8
-        for (int r = 0; r < 32; ++r) {
-            uint16_t v = 0;
-            if (r < rows && st.lane < cols)
-                v = reinterpret_cast<const uint16_t*>(src)[(int64_t)r * ld + st.lane];
-            put_half(st.at(r, st.lane * 2), v);
-        }
-    }
-}
-
-// sums over the warp's rows of 16 columns that each lane holds of its own row, before they are
-// rounded. Every step halves the columns that a lane keeps; then two lanes have one column.
-__device__ __forceinline__ void column_sums(const Two (&z)[8], int lane, int64_t cols,
-                                            float* sums) {
-    float a[16];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) split(z[j], a[2 * j], a[2 * j + 1]);
-    int column = 0;
-#pragma unroll
-    for (int n = 8; n > 0; n >>= 1) {
-        const bool upper = lane & (2 * n);
-#pragma unroll
-        for (int j = 0; j < n; ++j) {
-            const float give = upper ? a[j] : a[n + j];
-            a[j] = (upper ? a[n + j] : a[j]) + __shfl_xor_sync(0xffffffffu, give, 2 * n);
-        }
-        column += upper ? n : 0;
-    }
-    a[0] += __shfl_xor_sync(0xffffffffu, a[0], 1);
-    if (!(lane & 1) && column < cols) sums[column] = a[0];
-}
-
-// the buffer's rows x cols to dst, value by value: outputs whose rows are off 16 bytes
-template <typename T>
-__device__ __forceinline__ void store_rows(const Stage& st, T* dst, int64_t ld, int rows,
-                                           int64_t cols) {
-#pragma unroll 8
-    for (int r = 0; r < 32; ++r) {
-        const uint16_t h = get_half(st.at(r, st.lane * 2));
-        if (r < rows && st.lane < cols)
-            reinterpret_cast<uint16_t*>(dst)[(int64_t)r * ld + st.lane] = h;
-    }
-}
-
-// a warp's 32 rows x 16 columns of float32, each lane its row, through the buffer to memory whose
-// rows are padded to 16 bytes
-__device__ __forceinline__ void store_rows32(const Stage& st, const float (&v)[16], float* dst,
-                                             int64_t ld, int rows, int64_t cols) {
-    __syncwarp();
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-        put16(st.own(c), make_uint4(__float_as_uint(v[4 * c]), __float_as_uint(v[4 * c + 1]),
-                                    __float_as_uint(v[4 * c + 2]), __float_as_uint(v[4 * c + 3])));
-    __syncwarp();
-    const int r0 = st.lane >> 2, c = (st.lane & 3) * 4;
-    float* p = dst + r0 * ld + c;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (c < cols && r0 + 8 * i < rows)
-            *reinterpret_cast<uint4*>(p + i * 8 * ld) = get16(st.turn(i));
-    __syncwarp();
-}
-
-// Bias of 16 columns from `col` (left of them inside), read by all lanes at once and before the
-// accumulator, so that the two waits overlap.
-template <typename T>
-struct Bias {
-    uint32_t w[8];
-    __device__ __forceinline__ void load(const TileParams& p, int64_t col, int64_t left) {
-        const T* bias = static_cast<const T*>(p.bias) + col;
-        if (!p.bias) return;
-        if (p.vec_bias) {
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                uint4 q = make_uint4(0, 0, 0, 0);
-                if (g * 8 < left) q = reinterpret_cast<const uint4*>(bias)[g];
-                w[4 * g] = q.x, w[4 * g + 1] = q.y, w[4 * g + 2] = q.z, w[4 * g + 3] = q.w;
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                w[j] = pack2<T>(2 * j < left ? to_float(bias[2 * j]) : 0.0f,
-                                2 * j + 1 < left ? to_float(bias[2 * j + 1]) : 0.0f);
-        }
-    }
-};
-
-// acc -> z: scales of e4m3 operands and bias
-template <typename T, bool FP8>
-__device__ __forceinline__ void finish_z(const float (&v)[16], Two (&z)[8], const Bias<T>& bias,
-                                         const TileParams& p, int64_t col, int64_t left,
-                                         float x_scale) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        z[j] = two(v[2 * j], v[2 * j + 1]);
-        if constexpr (FP8) {
-            const float s0 = 2 * j < left ? p.w_scale[col + 2 * j] : 0.0f;
-            const float s1 = 2 * j + 1 < left ? p.w_scale[col + 2 * j + 1] : 0.0f;
-            z[j] = z[j] * (two(x_scale) * two(s0, s1));
-        }
-        if (p.bias) {
-            const float2 f = unpack2<T>(bias.w[j]);
-            z[j] = z[j] + two(f.x, f.y);
-        }
-    }
-}
-
-// 16 values of a lane's row to and from pieces 2 half, 2 half + 1 of its line
-template <typename T>
-__device__ __forceinline__ void put_row(const Stage& st, int half, const Two (&v)[8]) {
-    uint32_t w[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        float a, b;
-        split(v[j], a, b);
-        w[j] = pack2<T>(a, b);
-    }
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-        put16(st.own(half * 2 + c), make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]));
-}
-
-template <typename T>
-__device__ __forceinline__ void get_row(const Stage& st, int half, Two (&v)[8]) {
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-        const uint4 q = get16(st.own(half * 2 + c));
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 f = unpack2<T>(w[j]);
-            v[4 * c + j] = two(f.x, f.y);
-        }
-    }
-}
-
-// One warp's part of a finished tile: 32 rows (a warp reads the quarter of TMEM's lanes that its
-// number gives) and every fourth group of 32 columns, the rest being its three partners'. `release` is
-// called when the accumulator has been read. `wait` comes back when the accumulator is complete;
-// what the first group reads from memory is asked for before.
-template <int MODE, typename T, bool FP8, typename Wait, typename Release>
-__device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uint32_t acc,
-                                         const Stage& st, const Stage& st2, int warp,
-                                         const CUtensorMap* out_map, const CUtensorMap* out2_map,
-                                         Wait&& wait, Release&& release) {
-    const int quarter = warp & 3, share = warp >> 2;
-    const int row0 = t.mt * kBM + quarter * 32;
-    const int rows = (int)max((int64_t)0, min((int64_t)32, p.m - row0));
-    constexpr bool kGate = MODE == kGated || MODE == kGatedGrad;
-    const int width = kGate ? p.bn / 2 : p.bn;  // output columns of the tile
-    const int64_t col0 = (int64_t)t.nt * width;
-    const int end = (int)min((int64_t)width, p.n - col0);
-    const int lane = st.lane;
-    constexpr bool kReads = MODE == kGrad || MODE == kGatedGrad;
-    const bool reads = kReads || (MODE == kForward && p.in);
-    auto read_in = [&](int c) {  // residual or dy of the group
-        load_rows(st, static_cast<const T*>(p.in) + (int64_t)row0 * p.ld_in + col0 + c, p.ld_in,
-                  rows, end - c, p.vec_in);
-    };
-    // the buffers are free again when the last copy out has read them
-    auto reuse = [&] {
-        if (lane == 0) bulk_store_read();
-        __syncwarp();
-    };
-    const bool ahead = reads && !(MODE == kForward && p.z) && share * 32 < end;
-    if (ahead) {
-        reuse();
-        read_in(share * 32);
-    }
-    if (!wait()) return;
-    if constexpr (MODE == kPartial) {
-        for (int c = share * 16; c < end; c += 64) {
-            float v[16];
-            tc::tmem_ld16(acc + c, v);
-            store_rows32(st, v, p.z + ((int64_t)t.split * p.m + row0) * p.ld_z + col0 + c,
-                         p.ld_z, rows, end - c);
-        }
-        release();
-        return;
-    }
-    float* sums = nullptr;  // this warp's row of the parts of dbias
-    if (kReads && p.colsum)
-        sums = p.colsum + ((int64_t)t.mt * 4 + quarter) * (kGate ? 2 * p.n : p.n);
-    const float xs = FP8 && lane < rows ? p.x_scale[row0 + lane] : 0.0f;
-    for (int c = share * 32; c < end; c += 128) {
-        const int64_t col = col0 + c, left = p.n - col;
-        if constexpr (MODE == kForward || MODE == kGated) {
-            if (p.z) {  // the pre-activations, in float32
-                reuse();
-                for (int part = 0; part < (kGate ? 2 : 1); ++part) {
-                    for (int half = 0; half < 2 && half * 16 < left; ++half) {
-                        const int64_t at = part * p.n + col + half * 16;
-                        float v[16];
-                        Two z[8];
-                        Bias<T> bias;
-                        bias.load(p, at, left - half * 16);
-                        tc::tmem_ld16(acc + c + part * width + half * 16, v);
-                        finish_z<T, FP8>(v, z, bias, p, at, left - half * 16, xs);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) split(z[j], v[2 * j], v[2 * j + 1]);
-                        store_rows32(st, v,
-                                     p.z + (int64_t)row0 * p.ld_z + part * p.ld_part + col +
-                                         half * 16,
-                                     p.ld_z, rows, left - half * 16);
-                    }
-                }
-            }
-        }
-        if (!ahead || c != share * 32) {
-            reuse();
-            if (reads) read_in(c);
-        }
-        __syncwarp();
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-            const int at = c + half * 16;
-            const int64_t zcol = col + half * 16, zleft = left - half * 16;
-            Two z[8], u[8];
-            {
-                float v[16], w[16];
-                Bias<T> bias, bias_up;
-                bias.load(p, zcol, zleft);
-                if constexpr (kGate) {
-                    bias_up.load(p, p.n + zcol, zleft);
-                    tmem_ld16x2(acc + at, acc + at + width, v, w);
-                } else {
-                    tc::tmem_ld16(acc + at, v);
-                }
-                if (half == 1 && c + 128 >= end) release();
-                finish_z<T, FP8>(v, z, bias, p, zcol, zleft, xs);
-                if constexpr (kGate) finish_z<T, FP8>(w, u, bias_up, p, p.n + zcol, zleft, xs);
-            }
-            if constexpr (MODE == kForward) {
-                with_activation(p.act, [&](auto a) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) z[j] = act_value<decltype(a)::value>(z[j]);
-                });
-                if (p.in) {
-                    get_row<T>(st, half, u);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) z[j] = z[j] + u[j];
-                }
-            } else if constexpr (MODE == kGrad) {
-                get_row<T>(st, half, u);
-                with_activation(p.act, [&](auto a) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        Two y, da;
-                        act_both<decltype(a)::value>(z[j], y, da);
-                        z[j] = u[j] * da;
-                    }
-                });
-            } else if constexpr (MODE == kGated) {
-                with_activation(p.act, [&](auto a) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        z[j] = act_value<decltype(a)::value>(z[j]) * u[j];
-                });
-            } else {
-                Two d[8];
-                get_row<T>(st, half, d);
-                with_activation(p.act, [&](auto a) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        Two y, da;
-                        act_both<decltype(a)::value>(z[j], y, da);
-                        z[j] = d[j] * u[j] * da;
-                        u[j] = d[j] * y;
-                    }
-                });
-                put_row<T>(st2, half, u);
-            }
-            if constexpr (kReads) {
-                if (sums) {
-                    if (lane >= rows) {  // beyond the last row: nothing, whatever the bias is
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) z[j] = u[j] = two(0.0f);
-                    }
-                    column_sums(z, lane, zleft, sums + zcol);
-                    if constexpr (kGate) column_sums(u, lane, zleft, sums + p.n + zcol);
-                }
-            }
-            put_row<T>(st, half, z);
-        }
-        if (p.tma_out) tc::fence_async_smem();
-        __syncwarp();
-        if (p.tma_out) {
-            if (lane == 0 && rows > 0) {
-                bulk_store(out_map, st.base, (int)col, row0);
-                if constexpr (MODE == kGatedGrad) bulk_store(out2_map, st2.base, (int)col, row0);
-                bulk_store_commit();
-            }
-        } else {
-            T* out = static_cast<T*>(p.out) + (int64_t)row0 * p.ld_out + col;
-            store_rows<T>(st, out, p.ld_out, rows, left);
-            if constexpr (MODE == kGatedGrad)
-                store_rows<T>(st2, out + p.n, p.ld_out, rows, left);
-        }
-        __syncwarp();
-    }
-    if (share * 32 >= end) release();  // no columns here
-}
-
-// After a wait gave up: lets what is in flight land (bounded) before the blocks' memory goes. The
-// copies of both blocks count on the even one's barriers; a stage that only one of them had filled
-// when the other gave up gets the other's part from here. Not inlined: among the kernels' own code
-// it cost the gated forward 3 % (110592 x 256 -> 512 65.6 against 63.7 us).
-template <bool PAIR>
-__device__ __noinline__ void drain(TileShared* sh, unsigned* flag, int stages,
-                                   uint32_t stage_bytes) {
-    using namespace tc;
-    const int rank = PAIR ? (int)cluster_rank() : 0, warp = threadIdx.x >> 5;
-    const volatile int* fail = &sh->fail;
-    if (threadIdx.x == 0 && *fail) atomicExch_system(flag, (unsigned)*fail);
-    if (threadIdx.x == 0 && rank == 0) {
-        const int mine = sh->issued;
-        const int theirs = PAIR ? (int)peer_word(peer_address(smem_u32(&sh->issued), 1)) : mine;
-        const int issued = max(mine, theirs);
-        for (int i = max(0, issued - stages); i < issued; ++i) {
-            const uint32_t bar = smem_u32(&sh->full[i % stages]);
-            if (i >= theirs) mbar_complete_tx(bar, stage_bytes);
-            if (i >= mine) mbar_expect_tx(bar, stage_bytes);
-            mbar_wait(bar, (i / stages) & 1);
-        }
-    }
-    __syncwarp();
-    // the products, and on the odd block the arrivals that their completion sends there
-    if (warp == kMmaWarp) {
-        if (rank == 0 && elect_one()) {
-            if constexpr (PAIR) mma_commit_pair(smem_u32(&sh->drained));
-            else mma_commit(smem_u32(&sh->drained));
-        }
-        __syncwarp();
-        mbar_wait(smem_u32(&sh->drained), 0);
-    }
-    __syncwarp();
-}
-
-// PAIR: two blocks of a cluster (the two SMs of a TPC) work on one tile of 256 rows. Each holds its
-// 128 rows of A and of the accumulator and half of the tile's B, which the tensor cores of both
-// read: half the shared-memory traffic and half the copies for B. The even block issues the
-// products; copies of both count on its barriers, completed products on both blocks'.
-template <int MODE, typename T, bool FP8, bool PAIR>
-__global__ void __launch_bounds__(kThreads, 1)
-k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-       const __grid_constant__ CUtensorMap map_o, const __grid_constant__ CUtensorMap map_o2,
-       const TileParams p) {
-    using namespace tc;
-    extern __shared__ __align__(1024) unsigned char smem[];
-    const int b_rows = PAIR ? p.bn / 2 : p.bn;  // of B in this block's stages
-    const uint32_t stage_bytes = kAStage + (uint32_t)b_rows * kLineBytes;
-    unsigned char* bufs = smem + (size_t)p.stages * stage_bytes;
-    auto* sh = reinterpret_cast<TileShared*>(bufs + kEpiWarps * kWarpBufs<MODE> * kWarpBuf);
-    const int tid = threadIdx.x, lane = tid & 31;
-    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform, and known to be
-    constexpr bool kGate = MODE == kGated || MODE == kGatedGrad;
-    const unsigned tiles = (unsigned)p.tiles_m * p.tiles_n, work = tiles * p.splits;
-    const int rank = PAIR ? (int)cluster_rank() : 0;
-    const unsigned first = PAIR ? blockIdx.x >> 1 : blockIdx.x;
-    const unsigned stride = PAIR ? gridDim.x >> 1 : gridDim.x;
-
-    if (tid == 0) {
-        for (int s = 0; s < p.stages; ++s) {
-            mbar_init(smem_u32(&sh->full[s]), 1);
-            mbar_init(smem_u32(&sh->empty[s]), 1);
-        }
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(smem_u32(&sh->acc_full[b]), 1);
-            mbar_init(smem_u32(&sh->acc_empty[b]), kEpiWarps * (PAIR ? 2 : 1));
-        }
-        mbar_init(smem_u32(&sh->drained), 1);
-        sh->fail = 0;
-        sh->issued = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;");
-    }
-    if (warp == kTmaWarp && elect_one()) {
-        prefetch_map(&map_a);
-        prefetch_map(&map_b);
-    }
-    if (warp == kMmaWarp) {
-        if constexpr (PAIR) tmem_alloc_pair(&sh->tmem, 512);
-        else tmem_alloc(&sh->tmem, 512);
-    }
-    fence_before_sync();
-    __syncwarp();
-    if constexpr (PAIR) cluster_sync();
-    else __syncthreads();
-    fence_after_sync();
-    const uint32_t tmem = __shfl_sync(0xffffffffu, sh->tmem, 0);
-    volatile int* fail = &sh->fail;
-    follow_on();
-
-    if (warp == kTmaWarp) {
-        // ---- TMA producer
-        const bool one = elect_one();
-        const int bw = kGate ? p.bn / 2 : p.bn;
-        // barriers of the pair: the even block's
-        const uint32_t full0 = PAIR ? peer_address(smem_u32(sh->full), 0) : smem_u32(sh->full);
-        auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-            if constexpr (PAIR) tma_load_pair(dst, map, x, y, bar);
-            else tma_load(dst, map, x, y, bar);
-        };
-        int st = 0, issued = 0;
-        uint32_t parity = 1;  // of the stage's last release; a fresh barrier passes for 1
-        bool ok = true;
-        for (unsigned w = first; w < work && ok; w += stride) {
-            const Tile t = tile_of(p, w);
-            const int kb0 = t.split * p.kb_per_split;
-            const int kb1 = min(p.kblocks, kb0 + p.kb_per_split);
-            const int m0 = (PAIR ? t.mt * 2 + rank : t.mt) * kBM;
-            // first row of B here: a pair's blocks take halves of the tile, gate and up or not
-            int n0 = t.nt * bw;
-            if (PAIR && rank) n0 += kGate ? (int)p.n : b_rows;
-            for (int kb = kb0; kb < kb1; ++kb) {
-                ok = mbar_wait(smem_u32(&sh->empty[st]), parity, p.polls) && !*fail;
-                if (!__all_sync(0xffffffffu, ok)) {
-                    ok = false;
-                    break;
-                }
-                const uint32_t bar = full0 + (uint32_t)st * 8;
-                const uint32_t a = smem_u32(smem) + (uint32_t)st * stage_bytes, b = a + kAStage;
-                if (one) {
-                    if (!PAIR || rank == 0)
-                        mbar_expect_tx(smem_u32(&sh->full[st]), (PAIR ? 2 : 1) * stage_bytes);
-                    const int x = kb * (FP8 ? 128 : 64);
-                    if (p.a_mn) {
-                        load(a, &map_a, m0, kb * 64, bar);
-                        load(a + kMnChunk, &map_a, m0 + 64, kb * 64, bar);
-                    } else {
-                        load(a, &map_a, x, m0, bar);
-                    }
-                    if (p.b_mn) {
-                        for (int i = 0; i < b_rows / 64; ++i)
-                            load(b + i * kMnChunk, &map_b, n0 + i * 64, kb * 64, bar);
-                    } else {
-                        load(b, &map_b, x, n0, bar);
-                        if (kGate && !PAIR)
-                            load(b + bw * kLineBytes, &map_b, x, (int)p.n + n0, bar);
-                    }
-                }
-                __syncwarp();  // the other lanes' polling must not hold up the copies' issue
-                ++issued;
-                if (++st == p.stages) st = 0, parity ^= 1;
-            }
-        }
-        // the last releases of every stage arrive here (a pair's from the even block) before this
-        // block's memory may go
-        for (int i = max(0, issued - p.stages); i < issued && ok; ++i) {
-            ok = mbar_wait(smem_u32(&sh->empty[i % p.stages]), (i / p.stages) & 1, p.polls) && !*fail;
-            ok = __all_sync(0xffffffffu, ok);
-        }
-        if (!ok && !*fail) *fail = 1;
-        if (one) sh->issued = issued;
-    } else if (warp == kMmaWarp && rank == 0) {
-        // ---- MMA issuer. The whole warp runs the loop and one elected lane issues: control flow
-        // and descriptors are uniform then, and stay in the uniform registers that the tensor
-        // core instructions take (issued from a divergent thread they came too slowly).
-        const bool one = elect_one();
-        const uint64_t step_a = p.a_mn ? 2048 >> 4 : 32 >> 4;
-        const uint64_t step_b = p.b_mn ? 2048 >> 4 : 32 >> 4;
-        const uint64_t desc_a = operand_desc(smem_u32(smem), p.a_mn);
-        const uint64_t desc_b = operand_desc(smem_u32(smem) + kAStage, p.b_mn);
-        auto commit = [&](unsigned long long* bar) {
-            if constexpr (PAIR) mma_commit_pair(smem_u32(bar));
-            else mma_commit(smem_u32(bar));
-        };
-        int st = 0, buf = 0;
-        uint32_t parity = 0, acc_parity = 1;
-        bool ok = true;
-        for (unsigned w = first; w < work && ok; w += stride) {
-            const int split = p.splits > 1 ? (int)p.by_tiles.quotient(w) : 0;
-            const int kb0 = split * p.kb_per_split;
-            const int kb1 = min(p.kblocks, kb0 + p.kb_per_split);
-            ok = mbar_wait(smem_u32(&sh->acc_empty[buf]), acc_parity, p.polls) && !*fail;
-            if (!__all_sync(0xffffffffu, ok)) {
-                if (!*fail) *fail = 2;
-                ok = false;
-                break;
-            }
-            fence_after_sync();
-            const uint32_t acc = tmem + buf * 256;
-            for (int kb = kb0; kb < kb1; ++kb) {
-                ok = mbar_wait(smem_u32(&sh->full[st]), parity, p.polls) && !*fail;
-                if (!__all_sync(0xffffffffu, ok)) {
-                    ok = false;
-                    break;
-                }
-                fence_after_sync();
-                const uint64_t at = (uint64_t)((uint32_t)st * (stage_bytes >> 4));
-                if (one) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const bool more = kb > kb0 || k > 0;
-                        mma<FP8, PAIR>(acc, desc_a + at + k * step_a, desc_b + at + k * step_b,
-                                       p.idesc, more);
-                    }
-                    commit(&sh->empty[st]);
-                }
-                __syncwarp();
-                if (++st == p.stages) st = 0, parity ^= 1;
-            }
-            if (one) commit(&sh->acc_full[buf]);
-            __syncwarp();
-            buf ^= 1;
-            if (buf == 0) acc_parity ^= 1;
-        }
-        if (!ok && !*fail) *fail = 3;
-        // and the last arrivals of the epilogues (both blocks')
-        for (int i = 0; i < 2 && ok; ++i) {
-            ok = mbar_wait(smem_u32(&sh->acc_empty[buf]), acc_parity, p.polls) && !*fail;
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok && !*fail) *fail = 2;
-            buf ^= 1;
-            if (buf == 0) acc_parity ^= 1;
-        }
-    } else if (warp < kEpiWarps) {
-        // ---- epilogue
-        int n_tile = 0;
-        const uint32_t buf = smem_u32(bufs) + warp * kWarpBufs<MODE> * kWarpBuf;
-        const Stage st(buf, lane), st2(buf + (kWarpBufs<MODE> - 1) * kWarpBuf, lane);
-        const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
-        bool ok = true;
-        for (unsigned w = first; w < work && ok; w += stride, ++n_tile) {
-            Tile t = tile_of(p, w);
-            if (PAIR) t.mt = t.mt * 2 + rank;
-            const int b = n_tile & 1, round = n_tile >> 1;
-            epilogue<MODE, T, FP8>(
-                p, t, tmem + b * 256 + quarter, st, st2, warp, &map_o, &map_o2,
-                [&] {
-                    ok = mbar_wait(smem_u32(&sh->acc_full[b]), round & 1, p.polls) && !*fail;
-                    ok = __all_sync(0xffffffffu, ok);
-                    fence_after_sync();
-                    return ok;
-                },
-                [&] {
-                    fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if constexpr (PAIR)
-                            mbar_arrive_peer(peer_address(smem_u32(&sh->acc_empty[b]), 0));
-                        else
-                            mbar_arrive(smem_u32(&sh->acc_empty[b]));
-                    }
-                    __syncwarp();
-                });
-        }
-        if (lane == 0) bulk_store_read();  // the copies out have read the buffers
-        if (!ok && !*fail) *fail = 4;
-    }
-    __syncwarp();
-    if constexpr (PAIR) cluster_sync();
-    else __syncthreads();
-    bool failed = *fail;
-    if constexpr (PAIR)
-        failed = failed || peer_word(peer_address(smem_u32(&sh->fail), rank ^ 1)) != 0;
-    if (failed) {
-        drain<PAIR>(sh, p.flag, p.stages, stage_bytes);
-    }
-    fence_before_sync();
-    if constexpr (PAIR) cluster_sync();
-    else __syncthreads();
-    if (warp == kMmaWarp) {
-        fence_after_sync();
-        if constexpr (PAIR) tmem_dealloc_pair(tmem, 512);
-        else tmem_dealloc(tmem, 512);
-    }
-}
 
 // ----------------------------------------------------------------------------- joins
 // y (and z) from the float32 sums of `splits` ranges of k, added in order. Four columns a
@@ -995,31 +277,6 @@ k_pack(const uint8_t* src, int64_t rows, int64_t bytes, int64_t ld,
 }
 
 // ----------------------------------------------------------------------------- host
-// Scratch carved from the caller's workspace; with a null base it only adds up the bytes.
-struct Scratch {
-    char* base;
-    int64_t off = 0;
-    template <typename T>
-    T* take(int64_t n) {
-        char* p = base ? base + off : nullptr;
-        off += (n * (int64_t)sizeof(T) + 255) / 256 * 256;
-        return reinterpret_cast<T*>(p);
-    }
-    bool sizing() const { return base == nullptr; }
-};
-
-struct Plan {
-    int bn, splits, kb_per_split, stages;
-    bool pair;
-};
-
-// Cycles that a k-block of 64 takes (measured on B200 at sizes that fill it): the tensor cores'
-// 2 cycles a column for the widest tile of a pair, more for the others, which read more shared
-// memory for a product.
-double block_cycles(bool pair, int bn) {
-    return pair ? (bn == 256 ? 520.0 : 370.0) : bn == 256 ? 660.0 : bn == 128 ? 400.0 : 300.0;
-}
-
 // Tile, range of k and pairing of one product, by a model of its time in cycles: the k-blocks, an
 // epilogue (16 cycles a column, 25 with an activation: measured at 110592 x 256 -> 512, 35 and
 // 51 us), hidden behind the next tile's products, and for ranges of k the launch and the traffic of
@@ -1052,13 +309,9 @@ Plan plan_product(int64_t m, int64_t n_cols, int kblocks, bool can_split, bool g
             }
         }
     }
-    const uint32_t stage =
-        kAStage + (uint32_t)(best.pair ? best.bn / 2 : best.bn) * kLineBytes;
-    best.stages = (int)std::min<uint32_t>(kMaxStages, (kSmemMax - fixed) / stage);
+    best.stages = ring_stages(best.pair, best.bn, fixed);
     return best;
 }
-
-CUtensorMap make_out_map(const void* p, int64_t rows, int64_t cols, int64_t ld);
 
 template <int MODE, typename T, bool FP8, bool PAIR>
 void launch_tile(const CUtensorMap& a, const CUtensorMap& b, TileParams p, int sms, int device,
@@ -1069,23 +322,13 @@ void launch_tile(const CUtensorMap& a, const CUtensorMap& b, TileParams p, int s
         if (MODE == kGatedGrad)
             o2 = make_out_map(static_cast<T*>(p.out) + p.n, p.m, p.n, p.ld_out);
     }
-    static std::atomic<uint64_t> allowed{0};  // devices whose limit is raised
-    if (device >= 64 || !(allowed.load(std::memory_order_relaxed) >> device & 1)) {
-        RUNE_CUDA_TRY(cudaFuncSetAttribute(k_tile<MODE, T, FP8, PAIR>,
-                                           cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           (int)kSmemMax));
-        if (device < 64) allowed.fetch_or(uint64_t(1) << device, std::memory_order_relaxed);
-    }
     const int64_t work = (int64_t)p.tiles_m * p.tiles_n * p.splits;
     require(work < (1LL << 31) - 1024, "too many tiles");
     p.by_tiles = make_divisor((unsigned)p.tiles_m * p.tiles_n);
     p.by_group = make_divisor(kGroup * p.tiles_n);
     p.by_last = make_divisor(std::max(1u, (unsigned)p.tiles_m % kGroup));
-    const int b_rows = PAIR ? p.bn / 2 : p.bn;
-    const unsigned grid = PAIR ? 2 * (unsigned)std::min<int64_t>(work, sms / 2)
-                               : (unsigned)std::min<int64_t>(work, sms);
-    const size_t smem = (size_t)p.stages * (kAStage + (size_t)b_rows * kLineBytes) + kFixedSmem<MODE>;
-    launch(k_tile<MODE, T, FP8, PAIR>, grid, kThreads, smem, PAIR ? 2 : 0, stream, a, b, o, o2, p);
+    launch_blocks<MODE, kWhole, T, FP8, PAIR>(a, b, o, o2, p, work, kFixedSmem<MODE>, sms, device,
+                                              stream);
 }
 
 // One product D[m, n] = A B^T: operands, epilogue (in p) and scratch for a split.
@@ -1181,37 +424,12 @@ void run_product(const Product& g, const TileParams& p, Scratch& ws, int device,
     else typed(__nv_bfloat16());
 }
 
-int64_t pad16(int64_t cols, int elem_bytes) {
-    const int64_t v = 16 / elem_bytes;
-    return (cols + v - 1) / v * v;
-}
-
 void pad_rows(const void* src, int64_t rows, int64_t bytes, int64_t ld, void* dst, int64_t ld_dst,
               cudaStream_t stream) {
     const dim3 grid((unsigned)((ld_dst / 16 + 31) / 32),
                     (unsigned)std::min<int64_t>((rows + 7) / 8, 65535));
     launch(k_pack, grid, dim3(32, 8), 0, 0, stream, static_cast<const uint8_t*>(src), rows, bytes,
            ld, static_cast<uint8_t*>(dst), ld_dst);
-}
-
-// the operand itself, or its padded copy in the scratch
-Matrix readable(Matrix m, int elem_bytes, Scratch& ws, cudaStream_t stream) {
-    if (m.rows == 1) m.ld = pad16(m.cols, elem_bytes);  // no second line to reach
-    if (tma_ready(m, elem_bytes)) return m;
-    Matrix d = m;
-    d.ld = pad16(m.cols, elem_bytes);
-    void* to = ws.take<char>(m.rows * d.ld * elem_bytes);
-    d.p = to;
-    if (ws.sizing()) {
-        d.p = reinterpret_cast<const void*>(256);  // any aligned address: only sizes are asked
-        return d;
-    }
-    pad_rows(m.p, m.rows, m.cols * elem_bytes, m.ld * elem_bytes, to, d.ld * elem_bytes, stream);
-    return d;
-}
-
-bool wide16(const void* p, int64_t ld, int64_t cols) {
-    return aligned(p, 16) && ld % 8 == 0 && cols % 8 == 0;
 }
 
 // values of a row of the saved z for `outputs` columns (each of gate and up)
@@ -1430,6 +648,21 @@ unsigned* g_flag_dev[kMaxDevices];
 
 }  // namespace
 
+Matrix readable(Matrix m, int elem_bytes, Scratch& ws, cudaStream_t stream) {
+    if (m.rows == 1) m.ld = pad16(m.cols, elem_bytes);  // no second line to reach
+    if (tma_ready(m, elem_bytes)) return m;
+    Matrix d = m;
+    d.ld = pad16(m.cols, elem_bytes);
+    void* to = ws.take<char>(m.rows * d.ld * elem_bytes);
+    d.p = to;
+    if (ws.sizing()) {
+        d.p = reinterpret_cast<const void*>(256);  // any aligned address: only sizes are asked
+        return d;
+    }
+    pad_rows(m.p, m.rows, m.cols * elem_bytes, m.ld * elem_bytes, to, d.ld * elem_bytes, stream);
+    return d;
+}
+
 CUtensorMap make_map(const Matrix& m, int elem_bytes, int box_rows) {
     CUtensorMap map;
     const cuuint64_t dims[2] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows};
@@ -1447,9 +680,23 @@ CUtensorMap make_map(const Matrix& m, int elem_bytes, int box_rows) {
     return map;
 }
 
-namespace {
+CUtensorMap make_map3(const Matrix& m, int64_t count, int64_t step, int elem_bytes, int box_rows) {
+    CUtensorMap map;
+    const cuuint64_t dims[3] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows, (cuuint64_t)count};
+    const cuuint64_t strides[2] = {(cuuint64_t)(m.ld * elem_bytes), (cuuint64_t)(step * elem_bytes)};
+    const cuuint32_t box[3] = {kLineBytes / (cuuint32_t)elem_bytes, (cuuint32_t)box_rows, 1};
+    const cuuint32_t each[3] = {1, 1, 1};
+    CUresult r = encode_tiled()(
+        &map, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3,
+        const_cast<void*>(m.p), dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
+        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        throw Error(RUNE_ERR_INVALID,
+                    "an operand cannot be described to TMA (status " + std::to_string(r) + ")");
+    return map;
+}
 
-// 32 x 32 boxes of a 16-bit output with the 64-byte swizzle, which is the buffers' own
 CUtensorMap make_out_map(const void* p, int64_t rows, int64_t cols, int64_t ld) {
     CUtensorMap map;
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
@@ -1465,7 +712,21 @@ CUtensorMap make_out_map(const void* p, int64_t rows, int64_t cols, int64_t ld) 
     return map;
 }
 
-}  // namespace
+CUtensorMap make_out_map3(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t count,
+                          int64_t step) {
+    CUtensorMap map;
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)count};
+    const cuuint64_t strides[2] = {(cuuint64_t)(ld * 2), (cuuint64_t)(step * 2)};
+    const cuuint32_t box[3] = {32, 32, 1}, each[3] = {1, 1, 1};
+    CUresult r = encode_tiled()(&map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(p),
+                                dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        throw Error(RUNE_ERR_INVALID,
+                    "an output cannot be described to TMA (status " + std::to_string(r) + ")");
+    return map;
+}
 
 unsigned wait_polls() { return g_polls.load(std::memory_order_relaxed); }
 

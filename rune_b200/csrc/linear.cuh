@@ -155,6 +155,35 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
         : "memory");
 }
 
+// the same of 3-D maps (a stack of matrices)
+__device__ __forceinline__ void tma_load3(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
+                                          uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load3_pair(uint32_t dst, const CUtensorMap* map, int x, int y,
+                                               int z, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        ".cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void bulk_store3(const CUtensorMap* map, uint32_t src, int x, int y,
+                                            int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];"
+                 ::"l"(map), "r"(x), "r"(y), "r"(z), "r"(src)
+                 : "memory");
+}
+
+// Tensor maps that a kernel before wrote to global memory: before this thread's first use of each.
+__device__ __forceinline__ void map_acquire(const CUtensorMap* map) {
+    asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(map) : "memory");
+}
+
 // the same tile as far as L2
 __device__ __forceinline__ void prefetch_tile(const CUtensorMap* map, int x, int y) {
     asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];"
@@ -213,6 +242,37 @@ inline bool tma_ready(const Matrix& m, int elem_bytes) {
 
 // Tensor map of `m` with boxes of one 128-byte line x box_rows lines, zeros outside.
 CUtensorMap make_map(const Matrix& m, int elem_bytes, int box_rows);
+// The same of a stack of `count` matrices, the first of which is `m`, `step` values apart.
+CUtensorMap make_map3(const Matrix& m, int64_t count, int64_t step, int elem_bytes, int box_rows);
+// 32 x 32 boxes of a 16-bit output with the 64-byte swizzle, which is the warps' buffers' own
+CUtensorMap make_out_map(const void* p, int64_t rows, int64_t cols, int64_t ld);
+CUtensorMap make_out_map3(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t count,
+                          int64_t step);
+
+// Scratch carved from the caller's workspace; with a null base it only adds up the bytes.
+struct Scratch {
+    char* base;
+    int64_t off = 0;
+    template <typename T>
+    T* take(int64_t n) {
+        char* p = base ? base + off : nullptr;
+        off += (n * (int64_t)sizeof(T) + 255) / 256 * 256;
+        return reinterpret_cast<T*>(p);
+    }
+    bool sizing() const { return base == nullptr; }
+};
+
+inline int64_t pad16(int64_t cols, int elem_bytes) {
+    const int64_t v = 16 / elem_bytes;
+    return (cols + v - 1) / v * v;
+}
+
+inline bool wide16(const void* p, int64_t ld, int64_t cols) {
+    return aligned(p, 16) && ld % 8 == 0 && cols % 8 == 0;
+}
+
+// the operand itself, or its padded copy in the scratch
+Matrix readable(Matrix m, int elem_bytes, Scratch& ws, cudaStream_t stream);
 
 // Largest number of rows of x that linear_few takes. B200, bf16, us on the GPU with the weights in
 // L2, few rows / tiles at 1, 16, 32 and 48 rows:
