@@ -393,6 +393,132 @@ typedef struct {
 int rune_linear_backward(const rune_linear_grad_args* args, void* stream);
 int rune_linear_backward_workspace(const rune_linear_grad_args* args, int64_t* bytes);
 
+/* ------------------------------------------------------------------------------------------
+ * Operators whose weights depend on the row: the choice of groups (experts), the sort of rows by
+ * group, the moves of rows into that order and back, the groups' linear and gated layers, with
+ * their gradients (rune/nep/model.py:157-170 evaluates one network per element by a loop over the
+ * elements). The rules of the operators above hold: device pointers, no synchronisation, scratch
+ * from the caller, equal bits for equal inputs. Groups' sizes stay on the GPU. At most 1024 groups. */
+typedef struct {
+    int64_t rows, groups, k;
+    int64_t logits_stride;
+    int32_t device;
+    int32_t dtype;          /* of logits and dlogits: RUNE_F32, RUNE_F16 or RUNE_BF16 */
+    const void* logits;     /* [rows, groups] */
+    int32_t* index;         /* [rows, k]: written by rune_route, read by its gradient */
+    float* weights;         /* [rows, k]: likewise */
+    const float* dweights;  /* [rows, k], gradient only */
+    void* dlogits;          /* [rows, groups], gradient only */
+} rune_route_args;
+
+/* The k (1 to 32) largest logits of each row, largest first, ties to the lowest index, NaN above
+ * all, and the softmax over them. A logit of -inf is not chosen: index -1, weight 0. */
+int rune_route(const rune_route_args* args, void* stream);
+int rune_route_backward(const rune_route_args* args, void* stream);
+
+typedef struct {
+    int64_t rows, groups, k; /* rows * k slots */
+    int32_t device;
+    int32_t index_bytes;    /* 4 or 8 */
+    const void* index;      /* [rows, k]; outside 0 .. groups - 1: in no group */
+    int32_t* offsets;       /* [groups + 1]: the groups' first places, and the end of the last */
+    int32_t* order;         /* [rows * k]: slot of each place; -1 behind the last group */
+    int32_t* place;         /* [rows, k]: place of each slot; -1 of those in no group */
+    void* workspace;
+    int64_t workspace_bytes;
+} rune_row_groups_args;
+
+/* Stable sort of slots by group. */
+int rune_row_groups(const rune_row_groups_args* args, void* stream);
+int rune_row_groups_workspace(const rune_row_groups_args* args, int64_t* bytes);
+
+typedef struct {
+    int64_t rows, k, width; /* rows * k slots */
+    int64_t in_stride, y_stride;
+    int32_t device;
+    int32_t dtype;          /* RUNE_F32, RUNE_F16 or RUNE_BF16 */
+    const void* in;
+    const void* y;
+    const int32_t* order;   /* of rune_row_groups; values outside 0 .. rows * k - 1 count as -1 */
+    const int32_t* place;
+    const float* weights;   /* [rows, k] or NULL (all 1) */
+    void* out;
+    float* dweights;        /* [rows, k] */
+} rune_group_move_args;
+
+/* out[p] = in[order[p] / k] * weights[order[p]], zeros where order[p] is -1: in [rows, width], out
+ * [rows * k, width]. */
+int rune_to_groups(const rune_group_move_args* args, void* stream);
+/* out[r] = sum_j in[place[r, j]] * weights[r, j] without the slots whose place is -1: in [rows * k,
+ * width], out [rows, width]. Also the gradient of rune_to_groups. */
+int rune_from_groups(const rune_group_move_args* args, void* stream);
+/* Of rune_from_groups with weights: in = dout [rows, width], y its input; out = dy [rows * k, width]
+ * (or NULL), dweights (or NULL). Without weights dy is rune_to_groups of dout. */
+int rune_from_groups_backward(const rune_group_move_args* args, void* stream);
+
+typedef struct {
+    int64_t rows, inputs, outputs, groups;
+    int64_t x_stride, weight_stride;
+    int32_t device;
+    int32_t dtype;          /* RUNE_F16 or RUNE_BF16, of all matrices */
+    int32_t activation;     /* RUNE_ACT_* */
+    int32_t gated;          /* as in rune_linear_args */
+    const void* x;          /* [rows, inputs], sorted by group */
+    const void* weight;     /* [groups, n, inputs], n = outputs or 2 outputs; rows weight_stride
+                               apart throughout */
+    const void* bias;       /* [groups, n] or NULL */
+    const int32_t* offsets; /* [groups + 1]; values outside 0 .. rows are taken as the nearer end */
+    void* y;                /* [rows, outputs]; zeros behind the last group */
+    void* workspace;
+    int64_t workspace_bytes;
+} rune_grouped_linear_args;
+
+/* rune_linear of the rows of each group with the group's weights. */
+int rune_grouped_linear(const rune_grouped_linear_args* args, void* stream);
+int rune_grouped_linear_workspace(const rune_grouped_linear_args* args, int64_t* bytes);
+
+typedef struct {
+    int64_t rows, inputs, outputs, groups;
+    int64_t x_stride, weight_stride, dy_stride;
+    int32_t device, dtype, activation, gated;
+    const void* x;
+    const void* weight;
+    const void* bias;
+    const int32_t* offsets;
+    const void* dy;         /* [rows, outputs]; not read behind the last group */
+    void* dx;               /* [rows, inputs], zeros behind the last group; or NULL */
+    void* dweight;          /* [groups, n, inputs], zeros for groups without rows; or NULL */
+    void* dbias;            /* [groups, n], or NULL */
+    void* workspace;
+    int64_t workspace_bytes;
+} rune_grouped_linear_grad_args;
+
+int rune_grouped_linear_backward(const rune_grouped_linear_grad_args* args, void* stream);
+int rune_grouped_linear_backward_workspace(const rune_grouped_linear_grad_args* args,
+                                           int64_t* bytes);
+
+/* ------------------------------------------------------------------------------------------
+ * Newton-Schulz orthogonalisation of a stack of matrices, for optimisers that update weights by it:
+ * X = x / (|x|_F + eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T (or, where
+ * there are more rows than columns, X <- a X + X (b A + c A A) with A = X^T X). Products of float16
+ * operands with float32 sums. */
+typedef struct {
+    int64_t count, rows, cols;
+    int64_t x_step, x_row, x_col; /* strides in elements: matrix, row, column */
+    int32_t device;
+    int32_t dtype;          /* of x: RUNE_F32, RUNE_F16 or RUNE_BF16 */
+    int32_t steps;          /* 0 to 64 */
+    float a, b, c, eps;
+    int32_t reserved;
+    const void* x;
+    void* y;                /* [count, rows, cols], RUNE_BF16 */
+    void* workspace;
+    int64_t workspace_bytes;
+} rune_orthogonalize_args;
+
+int rune_orthogonalize(const rune_orthogonalize_args* args, void* stream);
+int rune_orthogonalize_workspace(const rune_orthogonalize_args* args, int64_t* bytes);
+
 /* Release the engine and its device memory. */
 void rune_engine_destroy(rune_engine* engine);
 

@@ -1,0 +1,618 @@
+// Linear and gated layers whose rows come in groups, each with its own weights, and their gradients:
+//   y[p] = act(x[p] W_g^T + b_g),   gated: act(x[p] Wg_g^T + bg_g) * (x[p] Wu_g^T + bu_g),
+//   dx[p] = dz[p] W_g,  dW_g = sum over p in g of dz[p]^T x[p],  db_g = sum over p in g of dz[p],
+// for the places p of group g that the sort left in offsets[g] .. offsets[g + 1] - 1.
+//
+// The tile kernel of the linear layers runs them in one launch each. The groups' sizes are known on
+// the GPU alone, so a block works its tiles out from the offsets:
+//   forward, dz, dx   tiles of the rows of each group. A tile that reaches past its group's end
+//                     reads rows of the next, whose results no one stores: boxes of whole rows leave
+//                     by TMA, the last ones by the lanes. Weights are a 3-D map, zeros beyond a
+//                     group's matrix, since dx contracts over its rows.
+//   dW                a product per group over its rows. What lies behind the last row must be
+//                     zeros in both operands (the next group's row may hold an infinity), so each
+//                     group has tensor maps of its own, cut to its rows: k_group_maps writes them.
+// z of an activated layer is computed again in the backward pass: a copy in float32 would cost 8
+// bytes of traffic and 4 of memory a value, for all slots of every layer.
+
+#include "tile.cuh"
+
+namespace rune {
+namespace ops {
+
+namespace {
+
+constexpr int64_t kMaxSize = INT32_MAX - 512;  // tile coordinates are 32-bit
+constexpr int64_t kMaxGroups = 1024;
+
+// ----------------------------------------------------------------------------- kernels
+// Maps of two matrices' rows [offsets[g], offsets[g + 1]): the whole ones with another address and
+// number of rows. A warp writes one, from shared memory.
+struct MapParams {
+    const int32_t* offsets;
+    int64_t rows;
+    int groups;
+    const char *a, *b;
+    int64_t line_a, line_b;  // bytes
+    CUtensorMap* maps;       // [groups][2]
+};
+constexpr int kMapWarps = 4;
+__global__ void __launch_bounds__(32 * kMapWarps)
+k_group_maps(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+             const MapParams p) {
+    __shared__ __align__(128) uint32_t copy[kMapWarps][32];
+    follow_on();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int at = blockIdx.x * kMapWarps + warp, g = at >> 1;
+    if (g >= p.groups) return;
+    const bool second = at & 1;
+    const int64_t first = min((int64_t)max(p.offsets[g], 0), p.rows);
+    const int64_t end = min((int64_t)max(p.offsets[g + 1], 0), p.rows);
+    if (first >= end) return;  // nothing to read: no one asks for the map
+    copy[warp][lane] = reinterpret_cast<const uint32_t*>(second ? &map_b : &map_a)[lane];
+    __syncwarp();
+    const uint32_t own = tc::smem_u32(copy[warp]);
+    if (lane == 0) {
+        const char* start = second ? p.b + first * p.line_b : p.a + first * p.line_a;
+        asm volatile("tensormap.replace.tile.global_address.shared::cta.b1024.b64 [%0], %1;"
+                     ::"r"(own), "l"(start)
+                     : "memory");
+        asm volatile("tensormap.replace.tile.global_dim.shared::cta.b1024.b32 [%0], 1, %1;"
+                     ::"r"(own), "r"((uint32_t)(end - first))
+                     : "memory");
+    }
+    __syncwarp();
+    asm volatile(
+        "tensormap.cp_fenceproxy.global.shared::cta.tensormap::generic.release.gpu.sync.aligned"
+        " [%0], [%1], 128;" ::"l"(p.maps + at), "r"(own)
+        : "memory");
+}
+
+// Lines of `high` rows that the groups before g fill: lines[g], for all groups and the end.
+__device__ __forceinline__ void count_lines(const int32_t* offsets, int64_t rows, int groups,
+                                            int high, int32_t* first_row, int32_t* lines) {
+    for (int g = threadIdx.x; g <= groups; g += blockDim.x)
+        first_row[g] = (int)min((int64_t)max(offsets[g], 0), rows);
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        int before = 0;
+        for (int g0 = 0; g0 < groups; g0 += 32) {
+            const int g = g0 + threadIdx.x;
+            const int n = g < groups
+                              ? (max(0, first_row[g + 1] - first_row[g]) + high - 1) / high : 0;
+            int sum = n;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const int other = __shfl_up_sync(0xffffffffu, sum, o);
+                sum += (int)threadIdx.x >= o ? other : 0;
+            }
+            if (g < groups) lines[g] = before + sum - n;
+            before += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (threadIdx.x == 0) lines[groups] = before;
+    }
+    __syncthreads();
+}
+
+struct SumParams {
+    const int32_t* offsets;
+    int64_t rows, n;
+    int groups, high, each;  // rows of a line, parts that each line left
+    int64_t ld;              // k_group_columns: of x
+    const void* x;
+    float* parts;            // [lines * each][n]
+    void* out;               // [groups][n]
+};
+
+// sums of the columns of each line of rows, which no line of another group's shares: 64 columns a
+// block, four rows at a time
+template <typename T>
+__global__ void __launch_bounds__(256) k_group_columns(const SumParams p) {
+    follow_on();
+    extern __shared__ int32_t table[];
+    int32_t *first = table, *lines = table + p.groups + 1;
+    __shared__ float joined[4][64];
+    count_lines(p.offsets, p.rows, p.groups, p.high, first, lines);
+    const int c = threadIdx.x & 63, part = threadIdx.x >> 6;
+    const int64_t col = (int64_t)blockIdx.x * 64 + c;
+    for (int line = blockIdx.y; line < lines[p.groups]; line += gridDim.y) {
+        int g = 0, above = p.groups;
+        while (above - g > 1) {
+            const int mid = (g + above) >> 1;
+            if (lines[mid] <= line) g = mid;
+            else above = mid;
+        }
+        const int r0 = first[g] + (line - lines[g]) * p.high, r1 = min(r0 + p.high, first[g + 1]);
+        float s = 0.0f;
+        if (col < p.n) {
+            const T* x = static_cast<const T*>(p.x) + col;
+#pragma unroll 8
+            for (int r = r0 + part; r < r1; r += 4) s += to_float(x[r * p.ld]);
+        }
+        __syncthreads();
+        joined[part][c] = s;
+        __syncthreads();
+        if (part == 0 && col < p.n)
+            p.parts[line * p.n + col] = joined[0][c] + joined[1][c] + joined[2][c] + joined[3][c];
+    }
+}
+
+// The parts of each group's lines, added up: 32 columns and a group a block; 32 threads of a column
+// take the parts in turn and join their sums in order.
+template <typename T>
+__global__ void __launch_bounds__(1024) k_group_sums(const SumParams p) {
+    follow_on();
+    extern __shared__ int32_t table[];
+    int32_t *first = table, *lines = table + p.groups + 1;
+    __shared__ float joined[32][33];
+    count_lines(p.offsets, p.rows, p.groups, p.high, first, lines);
+    const int c = threadIdx.x & 31, turn = threadIdx.x >> 5;
+    const int64_t col = (int64_t)blockIdx.x * 32 + c;
+    for (int g = blockIdx.y; g < p.groups; g += gridDim.y) {
+        const int64_t from = (int64_t)lines[g] * p.each, to = (int64_t)lines[g + 1] * p.each;
+        float s = 0.0f;
+        if (col < p.n) {
+#pragma unroll 4
+            for (int64_t i = from + turn; i < to; i += 32) s += p.parts[i * p.n + col];
+        }
+        __syncthreads();
+        joined[turn][c] = s;
+        __syncthreads();
+        // warp `turn` adds up the column `turn`
+        const float all = warp_sum(joined[c][turn]);
+        const int64_t mine = (int64_t)blockIdx.x * 32 + turn;
+        if (c == 0 && mine < p.n) static_cast<T*>(p.out)[g * p.n + mine] = from_float<T>(all);
+    }
+}
+
+// out[i] = sum over the splits of part[s][i], rows of n values from lines of ld
+template <typename T>
+__global__ void __launch_bounds__(256)
+k_join_depth(const float* part, int splits, int64_t rows, int64_t n, int64_t ld, bool wide, T* out) {
+    follow_on();
+    const int64_t groups = ld / 4, total = rows * groups;
+    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
+         i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t row = i / groups, col = (i - row * groups) * 4;
+        float v[4] = {};
+#pragma unroll 4
+        for (int s = 0; s < splits; ++s) {
+            const float4 q =
+                *reinterpret_cast<const float4*>(part + (s * rows + row) * ld + col);
+            v[0] += q.x, v[1] += q.y, v[2] += q.z, v[3] += q.w;
+        }
+        T* to = out + row * n + col;
+        if (wide)
+            *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+        else
+            for (int j = 0; j < 4 && col + j < n; ++j) to[j] = from_float<T>(v[j]);
+    }
+}
+
+// ----------------------------------------------------------------------------- host
+uint32_t table_bytes(int64_t groups) {
+    return (uint32_t)((2 * groups + 2) * 4 + 127) / 128 * 128;
+}
+
+int64_t line_bound(int64_t rows, int64_t groups, int high) {
+    return rows / high + std::min(rows, groups);
+}
+
+// Tile and pairing of a product of rows by group, by the time of the whole product's model. Each
+// group that has rows ends inside a line of tiles.
+Plan plan_rows(int64_t rows, int64_t groups, int64_t n_cols, int kblocks, bool gate, bool act,
+               int sms, uint32_t fixed) {
+    Plan best{};
+    double best_cost = 0.0;
+    const double met = (double)std::min(rows, groups);
+    for (int pair = 1; pair >= 0; --pair) {
+        for (int bn : {256, 128, 64}) {
+            if ((gate || pair) && bn == 64) continue;  // halves of at least 64 columns
+            const int high = pair ? 2 * kBM : kBM, units = pair ? sms / 2 : sms;
+            const double lines = std::max(met, rows / (double)high + 0.5 * met);
+            const double tiles = lines * ((n_cols + bn - 1) / bn);
+            const double waves = std::max(1.0, tiles / units + (tiles > units ? 0.5 : 0.0));
+            const double main = kblocks * block_cycles(pair, bn);
+            const double epi = 1000.0 + (act ? (gate ? 15.0 : 25.0) : 16.0) * bn;
+            const double cost = waves * std::max(main, epi) + std::min(main, epi);
+            if (best.bn == 0 || cost < best_cost) {
+                best_cost = cost;
+                best = {bn, 1, kblocks, 0, pair == 1};
+            }
+        }
+    }
+    best.stages = ring_stages(best.pair, best.bn, fixed);
+    return best;
+}
+
+// Tile, pairing and ranges of k of the groups' products over their rows. The work divides among the
+// blocks but for its largest piece, a range of the largest group's rows, taken as three times the
+// mean; ranges cost the traffic of their join.
+Plan plan_depth(int64_t rows, int64_t groups, int64_t m, int64_t n, int sms, uint32_t fixed) {
+    Plan best{};
+    double best_cost = 0.0;
+    const double depth = std::max(1.0, rows / 64.0 / groups + 0.5);  // k-blocks of a group
+    for (int pair = 1; pair >= 0; --pair) {
+        for (int bn : {256, 128, 64}) {
+            if (pair && bn == 64) continue;
+            const int high = pair ? 2 * kBM : kBM, units = pair ? sms / 2 : sms;
+            const double tiles = (double)((m + high - 1) / high) * ((n + bn - 1) / bn) * groups;
+            for (int splits = 1; splits <= 64; splits *= 2) {
+                if (splits > 1 && 3.0 * depth / splits < 4.0) break;
+                const double epi = 1000.0 + 16.0 * bn, block = block_cycles(pair, bn);
+                const double all = tiles * std::max(depth * block, splits * epi) / units;
+                double cost = all + 3.0 * depth / splits * block + epi;
+                if (splits > 1)
+                    cost += 5000.0 + (double)groups * m * n * (splits + 1) * 4.0 / 3000.0;
+                if (best.bn == 0 || cost < best_cost) {
+                    best_cost = cost;
+                    best = {bn, splits, 0, 0, pair == 1};
+                }
+            }
+        }
+    }
+    best.stages = ring_stages(best.pair, best.bn, fixed);
+    return best;
+}
+
+// A stack of `groups` matrices, rows and matrices alike `ld` values apart.
+struct Weights {
+    Matrix all;
+    int64_t rows;  // of each
+    CUtensorMap map(int64_t groups, int box_rows) const {
+        Matrix one = all;
+        one.rows = rows;
+        return make_map3(one, groups, rows * all.ld, 2, box_rows);
+    }
+};
+
+template <int MODE, int KIND, typename T>
+void launch_kind(bool pair, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o,
+                 const CUtensorMap& o2, const TileParams& p, int64_t work, uint32_t fixed, int sms,
+                 int device, cudaStream_t stream) {
+    require(work < (1LL << 31) - 1024, "too many tiles");
+    if (pair)
+        launch_blocks<MODE, KIND, T, false, true>(a, b, o, o2, p, work, fixed, sms, device, stream);
+    else
+        launch_blocks<MODE, KIND, T, false, false>(a, b, o, o2, p, work, fixed, sms, device,
+                                                   stream);
+}
+
+// Rows of A by group, each with its matrix of w (K-major, or MN-major for dx).
+struct RowProduct {
+    Matrix a;
+    Weights w;
+    bool w_mn = false;
+    int64_t k = 0, groups = 0;
+    const int32_t* offsets = nullptr;
+    int device = 0, dtype = 0;
+};
+
+// Height of the tiles' lines: dbias needs it for its parts.
+template <int MODE, typename T>
+int run_rows(const RowProduct& g, TileParams p, bool launch_it, cudaStream_t stream) {
+    constexpr bool kGate = MODE == kGated || MODE == kGatedGrad;
+    const int sms = sm_count(g.device);
+    const int64_t n_cols = kGate ? 2 * p.n : p.n;
+    const uint32_t fixed = kFixedSmem<MODE> + table_bytes(g.groups);
+    p.kblocks = (int)((g.k + 63) / 64);
+    const Plan plan = plan_rows(g.a.rows, g.groups, n_cols, p.kblocks, kGate,
+                                p.act != RUNE_ACT_NONE, sms, fixed);
+    const int high = plan.pair ? 2 * kBM : kBM;
+    if (!launch_it) return high;
+    p.m = p.m_all = g.a.rows;
+    p.groups = (int)g.groups;
+    p.offsets = g.offsets;
+    p.bias_step = n_cols;
+    p.bn = plan.bn, p.stages = plan.stages;
+    p.splits = 1, p.kb_per_split = p.kblocks;
+    const int width = kGate ? p.bn / 2 : p.bn;
+    p.tiles_n = (int)((p.n + width - 1) / width);
+    p.by_tiles = make_divisor((unsigned)p.tiles_n);
+    p.by_group = make_divisor(kGroup * (unsigned)p.tiles_n);
+    p.b_mn = g.w_mn;
+    p.idesc = operand_idesc(g.dtype == RUNE_BF16 ? 1 : 0, false, g.w_mn, high, p.bn);
+    p.flag = wait_flag(g.device);
+    p.polls = wait_polls();
+    const CUtensorMap a = make_map(g.a, 2, kBM);
+    const CUtensorMap b =
+        g.w.map(g.groups, g.w_mn ? 64 : plan.pair || kGate ? p.bn / 2 : p.bn);
+    CUtensorMap o = a, o2 = a;  // unused unless the output goes by TMA
+    if (p.tma_out) {
+        o = make_out_map(p.out, p.m_all, p.n, p.ld_out);
+        if (MODE == kGatedGrad)
+            o2 = make_out_map(static_cast<T*>(p.out) + p.n, p.m_all, p.n, p.ld_out);
+    }
+    launch_kind<MODE, kRowGroups, T>(plan.pair, a, b, o, o2, p,
+                                     line_bound(p.m_all, g.groups, high) * p.tiles_n, fixed, sms,
+                                     g.device, stream);
+    return high;
+}
+
+int run_rows(int mode, const RowProduct& g, const TileParams& p, bool launch_it,
+             cudaStream_t stream) {
+    auto typed = [&](auto t) {
+        using T = decltype(t);
+        switch (mode) {
+            case kForward: return run_rows<kForward, T>(g, p, launch_it, stream);
+            case kGated: return run_rows<kGated, T>(g, p, launch_it, stream);
+            case kGrad: return run_rows<kGrad, T>(g, p, launch_it, stream);
+            default: return run_rows<kGatedGrad, T>(g, p, launch_it, stream);
+        }
+    };
+    return g.dtype == RUNE_F16 ? typed(__half()) : typed(__nv_bfloat16());
+}
+
+void forward(const rune_grouped_linear_args& a, Scratch& ws, cudaStream_t stream) {
+    const int64_t n_all = a.gated ? 2 * a.outputs : a.outputs;
+    RowProduct g;
+    g.a = readable({a.x, a.rows, a.inputs, a.x_stride}, 2, ws, stream);
+    g.w = {readable({a.weight, a.groups * n_all, a.inputs, a.weight_stride}, 2, ws, stream), n_all};
+    if (ws.sizing()) return;
+    g.k = a.inputs, g.groups = a.groups;
+    g.offsets = a.offsets;
+    g.device = a.device, g.dtype = a.dtype;
+    TileParams p{};
+    p.n = a.outputs;
+    p.act = a.activation;
+    p.out = a.y, p.ld_out = a.outputs;
+    p.tma_out = wide16(a.y, a.outputs, a.outputs);
+    p.zero_tail = 1;
+    p.bias = a.bias;
+    p.vec_bias = aligned(a.bias, 16) && a.outputs % 8 == 0;
+    run_rows(a.gated ? kGated : kForward, g, p, true, stream);
+}
+
+template <typename T>
+void run_depth(const rune_grouped_linear_grad_args& a, const Matrix& dz, const Matrix& x,
+               Scratch& ws, cudaStream_t stream) {
+    const int64_t m = dz.cols, n = x.cols;
+    const int sms = sm_count(a.device);
+    const uint32_t fixed =
+        std::max(kFixedSmem<kForward>, kFixedSmem<kPartial>) + table_bytes(a.groups);
+    const Plan plan = plan_depth(a.rows, a.groups, m, n, sms, fixed);
+    const int64_t ld = (n + 3) / 4 * 4;
+    auto* maps = ws.take<CUtensorMap>(2 * a.groups);
+    float* part = plan.splits > 1 ? ws.take<float>(plan.splits * a.groups * m * ld) : nullptr;
+    if (ws.sizing()) return;
+    const CUtensorMap ma = make_map(dz, 2, 64), mb = make_map(x, 2, 64);
+    const MapParams mp{a.offsets,
+                       a.rows,
+                       (int)a.groups,
+                       static_cast<const char*>(dz.p),
+                       static_cast<const char*>(x.p),
+                       dz.ld * 2,
+                       x.ld * 2,
+                       maps};
+    launch(k_group_maps, (unsigned)((2 * a.groups + kMapWarps - 1) / kMapWarps), 32 * kMapWarps, 0,
+           0, stream, ma, mb, mp);
+    TileParams p{};
+    p.m = m, p.n = n;
+    p.act = RUNE_ACT_NONE;
+    p.m_all = a.rows, p.groups = (int)a.groups, p.offsets = a.offsets;
+    p.group_maps = maps;
+    p.bn = plan.bn, p.stages = plan.stages, p.splits = plan.splits;
+    const int high = plan.pair ? 2 * kBM : kBM;
+    p.tiles_m = (int)((m + high - 1) / high);
+    p.tiles_n = (int)((n + p.bn - 1) / p.bn);
+    p.by_tiles = make_divisor((unsigned)p.tiles_m * p.tiles_n);
+    p.by_group = make_divisor(kGroup * (unsigned)p.tiles_n);
+    p.by_last = make_divisor(std::max(1u, (unsigned)p.tiles_m % kGroup));
+    p.a_mn = p.b_mn = 1;
+    p.idesc = operand_idesc(a.dtype == RUNE_BF16 ? 1 : 0, true, true, high, p.bn);
+    p.flag = wait_flag(a.device);
+    p.polls = wait_polls();
+    const int64_t work = (int64_t)p.tiles_m * p.tiles_n * p.splits * a.groups;
+    if (plan.splits == 1) {
+        p.out = a.dweight, p.ld_out = n, p.out_step = m * n;
+        p.tma_out = wide16(a.dweight, n, n);
+        const CUtensorMap o =
+            p.tma_out ? make_out_map3(a.dweight, m, n, n, a.groups, m * n) : ma;
+        launch_kind<kForward, kDepthGroups, T>(plan.pair, ma, mb, o, o, p, work, fixed, sms,
+                                               a.device, stream);
+        return;
+    }
+    p.z = part, p.ld_z = ld;
+    launch_kind<kPartial, kDepthGroups, __half>(plan.pair, ma, mb, ma, ma, p, work, fixed, sms,
+                                                a.device, stream);
+    const int64_t items = a.groups * m * (ld / 4);
+    launch(k_join_depth<T>, (unsigned)std::min<int64_t>((items + 255) / 256, (int64_t)sms * 16),
+           256, 0, 0, stream, part, plan.splits, a.groups * m, n, ld,
+           n % 4 == 0 && aligned(a.dweight, 8), static_cast<T*>(a.dweight));
+}
+
+void backward(const rune_grouped_linear_grad_args& a, Scratch& ws, cudaStream_t stream) {
+    const int64_t n_all = a.gated ? 2 * a.outputs : a.outputs;
+    const bool plain = !a.gated && a.activation == RUNE_ACT_NONE;
+    const bool half = a.dtype == RUNE_F16;
+    Matrix x{a.x, a.rows, a.inputs, a.x_stride};
+    Weights w{{a.weight, a.groups * n_all, a.inputs, a.weight_stride}, n_all};
+    if (!plain || a.dweight) x = readable(x, 2, ws, stream);
+    if (!plain || a.dx) w.all = readable(w.all, 2, ws, stream);
+    RowProduct g;
+    g.groups = a.groups, g.offsets = a.offsets;
+    g.device = a.device, g.dtype = a.dtype;
+    Matrix dz{a.dy, a.rows, n_all, a.dy_stride};
+    SumParams sum{a.offsets, a.rows, n_all, (int)a.groups, 0, 0, a.dy_stride, a.dy, nullptr,
+                  a.dbias};
+    if (plain) {
+        if (a.dx || a.dweight) dz = readable(dz, 2, ws, stream);
+        sum.high = 64, sum.each = 1;
+    } else {
+        dz.ld = pad16(n_all, 2);
+        dz.p = ws.take<uint16_t>(a.rows * dz.ld);
+        g.a = x, g.w = w, g.k = a.inputs;
+    }
+    TileParams p{};
+    if (!plain) {
+        p.n = a.outputs;
+        p.act = a.activation;
+        p.out = const_cast<void*>(dz.p), p.ld_out = dz.ld;
+        p.tma_out = !a.gated || a.outputs % 8 == 0;
+        p.in = a.dy, p.ld_in = a.dy_stride;
+        p.vec_in = wide16(a.dy, a.dy_stride, a.outputs);
+        p.bias = a.bias;
+        p.vec_bias = aligned(a.bias, 16) && a.outputs % 8 == 0;
+        sum.high = run_rows(a.gated ? kGatedGrad : kGrad, g, p, false, stream);
+        sum.each = sum.high / 32;  // one a warp
+    }
+    if (a.dbias)
+        sum.parts =
+            ws.take<float>(line_bound(a.rows, a.groups, sum.high) * sum.each * n_all);
+    const uint32_t table = table_bytes(a.groups);
+    const int sms = sm_count(a.device);
+    if (!ws.sizing()) {
+        if (!plain) {
+            p.colsum = sum.parts;
+            run_rows(a.gated ? kGatedGrad : kGrad, g, p, true, stream);
+        } else if (a.dbias) {
+            const dim3 grid((unsigned)((n_all + 63) / 64),
+                            (unsigned)std::min<int64_t>(
+                                line_bound(a.rows, a.groups, sum.high), 8 * sms));
+            if (half) launch(k_group_columns<__half>, grid, 256, table, 0, stream, sum);
+            else launch(k_group_columns<__nv_bfloat16>, grid, 256, table, 0, stream, sum);
+        }
+        if (a.dbias) {
+            const dim3 grid((unsigned)((n_all + 31) / 32), (unsigned)a.groups);
+            if (half) launch(k_group_sums<__half>, grid, 1024, table, 0, stream, sum);
+            else launch(k_group_sums<__nv_bfloat16>, grid, 1024, table, 0, stream, sum);
+        }
+        RUNE_LAUNCH_CHECK();
+    } else if (!plain) {
+        dz.p = reinterpret_cast<const void*>(256);
+    }
+    if (a.dx && !ws.sizing()) {
+        RowProduct d = g;
+        d.a = dz, d.w = w, d.w_mn = true;
+        d.k = n_all;
+        TileParams q{};
+        q.n = a.inputs;
+        q.act = RUNE_ACT_NONE;
+        q.out = a.dx, q.ld_out = a.inputs;
+        q.tma_out = wide16(a.dx, a.inputs, a.inputs);
+        q.zero_tail = 1;
+        run_rows(kForward, d, q, true, stream);
+    }
+    if (a.dweight) {
+        if (half) run_depth<__half>(a, dz, x, ws, stream);
+        else run_depth<__nv_bfloat16>(a, dz, x, ws, stream);
+    }
+}
+
+template <typename Args>
+void check_args(const Args& a) {
+    require(a.rows >= 0 && a.rows <= kMaxSize, "rows out of range");
+    require(a.groups >= 1 && a.groups <= kMaxGroups, "groups out of range: 1 to 1024");
+    require(a.inputs >= 1 && a.inputs <= kMaxSize && a.outputs >= 1 && a.outputs <= kMaxSize / 2,
+            "inputs or outputs out of range");
+    require(a.outputs * 2 <= kMaxSize / a.groups, "groups times outputs out of range");
+    require(a.activation == RUNE_ACT_NONE || a.activation == RUNE_ACT_TANH ||
+                a.activation == RUNE_ACT_SILU || a.activation == RUNE_ACT_GELU,
+            "unknown activation");
+    require(!a.gated || a.activation != RUNE_ACT_NONE, "a gated layer needs an activation");
+    require(a.dtype == RUNE_F16 || a.dtype == RUNE_BF16,
+            "a grouped layer takes float16 or bfloat16 operands");
+    require(a.rows == 0 || (a.x && a.weight && a.offsets), "null argument");
+    require_aligned({a.x, a.weight, a.bias}, 2);
+    require_aligned({a.offsets}, 4);
+}
+
+template <typename Args>
+Scratch carve(const Args& a, int64_t need) {
+    require(need == 0 || (a.workspace && aligned(a.workspace, 256) && a.workspace_bytes >= need),
+            "the workspace is too small or not 256-byte aligned");
+    return {need ? static_cast<char*>(a.workspace) : reinterpret_cast<char*>(256)};
+}
+
+}  // namespace
+}  // namespace ops
+}  // namespace rune
+
+using namespace rune;
+using namespace rune::ops;
+
+extern "C" {
+
+int rune_grouped_linear_workspace(const rune_grouped_linear_args* args, int64_t* bytes) {
+    if (!args || !bytes) {
+        set_error("null argument");
+        return RUNE_ERR_INVALID;
+    }
+    const rune_grouped_linear_args a = *args;
+    return guarded(a.device, [&] {
+        check_args(a);
+        Scratch ws{nullptr};
+        if (a.rows > 0) forward(a, ws, nullptr);
+        *bytes = ws.off;
+    });
+}
+
+int rune_grouped_linear(const rune_grouped_linear_args* args, void* stream_) {
+    if (!args) {
+        set_error("null argument");
+        return RUNE_ERR_INVALID;
+    }
+    const rune_grouped_linear_args a = *args;
+    auto stream = static_cast<cudaStream_t>(stream_);
+    return guarded(a.device, [&] {
+        check_args(a);
+        require_aligned({a.y}, 2);
+        check_waits(a.device);
+        if (a.rows == 0) return;
+        require(a.y, "null argument");
+        Scratch need{nullptr};
+        forward(a, need, stream);
+        if (need.off > 0 && !a.workspace)
+            throw Error(RUNE_ERR_RETRY, "the call needs a workspace");
+        Scratch ws = carve(a, need.off);
+        forward(a, ws, stream);
+        RUNE_LAUNCH_CHECK();
+    });
+}
+
+int rune_grouped_linear_backward_workspace(const rune_grouped_linear_grad_args* args,
+                                           int64_t* bytes) {
+    if (!args || !bytes) {
+        set_error("null argument");
+        return RUNE_ERR_INVALID;
+    }
+    const rune_grouped_linear_grad_args a = *args;
+    return guarded(a.device, [&] {
+        check_args(a);
+        Scratch ws{nullptr};
+        if (a.rows > 0) backward(a, ws, nullptr);
+        *bytes = ws.off;
+    });
+}
+
+int rune_grouped_linear_backward(const rune_grouped_linear_grad_args* args, void* stream_) {
+    if (!args) {
+        set_error("null argument");
+        return RUNE_ERR_INVALID;
+    }
+    const rune_grouped_linear_grad_args a = *args;
+    auto stream = static_cast<cudaStream_t>(stream_);
+    return guarded(a.device, [&] {
+        check_args(a);
+        require_aligned({a.dy, a.dx, a.dweight, a.dbias}, 2);
+        check_waits(a.device);
+        const int64_t n_all = a.gated ? 2 * a.outputs : a.outputs;
+        if (a.rows == 0) {
+            if (a.dweight)
+                RUNE_CUDA_TRY(cudaMemsetAsync(
+                    a.dweight, 0, (size_t)(a.groups * n_all * a.inputs * 2), stream));
+            if (a.dbias)
+                RUNE_CUDA_TRY(
+                    cudaMemsetAsync(a.dbias, 0, (size_t)(a.groups * n_all * 2), stream));
+            return;
+        }
+        require(a.dy, "null argument");
+        Scratch need{nullptr};
+        backward(a, need, stream);
+        Scratch ws = carve(a, need.off);
+        backward(a, ws, stream);
+        RUNE_LAUNCH_CHECK();
+    });
+}
+
+}  // extern "C"

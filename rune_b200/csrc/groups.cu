@@ -1,0 +1,832 @@
+// Rows by group: the choice of groups (route), the stable sort of rows by group (row_groups), and the
+// moves of rows into that order and back (to_groups, from_groups) with their gradients. Groups are
+// elements with a network each (rune/nep/model.py:157-170 loops over them) or experts.
+//
+//   route        the k largest of a row's logits, ties to the lowest index, and their softmax
+//                w_j = e^(l_j - l_0) / sum_i e^(l_i - l_0);   dl_j = w_j (dw_j - sum_i w_i dw_i)
+//   row_groups   slot s = (row, choice) of group g(s) goes to place(s) = #{t: g(t) < g(s)} +
+//                #{t < s: g(t) = g(s)}; order is the inverse, offsets the groups' first places
+//   to_groups    xs[p] = x[order(p) / k];                 dx[r] = sum_j dxs[place(r, j)]
+//   from_groups  out[r] = sum_j w[r, j] y[place(r, j)];   dy[p] = w[order(p)] dout[order(p) / k],
+//                dw[r, j] = <dout[r], y[place(r, j)]>
+//
+// All are bound by memory or, small, by latency. Every gradient of a move is the other move read by
+// its own index, so nothing is added by atomics and equal inputs give equal bits. Slots without a
+// group have place -1; the places behind the last group have order -1 and rows of zeros. Indexes
+// are checked where they are used: a wrong order or place selects nothing and reads nothing.
+
+#include <algorithm>
+#include <atomic>
+
+#include "ops.cuh"
+
+namespace rune {
+namespace ops {
+
+namespace {
+
+constexpr int kMaxGroups = 1024, kMaxChoices = 32;
+
+// ------------------------------------------------------------------------------------ route
+// Orders as the values do: NaN above all, -0 as 0.
+__device__ __forceinline__ uint32_t order_key(float v) {
+    const uint32_t u = __float_as_uint(v + 0.0f);
+    if (v != v) return 0xffffffffu;
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+constexpr uint32_t kKeyMasked = 0x007fffffu;  // of -inf
+
+template <typename T>
+struct RouteParams {
+    int64_t rows, ld;
+    int groups, k;
+    const T* logits;
+    int32_t* index;
+    float* weights;
+};
+
+// A warp per row; a lane has the values lane, lane + 32, ... A round of the selection is a maximum
+// over the warp and the lowest index that has it, both by one reduction instruction.
+template <typename T, int PER>
+__global__ void __launch_bounds__(256) k_route(const RouteParams<T> p) {
+    follow_on();
+    const int lane = threadIdx.x & 31;
+    for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < p.rows;
+         row += (int64_t)gridDim.x * 8) {
+        const T* at = p.logits + row * p.ld;
+        uint32_t key[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int g = lane + 32 * i;
+            key[i] = g < p.groups ? order_key(to_float(at[g])) : 0u;
+        }
+        uint32_t mine = 0;
+        int chosen = -1;
+        for (int j = 0; j < p.k; ++j) {
+            uint32_t top = key[0];
+#pragma unroll
+            for (int i = 1; i < PER; ++i) top = max(top, key[i]);
+            top = __reduce_max_sync(0xffffffffu, top);
+            uint32_t first = 0xffffffffu;
+#pragma unroll
+            for (int i = PER - 1; i >= 0; --i)
+                if (key[i] == top) first = lane + 32 * i;
+            first = __reduce_min_sync(0xffffffffu, first);
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (first == lane + 32 * i) key[i] = 0u;
+            if (lane == j) mine = top, chosen = (int)first;
+        }
+        const float value = mine == 0xffffffffu
+                                ? __uint_as_float(0x7fc00000u)
+                                : __uint_as_float(mine & 0x80000000u ? mine ^ 0x80000000u : ~mine);
+        const float largest = __shfl_sync(0xffffffffu, value, 0);
+        const bool some = lane < p.k && mine != kKeyMasked;  // -inf: not to be chosen
+        const float e = some ? expf(value - largest) : 0.0f;
+        const float sum = warp_sum(e);
+        if (lane < p.k) {
+            p.index[row * p.k + lane] = some ? chosen : -1;
+            p.weights[row * p.k + lane] = some ? e / sum : 0.0f;
+        }
+    }
+}
+
+template <typename T>
+struct RouteGradParams {
+    int64_t rows;
+    int groups, k;
+    bool wide;  // rows of dlogits on 16 bytes
+    const int32_t* index;
+    const float* weights;
+    const float* dweights;
+    T* dlogits;
+};
+
+// A warp per row: zeros, then the chosen ones' gradients over them.
+template <typename T>
+__global__ void __launch_bounds__(256) k_route_grad(const RouteGradParams<T> p) {
+    follow_on();
+    const int lane = threadIdx.x & 31;
+    for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < p.rows;
+         row += (int64_t)gridDim.x * 8) {
+        int g = -1;
+        float w = 0.0f, d = 0.0f;
+        if (lane < p.k) {
+            g = p.index[row * p.k + lane];
+            w = p.weights[row * p.k + lane];
+            d = p.dweights[row * p.k + lane];
+        }
+        const float dot = warp_sum(g >= 0 ? w * d : 0.0f);
+        T* out = p.dlogits + row * p.groups;
+        if (p.wide) {
+            const int pieces = p.groups * (int)sizeof(T) / 16;
+            for (int i = lane; i < pieces; i += 32)
+                reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
+        } else {
+            for (int i = lane; i < p.groups; i += 32) out[i] = from_float<T>(0.0f);
+        }
+        __syncwarp();
+        if (g >= 0 && g < p.groups) out[g] = from_float<T>(w * (d - dot));
+    }
+}
+
+// ------------------------------------------------------------------------------------ sort
+// Each warp of each block owns a range of slots, in order. k_count leaves the blocks' counts of
+// each group; k_place adds up those before its own, then walks its slots again: a slot's rank
+// among the warp's 32 comes from the lanes that match it. One block alone needs no first kernel.
+constexpr int kSortWarps = 16, kSortThreads = 32 * kSortWarps;
+constexpr int64_t kSortAlone = 16384;  // slots that one block sorts by itself
+
+struct SortParams {
+    int64_t slots, per_warp;
+    int groups, blocks;
+    const void* index;
+    int32_t* counts;  // [blocks][groups]
+    int32_t *offsets, *order, *place;
+};
+
+// group of a slot, or -1
+template <typename I>
+__device__ __forceinline__ int group_of(const SortParams& p, int64_t slot) {
+    const I g = static_cast<const I*>(p.index)[slot];
+    return g >= 0 && g < p.groups ? (int)g : -1;
+}
+
+// this warp's counts into hist[warp][groups] and the block's sums into total[groups]
+template <typename I>
+__device__ __forceinline__ void count_slots(const SortParams& p, int32_t* hist, int32_t* total) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int32_t* own = hist + warp * p.groups;
+    for (int i = lane; i < p.groups; i += 32) own[i] = 0;
+    __syncwarp();
+    const int64_t first = ((int64_t)blockIdx.x * kSortWarps + warp) * p.per_warp;
+    const int64_t last = min(first + p.per_warp, p.slots);
+    constexpr int kAhead = 4;
+    for (int64_t s = first; s < last; s += 32 * kAhead) {
+        int g[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int64_t slot = s + 32 * i + lane;
+            g[i] = slot < last ? group_of<I>(p, slot) : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const unsigned same = __match_any_sync(0xffffffffu, g[i]);
+            if (g[i] >= 0 && lane == __ffs(same) - 1) own[g[i]] += __popc(same);
+            __syncwarp();
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.groups; i += kSortThreads) {
+        int sum = 0;
+#pragma unroll
+        for (int w = 0; w < kSortWarps; ++w) sum += hist[w * p.groups + i];
+        total[i] = sum;
+    }
+}
+
+template <typename I>
+__global__ void __launch_bounds__(kSortThreads) k_count(const SortParams p) {
+    follow_on();
+    extern __shared__ int32_t words[];
+    count_slots<I>(p, words, p.counts + (int64_t)blockIdx.x * p.groups);
+}
+
+template <typename I>
+__global__ void __launch_bounds__(kSortThreads) k_place(const SortParams p) {
+    follow_on();
+    extern __shared__ int32_t words[];
+    int32_t* hist = words;                           // [warps][groups]
+    int32_t* base = hist + kSortWarps * p.groups;    // [groups]: first place of this block's slots
+    int32_t* total = base + p.groups;                // [groups]
+    __shared__ int32_t sums[kSortWarps + 1];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    count_slots<I>(p, hist, base);
+    __syncthreads();
+    if (p.blocks == 1) {
+        for (int i = tid; i < p.groups; i += kSortThreads) total[i] = base[i], base[i] = 0;
+    } else {
+        // `parts` threads add up a group's counts, in ranges of blocks
+        for (int i = tid; i < p.groups; i += kSortThreads) total[i] = 0, base[i] = 0;
+        __syncthreads();
+        int width = 1;
+        while (width < p.groups) width *= 2;
+        const int parts = max(1, kSortThreads / width), step = kSortThreads / parts;
+        for (int g = tid % step; g < p.groups; g += step) {
+            int before = 0, all = 0;
+#pragma unroll 8
+            for (int b = tid / step; b < p.blocks; b += parts) {
+                const int c = p.counts[(int64_t)b * p.groups + g];
+                all += c;
+                before += b < (int)blockIdx.x ? c : 0;
+            }
+            atomicAdd(&total[g], all);  // whole numbers: their order does not matter
+            atomicAdd(&base[g], before);
+        }
+    }
+    __syncthreads();
+    // exclusive sums over the groups: two of them a thread
+    const int g0 = 2 * tid, a = g0 < p.groups ? total[g0] : 0;
+    const int b = g0 + 1 < p.groups ? total[g0 + 1] : 0;
+    int sum = a + b;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const int other = __shfl_up_sync(0xffffffffu, sum, o);
+        sum += lane >= o ? other : 0;
+    }
+    if (lane == 31) sums[warp] = sum;
+    __syncthreads();
+    if (warp == 0) {
+        int s = lane < kSortWarps ? sums[lane] : 0;
+        const int own = s;
+#pragma unroll
+        for (int o = 1; o < kSortWarps; o *= 2) {
+            const int other = __shfl_up_sync(0xffffffffu, s, o);
+            s += lane >= o ? other : 0;
+        }
+        if (lane < kSortWarps) sums[lane] = s - own;
+        if (lane == kSortWarps - 1) sums[kSortWarps] = s;
+    }
+    __syncthreads();
+    const int before = sums[warp] + sum - a - b;
+    if (g0 < p.groups) base[g0] += before;
+    if (g0 + 1 < p.groups) base[g0 + 1] += before + a;
+    if (blockIdx.x == 0) {
+        if (g0 < p.groups) p.offsets[g0] = before;
+        if (g0 + 1 < p.groups) p.offsets[g0 + 1] = before + a;
+        if (tid == 0) p.offsets[p.groups] = sums[kSortWarps];
+    }
+    __syncthreads();
+    for (int i = tid; i < p.groups; i += kSortThreads) {  // counts to first places of the warps
+        int at = base[i];
+#pragma unroll
+        for (int w = 0; w < kSortWarps; ++w) {
+            const int c = hist[w * p.groups + i];
+            hist[w * p.groups + i] = at;
+            at += c;
+        }
+    }
+    __syncthreads();
+    int32_t* own = hist + warp * p.groups;
+    const int64_t first = ((int64_t)blockIdx.x * kSortWarps + warp) * p.per_warp;
+    const int64_t last = min(first + p.per_warp, p.slots);
+    constexpr int kAhead = 4;
+    for (int64_t s = first; s < last; s += 32 * kAhead) {
+        int g[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int64_t slot = s + 32 * i + lane;
+            g[i] = slot < last ? group_of<I>(p, slot) : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int64_t slot = s + 32 * i + lane;
+            const unsigned same = __match_any_sync(0xffffffffu, g[i]);
+            int at = -1;
+            if (g[i] >= 0) at = own[g[i]] + __popc(same & ((1u << lane) - 1));
+            __syncwarp();
+            if (g[i] >= 0 && lane == __ffs(same) - 1) own[g[i]] += __popc(same);
+            __syncwarp();
+            if (slot < last) p.place[slot] = at;
+            if (at >= 0) p.order[at] = (int32_t)slot;
+        }
+    }
+    // the places behind the last group
+    for (int64_t at = sums[kSortWarps] + (int64_t)blockIdx.x * kSortThreads + tid; at < p.slots;
+         at += (int64_t)gridDim.x * kSortThreads)
+        p.order[at] = -1;
+}
+
+// ------------------------------------------------------------------------------------ moves
+// N values of T in one access of N * sizeof(T) bytes.
+template <typename T, int N>
+struct Piece {
+    static constexpr int kBytes = N * (int)sizeof(T);
+    static_assert(kBytes == 2 || kBytes == 4 || kBytes == 8 || kBytes == 16, "one access");
+    using Raw = std::conditional_t<
+        kBytes == 16, uint4,
+        std::conditional_t<kBytes == 8, uint2,
+                           std::conditional_t<kBytes == 4, uint32_t, uint16_t>>>;
+    union {
+        Raw raw;
+        uint16_t half[kBytes / 2];
+        uint32_t word[kBytes / 4 ? kBytes / 4 : 1];
+    };
+    __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const Raw*>(p); }
+    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Raw*>(p) = raw; }
+    __device__ __forceinline__ void clear() { raw = Raw{}; }
+    __device__ __forceinline__ void get(float (&v)[N]) const {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = __uint_as_float(word[i]);
+        } else if constexpr (N == 1) {
+            v[0] = to_float(*reinterpret_cast<const T*>(&half[0]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) {
+                const float2 f = unpack2<T>(word[i]);
+                v[2 * i] = f.x, v[2 * i + 1] = f.y;
+            }
+        }
+    }
+    __device__ __forceinline__ void set(const float (&v)[N]) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) word[i] = __float_as_uint(v[i]);
+        } else if constexpr (N == 1) {
+            const T t = from_float<T>(v[0]);
+            half[0] = *reinterpret_cast<const uint16_t*>(&t);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) word[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+        }
+    }
+};
+
+struct MoveParams {
+    int64_t rows, slots;       // slots = rows * k
+    int64_t ld_in, ld_more;
+    int width, k;
+    const void* in;            // to_groups: x; from_groups: y; its gradient: dout
+    const void* more;          // the gradient's y
+    const int32_t *order, *place;
+    const float* weights;      // [slots] or null
+    void* out;                 // contiguous
+    float* dweights;           // [slots]
+};
+
+// Items are (output row, `lanes` pieces of it); a team of `lanes` lanes has one, kItems of them at a
+// time, so that a row's index and then its pieces are under way for several rows at once.
+constexpr int kItems = 4, kMoveThreads = 256;
+
+template <typename T, int N, bool SCALED>
+__global__ void __launch_bounds__(kMoveThreads)
+k_to_groups(const MoveParams p, int lanes, int chunks) {
+    follow_on();
+    const int team = threadIdx.x / lanes, at = threadIdx.x % lanes;
+    const int teams = kMoveThreads / lanes;
+    const int64_t items = p.slots * chunks;
+    for (int64_t i0 = ((int64_t)blockIdx.x * kItems) * teams + team; i0 < items;
+         i0 += (int64_t)gridDim.x * kItems * teams) {
+        int64_t row[kItems];
+        int col[kItems], slot[kItems];
+        float w[kItems];
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+            const int64_t item = i0 + (int64_t)i * teams;
+            row[i] = chunks == 1 ? item : item / chunks;
+            col[i] = ((int)(item - row[i] * chunks) * lanes + at) * N;
+            if (item >= items || col[i] >= p.width) row[i] = -1;
+            slot[i] = row[i] >= 0 ? p.order[row[i]] : -1;
+            if (slot[i] >= p.slots) slot[i] = -1;
+        }
+        if constexpr (SCALED) {
+#pragma unroll
+            for (int i = 0; i < kItems; ++i) w[i] = slot[i] >= 0 ? p.weights[slot[i]] : 0.0f;
+        }
+        Piece<T, N> v[kItems];
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+            v[i].clear();
+            if (slot[i] >= 0)
+                v[i].load(static_cast<const T*>(p.in) + (int64_t)(slot[i] / p.k) * p.ld_in + col[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+            if constexpr (SCALED) {
+                float f[N];
+                v[i].get(f);
+#pragma unroll
+                for (int j = 0; j < N; ++j) f[j] = slot[i] >= 0 ? f[j] * w[i] : 0.0f;
+                v[i].set(f);
+            }
+            if (row[i] >= 0) v[i].store(static_cast<T*>(p.out) + row[i] * p.width + col[i]);
+        }
+    }
+}
+
+template <typename T, int N>
+__global__ void __launch_bounds__(kMoveThreads)
+k_from_groups(const MoveParams p, int lanes, int chunks) {
+    follow_on();
+    const int team = threadIdx.x / lanes, at = threadIdx.x % lanes;
+    const int teams = kMoveThreads / lanes;
+    const int64_t items = p.rows * chunks;
+    constexpr int kAhead = 4;  // choices whose pieces are under way at once
+    for (int64_t item = (int64_t)blockIdx.x * teams + team; item < items;
+         item += (int64_t)gridDim.x * teams) {
+        const int64_t row = chunks == 1 ? item : item / chunks;
+        const int col = ((int)(item - row * chunks) * lanes + at) * N;
+        if (col >= p.width) continue;
+        float sum[N] = {};
+        for (int j0 = 0; j0 < p.k; j0 += kAhead) {
+            int place[kAhead];
+            float w[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                place[j] = j0 + j < p.k ? p.place[row * p.k + j0 + j] : -1;
+                if (place[j] >= p.slots) place[j] = -1;
+                w[j] = 1.0f;
+                if (p.weights && place[j] >= 0) w[j] = p.weights[row * p.k + j0 + j];
+            }
+            Piece<T, N> v[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j)
+                if (place[j] >= 0)
+                    v[j].load(static_cast<const T*>(p.in) + place[j] * p.ld_in + col);
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                if (place[j] < 0) continue;
+                float f[N];
+                v[j].get(f);
+#pragma unroll
+                for (int i = 0; i < N; ++i) sum[i] = fmaf(f[i], w[j], sum[i]);
+            }
+        }
+        Piece<T, N> o;
+        o.set(sum);
+        o.store(static_cast<T*>(p.out) + row * p.width + col);
+    }
+}
+
+// A warp per slot: dy of its place and the weight's gradient; the slots of one row follow one
+// another, so that dout comes from L1 after the first. The warp also clears the row of dy that is
+// nobody's place.
+template <typename T, int N>
+__global__ void __launch_bounds__(kMoveThreads) k_from_groups_grad(const MoveParams p) {
+    follow_on();
+    const int lane = threadIdx.x & 31;
+    constexpr int kWarps = kMoveThreads / 32, kAhead = 4;
+    const int pieces = p.width / N;
+    for (int64_t slot = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); slot < p.slots;
+         slot += (int64_t)gridDim.x * kWarps) {
+        int64_t place = p.place[slot];
+        if (place >= p.slots) place = -1;
+        const int owner = p.order[slot];
+        const float w = p.weights[slot];
+        T* dy = static_cast<T*>(p.out);
+        if (dy && (owner < 0 || owner >= p.slots)) {
+            Piece<T, N> zero;
+            zero.clear();
+            for (int i = lane; i < pieces; i += 32) zero.store(dy + slot * p.width + i * N);
+        }
+        float dot = 0.0f;
+        if (place >= 0) {
+            const T* dout = static_cast<const T*>(p.in) + slot / p.k * p.ld_in;
+            const T* y = static_cast<const T*>(p.more) + place * p.ld_more;
+            for (int i0 = lane; i0 < pieces; i0 += 32 * kAhead) {
+                Piece<T, N> a[kAhead], b[kAhead];
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    a[i].clear(), b[i].clear();
+                    if (i0 + 32 * i >= pieces) continue;
+                    a[i].load(dout + (i0 + 32 * i) * N);
+                    if (p.dweights) b[i].load(y + (i0 + 32 * i) * N);
+                }
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    float f[N], h[N];
+                    a[i].get(f), b[i].get(h);
+                    if (i0 + 32 * i < pieces) {
+#pragma unroll
+                        for (int j = 0; j < N; ++j) {
+                            dot = fmaf(f[j], h[j], dot);
+                            f[j] *= w;
+                        }
+                        if (dy) {
+                            a[i].set(f);
+                            a[i].store(dy + place * p.width + (i0 + 32 * i) * N);
+                        }
+                    }
+                }
+            }
+        }
+        if (p.dweights) {
+            dot = warp_sum(dot);
+            if (lane == 0) p.dweights[slot] = place >= 0 ? dot : 0.0f;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------ host
+// values in one access: as many as divide every row's start and its width, 16 bytes at most
+int piece_values(int elem_bytes, int64_t width,
+                 std::initializer_list<std::pair<const void*, int64_t>> rows) {
+    int n = 16 / elem_bytes;
+    for (auto [p, ld] : rows)
+        while (n > 1 && p &&
+               ((uintptr_t)p % (n * elem_bytes) != 0 || ld % n != 0 || width % n != 0))
+            n /= 2;
+    return n;
+}
+
+// fn(T(), std::integral_constant<int, N>) for the type and the piece
+template <typename Fn>
+void with_piece(int dtype, int n, Fn&& fn) {
+    auto narrow = [&](auto t) {
+        switch (n) {
+            case 8: fn(t, std::integral_constant<int, 8>()); break;
+            case 4: fn(t, std::integral_constant<int, 4>()); break;
+            case 2: fn(t, std::integral_constant<int, 2>()); break;
+            default: fn(t, std::integral_constant<int, 1>()); break;
+        }
+    };
+    if (dtype == RUNE_F16) narrow(__half());
+    else if (dtype == RUNE_BF16) narrow(__nv_bfloat16());
+    else if (n == 4) fn(float(), std::integral_constant<int, 4>());
+    else if (n == 2) fn(float(), std::integral_constant<int, 2>());
+    else fn(float(), std::integral_constant<int, 1>());
+}
+
+template <typename Fn>
+void with_type(int dtype, Fn&& fn) {
+    if (dtype == RUNE_F16) fn(__half());
+    else if (dtype == RUNE_BF16) fn(__nv_bfloat16());
+    else fn(float());
+}
+
+struct Teams {
+    int lanes, chunks;
+    unsigned grid;
+};
+// lanes that share a row, chunks of a row, and the blocks for `rows` of them, `items` at a time
+Teams teams_of(int64_t rows, int pieces, int items, int device) {
+    int lanes = 1;
+    while (lanes < 32 && lanes < pieces) lanes *= 2;
+    const int chunks = (pieces + lanes - 1) / lanes, teams = kMoveThreads / lanes * items;
+    const int64_t blocks = (rows * chunks + teams - 1) / teams;
+    return {lanes, chunks, (unsigned)std::min<int64_t>(blocks, (int64_t)sm_count(device) * 32)};
+}
+
+bool value_type(int dtype) {
+    return dtype == RUNE_F32 || dtype == RUNE_F16 || dtype == RUNE_BF16;
+}
+
+void check_move(const rune_group_move_args& a) {
+    require(a.rows >= 0 && a.k >= 1 && a.rows <= (INT32_MAX - 1024) / a.k,
+            "rows or k out of range");
+    require(a.width >= 1 && a.width <= INT32_MAX / 2, "width out of range");
+    require(value_type(a.dtype), "rows are float32, float16 or bfloat16");
+    require_aligned({a.order, a.place, a.weights, a.dweights}, 4);
+    require_aligned({a.in, a.y, a.out}, dtype_bytes(a.dtype));
+}
+
+MoveParams move_params(const rune_group_move_args& a) {
+    MoveParams p{};
+    p.rows = a.rows, p.slots = a.rows * a.k;
+    p.ld_in = a.in_stride, p.ld_more = a.y_stride;
+    p.width = (int)a.width, p.k = (int)a.k;
+    p.in = a.in, p.more = a.y;
+    p.order = a.order, p.place = a.place;
+    p.weights = a.weights;
+    p.out = a.out, p.dweights = a.dweights;
+    return p;
+}
+
+int sort_blocks(const rune_row_groups_args& a) {
+    const int64_t slots = a.rows * a.k;
+    if (slots <= kSortAlone) return 1;
+    // a block for 1024 slots at least, and no more counts than every block can add up
+    return (int)std::max<int64_t>(
+        1, std::min({(slots + 1023) / 1024, (int64_t)sm_count(a.device),
+                     (int64_t)65536 / a.groups}));
+}
+
+void check_sort(const rune_row_groups_args& a) {
+    require(a.rows >= 0 && a.k >= 1 && a.rows <= (INT32_MAX - 1024) / a.k,
+            "rows or k out of range");
+    require(a.groups >= 1 && a.groups <= kMaxGroups, "groups out of range: 1 to 1024");
+    require(a.index_bytes == 4 || a.index_bytes == 8, "an index is int32 or int64");
+    require(a.offsets && (a.rows == 0 || (a.index && a.order && a.place)), "null argument");
+    require(aligned(a.index, a.index_bytes), "index does not start on a multiple of its size");
+    require_aligned({a.offsets, a.order, a.place}, 4);
+}
+
+void check_route(const rune_route_args& a) {
+    require(a.rows >= 0, "rows out of range");
+    require(a.groups >= 1 && a.groups <= kMaxGroups, "groups out of range: 1 to 1024");
+    require(a.k >= 1 && a.k <= kMaxChoices && a.k <= a.groups,
+            "k out of range: 1 to 32, and no more than there are groups");
+    require(a.rows <= (INT32_MAX - 1024) / a.k, "rows out of range");
+    require(value_type(a.dtype), "logits are float32, float16 or bfloat16");
+    require_aligned({a.logits, a.dlogits}, dtype_bytes(a.dtype));
+    require_aligned({a.index, a.weights, a.dweights}, 4);
+    require(a.rows == 0 || (a.index && a.weights), "null argument");
+}
+
+}  // namespace
+}  // namespace ops
+}  // namespace rune
+
+using namespace rune;
+using namespace rune::ops;
+
+extern "C" {
+
+int rune_route(const rune_route_args* args, void* stream_) {
+    if (!args) {
+        set_error("null argument");
+        return RUNE_ERR_INVALID;
+    }
+    const rune_route_args a = *args;
+    auto stream = static_cast<cudaStream_t>(stream_);
+    return guarded(a.device, [&] {
+        check_route(a);
+        check_waits(a.device);
+        if (a.rows == 0) return;
+        require(a.logits, "null argument");
+        const unsigned grid =
+            (unsigned)std::min<int64_t>((a.rows + 7) / 8, (int64_t)sm_count(a.device) * 16);
+        with_type(a.dtype, [&](auto t) {
+            using T = decltype(t);
+            const RouteParams<T> p{a.rows,   a.logits_stride,
+                                   (int)a.groups, (int)a.k,
+                                   static_cast<const T*>(a.logits), a.index, a.weights};
+            auto go = [&](auto per) {
+                launch(k_route<T, decltype(per)::value>, grid, 256, 0, 0, stream, p);
+            };
+            const int per = (int)((a.groups + 31) / 32);
+            if (per <= 1) go(std::integral_constant<int, 1>());
+            else if (per <= 2) go(std::integral_constant<int, 2>());
+            else if (per <= 4) go(std::integral_constant<int, 4>());
+            else if (per <= 8) go(std::integral_constant<int, 8>());
+            else if (per <= 16) go(std::integral_constant<int, 16>());
+            else go(std::integral_constant<int, 32>());
+        });
+        RUNE_LAUNCH_CHECK();
+    });
+}
+
+int rune_route_backward(const rune_route_args* args, void* stream_) {
+    if (!args) {
+        set_error("null argument");
+        return RUNE_ERR_INVALID;
+    }
+    const rune_route_args a = *args;
+    auto stream = static_cast<cudaStream_t>(stream_);
+    return guarded(a.device, [&] {
+        check_route(a);
+        check_waits(a.device);
+        if (a.rows == 0) return;
+        require(a.dweights && a.dlogits, "null argument");
+        const unsigned grid =
+            (unsigned)std::min<int64_t>((a.rows + 7) / 8, (int64_t)sm_count(a.device) * 16);
+        with_type(a.dtype, [&](auto t) {
+            using T = decltype(t);
+            const RouteGradParams<T> p{a.rows, (int)a.groups, (int)a.k,
+                                       aligned(a.dlogits, 16) && a.groups * sizeof(T) % 16 == 0,
+                                       a.index, a.weights, a.dweights,
+                                       static_cast<T*>(a.dlogits)};
+            launch(k_route_grad<T>, grid, 256, 0, 0, stream, p);
+        });
+        RUNE_LAUNCH_CHECK();
+    });
+}
+
+int rune_row_groups_workspace(const rune_row_groups_args* args, int64_t* bytes) {
+    if (!args || !bytes) {
+        set_error("null argument");
+        return RUNE_ERR_INVALID;
+    }
+    const rune_row_groups_args a = *args;
+    return guarded(a.device, [&] {
+        check_sort(a);
+        const int blocks = sort_blocks(a);
+        *bytes = blocks > 1 ? (int64_t)blocks * a.groups * 4 : 0;
+    });
+}
+
+int rune_row_groups(const rune_row_groups_args* args, void* stream_) {
+    if (!args) {
+        set_error("null argument");
+        return RUNE_ERR_INVALID;
+    }
+    const rune_row_groups_args a = *args;
+    auto stream = static_cast<cudaStream_t>(stream_);
+    return guarded(a.device, [&] {
+        check_sort(a);
+        check_waits(a.device);
+        SortParams p{};
+        p.slots = a.rows * a.k;
+        p.groups = (int)a.groups;
+        p.blocks = sort_blocks(a);
+        const int64_t warps = (int64_t)p.blocks * kSortWarps;
+        p.per_warp = ((p.slots + warps - 1) / warps + 31) / 32 * 32;
+        p.index = a.index;
+        p.offsets = a.offsets, p.order = a.order, p.place = a.place;
+        if (p.blocks > 1) {
+            require(a.workspace && aligned(a.workspace, 256) &&
+                        a.workspace_bytes >= (int64_t)p.blocks * p.groups * 4,
+                    "the workspace is too small or not 256-byte aligned");
+            p.counts = static_cast<int32_t*>(a.workspace);
+        }
+        const size_t count_smem = (size_t)kSortWarps * p.groups * 4;
+        const size_t place_smem = count_smem + (size_t)p.groups * 8;
+        auto go = [&](auto i) {
+            using I = decltype(i);
+            static std::atomic<uint64_t> allowed{0};  // devices whose limit is raised
+            if (a.device >= 64 || !(allowed.load(std::memory_order_relaxed) >> a.device & 1)) {
+                constexpr int most = (kSortWarps + 2) * kMaxGroups * 4;
+                for (auto kernel : {k_count<I>, k_place<I>})
+                    RUNE_CUDA_TRY(cudaFuncSetAttribute(
+                        kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+                if (a.device < 64)
+                    allowed.fetch_or(uint64_t(1) << a.device, std::memory_order_relaxed);
+            }
+            if (p.blocks > 1)
+                launch(k_count<I>, p.blocks, kSortThreads, count_smem, 0, stream, p);
+            launch(k_place<I>, p.blocks, kSortThreads, place_smem, 0, stream, p);
+        };
+        if (a.index_bytes == 8) go(int64_t());
+        else go(int32_t());
+        RUNE_LAUNCH_CHECK();
+    });
+}
+
+int rune_to_groups(const rune_group_move_args* args, void* stream_) {
+    if (!args) {
+        set_error("null argument");
+        return RUNE_ERR_INVALID;
+    }
+    const rune_group_move_args a = *args;
+    auto stream = static_cast<cudaStream_t>(stream_);
+    return guarded(a.device, [&] {
+        check_move(a);
+        check_waits(a.device);
+        if (a.rows == 0) return;
+        require(a.in && a.order && a.out, "null argument");
+        const MoveParams p = move_params(a);
+        const int n = piece_values(dtype_bytes(a.dtype), a.width,
+                                   {{a.in, a.rows > 1 ? a.in_stride : a.width}, {a.out, a.width}});
+        with_piece(a.dtype, n, [&](auto t, auto n_c) {
+            using T = decltype(t);
+            constexpr int N = decltype(n_c)::value;
+            const Teams team = teams_of(p.slots, (int)(a.width / N), kItems, a.device);
+            if (a.weights)
+                launch(k_to_groups<T, N, true>, team.grid, kMoveThreads, 0, 0, stream, p,
+                       team.lanes, team.chunks);
+            else
+                launch(k_to_groups<T, N, false>, team.grid, kMoveThreads, 0, 0, stream, p,
+                       team.lanes, team.chunks);
+        });
+        RUNE_LAUNCH_CHECK();
+    });
+}
+
+int rune_from_groups(const rune_group_move_args* args, void* stream_) {
+    if (!args) {
+        set_error("null argument");
+        return RUNE_ERR_INVALID;
+    }
+    const rune_group_move_args a = *args;
+    auto stream = static_cast<cudaStream_t>(stream_);
+    return guarded(a.device, [&] {
+        check_move(a);
+        check_waits(a.device);
+        if (a.rows == 0) return;
+        require(a.in && a.place && a.out, "null argument");
+        const MoveParams p = move_params(a);
+        const int n = piece_values(
+            dtype_bytes(a.dtype), a.width,
+            {{a.in, a.rows * a.k > 1 ? a.in_stride : a.width}, {a.out, a.width}});
+        with_piece(a.dtype, n, [&](auto t, auto n_c) {
+            using T = decltype(t);
+            constexpr int N = decltype(n_c)::value;
+            const Teams team = teams_of(p.rows, (int)(a.width / N), 1, a.device);
+            launch(k_from_groups<T, N>, team.grid, kMoveThreads, 0, 0, stream, p, team.lanes,
+                   team.chunks);
+        });
+        RUNE_LAUNCH_CHECK();
+    });
+}
+
+int rune_from_groups_backward(const rune_group_move_args* args, void* stream_) {
+    if (!args) {
+        set_error("null argument");
+        return RUNE_ERR_INVALID;
+    }
+    const rune_group_move_args a = *args;
+    auto stream = static_cast<cudaStream_t>(stream_);
+    return guarded(a.device, [&] {
+        check_move(a);
+        check_waits(a.device);
+        if (a.rows == 0) return;
+        require(a.in && a.order && a.place && a.weights && (a.out || a.dweights) &&
+                    (a.y || !a.dweights),
+                "null argument");
+        const MoveParams p = move_params(a);
+        const int n = piece_values(dtype_bytes(a.dtype), a.width,
+                                   {{a.in, a.rows > 1 ? a.in_stride : a.width},
+                                    {a.y, a.rows * a.k > 1 ? a.y_stride : a.width},
+                                    {a.out, a.width}});
+        with_piece(a.dtype, n, [&](auto t, auto n_c) {
+            const int64_t blocks = (p.slots + 7) / 8;
+            launch(k_from_groups_grad<decltype(t), decltype(n_c)::value>,
+                   (unsigned)std::min<int64_t>(blocks, (int64_t)sm_count(a.device) * 32),
+                   kMoveThreads, 0, 0, stream, p);
+        });
+        RUNE_LAUNCH_CHECK();
+    });
+}
+
+}  // extern "C"

@@ -40,6 +40,19 @@ struct Api {
     decltype(&rune_linear_backward) linear_bwd;
     decltype(&rune_linear_backward_workspace) linear_bwd_ws;
     decltype(&rune_pad_rows) pad_rows;
+    decltype(&rune_route) route;
+    decltype(&rune_route_backward) route_bwd;
+    decltype(&rune_row_groups) row_groups;
+    decltype(&rune_row_groups_workspace) row_groups_ws;
+    decltype(&rune_to_groups) to_groups;
+    decltype(&rune_from_groups) from_groups;
+    decltype(&rune_from_groups_backward) from_groups_bwd;
+    decltype(&rune_grouped_linear) grouped;
+    decltype(&rune_grouped_linear_workspace) grouped_ws;
+    decltype(&rune_grouped_linear_backward) grouped_bwd;
+    decltype(&rune_grouped_linear_backward_workspace) grouped_bwd_ws;
+    decltype(&rune_orthogonalize) orthogonalize;
+    decltype(&rune_orthogonalize_workspace) orthogonalize_ws;
     decltype(&rune_last_error) last_error;
 } api;
 PyObject* g_raise = nullptr;        // runtime.library.check's exceptions by status
@@ -113,8 +126,9 @@ void check_tensor(const Tensor& t, const char* name, ScalarType dtype, at::IntAr
     if (t.device() != x.device()) bad(name, " must be on ", x.device(), ", not ", t.device(), ".");
 }
 
-void check_cuda(const Tensor& x) {
-    if (!x.defined() || !x.is_cuda()) bad("x must be a CUDA tensor; there is no CPU path.");
+void check_cuda(const Tensor& x, const char* name = "x") {
+    if (!x.defined() || !x.is_cuda())
+        bad(name, " must be a CUDA tensor; there is no CPU path.");
 }
 
 // A tensor as rows of its last axis with unit column stride, copied only where no view has one.
@@ -426,6 +440,354 @@ Tensor layer(const Tensor& x, const Tensor& weight, Tensor bias, const Tensor& r
     return linear_call(x, weight, bias, residual, x_scale, w_scale, act, gated, out, false).y;
 }
 
+// ----------------------------------------------------------------------------- rows by group
+bool value_type(ScalarType t) {
+    return t == ScalarType::Float || t == ScalarType::Half || t == ScalarType::BFloat16;
+}
+
+struct RouteOut {
+    Tensor index, weights;
+};
+
+RouteOut route_call(const Tensor& logits, int64_t k) {
+    const Rows r(logits);
+    RouteOut o{empty_like_type(logits, {logits.size(0), k}, ScalarType::Int),
+               empty_like_type(logits, {logits.size(0), k}, ScalarType::Float)};
+    rune_route_args a{};
+    a.rows = logits.size(0), a.groups = logits.size(1), a.k = k;
+    a.logits_stride = r.ld;
+    a.device = logits.get_device(), a.dtype = code_of(logits.scalar_type());
+    a.logits = r.p();
+    a.index = (int32_t*)ptr(o.index), a.weights = (float*)ptr(o.weights);
+    check(api.route(&a, stream_of(logits)));
+    return o;
+}
+
+struct RouteFn : torch::autograd::Function<RouteFn> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& logits, int64_t k) {
+        const RouteOut o = route_call(logits, k);
+        ctx->save_for_backward({o.index, o.weights});
+        ctx->mark_non_differentiable({o.index});
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["groups"] = logits.size(1);
+        ctx->saved_data["type"] = (int64_t)logits.scalar_type();
+        return {o.index, o.weights};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        return in_backward([&] { return gradients(ctx, grads); });
+    }
+    static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
+        first_order_only(grads);
+        if (!grads[1].defined()) return {Tensor(), Tensor()};
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &index = saved[0], &weights = saved[1], dw = grads[1].contiguous();
+        const auto type = (ScalarType)ctx->saved_data["type"].toInt();
+        rune_route_args a{};
+        a.rows = index.size(0), a.k = index.size(1);
+        a.groups = ctx->saved_data["groups"].toInt();
+        a.device = index.get_device(), a.dtype = code_of(type);
+        const Tensor dlogits = empty_like_type(index, {a.rows, a.groups}, type);
+        a.index = (int32_t*)ptr(index), a.weights = (float*)ptr(weights);
+        a.dweights = (const float*)ptr(dw), a.dlogits = ptr(dlogits);
+        check(api.route_bwd(&a, stream_of(index)));
+        return {dlogits, Tensor()};
+    }
+};
+
+RouteOut route(const Tensor& logits, int64_t k) {
+    no_transforms({&logits});
+    check_cuda(logits, "logits");
+    if (!value_type(logits.scalar_type()))
+        bad("logits must be float32, float16 or bfloat16, not ", name_of(logits.scalar_type()),
+            ".");
+    if (logits.dim() != 2 || logits.size(1) == 0)
+        bad("logits needs two axes, rows and groups, and the last one cannot be empty.");
+    if (k < 1 || k > 32 || k > logits.size(1))
+        bad("k must be 1 to 32 and no more than the ", logits.size(1), " groups, not ", k, ".");
+    if (at::GradMode::is_enabled() && logits.requires_grad()) {
+        const variable_list got = RouteFn::apply(logits, k);
+        return {got[0], got[1]};
+    }
+    return route_call(logits, k);
+}
+
+struct Groups {
+    Tensor offsets, order, place;
+    int64_t rows() const { return place.size(0); }
+    int64_t k() const { return place.dim() == 2 ? place.size(1) : 1; }
+};
+
+Groups row_groups(const Tensor& index_, int64_t groups) {
+    no_transforms({&index_});
+    check_cuda(index_, "index");
+    const ScalarType t = index_.scalar_type();
+    if (t != ScalarType::Int && t != ScalarType::Long)
+        bad("index must be int32 or int64, not ", name_of(t), ".");
+    if (index_.dim() < 1 || index_.dim() > 2 || (index_.dim() == 2 && index_.size(1) == 0))
+        bad("index must have shape [rows] or [rows, choices].");
+    if (groups < 1 || groups > 1024) bad("groups must be 1 to 1024, not ", groups, ".");
+    const Tensor index = index_.contiguous();
+    Groups o{empty_like_type(index, {groups + 1}, ScalarType::Int),
+             empty_like_type(index, {index.numel()}, ScalarType::Int),
+             empty_like_type(index, index.sizes(), ScalarType::Int)};
+    rune_row_groups_args a{};
+    a.rows = o.rows(), a.groups = groups, a.k = o.k();
+    a.device = index.get_device();
+    a.index_bytes = t == ScalarType::Long ? 8 : 4;
+    a.index = ptr(index);
+    a.offsets = (int32_t*)ptr(o.offsets), a.order = (int32_t*)ptr(o.order);
+    a.place = (int32_t*)ptr(o.place);
+    const Tensor ws = scratch(api.row_groups_ws, a, index);
+    check(api.row_groups(&a, stream_of(index)));
+    return o;
+}
+
+void check_groups(Groups& g, const Tensor& x) {
+    for (const Tensor* t : {&g.offsets, &g.order, &g.place})
+        if (!t->defined() || t->scalar_type() != ScalarType::Int || t->device() != x.device())
+            bad("groups must be the int32 tensors of row_groups, on ", x.device(), ".");
+    if (g.offsets.dim() != 1 || g.offsets.size(0) < 2 || g.place.dim() < 1 || g.place.dim() > 2 ||
+        (g.place.dim() == 2 && g.place.size(1) == 0) || g.order.dim() != 1 ||
+        g.order.numel() != g.place.numel())
+        bad("groups must be a result of row_groups: offsets [groups + 1], order [slots], place "
+            "[rows] or [rows, choices].");
+    g.offsets = g.offsets.contiguous(), g.order = g.order.contiguous();
+    g.place = g.place.contiguous();
+}
+
+rune_group_move_args move_args(const Rows& in, const Groups& g, const Tensor& out) {
+    rune_group_move_args a{};
+    a.rows = g.rows(), a.k = g.k(), a.width = in.t.size(-1);
+    a.in_stride = in.ld;
+    a.device = in.t.get_device(), a.dtype = code_of(in.t.scalar_type());
+    a.in = in.p(), a.out = ptr(out);
+    a.order = (const int32_t*)ptr(g.order), a.place = (const int32_t*)ptr(g.place);
+    return a;
+}
+
+Tensor to_groups_call(const Tensor& x, const Groups& g) {
+    const Rows r(x);
+    Tensor out = empty_like_type(x, {g.order.numel(), x.size(1)}, x.scalar_type());
+    const rune_group_move_args a = move_args(r, g, out);
+    check(api.to_groups(&a, stream_of(x)));
+    return out;
+}
+
+Tensor from_groups_call(const Tensor& y, const Groups& g, const Tensor& weights) {
+    const Rows r(y);
+    Tensor out = empty_like_type(y, {g.rows(), y.size(1)}, y.scalar_type());
+    rune_group_move_args a = move_args(r, g, out);
+    a.weights = (const float*)ptr(weights);
+    check(api.from_groups(&a, stream_of(y)));
+    return out;
+}
+
+struct ToGroupsFn : torch::autograd::Function<ToGroupsFn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& offsets,
+                          const Tensor& order, const Tensor& place) {
+        ctx->save_for_backward({offsets, order, place});
+        return to_groups_call(x, {offsets, order, place});
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        return in_backward([&] { return gradients(ctx, grads); });
+    }
+    static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
+        first_order_only(grads);
+        const auto saved = ctx->get_saved_variables();
+        return {from_groups_call(grads[0], {saved[0], saved[1], saved[2]}, Tensor()), Tensor(),
+                Tensor(), Tensor()};
+    }
+};
+
+struct FromGroupsFn : torch::autograd::Function<FromGroupsFn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& y, const Tensor& offsets,
+                          const Tensor& order, const Tensor& place,
+                          const std::optional<Tensor>& weights_) {
+        const Tensor weights = weights_.value_or(Tensor());
+        // y goes into the weights' gradient alone
+        ctx->save_for_backward({wants_grad(weights) ? y : Tensor(), offsets, order, place, weights});
+        return from_groups_call(y, {offsets, order, place}, weights);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        return in_backward([&] { return gradients(ctx, grads); });
+    }
+    static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
+        first_order_only(grads);
+        const auto saved = ctx->get_saved_variables();
+        const Groups g{saved[1], saved[2], saved[3]};
+        const Tensor &y = saved[0], &weights = saved[4], &dout = grads[0];
+        const bool need_y = ctx->needs_input_grad(0);
+        if (!weights.defined())
+            return {need_y ? to_groups_call(dout, g) : Tensor(), Tensor(), Tensor(), Tensor(),
+                    Tensor()};
+        const Rows r(dout), ry(y);
+        Tensor dy, dw;
+        if (need_y) dy = empty_like_type(dout, {g.order.numel(), dout.size(1)}, dout.scalar_type());
+        if (y.defined()) dw = empty_like_type(weights, weights.sizes(), weights.scalar_type());
+        rune_group_move_args a = move_args(r, g, dy);
+        a.y = ry.p(), a.y_stride = ry.ld;
+        a.weights = (const float*)ptr(weights), a.dweights = (float*)ptr(dw);
+        if (need_y || dw.defined()) check(api.from_groups_bwd(&a, stream_of(dout)));
+        return {dy, Tensor(), Tensor(), Tensor(), dw};
+    }
+};
+
+void check_rows(const Tensor& x, const char* name) {
+    check_cuda(x, name);
+    if (!value_type(x.scalar_type()))
+        bad(name, " must be float32, float16 or bfloat16, not ", name_of(x.scalar_type()), ".");
+    if (x.dim() != 2 || x.size(1) == 0)
+        bad(name, " needs two axes, rows and columns, and the last one cannot be empty.");
+}
+
+Tensor to_groups(const Tensor& x, Groups g) {
+    no_transforms({&x});
+    check_rows(x, "x");
+    check_groups(g, x);
+    if (x.size(0) != g.rows()) bad("x has ", x.size(0), " rows, the groups ", g.rows(), ".");
+    if (at::GradMode::is_enabled() && x.requires_grad())
+        return ToGroupsFn::apply(x, g.offsets, g.order, g.place);
+    return to_groups_call(x, g);
+}
+
+Tensor from_groups(const Tensor& y, Groups g, Tensor weights) {
+    no_transforms({&y, &weights});
+    check_rows(y, "y");
+    check_groups(g, y);
+    if (y.size(0) != g.order.numel())
+        bad("y has ", y.size(0), " rows, the groups ", g.order.numel(), " slots.");
+    if (weights.defined()) {
+        check_tensor(weights, "weights", ScalarType::Float, g.place.sizes(), y);
+        weights = weights.contiguous();
+    }
+    if (at::GradMode::is_enabled() && (y.requires_grad() || wants_grad(weights)))
+        return FromGroupsFn::apply(y, g.offsets, g.order, g.place, given(weights));
+    return from_groups_call(y, g, weights);
+}
+
+// weight: the groups' matrices one below the other
+Tensor grouped_call(const Tensor& x, const Tensor& weight, const Tensor& bias,
+                    const Tensor& offsets, int64_t act, bool gated) {
+    const Rows rx(x), rw(weight);
+    rune_grouped_linear_args a{};
+    a.rows = x.size(0), a.inputs = x.size(1), a.groups = offsets.size(0) - 1;
+    a.outputs = weight.size(0) / a.groups / (gated ? 2 : 1);
+    a.x_stride = rx.ld, a.weight_stride = rw.ld;
+    a.device = x.get_device(), a.dtype = code_of(x.scalar_type());
+    a.activation = (int32_t)act, a.gated = gated;
+    Tensor y = empty_like_type(x, {a.rows, a.outputs}, x.scalar_type());
+    a.x = rx.p(), a.weight = rw.p(), a.bias = ptr(bias);
+    a.offsets = (const int32_t*)ptr(offsets), a.y = ptr(y);
+    int status = api.grouped(&a, stream_of(x));
+    if (status == RUNE_ERR_RETRY) {  // this call needs scratch
+        const Tensor ws = scratch(api.grouped_ws, a, x);
+        status = api.grouped(&a, stream_of(x));
+    }
+    check(status);
+    return y;
+}
+
+struct GroupedFn : torch::autograd::Function<GroupedFn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& weight_,
+                          const std::optional<Tensor>& bias_, const Tensor& offsets, int64_t act,
+                          bool gated) {
+        const Tensor bias = bias_.value_or(Tensor());
+        const Tensor x = in_place(x_);
+        const Tensor weight = in_place(weight_.reshape({-1, weight_.size(2)}));
+        ctx->save_for_backward({x, weight, bias, offsets});
+        ctx->saved_data["act"] = act;
+        ctx->saved_data["gated"] = gated;
+        return grouped_call(x, weight, bias, offsets, act, gated);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        return in_backward([&] { return gradients(ctx, grads); });
+    }
+    static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
+        first_order_only(grads);
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &offsets = saved[3];
+        const Rows rx(x), rw(weight), dy(grads[0]);
+        rune_grouped_linear_grad_args a{};
+        a.rows = x.size(0), a.inputs = x.size(1), a.groups = offsets.size(0) - 1;
+        a.outputs = grads[0].size(1);
+        a.x_stride = rx.ld, a.weight_stride = rw.ld, a.dy_stride = dy.ld;
+        a.device = x.get_device(), a.dtype = code_of(x.scalar_type());
+        a.activation = (int32_t)ctx->saved_data["act"].toInt();
+        a.gated = ctx->saved_data["gated"].toBool();
+        Tensor dx, dw, db;
+        if (ctx->needs_input_grad(0)) dx = empty_like_type(x, x.sizes(), x.scalar_type());
+        if (ctx->needs_input_grad(1))
+            dw = empty_like_type(weight, {a.groups, weight.size(0) / a.groups, a.inputs},
+                                 weight.scalar_type());
+        if (bias.defined() && ctx->needs_input_grad(2))
+            db = empty_like_type(bias, bias.sizes(), bias.scalar_type());
+        a.x = rx.p(), a.weight = rw.p(), a.bias = ptr(bias);
+        a.offsets = (const int32_t*)ptr(offsets), a.dy = dy.p();
+        a.dx = ptr(dx), a.dweight = ptr(dw), a.dbias = ptr(db);
+        if (dx.defined() || dw.defined() || db.defined()) {
+            const Tensor ws = scratch(api.grouped_bwd_ws, a, x);
+            check(api.grouped_bwd(&a, stream_of(x)));
+        }
+        return {dx, dw, db, Tensor(), Tensor(), Tensor()};
+    }
+};
+
+Tensor grouped(const Tensor& x, const Tensor& weight, Tensor bias, Groups g, int64_t act,
+               bool gated) {
+    no_transforms({&x, &weight, &bias});
+    check_cuda(x);
+    const ScalarType t = x.scalar_type();
+    if (t != ScalarType::Half && t != ScalarType::BFloat16)
+        bad("x must be float16 or bfloat16, not ", name_of(t), ".");
+    if (!weight.defined() || x.dim() != 2 || x.size(1) == 0 || weight.dim() != 3 ||
+        weight.size(0) == 0 || weight.size(1) == 0)
+        bad("x needs two axes and weight three, groups, outputs and inputs, none of them empty "
+            "but the rows.");
+    check_groups(g, x);
+    const int64_t groups = g.offsets.size(0) - 1, n_all = weight.size(1);
+    if (gated && n_all % 2)
+        bad("weight of a gated layer has the gate's rows, then as many for the other factor; ",
+            n_all, " rows are odd.");
+    check_tensor(weight, "weight", t, {groups, n_all, x.size(1)}, x);
+    if (x.size(0) != g.order.numel())
+        bad("x has ", x.size(0), " rows, the groups ", g.order.numel(), " slots.");
+    if (bias.defined()) {
+        check_tensor(bias, "bias", t, {groups, n_all}, x);
+        bias = bias.contiguous();
+    }
+    if (at::GradMode::is_enabled() &&
+        (x.requires_grad() || weight.requires_grad() || wants_grad(bias)))
+        return GroupedFn::apply(x, weight, given(bias), g.offsets, act, gated);
+    return grouped_call(x, weight.reshape({-1, x.size(1)}), bias, g.offsets, act, gated);
+}
+
+// -------------------------------------------------------------------------------- updates
+Tensor orthogonalize(const Tensor& x, int64_t steps, const double (&c)[3], double eps) {
+    no_transforms({&x});
+    check_cuda(x);
+    if (!value_type(x.scalar_type()))
+        bad("x must be float32, float16 or bfloat16, not ", name_of(x.scalar_type()), ".");
+    if (x.dim() < 2) bad("x needs two axes at least, rows and columns.");
+    if (steps < 0 || steps > 64) bad("steps must be 0 to 64, not ", steps, ".");
+    if (!(eps >= 0.0)) bad("eps cannot be negative.");
+    if (at::GradMode::is_enabled() && x.requires_grad())
+        bad("an orthogonalised update has no gradient; call under torch.no_grad().");
+    Tensor y = empty_like_type(x, x.sizes(), ScalarType::BFloat16);
+    if (x.numel() == 0) return y;
+    // as [count, rows, columns], by a copy where no view has one stride for all matrices
+    const Tensor stack = x.dim() == 3 ? x : x.reshape({-1, x.size(-2), x.size(-1)});
+    rune_orthogonalize_args a{};
+    a.count = stack.size(0), a.rows = stack.size(1), a.cols = stack.size(2);
+    a.x_step = stack.stride(0), a.x_row = stack.stride(1), a.x_col = stack.stride(2);
+    a.device = x.get_device(), a.dtype = code_of(x.scalar_type());
+    a.steps = (int32_t)steps;
+    a.a = (float)c[0], a.b = (float)c[1], a.c = (float)c[2], a.eps = (float)eps;
+    a.x = ptr(stack), a.y = ptr(y);
+    const Tensor ws = scratch(api.orthogonalize_ws, a, x);
+    check(api.orthogonalize(&a, stream_of(x)));
+    return y;
+}
+
 // ---------------------------------------------------------------------------------- Python
 Tensor tensor_arg(PyObject* o, const char* name) {
     if (o == Py_None) return Tensor();
@@ -545,6 +907,75 @@ PyObject* py_layer(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
+// route(logits, k): (index, weights)
+PyObject* py_route(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (!count_is(n, 2)) return nullptr;
+    return guarded([&] {
+        const int64_t k = PyLong_AsLongLong(args[1]);
+        if (PyErr_Occurred()) throw 0;
+        const RouteOut o = route(tensor_arg(args[0], "logits"), k);
+        return pack(o.index, o.weights, Tensor());
+    });
+}
+
+// row_groups(index, groups): (offsets, order, place)
+PyObject* py_row_groups(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (!count_is(n, 2)) return nullptr;
+    return guarded([&] {
+        const int64_t groups = PyLong_AsLongLong(args[1]);
+        if (PyErr_Occurred()) throw 0;
+        const Groups g = row_groups(tensor_arg(args[0], "index"), groups);
+        return pack(g.offsets, g.order, g.place);
+    });
+}
+
+Groups groups_arg(PyObject* const* args) {
+    return {tensor_arg(args[0], "offsets"), tensor_arg(args[1], "order"),
+            tensor_arg(args[2], "place")};
+}
+
+// to_groups(x, offsets, order, place): xs
+PyObject* py_to_groups(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (!count_is(n, 4)) return nullptr;
+    return guarded([&] {
+        return THPVariable_Wrap(to_groups(tensor_arg(args[0], "x"), groups_arg(args + 1)));
+    });
+}
+
+// from_groups(y, offsets, order, place, weights or None): rows
+PyObject* py_from_groups(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (!count_is(n, 5)) return nullptr;
+    return guarded([&] {
+        return THPVariable_Wrap(from_groups(tensor_arg(args[0], "y"), groups_arg(args + 1),
+                                            tensor_arg(args[4], "weights")));
+    });
+}
+
+// grouped(x, weight, bias, offsets, order, place, activation, gated): y
+PyObject* py_grouped(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (!count_is(n, 8)) return nullptr;
+    return guarded([&] {
+        const long act = PyLong_AsLong(args[6]), gated = PyLong_AsLong(args[7]);
+        if (PyErr_Occurred()) throw 0;
+        return THPVariable_Wrap(grouped(tensor_arg(args[0], "x"), tensor_arg(args[1], "weight"),
+                                        tensor_arg(args[2], "bias"), groups_arg(args + 3), act,
+                                        gated != 0));
+    });
+}
+
+// orthogonalize(x, steps, a, b, c, eps): y
+PyObject* py_orthogonalize(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (!count_is(n, 6)) return nullptr;
+    return guarded([&] {
+        const int64_t steps = PyLong_AsLongLong(args[1]);
+        const double c[3] = {PyFloat_AsDouble(args[2]), PyFloat_AsDouble(args[3]),
+                             PyFloat_AsDouble(args[4])};
+        const double eps = PyFloat_AsDouble(args[5]);
+        if (PyErr_Occurred()) throw 0;
+        return THPVariable_Wrap(orthogonalize(tensor_arg(args[0], "x"), steps, c, eps));
+    });
+}
+
 // bind(addresses of the entry points in Api's order, raise(status, message), recompute inputs)
 PyObject* py_bind(PyObject*, PyObject* args) {
     PyObject *list, *raise;
@@ -577,6 +1008,12 @@ PyMethodDef methods[] = {
     {"to_fp8", reinterpret_cast<PyCFunction>(py_to_fp8), METH_FASTCALL, nullptr},
     {"padded", reinterpret_cast<PyCFunction>(py_padded), METH_FASTCALL, nullptr},
     {"layer", reinterpret_cast<PyCFunction>(py_layer), METH_FASTCALL, nullptr},
+    {"route", reinterpret_cast<PyCFunction>(py_route), METH_FASTCALL, nullptr},
+    {"row_groups", reinterpret_cast<PyCFunction>(py_row_groups), METH_FASTCALL, nullptr},
+    {"to_groups", reinterpret_cast<PyCFunction>(py_to_groups), METH_FASTCALL, nullptr},
+    {"from_groups", reinterpret_cast<PyCFunction>(py_from_groups), METH_FASTCALL, nullptr},
+    {"grouped", reinterpret_cast<PyCFunction>(py_grouped), METH_FASTCALL, nullptr},
+    {"orthogonalize", reinterpret_cast<PyCFunction>(py_orthogonalize), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ops", nullptr, -1, methods};
 

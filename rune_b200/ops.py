@@ -1,4 +1,5 @@
-"""Network operators in mixed precision, with gradients: normalisation, linear and gated layers.
+"""Network operators in mixed precision, with gradients: normalisation, linear and gated layers,
+the same by group of rows, and the orthogonalised update of an optimiser.
 
 The layers of the Möbius networks (rune/mobius/layers.py:26-67) as differentiable operators on
 CUDA tensors, for training, distilling or serving networks beside the engine's float32 inference:
@@ -9,6 +10,10 @@ CUDA tensors, for training, distilling or serving networks beside the engine's f
 * ``gated_linear``: ``act(x Wg^T + bg) * (x Wu^T + bu)`` in one kernel.
 * ``padded``: a copy of a matrix whose rows start on 16 bytes each, for weights of odd widths.
 * ``quantize_fp8``: rows to e4m3 with a scale per row (weights once, activations per call).
+* ``route``, ``row_groups``, ``to_groups``, ``from_groups``: rows to the groups (experts, elements)
+  whose weights they take, sorted by group, and back.
+* ``grouped_linear``, ``grouped_gated_linear``: the layers with each group's own weights.
+* ``orthogonalize``: a stack of updates, orthogonalised by Newton-Schulz products.
 * ``check_waits``: whether a kernel of these gave up waiting, where no operator call follows.
 
 Every function works on the last axis of its input, takes row-strided views, runs on the current
@@ -22,6 +27,7 @@ the layers are products of a dz that is rounded to 16 bits first. Equal inputs g
 from __future__ import annotations
 
 import ctypes
+from collections import namedtuple
 from importlib.machinery import ExtensionFileLoader
 from importlib.util import module_from_spec, spec_from_loader
 
@@ -30,7 +36,9 @@ import torch
 from .runtime import library as L
 from .runtime.build import BINDING
 
-__all__ = ["check_waits", "gated_linear", "linear", "padded", "quantize_fp8", "rms_norm", "rms_norm_fp8"]
+__all__ = ["RowGroups", "check_waits", "from_groups", "gated_linear", "grouped_gated_linear",
+           "grouped_linear", "linear", "orthogonalize", "padded", "quantize_fp8", "rms_norm",
+           "rms_norm_fp8", "route", "row_groups", "to_groups"]
 
 _ACTS = {None: L.RUNE_ACT_NONE, **L.RUNE_ACT}
 _OUT = {None: -1, torch.float16: L.RUNE_F16, torch.bfloat16: L.RUNE_BF16}
@@ -41,6 +49,10 @@ _OUT = {None: -1, torch.float16: L.RUNE_F16, torch.bfloat16: L.RUNE_BF16}
 # and 1024 outputs, recomputed / saved: 512 inputs 177 / 191 us (gated 257 / 323), 1024 inputs
 # 248 / 243 (424 / 432), 2048 inputs 428 / 379 (770 / 682).
 RECOMPUTE_INPUTS = 1024
+
+# Coefficients a, b, c of the quintic a x + b x^3 + c x^5 that ``orthogonalize`` iterates: steep at
+# zero, so that five steps bring singular values from 0.01 and up to between 0.7 and 1.2.
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
 
 _BINDING = None
 
@@ -60,7 +72,13 @@ def _native():
         entries = (lib.rune_rms_norm, lib.rune_rms_norm_backward,
                    lib.rune_rms_norm_backward_workspace, lib.rune_linear,
                    lib.rune_linear_workspace, lib.rune_linear_backward,
-                   lib.rune_linear_backward_workspace, lib.rune_pad_rows, lib.rune_last_error)
+                   lib.rune_linear_backward_workspace, lib.rune_pad_rows, lib.rune_route,
+                   lib.rune_route_backward, lib.rune_row_groups, lib.rune_row_groups_workspace,
+                   lib.rune_to_groups, lib.rune_from_groups, lib.rune_from_groups_backward,
+                   lib.rune_grouped_linear, lib.rune_grouped_linear_workspace,
+                   lib.rune_grouped_linear_backward, lib.rune_grouped_linear_backward_workspace,
+                   lib.rune_orthogonalize, lib.rune_orthogonalize_workspace,
+                   lib.rune_last_error)
         module.bind(tuple(ctypes.cast(f, ctypes.c_void_p).value for f in entries), L.fail,
                     RECOMPUTE_INPUTS)
         _BINDING = module
@@ -163,3 +181,81 @@ def gated_linear(x, weight, bias=None, activation="silu", *, x_scale=None, weigh
         raise ValueError("gated_linear needs an activation.")
     return (_BINDING or _native()).layer(x, weight, bias, None, x_scale, weight_scale, act, 1,
                                          _out_code(out_dtype))
+
+
+RowGroups = namedtuple("RowGroups", ["offsets", "order", "place"])
+RowGroups.__doc__ = """Rows sorted by group, as int32 tensors on the GPU; a slot is a row's choice.
+
+offsets [groups + 1]: the groups' first places, and the end of the last. order [slots]: the slot
+of each place, -1 behind the last group. place: the place of each slot, of the index's shape, -1
+for slots in no group."""
+
+
+def route(logits, k):
+    """The k groups of each row with the largest logits, and the softmax over them:
+    ``(index, weights)``, int32 and float32 [rows, k], largest first, ties to the lowest index.
+
+    logits [rows, groups] (at most 1024 groups, k at most 32): float32, float16 or bfloat16. A logit
+    of -inf is never chosen: index -1 and weight 0 in its place. NaN counts as the largest, and the
+    row's weights are NaN. weights is differentiable in logits.
+    """
+    return (_BINDING or _native()).route(logits, k)
+
+
+def row_groups(index, groups):
+    """Sorts rows by group: ``RowGroups`` for ``to_groups``, ``grouped_linear`` and ``from_groups``.
+
+    index [rows] or [rows, choices] (int32 or int64): the group of each slot; an index outside
+    0 .. groups - 1 puts the slot in no group. Slots of a group keep their order. groups: at most
+    1024.
+    """
+    return RowGroups(*(_BINDING or _native()).row_groups(index, groups))
+
+
+def to_groups(x, groups):
+    """The rows of x in the order of their groups: ``[slots, width]``, a row once for each of its
+    choices, zeros behind the last group. x [rows, width]: float32, float16 or bfloat16,
+    differentiable."""
+    return (_BINDING or _native()).to_groups(x, *groups)
+
+
+def from_groups(y, groups, weights=None):
+    """Rows sorted by group back in their places: row r is ``sum_j weights[r, j] * y[place[r, j]]``.
+
+    y [slots, width] (float32, float16 or bfloat16) and weights (float32, of the index's shape;
+    None: all 1) are differentiable. Slots in no group add nothing, whatever their weight is.
+    """
+    return (_BINDING or _native()).from_groups(y, *groups, weights)
+
+
+def grouped_linear(x, weight, groups, bias=None, activation=None):
+    """``act(x weight[g]^T + bias[g])`` for the rows of each group g, as ``to_groups`` sorted them.
+
+    x [slots, inputs], weight [groups, outputs, inputs] and bias [groups, outputs]: float16 or
+    bfloat16, one type, differentiable. Rows behind the last group are zeros, and have no gradient.
+    """
+    return (_BINDING or _native()).grouped(x, weight, bias, *groups, _activation(activation), 0)
+
+
+def grouped_gated_linear(x, weight, groups, bias=None, activation="silu"):
+    """``act(x Wg[g]^T + bg[g]) * (x Wu[g]^T + bu[g])`` for the rows of each group g.
+
+    weight [groups, 2 * outputs, inputs] and bias [groups, 2 * outputs] hold the gate's rows first.
+    Types, order and gradients as in ``grouped_linear``.
+    """
+    act = _activation(activation)
+    if act == L.RUNE_ACT_NONE:
+        raise ValueError("grouped_gated_linear needs an activation.")
+    return (_BINDING or _native()).grouped(x, weight, bias, *groups, act, 1)
+
+
+def orthogonalize(x, steps=5, coefficients=NEWTON_SCHULZ, eps=1.0e-7):
+    """x [..., rows, columns] with its singular values brought near 1, in bfloat16: ``steps`` times
+    ``X <- a X + (b A + c A A) X`` with ``A = X X^T``, from ``x / (norm(x) + eps)``.
+
+    For the update of a weight matrix, or of a stack of them. x: float32, float16 or bfloat16. The
+    products take float16 operands and add in float32: a step rounds X, A and b A + c A A to 11
+    bits. Not differentiable.
+    """
+    a, b, c = coefficients
+    return (_BINDING or _native()).orthogonalize(x, steps, a, b, c, eps)

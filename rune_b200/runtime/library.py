@@ -49,6 +49,11 @@ EXPORTED = [
     "rune_linear", "rune_linear_workspace", "rune_linear_backward",
     "rune_linear_backward_workspace", "rune_pad_rows", "rune_linear_set_wait_polls",
     "rune_linear_check_waits",
+    "rune_route", "rune_route_backward", "rune_row_groups", "rune_row_groups_workspace",
+    "rune_to_groups", "rune_from_groups", "rune_from_groups_backward",
+    "rune_grouped_linear", "rune_grouped_linear_workspace", "rune_grouped_linear_backward",
+    "rune_grouped_linear_backward_workspace",
+    "rune_orthogonalize", "rune_orthogonalize_workspace",
 ]
 
 
@@ -136,6 +141,63 @@ class LinearGradArgs(ctypes.Structure):
     ]
 
 
+class RouteArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_int64), ("groups", c_int64), ("k", c_int64), ("logits_stride", c_int64),
+        ("device", c_int32), ("dtype", c_int32), ("logits", c_void_p), ("index", c_void_p),
+        ("weights", c_void_p), ("dweights", c_void_p), ("dlogits", c_void_p),
+    ]
+
+
+class RowGroupsArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_int64), ("groups", c_int64), ("k", c_int64), ("device", c_int32),
+        ("index_bytes", c_int32), ("index", c_void_p), ("offsets", c_void_p),
+        ("order", c_void_p), ("place", c_void_p), ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+    ]
+
+
+class GroupMoveArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_int64), ("k", c_int64), ("width", c_int64), ("in_stride", c_int64),
+        ("y_stride", c_int64), ("device", c_int32), ("dtype", c_int32), ("input", c_void_p),
+        ("y", c_void_p), ("order", c_void_p), ("place", c_void_p), ("weights", c_void_p),
+        ("out", c_void_p), ("dweights", c_void_p),
+    ]
+
+
+class GroupedLinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_int64), ("inputs", c_int64), ("outputs", c_int64), ("groups", c_int64),
+        ("x_stride", c_int64), ("weight_stride", c_int64), ("device", c_int32),
+        ("dtype", c_int32), ("activation", c_int32), ("gated", c_int32), ("x", c_void_p),
+        ("weight", c_void_p), ("bias", c_void_p), ("offsets", c_void_p), ("y", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_int64),
+    ]
+
+
+class GroupedLinearGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_int64), ("inputs", c_int64), ("outputs", c_int64), ("groups", c_int64),
+        ("x_stride", c_int64), ("weight_stride", c_int64), ("dy_stride", c_int64),
+        ("device", c_int32), ("dtype", c_int32), ("activation", c_int32), ("gated", c_int32),
+        ("x", c_void_p), ("weight", c_void_p), ("bias", c_void_p), ("offsets", c_void_p),
+        ("dy", c_void_p), ("dx", c_void_p), ("dweight", c_void_p), ("dbias", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_int64),
+    ]
+
+
+class OrthogonalizeArgs(ctypes.Structure):
+    _fields_ = [
+        ("count", c_int64), ("rows", c_int64), ("cols", c_int64), ("x_step", c_int64),
+        ("x_row", c_int64), ("x_col", c_int64), ("device", c_int32), ("dtype", c_int32),
+        ("steps", c_int32), ("a", c_float), ("b", c_float), ("c", c_float), ("eps", c_float),
+        ("reserved", c_int32), ("x", c_void_p), ("y", c_void_p), ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+    ]
+
+
 _LIB = None
 
 
@@ -197,6 +259,16 @@ def load_library(path: Path | None = None):
                        ("rune_linear", LinearArgs), ("rune_linear_backward", LinearGradArgs)):
         getattr(lib, name).argtypes = [POINTER(args), c_void_p]
         if name != "rune_rms_norm":
+            getattr(lib, name + "_workspace").argtypes = [POINTER(args), POINTER(c_int64)]
+    for name, args in (("rune_route", RouteArgs), ("rune_route_backward", RouteArgs),
+                       ("rune_row_groups", RowGroupsArgs), ("rune_to_groups", GroupMoveArgs),
+                       ("rune_from_groups", GroupMoveArgs),
+                       ("rune_from_groups_backward", GroupMoveArgs),
+                       ("rune_grouped_linear", GroupedLinearArgs),
+                       ("rune_grouped_linear_backward", GroupedLinearGradArgs),
+                       ("rune_orthogonalize", OrthogonalizeArgs)):
+        getattr(lib, name).argtypes = [POINTER(args), c_void_p]
+        if name + "_workspace" in EXPORTED:
             getattr(lib, name + "_workspace").argtypes = [POINTER(args), POINTER(c_int64)]
     for name in EXPORTED:
         if name not in ("rune_engine_destroy", "rune_last_error"):
