@@ -15,6 +15,8 @@
 // z of an activated layer is computed again in the backward pass: a copy in float32 would cost 8
 // bytes of traffic and 4 of memory a value, for all slots of every layer.
 
+#include <cmath>
+
 #include "tile.cuh"
 
 namespace rune {
@@ -68,125 +70,166 @@ k_group_maps(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
         : "memory");
 }
 
-// Lines of `high` rows that the groups before g fill: lines[g], for all groups and the end.
-__device__ __forceinline__ void count_lines(const int32_t* offsets, int64_t rows, int groups,
-                                            int high, int32_t* first_row, int32_t* lines) {
-    for (int g = threadIdx.x; g <= groups; g += blockDim.x)
-        first_row[g] = (int)min((int64_t)max(offsets[g], 0), rows);
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        int before = 0;
-        for (int g0 = 0; g0 < groups; g0 += 32) {
-            const int g = g0 + threadIdx.x;
-            const int n = g < groups
-                              ? (max(0, first_row[g + 1] - first_row[g]) + high - 1) / high : 0;
-            int sum = n;
-#pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-                const int other = __shfl_up_sync(0xffffffffu, sum, o);
-                sum += (int)threadIdx.x >= o ? other : 0;
-            }
-            if (g < groups) lines[g] = before + sum - n;
-            before += __shfl_sync(0xffffffffu, sum, 31);
-        }
-        if (threadIdx.x == 0) lines[groups] = before;
+// Number of lines of `high` rows that the groups before g fill (0), and up to g (1) or all (2).
+struct LineCount {
+    int before, with, all;
+};
+__device__ __forceinline__ int group_lines(const int32_t* offsets, int64_t rows, int g, int high) {
+    const int64_t a = min((int64_t)max(offsets[g], 0), rows);
+    const int64_t b = min((int64_t)max(offsets[g + 1], 0), rows);
+    return (int)((max((int64_t)0, b - a) + high - 1) / high);
+}
+__device__ __forceinline__ LineCount count_lines(const int32_t* offsets, int64_t rows, int groups,
+                                                 int g, int high) {
+    __shared__ int sums[2][32];
+    int before = 0, all = 0;
+    for (int i = threadIdx.x; i < groups; i += blockDim.x) {
+        const int n = group_lines(offsets, rows, i, high);
+        all += n;
+        before += i < g ? n : 0;
     }
+    all = (int)__reduce_add_sync(0xffffffffu, (unsigned)all);
+    before = (int)__reduce_add_sync(0xffffffffu, (unsigned)before);
+    if ((threadIdx.x & 31) == 0) sums[0][threadIdx.x >> 5] = before, sums[1][threadIdx.x >> 5] = all;
     __syncthreads();
+    before = all = 0;
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) before += sums[0][w], all += sums[1][w];
+    return {before, before + group_lines(offsets, rows, g, high), all};
 }
 
 struct SumParams {
     const int32_t* offsets;
     int64_t rows, n;
-    int groups, high, each;  // rows of a line, parts that each line left
+    int groups, high, each;  // rows of a line of tiles, parts that each line left
     int64_t ld;              // k_group_columns: of x
     const void* x;
     float* parts;            // [lines * each][n]
     void* out;               // [groups][n]
+    int ranges;              // of a group's rows or parts, summed apart
+    int64_t line;
+    float* sums;             // [ranges][groups][line]
 };
 
-// sums of the columns of each line of rows, which no line of another group's shares: 64 columns a
-// block, four rows at a time
+// sums of the columns of a range of a group's rows: 64 columns a block, four rows at a time
 template <typename T>
 __global__ void __launch_bounds__(256) k_group_columns(const SumParams p) {
     follow_on();
-    extern __shared__ int32_t table[];
-    int32_t *first = table, *lines = table + p.groups + 1;
     __shared__ float joined[4][64];
-    count_lines(p.offsets, p.rows, p.groups, p.high, first, lines);
-    const int c = threadIdx.x & 63, part = threadIdx.x >> 6;
+    const int c = threadIdx.x & 63, turn = threadIdx.x >> 6;
     const int64_t col = (int64_t)blockIdx.x * 64 + c;
-    for (int line = blockIdx.y; line < lines[p.groups]; line += gridDim.y) {
-        int g = 0, above = p.groups;
-        while (above - g > 1) {
-            const int mid = (g + above) >> 1;
-            if (lines[mid] <= line) g = mid;
-            else above = mid;
-        }
-        const int r0 = first[g] + (line - lines[g]) * p.high, r1 = min(r0 + p.high, first[g + 1]);
-        float s = 0.0f;
-        if (col < p.n) {
-            const T* x = static_cast<const T*>(p.x) + col;
+    const int g = blockIdx.y, range = blockIdx.z;
+    const int64_t a = min((int64_t)max(p.offsets[g], 0), p.rows);
+    const int64_t n = max((int64_t)0, min((int64_t)max(p.offsets[g + 1], 0), p.rows) - a);
+    const int64_t r0 = a + n * range / p.ranges, r1 = a + n * (range + 1) / p.ranges;
+    float s = 0.0f;
+    if (col < p.n) {
+        const T* x = static_cast<const T*>(p.x) + col;
 #pragma unroll 8
-            for (int r = r0 + part; r < r1; r += 4) s += to_float(x[r * p.ld]);
-        }
-        __syncthreads();
-        joined[part][c] = s;
-        __syncthreads();
-        if (part == 0 && col < p.n)
-            p.parts[line * p.n + col] = joined[0][c] + joined[1][c] + joined[2][c] + joined[3][c];
+        for (int64_t r = r0 + turn; r < r1; r += 4) s += to_float(x[r * p.ld]);
     }
+    joined[turn][c] = s;
+    __syncthreads();
+    if (turn != 0 || col >= p.n) return;
+    const float sum = joined[0][c] + joined[1][c] + joined[2][c] + joined[3][c];
+    if (p.ranges == 1) static_cast<T*>(p.out)[g * p.n + col] = from_float<T>(sum);
+    else p.sums[((int64_t)range * p.groups + g) * p.line + col] = sum;
 }
 
-// The parts of each group's lines, added up: 32 columns and a group a block; 32 threads of a column
-// take the parts in turn and join their sums in order.
+// the same of the parts that each group's lines of tiles left
 template <typename T>
-__global__ void __launch_bounds__(1024) k_group_sums(const SumParams p) {
+__global__ void __launch_bounds__(256) k_group_sums(const SumParams p) {
     follow_on();
-    extern __shared__ int32_t table[];
-    int32_t *first = table, *lines = table + p.groups + 1;
-    __shared__ float joined[32][33];
-    count_lines(p.offsets, p.rows, p.groups, p.high, first, lines);
-    const int c = threadIdx.x & 31, turn = threadIdx.x >> 5;
-    const int64_t col = (int64_t)blockIdx.x * 32 + c;
-    for (int g = blockIdx.y; g < p.groups; g += gridDim.y) {
-        const int64_t from = (int64_t)lines[g] * p.each, to = (int64_t)lines[g + 1] * p.each;
+    __shared__ float joined[4][64];
+    const int c = threadIdx.x & 63, turn = threadIdx.x >> 6;
+    const int64_t col = (int64_t)blockIdx.x * 64 + c;
+    const int g = blockIdx.y, range = blockIdx.z;
+    const LineCount lines = count_lines(p.offsets, p.rows, p.groups, g, p.high);
+    const int64_t n = (int64_t)(lines.with - lines.before) * p.each;
+    const int64_t first = (int64_t)lines.before * p.each;
+    const int64_t from = first + n * range / p.ranges, to = first + n * (range + 1) / p.ranges;
+    float s = 0.0f;
+    if (col < p.n) {
+#pragma unroll 8
+        for (int64_t i = from + turn; i < to; i += 4) s += p.parts[i * p.n + col];
+    }
+    joined[turn][c] = s;
+    __syncthreads();
+    if (turn != 0 || col >= p.n) return;
+    const float sum = joined[0][c] + joined[1][c] + joined[2][c] + joined[3][c];
+    if (p.ranges == 1) static_cast<T*>(p.out)[g * p.n + col] = from_float<T>(sum);
+    else p.sums[((int64_t)range * p.groups + g) * p.line + col] = sum;
+}
+
+// dbias from the sums of the ranges, in order
+template <typename T>
+__global__ void __launch_bounds__(256) k_join_sums(const SumParams p) {
+    follow_on();
+    const int64_t total = p.groups * p.n;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+         i += (int64_t)gridDim.x * 256) {
+        const int64_t g = i / p.n, col = i - g * p.n;
         float s = 0.0f;
-        if (col < p.n) {
-#pragma unroll 4
-            for (int64_t i = from + turn; i < to; i += 32) s += p.parts[i * p.n + col];
-        }
-        __syncthreads();
-        joined[turn][c] = s;
-        __syncthreads();
-        // warp `turn` adds up the column `turn`
-        const float all = warp_sum(joined[c][turn]);
-        const int64_t mine = (int64_t)blockIdx.x * 32 + turn;
-        if (c == 0 && mine < p.n) static_cast<T*>(p.out)[g * p.n + mine] = from_float<T>(all);
+#pragma unroll 8
+        for (int r = 0; r < p.ranges; ++r)
+            s += p.sums[((int64_t)r * p.groups + g) * p.line + col];
+        static_cast<T*>(p.out)[i] = from_float<T>(s);
     }
 }
 
-// out[i] = sum over the splits of part[s][i], rows of n values from lines of ld
+// dW from the parts of its tiles (kDepthRanges), added in the order of k: a block has 1024 / `lanes`
+// values of a tile, four a thread; `lanes` threads share the parts and join their sums in order.
+struct JoinParams {
+    const int32_t* offsets;
+    int64_t rows, m, n;
+    int groups, tiles_m, tiles_n, high, bn, ranges, lanes;
+    bool wide;         // rows of the output on 8 bytes
+    const float* parts;
+    void* out;         // [groups][m][n]
+};
+constexpr int kJoinThreads = 256;
 template <typename T>
-__global__ void __launch_bounds__(256)
-k_join_depth(const float* part, int splits, int64_t rows, int64_t n, int64_t ld, bool wide, T* out) {
+__global__ void __launch_bounds__(kJoinThreads) k_join_parts(const JoinParams p) {
     follow_on();
-    const int64_t groups = ld / 4, total = rows * groups;
-    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
-         i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t row = i / groups, col = (i - row * groups) * 4;
-        float v[4] = {};
+    __shared__ float4 joined[kJoinThreads];
+    const int tiles = p.tiles_m * p.tiles_n, g = blockIdx.x / tiles, at = blockIdx.x - g * tiles;
+    const LineCount lines = count_lines(p.offsets, p.rows, p.groups, g, 64);
+    // the ranges in which the group's first and last k-blocks lie
+    int r0 = 0, r1 = -1;
+    if (lines.with > lines.before) {
+        r0 = (int)((((uint64_t)lines.before + 1) * p.ranges - 1) / (unsigned)lines.all);
+        r1 = (int)(((uint64_t)lines.with * p.ranges - 1) / (unsigned)lines.all);
+    }
+    const int each = kJoinThreads / p.lanes;
+    const int item = threadIdx.x % each, lane = threadIdx.x / each;
+    const int i = (blockIdx.y * each + item) * 4, row = i / p.bn, col = i - row * p.bn;
+    const int64_t out_row = (int64_t)(at / p.tiles_n) * p.high + row;
+    const int64_t out_col = (int64_t)(at % p.tiles_n) * p.bn + col;
+    const bool in = out_row < p.m && out_col < p.n;
+    float v[4] = {};
+    if (in) {
+        const int64_t size = (int64_t)p.high * p.bn;
+        const float* part = p.parts + ((int64_t)g * tiles + at) * size + i;
 #pragma unroll 4
-        for (int s = 0; s < splits; ++s) {
-            const float4 q =
-                *reinterpret_cast<const float4*>(part + (s * rows + row) * ld + col);
+        for (int r = r0 + lane; r <= r1; r += p.lanes) {
+            const float4 q = *reinterpret_cast<const float4*>(part + r * tiles * size);
             v[0] += q.x, v[1] += q.y, v[2] += q.z, v[3] += q.w;
         }
-        T* to = out + row * n + col;
-        if (wide)
-            *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
-        else
-            for (int j = 0; j < 4 && col + j < n; ++j) to[j] = from_float<T>(v[j]);
     }
+    if (p.lanes > 1) {
+        joined[threadIdx.x] = make_float4(v[0], v[1], v[2], v[3]);
+        __syncthreads();
+        if (lane > 0) return;
+        for (int s = 1; s < p.lanes; ++s) {
+            const float4 q = joined[s * each + item];
+            v[0] += q.x, v[1] += q.y, v[2] += q.z, v[3] += q.w;
+        }
+    }
+    if (!in) return;
+    T* to = static_cast<T*>(p.out) + (g * p.m + out_row) * p.n + out_col;
+    if (p.wide)
+        *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+    else
+        for (int j = 0; j < 4 && out_col + j < p.n; ++j) to[j] = from_float<T>(v[j]);
 }
 
 // ----------------------------------------------------------------------------- host
@@ -225,9 +268,9 @@ Plan plan_rows(int64_t rows, int64_t groups, int64_t n_cols, int kblocks, bool g
     return best;
 }
 
-// Tile, pairing and ranges of k of the groups' products over their rows. The work divides among the
-// blocks but for its largest piece, a range of the largest group's rows, taken as three times the
-// mean; ranges cost the traffic of their join.
+// Tile and pairing of the groups' products over their rows. Either a tile is a block's own (splits
+// 1), and the last block's tiles, of a group of perhaps three times the mean, end late; or the
+// k-blocks of all groups divide into `splits` equal ranges, for the traffic and the launch of a join.
 Plan plan_depth(int64_t rows, int64_t groups, int64_t m, int64_t n, int sms, uint32_t fixed) {
     Plan best{};
     double best_cost = 0.0;
@@ -236,18 +279,26 @@ Plan plan_depth(int64_t rows, int64_t groups, int64_t m, int64_t n, int sms, uin
         for (int bn : {256, 128, 64}) {
             if (pair && bn == 64) continue;
             const int high = pair ? 2 * kBM : kBM, units = pair ? sms / 2 : sms;
-            const double tiles = (double)((m + high - 1) / high) * ((n + bn - 1) / bn) * groups;
-            for (int splits = 1; splits <= 64; splits *= 2) {
-                if (splits > 1 && 3.0 * depth / splits < 4.0) break;
-                const double epi = 1000.0 + 16.0 * bn, block = block_cycles(pair, bn);
-                const double all = tiles * std::max(depth * block, splits * epi) / units;
-                double cost = all + 3.0 * depth / splits * block + epi;
-                if (splits > 1)
-                    cost += 5000.0 + (double)groups * m * n * (splits + 1) * 4.0 / 3000.0;
+            const double tiles = (double)((m + high - 1) / high) * ((n + bn - 1) / bn);
+            const double epi = 1000.0 + 16.0 * bn, block = block_cycles(pair, bn);
+            auto offer = [&](double cost, int splits) {
                 if (best.bn == 0 || cost < best_cost) {
                     best_cost = cost;
                     best = {bn, splits, 0, 0, pair == 1};
                 }
+            };
+            offer(std::max(1.0, tiles * groups / units) * std::max(depth * block, epi) +
+                      2.0 * depth * block + epi, 1);
+            if (tiles * (rows / 64.0 + groups) > 1.0e9) continue;  // its counter has 32 bits
+            for (int waves = 1; waves <= 4; ++waves) {
+                // one to four items a block, of four k-blocks at least
+                const int ranges = (int)std::min(std::floor(waves * units / tiles),
+                                                 depth * groups / 4.0);
+                if (ranges < 2) continue;
+                const double items = std::ceil(ranges * tiles / units);
+                const double each = depth * groups / ranges * block;
+                offer(items * (each + (1.0 + (double)groups / ranges) * epi) + 6000.0 +
+                          (ranges + groups) * tiles * high * bn * 8.0 / 3000.0, ranges);
             }
         }
     }
@@ -371,9 +422,14 @@ void run_depth(const rune_grouped_linear_grad_args& a, const Matrix& dz, const M
     const uint32_t fixed =
         std::max(kFixedSmem<kForward>, kFixedSmem<kPartial>) + table_bytes(a.groups);
     const Plan plan = plan_depth(a.rows, a.groups, m, n, sms, fixed);
-    const int64_t ld = (n + 3) / 4 * 4;
+    const int high = plan.pair ? 2 * kBM : kBM;
+    const int tiles_m = (int)((m + high - 1) / high), tiles_n = (int)((n + plan.bn - 1) / plan.bn);
+    const int64_t tiles = (int64_t)tiles_m * tiles_n * a.groups;
     auto* maps = ws.take<CUtensorMap>(2 * a.groups);
-    float* part = plan.splits > 1 ? ws.take<float>(plan.splits * a.groups * m * ld) : nullptr;
+    float* parts =
+        plan.splits > 1
+            ? ws.take<float>((a.groups + plan.splits) * tiles_m * tiles_n * high * plan.bn)
+            : nullptr;
     if (ws.sizing()) return;
     const CUtensorMap ma = make_map(dz, 2, 64), mb = make_map(x, 2, 64);
     const MapParams mp{a.offsets,
@@ -391,34 +447,36 @@ void run_depth(const rune_grouped_linear_grad_args& a, const Matrix& dz, const M
     p.act = RUNE_ACT_NONE;
     p.m_all = a.rows, p.groups = (int)a.groups, p.offsets = a.offsets;
     p.group_maps = maps;
-    p.bn = plan.bn, p.stages = plan.stages, p.splits = plan.splits;
-    const int high = plan.pair ? 2 * kBM : kBM;
-    p.tiles_m = (int)((m + high - 1) / high);
-    p.tiles_n = (int)((n + p.bn - 1) / p.bn);
-    p.by_tiles = make_divisor((unsigned)p.tiles_m * p.tiles_n);
-    p.by_group = make_divisor(kGroup * (unsigned)p.tiles_n);
-    p.by_last = make_divisor(std::max(1u, (unsigned)p.tiles_m % kGroup));
+    p.bn = plan.bn, p.stages = plan.stages, p.splits = 1;
+    p.tiles_m = tiles_m, p.tiles_n = tiles_n;
+    p.by_tiles = make_divisor((unsigned)tiles_m * tiles_n);
+    p.by_group = make_divisor(kGroup * (unsigned)tiles_n);
+    p.by_last = make_divisor(std::max(1u, (unsigned)tiles_m % kGroup));
     p.a_mn = p.b_mn = 1;
     p.idesc = operand_idesc(a.dtype == RUNE_BF16 ? 1 : 0, true, true, high, p.bn);
     p.flag = wait_flag(a.device);
     p.polls = wait_polls();
-    const int64_t work = (int64_t)p.tiles_m * p.tiles_n * p.splits * a.groups;
     if (plan.splits == 1) {
         p.out = a.dweight, p.ld_out = n, p.out_step = m * n;
         p.tma_out = wide16(a.dweight, n, n);
         const CUtensorMap o =
             p.tma_out ? make_out_map3(a.dweight, m, n, n, a.groups, m * n) : ma;
-        launch_kind<kForward, kDepthGroups, T>(plan.pair, ma, mb, o, o, p, work, fixed, sms,
+        launch_kind<kForward, kDepthGroups, T>(plan.pair, ma, mb, o, o, p, tiles, fixed, sms,
                                                a.device, stream);
         return;
     }
-    p.z = part, p.ld_z = ld;
-    launch_kind<kPartial, kDepthGroups, __half>(plan.pair, ma, mb, ma, ma, p, work, fixed, sms,
-                                                a.device, stream);
-    const int64_t items = a.groups * m * (ld / 4);
-    launch(k_join_depth<T>, (unsigned)std::min<int64_t>((items + 255) / 256, (int64_t)sms * 16),
-           256, 0, 0, stream, part, plan.splits, a.groups * m, n, ld,
-           n % 4 == 0 && aligned(a.dweight, 8), static_cast<T*>(a.dweight));
+    p.ranges = plan.splits;
+    p.z = parts, p.ld_part = high;
+    launch_kind<kPartial, kDepthRanges, __half>(plan.pair, ma, mb, ma, ma, p,
+                                                (int64_t)plan.splits * tiles_m * tiles_n, fixed,
+                                                sms, a.device, stream);
+    // sixteen threads share the parts of a tile where these are many
+    const int lanes = plan.splits >= 16 * a.groups ? 16 : 1;
+    const JoinParams j{a.offsets, a.rows, m, n, (int)a.groups, tiles_m, tiles_n, high, plan.bn,
+                       plan.splits, lanes, n % 4 == 0 && aligned(a.dweight, 8), parts, a.dweight};
+    launch(k_join_parts<T>,
+           dim3((unsigned)tiles, (unsigned)(high * plan.bn / 4 * lanes / kJoinThreads)),
+           kJoinThreads, 0, 0, stream, j);
 }
 
 void backward(const rune_grouped_linear_grad_args& a, Scratch& ws, cudaStream_t stream) {
@@ -434,10 +492,10 @@ void backward(const rune_grouped_linear_grad_args& a, Scratch& ws, cudaStream_t 
     g.device = a.device, g.dtype = a.dtype;
     Matrix dz{a.dy, a.rows, n_all, a.dy_stride};
     SumParams sum{a.offsets, a.rows, n_all, (int)a.groups, 0, 0, a.dy_stride, a.dy, nullptr,
-                  a.dbias};
+                  a.dbias, 1, 0, nullptr};
     if (plain) {
         if (a.dx || a.dweight) dz = readable(dz, 2, ws, stream);
-        sum.high = 64, sum.each = 1;
+        sum.high = sum.each = 1;  // a row is a part
     } else {
         dz.ld = pad16(n_all, 2);
         dz.p = ws.take<uint16_t>(a.rows * dz.ld);
@@ -456,26 +514,36 @@ void backward(const rune_grouped_linear_grad_args& a, Scratch& ws, cudaStream_t 
         sum.high = run_rows(a.gated ? kGatedGrad : kGrad, g, p, false, stream);
         sum.each = sum.high / 32;  // one a warp
     }
-    if (a.dbias)
-        sum.parts =
-            ws.take<float>(line_bound(a.rows, a.groups, sum.high) * sum.each * n_all);
-    const uint32_t table = table_bytes(a.groups);
+    if (a.dbias) {
+        const int64_t parts = plain ? a.rows : line_bound(a.rows, a.groups, sum.high) * sum.each;
+        if (!plain) sum.parts = ws.take<float>(parts * n_all);
+        // 64 parts a range where groups are alike; more ranges than one cost a launch
+        const int64_t mean = parts / a.groups;
+        sum.ranges = mean < 256 ? 1 : (int)std::min<int64_t>(256, mean / 64);
+        sum.line = (n_all + 3) / 4 * 4;
+        if (sum.ranges > 1) sum.sums = ws.take<float>(sum.ranges * a.groups * sum.line);
+    }
     const int sms = sm_count(a.device);
     if (!ws.sizing()) {
         if (!plain) {
             p.colsum = sum.parts;
             run_rows(a.gated ? kGatedGrad : kGrad, g, p, true, stream);
-        } else if (a.dbias) {
-            const dim3 grid((unsigned)((n_all + 63) / 64),
-                            (unsigned)std::min<int64_t>(
-                                line_bound(a.rows, a.groups, sum.high), 8 * sms));
-            if (half) launch(k_group_columns<__half>, grid, 256, table, 0, stream, sum);
-            else launch(k_group_columns<__nv_bfloat16>, grid, 256, table, 0, stream, sum);
         }
         if (a.dbias) {
-            const dim3 grid((unsigned)((n_all + 31) / 32), (unsigned)a.groups);
-            if (half) launch(k_group_sums<__half>, grid, 1024, table, 0, stream, sum);
-            else launch(k_group_sums<__nv_bfloat16>, grid, 1024, table, 0, stream, sum);
+            const dim3 grid((unsigned)((n_all + 63) / 64), (unsigned)a.groups,
+                            (unsigned)sum.ranges);
+            auto go = [&](auto t) {
+                using T = decltype(t);
+                if (plain) launch(k_group_columns<T>, grid, 256, 0, 0, stream, sum);
+                else launch(k_group_sums<T>, grid, 256, 0, 0, stream, sum);
+                if (sum.ranges > 1) {
+                    const int64_t blocks = (a.groups * n_all + 255) / 256;
+                    launch(k_join_sums<T>, (unsigned)std::min<int64_t>(blocks, 16 * sms), 256, 0, 0,
+                           stream, sum);
+                }
+            };
+            if (half) go(__half());
+            else go(__nv_bfloat16());
         }
         RUNE_LAUNCH_CHECK();
     } else if (!plain) {

@@ -347,6 +347,7 @@ struct MoveParams {
     int64_t rows, slots;       // slots = rows * k
     int64_t ld_in, ld_more;
     int width, k;
+    int lanes;                 // of a team, which has a row (or a part of it) to itself
     const void* in;            // to_groups: x; from_groups: y; its gradient: dout
     const void* more;          // the gradient's y
     const int32_t *order, *place;
@@ -355,155 +356,197 @@ struct MoveParams {
     float* dweights;           // [slots]
 };
 
-// Items are (output row, `lanes` pieces of it); a team of `lanes` lanes has one, kItems of them at a
-// time, so that a row's index and then its pieces are under way for several rows at once.
-constexpr int kItems = 4, kMoveThreads = 256;
+// A team of lanes moves R rows at a time, C pieces of each a lane, so that enough is under way while
+// the rows' indexes, and then their pieces, arrive: narrow rows four at a time, wide ones in parts of
+// four pieces a lane, the parts of a row along the grid's y. B200, 110592 x 256 bf16 to two groups
+// each and back, us: to 32 -> 27, from 37 -> 30, from's gradient 101 -> 54 against one row a team.
+constexpr int kMoveThreads = 256;
+template <int R_, int C_>
+struct Shape {
+    static constexpr int R = R_, C = C_;
+};
 
-template <typename T, int N, bool SCALED>
-__global__ void __launch_bounds__(kMoveThreads)
-k_to_groups(const MoveParams p, int lanes, int chunks) {
+struct Team {
+    int index, at, count;
+    __device__ __forceinline__ explicit Team(int lanes)
+        : index(threadIdx.x / lanes), at(threadIdx.x % lanes), count(kMoveThreads / lanes) {}
+};
+
+template <typename T, int N, int R, int C, bool SCALED>
+__global__ void __launch_bounds__(kMoveThreads) k_to_groups(const MoveParams p) {
     follow_on();
-    const int team = threadIdx.x / lanes, at = threadIdx.x % lanes;
-    const int teams = kMoveThreads / lanes;
-    const int64_t items = p.slots * chunks;
-    for (int64_t i0 = ((int64_t)blockIdx.x * kItems) * teams + team; i0 < items;
-         i0 += (int64_t)gridDim.x * kItems * teams) {
-        int64_t row[kItems];
-        int col[kItems], slot[kItems];
-        float w[kItems];
+    const Team t(p.lanes);
+    const int col0 = ((int)blockIdx.y * C * p.lanes + t.at) * N, step = p.lanes * N;
+    for (int64_t r0 = (int64_t)blockIdx.x * t.count * R + t.index; r0 < p.slots;
+         r0 += (int64_t)gridDim.x * t.count * R) {
+        int slot[R];
+        float w[R];
 #pragma unroll
-        for (int i = 0; i < kItems; ++i) {
-            const int64_t item = i0 + (int64_t)i * teams;
-            row[i] = chunks == 1 ? item : item / chunks;
-            col[i] = ((int)(item - row[i] * chunks) * lanes + at) * N;
-            if (item >= items || col[i] >= p.width) row[i] = -1;
-            slot[i] = row[i] >= 0 ? p.order[row[i]] : -1;
+        for (int i = 0; i < R; ++i) {
+            const int64_t row = r0 + i * t.count;
+            slot[i] = row < p.slots ? p.order[row] : -1;
             if (slot[i] >= p.slots) slot[i] = -1;
         }
-        if constexpr (SCALED) {
 #pragma unroll
-            for (int i = 0; i < kItems; ++i) w[i] = slot[i] >= 0 ? p.weights[slot[i]] : 0.0f;
-        }
-        Piece<T, N> v[kItems];
+        for (int i = 0; i < R; ++i) w[i] = SCALED && slot[i] >= 0 ? p.weights[slot[i]] : 0.0f;
+        Piece<T, N> v[R][C];
 #pragma unroll
-        for (int i = 0; i < kItems; ++i) {
-            v[i].clear();
-            if (slot[i] >= 0)
-                v[i].load(static_cast<const T*>(p.in) + (int64_t)(slot[i] / p.k) * p.ld_in + col[i]);
-        }
+        for (int i = 0; i < R; ++i) {
+            const T* from = static_cast<const T*>(p.in) + (int64_t)(slot[i] / p.k) * p.ld_in;
 #pragma unroll
-        for (int i = 0; i < kItems; ++i) {
-            if constexpr (SCALED) {
-                float f[N];
-                v[i].get(f);
-#pragma unroll
-                for (int j = 0; j < N; ++j) f[j] = slot[i] >= 0 ? f[j] * w[i] : 0.0f;
-                v[i].set(f);
+            for (int c = 0; c < C; ++c) {
+                v[i][c].clear();
+                if (slot[i] >= 0 && col0 + c * step < p.width) v[i][c].load(from + col0 + c * step);
             }
-            if (row[i] >= 0) v[i].store(static_cast<T*>(p.out) + row[i] * p.width + col[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int64_t row = r0 + i * t.count;
+            T* to = static_cast<T*>(p.out) + row * p.width;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                if constexpr (SCALED) {
+                    float f[N];
+                    v[i][c].get(f);
+#pragma unroll
+                    for (int j = 0; j < N; ++j) f[j] = slot[i] >= 0 ? f[j] * w[i] : 0.0f;
+                    v[i][c].set(f);
+                }
+                if (row < p.slots && col0 + c * step < p.width) v[i][c].store(to + col0 + c * step);
+            }
         }
     }
 }
 
-template <typename T, int N>
-__global__ void __launch_bounds__(kMoveThreads)
-k_from_groups(const MoveParams p, int lanes, int chunks) {
+template <typename T, int N, int R, int C>
+__global__ void __launch_bounds__(kMoveThreads) k_from_groups(const MoveParams p) {
     follow_on();
-    const int team = threadIdx.x / lanes, at = threadIdx.x % lanes;
-    const int teams = kMoveThreads / lanes;
-    const int64_t items = p.rows * chunks;
-    constexpr int kAhead = 4;  // choices whose pieces are under way at once
-    for (int64_t item = (int64_t)blockIdx.x * teams + team; item < items;
-         item += (int64_t)gridDim.x * teams) {
-        const int64_t row = chunks == 1 ? item : item / chunks;
-        const int col = ((int)(item - row * chunks) * lanes + at) * N;
-        if (col >= p.width) continue;
-        float sum[N] = {};
+    const Team t(p.lanes);
+    const int col0 = ((int)blockIdx.y * C * p.lanes + t.at) * N, step = p.lanes * N;
+    constexpr int kAhead = 2;  // choices whose pieces are under way at once
+    for (int64_t r0 = (int64_t)blockIdx.x * t.count * R + t.index; r0 < p.rows;
+         r0 += (int64_t)gridDim.x * t.count * R) {
+        float sum[R][C][N] = {};
         for (int j0 = 0; j0 < p.k; j0 += kAhead) {
-            int place[kAhead];
-            float w[kAhead];
+            int place[R][kAhead];
+            float w[R][kAhead];
 #pragma unroll
-            for (int j = 0; j < kAhead; ++j) {
-                place[j] = j0 + j < p.k ? p.place[row * p.k + j0 + j] : -1;
-                if (place[j] >= p.slots) place[j] = -1;
-                w[j] = 1.0f;
-                if (p.weights && place[j] >= 0) w[j] = p.weights[row * p.k + j0 + j];
-            }
-            Piece<T, N> v[kAhead];
+            for (int i = 0; i < R; ++i)
 #pragma unroll
-            for (int j = 0; j < kAhead; ++j)
-                if (place[j] >= 0)
-                    v[j].load(static_cast<const T*>(p.in) + place[j] * p.ld_in + col);
+                for (int j = 0; j < kAhead; ++j) {
+                    const int64_t row = r0 + i * t.count;
+                    const bool in = row < p.rows && j0 + j < p.k;
+                    place[i][j] = in ? p.place[row * p.k + j0 + j] : -1;
+                    w[i][j] = in && p.weights ? p.weights[row * p.k + j0 + j] : 1.0f;
+                    if (place[i][j] >= p.slots) place[i][j] = -1;
+                }
+            Piece<T, N> v[R][C][kAhead];
 #pragma unroll
-            for (int j = 0; j < kAhead; ++j) {
-                if (place[j] < 0) continue;
-                float f[N];
-                v[j].get(f);
+            for (int i = 0; i < R; ++i)
 #pragma unroll
-                for (int i = 0; i < N; ++i) sum[i] = fmaf(f[i], w[j], sum[i]);
-            }
-        }
-        Piece<T, N> o;
-        o.set(sum);
-        o.store(static_cast<T*>(p.out) + row * p.width + col);
-    }
-}
-
-// A warp per slot: dy of its place and the weight's gradient; the slots of one row follow one
-// another, so that dout comes from L1 after the first. The warp also clears the row of dy that is
-// nobody's place.
-template <typename T, int N>
-__global__ void __launch_bounds__(kMoveThreads) k_from_groups_grad(const MoveParams p) {
-    follow_on();
-    const int lane = threadIdx.x & 31;
-    constexpr int kWarps = kMoveThreads / 32, kAhead = 4;
-    const int pieces = p.width / N;
-    for (int64_t slot = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); slot < p.slots;
-         slot += (int64_t)gridDim.x * kWarps) {
-        int64_t place = p.place[slot];
-        if (place >= p.slots) place = -1;
-        const int owner = p.order[slot];
-        const float w = p.weights[slot];
-        T* dy = static_cast<T*>(p.out);
-        if (dy && (owner < 0 || owner >= p.slots)) {
-            Piece<T, N> zero;
-            zero.clear();
-            for (int i = lane; i < pieces; i += 32) zero.store(dy + slot * p.width + i * N);
-        }
-        float dot = 0.0f;
-        if (place >= 0) {
-            const T* dout = static_cast<const T*>(p.in) + slot / p.k * p.ld_in;
-            const T* y = static_cast<const T*>(p.more) + place * p.ld_more;
-            for (int i0 = lane; i0 < pieces; i0 += 32 * kAhead) {
-                Piece<T, N> a[kAhead], b[kAhead];
+                for (int j = 0; j < kAhead; ++j) {
+                    const T* from = static_cast<const T*>(p.in) + place[i][j] * p.ld_in;
 #pragma unroll
-                for (int i = 0; i < kAhead; ++i) {
-                    a[i].clear(), b[i].clear();
-                    if (i0 + 32 * i >= pieces) continue;
-                    a[i].load(dout + (i0 + 32 * i) * N);
-                    if (p.dweights) b[i].load(y + (i0 + 32 * i) * N);
+                    for (int c = 0; c < C; ++c)
+                        if (place[i][j] >= 0 && col0 + c * step < p.width)
+                            v[i][c][j].load(from + col0 + c * step);
                 }
 #pragma unroll
-                for (int i = 0; i < kAhead; ++i) {
-                    float f[N], h[N];
-                    a[i].get(f), b[i].get(h);
-                    if (i0 + 32 * i < pieces) {
+            for (int i = 0; i < R; ++i)
 #pragma unroll
-                        for (int j = 0; j < N; ++j) {
-                            dot = fmaf(f[j], h[j], dot);
-                            f[j] *= w;
-                        }
-                        if (dy) {
-                            a[i].set(f);
-                            a[i].store(dy + place * p.width + (i0 + 32 * i) * N);
-                        }
+                for (int j = 0; j < kAhead; ++j) {
+                    if (place[i][j] < 0) continue;
+#pragma unroll
+                    for (int c = 0; c < C; ++c) {
+                        float f[N];
+                        v[i][c][j].get(f);
+#pragma unroll
+                        for (int n = 0; n < N; ++n)
+                            sum[i][c][n] = fmaf(f[n], w[i][j], sum[i][c][n]);
                     }
                 }
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int64_t row = r0 + i * t.count;
+            T* to = static_cast<T*>(p.out) + row * p.width;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                Piece<T, N> o;
+                o.set(sum[i][c]);
+                if (row < p.rows && col0 + c * step < p.width) o.store(to + col0 + c * step);
             }
         }
-        if (p.dweights) {
-            dot = warp_sum(dot);
-            if (lane == 0) p.dweights[slot] = place >= 0 ? dot : 0.0f;
+    }
+}
+
+// A team per slot: dy of its place and the weight's gradient, over the whole row; the slots of one
+// row are neighbours, so that dout comes from L1 after the first. The team also clears the row of
+// dy that is nobody's place.
+template <typename T, int N, int R, int C>
+__global__ void __launch_bounds__(kMoveThreads) k_from_groups_grad(const MoveParams p) {
+    follow_on();
+    const Team t(p.lanes);
+    const int step = p.lanes * N;
+    T* dy = static_cast<T*>(p.out);
+    for (int64_t b0 = (int64_t)blockIdx.x * t.count * R; b0 < p.slots;
+         b0 += (int64_t)gridDim.x * t.count * R) {  // all teams, for the sums
+        const int64_t s0 = b0 + t.index;
+        int place[R], owner[R];
+        float w[R], dot[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int64_t slot = s0 + i * t.count;
+            place[i] = slot < p.slots ? p.place[slot] : -1;
+            owner[i] = slot < p.slots ? p.order[slot] : 0;
+            w[i] = slot < p.slots ? p.weights[slot] : 0.0f;
+            if (place[i] >= p.slots) place[i] = -1;
+            dot[i] = 0.0f;
+        }
+        for (int col0 = t.at * N; col0 < p.width; col0 += C * step) {
+            Piece<T, N> a[R][C], b[R][C];
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const int64_t slot = s0 + i * t.count;
+                const T* dout = static_cast<const T*>(p.in) + slot / p.k * p.ld_in;
+                const T* y = static_cast<const T*>(p.more) + place[i] * p.ld_more;
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    a[i][c].clear(), b[i][c].clear();
+                    if (place[i] < 0 || col0 + c * step >= p.width) continue;
+                    a[i][c].load(dout + col0 + c * step);
+                    if (p.dweights) b[i][c].load(y + col0 + c * step);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    float f[N], h[N];
+                    a[i][c].get(f), b[i][c].get(h);
+#pragma unroll
+                    for (int n = 0; n < N; ++n) {
+                        dot[i] = fmaf(f[n], h[n], dot[i]);
+                        f[n] *= w[i];
+                    }
+                    if (!dy || col0 + c * step >= p.width) continue;
+                    a[i][c].set(f);
+                    if (place[i] >= 0)
+                        a[i][c].store(dy + (int64_t)place[i] * p.width + col0 + c * step);
+                    if (owner[i] < 0 || owner[i] >= p.slots) {
+                        Piece<T, N> zero;
+                        zero.clear();
+                        zero.store(dy + (s0 + i * t.count) * p.width + col0 + c * step);
+                    }
+                }
+        }
+        if (!p.dweights) continue;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            for (int o = p.lanes / 2; o > 0; o >>= 1)
+                dot[i] += __shfl_xor_sync(0xffffffffu, dot[i], o);
+            const int64_t slot = s0 + i * t.count;
+            if (t.at == 0 && slot < p.slots) p.dweights[slot] = place[i] >= 0 ? dot[i] : 0.0f;
         }
     }
 }
@@ -545,17 +588,23 @@ void with_type(int dtype, Fn&& fn) {
     else fn(float());
 }
 
-struct Teams {
-    int lanes, chunks;
-    unsigned grid;
-};
-// lanes that share a row, chunks of a row, and the blocks for `rows` of them, `items` at a time
-Teams teams_of(int64_t rows, int pieces, int items, int device) {
-    int lanes = 1;
-    while (lanes < 32 && lanes < pieces) lanes *= 2;
-    const int chunks = (pieces + lanes - 1) / lanes, teams = kMoveThreads / lanes * items;
-    const int64_t blocks = (rows * chunks + teams - 1) / teams;
-    return {lanes, chunks, (unsigned)std::min<int64_t>(blocks, (int64_t)sm_count(device) * 32)};
+// fn(Shape<R, C>()) and the grid for `rows` rows of `pieces`; sets p.lanes. parts: whether the parts
+// of wide rows lie along the grid's y.
+template <typename Fn>
+void with_shape(MoveParams& p, int64_t rows, int pieces, bool parts, int device, Fn&& fn) {
+    p.lanes = 1;
+    while (p.lanes < 32 && p.lanes < pieces) p.lanes *= 2;
+    auto go = [&](auto shape) {
+        constexpr int R = decltype(shape)::R, C = decltype(shape)::C;
+        const int64_t teams = kMoveThreads / p.lanes * R;
+        const unsigned y = parts ? (unsigned)((pieces + 32 * C - 1) / (32 * C)) : 1u;
+        require(y <= 65535, "width out of range");
+        const int64_t most = std::max<int64_t>(1, (int64_t)sm_count(device) * 32 / y);
+        fn(shape, dim3((unsigned)std::min<int64_t>((rows + teams - 1) / teams, most), y));
+    };
+    if (pieces <= 32) go(Shape<4, 1>());
+    else if (pieces <= 64) go(Shape<2, 2>());
+    else go(Shape<1, 4>());
 }
 
 bool value_type(int dtype) {
@@ -755,19 +804,19 @@ int rune_to_groups(const rune_group_move_args* args, void* stream_) {
         check_waits(a.device);
         if (a.rows == 0) return;
         require(a.in && a.order && a.out, "null argument");
-        const MoveParams p = move_params(a);
+        MoveParams p = move_params(a);
         const int n = piece_values(dtype_bytes(a.dtype), a.width,
                                    {{a.in, a.rows > 1 ? a.in_stride : a.width}, {a.out, a.width}});
         with_piece(a.dtype, n, [&](auto t, auto n_c) {
             using T = decltype(t);
             constexpr int N = decltype(n_c)::value;
-            const Teams team = teams_of(p.slots, (int)(a.width / N), kItems, a.device);
-            if (a.weights)
-                launch(k_to_groups<T, N, true>, team.grid, kMoveThreads, 0, 0, stream, p,
-                       team.lanes, team.chunks);
-            else
-                launch(k_to_groups<T, N, false>, team.grid, kMoveThreads, 0, 0, stream, p,
-                       team.lanes, team.chunks);
+            with_shape(p, p.slots, (int)(a.width / N), true, a.device, [&](auto shape, dim3 grid) {
+                constexpr int R = decltype(shape)::R, C = decltype(shape)::C;
+                if (a.weights)
+                    launch(k_to_groups<T, N, R, C, true>, grid, kMoveThreads, 0, 0, stream, p);
+                else
+                    launch(k_to_groups<T, N, R, C, false>, grid, kMoveThreads, 0, 0, stream, p);
+            });
         });
         RUNE_LAUNCH_CHECK();
     });
@@ -785,16 +834,17 @@ int rune_from_groups(const rune_group_move_args* args, void* stream_) {
         check_waits(a.device);
         if (a.rows == 0) return;
         require(a.in && a.place && a.out, "null argument");
-        const MoveParams p = move_params(a);
+        MoveParams p = move_params(a);
         const int n = piece_values(
             dtype_bytes(a.dtype), a.width,
             {{a.in, a.rows * a.k > 1 ? a.in_stride : a.width}, {a.out, a.width}});
         with_piece(a.dtype, n, [&](auto t, auto n_c) {
             using T = decltype(t);
             constexpr int N = decltype(n_c)::value;
-            const Teams team = teams_of(p.rows, (int)(a.width / N), 1, a.device);
-            launch(k_from_groups<T, N>, team.grid, kMoveThreads, 0, 0, stream, p, team.lanes,
-                   team.chunks);
+            with_shape(p, p.rows, (int)(a.width / N), true, a.device, [&](auto shape, dim3 grid) {
+                constexpr int R = decltype(shape)::R, C = decltype(shape)::C;
+                launch(k_from_groups<T, N, R, C>, grid, kMoveThreads, 0, 0, stream, p);
+            });
         });
         RUNE_LAUNCH_CHECK();
     });
@@ -814,16 +864,18 @@ int rune_from_groups_backward(const rune_group_move_args* args, void* stream_) {
         require(a.in && a.order && a.place && a.weights && (a.out || a.dweights) &&
                     (a.y || !a.dweights),
                 "null argument");
-        const MoveParams p = move_params(a);
+        MoveParams p = move_params(a);
         const int n = piece_values(dtype_bytes(a.dtype), a.width,
                                    {{a.in, a.rows > 1 ? a.in_stride : a.width},
                                     {a.y, a.rows * a.k > 1 ? a.y_stride : a.width},
                                     {a.out, a.width}});
         with_piece(a.dtype, n, [&](auto t, auto n_c) {
-            const int64_t blocks = (p.slots + 7) / 8;
-            launch(k_from_groups_grad<decltype(t), decltype(n_c)::value>,
-                   (unsigned)std::min<int64_t>(blocks, (int64_t)sm_count(a.device) * 32),
-                   kMoveThreads, 0, 0, stream, p);
+            using T = decltype(t);
+            constexpr int N = decltype(n_c)::value;
+            with_shape(p, p.slots, (int)(a.width / N), false, a.device, [&](auto shape, dim3 grid) {
+                constexpr int R = decltype(shape)::R, C = decltype(shape)::C;
+                launch(k_from_groups_grad<T, N, R, C>, grid, kMoveThreads, 0, 0, stream, p);
+            });
         });
         RUNE_LAUNCH_CHECK();
     });

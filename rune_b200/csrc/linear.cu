@@ -239,11 +239,13 @@ __global__ void __launch_bounds__(256)
 k_pack(const uint8_t* src, int64_t rows, int64_t bytes, int64_t ld,
        uint8_t* dst, int64_t ld_dst) {
     follow_on();
-    const int64_t pieces = ld_dst / 16;
+    const int64_t pieces = ld_dst / 16, total = rows * pieces;
     const uint8_t* const end = src + (rows - 1) * ld + bytes;
-    const int64_t piece = (int64_t)blockIdx.x * 32 + threadIdx.x, at = piece * 16;
-    if (piece >= pieces) return;
-    for (int64_t r = (int64_t)blockIdx.y * 8 + threadIdx.y; r < rows; r += (int64_t)gridDim.y * 8) {
+    const bool small = total <= INT32_MAX;  // quotients of 32 bits are a few instructions
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+         i += (int64_t)gridDim.x * 256) {
+        const int64_t r = small ? (int64_t)((unsigned)i / (unsigned)pieces) : i / pieces;
+        const int64_t at = (i - r * pieces) * 16;
         const uint8_t* from = src + r * ld + at;
         const unsigned off = (unsigned)((uintptr_t)from & 15);
         const uint8_t* word = from - off;
@@ -426,9 +428,8 @@ void run_product(const Product& g, const TileParams& p, Scratch& ws, int device,
 
 void pad_rows(const void* src, int64_t rows, int64_t bytes, int64_t ld, void* dst, int64_t ld_dst,
               cudaStream_t stream) {
-    const dim3 grid((unsigned)((ld_dst / 16 + 31) / 32),
-                    (unsigned)std::min<int64_t>((rows + 7) / 8, 65535));
-    launch(k_pack, grid, dim3(32, 8), 0, 0, stream, static_cast<const uint8_t*>(src), rows, bytes,
+    const int64_t blocks = (rows * (ld_dst / 16) + 255) / 256;
+    launch(k_pack, (unsigned)std::min<int64_t>(blocks, 1 << 20), 256, 0, 0, stream, static_cast<const uint8_t*>(src), rows, bytes,
            ld, static_cast<uint8_t*>(dst), ld_dst);
 }
 

@@ -28,8 +28,10 @@ enum Kind {
     kWhole,        // one product
     kRowGroups,    // the rows of A by group, each with its own matrix B (and bias)
     kDepthGroups,  // the contraction by group: a product of its own for the rows of each
+    kDepthRanges,  // the same in parts: the k-blocks of all groups in equal ranges
     kBatch         // a stack of products
 };
+__host__ __device__ constexpr bool by_depth(int kind) { return kind == kDepthGroups || kind == kDepthRanges; }
 
 constexpr int kBM = 128;
 constexpr int kEpiWarps = 16, kTmaWarp = 16, kMmaWarp = 17;
@@ -77,7 +79,8 @@ struct TileParams {
     const int32_t* offsets;
     int64_t m_all, bias_step;
     int groups, zero_tail;  // zero_tail: rows of the output behind the last group are cleared
-    const CUtensorMap* group_maps;  // kDepthGroups: of A and B, cut to each group's rows
+    const CUtensorMap* group_maps;  // by depth: of A and B, cut to each group's rows
+    int ranges;                     // kDepthRanges
     // batches, and kUpdate
     int64_t in_step, out_step;
     float alpha, beta;
@@ -100,7 +103,8 @@ constexpr uint32_t kFixedSmem =
     kEpiWarps * kWarpBufs<MODE> * kWarpBuf + (uint32_t)((sizeof(TileShared) + 127) / 128 * 128);
 
 struct Tile {
-    int mt, nt, split;
+    int mt, nt;
+    int split;          // range of k; kDepthRanges: the part that it leaves
     int z;              // group, or product of the batch
     int row0, row_end;  // of the block's rows of the output: the first, and where they end
     bool empty;         // nothing to add up
@@ -122,10 +126,22 @@ __device__ __forceinline__ Tile tile_of(const TileParams& p, unsigned w) {
     return t;
 }
 
-// The tiles of one launch, in the order in which blocks (or pairs) `first`, `first` + stride, ...
-// take them, and the range of k of each. Of groups, whose sizes only the GPU knows, a table in
-// shared memory: rows[g], the groups' first rows, and (kRowGroups) lines[g], the number of lines of
-// tiles before group g.
+// A value that all lanes of a converged warp have, in a uniform register, where a reduction leaves
+// it: what comes from shared memory would stay in every lane's registers, and the epilogues have none
+// left (gated 221184 x 256 -> 2 x 512, dz: 330 us with 124 bytes spilled).
+__device__ __forceinline__ int uniform(int v) { return (int)__reduce_or_sync(0xffffffffu, (unsigned)v); }
+
+// The tiles of one launch in the order in which a block (or pair) takes them, and the range of k of
+// each. Of groups, whose sizes only the GPU knows, a table in shared memory: rows[g], the groups'
+// first rows, and lines[g], before group g the number of lines of tiles (kRowGroups) or of k-blocks
+// (kDepthRanges).
+//   kDepthRanges   the k-blocks of all groups, one after the other, in equal ranges. An item is a
+//                  range of one tile of every group, and leaves a part for each group that it
+//                  meets: part (range + group) tiles + tile, since along the k-blocks each part
+//                  begins with the next range or the next group. Blocks at work at one time have
+//                  the tiles of few ranges, whose operands they share in L2 (110592 x 1024 x 256 in
+//                  8 groups, all tiles one after the other instead: 121 us, so 97). Its counter w is
+//                  k-block * tiles + tile.
 template <int KIND, bool PAIR>
 struct Schedule {
     static constexpr int kTileRows = PAIR ? 2 * kBM : kBM;
@@ -133,33 +149,37 @@ struct Schedule {
     int32_t* rows;
     int32_t* lines;
     int rank;
-    unsigned work;
+    unsigned unit, step;     // this block (or pair) among how many
+    unsigned begin, end;     // of the counter of work
 
     __device__ __forceinline__ Schedule(const TileParams& params, int32_t* table, int r)
-        : p(params), rows(table), lines(table + params.groups + 1), rank(r) {}
+        : p(params), rows(table), lines(table + params.groups + 1), rank(r),
+          unit(PAIR ? blockIdx.x >> 1 : blockIdx.x), step(PAIR ? gridDim.x >> 1 : gridDim.x),
+          begin(unit) {}
 
     // all threads, once the offsets may be read
     __device__ __forceinline__ void fill() {
         const unsigned tiles = (unsigned)p.tiles_m * p.tiles_n;
         if constexpr (KIND == kWhole) {
-            work = tiles * p.splits;
+            end = tiles * p.splits;
         } else if constexpr (KIND == kBatch) {
             // symmetric: of square tiles those on and below the diagonal
-            work = (p.symmetric ? (unsigned)p.tiles_m * (p.tiles_m + 1) / 2 : tiles) * p.groups;
+            end = (p.symmetric ? (unsigned)p.tiles_m * (p.tiles_m + 1) / 2 : tiles) * p.groups;
         } else {
             for (int g = threadIdx.x; g <= p.groups; g += kThreads)
                 rows[g] = (int)min((int64_t)max(p.offsets[g], 0), p.m_all);
             __syncthreads();
             if constexpr (KIND == kDepthGroups) {
-                work = tiles * p.splits * p.groups;
+                end = tiles * p.groups;
             } else {
                 if (threadIdx.x < 32) {
+                    constexpr int kLine = KIND == kRowGroups ? kTileRows : 64;
                     int before = 0;
                     for (int g0 = 0; g0 < p.groups; g0 += 32) {
                         const int g = g0 + threadIdx.x;
                         int n = 0;
                         if (g < p.groups)
-                            n = (max(0, rows[g + 1] - rows[g]) + kTileRows - 1) / kTileRows;
+                            n = (max(0, rows[g + 1] - rows[g]) + kLine - 1) / kLine;
                         int sum = n;
 #pragma unroll
                         for (int o = 1; o < 32; o *= 2) {
@@ -172,9 +192,55 @@ struct Schedule {
                     if (threadIdx.x == 0) lines[p.groups] = before;
                 }
                 __syncthreads();
-                work = (unsigned)lines[p.groups] * p.tiles_n;
+                const unsigned all = (unsigned)uniform(lines[p.groups]);
+                if constexpr (KIND == kRowGroups) {
+                    end = all * p.tiles_n;
+                } else {
+                    end = all * tiles;
+                    begin = item(unit);
+                }
             }
         }
+    }
+
+    // the group g with lines[g] <= line < lines[g + 1]
+    __device__ __forceinline__ int group_at(int line) const {
+        int g = 0, above = p.groups;
+        while (above - g > 1) {
+            const int mid = (g + above) >> 1;
+            if (lines[mid] <= line) g = mid;
+            else above = mid;
+        }
+        return uniform(g);
+    }
+
+    // kDepthRanges: the range of k-block x, the last that begins at or before it; where range r
+    // begins; and the counter at which item i begins (the end behind the last)
+    __device__ __forceinline__ unsigned range_of(unsigned x) const {
+        return (unsigned)((((uint64_t)x + 1) * p.ranges - 1) / (unsigned)uniform(lines[p.groups]));
+    }
+    __device__ __forceinline__ unsigned start(unsigned r) const {
+        return (unsigned)((uint64_t)(unsigned)uniform(lines[p.groups]) * r / p.ranges);
+    }
+    __device__ __forceinline__ unsigned item(unsigned i) const {
+        const unsigned tiles = p.by_tiles.by;
+        for (; i < p.ranges * tiles; i += step) {
+            const unsigned r = p.by_tiles.quotient(i), x = start(r);
+            if (x < start(r + 1)) return x * tiles + i - r * tiles;
+        }
+        return end;
+    }
+
+    __device__ __forceinline__ unsigned next(unsigned w) const {
+        if constexpr (KIND == kDepthRanges) {
+            const unsigned tiles = p.by_tiles.by, x = p.by_tiles.quotient(w), r = range_of(x);
+            int kb0, kb1;
+            range(w, kb0, kb1);
+            const unsigned on = x + kb1 - kb0;
+            return on < start(r + 1) ? w + (kb1 - kb0) * tiles
+                                     : item(r * tiles + (w - x * tiles) + step);
+        }
+        return w + step;
     }
 
     __device__ __forceinline__ Tile tile(unsigned w) const {
@@ -184,30 +250,28 @@ struct Schedule {
             t.row_end = (int)p.m;
         } else if constexpr (KIND == kRowGroups) {
             const int line = (int)p.by_tiles.quotient(w);  // by the tiles of a line
-            int g = 0, above = p.groups;
-            while (above - g > 1) {
-                const int mid = (g + above) >> 1;
-                if (lines[mid] <= line) g = mid;
-                else above = mid;
-            }
-            const unsigned first = lines[g], n = lines[g + 1] - first;
+            const int g = group_at(line);
+            const unsigned first = uniform(lines[g]), n = uniform(lines[g + 1]) - first;
             const unsigned at = w - first * p.tiles_n, part = p.by_group.quotient(at);
             const unsigned in = at - part * p.by_group.by, high = min(kGroup, n - part * kGroup);
             t.nt = in / high;
             const int mt = part * kGroup + (in - t.nt * high);
             t.split = 0, t.z = g, t.empty = false;
-            t.row0 = rows[g] + mt * kTileRows + rank * kBM;
-            t.row_end = rows[g + 1];
+            t.row0 = uniform(rows[g]) + mt * kTileRows + rank * kBM;
+            t.row_end = uniform(rows[g + 1]);
             t.mt = ((int)first + mt) * (kTileRows / kBM) + rank;
             return t;
         } else if constexpr (KIND == kDepthGroups) {
-            const unsigned each = p.by_tiles.by * p.splits;
-            t = tile_of(p, w % each);
-            t.z = w / each;
-            int kb0, kb1;
-            range(w, kb0, kb1);
-            t.empty = kb0 >= kb1;
+            const unsigned z = p.by_tiles.quotient(w);
+            t = tile_of(p, w - z * p.by_tiles.by);
+            t.z = z;
+            t.empty = uniform(rows[z + 1] - rows[z]) <= 0;
             t.row_end = (int)p.m;
+        } else if constexpr (KIND == kDepthRanges) {
+            const unsigned x = p.by_tiles.quotient(w), at = w - x * p.by_tiles.by;
+            const int g = group_at((int)x), mt = at / p.tiles_n;
+            t = Tile{mt, (int)(at - mt * p.tiles_n),
+                     (int)((range_of(x) + g) * p.by_tiles.by + at), g, 0, (int)p.m, false};
         } else {
             if (p.symmetric) {
                 const unsigned each = (unsigned)p.tiles_m * (p.tiles_m + 1) / 2, in = w % each;
@@ -230,11 +294,14 @@ struct Schedule {
     // lines of k of work item w: [kb0, kb1)
     __device__ __forceinline__ void range(unsigned w, int& kb0, int& kb1) const {
         if constexpr (KIND == kDepthGroups) {
-            const unsigned each = p.by_tiles.by * p.splits, z = w / each;
-            const int split = (int)p.by_tiles.quotient(w - z * each);
-            const int blocks = (max(0, rows[z + 1] - rows[z]) + 63) / 64;
-            kb0 = (int)((int64_t)blocks * split / p.splits);
-            kb1 = (int)((int64_t)blocks * (split + 1) / p.splits);
+            const unsigned z = p.by_tiles.quotient(w);
+            kb0 = 0;
+            kb1 = (max(0, uniform(rows[z + 1] - rows[z])) + 63) / 64;
+        } else if constexpr (KIND == kDepthRanges) {
+            const unsigned x = p.by_tiles.quotient(w);
+            const int g = group_at((int)x);
+            kb0 = (int)x - uniform(lines[g]);
+            kb1 = min(uniform(lines[g + 1]), (int)start(range_of(x) + 1)) - uniform(lines[g]);
         } else {
             const int split =
                 KIND == kWhole && p.splits > 1 ? (int)p.by_tiles.quotient(w) : 0;
@@ -317,6 +384,18 @@ __device__ __forceinline__ void load_rows(const Stage& st, const T* src, int64_t
     }
 }
 
+// the buffer's rows x cols to dst, value by value: outputs whose rows are off 16 bytes
+template <typename T>
+__device__ __forceinline__ void store_rows(const Stage& st, T* dst, int64_t ld, int rows,
+                                           int64_t cols) {
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r) {
+        const uint16_t h = get_half(st.at(r, st.lane * 2));
+        if (r < rows && st.lane < cols)
+            reinterpret_cast<uint16_t*>(dst)[(int64_t)r * ld + st.lane] = h;
+    }
+}
+
 // the same of a part of a box, where rows are on 16 bytes
 template <typename T>
 __device__ __forceinline__ void store_rows16(const Stage& st, T* dst, int64_t ld, int rows,
@@ -327,6 +406,16 @@ __device__ __forceinline__ void store_rows16(const Stage& st, T* dst, int64_t ld
     for (int i = 0; i < 4; ++i)
         if (c < cols && r0 + 8 * i < rows)
             *reinterpret_cast<uint4*>(p + i * 8 * ld) = get16(st.turn(i));
+}
+
+// The box's part of a group's last rows. Not inlined: it is rare, and among the gradients' code it
+// took registers that they have not (gated 221184 x 256 -> 2 x 512, dz 330 -> 250 us).
+template <typename T>
+__device__ __noinline__ void store_part(uint32_t buf, T* dst, int64_t ld, int rows, int cols,
+                                        bool wide) {
+    const Stage st(buf, threadIdx.x & 31);
+    if (wide) store_rows16<T>(st, dst, ld, rows, cols);
+    else store_rows<T>(st, dst, ld, rows, cols);
 }
 
 // sums over the warp's rows of 16 columns that each lane holds of its own row, before they are
@@ -349,18 +438,6 @@ __device__ __forceinline__ void column_sums(const Two (&z)[8], int lane, int64_t
     }
     a[0] += __shfl_xor_sync(0xffffffffu, a[0], 1);
     if (!(lane & 1) && column < cols) sums[column] = a[0];
-}
-
-// the buffer's rows x cols to dst, value by value: outputs whose rows are off 16 bytes
-template <typename T>
-__device__ __forceinline__ void store_rows(const Stage& st, T* dst, int64_t ld, int rows,
-                                           int64_t cols) {
-#pragma unroll 8
-    for (int r = 0; r < 32; ++r) {
-        const uint16_t h = get_half(st.at(r, st.lane * 2));
-        if (r < rows && st.lane < cols)
-            reinterpret_cast<uint16_t*>(dst)[(int64_t)r * ld + st.lane] = h;
-    }
 }
 
 // a warp's 32 rows x 16 columns of float32, each lane its row, through the buffer to memory whose
@@ -388,7 +465,7 @@ template <typename T>
 struct Bias {
     uint32_t w[8];
     __device__ __forceinline__ void load(const TileParams& p, int64_t col, int64_t left,
-                                         int64_t at = 0) {
+                                         int at = 0) {
         const T* bias = static_cast<const T*>(p.bias) + at + col;
         if (!p.bias) return;
         if (p.vec_bias) {
@@ -488,7 +565,7 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
     const int lane = st.lane;
     constexpr bool kReads = MODE == kGrad || MODE == kGatedGrad;
     const bool reads = kReads || ((MODE == kForward || MODE == kUpdate) && p.in);
-    const int64_t bias_at = KIND == kRowGroups ? t.z * p.bias_step : 0;
+    const int bias_at = KIND == kRowGroups ? uniform(t.z * (int)p.bias_step) : 0;
     auto read_in = [&](int c) {  // residual or dy of the group
         const T* in = static_cast<const T*>(p.in);
         if constexpr (KIND == kBatch) in += t.z * p.in_step;
@@ -506,16 +583,14 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
     }
     if (!wait()) return;
     if constexpr (MODE == kPartial) {
-        const int64_t part = KIND == kDepthGroups ? (int64_t)t.split * p.groups + t.z : t.split;
         for (int c = share * 16; c < end; c += 64) {
             float v[16];
             tc::tmem_ld16(acc + c, v);
-            if (KIND == kDepthGroups && t.empty) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = 0.0f;
-            }
-            store_rows32(st, v, p.z + (part * p.m + row0) * p.ld_z + col0 + c, p.ld_z, rows,
-                         end - c);
+            // kDepthRanges: parts of whole tiles, this block's half of a pair's second
+            float* to = KIND == kDepthRanges
+                            ? p.z + ((int64_t)t.split * p.ld_part + row0 % p.ld_part) * p.bn + c
+                            : p.z + ((int64_t)t.split * p.m + row0) * p.ld_z + col0 + c;
+            store_rows32(st, v, to, KIND == kDepthRanges ? p.bn : p.ld_z, rows, end - c);
         }
         release();
         return;
@@ -659,17 +734,18 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
                 }
                 bulk_store_commit();
             }
-        } else if (KIND == kRowGroups && p.tma_out) {
-            T* out = static_cast<T*>(p.out) + (int64_t)row0 * p.ld_out + col;
-            store_rows16<T>(st, out, p.ld_out, rows, left);
-            if constexpr (MODE == kGatedGrad)
-                store_rows16<T>(st2, out + p.n, p.ld_out, rows, left);
         } else {
             T* out = static_cast<T*>(p.out) + (int64_t)row0 * p.ld_out + col;
-            if constexpr (KIND == kDepthGroups || KIND == kBatch) out += t.z * p.out_step;
-            store_rows<T>(st, out, p.ld_out, rows, left);
-            if constexpr (MODE == kGatedGrad)
-                store_rows<T>(st2, out + p.n, p.ld_out, rows, left);
+            if constexpr (KIND == kRowGroups) {
+                store_part<T>(st.base, out, p.ld_out, rows, (int)left, p.tma_out);
+                if constexpr (MODE == kGatedGrad)
+                    store_part<T>(st2.base, out + p.n, p.ld_out, rows, (int)left, p.tma_out);
+            } else {
+                if constexpr (KIND == kDepthGroups || KIND == kBatch) out += t.z * p.out_step;
+                store_rows<T>(st, out, p.ld_out, rows, left);
+                if constexpr (MODE == kGatedGrad)
+                    store_rows<T>(st2, out + p.n, p.ld_out, rows, left);
+            }
         }
         __syncwarp();
     }
@@ -731,8 +807,6 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
     constexpr bool kGate = MODE == kGated || MODE == kGatedGrad;
     const int rank = PAIR ? (int)cluster_rank() : 0;
     Schedule<KIND, PAIR> plan(p, reinterpret_cast<int32_t*>(sh + 1), rank);
-    const unsigned first = PAIR ? blockIdx.x >> 1 : blockIdx.x;
-    const unsigned stride = PAIR ? gridDim.x >> 1 : gridDim.x;
 
     if (tid == 0) {
         for (int s = 0; s < p.stages; ++s) {
@@ -765,7 +839,6 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
     volatile int* fail = &sh->fail;
     follow_on();
     plan.fill();
-    const unsigned work = plan.work;
 
     if (warp == kTmaWarp) {
         // ---- TMA producer
@@ -792,13 +865,13 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
         int st = 0, issued = 0;
         uint32_t parity = 1;  // of the stage's last release; a fresh barrier passes for 1
         bool ok = true;
-        for (unsigned w = first; w < work && ok; w += stride) {
+        for (unsigned w = plan.begin; w < plan.end && ok; w = plan.next(w)) {
             const Tile t = plan.tile(w);
             int kb0, kb1;
             plan.range(w, kb0, kb1);
             const int m0 = t.row0;
             const CUtensorMap *a_map = &map_a, *b_map = &map_b;
-            if constexpr (KIND == kDepthGroups) {
+            if constexpr (by_depth(KIND)) {
                 a_map = p.group_maps + 2 * t.z, b_map = a_map + 1;
                 if (one && kb0 < kb1) map_acquire(a_map), map_acquire(b_map);
             }
@@ -861,7 +934,7 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
         int st = 0, buf = 0;
         uint32_t parity = 0, acc_parity = 1;
         bool ok = true;
-        for (unsigned w = first; w < work && ok; w += stride) {
+        for (unsigned w = plan.begin; w < plan.end && ok; w = plan.next(w)) {
             int kb0, kb1;
             plan.range(w, kb0, kb1);
             ok = mbar_wait(smem_u32(&sh->acc_empty[buf]), acc_parity, p.polls) && !*fail;
@@ -913,7 +986,7 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
         const Stage st(buf, lane), st2(buf + (kWarpBufs<MODE> - 1) * kWarpBuf, lane);
         const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
         bool ok = true;
-        for (unsigned w = first; w < work && ok; w += stride, ++n_tile) {
+        for (unsigned w = plan.begin; w < plan.end && ok; w = plan.next(w), ++n_tile) {
             const Tile t = plan.tile(w);
             const int b = n_tile & 1, round = n_tile >> 1;
             epilogue<MODE, KIND, T, FP8>(

@@ -651,3 +651,30 @@ def test_a_wait_that_gives_up_is_reported(polls):
     y = ops.grouped_linear(x, w, g, activation="silu")
     got = [y.detach(), *torch.autograd.grad(y, [x, w], torch.ones_like(y))]
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu
+@pytest.mark.parametrize("sizes,inputs,outputs", [
+    ([5000, 0, 1, 63, 64, 65, 9000], 35, 30), ([30000], 64, 24), ([0, 20011, 0], 136, 200),
+    ([1, 2, 40000], 512, 520), ([700] * 40, 300, 264), ([2] * 900 + [3000], 24, 16)])
+def test_weight_gradients_over_long_groups(sizes, inputs, outputs):
+    """Groups whose rows many blocks share, and groups that end inside a block's range."""
+    dt, u = torch.bfloat16, U[torch.bfloat16]
+    g, index = by_sizes(sizes, 3)
+    rows = len(index)
+    x, dy = normal(131, rows, inputs, dtype=dt), normal(132, rows, outputs, dtype=dt)
+    w = normal(133, len(sizes), outputs, inputs, dtype=dt, scale=inputs ** -0.5)
+    b = normal(134, len(sizes), outputs, dtype=dt)
+    w, b = w.requires_grad_(True), b.requires_grad_(True)
+    dw, db = torch.autograd.grad(ops.grouped_linear(x, w, g, bias=b), [w, b], dy)
+    at = 0
+    for i, n in enumerate(sizes):
+        d, part = dy[at:at + n].double(), x[at:at + n].double()
+        at += n
+        s = d.abs().t() @ part.abs()
+        within(dw[i], d.t() @ part, *[(n + 2) * 2.0 ** -23 * s + u * (d.t() @ part).abs() * 1.01],
+               "dweight")
+        within(db[i], d.sum(0), (n + 2) * 2.0 ** -23 * d.abs().sum(0) + u * d.sum(0).abs() * 1.01,
+               "dbias")
+    again = torch.autograd.grad(ops.grouped_linear(x, w, g, bias=b), [w, b], dy)
+    assert torch.equal(again[0], dw) and torch.equal(again[1], db)
