@@ -29,33 +29,30 @@ constexpr int64_t kMaxGroups = 1024;
 
 // ----------------------------------------------------------------------------- kernels
 // Maps of two matrices' rows [offsets[g], offsets[g + 1]): the whole ones with another address and
-// number of rows. A warp writes one, from shared memory.
+// number of rows. A warp writes one, number `at`, from shared memory.
 struct MapParams {
+    CUtensorMap a, b;
     const int32_t* offsets;
     int64_t rows;
     int groups;
-    const char *a, *b;
+    const char *start_a, *start_b;
     int64_t line_a, line_b;  // bytes
-    CUtensorMap* maps;       // [groups][2]
+    CUtensorMap* maps;       // [groups][2]; null: none wanted
 };
-constexpr int kMapWarps = 4;
-__global__ void __launch_bounds__(32 * kMapWarps)
-k_group_maps(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-             const MapParams p) {
+constexpr int kMapWarps = 8;
+__device__ __forceinline__ void write_map(const MapParams& p, int at) {
     __shared__ __align__(128) uint32_t copy[kMapWarps][32];
-    follow_on();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int at = blockIdx.x * kMapWarps + warp, g = at >> 1;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = at >> 1;
     if (g >= p.groups) return;
     const bool second = at & 1;
     const int64_t first = min((int64_t)max(p.offsets[g], 0), p.rows);
     const int64_t end = min((int64_t)max(p.offsets[g + 1], 0), p.rows);
     if (first >= end) return;  // nothing to read: no one asks for the map
-    copy[warp][lane] = reinterpret_cast<const uint32_t*>(second ? &map_b : &map_a)[lane];
+    copy[warp][lane] = reinterpret_cast<const uint32_t*>(second ? &p.b : &p.a)[lane];
     __syncwarp();
     const uint32_t own = tc::smem_u32(copy[warp]);
     if (lane == 0) {
-        const char* start = second ? p.b + first * p.line_b : p.a + first * p.line_a;
+        const char* start = second ? p.start_b + first * p.line_b : p.start_a + first * p.line_a;
         asm volatile("tensormap.replace.tile.global_address.shared::cta.b1024.b64 [%0], %1;"
                      ::"r"(own), "l"(start)
                      : "memory");
@@ -68,6 +65,11 @@ k_group_maps(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
         "tensormap.cp_fenceproxy.global.shared::cta.tensormap::generic.release.gpu.sync.aligned"
         " [%0], [%1], 128;" ::"l"(p.maps + at), "r"(own)
         : "memory");
+}
+__global__ void __launch_bounds__(32 * kMapWarps)
+k_group_maps(const __grid_constant__ MapParams p) {
+    follow_on();
+    write_map(p, blockIdx.x * kMapWarps + (threadIdx.x >> 5));
 }
 
 // Number of lines of `high` rows that the groups before g fill (0), and up to g (1) or all (2).
@@ -110,10 +112,19 @@ struct SumParams {
     float* sums;             // [ranges][groups][line]
 };
 
+// The last slice of the sums' grids writes the groups' maps, which saves a launch.
+__device__ __forceinline__ bool maps_here(const MapParams& maps, int ranges) {
+    if ((int)blockIdx.z < ranges) return false;
+    write_map(maps, (blockIdx.y * gridDim.x + blockIdx.x) * kMapWarps + (threadIdx.x >> 5));
+    return true;
+}
+
 // sums of the columns of a range of a group's rows: 64 columns a block, four rows at a time
 template <typename T>
-__global__ void __launch_bounds__(256) k_group_columns(const SumParams p) {
+__global__ void __launch_bounds__(256)
+k_group_columns(const SumParams p, const __grid_constant__ MapParams maps) {
     follow_on();
+    if (maps_here(maps, p.ranges)) return;
     __shared__ float joined[4][64];
     const int c = threadIdx.x & 63, turn = threadIdx.x >> 6;
     const int64_t col = (int64_t)blockIdx.x * 64 + c;
@@ -137,8 +148,10 @@ __global__ void __launch_bounds__(256) k_group_columns(const SumParams p) {
 
 // the same of the parts that each group's lines of tiles left
 template <typename T>
-__global__ void __launch_bounds__(256) k_group_sums(const SumParams p) {
+__global__ void __launch_bounds__(256)
+k_group_sums(const SumParams p, const __grid_constant__ MapParams maps) {
     follow_on();
+    if (maps_here(maps, p.ranges)) return;
     __shared__ float joined[4][64];
     const int c = threadIdx.x & 63, turn = threadIdx.x >> 6;
     const int64_t col = (int64_t)blockIdx.x * 64 + c;
@@ -160,24 +173,25 @@ __global__ void __launch_bounds__(256) k_group_sums(const SumParams p) {
     else p.sums[((int64_t)range * p.groups + g) * p.line + col] = sum;
 }
 
-// dbias from the sums of the ranges, in order
+// value i of dbias from the sums of the ranges, in order
+template <typename T>
+__device__ __forceinline__ void join_sums(const SumParams& p, int64_t i) {
+    if (i >= p.groups * p.n) return;
+    const int64_t g = i / p.n, col = i - g * p.n;
+    float s = 0.0f;
+#pragma unroll 8
+    for (int r = 0; r < p.ranges; ++r) s += p.sums[((int64_t)r * p.groups + g) * p.line + col];
+    static_cast<T*>(p.out)[i] = from_float<T>(s);
+}
 template <typename T>
 __global__ void __launch_bounds__(256) k_join_sums(const SumParams p) {
     follow_on();
-    const int64_t total = p.groups * p.n;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
-         i += (int64_t)gridDim.x * 256) {
-        const int64_t g = i / p.n, col = i - g * p.n;
-        float s = 0.0f;
-#pragma unroll 8
-        for (int r = 0; r < p.ranges; ++r)
-            s += p.sums[((int64_t)r * p.groups + g) * p.line + col];
-        static_cast<T*>(p.out)[i] = from_float<T>(s);
-    }
+    join_sums<T>(p, (int64_t)blockIdx.x * 256 + threadIdx.x);
 }
 
 // dW from the parts of its tiles (kDepthRanges), added in the order of k: a block has 1024 / `lanes`
-// values of a tile, four a thread; `lanes` threads share the parts and join their sums in order.
+// values of a tile, four a thread; `lanes` threads share the parts and join their sums in order. The
+// blocks behind the tiles' finish dbias.
 struct JoinParams {
     const int32_t* offsets;
     int64_t rows, m, n;
@@ -188,10 +202,16 @@ struct JoinParams {
 };
 constexpr int kJoinThreads = 256;
 template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) k_join_parts(const JoinParams p) {
+__global__ void __launch_bounds__(kJoinThreads)
+k_join_parts(const JoinParams p, const SumParams sum) {
     follow_on();
     __shared__ float4 joined[kJoinThreads];
     const int tiles = p.tiles_m * p.tiles_n, g = blockIdx.x / tiles, at = blockIdx.x - g * tiles;
+    if (g >= p.groups) {
+        const int64_t block = (int64_t)at * gridDim.y + blockIdx.y;
+        join_sums<T>(sum, block * kJoinThreads + threadIdx.x);
+        return;
+    }
     const LineCount lines = count_lines(p.offsets, p.rows, p.groups, g, 64);
     // the ranges in which the group's first and last k-blocks lie
     int r0 = 0, r1 = -1;
@@ -388,6 +408,7 @@ int run_rows(int mode, const RowProduct& g, const TileParams& p, bool launch_it,
             case kForward: return run_rows<kForward, T>(g, p, launch_it, stream);
             case kGated: return run_rows<kGated, T>(g, p, launch_it, stream);
             case kGrad: return run_rows<kGrad, T>(g, p, launch_it, stream);
+            case kPlain: return run_rows<kPlain, T>(g, p, launch_it, stream);
             default: return run_rows<kGatedGrad, T>(g, p, launch_it, stream);
         }
     };
@@ -411,72 +432,84 @@ void forward(const rune_grouped_linear_args& a, Scratch& ws, cudaStream_t stream
     p.zero_tail = 1;
     p.bias = a.bias;
     p.vec_bias = aligned(a.bias, 16) && a.outputs % 8 == 0;
-    run_rows(a.gated ? kGated : kForward, g, p, true, stream);
+    const bool plain = a.activation == RUNE_ACT_NONE && !a.bias;
+    run_rows(a.gated ? kGated : plain ? kPlain : kForward, g, p, true, stream);
 }
 
-template <typename T>
-void run_depth(const rune_grouped_linear_grad_args& a, const Matrix& dz, const Matrix& x,
-               Scratch& ws, cudaStream_t stream) {
+// The groups' products dW = dz^T x: its plan and scratch, and the maps that it wants.
+struct Depth {
+    Plan plan{};
+    uint32_t fixed = 0;
+    int high = 0, tiles_m = 0, tiles_n = 0;
+    float* parts = nullptr;
+    MapParams maps{};
+};
+
+Depth plan_weights(const rune_grouped_linear_grad_args& a, const Matrix& dz, const Matrix& x,
+                   Scratch& ws) {
+    Depth d;
     const int64_t m = dz.cols, n = x.cols;
+    d.fixed = std::max(kFixedSmem<kPlain>, kFixedSmem<kPartial>) + table_bytes(a.groups);
+    d.plan = plan_depth(a.rows, a.groups, m, n, sm_count(a.device), d.fixed);
+    d.high = d.plan.pair ? 2 * kBM : kBM;
+    d.tiles_m = (int)((m + d.high - 1) / d.high);
+    d.tiles_n = (int)((n + d.plan.bn - 1) / d.plan.bn);
+    d.maps.maps = ws.take<CUtensorMap>(2 * a.groups);
+    if (d.plan.splits > 1)
+        d.parts = ws.take<float>((a.groups + d.plan.splits) * d.tiles_m * d.tiles_n * d.high *
+                                 d.plan.bn);
+    if (ws.sizing()) return d;
+    d.maps.a = make_map(dz, 2, 64), d.maps.b = make_map(x, 2, 64);
+    d.maps.offsets = a.offsets, d.maps.rows = a.rows, d.maps.groups = (int)a.groups;
+    d.maps.start_a = static_cast<const char*>(dz.p), d.maps.line_a = dz.ld * 2;
+    d.maps.start_b = static_cast<const char*>(x.p), d.maps.line_b = x.ld * 2;
+    return d;
+}
+
+// sum: of dbias, whose ranges this call's last kernel joins; true if it did
+template <typename T>
+bool run_weights(const rune_grouped_linear_grad_args& a, const Matrix& dz, const Matrix& x,
+                 const Depth& d, const SumParams& sum, cudaStream_t stream) {
+    const int64_t m = dz.cols, n = x.cols, each = (int64_t)d.tiles_m * d.tiles_n;
     const int sms = sm_count(a.device);
-    const uint32_t fixed =
-        std::max(kFixedSmem<kForward>, kFixedSmem<kPartial>) + table_bytes(a.groups);
-    const Plan plan = plan_depth(a.rows, a.groups, m, n, sms, fixed);
-    const int high = plan.pair ? 2 * kBM : kBM;
-    const int tiles_m = (int)((m + high - 1) / high), tiles_n = (int)((n + plan.bn - 1) / plan.bn);
-    const int64_t tiles = (int64_t)tiles_m * tiles_n * a.groups;
-    auto* maps = ws.take<CUtensorMap>(2 * a.groups);
-    float* parts =
-        plan.splits > 1
-            ? ws.take<float>((a.groups + plan.splits) * tiles_m * tiles_n * high * plan.bn)
-            : nullptr;
-    if (ws.sizing()) return;
-    const CUtensorMap ma = make_map(dz, 2, 64), mb = make_map(x, 2, 64);
-    const MapParams mp{a.offsets,
-                       a.rows,
-                       (int)a.groups,
-                       static_cast<const char*>(dz.p),
-                       static_cast<const char*>(x.p),
-                       dz.ld * 2,
-                       x.ld * 2,
-                       maps};
-    launch(k_group_maps, (unsigned)((2 * a.groups + kMapWarps - 1) / kMapWarps), 32 * kMapWarps, 0,
-           0, stream, ma, mb, mp);
+    const CUtensorMap &ma = d.maps.a, &mb = d.maps.b;
     TileParams p{};
     p.m = m, p.n = n;
     p.act = RUNE_ACT_NONE;
     p.m_all = a.rows, p.groups = (int)a.groups, p.offsets = a.offsets;
-    p.group_maps = maps;
-    p.bn = plan.bn, p.stages = plan.stages, p.splits = 1;
-    p.tiles_m = tiles_m, p.tiles_n = tiles_n;
-    p.by_tiles = make_divisor((unsigned)tiles_m * tiles_n);
-    p.by_group = make_divisor(kGroup * (unsigned)tiles_n);
-    p.by_last = make_divisor(std::max(1u, (unsigned)tiles_m % kGroup));
+    p.group_maps = d.maps.maps;
+    p.bn = d.plan.bn, p.stages = d.plan.stages, p.splits = 1;
+    p.tiles_m = d.tiles_m, p.tiles_n = d.tiles_n;
+    p.by_tiles = make_divisor((unsigned)each);
+    p.by_group = make_divisor(kGroup * (unsigned)d.tiles_n);
+    p.by_last = make_divisor(std::max(1u, (unsigned)d.tiles_m % kGroup));
     p.a_mn = p.b_mn = 1;
-    p.idesc = operand_idesc(a.dtype == RUNE_BF16 ? 1 : 0, true, true, high, p.bn);
+    p.idesc = operand_idesc(a.dtype == RUNE_BF16 ? 1 : 0, true, true, d.high, p.bn);
     p.flag = wait_flag(a.device);
     p.polls = wait_polls();
-    if (plan.splits == 1) {
+    if (d.plan.splits == 1) {
         p.out = a.dweight, p.ld_out = n, p.out_step = m * n;
         p.tma_out = wide16(a.dweight, n, n);
         const CUtensorMap o =
             p.tma_out ? make_out_map3(a.dweight, m, n, n, a.groups, m * n) : ma;
-        launch_kind<kForward, kDepthGroups, T>(plan.pair, ma, mb, o, o, p, tiles, fixed, sms,
-                                               a.device, stream);
-        return;
+        launch_kind<kPlain, kDepthGroups, T>(d.plan.pair, ma, mb, o, o, p, each * a.groups, d.fixed,
+                                             sms, a.device, stream);
+        return false;
     }
-    p.ranges = plan.splits;
-    p.z = parts, p.ld_part = high;
-    launch_kind<kPartial, kDepthRanges, __half>(plan.pair, ma, mb, ma, ma, p,
-                                                (int64_t)plan.splits * tiles_m * tiles_n, fixed,
-                                                sms, a.device, stream);
+    p.ranges = d.plan.splits;
+    p.z = d.parts, p.ld_part = d.high;
+    launch_kind<kPartial, kDepthRanges, __half>(d.plan.pair, ma, mb, ma, ma, p, p.ranges * each,
+                                                d.fixed, sms, a.device, stream);
     // sixteen threads share the parts of a tile where these are many
-    const int lanes = plan.splits >= 16 * a.groups ? 16 : 1;
-    const JoinParams j{a.offsets, a.rows, m, n, (int)a.groups, tiles_m, tiles_n, high, plan.bn,
-                       plan.splits, lanes, n % 4 == 0 && aligned(a.dweight, 8), parts, a.dweight};
-    launch(k_join_parts<T>,
-           dim3((unsigned)tiles, (unsigned)(high * plan.bn / 4 * lanes / kJoinThreads)),
-           kJoinThreads, 0, 0, stream, j);
+    const int lanes = p.ranges >= 16 * a.groups ? 16 : 1;
+    const JoinParams j{a.offsets, a.rows, m, n, (int)a.groups, d.tiles_m, d.tiles_n, d.high, p.bn,
+                       p.ranges, lanes, n % 4 == 0 && aligned(a.dweight, 8), d.parts, a.dweight};
+    const int64_t rows_y = d.high * p.bn / 4 * lanes / kJoinThreads;
+    const int64_t more = sum.ranges > 1 ? (a.groups * sum.n + rows_y * kJoinThreads - 1) /
+                                              (rows_y * kJoinThreads) : 0;
+    launch(k_join_parts<T>, dim3((unsigned)(each * a.groups + more), (unsigned)rows_y),
+           kJoinThreads, 0, 0, stream, j, sum);
+    return true;
 }
 
 void backward(const rune_grouped_linear_grad_args& a, Scratch& ws, cudaStream_t stream) {
@@ -493,16 +526,14 @@ void backward(const rune_grouped_linear_grad_args& a, Scratch& ws, cudaStream_t 
     Matrix dz{a.dy, a.rows, n_all, a.dy_stride};
     SumParams sum{a.offsets, a.rows, n_all, (int)a.groups, 0, 0, a.dy_stride, a.dy, nullptr,
                   a.dbias, 1, 0, nullptr};
+    TileParams p{};
+    const int mode = a.gated ? kGatedGrad : kGrad;
     if (plain) {
         if (a.dx || a.dweight) dz = readable(dz, 2, ws, stream);
-        sum.high = sum.each = 1;  // a row is a part
     } else {
         dz.ld = pad16(n_all, 2);
         dz.p = ws.take<uint16_t>(a.rows * dz.ld);
         g.a = x, g.w = w, g.k = a.inputs;
-    }
-    TileParams p{};
-    if (!plain) {
         p.n = a.outputs;
         p.act = a.activation;
         p.out = const_cast<void*>(dz.p), p.ld_out = dz.ld;
@@ -511,60 +542,55 @@ void backward(const rune_grouped_linear_grad_args& a, Scratch& ws, cudaStream_t 
         p.vec_in = wide16(a.dy, a.dy_stride, a.outputs);
         p.bias = a.bias;
         p.vec_bias = aligned(a.bias, 16) && a.outputs % 8 == 0;
-        sum.high = run_rows(a.gated ? kGatedGrad : kGrad, g, p, false, stream);
+        sum.high = run_rows(mode, g, p, false, stream);
         sum.each = sum.high / 32;  // one a warp
     }
     if (a.dbias) {
         const int64_t parts = plain ? a.rows : line_bound(a.rows, a.groups, sum.high) * sum.each;
         if (!plain) sum.parts = ws.take<float>(parts * n_all);
-        // 64 parts a range where groups are alike; more ranges than one cost a launch
+        // 64 parts a range where groups are alike
         const int64_t mean = parts / a.groups;
         sum.ranges = mean < 256 ? 1 : (int)std::min<int64_t>(256, mean / 64);
         sum.line = (n_all + 3) / 4 * 4;
         if (sum.ranges > 1) sum.sums = ws.take<float>(sum.ranges * a.groups * sum.line);
     }
-    const int sms = sm_count(a.device);
-    if (!ws.sizing()) {
-        if (!plain) {
-            p.colsum = sum.parts;
-            run_rows(a.gated ? kGatedGrad : kGrad, g, p, true, stream);
-        }
+    Depth depth;
+    if (a.dweight) depth = plan_weights(a, dz, x, ws);
+    if (ws.sizing()) return;
+    if (!plain) {
+        p.colsum = sum.parts;
+        run_rows(mode, g, p, true, stream);
+    }
+    auto typed = [&](auto t) {
+        using T = decltype(t);
         if (a.dbias) {
             const dim3 grid((unsigned)((n_all + 63) / 64), (unsigned)a.groups,
-                            (unsigned)sum.ranges);
-            auto go = [&](auto t) {
-                using T = decltype(t);
-                if (plain) launch(k_group_columns<T>, grid, 256, 0, 0, stream, sum);
-                else launch(k_group_sums<T>, grid, 256, 0, 0, stream, sum);
-                if (sum.ranges > 1) {
-                    const int64_t blocks = (a.groups * n_all + 255) / 256;
-                    launch(k_join_sums<T>, (unsigned)std::min<int64_t>(blocks, 16 * sms), 256, 0, 0,
-                           stream, sum);
-                }
-            };
-            if (half) go(__half());
-            else go(__nv_bfloat16());
+                            (unsigned)(sum.ranges + (a.dweight ? 1 : 0)));
+            if (plain) launch(k_group_columns<T>, grid, 256, 0, 0, stream, sum, depth.maps);
+            else launch(k_group_sums<T>, grid, 256, 0, 0, stream, sum, depth.maps);
+        } else if (a.dweight) {
+            launch(k_group_maps, (unsigned)((2 * a.groups + kMapWarps - 1) / kMapWarps),
+                   32 * kMapWarps, 0, 0, stream, depth.maps);
         }
-        RUNE_LAUNCH_CHECK();
-    } else if (!plain) {
-        dz.p = reinterpret_cast<const void*>(256);
-    }
-    if (a.dx && !ws.sizing()) {
-        RowProduct d = g;
-        d.a = dz, d.w = w, d.w_mn = true;
-        d.k = n_all;
-        TileParams q{};
-        q.n = a.inputs;
-        q.act = RUNE_ACT_NONE;
-        q.out = a.dx, q.ld_out = a.inputs;
-        q.tma_out = wide16(a.dx, a.inputs, a.inputs);
-        q.zero_tail = 1;
-        run_rows(kForward, d, q, true, stream);
-    }
-    if (a.dweight) {
-        if (half) run_depth<__half>(a, dz, x, ws, stream);
-        else run_depth<__nv_bfloat16>(a, dz, x, ws, stream);
-    }
+        if (a.dx) {
+            RowProduct d = g;
+            d.a = dz, d.w = w, d.w_mn = true;
+            d.k = n_all;
+            TileParams q{};
+            q.n = a.inputs;
+            q.act = RUNE_ACT_NONE;
+            q.out = a.dx, q.ld_out = a.inputs;
+            q.tma_out = wide16(a.dx, a.inputs, a.inputs);
+            q.zero_tail = 1;
+            run_rows(kPlain, d, q, true, stream);
+        }
+        const bool joined = a.dweight && run_weights<T>(a, dz, x, depth, sum, stream);
+        if (sum.ranges > 1 && !joined)
+            launch(k_join_sums<T>, (unsigned)((a.groups * n_all + 255) / 256), 256, 0, 0, stream,
+                   sum);
+    };
+    if (half) typed(__half());
+    else typed(__nv_bfloat16());
 }
 
 template <typename Args>

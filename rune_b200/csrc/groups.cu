@@ -357,9 +357,9 @@ struct MoveParams {
 };
 
 // A team of lanes moves R rows at a time, C pieces of each a lane, so that enough is under way while
-// the rows' indexes, and then their pieces, arrive: narrow rows four at a time, wide ones in parts of
+// the rows' indexes, and then their pieces, arrive: narrow rows two at a time, wide ones in parts of
 // four pieces a lane, the parts of a row along the grid's y. B200, 110592 x 256 bf16 to two groups
-// each and back, us: to 32 -> 27, from 37 -> 30, from's gradient 101 -> 54 against one row a team.
+// each and back with gradients: one row a team 223 us, two 176, four (fewer threads an SM) 204.
 constexpr int kMoveThreads = 256;
 template <int R_, int C_>
 struct Shape {
@@ -418,12 +418,12 @@ __global__ void __launch_bounds__(kMoveThreads) k_to_groups(const MoveParams p) 
     }
 }
 
-template <typename T, int N, int R, int C>
+// kAhead: choices whose pieces are under way at once
+template <typename T, int N, int R, int C, int kAhead>
 __global__ void __launch_bounds__(kMoveThreads) k_from_groups(const MoveParams p) {
     follow_on();
     const Team t(p.lanes);
     const int col0 = ((int)blockIdx.y * C * p.lanes + t.at) * N, step = p.lanes * N;
-    constexpr int kAhead = 2;  // choices whose pieces are under way at once
     for (int64_t r0 = (int64_t)blockIdx.x * t.count * R + t.index; r0 < p.rows;
          r0 += (int64_t)gridDim.x * t.count * R) {
         float sum[R][C][N] = {};
@@ -602,7 +602,7 @@ void with_shape(MoveParams& p, int64_t rows, int pieces, bool parts, int device,
         const int64_t most = std::max<int64_t>(1, (int64_t)sm_count(device) * 32 / y);
         fn(shape, dim3((unsigned)std::min<int64_t>((rows + teams - 1) / teams, most), y));
     };
-    if (pieces <= 32) go(Shape<4, 1>());
+    if (pieces <= 32) go(Shape<2, 1>());
     else if (pieces <= 64) go(Shape<2, 2>());
     else go(Shape<1, 4>());
 }
@@ -835,6 +835,7 @@ int rune_from_groups(const rune_group_move_args* args, void* stream_) {
         if (a.rows == 0) return;
         require(a.in && a.place && a.out, "null argument");
         MoveParams p = move_params(a);
+        if (a.k == 1) p.order = p.place;
         const int n = piece_values(
             dtype_bytes(a.dtype), a.width,
             {{a.in, a.rows * a.k > 1 ? a.in_stride : a.width}, {a.out, a.width}});
@@ -843,7 +844,12 @@ int rune_from_groups(const rune_group_move_args* args, void* stream_) {
             constexpr int N = decltype(n_c)::value;
             with_shape(p, p.rows, (int)(a.width / N), true, a.device, [&](auto shape, dim3 grid) {
                 constexpr int R = decltype(shape)::R, C = decltype(shape)::C;
-                launch(k_from_groups<T, N, R, C>, grid, kMoveThreads, 0, 0, stream, p);
+                if (p.k > 1)
+                    launch(k_from_groups<T, N, R, C, 2>, grid, kMoveThreads, 0, 0, stream, p);
+                else if (p.weights)
+                    launch(k_from_groups<T, N, R, C, 1>, grid, kMoveThreads, 0, 0, stream, p);
+                else  // one choice: the rows in another order, and no sum
+                    launch(k_to_groups<T, N, R, C, false>, grid, kMoveThreads, 0, 0, stream, p);
             });
         });
         RUNE_LAUNCH_CHECK();

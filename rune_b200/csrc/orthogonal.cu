@@ -13,6 +13,12 @@
 // numbers (2^-24 after scaling) and of its largest (64). bfloat16 would need no scale, but every
 // step rounds X, A and B, and 8 bits instead of 11 cost eight times the error of the result.
 // The norm is summed in float64, products in float32.
+//
+// Small matrices spend a product's time between launches (5.5 us each for 256 x 512), so k_small
+// takes one matrix through all steps in a cluster of eight blocks, which meet between products:
+// 8 x 256 x 512, five steps, 95 us as a chain of launches, @@ us so.
+
+#include <cmath>
 
 #include "tile.cuh"
 
@@ -82,6 +88,292 @@ __global__ void __launch_bounds__(kNormThreads) k_scale(const NormParams p) {
             else
                 p.out[z * p.out_step + r * p.ld + c] = __float2half_rn((float)(v * kScale));
         }
+}
+
+// ----------------------------------------------------------------------------- small matrices
+// All steps of one matrix in a cluster of kCluster blocks. Each product's tiles of 128 x bn go round
+// the blocks; X, A and B stay in scratch, that is in L2. Every block runs every cluster barrier
+// whatever failed in it, so none waits for another that has left.
+constexpr int kCluster = 8, kSmallEpi = 8, kSmallTma = 8, kSmallMma = 9;
+constexpr int kSmallThreads = 32 * 10, kSmallStages = 5;
+constexpr uint32_t kBox = 64 * kLineBytes;                     // 64 lines
+constexpr uint32_t kSmallStage = 4 * kBox;                     // 128 x 64 of A, up to 128 x 64 of B
+constexpr uint32_t kSmallBufs = kSmallEpi * 2 * kWarpBuf;
+
+struct SmallProduct {
+    int m, n, kblocks, bn, tiles;
+    int symmetric;
+};
+struct SmallParams {
+    CUtensorMap x[2], g, h;                     // boxes of 64 x 64: operands in either order
+    CUtensorMap x_out[2], g_out, h_out, y_out;  // boxes of 32 x 32
+    SmallProduct gram, poly, next;
+    const __half* in_x[2];
+    const __half* in_g;
+    int64_t ld_x, step_x, ld_g, step_g;
+    __nv_bfloat16* y;
+    int rows, cols, steps, tall, tma_y;
+    float a, b, c;
+    unsigned* flag;
+    unsigned polls;
+};
+struct SmallShared {
+    unsigned long long full[kSmallStages], empty[kSmallStages], acc_full[2], acc_empty[2], drained;
+    uint32_t tmem;
+    int fail, issued;
+};
+
+__device__ __forceinline__ void bulk_store_done() {
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+// between what other threads wrote and this thread's copies of it, either way
+__device__ __forceinline__ void fence_async_all() {
+    asm volatile("fence.proxy.async;" ::: "memory");
+}
+
+// tile w of a product: rows mt * 128, columns nt * bn. Symmetric ones have the tiles that begin on or
+// left of the diagonal: mt + 1 lots of 128 / bn in line mt.
+__device__ __forceinline__ void small_tile(const SmallProduct& q, int w, int& mt, int& nt) {
+    if (q.symmetric) {
+        const int each = 128 / q.bn;
+        mt = 0;
+        while (w >= (mt + 1) * each) w -= (mt + 1) * each, ++mt;
+        nt = w;
+    } else {
+        const int across = (q.n + q.bn - 1) / q.bn;
+        mt = w / across, nt = w - mt * across;
+    }
+}
+
+__global__ void __launch_bounds__(kSmallThreads, 1)
+k_small(const __grid_constant__ SmallParams p) {
+    using namespace tc;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    unsigned char* bufs = smem + kSmallStages * kSmallStage;
+    auto* sh = reinterpret_cast<SmallShared*>(bufs + kSmallBufs);
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    const int rank = (int)cluster_rank(), z = blockIdx.x / kCluster;
+    if (tid == 0) {
+        for (int i = 0; i < kSmallStages; ++i) {
+            mbar_init(smem_u32(&sh->full[i]), 1);
+            mbar_init(smem_u32(&sh->empty[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&sh->acc_full[i]), 1);
+            mbar_init(smem_u32(&sh->acc_empty[i]), kSmallEpi);
+        }
+        mbar_init(smem_u32(&sh->drained), 1);
+        sh->fail = 0;
+        sh->issued = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;");
+    }
+    if (warp == kSmallMma) tmem_alloc(&sh->tmem, 256);
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sh->tmem, 0);
+    volatile int* fail = &sh->fail;
+    follow_on();
+
+    const bool one = elect_one();
+    int st = 0, issued = 0, buf = 0;
+    uint32_t parity = warp == kSmallTma ? 1 : 0;         // of the stage's next wait
+    uint32_t acc_parity = warp == kSmallMma ? 1 : 0;     // of the accumulator's
+    const Stage s0(smem_u32(bufs) + warp * 2 * kWarpBuf, lane);
+    const Stage s1(smem_u32(bufs) + (warp * 2 + 1) * kWarpBuf, lane);
+
+    for (int phase = 0; phase < 3 * p.steps; ++phase) {
+        const int step = phase / 3, kind = phase - 3 * step;
+        const bool last = phase + 1 == 3 * p.steps;
+        const SmallProduct& q = kind == 0 ? p.gram : kind == 1 ? p.poly : p.next;
+        const int from = step & 1;
+        // gram: A and B are X; poly: A; next: B X, or X B of tall ones
+        const bool a_mn = kind == 0 && p.tall, b_mn = kind == 0 ? p.tall : kind == 2 && !p.tall;
+        if (warp == kSmallTma) {
+            const CUtensorMap* x = &p.x[from];
+            const CUtensorMap* am = kind == 0 ? x : kind == 1 ? &p.g : p.tall ? x : &p.h;
+            const CUtensorMap* bm = kind == 0 ? x : kind == 1 ? &p.g : p.tall ? &p.h : x;
+            fence_async_all();
+            bool ok = !*fail;
+            for (int w = rank; w < q.tiles && ok; w += kCluster) {
+                int mt, nt;
+                small_tile(q, w, mt, nt);
+                for (int kb = 0; kb < q.kblocks; ++kb) {
+                    ok = mbar_wait(smem_u32(&sh->empty[st]), parity, p.polls) && !*fail;
+                    if (!__all_sync(0xffffffffu, ok)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t bar = smem_u32(&sh->full[st]);
+                    const uint32_t a = smem_u32(smem) + (uint32_t)st * kSmallStage;
+                    if (one) {
+                        mbar_expect_tx(bar, (2 + q.bn / 64) * kBox);
+                        for (int i = 0; i < 2 + q.bn / 64; ++i) {
+                            const bool is_b = i >= 2;
+                            const int line = is_b ? nt * q.bn + (i - 2) * 64 : mt * 128 + i * 64;
+                            const bool mn = is_b ? b_mn : a_mn;
+                            tma_load3(a + i * kBox, is_b ? bm : am, mn ? line : kb * 64,
+                                      mn ? kb * 64 : line, z, bar);
+                        }
+                    }
+                    __syncwarp();
+                    ++issued;
+                    if (++st == kSmallStages) st = 0, parity ^= 1;
+                }
+            }
+            if (!ok && !*fail) *fail = 1;
+            if (one) sh->issued = issued;
+            __syncwarp();
+        } else if (warp == kSmallMma) {
+            const uint64_t step_a = a_mn ? 2048 >> 4 : 32 >> 4, step_b = b_mn ? 2048 >> 4 : 32 >> 4;
+            const uint64_t desc_a = operand_desc(smem_u32(smem), a_mn);
+            const uint64_t desc_b = operand_desc(smem_u32(smem) + 2 * kBox, b_mn);
+            const uint32_t idesc = operand_idesc(0, a_mn, b_mn, 128, q.bn);
+            bool ok = !*fail;
+            for (int w = rank; w < q.tiles && ok; w += kCluster) {
+                ok = mbar_wait(smem_u32(&sh->acc_empty[buf]), acc_parity, p.polls) && !*fail;
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
+                    break;
+                }
+                fence_after_sync();
+                const uint32_t acc = tmem + buf * 128;
+                for (int kb = 0; kb < q.kblocks; ++kb) {
+                    ok = mbar_wait(smem_u32(&sh->full[st]), parity, p.polls) && !*fail;
+                    if (!__all_sync(0xffffffffu, ok)) {
+                        ok = false;
+                        break;
+                    }
+                    fence_after_sync();
+                    const uint64_t at = (uint64_t)((uint32_t)st * (kSmallStage >> 4));
+                    if (one) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            mma<false, false>(acc, desc_a + at + k * step_a,
+                                              desc_b + at + k * step_b, idesc, kb > 0 || k > 0);
+                        mma_commit(smem_u32(&sh->empty[st]));
+                    }
+                    __syncwarp();
+                    if (++st == kSmallStages) st = 0, parity ^= 1;
+                }
+                if (one) mma_commit(smem_u32(&sh->acc_full[buf]));
+                __syncwarp();
+                buf ^= 1;
+                if (buf == 0) acc_parity ^= 1;
+            }
+            if (!ok && !*fail) *fail = 2;
+        } else {
+            // sums are of scaled values, 2^20 of the products'; the last result leaves without scale
+            const float unit = last ? 1.0f / kScale : 1.0f;
+            const float alpha = kind == 0 ? 1.0f / kScale : kind == 1 ? p.c / kScale : unit / kScale;
+            const float beta = kind == 1 ? p.b : p.a * unit;
+            const CUtensorMap* out = kind == 0 ? &p.g_out : kind == 1 ? &p.h_out
+                                     : last   ? &p.y_out : &p.x_out[from ^ 1];
+            const __half* in = kind == 0 ? nullptr
+                               : kind == 1 ? p.in_g + z * p.step_g : p.in_x[from] + z * p.step_x;
+            const int64_t ld = kind == 1 ? p.ld_g : p.ld_x;
+            const bool tma = !last || p.tma_y;
+            const int quarter = warp & 3, share = warp >> 2;
+            bool ok = !*fail;
+            for (int w = rank; w < q.tiles && ok; w += kCluster) {
+                int mt, nt;
+                small_tile(q, w, mt, nt);
+                const int row0 = mt * 128 + quarter * 32, rows = max(0, min(32, q.m - row0));
+                const uint32_t acc = tmem + buf * 128 + ((uint32_t)(quarter * 32) << 16);
+                const bool mirror = q.symmetric && nt * q.bn + q.bn <= mt * 128;
+                for (int c = share * 32; c < q.bn; c += 64) {
+                    const int col = nt * q.bn + c;
+                    if (lane == 0) bulk_store_read();
+                    __syncwarp();
+                    if (in) {
+                        // past L1, which may hold these lines as they were a step before
+                        const int r0 = lane >> 2, cc = (lane & 3) * 8;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            uint4 v = make_uint4(0, 0, 0, 0);
+                            if (r0 + 8 * i < rows && col + cc < q.n)
+                                v = __ldcg(reinterpret_cast<const uint4*>(
+                                    in + (int64_t)(row0 + r0 + 8 * i) * ld + col + cc));
+                            put16(s0.turn(i), v);
+                        }
+                        __syncwarp();
+                    }
+                    if (c == share * 32) {
+                        ok = mbar_wait(smem_u32(&sh->acc_full[buf]), acc_parity, p.polls) && !*fail;
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        fence_after_sync();
+                    }
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        float v[16];
+                        Two t[8], u[8];
+                        tmem_ld16(acc + c + half * 16, v);
+                        if (in) get_row<__half>(s0, half, u);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            t[j] = two(v[2 * j], v[2 * j + 1]) * two(alpha);
+                            if (in) t[j] = fma(u[j], two(beta), t[j]);
+                        }
+                        if (mirror) put_column<__half>(s1, half, t);
+                        if (last) put_row<__nv_bfloat16>(s0, half, t);
+                        else put_row<__half>(s0, half, t);
+                    }
+                    if (tma) fence_async_smem();
+                    __syncwarp();
+                    if (tma) {
+                        if (lane == 0 && rows > 0 && col < q.n) {
+                            bulk_store3(out, s0.base, col, row0, z);
+                            if (mirror) bulk_store3(out, s1.base, row0, col, z);
+                            bulk_store_commit();
+                        }
+                    } else {
+                        store_rows<__nv_bfloat16>(
+                            s0, p.y + ((int64_t)z * p.rows + row0) * p.cols + col, p.cols, rows,
+                            q.n - col);
+                    }
+                    __syncwarp();
+                }
+                if (!ok) break;
+                fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sh->acc_empty[buf]));
+                __syncwarp();
+                buf ^= 1;
+                if (buf == 0) acc_parity ^= 1;
+            }
+            if (!ok && !*fail) *fail = 4;
+            if (lane == 0) {  // the results are in L2
+                bulk_store_done();
+                fence_async_all();
+            }
+        }
+        __syncwarp();
+        cluster_sync();
+    }
+    // what is in flight after a wait that gave up lands before the block's memory goes
+    __syncthreads();
+    if (*fail) {
+        if (tid == 0) {
+            atomicExch_system(p.flag, (unsigned)*fail);
+            for (int i = max(0, sh->issued - kSmallStages); i < sh->issued; ++i)
+                mbar_wait(smem_u32(&sh->full[i % kSmallStages]), (i / kSmallStages) & 1);
+        }
+        __syncwarp();
+        if (warp == kSmallMma) {
+            if (one) mma_commit(smem_u32(&sh->drained));
+            __syncwarp();
+            mbar_wait(smem_u32(&sh->drained), 0);
+        }
+        __syncwarp();
+    }
+    fence_before_sync();
+    __syncthreads();
+    if (warp == kSmallMma) {
+        fence_after_sync();
+        tmem_dealloc(tmem, 256);
+    }
 }
 
 // A stack of matrices in scratch or of results.
@@ -166,6 +458,87 @@ void run_step(const Step& s, cudaStream_t stream) {
                                                         stream);
 }
 
+// The products of a matrix of rows x cols in tiles of 128 x 64 or 128 x 128, whichever takes the
+// blocks of a cluster less time, and the cycles that a step takes.
+struct SmallPlan {
+    SmallProduct gram, poly, next;
+    double cycles;
+};
+SmallPlan plan_small(int64_t rows, int64_t cols) {
+    SmallPlan plan{};
+    const int64_t small = std::min(rows, cols), large = std::max(rows, cols);
+    auto product = [&](int64_t m, int64_t n, int64_t k, bool symmetric) {
+        SmallProduct best{};
+        double best_cost = 0.0;
+        for (int bn : {128, 64}) {
+            const int64_t tm = (m + 127) / 128, tn = (n + bn - 1) / bn;
+            const int64_t tiles = symmetric ? tm * (tm + 1) / 2 * (128 / bn) : tm * tn;
+            const int kblocks = (int)((k + 63) / 64);
+            const double main = kblocks * block_cycles(false, bn), epi = 600.0 + 16.0 * bn;
+            const double turns = (double)((tiles + kCluster - 1) / kCluster);
+            const double cost = 3000.0 + turns * std::max(main, epi) + std::min(main, epi);
+            if (best.bn == 0 || cost < best_cost) {
+                best_cost = cost;
+                best = {(int)m, (int)n, kblocks, bn, (int)tiles, symmetric};
+            }
+        }
+        plan.cycles += best_cost;
+        return best;
+    };
+    plan.gram = product(small, small, large, true);
+    plan.poly = product(small, small, small, true);
+    plan.next = product(rows, cols, small, false);
+    return plan;
+}
+
+void run_small(const rune_orthogonalize_args& a, const SmallPlan& plan, const Stack (&x)[2],
+               const Stack& g, const Stack& h, cudaStream_t stream) {
+    SmallParams p{};
+    const Stack y{a.y, a.rows, a.cols, a.cols, a.rows * a.cols};
+    auto out = [&](const Stack& t) {
+        return make_out_map3(t.p, t.rows, t.cols, t.ld, a.count, t.step);
+    };
+    for (int i = 0; i < 2; ++i) {
+        const Stack& t = a.steps > 1 ? x[i] : x[0];
+        p.x[i] = t.map(a.count, 64), p.x_out[i] = out(t);
+        p.in_x[i] = static_cast<const __half*>(t.p);
+    }
+    p.g = g.map(a.count, 64), p.g_out = out(g);
+    p.h = h.map(a.count, 64), p.h_out = out(h);
+    p.tma_y = wide16(a.y, a.cols, a.cols);
+    p.y_out = p.tma_y ? out(y) : p.g_out;
+    p.gram = plan.gram, p.poly = plan.poly, p.next = plan.next;
+    p.in_g = static_cast<const __half*>(g.p);
+    p.ld_x = x[0].ld, p.step_x = x[0].step, p.ld_g = g.ld, p.step_g = g.step;
+    p.y = static_cast<__nv_bfloat16*>(a.y);
+    p.rows = (int)a.rows, p.cols = (int)a.cols;
+    p.steps = a.steps, p.tall = a.rows > a.cols;
+    p.a = a.a, p.b = a.b, p.c = a.c;
+    p.flag = wait_flag(a.device);
+    p.polls = wait_polls();
+    const size_t smem = kSmallStages * kSmallStage + kSmallBufs + sizeof(SmallShared);
+    static std::atomic<uint64_t> allowed{0};  // devices whose limit is raised
+    if (a.device >= 64 || !(allowed.load(std::memory_order_relaxed) >> a.device & 1)) {
+        RUNE_CUDA_TRY(cudaFuncSetAttribute(k_small, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           (int)smem));
+        if (a.device < 64) allowed.fetch_or(uint64_t(1) << a.device, std::memory_order_relaxed);
+    }
+    launch(k_small, (unsigned)(a.count * kCluster), kSmallThreads, smem, kCluster, stream, p);
+}
+
+// Whether the clusters take less time than a chain of launches, of 10000 cycles a product at least
+// and then at the tensor cores' rate of all SMs.
+bool use_small(const rune_orthogonalize_args& a, const SmallPlan& plan) {
+    const int64_t small = std::min(a.rows, a.cols), large = std::max(a.rows, a.cols);
+    if (a.steps == 0 || large > (1 << 20) || a.count > (1 << 16)) return false;
+    const int sms = sm_count(a.device);
+    // clusters at once: blocks of one lie in one group of SMs, so not all SMs find a place
+    const double waves = std::ceil((double)a.count * kCluster / (sms * 0.85));
+    const double kb = (double)a.count * ((small + 127) / 128) * ((large + 63) / 64) / sms;
+    const double chain = 3.0 * std::max(10000.0, 3000.0 + kb * ((small + 127) / 128) * 350.0);
+    return waves * plan.cycles < chain;
+}
+
 int norm_blocks(const rune_orthogonalize_args& a) {
     const int64_t most = std::max<int64_t>(1, (int64_t)sm_count(a.device) * 8 / a.count);
     return (int)std::min<int64_t>(a.rows, most);
@@ -194,6 +567,7 @@ void orthogonalize(const rune_orthogonalize_args& a, Scratch& ws, cudaStream_t s
     n.out = static_cast<__half*>(x[0].p);
     n.final = a.steps == 0 ? static_cast<__nv_bfloat16*>(a.y) : nullptr;
     const dim3 grid((unsigned)n.blocks, (unsigned)a.count);
+    const SmallPlan plan = plan_small(a.rows, a.cols);
     auto prepare = [&](auto t) {
         using T = decltype(t);
         launch(k_squares<T>, grid, kNormThreads, 0, 0, stream, n);
@@ -202,6 +576,10 @@ void orthogonalize(const rune_orthogonalize_args& a, Scratch& ws, cudaStream_t s
     if (a.dtype == RUNE_F16) prepare(__half());
     else if (a.dtype == RUNE_BF16) prepare(__nv_bfloat16());
     else prepare(float());
+    if (use_small(a, plan)) {
+        run_small(a, plan, x, g, h, stream);
+        return;
+    }
     for (int i = 0; i < a.steps; ++i) {
         const Stack from = x[i & 1];
         const bool last = i + 1 == a.steps;

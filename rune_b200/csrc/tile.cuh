@@ -19,6 +19,7 @@ enum Mode {
     kGated,      // y = act(gate) * up; the tile's columns are half gate, half up
     kGrad,       // dz = dy act'(acc + bias), column sums of dz
     kGatedGrad,  // d gate = dy up act'(gate), d up = dy act(gate), column sums
+    kPlain,      // y = acc: weight gradients and dx, whose epilogue bounds short contractions
     kPartial,    // float32 sums of one range of k
     kUpdate      // alpha acc + beta in; of a symmetric product the tiles below the diagonal, twice
 };
@@ -595,6 +596,41 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
         release();
         return;
     }
+    if constexpr (MODE == kPlain) {
+        // 32 columns at a time, in a fifth of the instructions that kForward takes for nothing
+        for (int c = share * 32; c < end; c += 128) {
+            float v[32];
+            tc::tmem_ld32(acc + c, v);
+            if (c + 128 >= end) release();
+            if (KIND == kDepthGroups && t.empty) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+            }
+            reuse();
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                put16(st.own(q), make_uint4(pack2<T>(v[8 * q], v[8 * q + 1]),
+                                            pack2<T>(v[8 * q + 2], v[8 * q + 3]),
+                                            pack2<T>(v[8 * q + 4], v[8 * q + 5]),
+                                            pack2<T>(v[8 * q + 6], v[8 * q + 7])));
+            const bool tma = p.tma_out && (KIND != kRowGroups || rows == 32);
+            if (tma) tc::fence_async_smem();
+            __syncwarp();
+            const int64_t col = col0 + c;
+            if (!tma) {
+                T* out = static_cast<T*>(p.out) + (int64_t)row0 * p.ld_out + col;
+                if constexpr (KIND == kDepthGroups) out += t.z * p.out_step;
+                store_part<T>(st.base, out, p.ld_out, rows, (int)(p.n - col), p.tma_out);
+            } else if (lane == 0 && rows > 0) {
+                if constexpr (KIND == kDepthGroups) bulk_store3(out_map, st.base, (int)col, row0, t.z);
+                else bulk_store(out_map, st.base, (int)col, row0);
+                bulk_store_commit();
+            }
+            __syncwarp();
+        }
+        if (share * 32 >= end) release();
+        return;
+    }
     float* sums = nullptr;  // this warp's row of the parts of dbias
     if (kReads && p.colsum)
         sums = p.colsum + ((int64_t)t.mt * 4 + quarter) * (kGate ? 2 * p.n : p.n);
@@ -644,10 +680,6 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
                     tc::tmem_ld16(acc + at, v);
                 }
                 if (half == 1 && c + 128 >= end) release();
-                if (KIND == kDepthGroups && t.empty) {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) v[j] = 0.0f;
-                }
                 finish_z<T, FP8>(v, z, bias, p, zcol, zleft, xs);
                 if constexpr (kGate) finish_z<T, FP8>(w, u, bias_up, p, p.n + zcol, zleft, xs);
             }
@@ -720,7 +752,7 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
         __syncwarp();
         if (tma) {
             if (lane == 0 && rows > 0) {
-                if constexpr (KIND == kDepthGroups || KIND == kBatch) {
+                if constexpr (KIND == kBatch) {
                     bulk_store3(out_map, st.base, (int)col, row0, t.z);
                     if constexpr (MODE == kUpdate) {
                         // and its mirror image, left of the diagonal's tiles
@@ -741,7 +773,7 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
                 if constexpr (MODE == kGatedGrad)
                     store_part<T>(st2.base, out + p.n, p.ld_out, rows, (int)left, p.tma_out);
             } else {
-                if constexpr (KIND == kDepthGroups || KIND == kBatch) out += t.z * p.out_step;
+                if constexpr (KIND == kBatch) out += t.z * p.out_step;
                 store_rows<T>(st, out, p.ld_out, rows, left);
                 if constexpr (MODE == kGatedGrad)
                     store_rows<T>(st2, out + p.n, p.ld_out, rows, left);
@@ -1009,7 +1041,7 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
                     __syncwarp();
                 });
         }
-        if constexpr (KIND == kRowGroups && MODE == kForward || KIND == kRowGroups && MODE == kGated) {
+        if constexpr (KIND == kRowGroups && (MODE == kForward || MODE == kGated || MODE == kPlain)) {
             // the rows that no group has
             if (p.zero_tail && ok) {
                 const int64_t from = plan.rows[p.groups], n = (p.m_all - from) * p.n;
