@@ -16,7 +16,7 @@
 //
 // Small matrices spend a product's time between launches (5.5 us each for 256 x 512), so k_small
 // takes one matrix through all steps in a cluster of eight blocks, which meet between products:
-// 8 x 256 x 512, five steps, 95 us as a chain of launches, @@ us so.
+// 8 x 256 x 512, five steps, 96 us as a chain of launches, 75 us so.
 
 #include <cmath>
 
@@ -46,17 +46,57 @@ __device__ __forceinline__ float value_at(const NormParams& p, int64_t z, int64_
     return to_float(static_cast<const T*>(p.x)[z * p.step + r * p.row + c * p.col]);
 }
 
-// squares of a block's share of a matrix: rows blockIdx.x, + blocks, ...
+// fn(r, c, values of columns c, c + 32, ...) for a lane's part of the rows `row`, + every, ... of which
+// a warp has each: enough under way at once
+constexpr int kAhead = 8;
+template <typename T, typename Fn>
+__device__ __forceinline__ void values_of(const NormParams& p, int64_t z, int64_t row, int64_t every,
+                                          Fn&& fn) {
+    for (int64_t r = row; r < p.rows; r += every)
+        for (int64_t c = threadIdx.x & 31; c < p.cols; c += 32 * kAhead) {
+            float v[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+                v[i] = c + 32 * i < p.cols ? value_at<T>(p, z, r, c + 32 * i) : 0.0f;
+            fn(r, c, v);
+        }
+}
+
+// sum of a few squares, in float64 where float32 would leave its range
+__device__ __forceinline__ double squares(const float (&v)[kAhead]) {
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) s = fmaf(v[i], v[i], s);
+    if (s > 1.0e-25f && s < 1.0e35f) return s;
+    double d = 0.0;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) d += (double)v[i] * v[i];
+    return d;
+}
+
+// v f for any float64 f > 0 in three float32 products, of which the outer ones are exact: a power of
+// two, f's fraction, and the rest of the power (float64 products of all values took as long as reading
+// them three times)
+struct Factor {
+    float first, fraction, last;
+    __device__ __forceinline__ explicit Factor(double f) {
+        int e = 0;
+        fraction = (float)frexp(f, &e);
+        e = max(-250, min(250, e));
+        first = exp2f((float)(e / 2)), last = exp2f((float)(e - e / 2));
+    }
+    __device__ __forceinline__ float times(float v) const { return v * first * fraction * last; }
+};
+
+// squares of a block's share of a matrix
 template <typename T>
 __global__ void __launch_bounds__(kNormThreads) k_squares(const NormParams p) {
     follow_on();
     const int64_t z = blockIdx.y;
     double sum = 0.0;
-    for (int64_t r = blockIdx.x; r < p.rows; r += p.blocks)
-        for (int64_t c = threadIdx.x; c < p.cols; c += kNormThreads) {
-            const double v = value_at<T>(p, z, r, c);
-            sum += v * v;
-        }
+    constexpr int kWarps = kNormThreads / 32;
+    values_of<T>(p, z, blockIdx.x * kWarps + (threadIdx.x >> 5), p.blocks * kWarps,
+                 [&](int64_t, int64_t, const float(&v)[kAhead]) { sum += squares(v); });
     sum = warp_sum(sum);
     __shared__ double joined[kNormThreads / 32];
     if ((threadIdx.x & 31) == 0) joined[threadIdx.x >> 5] = sum;
@@ -79,40 +119,46 @@ __global__ void __launch_bounds__(kNormThreads) k_scale(const NormParams p) {
         if (threadIdx.x == 0) factor = 1.0 / (sqrt(sum) + (double)p.eps);
     }
     __syncthreads();
-    const double f = factor;
-    for (int64_t r = blockIdx.x; r < p.rows; r += p.blocks)
-        for (int64_t c = threadIdx.x; c < p.cols; c += kNormThreads) {
-            const double v = value_at<T>(p, z, r, c) * f;
-            if (p.final)
-                p.final[(z * p.rows + r) * p.cols + c] = __float2bfloat16_rn((float)v);
-            else
-                p.out[z * p.out_step + r * p.ld + c] = __float2half_rn((float)(v * kScale));
-        }
+    const Factor f(p.final ? factor : factor * kScale);
+    constexpr int kWarps = kNormThreads / 32;
+    values_of<T>(p, z, blockIdx.x * kWarps + (threadIdx.x >> 5), p.blocks * kWarps,
+                 [&](int64_t r, int64_t c, const float(&v)[kAhead]) {
+#pragma unroll
+                     for (int i = 0; i < kAhead; ++i) {
+                         const int64_t at = c + 32 * i;
+                         if (at >= p.cols) break;
+                         const float x = f.times(v[i]);
+                         if (p.final)
+                             p.final[(z * p.rows + r) * p.cols + at] = __float2bfloat16_rn(x);
+                         else
+                             p.out[z * p.out_step + r * p.ld + at] = __float2half_rn(x);
+                     }
+                 });
 }
 
 // ----------------------------------------------------------------------------- small matrices
 // All steps of one matrix in a cluster of kCluster blocks. Each product's tiles of 128 x bn go round
-// the blocks; X, A and B stay in scratch, that is in L2. Every block runs every cluster barrier
+// the blocks; X, A and B stay in scratch, that is in L2. With a tile or two a block there is nothing
+// to gain from symmetry, and the lanes write their rows' values themselves: what counts is the time
+// from one product's last value to the next one's first. Every block runs every cluster barrier
 // whatever failed in it, so none waits for another that has left.
-constexpr int kCluster = 8, kSmallEpi = 8, kSmallTma = 8, kSmallMma = 9;
-constexpr int kSmallThreads = 32 * 10, kSmallStages = 5;
+// 8 x 256 x 512: 7800 to 9000 cycles a product, of which 2300 pass before the first copies land, 450
+// are a k-block's (an SM's share of L2 for 24 to 32 KB), 1500 the epilogue's and 1000 the barrier's.
+constexpr int kCluster = 8, kSmallStages = 6;
 constexpr uint32_t kBox = 64 * kLineBytes;                     // 64 lines
 constexpr uint32_t kSmallStage = 4 * kBox;                     // 128 x 64 of A, up to 128 x 64 of B
-constexpr uint32_t kSmallBufs = kSmallEpi * 2 * kWarpBuf;
 
 struct SmallProduct {
     int m, n, kblocks, bn, tiles;
-    int symmetric;
 };
 struct SmallParams {
-    CUtensorMap x[2], g, h;                     // boxes of 64 x 64: operands in either order
-    CUtensorMap x_out[2], g_out, h_out, y_out;  // boxes of 32 x 32
+    CUtensorMap map_x[2], map_g, map_h;  // boxes of 64 x 64: operands in either order
     SmallProduct gram, poly, next;
-    const __half* in_x[2];
-    const __half* in_g;
+    __half *x[2], *g, *h;
     int64_t ld_x, step_x, ld_g, step_g;
+    NormParams norm;                     // of the matrices as they come
     __nv_bfloat16* y;
-    int rows, cols, steps, tall, tma_y;
+    int rows, cols, steps, tall, wide_y;
     float a, b, c;
     unsigned* flag;
     unsigned polls;
@@ -121,36 +167,30 @@ struct SmallShared {
     unsigned long long full[kSmallStages], empty[kSmallStages], acc_full[2], acc_empty[2], drained;
     uint32_t tmem;
     int fail, issued;
+    double squares[kEpiWarps + 3];  // of the warps, and the block's
 };
 
-__device__ __forceinline__ void bulk_store_done() {
-    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+__device__ __forceinline__ double peer_double(uint32_t addr) {
+    double v;
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(addr));
+    return v;
 }
-// between what other threads wrote and this thread's copies of it, either way
-__device__ __forceinline__ void fence_async_all() {
-    asm volatile("fence.proxy.async;" ::: "memory");
+// between accesses to global memory by threads and by copies
+__device__ __forceinline__ void fence_async_global() {
+    asm volatile("fence.proxy.async.global;" ::: "memory");
 }
 
-// tile w of a product: rows mt * 128, columns nt * bn. Symmetric ones have the tiles that begin on or
-// left of the diagonal: mt + 1 lots of 128 / bn in line mt.
+// tile w of a product: rows mt * 128, columns nt * bn
 __device__ __forceinline__ void small_tile(const SmallProduct& q, int w, int& mt, int& nt) {
-    if (q.symmetric) {
-        const int each = 128 / q.bn;
-        mt = 0;
-        while (w >= (mt + 1) * each) w -= (mt + 1) * each, ++mt;
-        nt = w;
-    } else {
-        const int across = (q.n + q.bn - 1) / q.bn;
-        mt = w / across, nt = w - mt * across;
-    }
+    const int across = (q.n + q.bn - 1) / q.bn;
+    mt = w / across, nt = w - mt * across;
 }
 
-__global__ void __launch_bounds__(kSmallThreads, 1)
-k_small(const __grid_constant__ SmallParams p) {
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1) k_small(const __grid_constant__ SmallParams p) {
     using namespace tc;
     extern __shared__ __align__(1024) unsigned char smem[];
-    unsigned char* bufs = smem + kSmallStages * kSmallStage;
-    auto* sh = reinterpret_cast<SmallShared*>(bufs + kSmallBufs);
+    auto* sh = reinterpret_cast<SmallShared*>(smem + kSmallStages * kSmallStage);
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int rank = (int)cluster_rank(), z = blockIdx.x / kCluster;
@@ -161,14 +201,15 @@ k_small(const __grid_constant__ SmallParams p) {
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&sh->acc_full[i]), 1);
-            mbar_init(smem_u32(&sh->acc_empty[i]), kSmallEpi);
+            mbar_init(smem_u32(&sh->acc_empty[i]), kEpiWarps);
         }
         mbar_init(smem_u32(&sh->drained), 1);
         sh->fail = 0;
         sh->issued = 0;
         asm volatile("fence.mbarrier_init.release.cluster;");
     }
-    if (warp == kSmallMma) tmem_alloc(&sh->tmem, 256);
+    if (warp == kMmaWarp) tmem_alloc(&sh->tmem, 256);
+    if (warp == kTmaWarp && lane < 4) prefetch_map(&p.map_x[0] + lane);  // all of them
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
@@ -176,12 +217,51 @@ k_small(const __grid_constant__ SmallParams p) {
     volatile int* fail = &sh->fail;
     follow_on();
 
+    // X = x / (|x|_F + eps): a row a warp, every kCluster-th block's; the rows come again from L2
+    {
+        const NormParams& n = p.norm;
+        const int first = rank * kThreads / 32 + warp, every = kCluster * kThreads / 32;
+        double sum = 0.0;
+        values_of<T>(n, z, first, every,
+                     [&](int64_t, int64_t, const float(&v)[kAhead]) { sum += squares(v); });
+        sum = warp_sum(sum);
+        if (lane == 0) sh->squares[warp] = sum;
+        __syncthreads();
+        if (tid == 0) {
+            sum = 0.0;
+            for (int i = 0; i < kThreads / 32; ++i) sum += sh->squares[i];
+            sh->squares[kThreads / 32] = sum;
+        }
+        __syncthreads();
+        cluster_sync();
+        sum = 0.0;
+        for (int i = 0; i < kCluster; ++i)
+            sum += peer_double(peer_address(smem_u32(&sh->squares[kThreads / 32]), i));
+        const Factor f(kScale / (sqrt(sum) + (double)n.eps));
+        values_of<T>(n, z, first, every, [&](int64_t r, int64_t c, const float(&v)[kAhead]) {
+            __half* to = p.x[0] + z * p.step_x + r * p.ld_x;
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+                if (c + 32 * i < p.cols) to[c + 32 * i] = __float2half_rn(f.times(v[i]));
+        });
+        fence_async_global();
+        __syncwarp();
+        cluster_sync();
+    }
+
     const bool one = elect_one();
     int st = 0, issued = 0, buf = 0;
-    uint32_t parity = warp == kSmallTma ? 1 : 0;         // of the stage's next wait
-    uint32_t acc_parity = warp == kSmallMma ? 1 : 0;     // of the accumulator's
-    const Stage s0(smem_u32(bufs) + warp * 2 * kWarpBuf, lane);
-    const Stage s1(smem_u32(bufs) + (warp * 2 + 1) * kWarpBuf, lane);
+    uint32_t parity = warp == kTmaWarp ? 1 : 0;         // of the stage's next wait
+    uint32_t acc_parity = warp == kMmaWarp ? 1 : 0;     // of the accumulator's
+
+    // `boxes` of a stage from its box `at` on: 64 lines each from `line` on, k-block kb
+    auto load = [&](int line, int boxes, const CUtensorMap* map, bool mn, int stage, int at,
+                    int kb) {
+        const uint32_t to = smem_u32(smem) + (uint32_t)stage * kSmallStage + at * kBox;
+        for (int i = 0; i < boxes; ++i)
+            tma_load3(to + i * kBox, map, mn ? line + i * 64 : kb * 64,
+                      mn ? kb * 64 : line + i * 64, z, smem_u32(&sh->full[stage]));
+    };
 
     for (int phase = 0; phase < 3 * p.steps; ++phase) {
         const int step = phase / 3, kind = phase - 3 * step;
@@ -190,11 +270,11 @@ k_small(const __grid_constant__ SmallParams p) {
         const int from = step & 1;
         // gram: A and B are X; poly: A; next: B X, or X B of tall ones
         const bool a_mn = kind == 0 && p.tall, b_mn = kind == 0 ? p.tall : kind == 2 && !p.tall;
-        if (warp == kSmallTma) {
-            const CUtensorMap* x = &p.x[from];
-            const CUtensorMap* am = kind == 0 ? x : kind == 1 ? &p.g : p.tall ? x : &p.h;
-            const CUtensorMap* bm = kind == 0 ? x : kind == 1 ? &p.g : p.tall ? &p.h : x;
-            fence_async_all();
+        if (warp == kTmaWarp) {
+            const CUtensorMap* x = &p.map_x[from];
+            const CUtensorMap* am = kind == 0 ? x : kind == 1 ? &p.map_g : p.tall ? x : &p.map_h;
+            const CUtensorMap* bm = kind == 0 ? x : kind == 1 ? &p.map_g : p.tall ? &p.map_h : x;
+            fence_async_global();
             bool ok = !*fail;
             for (int w = rank; w < q.tiles && ok; w += kCluster) {
                 int mt, nt;
@@ -205,17 +285,10 @@ k_small(const __grid_constant__ SmallParams p) {
                         ok = false;
                         break;
                     }
-                    const uint32_t bar = smem_u32(&sh->full[st]);
-                    const uint32_t a = smem_u32(smem) + (uint32_t)st * kSmallStage;
                     if (one) {
-                        mbar_expect_tx(bar, (2 + q.bn / 64) * kBox);
-                        for (int i = 0; i < 2 + q.bn / 64; ++i) {
-                            const bool is_b = i >= 2;
-                            const int line = is_b ? nt * q.bn + (i - 2) * 64 : mt * 128 + i * 64;
-                            const bool mn = is_b ? b_mn : a_mn;
-                            tma_load3(a + i * kBox, is_b ? bm : am, mn ? line : kb * 64,
-                                      mn ? kb * 64 : line, z, bar);
-                        }
+                        mbar_expect_tx(smem_u32(&sh->full[st]), (2 + q.bn / 64) * kBox);
+                        load(mt * 128, 2, am, a_mn, st, 0, kb);
+                        load(nt * q.bn, q.bn / 64, bm, b_mn, st, 2, kb);
                     }
                     __syncwarp();
                     ++issued;
@@ -225,7 +298,7 @@ k_small(const __grid_constant__ SmallParams p) {
             if (!ok && !*fail) *fail = 1;
             if (one) sh->issued = issued;
             __syncwarp();
-        } else if (warp == kSmallMma) {
+        } else if (warp == kMmaWarp) {
             const uint64_t step_a = a_mn ? 2048 >> 4 : 32 >> 4, step_b = b_mn ? 2048 >> 4 : 32 >> 4;
             const uint64_t desc_a = operand_desc(smem_u32(smem), a_mn);
             const uint64_t desc_b = operand_desc(smem_u32(smem) + 2 * kBox, b_mn);
@@ -268,74 +341,81 @@ k_small(const __grid_constant__ SmallParams p) {
             const float unit = last ? 1.0f / kScale : 1.0f;
             const float alpha = kind == 0 ? 1.0f / kScale : kind == 1 ? p.c / kScale : unit / kScale;
             const float beta = kind == 1 ? p.b : p.a * unit;
-            const CUtensorMap* out = kind == 0 ? &p.g_out : kind == 1 ? &p.h_out
-                                     : last   ? &p.y_out : &p.x_out[from ^ 1];
             const __half* in = kind == 0 ? nullptr
-                               : kind == 1 ? p.in_g + z * p.step_g : p.in_x[from] + z * p.step_x;
-            const int64_t ld = kind == 1 ? p.ld_g : p.ld_x;
-            const bool tma = !last || p.tma_y;
+                               : kind == 1 ? p.g + z * p.step_g : p.x[from] + z * p.step_x;
+            const int64_t ld_in = kind == 1 ? p.ld_g : p.ld_x;
+            __half* out = kind == 0 ? p.g + z * p.step_g
+                          : kind == 1 ? p.h + z * p.step_g : p.x[from ^ 1] + z * p.step_x;
+            const int64_t ld_out = kind < 2 ? p.ld_g : p.ld_x;
             const int quarter = warp & 3, share = warp >> 2;
             bool ok = !*fail;
             for (int w = rank; w < q.tiles && ok; w += kCluster) {
                 int mt, nt;
                 small_tile(q, w, mt, nt);
-                const int row0 = mt * 128 + quarter * 32, rows = max(0, min(32, q.m - row0));
+                const int row = mt * 128 + quarter * 32 + lane;
                 const uint32_t acc = tmem + buf * 128 + ((uint32_t)(quarter * 32) << 16);
-                const bool mirror = q.symmetric && nt * q.bn + q.bn <= mt * 128;
-                for (int c = share * 32; c < q.bn; c += 64) {
-                    const int col = nt * q.bn + c;
-                    if (lane == 0) bulk_store_read();
-                    __syncwarp();
+                // the lane's 16 values in two pieces of 16 bytes; lines are padded to these
+                auto pieces = [&](int col, auto&& fn) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        if (row < q.m && col + 8 * i < q.n) fn(i, col + 8 * i);
+                };
+                uint4 given[2][2] = {};
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    if (in && share * 16 + t * 64 < q.bn)
+                        pieces(nt * q.bn + share * 16 + t * 64, [&](int i, int col) {
+                            // past L1, which may hold these lines as they were a step before
+                            given[t][i] =
+                                __ldcg(reinterpret_cast<const uint4*>(in + row * ld_in + col));
+                        });
+                ok = mbar_wait(smem_u32(&sh->acc_full[buf]), acc_parity, p.polls) && !*fail;
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                fence_after_sync();
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int c = share * 16 + t * 64, col0 = nt * q.bn + c;
+                    if (c >= q.bn) break;
+                    float v[16];
+                    tmem_ld16(acc + c, v);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[j] *= alpha;
                     if (in) {
-                        // past L1, which may hold these lines as they were a step before
-                        const int r0 = lane >> 2, cc = (lane & 3) * 8;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            uint4 v = make_uint4(0, 0, 0, 0);
-                            if (r0 + 8 * i < rows && col + cc < q.n)
-                                v = __ldcg(reinterpret_cast<const uint4*>(
-                                    in + (int64_t)(row0 + r0 + 8 * i) * ld + col + cc));
-                            put16(s0.turn(i), v);
-                        }
-                        __syncwarp();
-                    }
-                    if (c == share * 32) {
-                        ok = mbar_wait(smem_u32(&sh->acc_full[buf]), acc_parity, p.polls) && !*fail;
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) break;
-                        fence_after_sync();
-                    }
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        float v[16];
-                        Two t[8], u[8];
-                        tmem_ld16(acc + c + half * 16, v);
-                        if (in) get_row<__half>(s0, half, u);
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
-                            t[j] = two(v[2 * j], v[2 * j + 1]) * two(alpha);
-                            if (in) t[j] = fma(u[j], two(beta), t[j]);
+                            const uint4& g = given[t][j / 4];
+                            const uint32_t word = j % 4 == 0 ? g.x : j % 4 == 1 ? g.y
+                                                  : j % 4 == 2 ? g.z : g.w;
+                            const float2 f = unpack2<__half>(word);
+                            v[2 * j] = fmaf(f.x, beta, v[2 * j]);
+                            v[2 * j + 1] = fmaf(f.y, beta, v[2 * j + 1]);
                         }
-                        if (mirror) put_column<__half>(s1, half, t);
-                        if (last) put_row<__nv_bfloat16>(s0, half, t);
-                        else put_row<__half>(s0, half, t);
                     }
-                    if (tma) fence_async_smem();
-                    __syncwarp();
-                    if (tma) {
-                        if (lane == 0 && rows > 0 && col < q.n) {
-                            bulk_store3(out, s0.base, col, row0, z);
-                            if (mirror) bulk_store3(out, s1.base, row0, col, z);
-                            bulk_store_commit();
-                        }
+                    auto packed = [&](auto type, int i) {
+                        using O = decltype(type);
+                        const float* f = v + 8 * i;
+                        return make_uint4(pack2<O>(f[0], f[1]), pack2<O>(f[2], f[3]),
+                                          pack2<O>(f[4], f[5]), pack2<O>(f[6], f[7]));
+                    };
+                    if (!last) {
+                        pieces(col0, [&](int i, int col) {
+                            *reinterpret_cast<uint4*>(out + row * ld_out + col) =
+                                packed(__half(), i);
+                        });
                     } else {
-                        store_rows<__nv_bfloat16>(
-                            s0, p.y + ((int64_t)z * p.rows + row0) * p.cols + col, p.cols, rows,
-                            q.n - col);
+                        __nv_bfloat16* to = p.y + ((int64_t)z * p.rows + row) * p.cols;
+                        if (p.wide_y) {
+                            pieces(col0, [&](int i, int col) {
+                                *reinterpret_cast<uint4*>(to + col) = packed(__nv_bfloat16(), i);
+                            });
+                        } else if (row < q.m) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j)
+                                if (col0 + j < q.n) to[col0 + j] = __float2bfloat16_rn(v[j]);
+                        }
                     }
-                    __syncwarp();
                 }
-                if (!ok) break;
                 fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&sh->acc_empty[buf]));
@@ -344,10 +424,7 @@ k_small(const __grid_constant__ SmallParams p) {
                 if (buf == 0) acc_parity ^= 1;
             }
             if (!ok && !*fail) *fail = 4;
-            if (lane == 0) {  // the results are in L2
-                bulk_store_done();
-                fence_async_all();
-            }
+            fence_async_global();  // copies will read what was written
         }
         __syncwarp();
         cluster_sync();
@@ -361,7 +438,7 @@ k_small(const __grid_constant__ SmallParams p) {
                 mbar_wait(smem_u32(&sh->full[i % kSmallStages]), (i / kSmallStages) & 1);
         }
         __syncwarp();
-        if (warp == kSmallMma) {
+        if (warp == kMmaWarp) {
             if (one) mma_commit(smem_u32(&sh->drained));
             __syncwarp();
             mbar_wait(smem_u32(&sh->drained), 0);
@@ -370,7 +447,7 @@ k_small(const __grid_constant__ SmallParams p) {
     }
     fence_before_sync();
     __syncthreads();
-    if (warp == kSmallMma) {
+    if (warp == kMmaWarp) {
         fence_after_sync();
         tmem_dealloc(tmem, 256);
     }
@@ -459,7 +536,7 @@ void run_step(const Step& s, cudaStream_t stream) {
 }
 
 // The products of a matrix of rows x cols in tiles of 128 x 64 or 128 x 128, whichever takes the
-// blocks of a cluster less time, and the cycles that a step takes.
+// blocks of a cluster less time, and the cycles that a step takes (the figures beside k_small).
 struct SmallPlan {
     SmallProduct gram, poly, next;
     double cycles;
@@ -467,48 +544,42 @@ struct SmallPlan {
 SmallPlan plan_small(int64_t rows, int64_t cols) {
     SmallPlan plan{};
     const int64_t small = std::min(rows, cols), large = std::max(rows, cols);
-    auto product = [&](int64_t m, int64_t n, int64_t k, bool symmetric) {
+    auto product = [&](int64_t m, int64_t n, int64_t k) {
         SmallProduct best{};
         double best_cost = 0.0;
         for (int bn : {128, 64}) {
             const int64_t tm = (m + 127) / 128, tn = (n + bn - 1) / bn;
-            const int64_t tiles = symmetric ? tm * (tm + 1) / 2 * (128 / bn) : tm * tn;
             const int kblocks = (int)((k + 63) / 64);
-            const double main = kblocks * block_cycles(false, bn), epi = 600.0 + 16.0 * bn;
-            const double turns = (double)((tiles + kCluster - 1) / kCluster);
-            const double cost = 3000.0 + turns * std::max(main, epi) + std::min(main, epi);
+            const double turns = (double)((tm * tn + kCluster - 1) / kCluster);
+            const double cost = 6800.0 + (turns - 1.0) * 1500.0 +
+                                turns * kblocks * (bn == 64 ? 250.0 : 500.0);
             if (best.bn == 0 || cost < best_cost) {
                 best_cost = cost;
-                best = {(int)m, (int)n, kblocks, bn, (int)tiles, symmetric};
+                best = {(int)m, (int)n, kblocks, bn, (int)(tm * tn)};
             }
         }
         plan.cycles += best_cost;
         return best;
     };
-    plan.gram = product(small, small, large, true);
-    plan.poly = product(small, small, small, true);
-    plan.next = product(rows, cols, small, false);
+    plan.gram = product(small, small, large);
+    plan.poly = product(small, small, small);
+    plan.next = product(rows, cols, small);
     return plan;
 }
 
 void run_small(const rune_orthogonalize_args& a, const SmallPlan& plan, const Stack (&x)[2],
-               const Stack& g, const Stack& h, cudaStream_t stream) {
+               const Stack& g, const Stack& h, const NormParams& norm, cudaStream_t stream) {
     SmallParams p{};
-    const Stack y{a.y, a.rows, a.cols, a.cols, a.rows * a.cols};
-    auto out = [&](const Stack& t) {
-        return make_out_map3(t.p, t.rows, t.cols, t.ld, a.count, t.step);
-    };
+    p.norm = norm;
     for (int i = 0; i < 2; ++i) {
         const Stack& t = a.steps > 1 ? x[i] : x[0];
-        p.x[i] = t.map(a.count, 64), p.x_out[i] = out(t);
-        p.in_x[i] = static_cast<const __half*>(t.p);
+        p.map_x[i] = t.map(a.count, 64);
+        p.x[i] = static_cast<__half*>(t.p);
     }
-    p.g = g.map(a.count, 64), p.g_out = out(g);
-    p.h = h.map(a.count, 64), p.h_out = out(h);
-    p.tma_y = wide16(a.y, a.cols, a.cols);
-    p.y_out = p.tma_y ? out(y) : p.g_out;
+    p.map_g = g.map(a.count, 64), p.g = static_cast<__half*>(g.p);
+    p.map_h = h.map(a.count, 64), p.h = static_cast<__half*>(h.p);
+    p.wide_y = wide16(a.y, a.cols, a.cols);
     p.gram = plan.gram, p.poly = plan.poly, p.next = plan.next;
-    p.in_g = static_cast<const __half*>(g.p);
     p.ld_x = x[0].ld, p.step_x = x[0].step, p.ld_g = g.ld, p.step_g = g.step;
     p.y = static_cast<__nv_bfloat16*>(a.y);
     p.rows = (int)a.rows, p.cols = (int)a.cols;
@@ -516,18 +587,25 @@ void run_small(const rune_orthogonalize_args& a, const SmallPlan& plan, const St
     p.a = a.a, p.b = a.b, p.c = a.c;
     p.flag = wait_flag(a.device);
     p.polls = wait_polls();
-    const size_t smem = kSmallStages * kSmallStage + kSmallBufs + sizeof(SmallShared);
-    static std::atomic<uint64_t> allowed{0};  // devices whose limit is raised
-    if (a.device >= 64 || !(allowed.load(std::memory_order_relaxed) >> a.device & 1)) {
-        RUNE_CUDA_TRY(cudaFuncSetAttribute(k_small, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           (int)smem));
-        if (a.device < 64) allowed.fetch_or(uint64_t(1) << a.device, std::memory_order_relaxed);
-    }
-    launch(k_small, (unsigned)(a.count * kCluster), kSmallThreads, smem, kCluster, stream, p);
+    const size_t smem = kSmallStages * kSmallStage + sizeof(SmallShared);
+    auto typed = [&](auto t) {
+        using T = decltype(t);
+        static std::atomic<uint64_t> allowed{0};  // devices whose limit is raised
+        if (a.device >= 64 || !(allowed.load(std::memory_order_relaxed) >> a.device & 1)) {
+            RUNE_CUDA_TRY(cudaFuncSetAttribute(
+                k_small<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            if (a.device < 64) allowed.fetch_or(uint64_t(1) << a.device, std::memory_order_relaxed);
+        }
+        launch(k_small<T>, (unsigned)(a.count * kCluster), kThreads, smem, kCluster, stream, p);
+    };
+    if (a.dtype == RUNE_F16) typed(__half());
+    else if (a.dtype == RUNE_BF16) typed(__nv_bfloat16());
+    else typed(float());
 }
 
-// Whether the clusters take less time than a chain of launches, of 10000 cycles a product at least
-// and then at the tensor cores' rate of all SMs.
+// Whether the clusters take less time than a chain of launches, of 11500 cycles a product at least
+// and then at the tensor cores' rate of all SMs. B200, five steps, clusters / chain, us: 1 x 256 x 256
+// 59 / 80, 15 x 256 x 512 76 / 113, 12 x 128 x 1024 78 / 97; 16 x 256 x 512, in two waves, 150 / 110.
 bool use_small(const rune_orthogonalize_args& a, const SmallPlan& plan) {
     const int64_t small = std::min(a.rows, a.cols), large = std::max(a.rows, a.cols);
     if (a.steps == 0 || large > (1 << 20) || a.count > (1 << 16)) return false;
@@ -535,13 +613,13 @@ bool use_small(const rune_orthogonalize_args& a, const SmallPlan& plan) {
     // clusters at once: blocks of one lie in one group of SMs, so not all SMs find a place
     const double waves = std::ceil((double)a.count * kCluster / (sms * 0.85));
     const double kb = (double)a.count * ((small + 127) / 128) * ((large + 63) / 64) / sms;
-    const double chain = 3.0 * std::max(10000.0, 3000.0 + kb * ((small + 127) / 128) * 350.0);
+    const double chain = 3.0 * std::max(11500.0, 5000.0 + kb * ((small + 127) / 128) * 350.0);
     return waves * plan.cycles < chain;
 }
 
 int norm_blocks(const rune_orthogonalize_args& a) {
     const int64_t most = std::max<int64_t>(1, (int64_t)sm_count(a.device) * 8 / a.count);
-    return (int)std::min<int64_t>(a.rows, most);
+    return (int)std::min<int64_t>((a.rows + 7) / 8, most);  // eight rows a block at once
 }
 
 void orthogonalize(const rune_orthogonalize_args& a, Scratch& ws, cudaStream_t stream) {
@@ -568,6 +646,10 @@ void orthogonalize(const rune_orthogonalize_args& a, Scratch& ws, cudaStream_t s
     n.final = a.steps == 0 ? static_cast<__nv_bfloat16*>(a.y) : nullptr;
     const dim3 grid((unsigned)n.blocks, (unsigned)a.count);
     const SmallPlan plan = plan_small(a.rows, a.cols);
+    if (use_small(a, plan)) {
+        run_small(a, plan, x, g, h, n, stream);
+        return;
+    }
     auto prepare = [&](auto t) {
         using T = decltype(t);
         launch(k_squares<T>, grid, kNormThreads, 0, 0, stream, n);
@@ -576,10 +658,6 @@ void orthogonalize(const rune_orthogonalize_args& a, Scratch& ws, cudaStream_t s
     if (a.dtype == RUNE_F16) prepare(__half());
     else if (a.dtype == RUNE_BF16) prepare(__nv_bfloat16());
     else prepare(float());
-    if (use_small(a, plan)) {
-        run_small(a, plan, x, g, h, stream);
-        return;
-    }
     for (int i = 0; i < a.steps; ++i) {
         const Stack from = x[i & 1];
         const bool last = i + 1 == a.steps;
