@@ -5,7 +5,10 @@ atom of a periodic alloy, a histogram of its neighbours' distances by species, a
 teacher's per-atom energies. The training step runs the operators of ``rune_b200.ops`` forward and
 backward; at the end the 8-bit copy serves the same energies.
 
-    python examples/distil_network.py [--steps 300] [--cells 8] [--gated]
+    python examples/distil_network.py [--steps 300] [--cells 8] [--gated] [--experts 8] [--muon]
+
+``--experts`` gives the blocks as many feed-forward networks, two for each atom (and no 8-bit copy);
+``--muon`` updates the blocks' matrices by their orthogonalised momentum.
 """
 
 from __future__ import annotations
@@ -21,6 +24,7 @@ import torch
 
 from rune_b200.nep.plugin import build_model, resolve_params
 from rune_b200.network import ScalarNetwork
+from rune_b200.optim import Muon
 
 
 def alloy(cells, seed, a=3.6, jitter=0.1, species=3):
@@ -46,8 +50,9 @@ def features(pos, edge, types, species=3, bins=24, cutoff=6.0):
     return torch.stack(out, 1)
 
 
-def train(steps=300, cells=8, gated=False, hidden=128, blocks=3, seed=7, log=print):
-    """(first and last loss, the 8-bit copy's root-mean-square deviation from the network)."""
+def train(steps=300, cells=8, gated=False, hidden=128, blocks=3, seed=7, log=print, experts=0,
+          muon=False):
+    """(first and last loss, the 8-bit copy's root-mean-square deviation from the network, or None)."""
     dev = torch.device("cuda")
     torch.manual_seed(seed)
     teacher = build_model(resolve_params(dict(
@@ -64,25 +69,35 @@ def train(steps=300, cells=8, gated=False, hidden=128, blocks=3, seed=7, log=pri
         data.append((features(pos.float(), edge, types), types, out["energies"].float()))
     mean = torch.cat([e for _, _, e in data]).mean()
     spread = torch.cat([e for _, _, e in data]).std()
-    net = ScalarNetwork(3, data[0][0].shape[1], hidden, 2 * hidden, blocks, gated=gated).to(dev)
+    net = ScalarNetwork(3, data[0][0].shape[1], hidden, 2 * hidden, blocks, gated=gated,
+                        experts=experts).to(dev)
     net.q_scaler.copy_(1.0 / torch.cat([q for q, _, _ in data]).std(0).clamp(min=1e-3))
-    opt = torch.optim.AdamW(net.parameters(), lr=2e-3)
+    matrices = [p for p in net.residual_blocks.parameters()
+                if muon and (p.dim() == 3 or not experts and p.dim() == 2)]
+    inside = {id(p) for p in matrices}
+    opts = [torch.optim.AdamW([p for p in net.parameters() if id(p) not in inside], lr=2e-3)]
+    if matrices:
+        opts.append(Muon(matrices, lr=5e-3))
     losses = []
     for step in range(steps):
         q, types, energies = data[step % len(data)]
         loss = ((net(q, types) - (energies - mean) / spread) ** 2).mean()
-        opt.zero_grad(set_to_none=True)
+        net.zero_grad(set_to_none=True)
         loss.backward()
-        opt.step()
+        for opt in opts:
+            opt.step()
         losses.append(loss.detach())
         if log and step % max(1, steps // 10) == 0:
             log(f"step {step}: mean squared error {float(losses[-1]):.4f} of the variance")
     q, types, _ = data[0]
-    with torch.no_grad():
-        apart = float((net.quantized()(q, types) - net(q, types)).pow(2).mean().sqrt())
+    apart = None
+    if not experts:
+        with torch.no_grad():
+            apart = float((net.quantized()(q, types) - net(q, types)).pow(2).mean().sqrt())
     first, last = float(losses[0]), float(torch.stack(losses[-4:]).mean())
     if log:
-        log(f"mean squared error {first:.4f} -> {last:.4f}; 8-bit copy {apart:.4f} apart")
+        log(f"mean squared error {first:.4f} -> {last:.4f}"
+            + ("" if experts else f"; 8-bit copy {apart:.4f} apart"))
     return first, last, apart
 
 
@@ -91,5 +106,7 @@ if __name__ == "__main__":
     parser.add_argument("--steps", type=int, default=300)
     parser.add_argument("--cells", type=int, default=8)
     parser.add_argument("--gated", action="store_true")
+    parser.add_argument("--experts", type=int, default=0)
+    parser.add_argument("--muon", action="store_true")
     args = parser.parse_args()
-    train(args.steps, args.cells, args.gated)
+    train(args.steps, args.cells, args.gated, experts=args.experts, muon=args.muon)

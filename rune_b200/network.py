@@ -1,4 +1,5 @@
-"""The Möbius scalar network in mixed precision, trainable: projection, residual blocks, head.
+"""The Möbius scalar network in mixed precision, trainable: projection, residual blocks, head; with
+experts in its blocks on request; and NEP's networks, one per element.
 
 The engine evaluates Möbius models in float32 without parameter gradients. ``ScalarNetwork`` is
 the same per-atom network (rune/mobius/model.py:256-305 without messages, layers.py:26-89) on the
@@ -10,9 +11,14 @@ descriptors (the engine computes its own inside the kernels and returns none); n
 
 A block adds its output to the residual stream in the next block's normalisation, so the stream
 is read and written once per block.
+
+``ElementNetwork`` is the network of NEP models (rune/nep/model.py:157-170 loops over the elements):
+atoms sorted by element, one product for all of them.
 """
 
 from __future__ import annotations
+
+import math
 
 import torch
 import torch.nn as nn
@@ -21,28 +27,68 @@ from . import ops
 from .mobius.model import ElementwiseLinearHead, ResidualBlock, RMSNorm
 
 
+def _stack(groups, outputs, inputs):
+    """Weights and biases of ``groups`` linear layers, each initialised as nn.Linear's."""
+    bound = 1.0 / math.sqrt(inputs)
+    return (nn.Parameter(torch.empty(groups, outputs, inputs).uniform_(-bound, bound)),
+            nn.Parameter(torch.empty(groups, outputs).uniform_(-bound, bound)))
+
+
+class ExpertBlock(nn.Module):
+    """The residual block with ``experts`` feed-forward networks, ``top_k`` of them for each row,
+    weighted by the softmax of their router logits."""
+
+    def __init__(self, hidden, ffn, experts, top_k, activation, gated, norm_eps):
+        super().__init__()
+        self.activation, self.gated, self.top_k = activation, gated, top_k
+        self.norm = RMSNorm(hidden, eps=norm_eps)
+        self.router = nn.Linear(hidden, experts, bias=False)
+        self.weight_in, self.bias_in = _stack(experts, (2 if gated else 1) * ffn, hidden)
+        self.weight_out, self.bias_out = _stack(experts, hidden, ffn)
+
+    def forward(self, x):
+        """What the block adds to the stream, of its normalised rows."""
+        dtype, experts = x.dtype, self.weight_in.shape[0]
+        index, weights = ops.route(ops.linear(x, self.router.weight.to(dtype)), self.top_k)
+        groups = ops.row_groups(index, experts)
+        layer = ops.grouped_gated_linear if self.gated else ops.grouped_linear
+        x = layer(ops.to_groups(x, groups), self.weight_in.to(dtype), groups,
+                  bias=self.bias_in.to(dtype), activation=self.activation)
+        x = ops.grouped_linear(x, self.weight_out.to(dtype), groups, bias=self.bias_out.to(dtype))
+        return ops.from_groups(x, groups, weights)
+
+
 class ScalarNetwork(nn.Module):
     """Per-atom energies [N] (float32) of descriptors [N, inputs] and element indices [N].
 
     gated: the blocks' first layer is ``act(x Wg^T + bg) * (x Wu^T + bu)``; ``ffn.0`` then holds
-    2 * ffn rows, the gate's first. dtype: torch.bfloat16 or torch.float16, of the states.
+    2 * ffn rows, the gate's first. experts: the blocks are ``ExpertBlock``s of as many networks,
+    ``top_k`` of which each atom takes; 0: none. dtype: torch.bfloat16 or torch.float16, of the
+    states.
     """
 
     def __init__(self, n_elements, inputs, hidden, ffn, blocks, activation="silu", gated=False,
-                 norm_eps=1.0e-8, dtype=torch.bfloat16):
+                 norm_eps=1.0e-8, dtype=torch.bfloat16, experts=0, top_k=2):
         super().__init__()
-        if min(n_elements, inputs, hidden, ffn) <= 0 or blocks < 0:
+        if min(n_elements, inputs, hidden, ffn) <= 0 or blocks < 0 or experts < 0:
             raise ValueError("ScalarNetwork dimensions must be positive.")
+        if experts and not 1 <= top_k <= min(experts, 32):
+            raise ValueError(f"top_k must be 1 to 32 and at most the {experts} experts.")
         if dtype not in (torch.bfloat16, torch.float16):
             raise ValueError(f"dtype must be float16 or bfloat16, not {dtype}.")
         self.activation, self.gated, self.dtype = str(activation).strip().lower(), bool(gated), dtype
-        self.norm_eps = float(norm_eps)
+        self.norm_eps, self.experts = float(norm_eps), int(experts)
         self.register_buffer("q_scaler", torch.ones(inputs))
         self.input_projection = nn.Linear(inputs, hidden)
         self.element_embedding = nn.Embedding(n_elements, hidden)
-        self.residual_blocks = nn.ModuleList(
-            ResidualBlock(hidden, ffn, activation, norm_eps=norm_eps) for _ in range(blocks))
-        if gated:
+        if experts:
+            self.residual_blocks = nn.ModuleList(
+                ExpertBlock(hidden, ffn, experts, top_k, self.activation, self.gated, norm_eps)
+                for _ in range(blocks))
+        else:
+            self.residual_blocks = nn.ModuleList(
+                ResidualBlock(hidden, ffn, activation, norm_eps=norm_eps) for _ in range(blocks))
+        if gated and not experts:
             for block in self.residual_blocks:
                 block.ffn[0] = nn.Linear(hidden, 2 * ffn)
         self.output_norm = RMSNorm(hidden, eps=norm_eps)
@@ -83,6 +129,9 @@ class ScalarNetwork(nn.Module):
             else:
                 x, stream = ops.rms_norm(delta, block.norm.weight, residual=stream,
                                          eps=self.norm_eps)
+            if self.experts:
+                delta = block(x)
+                continue
             weight, bias = self._cast(block.ffn[0])
             if self.gated:
                 x = ops.gated_linear(x, weight, bias=bias, activation=self.activation)
@@ -94,7 +143,10 @@ class ScalarNetwork(nn.Module):
 
     def quantized(self):
         """A function like ``forward`` with the blocks' products in 8 bits: a copy of the network
-        as it is now, its weights laid out; later changes of the network do not reach it."""
+        as it is now, its weights laid out; later changes of the network do not reach it. Not of
+        networks with experts."""
+        if self.experts:
+            raise ValueError("The experts' products have no 8-bit form.")
         return _Quantized(self)
 
 
@@ -144,3 +196,51 @@ class _Quantized:
             x, sx = ops.quantize_fp8(x)
             delta = ops.linear(x, w1, bias=b1, x_scale=sx, weight_scale=s1, **more)
         return _energies(stream, delta, types, self.norm_eps, *self.ends)
+
+
+class ElementNetwork(nn.Module):
+    """Per-atom energies [N] (float32) of descriptors [N, inputs] and element indices [N], by a
+    network of its own for each element: ``head . act(W q + b) - shared_bias``, as NEP's.
+
+    An atom whose index is no element's gets ``-shared_bias``. dtype: torch.bfloat16 or
+    torch.float16, of the hidden layer.
+    """
+
+    def __init__(self, n_elements, inputs, hidden, activation="tanh", dtype=torch.bfloat16):
+        super().__init__()
+        if min(n_elements, inputs, hidden) <= 0:
+            raise ValueError("ElementNetwork dimensions must be positive.")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"dtype must be float16 or bfloat16, not {dtype}.")
+        self.activation, self.dtype = str(activation).strip().lower(), dtype
+        self.register_buffer("q_scaler", torch.ones(inputs))
+        self.weight, self.bias = _stack(n_elements, hidden, inputs)
+        # a table's rows with float32 gradients; the last one for atoms of no element
+        self.head = nn.Embedding(n_elements + 1, hidden, padding_idx=n_elements)
+        bound = 1.0 / math.sqrt(hidden)
+        with torch.no_grad():
+            self.head.weight[:n_elements].uniform_(-bound, bound)
+        self.shared_bias = nn.Parameter(torch.zeros(1))
+
+    @classmethod
+    def from_nep(cls, model, dtype=torch.bfloat16):
+        """The networks of a NEP model (``rune_b200.nep.plugin``), their weights copied."""
+        mlps = [model.element_mlps[e] for e in model.elements]
+        net = cls(len(mlps), model.input_dim, mlps[0][0].out_features, dtype=dtype)
+        with torch.no_grad():
+            net.q_scaler.copy_(model.q_scaler)
+            net.shared_bias.copy_(model.shared_bias)
+            for i, mlp in enumerate(mlps):
+                net.weight[i].copy_(mlp[0].weight)
+                net.bias[i].copy_(mlp[0].bias)
+                net.head.weight[i].copy_(mlp[2].weight[0])
+        return net.to(model.q_scaler.device)
+
+    def forward(self, descriptors, types):
+        elements = self.weight.shape[0]
+        groups = ops.row_groups(types, elements)
+        x = ops.to_groups((descriptors * self.q_scaler).to(self.dtype), groups)
+        h = ops.grouped_linear(x, self.weight.to(self.dtype), groups,
+                               bias=self.bias.to(self.dtype), activation=self.activation)
+        rows = torch.where((types >= 0) & (types < elements), types, elements)
+        return (ops.from_groups(h, groups).float() * self.head(rows)).sum(-1) - self.shared_bias
