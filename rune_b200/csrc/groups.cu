@@ -26,6 +26,8 @@ namespace ops {
 namespace {
 
 constexpr int kMaxGroups = 1024, kMaxChoices = 32;
+// Rows above which few groups' logits go a thread per row: below, a warp per row is sooner done.
+constexpr int64_t kRouteRows = 4096;
 
 // ------------------------------------------------------------------------------------ route
 // Orders as the values do: NaN above all, -0 as 0.
@@ -35,6 +37,10 @@ __device__ __forceinline__ uint32_t order_key(float v) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 constexpr uint32_t kKeyMasked = 0x007fffffu;  // of -inf
+__device__ __forceinline__ float key_value(uint32_t key) {
+    return key == 0xffffffffu ? __uint_as_float(0x7fc00000u)
+                              : __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
 
 template <typename T>
 struct RouteParams {
@@ -45,8 +51,80 @@ struct RouteParams {
     float* weights;
 };
 
+// The softmax over the choices, of which lane j has the j-th: its logit and its group (-1: none).
+template <typename T>
+__device__ __forceinline__ void finish_route(const RouteParams<T>& p, int64_t row, float value,
+                                             int chosen) {
+    const int lane = threadIdx.x & 31;
+    const float largest = __shfl_sync(0xffffffffu, value, 0);
+    const float e = chosen >= 0 ? expf(value - largest) : 0.0f;
+    const float sum = warp_sum(e);
+    if (lane < p.k) {
+        p.index[row * p.k + lane] = chosen;
+        p.weights[row * p.k + lane] = chosen >= 0 ? e / sum : 0.0f;
+    }
+}
+
+// 16-bit logits as words, the order of the value above the index's complement: one comparison
+// settles ties too. A lane sorts its PER words (Batcher's network), and each round of the selection
+// is the maximum of the lanes' first words, whose lane moves on to its next.
+template <typename T>
+__device__ __forceinline__ uint32_t short_key(T v) {
+    const uint32_t u = *reinterpret_cast<const uint16_t*>(&v);
+    if (to_float(v) != to_float(v)) return 0xffffu;
+    return u == 0x8000u ? 0x8000u : u & 0x8000u ? u ^ 0xffffu : u | 0x8000u;
+}
+template <int PER>
+__device__ __forceinline__ void sort_down(uint32_t (&w)[PER]) {
+#pragma unroll
+    for (int size = 1; size < PER; size *= 2)
+#pragma unroll
+        for (int k = size; k >= 1; k /= 2)
+#pragma unroll
+            for (int j = k % size; j + k < PER; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; ++i)
+                    if (i + j + k < PER && (i + j) / (2 * size) == (i + j + k) / (2 * size)) {
+                        const uint32_t a = w[i + j], b = w[i + j + k];
+                        w[i + j] = max(a, b), w[i + j + k] = min(a, b);
+                    }
+}
+template <typename T, int PER>
+__global__ void __launch_bounds__(256) k_route_short(const RouteParams<T> p) {
+    follow_on();
+    const int lane = threadIdx.x & 31;
+    for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < p.rows;
+         row += (int64_t)gridDim.x * 8) {
+        const T* at = p.logits + row * p.ld;
+        uint32_t word[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int g = lane + 32 * i;
+            word[i] = g < p.groups ? short_key(at[g]) << 16 | (0xffffu - g) : 0u;
+        }
+        sort_down(word);
+        uint32_t mine = 0;
+        for (int j = 0; j < p.k; ++j) {
+            const uint32_t top = __reduce_max_sync(0xffffffffu, word[0]);
+            if (lane == j) mine = top;
+            if (word[0] == top) {
+#pragma unroll
+                for (int i = 0; i + 1 < PER; ++i) word[i] = word[i + 1];
+                word[PER - 1] = 0u;
+            }
+        }
+        const uint32_t key = mine >> 16;
+        const uint16_t bits = (uint16_t)(key & 0x8000u ? key ^ 0x8000u : key ^ 0xffffu);
+        const float value = key == 0xffffu ? __uint_as_float(0x7fc00000u)
+                                           : to_float(*reinterpret_cast<const T*>(&bits));
+        const bool some = lane < p.k && value != -INFINITY;  // -inf: not to be chosen
+        finish_route(p, row, value, some ? (int)(0xffffu - (mine & 0xffffu)) : -1);
+    }
+}
+
 // A warp per row; a lane has the values lane, lane + 32, ... A round of the selection is a maximum
-// over the warp and the lowest index that has it, both by one reduction instruction.
+// over the warp and the lowest index that has it, both by one reduction instruction. 16384 x 256, 8
+// choices: 17 us, and 16-bit ones by their words 10; 16384 x 1000 70 us by either.
 template <typename T, int PER>
 __global__ void __launch_bounds__(256) k_route(const RouteParams<T> p) {
     follow_on();
@@ -77,17 +155,43 @@ __global__ void __launch_bounds__(256) k_route(const RouteParams<T> p) {
                 if (first == lane + 32 * i) key[i] = 0u;
             if (lane == j) mine = top, chosen = (int)first;
         }
-        const float value = mine == 0xffffffffu
-                                ? __uint_as_float(0x7fc00000u)
-                                : __uint_as_float(mine & 0x80000000u ? mine ^ 0x80000000u : ~mine);
-        const float largest = __shfl_sync(0xffffffffu, value, 0);
+        const float value = key_value(mine);
         const bool some = lane < p.k && mine != kKeyMasked;  // -inf: not to be chosen
-        const float e = some ? expf(value - largest) : 0.0f;
-        const float sum = warp_sum(e);
-        if (lane < p.k) {
-            p.index[row * p.k + lane] = some ? chosen : -1;
-            p.weights[row * p.k + lane] = some ? e / sum : 0.0f;
+        finish_route(p, row, value, some ? chosen : -1);
+    }
+}
+
+// Few groups: a thread per row, of which it holds all logits (131072 x 8, 2 choices: 22 -> 4 us).
+template <typename T, int PER>
+__global__ void __launch_bounds__(128) k_route_rows(const RouteParams<T> p) {
+    follow_on();
+    for (int64_t row = (int64_t)blockIdx.x * 128 + threadIdx.x; row < p.rows;
+         row += (int64_t)gridDim.x * 128) {
+        const T* at = p.logits + row * p.ld;
+        uint32_t key[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) key[i] = i < p.groups ? order_key(to_float(at[i])) : 0u;
+        int32_t* index = p.index + row * p.k;
+        float* weights = p.weights + row * p.k;
+        float largest = 0.0f, sum = 0.0f;
+        for (int j = 0; j < p.k; ++j) {
+            uint32_t top = key[0];
+            int first = 0;
+#pragma unroll
+            for (int i = 1; i < PER; ++i)
+                if (key[i] > top) top = key[i], first = i;
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (i == first) key[i] = 0u;
+            const float value = key_value(top);
+            if (j == 0) largest = value;
+            const float e = top != kKeyMasked ? expf(value - largest) : 0.0f;
+            index[j] = top != kKeyMasked ? first : -1;
+            weights[j] = e;  // divided by the sum below
+            sum += e;
         }
+        if (sum != 0.0f)  // NaN too
+            for (int j = 0; j < p.k; ++j) weights[j] = index[j] >= 0 ? weights[j] / sum : 0.0f;
     }
 }
 
@@ -135,7 +239,10 @@ __global__ void __launch_bounds__(256) k_route_grad(const RouteGradParams<T> p) 
 // each group; k_place adds up those before its own, then walks its slots again: a slot's rank
 // among the warp's 32 comes from the lanes that match it. One block alone needs no first kernel.
 constexpr int kSortWarps = 16, kSortThreads = 32 * kSortWarps;
-constexpr int64_t kSortAlone = 16384;  // slots that one block sorts by itself
+// groups from which counting takes shared memory's atomics, whose conflicts are few then, for the
+// matching of lanes (1048576 slots in 256 groups 41 -> 25 us)
+constexpr int kAtomicGroups = 32;
+constexpr int64_t kSortAlone = 2048;  // slots that one block sorts by itself
 
 struct SortParams {
     int64_t slots, per_warp;
@@ -171,6 +278,10 @@ __device__ __forceinline__ void count_slots(const SortParams& p, int32_t* hist, 
         }
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
+            if (p.groups >= kAtomicGroups) {  // whole numbers: their order does not matter
+                if (g[i] >= 0) atomicAdd(&own[g[i]], 1);
+                continue;
+            }
             const unsigned same = __match_any_sync(0xffffffffu, g[i]);
             if (g[i] >= 0 && lane == __ffs(same) - 1) own[g[i]] += __popc(same);
             __syncwarp();
@@ -214,7 +325,7 @@ __global__ void __launch_bounds__(kSortThreads) k_place(const SortParams p) {
         const int parts = max(1, kSortThreads / width), step = kSortThreads / parts;
         for (int g = tid % step; g < p.groups; g += step) {
             int before = 0, all = 0;
-#pragma unroll 8
+#pragma unroll 16
             for (int b = tid / step; b < p.blocks; b += parts) {
                 const int c = p.counts[(int64_t)b * p.groups + g];
                 all += c;
@@ -637,7 +748,7 @@ int sort_blocks(const rune_row_groups_args& a) {
     if (slots <= kSortAlone) return 1;
     // a block for 1024 slots at least, and no more counts than every block can add up
     return (int)std::max<int64_t>(
-        1, std::min({(slots + 1023) / 1024, (int64_t)sm_count(a.device),
+        2, std::min({(slots + 1023) / 1024, (int64_t)sm_count(a.device),
                      (int64_t)65536 / a.groups}));
 }
 
@@ -692,10 +803,23 @@ int rune_route(const rune_route_args* args, void* stream_) {
                                    (int)a.groups, (int)a.k,
                                    static_cast<const T*>(a.logits), a.index, a.weights};
             auto go = [&](auto per) {
-                launch(k_route<T, decltype(per)::value>, grid, 256, 0, 0, stream, p);
+                constexpr int PER = decltype(per)::value;
+                if constexpr (sizeof(T) == 2 && PER <= 16)
+                    launch(k_route_short<T, PER>, grid, 256, 0, 0, stream, p);
+                else
+                    launch(k_route<T, PER>, grid, 256, 0, 0, stream, p);
             };
             const int per = (int)((a.groups + 31) / 32);
-            if (per <= 1) go(std::integral_constant<int, 1>());
+            auto rows = [&](auto per_c) {
+                const int64_t blocks = (a.rows + 127) / 128;
+                launch(k_route_rows<T, decltype(per_c)::value>,
+                       (unsigned)std::min<int64_t>(blocks, (int64_t)sm_count(a.device) * 16), 128,
+                       0, 0, stream, p);
+            };
+            if (a.groups <= 8 && a.rows > kRouteRows) rows(std::integral_constant<int, 8>());
+            else if (a.groups <= 16 && a.rows > kRouteRows)
+                rows(std::integral_constant<int, 16>());
+            else if (per <= 1) go(std::integral_constant<int, 1>());
             else if (per <= 2) go(std::integral_constant<int, 2>());
             else if (per <= 4) go(std::integral_constant<int, 4>());
             else if (per <= 8) go(std::integral_constant<int, 8>());

@@ -142,6 +142,21 @@ def test_element_network_is_the_models():
 
 
 @gpu
+@pytest.mark.parametrize("atoms", [0, 1])
+def test_no_atoms_and_one(atoms):
+    torch.manual_seed(4)
+    q, types = torch.randn(atoms, 20, device="cuda"), torch.zeros(atoms, dtype=torch.int32,
+                                                                 device="cuda")
+    for net in (ScalarNetwork(3, 20, 64, 96, 2, experts=6, top_k=3).cuda(),
+                ElementNetwork(3, 20, 30).cuda()):
+        energies = net(q, types)
+        assert energies.shape == (atoms,) and bool(energies.isfinite().all())
+        energies.sum().backward()
+        for name, p in net.named_parameters():
+            assert p.grad is None or bool(p.grad.isfinite().all()), name
+
+
+@gpu
 def test_muon_step_is_its_formula():
     torch.manual_seed(2)
     shapes = [(64, 32), (3, 40, 96), (64, 32), (1, 40, 96)]

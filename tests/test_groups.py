@@ -105,7 +105,8 @@ def weights64(logits, index, masked):
 
 
 ROUTE_SIZES = [(1, 1, 1), (1, 64, 2), (3, 7, 7), (5, 33, 4), (130, 8, 2), (9, 256, 8),
-               (17, 1024, 32), (4, 1000, 1), (2000, 100, 3), (2, 513, 5)]
+               (17, 1024, 32), (4, 1000, 1), (2000, 100, 3), (2, 513, 5), (5000, 8, 2),
+               (4097, 16, 16), (4500, 3, 3), (6000, 11, 1), (0, 5, 2)]
 
 
 @gpu
@@ -130,15 +131,20 @@ def test_route_forward_and_backward(rows, groups, k, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", ALL, ids=str)
-def test_route_ties_masks_and_special_values(dtype):
+@pytest.mark.parametrize("rows", [9, 5000])
+def test_route_ties_masks_and_special_values(dtype, rows):
     inf, nan, low = torch.inf, torch.nan, torch.finfo(dtype).min
-    logits = torch.tensor([
+    table = torch.tensor([
         [1.0, 1.0, 1.0, 1.0, 1.0], [0.0, -0.0, 0.0, -0.0, 0.0], [-inf] * 5,
         [-inf, 2.0, -inf, 1.0, -inf], [low] * 5, [low, -inf, 3.0, low, -inf],
         [1.0, nan, 2.0, nan, 0.0], [inf, 0.0, 1.0, -inf, 2.0], [-1.0, -2.0, -1.0, -3.0, -2.0],
-    ], dtype=dtype, device="cuda", requires_grad=True)
+    ], dtype=dtype, device="cuda")
+    logits = table[torch.arange(rows, device="cuda") % 9].requires_grad_(True)
     index, w = ops.route(logits, 3)
-    assert index.tolist() == [[0, 1, 2], [0, 1, 2], [-1] * 3, [1, 3, -1], [0, 1, 2], [2, 0, 3],
+    repeat = torch.arange(rows, device="cuda") % 9
+    assert torch.equal(index, index[:9][repeat])
+    assert torch.equal(w.nan_to_num(-1.0), w[:9][repeat].nan_to_num(-1.0))
+    assert index[:9].tolist() == [[0, 1, 2], [0, 1, 2], [-1] * 3, [1, 3, -1], [0, 1, 2], [2, 0, 3],
                               [1, 3, 2], [0, 4, 2], [0, 2, 1]]
     third = 3 * [pytest.approx(1 / 3, rel=1e-6)]
     got = w.tolist()
@@ -347,7 +353,7 @@ GROUP_SIZES = [([1], 0, 8, 8), ([0, 0], 3, 16, 8), ([3, 0, 5], 0, 1, 1), ([1] * 
                ([40, 9, 0, 1], 6, 513, 96), ([127, 1, 128, 129, 0], 0, 64, 128),
                ([300, 77, 260], 31, 129, 255), ([64] * 5, 0, 256, 64), ([0, 700, 1, 0], 5, 72, 520),
                ([5] * 100, 0, 40, 24), ([513, 255, 1025], 0, 136, 264), ([0] * 30 + [200], 0, 35, 30),
-               ([2100, 3], 1, 320, 200)]
+               ([2100, 3], 1, 320, 200), ([3000, 1, 2500, 0, 4097], 7, 256, 512)]
 
 
 def per_group(fn, index, groups, *tensors):
