@@ -469,6 +469,8 @@ typedef struct {
     const void* bias;       /* [groups, n] or NULL */
     const int32_t* offsets; /* [groups + 1]; values outside 0 .. rows are taken as the nearer end */
     void* y;                /* [rows, outputs]; zeros behind the last group */
+    float* saved;           /* z for the backward, or NULL: as in rune_linear_args, rows behind the
+                               last group not written */
     void* workspace;
     int64_t workspace_bytes;
 } rune_grouped_linear_args;
@@ -486,6 +488,7 @@ typedef struct {
     const void* bias;
     const int32_t* offsets;
     const void* dy;         /* [rows, outputs]; not read behind the last group */
+    const float* saved;     /* the forward's z; NULL: recomputed from x, weight and bias */
     void* dx;               /* [rows, inputs], zeros behind the last group; or NULL */
     void* dweight;          /* [groups, n, inputs], zeros for groups without rows; or NULL */
     void* dbias;            /* [groups, n], or NULL */

@@ -12,11 +12,12 @@
 //   dW                a product per group over its rows. What lies behind the last row must be
 //                     zeros in both operands (the next group's row may hold an infinity), so each
 //                     group has tensor maps of its own, cut to its rows: k_group_maps writes them.
-// z of an activated layer is computed again in the backward pass: a copy in float32 would cost 8
-// bytes of traffic and 4 of memory a value, for all slots of every layer.
+// z of an activated layer is computed again in the backward pass or read from a float32 copy that the
+// forward saved: the caller's choice, by what each costs.
 
 #include <cmath>
 
+#include "act_grad.cuh"
 #include "tile.cuh"
 
 namespace rune {
@@ -171,6 +172,29 @@ k_group_sums(const SumParams p, const __grid_constant__ MapParams maps) {
     const float sum = joined[0][c] + joined[1][c] + joined[2][c] + joined[3][c];
     if (p.ranges == 1) static_cast<T*>(p.out)[g * p.n + col] = from_float<T>(sum);
     else p.sums[((int64_t)range * p.groups + g) * p.line + col] = sum;
+}
+
+// dz of a range of a group's rows from a saved z, and its columns' sums (in p.sums); p.ld and p.x are
+// of dy
+struct SavedParams {
+    const float* z;
+    int64_t outputs, ld_part, ld_dz;
+    void* dz;
+    int act;
+    bool wide_dy;
+};
+template <bool GATED, typename T>
+__global__ void __launch_bounds__(256, 3)
+k_group_act_grad(const SavedParams q, const SumParams p, const __grid_constant__ MapParams maps) {
+    follow_on();
+    if (maps_here(maps, p.ranges)) return;
+    const int g = blockIdx.y, range = blockIdx.z;
+    const int64_t a = min((int64_t)max(p.offsets[g], 0), p.rows);
+    const int64_t n = max((int64_t)0, min((int64_t)max(p.offsets[g + 1], 0), p.rows) - a);
+    act_grad_rows<GATED, T>(
+        a + n * range / p.ranges, a + n * (range + 1) / p.ranges, q.outputs, q.z, q.ld_part,
+        static_cast<const T*>(p.x), p.ld, q.wide_dy, static_cast<T*>(q.dz), q.ld_dz, q.act,
+        p.sums ? p.sums + ((int64_t)range * p.groups + g) * p.line : nullptr);
 }
 
 // value i of dbias from the sums of the ranges, in order
@@ -432,7 +456,9 @@ void forward(const rune_grouped_linear_args& a, Scratch& ws, cudaStream_t stream
     p.zero_tail = 1;
     p.bias = a.bias;
     p.vec_bias = aligned(a.bias, 16) && a.outputs % 8 == 0;
-    const bool plain = a.activation == RUNE_ACT_NONE && !a.bias;
+    p.z = a.saved, p.ld_part = (a.outputs + 3) / 4 * 4;
+    p.ld_z = (a.gated ? 2 : 1) * p.ld_part;
+    const bool plain = a.activation == RUNE_ACT_NONE && !a.bias && !a.saved;
     run_rows(a.gated ? kGated : plain ? kPlain : kForward, g, p, true, stream);
 }
 
@@ -505,7 +531,7 @@ bool run_weights(const rune_grouped_linear_grad_args& a, const Matrix& dz, const
     const JoinParams j{a.offsets, a.rows, m, n, (int)a.groups, d.tiles_m, d.tiles_n, d.high, p.bn,
                        p.ranges, lanes, n % 4 == 0 && aligned(a.dweight, 8), d.parts, a.dweight};
     const int64_t rows_y = d.high * p.bn / 4 * lanes / kJoinThreads;
-    const int64_t more = sum.ranges > 1 ? (a.groups * sum.n + rows_y * kJoinThreads - 1) /
+    const int64_t more = sum.sums ? (a.groups * sum.n + rows_y * kJoinThreads - 1) /
                                               (rows_y * kJoinThreads) : 0;
     launch(k_join_parts<T>, dim3((unsigned)(each * a.groups + more), (unsigned)rows_y),
            kJoinThreads, 0, 0, stream, j, sum);
@@ -518,8 +544,9 @@ void backward(const rune_grouped_linear_grad_args& a, Scratch& ws, cudaStream_t 
     const bool half = a.dtype == RUNE_F16;
     Matrix x{a.x, a.rows, a.inputs, a.x_stride};
     Weights w{{a.weight, a.groups * n_all, a.inputs, a.weight_stride}, n_all};
-    if (!plain || a.dweight) x = readable(x, 2, ws, stream);
-    if (!plain || a.dx) w.all = readable(w.all, 2, ws, stream);
+    const bool recompute = !plain && !a.saved;
+    if (recompute || a.dweight) x = readable(x, 2, ws, stream);
+    if (recompute || a.dx) w.all = readable(w.all, 2, ws, stream);
     RowProduct g;
     g.groups = a.groups, g.offsets = a.offsets;
     g.device = a.device, g.dtype = a.dtype;
@@ -533,6 +560,8 @@ void backward(const rune_grouped_linear_grad_args& a, Scratch& ws, cudaStream_t 
     } else {
         dz.ld = pad16(n_all, 2);
         dz.p = ws.take<uint16_t>(a.rows * dz.ld);
+    }
+    if (recompute) {
         g.a = x, g.w = w, g.k = a.inputs;
         p.n = a.outputs;
         p.act = a.activation;
@@ -545,27 +574,39 @@ void backward(const rune_grouped_linear_grad_args& a, Scratch& ws, cudaStream_t 
         sum.high = run_rows(mode, g, p, false, stream);
         sum.each = sum.high / 32;  // one a warp
     }
-    if (a.dbias) {
-        const int64_t parts = plain ? a.rows : line_bound(a.rows, a.groups, sum.high) * sum.each;
-        if (!plain) sum.parts = ws.take<float>(parts * n_all);
+    if (a.dbias || (!plain && a.saved)) {
+        const int64_t parts =
+            recompute ? line_bound(a.rows, a.groups, sum.high) * sum.each : a.rows;
+        if (recompute) sum.parts = ws.take<float>(parts * n_all);
         // 64 parts a range where groups are alike
         const int64_t mean = parts / a.groups;
-        sum.ranges = mean < 256 ? 1 : (int)std::min<int64_t>(256, mean / 64);
+        sum.ranges = mean < (a.saved ? 128 : 256) ? 1 : (int)std::min<int64_t>(256, mean / 64);
         sum.line = (n_all + 3) / 4 * 4;
-        if (sum.ranges > 1) sum.sums = ws.take<float>(sum.ranges * a.groups * sum.line);
+        if (a.dbias && (sum.ranges > 1 || a.saved))
+            sum.sums = ws.take<float>(sum.ranges * a.groups * sum.line);
     }
     Depth depth;
     if (a.dweight) depth = plan_weights(a, dz, x, ws);
     if (ws.sizing()) return;
-    if (!plain) {
+    if (recompute) {
         p.colsum = sum.parts;
         run_rows(mode, g, p, true, stream);
     }
     auto typed = [&](auto t) {
         using T = decltype(t);
-        if (a.dbias) {
-            const dim3 grid((unsigned)((n_all + 63) / 64), (unsigned)a.groups,
-                            (unsigned)(sum.ranges + (a.dweight ? 1 : 0)));
+        const unsigned slices = sum.ranges + (a.dweight ? 1 : 0);
+        if (!plain && a.saved) {
+            const SavedParams q{a.saved, a.outputs, (a.outputs + 3) / 4 * 4, dz.ld,
+                                const_cast<void*>(dz.p), a.activation,
+                                aligned(a.dy, 8) && a.dy_stride % 4 == 0};
+            const dim3 grid((unsigned)((a.outputs + kColumns - 1) / kColumns), (unsigned)a.groups,
+                            slices);
+            if (a.gated)
+                launch(k_group_act_grad<true, T>, grid, 256, 0, 0, stream, q, sum, depth.maps);
+            else
+                launch(k_group_act_grad<false, T>, grid, 256, 0, 0, stream, q, sum, depth.maps);
+        } else if (a.dbias) {
+            const dim3 grid((unsigned)((n_all + 63) / 64), (unsigned)a.groups, slices);
             if (plain) launch(k_group_columns<T>, grid, 256, 0, 0, stream, sum, depth.maps);
             else launch(k_group_sums<T>, grid, 256, 0, 0, stream, sum, depth.maps);
         } else if (a.dweight) {
@@ -585,7 +626,7 @@ void backward(const rune_grouped_linear_grad_args& a, Scratch& ws, cudaStream_t 
             run_rows(kPlain, d, q, true, stream);
         }
         const bool joined = a.dweight && run_weights<T>(a, dz, x, depth, sum, stream);
-        if (sum.ranges > 1 && !joined)
+        if (sum.sums && !joined)
             launch(k_join_sums<T>, (unsigned)((a.groups * n_all + 255) / 256), 256, 0, 0, stream,
                    sum);
     };
@@ -609,6 +650,7 @@ void check_args(const Args& a) {
     require(a.rows == 0 || (a.x && a.weight && a.offsets), "null argument");
     require_aligned({a.x, a.weight, a.bias}, 2);
     require_aligned({a.offsets}, 4);
+    require(aligned(a.saved, 16), "saved is not 16-byte aligned");
 }
 
 template <typename Args>

@@ -646,7 +646,7 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
                         float v[16];
                         Two z[8];
                         Bias<T> bias;
-                        bias.load(p, at, left - half * 16);
+                        bias.load(p, at, left - half * 16, bias_at);
                         tc::tmem_ld16(acc + c + part * width + half * 16, v);
                         finish_z<T, FP8>(v, z, bias, p, at, left - half * 16, xs);
 #pragma unroll

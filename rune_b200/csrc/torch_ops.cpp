@@ -17,6 +17,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <initializer_list>
 #include <sstream>
 #include <stdexcept>
@@ -57,6 +58,7 @@ struct Api {
 } api;
 PyObject* g_raise = nullptr;        // runtime.library.check's exceptions by status
 int64_t g_recompute_inputs = 0;     // rune_b200.ops.RECOMPUTE_INPUTS
+int64_t g_rows_to_inputs = 0;       // rune_b200.ops.ROWS_TO_INPUTS
 
 // A status of the library other than RUNE_OK.
 struct Failure : std::runtime_error {
@@ -666,8 +668,8 @@ Tensor from_groups(const Tensor& y, Groups g, Tensor weights) {
 }
 
 // weight: the groups' matrices one below the other
-Tensor grouped_call(const Tensor& x, const Tensor& weight, const Tensor& bias,
-                    const Tensor& offsets, int64_t act, bool gated) {
+LinearOut grouped_call(const Tensor& x, const Tensor& weight, const Tensor& bias,
+                       const Tensor& offsets, int64_t act, bool gated, bool want_z) {
     const Rows rx(x), rw(weight);
     rune_grouped_linear_args a{};
     a.rows = x.size(0), a.inputs = x.size(1), a.groups = offsets.size(0) - 1;
@@ -675,16 +677,20 @@ Tensor grouped_call(const Tensor& x, const Tensor& weight, const Tensor& bias,
     a.x_stride = rx.ld, a.weight_stride = rw.ld;
     a.device = x.get_device(), a.dtype = code_of(x.scalar_type());
     a.activation = (int32_t)act, a.gated = gated;
-    Tensor y = empty_like_type(x, {a.rows, a.outputs}, x.scalar_type());
+    LinearOut o;
+    o.y = empty_like_type(x, {a.rows, a.outputs}, x.scalar_type());
+    if (want_z)
+        o.z = empty_like_type(x, {a.rows, gated ? 2 : 1, (a.outputs + 3) / 4 * 4},
+                              ScalarType::Float);
     a.x = rx.p(), a.weight = rw.p(), a.bias = ptr(bias);
-    a.offsets = (const int32_t*)ptr(offsets), a.y = ptr(y);
+    a.offsets = (const int32_t*)ptr(offsets), a.y = ptr(o.y), a.saved = (float*)ptr(o.z);
     int status = api.grouped(&a, stream_of(x));
     if (status == RUNE_ERR_RETRY) {  // this call needs scratch
         const Tensor ws = scratch(api.grouped_ws, a, x);
         status = api.grouped(&a, stream_of(x));
     }
     check(status);
-    return y;
+    return o;
 }
 
 struct GroupedFn : torch::autograd::Function<GroupedFn> {
@@ -694,10 +700,16 @@ struct GroupedFn : torch::autograd::Function<GroupedFn> {
         const Tensor bias = bias_.value_or(Tensor());
         const Tensor x = in_place(x_);
         const Tensor weight = in_place(weight_.reshape({-1, weight_.size(2)}));
-        ctx->save_for_backward({x, weight, bias, offsets});
+        // recomputed, z costs a product of `inputs` and the weights of all groups that have rows
+        const int64_t inputs = x.size(1), rows = x.size(0);
+        const int64_t met = std::min(rows, offsets.size(0) - 1);
+        const bool save = act != RUNE_ACT_NONE &&
+                          (inputs > g_recompute_inputs || rows * g_rows_to_inputs < met * inputs);
+        LinearOut o = grouped_call(x, weight, bias, offsets, act, gated, save);
+        ctx->save_for_backward({x, weight, bias, offsets, o.z});
         ctx->saved_data["act"] = act;
         ctx->saved_data["gated"] = gated;
-        return grouped_call(x, weight, bias, offsets, act, gated);
+        return o.y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         return in_backward([&] { return gradients(ctx, grads); });
@@ -706,6 +718,7 @@ struct GroupedFn : torch::autograd::Function<GroupedFn> {
         first_order_only(grads);
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &offsets = saved[3];
+        const Tensor& z = saved[4];
         const Rows rx(x), rw(weight), dy(grads[0]);
         rune_grouped_linear_grad_args a{};
         a.rows = x.size(0), a.inputs = x.size(1), a.groups = offsets.size(0) - 1;
@@ -723,6 +736,7 @@ struct GroupedFn : torch::autograd::Function<GroupedFn> {
             db = empty_like_type(bias, bias.sizes(), bias.scalar_type());
         a.x = rx.p(), a.weight = rw.p(), a.bias = ptr(bias);
         a.offsets = (const int32_t*)ptr(offsets), a.dy = dy.p();
+        a.saved = (const float*)ptr(z);
         a.dx = ptr(dx), a.dweight = ptr(dw), a.dbias = ptr(db);
         if (dx.defined() || dw.defined() || db.defined()) {
             const Tensor ws = scratch(api.grouped_bwd_ws, a, x);
@@ -758,7 +772,7 @@ Tensor grouped(const Tensor& x, const Tensor& weight, Tensor bias, Groups g, int
     if (at::GradMode::is_enabled() &&
         (x.requires_grad() || weight.requires_grad() || wants_grad(bias)))
         return GroupedFn::apply(x, weight, given(bias), g.offsets, act, gated);
-    return grouped_call(x, weight.reshape({-1, x.size(1)}), bias, g.offsets, act, gated);
+    return grouped_call(x, weight.reshape({-1, x.size(1)}), bias, g.offsets, act, gated, false).y;
 }
 
 // -------------------------------------------------------------------------------- updates
@@ -976,11 +990,13 @@ PyObject* py_orthogonalize(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
-// bind(addresses of the entry points in Api's order, raise(status, message), recompute inputs)
+// bind(addresses of the entry points in Api's order, raise(status, message), recompute inputs, rows to
+// inputs)
 PyObject* py_bind(PyObject*, PyObject* args) {
     PyObject *list, *raise;
-    long long inputs;
-    if (!PyArg_ParseTuple(args, "O!OL", &PyTuple_Type, &list, &raise, &inputs)) return nullptr;
+    long long inputs, rows;
+    if (!PyArg_ParseTuple(args, "O!OLL", &PyTuple_Type, &list, &raise, &inputs, &rows))
+        return nullptr;
     constexpr Py_ssize_t kEntries = sizeof(Api) / sizeof(void*);
     if (PyTuple_GET_SIZE(list) != kEntries) {
         PyErr_SetString(PyExc_ValueError, "wrong number of entry points");
@@ -998,7 +1014,7 @@ PyObject* py_bind(PyObject*, PyObject* args) {
     memcpy(static_cast<void*>(&api), entry, sizeof(api));
     Py_INCREF(raise);
     Py_XSETREF(g_raise, raise);
-    g_recompute_inputs = inputs;
+    g_recompute_inputs = inputs, g_rows_to_inputs = rows;
     Py_RETURN_NONE;
 }
 

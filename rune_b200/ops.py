@@ -50,6 +50,13 @@ _OUT = {None: -1, torch.float16: L.RUNE_F16, torch.bfloat16: L.RUNE_BF16}
 # 248 / 243 (424 / 432), 2048 inputs 428 / 379 (770 / 682).
 RECOMPUTE_INPUTS = 1024
 
+# A grouped layer also saves z where its groups are small: where ``rows * ROWS_TO_INPUTS`` is less than
+# ``groups * inputs``, reading all groups' weights once more takes longer than z, written and read.
+# B200, training step of gated layers, recomputed / saved, us: 61 groups of 1024 -> 2 x 1408, 2000 rows
+# 284 / 232, 8001 rows 342 / 303, 32000 rows 721 / 670; 32 groups of 512 -> 2 x 512, 4096 rows 68 / 66,
+# 8192 rows 88 / 86, 16384 rows 121 / 131.
+ROWS_TO_INPUTS = 2
+
 # Coefficients a, b, c of the quintic a x + b x^3 + c x^5 that ``orthogonalize`` iterates: steep at
 # zero, so that five steps bring singular values from 0.01 and up to between 0.7 and 1.2.
 NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
@@ -80,7 +87,7 @@ def _native():
                    lib.rune_orthogonalize, lib.rune_orthogonalize_workspace,
                    lib.rune_last_error)
         module.bind(tuple(ctypes.cast(f, ctypes.c_void_p).value for f in entries), L.fail,
-                    RECOMPUTE_INPUTS)
+                    RECOMPUTE_INPUTS, ROWS_TO_INPUTS)
         _BINDING = module
     return _BINDING
 

@@ -173,7 +173,7 @@ class GroupedLinearArgs(ctypes.Structure):
         ("x_stride", c_int64), ("weight_stride", c_int64), ("device", c_int32),
         ("dtype", c_int32), ("activation", c_int32), ("gated", c_int32), ("x", c_void_p),
         ("weight", c_void_p), ("bias", c_void_p), ("offsets", c_void_p), ("y", c_void_p),
-        ("workspace", c_void_p), ("workspace_bytes", c_int64),
+        ("saved", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_int64),
     ]
 
 
@@ -183,8 +183,8 @@ class GroupedLinearGradArgs(ctypes.Structure):
         ("x_stride", c_int64), ("weight_stride", c_int64), ("dy_stride", c_int64),
         ("device", c_int32), ("dtype", c_int32), ("activation", c_int32), ("gated", c_int32),
         ("x", c_void_p), ("weight", c_void_p), ("bias", c_void_p), ("offsets", c_void_p),
-        ("dy", c_void_p), ("dx", c_void_p), ("dweight", c_void_p), ("dbias", c_void_p),
-        ("workspace", c_void_p), ("workspace_bytes", c_int64),
+        ("dy", c_void_p), ("saved", c_void_p), ("dx", c_void_p), ("dweight", c_void_p),
+        ("dbias", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_int64),
     ]
 
 
