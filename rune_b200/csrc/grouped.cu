@@ -8,7 +8,8 @@
 //   forward, dz, dx   tiles of the rows of each group. A tile that reaches past its group's end
 //                     reads rows of the next, whose results no one stores: boxes of whole rows leave
 //                     by TMA, the last ones by the lanes. Weights are a 3-D map, zeros beyond a
-//                     group's matrix, since dx contracts over its rows.
+//                     group's matrix, since dx contracts over its rows. Or, turned round, tiles of
+//                     outputs by as many rows as there are, which wastes less at the groups' ends.
 //   dW                a product per group over its rows. What lies behind the last row must be
 //                     zeros in both operands (the next group's row may hold an infinity), so each
 //                     group has tensor maps of its own, cut to its rows: k_group_maps writes them.
@@ -312,6 +313,18 @@ Plan plan_rows(int64_t rows, int64_t groups, int64_t n_cols, int kblocks, bool g
     return best;
 }
 
+// Whether a product of rows by group is sooner done turned round (kRowsAcross), where the lines that
+// the groups' ends leave part empty count: contractions that hide the epilogue, groups of some rows
+// but not of very many, outputs that fill their tiles. B200, kRowGroups / kRowsAcross, us:
+//   32768 x 2048 -> 4096, 64 groups, gelu 463 / 420    16000 x 512 -> 512, 16 groups 20.5 / 18.4
+//   20000 x 4096 -> 1024, 128 groups      219 / 213    200000 x 1024 -> 256, 8 groups  96 /  98
+//   2000 x 2816 -> 1024, 61 groups         66 /  70    100 x 4096 -> 4096, 16 groups   90 /  98
+bool across_pays(int64_t rows, int64_t groups, int64_t n, int kblocks) {
+    const int64_t met = std::min(rows, groups);
+    return kblocks >= 8 && rows >= 96 * met && rows <= 4096 * met &&
+           (n + 255) / 256 * 256 * 4 <= n * 5;
+}
+
 // Tile and pairing of the groups' products over their rows. Either a tile is a block's own (splits
 // 1), and the last block's tiles, of a group of perhaps three times the mean, end late; or the
 // k-blocks of all groups divide into `splits` equal ranges, for the traffic and the launch of a join.
@@ -424,8 +437,47 @@ int run_rows(const RowProduct& g, TileParams p, bool launch_it, cudaStream_t str
     return high;
 }
 
+// The same turned round, for kForward and kPlain.
+template <int MODE, typename T>
+void run_across(const RowProduct& g, TileParams p, cudaStream_t stream) {
+    const int sms = sm_count(g.device);
+    const uint32_t fixed = kFixedSmem<MODE> + table_bytes(g.groups);
+    p.kblocks = p.kb_per_split = (int)((g.k + 63) / 64), p.splits = 1;
+    p.m = p.m_all = g.a.rows;
+    p.groups = (int)g.groups;
+    p.offsets = g.offsets;
+    p.bias_step = p.n;
+    p.bn = 2 * kBM, p.stages = ring_stages(true, p.bn, fixed);
+    p.tiles_n = (int)((p.n + 2 * kBM - 1) / (2 * kBM));
+    p.by_tiles = make_divisor((unsigned)p.tiles_n);
+    p.by_group = make_divisor(kGroup * (unsigned)p.tiles_n);
+    p.a_mn = g.w_mn;
+    p.idesc = operand_idesc(g.dtype == RUNE_BF16 ? 1 : 0, g.w_mn, false, 2 * kBM, 0);  // and N
+    p.flag = wait_flag(g.device);
+    p.polls = wait_polls();
+    const CUtensorMap a = g.w.map(g.groups, g.w_mn ? 64 : kBM);
+    const CUtensorMap b = make_map(g.a, 2, 16), whole = make_map(g.a, 2, kBM);
+    const CUtensorMap o = p.tma_out ? make_out_map(p.out, p.m_all, p.n, p.ld_out) : a;
+    const int64_t work = line_bound(p.m_all, g.groups, 2 * kBM) * p.tiles_n;
+    require(work < (1LL << 31) - 1024, "too many tiles");
+    launch_blocks<MODE, kRowsAcross, T, false, true>(a, b, o, whole, p, work, fixed, sms, g.device,
+                                                     stream);
+}
+
 int run_rows(int mode, const RowProduct& g, const TileParams& p, bool launch_it,
              cudaStream_t stream) {
+    const int kblocks = (int)((g.k + 63) / 64);
+    if (launch_it && (mode == kForward || mode == kPlain) &&
+        across_pays(g.a.rows, g.groups, p.n, kblocks)) {
+        auto go = [&](auto t) {
+            using T = decltype(t);
+            if (mode == kPlain) run_across<kPlain, T>(g, p, stream);
+            else run_across<kForward, T>(g, p, stream);
+        };
+        if (g.dtype == RUNE_F16) go(__half());
+        else go(__nv_bfloat16());
+        return 0;
+    }
     auto typed = [&](auto t) {
         using T = decltype(t);
         switch (mode) {

@@ -28,6 +28,7 @@ enum Mode {
 enum Kind {
     kWhole,        // one product
     kRowGroups,    // the rows of A by group, each with its own matrix B (and bias)
+    kRowsAcross,   // the same turned round: the group's matrix is A, its rows are B
     kDepthGroups,  // the contraction by group: a product of its own for the rows of each
     kDepthRanges,  // the same in parts: the k-blocks of all groups in equal ranges
     kBatch         // a stack of products
@@ -90,6 +91,7 @@ struct TileParams {
 
 struct TileShared {
     unsigned long long full[kMaxStages], empty[kMaxStages];
+    unsigned bytes[kMaxStages];  // that this block's copies into the stage bring
     unsigned long long acc_full[2], acc_empty[2], drained;
     uint32_t tmem;
     int fail;
@@ -127,6 +129,11 @@ __device__ __forceinline__ Tile tile_of(const TileParams& p, unsigned w) {
     return t;
 }
 
+// rows of a kRowsAcross tile as the tensor core's N: halves of sixteens
+__device__ __forceinline__ int rows_across(const Tile& t) {
+    return min(2 * kBM, (t.row_end - t.row0 + 31) / 32 * 32);
+}
+
 // A value that all lanes of a converged warp have, in a uniform register, where a reduction leaves
 // it: what comes from shared memory would stay in every lane's registers, and the epilogues have none
 // left (gated 221184 x 256 -> 2 x 512, dz: 330 us with 124 bytes spilled).
@@ -134,8 +141,11 @@ __device__ __forceinline__ int uniform(int v) { return (int)__reduce_or_sync(0xf
 
 // The tiles of one launch in the order in which a block (or pair) takes them, and the range of k of
 // each. Of groups, whose sizes only the GPU knows, a table in shared memory: rows[g], the groups'
-// first rows, and lines[g], before group g the number of lines of tiles (kRowGroups) or of k-blocks
+// first rows, and lines[g], before group g the number of lines of tiles (by rows) or of k-blocks
 // (kDepthRanges).
+//   kRowsAcross    tiles of 256 outputs and up to 256 of a group's rows, rounded up to 32: a line's
+//                  cost goes with its rows, where kRowGroups' last line of a group costs a whole
+//                  one.
 //   kDepthRanges   the k-blocks of all groups, one after the other, in equal ranges. An item is a
 //                  range of one tile of every group, and leaves a part for each group that it
 //                  meets: part (range + group) tiles + tile, since along the k-blocks each part
@@ -174,7 +184,7 @@ struct Schedule {
                 end = tiles * p.groups;
             } else {
                 if (threadIdx.x < 32) {
-                    constexpr int kLine = KIND == kRowGroups ? kTileRows : 64;
+                    constexpr int kLine = by_depth(KIND) ? 64 : kTileRows;
                     int before = 0;
                     for (int g0 = 0; g0 < p.groups; g0 += 32) {
                         const int g = g0 + threadIdx.x;
@@ -194,7 +204,7 @@ struct Schedule {
                 }
                 __syncthreads();
                 const unsigned all = (unsigned)uniform(lines[p.groups]);
-                if constexpr (KIND == kRowGroups) {
+                if constexpr (KIND == kRowGroups || KIND == kRowsAcross) {
                     end = all * p.tiles_n;
                 } else {
                     end = all * tiles;
@@ -249,7 +259,7 @@ struct Schedule {
         if constexpr (KIND == kWhole) {
             t = tile_of(p, w);
             t.row_end = (int)p.m;
-        } else if constexpr (KIND == kRowGroups) {
+        } else if constexpr (KIND == kRowGroups || KIND == kRowsAcross) {
             const int line = (int)p.by_tiles.quotient(w);  // by the tiles of a line
             const int g = group_at(line);
             const unsigned first = uniform(lines[g]), n = uniform(lines[g + 1]) - first;
@@ -258,7 +268,7 @@ struct Schedule {
             t.nt = in / high;
             const int mt = part * kGroup + (in - t.nt * high);
             t.split = 0, t.z = g, t.empty = false;
-            t.row0 = uniform(rows[g]) + mt * kTileRows + rank * kBM;
+            t.row0 = uniform(rows[g]) + mt * kTileRows + (KIND == kRowGroups ? rank * kBM : 0);
             t.row_end = uniform(rows[g + 1]);
             t.mt = ((int)first + mt) * (kTileRows / kBM) + rank;
             return t;
@@ -784,13 +794,73 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
     if (share * 32 >= end) release();  // no columns here
 }
 
+// The same of kRowsAcross: a lane holds an output, and its columns are rows of the group. Values turn
+// as they enter the buffer, column by column.
+template <int MODE, typename T, typename Wait, typename Release>
+__device__ __forceinline__ void epilogue_across(const TileParams& p, const Tile& t, int rank,
+                                                uint32_t acc, const Stage& st, int warp,
+                                                const CUtensorMap* out_map, Wait&& wait,
+                                                Release&& release) {
+    const int quarter = warp & 3, share = warp >> 2, lane = st.lane;
+    const int f0 = t.nt * 2 * kBM + rank * kBM + quarter * 32;
+    const int rows = min(2 * kBM, t.row_end - t.row0), left = (int)p.n - f0;
+    float bias = 0.0f;
+    if (MODE == kForward && p.bias && lane < left)
+        bias = to_float(static_cast<const T*>(p.bias)[t.z * (int)p.bias_step + f0 + lane]);
+    if (!wait()) return;
+    for (int c = share * 32; c < rows; c += 128) {
+        if (lane == 0) bulk_store_read();
+        __syncwarp();
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+            float v[16];
+            Two z[8];
+            tc::tmem_ld16(acc + c + half * 16, v);
+            if (half == 1 && c + 128 >= rows) release();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                z[j] = two(v[2 * j], v[2 * j + 1]);
+                if (MODE == kForward) z[j] = z[j] + two(bias);
+            }
+            if constexpr (MODE == kForward) {
+                if (p.z && lane < left) {
+                    float* to = p.z + (int64_t)(t.row0 + c + half * 16) * p.ld_z + f0 + lane;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        float a, b;
+                        split(z[j / 2], a, b);
+                        if (c + half * 16 + j < rows) to[j * p.ld_z] = j % 2 ? b : a;
+                    }
+                }
+                with_activation(p.act, [&](auto a) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) z[j] = act_value<decltype(a)::value>(z[j]);
+                });
+            }
+            put_column<T>(st, half, z);
+        }
+        const int part = min(32, rows - c);
+        const bool tma = p.tma_out && part == 32;
+        if (tma) tc::fence_async_smem();
+        __syncwarp();
+        if (!tma) {
+            store_part<T>(st.base, static_cast<T*>(p.out) + (int64_t)(t.row0 + c) * p.ld_out + f0,
+                          p.ld_out, part, left, p.tma_out);
+        } else if (lane == 0 && left > 0) {
+            bulk_store(out_map, st.base, f0, t.row0 + c);
+            bulk_store_commit();
+        }
+        __syncwarp();
+    }
+    if (share * 32 >= rows) release();  // no rows here
+}
+
 // After a wait gave up: lets what is in flight land (bounded) before the blocks' memory goes. The
 // copies of both blocks count on the even one's barriers; a stage that only one of them had filled
 // when the other gave up gets the other's part from here. Not inlined: among the kernels' own code
 // it cost the gated forward 3 % (110592 x 256 -> 512 65.6 against 63.7 us).
 template <bool PAIR>
-__device__ __noinline__ void drain(TileShared* sh, unsigned* flag, int stages,
-                                   uint32_t stage_bytes) {
+__device__ __noinline__ void drain(TileShared* sh, unsigned* flag, int stages) {
     using namespace tc;
     const int rank = PAIR ? (int)cluster_rank() : 0, warp = threadIdx.x >> 5;
     const volatile int* fail = &sh->fail;
@@ -801,8 +871,9 @@ __device__ __noinline__ void drain(TileShared* sh, unsigned* flag, int stages,
         const int issued = max(mine, theirs);
         for (int i = max(0, issued - stages); i < issued; ++i) {
             const uint32_t bar = smem_u32(&sh->full[i % stages]);
-            if (i >= theirs) mbar_complete_tx(bar, stage_bytes);
-            if (i >= mine) mbar_expect_tx(bar, stage_bytes);
+            if (i >= theirs) mbar_complete_tx(bar, sh->bytes[i % stages]);
+            if (i >= mine)
+                mbar_expect_tx(bar, peer_word(peer_address(smem_u32(&sh->bytes[i % stages]), 1)));
             mbar_wait(bar, (i / stages) & 1);
         }
     }
@@ -844,6 +915,7 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
         for (int s = 0; s < p.stages; ++s) {
             mbar_init(smem_u32(&sh->full[s]), 1);
             mbar_init(smem_u32(&sh->empty[s]), 1);
+            sh->bytes[s] = stage_bytes;
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(smem_u32(&sh->acc_full[b]), 1);
@@ -918,7 +990,27 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
                 }
                 const uint32_t bar = full0 + (uint32_t)st * 8;
                 const uint32_t a = smem_u32(smem) + (uint32_t)st * stage_bytes, b = a + kAStage;
-                if (one) {
+                if constexpr (KIND == kRowsAcross) {
+                    // this block's outputs of the matrix, and its half of the rows
+                    const int f0 = t.nt * 2 * kBM + rank * kBM;
+                    const int half = rows_across(t) / 2, r0 = t.row0 + rank * half;
+                    if (one) {
+                        sh->bytes[st] = kAStage + half * kLineBytes;
+                        if (rank == 0) mbar_expect_tx(smem_u32(&sh->full[st]), 2 * sh->bytes[st]);
+                        if (p.a_mn) {
+                            load3(a, &map_a, f0, kb * 64, t.z, bar);
+                            load3(a + kMnChunk, &map_a, f0 + 64, kb * 64, t.z, bar);
+                        } else {
+                            load3(a, &map_a, kb * 64, f0, t.z, bar);
+                        }
+                        if (half == kBM) {
+                            load(b, &map_o2, kb * 64, r0, bar);  // in one box
+                        } else {
+                            for (int i = 0; i < half; i += 16)
+                                load(b + i * kLineBytes, &map_b, kb * 64, r0 + i, bar);
+                        }
+                    }
+                } else if (one) {
                     if (!PAIR || rank == 0)
                         mbar_expect_tx(smem_u32(&sh->full[st]), (PAIR ? 2 : 1) * stage_bytes);
                     const int x = kb * (FP8 ? 128 : 64);
@@ -977,6 +1069,9 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
             }
             fence_after_sync();
             const uint32_t acc = tmem + buf * 256;
+            uint32_t idesc = p.idesc;
+            if constexpr (KIND == kRowsAcross)
+                idesc |= (uint32_t)(rows_across(plan.tile(w)) >> 3) << 17;
             for (int kb = kb0; kb < kb1; ++kb) {
                 ok = mbar_wait(smem_u32(&sh->full[st]), parity, p.polls) && !*fail;
                 if (!__all_sync(0xffffffffu, ok)) {
@@ -990,7 +1085,7 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
                     for (int k = 0; k < 4; ++k) {
                         const bool more = kb > kb0 || k > 0;
                         mma<FP8, PAIR>(acc, desc_a + at + k * step_a, desc_b + at + k * step_b,
-                                       p.idesc, more);
+                                       idesc, more);
                     }
                     commit(&sh->empty[st]);
                 }
@@ -1021,27 +1116,32 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
         for (unsigned w = plan.begin; w < plan.end && ok; w = plan.next(w), ++n_tile) {
             const Tile t = plan.tile(w);
             const int b = n_tile & 1, round = n_tile >> 1;
-            epilogue<MODE, KIND, T, FP8>(
-                p, t, tmem + b * 256 + quarter, st, st2, warp, &map_o, &map_o2,
-                [&] {
-                    ok = mbar_wait(smem_u32(&sh->acc_full[b]), round & 1, p.polls) && !*fail;
-                    ok = __all_sync(0xffffffffu, ok);
-                    fence_after_sync();
-                    return ok;
-                },
-                [&] {
-                    fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if constexpr (PAIR)
-                            mbar_arrive_peer(peer_address(smem_u32(&sh->acc_empty[b]), 0));
-                        else
-                            mbar_arrive(smem_u32(&sh->acc_empty[b]));
-                    }
-                    __syncwarp();
-                });
+            auto wait = [&] {
+                ok = mbar_wait(smem_u32(&sh->acc_full[b]), round & 1, p.polls) && !*fail;
+                ok = __all_sync(0xffffffffu, ok);
+                fence_after_sync();
+                return ok;
+            };
+            auto release = [&] {
+                fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (PAIR)
+                        mbar_arrive_peer(peer_address(smem_u32(&sh->acc_empty[b]), 0));
+                    else
+                        mbar_arrive(smem_u32(&sh->acc_empty[b]));
+                }
+                __syncwarp();
+            };
+            if constexpr (KIND == kRowsAcross)
+                epilogue_across<MODE, T>(p, t, rank, tmem + b * 256 + quarter, st, warp, &map_o,
+                                         wait, release);
+            else
+                epilogue<MODE, KIND, T, FP8>(p, t, tmem + b * 256 + quarter, st, st2, warp, &map_o,
+                                             &map_o2, wait, release);
         }
-        if constexpr (KIND == kRowGroups && (MODE == kForward || MODE == kGated || MODE == kPlain)) {
+        if constexpr ((KIND == kRowGroups || KIND == kRowsAcross) &&
+                      (MODE == kForward || MODE == kGated || MODE == kPlain)) {
             // the rows that no group has
             if (p.zero_tail && ok) {
                 const int64_t from = plan.rows[p.groups], n = (p.m_all - from) * p.n;
@@ -1061,7 +1161,7 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
     if constexpr (PAIR)
         failed = failed || peer_word(peer_address(smem_u32(&sh->fail), rank ^ 1)) != 0;
     if (failed) {
-        drain<PAIR>(sh, p.flag, p.stages, stage_bytes);
+        drain<PAIR>(sh, p.flag, p.stages);
     }
     fence_before_sync();
     if constexpr (PAIR) cluster_sync();

@@ -353,7 +353,8 @@ GROUP_SIZES = [([1], 0, 8, 8), ([0, 0], 3, 16, 8), ([3, 0, 5], 0, 1, 1), ([1] * 
                ([40, 9, 0, 1], 6, 513, 96), ([127, 1, 128, 129, 0], 0, 64, 128),
                ([300, 77, 260], 31, 129, 255), ([64] * 5, 0, 256, 64), ([0, 700, 1, 0], 5, 72, 520),
                ([5] * 100, 0, 40, 24), ([513, 255, 1025], 0, 136, 264), ([0] * 30 + [200], 0, 35, 30),
-               ([2100, 3], 1, 320, 200), ([3000, 1, 2500, 0, 4097], 7, 256, 512)]
+               ([2100, 3], 1, 320, 200), ([97, 300, 255, 256, 1, 33, 600], 9, 520, 504),
+               ([129, 0, 640, 225], 3, 1030, 235), ([3000, 1, 2500, 0, 4097], 7, 256, 512)]
 
 
 def per_group(fn, index, groups, *tensors):
