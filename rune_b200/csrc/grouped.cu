@@ -630,9 +630,10 @@ void backward(const rune_grouped_linear_grad_args& a, Scratch& ws, cudaStream_t 
         const int64_t parts =
             recompute ? line_bound(a.rows, a.groups, sum.high) * sum.each : a.rows;
         if (recompute) sum.parts = ws.take<float>(parts * n_all);
-        // 64 parts a range where groups are alike
-        const int64_t mean = parts / a.groups;
-        sum.ranges = mean < (a.saved ? 128 : 256) ? 1 : (int)std::min<int64_t>(256, mean / 64);
+        // 64 parts a range where groups are alike, of dz from a saved z 16 rows (a block takes four at
+        // once, and the largest group's ranges end last)
+        const int64_t mean = parts / a.groups, each = recompute || plain ? 64 : 16;
+        sum.ranges = mean < 4 * each ? 1 : (int)std::min<int64_t>(256, mean / each);
         sum.line = (n_all + 3) / 4 * 4;
         if (a.dbias && (sum.ranges > 1 || a.saved))
             sum.sums = ws.take<float>(sum.ranges * a.groups * sum.line);
