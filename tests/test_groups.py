@@ -685,3 +685,155 @@ def test_weight_gradients_over_long_groups(sizes, inputs, outputs):
                "dbias")
     again = torch.autograd.grad(ops.grouped_linear(x, w, g, bias=b), [w, b], dy)
     assert torch.equal(again[0], dw) and torch.equal(again[1], db)
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """Rows whose values start behind the 2^31st, spot-checked."""
+    dt = torch.bfloat16
+    rows, width = 70_000, 40_000
+    x = torch.empty(rows, width, dtype=dt, device="cuda")
+    for at in range(0, rows, 10_000):
+        x[at:at + 10_000] = normal(at, 10_000, width, dtype=dt)
+    g = ops.row_groups(torch.arange(rows, device="cuda", dtype=torch.int32) % 3, 3)
+    xs = ops.to_groups(x, g)
+    some = torch.tensor([0, 1, 2, 54_000, 69_997, 69_998, 69_999], device="cuda")
+    assert torch.equal(xs[g.place.long()[some]], x[some])
+    back = ops.from_groups(xs, g)
+    assert torch.equal(back[some], x[some]) and torch.equal(back[53_680:53_700], x[53_680:53_700])
+    w = torch.full((rows,), 2.0, device="cuda").requires_grad_(True)
+    out = ops.from_groups(xs, g, w)
+    (dw,) = torch.autograd.grad(out, w, back)
+    want = (x[some].double() ** 2).sum(1)
+    assert bool(((dw[some].double() - want).abs() <= (width + 2) * 2.0 ** -24 * want).all())
+    del xs, back, out
+    # and a layer's results
+    rows, outputs = 280_000, 8_192
+    sizes = [100_000, 0, 179_999]
+    g, index = by_sizes(sizes, 1)
+    x, w = normal(141, rows, 64, dtype=dt), normal(142, 3, outputs, 64, dtype=dt, scale=0.1)
+    y = ops.grouped_linear(x, w, g)
+    for r in (0, 99_999, 100_000, 262_144, 279_998):
+        z, err = z64(x[r:r + 1], w[int(index[r])], None)
+        within(y[r:r + 1], *rounded((z, err), U[dt]), "y")
+    assert not bool(y[-1].any())
+
+
+@gpu
+def test_threads_at_once():
+    """Calls from several threads, each on its own stream."""
+    import threading
+
+    dt = torch.bfloat16
+    x = normal(151, 500, 96, dtype=dt)
+    w = normal(152, 5, 160, 96, dtype=dt, scale=0.1)
+    index = choice(153, 500, 2, 5)
+    dy = normal(154, 500, 160, dtype=dt)
+
+    def step():
+        leaf, weight = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        g = ops.row_groups(index, 5)
+        y = ops.from_groups(ops.grouped_linear(ops.to_groups(leaf, g), weight, g,
+                                               activation="silu"), g)
+        return (y, *torch.autograd.grad(y, [leaf, weight], dy))
+
+    want = step()
+    torch.cuda.synchronize()
+    got, errors = [], []
+
+    def run():
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(10):
+                    got.append(step())
+            stream.synchronize()
+        except Exception as e:  # noqa: BLE001 - reported below
+            errors.append(e)
+
+    threads = [threading.Thread(target=run) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors and len(got) == 40
+    for result in got:
+        assert all(torch.equal(a, b) for a, b in zip(result, want))
+
+
+@gpu
+def test_two_graphs_with_one_workspace_each():
+    """Two captured training steps, replayed in turn and on two streams at once."""
+    dt = torch.bfloat16
+    g, _ = by_sizes([130, 70, 0, 300], 5)
+    dy = normal(161, 505, 72, dtype=dt)
+
+    def make(seed):
+        x = normal(seed, 505, 64, dtype=dt).requires_grad_(True)
+        w = normal(seed + 1, 4, 72, 64, dtype=dt, scale=0.1).requires_grad_(True)
+        b = normal(seed + 2, 4, 72, dtype=dt).requires_grad_(True)
+
+        def step():
+            y = ops.grouped_linear(x, w, g, bias=b, activation="gelu")
+            return (y, *torch.autograd.grad(y, [x, w, b], dy))
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(2):
+                step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        return graph, out, [t.detach().clone() for t in step()]
+
+    graphs = [make(seed) for seed in (162, 172)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(4):
+        for (graph, _, _), stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, out, want in graphs:
+            assert all(torch.equal(a.detach(), b) for a, b in zip(out, want))
+    ops.check_waits()
+
+
+@gpu
+@pytest.mark.parametrize("polls", [0, 1, 3, 9, 40])
+def test_waits_that_give_up_in_training_steps(polls):
+    """Every kind of product of a step, among them ones turned round and over ranges of rows: whatever
+    gives up, the next step with the usual bound has the usual bits."""
+    lib = L.load_library()
+    dt = torch.bfloat16
+    g, _ = by_sizes([300, 97, 0, 1200, 513], 4)
+    x = normal(181, 2114, 576, dtype=dt).requires_grad_(True)
+    w0 = normal(182, 5, 512, 576, dtype=dt, scale=0.05).requires_grad_(True)
+    w1 = normal(183, 5, 512, 256, dtype=dt, scale=0.05).requires_grad_(True)
+    dy = normal(184, 2114, 512, dtype=dt)
+
+    def step():
+        h = ops.grouped_gated_linear(x, w0, g)
+        y = ops.grouped_linear(h, w1, g, activation="tanh")
+        z = ops.grouped_linear(y, w0.transpose(1, 2).contiguous(), g)
+        return (z, *torch.autograd.grad([y, z], [x, w0, w1], [dy, torch.ones_like(z)]))
+
+    want = step()
+    torch.cuda.synchronize()
+    try:
+        lib.rune_linear_set_wait_polls(polls)
+        for _ in range(3):
+            try:
+                step()
+            except L.RuneError:
+                pass
+        torch.cuda.synchronize()
+        try:
+            ops.check_waits()
+        except L.RuneError:
+            pass
+    finally:
+        lib.rune_linear_set_wait_polls(L.DEFAULT_WAIT_POLLS)
+    assert all(torch.equal(a, b) for a, b in zip(step(), want))

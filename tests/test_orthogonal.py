@@ -171,3 +171,29 @@ def test_a_wait_that_gives_up_is_reported():
     finally:
         lib.rune_linear_set_wait_polls(L.DEFAULT_WAIT_POLLS)
     assert torch.equal(want, ops.orthogonalize(x))
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """A stack of more than 2^31 values. The last matrix alone may take other tiles: both results are
+    off by a few float16 roundings of values that five steps amplify, and one to bfloat16."""
+    x = torch.empty(530, 2048, 2048, dtype=torch.bfloat16, device="cuda")
+    for at in range(0, 530, 53):
+        x[at:at + 53] = normal(at, 53, 2048, 2048, dtype=torch.bfloat16)
+    got = ops.orthogonalize(x)[-1].double()
+    alone = ops.orthogonalize(x[-1]).double()
+    assert float((got - alone).norm() / alone.norm()) <= 2.0 ** -6
+
+
+@gpu
+def test_captured_and_replayed():
+    x = normal(9, 6, 96, 160, dtype=torch.float32)
+    ops.orthogonalize(x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.orthogonalize(x)
+    for seed in (10, 11):
+        x.copy_(normal(seed, 6, 96, 160, dtype=torch.float32))
+        graph.replay()
+        assert torch.equal(y, ops.orthogonalize(x))
