@@ -497,6 +497,10 @@ void forward(const rune_grouped_linear_args& a, Scratch& ws, cudaStream_t stream
     g.a = readable({a.x, a.rows, a.inputs, a.x_stride}, 2, ws, stream);
     g.w = {readable({a.weight, a.groups * n_all, a.inputs, a.weight_stride}, 2, ws, stream), n_all};
     if (ws.sizing()) return;
+    if (a.rows <= kFewRows) {
+        grouped_few(a, g.a, g.w.all, stream);
+        return;
+    }
     g.k = a.inputs, g.groups = a.groups;
     g.offsets = a.offsets;
     g.device = a.device, g.dtype = a.dtype;

@@ -285,6 +285,8 @@ Matrix readable(Matrix m, int elem_bytes, Scratch& ws, cudaStream_t stream);
 // The rule looks at rows alone: narrow layers of 16 to 48 rows lose by it, up to half.
 constexpr int kFewRows = 48;
 void linear_few(const rune_linear_args& a, const Matrix& x, const Matrix& w, cudaStream_t stream);
+void grouped_few(const rune_grouped_linear_args& a, const Matrix& x, const Matrix& w,
+                 cudaStream_t stream);
 
 // Host-mapped word that a kernel sets when a wait gave up (ops::check_waits reads it).
 unsigned* wait_flag(int device);
