@@ -121,34 +121,35 @@ __device__ __forceinline__ bool maps_here(const MapParams& maps, int ranges) {
     return true;
 }
 
-// sums of the columns of a range of a group's rows: 64 columns a block, four rows at a time
+// sums (p.sums) of the columns of a range of a group's rows: kColumns a block, four rows at a time
 template <typename T>
 __global__ void __launch_bounds__(256)
-k_group_columns(const SumParams p, const __grid_constant__ MapParams maps) {
+k_group_columns(const SumParams p, bool wide, const __grid_constant__ MapParams maps) {
     follow_on();
     if (maps_here(maps, p.ranges)) return;
-    __shared__ float joined[4][64];
-    const int c = threadIdx.x & 63, turn = threadIdx.x >> 6;
-    const int64_t col = (int64_t)blockIdx.x * 64 + c;
+    const int64_t col = (int64_t)blockIdx.x * kColumns + (threadIdx.x & 63) * 4;
+    const int count = (int)max((int64_t)0, min((int64_t)4, p.n - col)), part = threadIdx.x >> 6;
     const int g = blockIdx.y, range = blockIdx.z;
     const int64_t a = min((int64_t)max(p.offsets[g], 0), p.rows);
     const int64_t n = max((int64_t)0, min((int64_t)max(p.offsets[g + 1], 0), p.rows) - a);
     const int64_t r0 = a + n * range / p.ranges, r1 = a + n * (range + 1) / p.ranges;
-    float s = 0.0f;
-    if (col < p.n) {
+    float s[4] = {};
+    auto rows = [&](auto whole) {
         const T* x = static_cast<const T*>(p.x) + col;
 #pragma unroll 8
-        for (int64_t r = r0 + turn; r < r1; r += 4) s += to_float(x[r * p.ld]);
-    }
-    joined[turn][c] = s;
-    __syncthreads();
-    if (turn != 0 || col >= p.n) return;
-    const float sum = joined[0][c] + joined[1][c] + joined[2][c] + joined[3][c];
-    if (p.ranges == 1) static_cast<T*>(p.out)[g * p.n + col] = from_float<T>(sum);
-    else p.sums[((int64_t)range * p.groups + g) * p.line + col] = sum;
+        for (int64_t r = r0 + part; r < r1; r += 4) {
+            float v[4];
+            get4<T, decltype(whole)::value>(x + r * p.ld, count, v);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[j] += v[j];
+        }
+    };
+    if (wide && count == 4) rows(std::true_type());
+    else if (count > 0) rows(std::false_type());
+    join4(s, p.sums + ((int64_t)range * p.groups + g) * p.line + col, count);
 }
 
-// the same of the parts that each group's lines of tiles left
+// sums of a range of the parts that a group's lines of tiles left: 64 columns a block
 template <typename T>
 __global__ void __launch_bounds__(256)
 k_group_sums(const SumParams p, const __grid_constant__ MapParams maps) {
@@ -614,7 +615,7 @@ void backward(const rune_grouped_linear_grad_args& a, Scratch& ws, cudaStream_t 
     if (plain) {
         if (a.dx || a.dweight) dz = readable(dz, 2, ws, stream);
     } else {
-        dz.ld = pad16(n_all, 2);
+        dz.ld = pad_line(n_all, 2);
         dz.p = ws.take<uint16_t>(a.rows * dz.ld);
     }
     if (recompute) {
@@ -634,12 +635,12 @@ void backward(const rune_grouped_linear_grad_args& a, Scratch& ws, cudaStream_t 
         const int64_t parts =
             recompute ? line_bound(a.rows, a.groups, sum.high) * sum.each : a.rows;
         if (recompute) sum.parts = ws.take<float>(parts * n_all);
-        // 64 parts a range where groups are alike, of dz from a saved z 16 rows (a block takes four at
-        // once, and the largest group's ranges end last)
-        const int64_t mean = parts / a.groups, each = recompute || plain ? 64 : 16;
+        // parts or rows of a range where groups are alike: few enough that the largest group's ranges do
+        // not end last, and enough to make up for a block's start
+        const int64_t mean = parts / a.groups, each = recompute ? 64 : plain ? 40 : 16;
         sum.ranges = mean < 4 * each ? 1 : (int)std::min<int64_t>(256, mean / each);
         sum.line = (n_all + 3) / 4 * 4;
-        if (a.dbias && (sum.ranges > 1 || a.saved))
+        if (a.dbias && (sum.ranges > 1 || !recompute))
             sum.sums = ws.take<float>(sum.ranges * a.groups * sum.line);
     }
     Depth depth;
@@ -652,10 +653,10 @@ void backward(const rune_grouped_linear_grad_args& a, Scratch& ws, cudaStream_t 
     auto typed = [&](auto t) {
         using T = decltype(t);
         const unsigned slices = sum.ranges + (a.dweight ? 1 : 0);
+        const bool wide_dy = aligned(a.dy, 8) && a.dy_stride % 4 == 0;
         if (!plain && a.saved) {
             const SavedParams q{a.saved, a.outputs, (a.outputs + 3) / 4 * 4, dz.ld,
-                                const_cast<void*>(dz.p), a.activation,
-                                aligned(a.dy, 8) && a.dy_stride % 4 == 0};
+                                const_cast<void*>(dz.p), a.activation, wide_dy};
             const dim3 grid((unsigned)((a.outputs + kColumns - 1) / kColumns), (unsigned)a.groups,
                             slices);
             if (a.gated)
@@ -663,9 +664,13 @@ void backward(const rune_grouped_linear_grad_args& a, Scratch& ws, cudaStream_t 
             else
                 launch(k_group_act_grad<false, T>, grid, 256, 0, 0, stream, q, sum, depth.maps);
         } else if (a.dbias) {
-            const dim3 grid((unsigned)((n_all + 63) / 64), (unsigned)a.groups, slices);
-            if (plain) launch(k_group_columns<T>, grid, 256, 0, 0, stream, sum, depth.maps);
-            else launch(k_group_sums<T>, grid, 256, 0, 0, stream, sum, depth.maps);
+            const int64_t columns = plain ? kColumns : 64;
+            const dim3 grid((unsigned)((n_all + columns - 1) / columns), (unsigned)a.groups,
+                            slices);
+            if (plain)
+                launch(k_group_columns<T>, grid, 256, 0, 0, stream, sum, wide_dy, depth.maps);
+            else
+                launch(k_group_sums<T>, grid, 256, 0, 0, stream, sum, depth.maps);
         } else if (a.dweight) {
             launch(k_group_maps, (unsigned)((2 * a.groups + kMapWarps - 1) / kMapWarps),
                    32 * kMapWarps, 0, 0, stream, depth.maps);

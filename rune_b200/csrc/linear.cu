@@ -418,7 +418,7 @@ void backward(const rune_linear_grad_args& a, Scratch& ws, cudaStream_t stream) 
             }
         }
     } else {
-        dz.ld = pad16(n_all, 2);
+        dz.ld = pad_line(n_all, 2);
         uint16_t* to = ws.take<uint16_t>(a.rows * dz.ld);
         dz.p = to;
         if (a.saved) {
@@ -567,7 +567,7 @@ Matrix readable(Matrix m, int elem_bytes, Scratch& ws, cudaStream_t stream) {
     if (m.rows == 1) m.ld = pad16(m.cols, elem_bytes);  // no second line to reach
     if (tma_ready(m, elem_bytes)) return m;
     Matrix d = m;
-    d.ld = pad16(m.cols, elem_bytes);
+    d.ld = pad_line(m.cols, elem_bytes);
     void* to = ws.take<char>(m.rows * d.ld * elem_bytes);
     d.p = to;
     if (ws.sizing()) {

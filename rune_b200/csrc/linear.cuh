@@ -267,6 +267,14 @@ inline int64_t pad16(int64_t cols, int elem_bytes) {
     return (cols + v - 1) / v * v;
 }
 
+// Values of a line of scratch that TMA reads: whole 128-byte lines where that adds little. A copied
+// line of a tile that starts off 128 bytes touches two (20 x 1384 x 1778, X X^T: 97 against 68 us).
+inline int64_t pad_line(int64_t cols, int elem_bytes) {
+    if (cols * elem_bytes < 512) return pad16(cols, elem_bytes);
+    const int64_t v = kLineBytes / elem_bytes;
+    return (cols + v - 1) / v * v;
+}
+
 inline bool wide16(const void* p, int64_t ld, int64_t cols) {
     return aligned(p, 16) && ld % 8 == 0 && cols % 8 == 0;
 }

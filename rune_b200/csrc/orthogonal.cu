@@ -625,7 +625,7 @@ int norm_blocks(const rune_orthogonalize_args& a) {
 void orthogonalize(const rune_orthogonalize_args& a, Scratch& ws, cudaStream_t stream) {
     const bool tall = a.rows > a.cols;
     const int64_t small = tall ? a.cols : a.rows;
-    const int64_t ld = pad16(a.cols, 2), lds = pad16(small, 2);
+    const int64_t ld = pad_line(a.cols, 2), lds = pad_line(small, 2);
     NormParams n{};
     n.rows = a.rows, n.cols = a.cols;
     n.step = a.x_step, n.row = a.x_row, n.col = a.x_col;

@@ -289,11 +289,11 @@ void check_norm(const Tensor& x, Tensor& weight, const Tensor& residual) {
 }
 
 // ---------------------------------------------------------------------------------- linear
-// A copy of the rows of t that start on 16 bytes each: a view of a padded buffer.
-Tensor padded(const Tensor& t) {
+// A copy of the rows of t that start on `unit` bytes each: a view of a padded buffer.
+Tensor padded(const Tensor& t, int64_t unit = 16) {
     const Rows r(t);
     const int64_t width = t.size(-1), eb = t.element_size();
-    const int64_t line = (width * eb + 15) / 16 * 16;
+    const int64_t line = (width * eb + unit - 1) / unit * unit;
     Tensor buffer = empty_like_type(t, {r.n, line / eb}, t.scalar_type());
     check(api.pad_rows(t.get_device(), r.n, width * eb, r.ld * eb, r.p(), line, ptr(buffer),
                        stream_of(t)));
@@ -306,7 +306,8 @@ Tensor in_place(const Tensor& t) {
     const int64_t eb = t.element_size();
     const bool ready = t.stride(0) * eb % 16 == 0 && t.stride(0) >= t.size(1) &&
                        reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-    return ready ? t : padded(t);
+    // whole lines of 128 bytes, which the products read faster, where they add little
+    return ready ? t : padded(t, t.size(1) * eb < 512 ? 16 : 128);
 }
 
 struct LinearOut {
