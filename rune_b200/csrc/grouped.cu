@@ -15,6 +15,12 @@
 //                     group has tensor maps of its own, cut to its rows: k_group_maps writes them.
 // z of an activated layer is computed again in the backward pass or read from a float32 copy that the
 // forward saved: the caller's choice, by what each costs.
+//
+// What bounds it (B200): wide layers the tensor cores under the power limit - 32768 x 2048 -> 4096 in
+// 64 groups 452 us, 1.2 PFLOP/s; narrow ones of many rows the epilogue - gated 221184 x 256 -> 2 x 512
+// in 8 groups 134 us forward, 270 dz with recomputed z, 98 dx (5.5 TB/s), 96 + 15 dW; small groups the
+// weights - 8001 rows in 61 groups of 1024 -> 2 x 1408 86 us forward (5.2 TB/s), 73 dx, 88 dW (353 MB
+// written; a write alone takes 92).
 
 #include <cmath>
 
@@ -177,7 +183,7 @@ k_group_sums(const SumParams p, const __grid_constant__ MapParams maps) {
 }
 
 // dz of a range of a group's rows from a saved z, and its columns' sums (in p.sums); p.ld and p.x are
-// of dy
+// of dy. Memory bounds it, and the largest group's last range: 8001 x 2816 in 61 groups 45 us, of 25.
 struct SavedParams {
     const float* z;
     int64_t outputs, ld_part, ld_dz;

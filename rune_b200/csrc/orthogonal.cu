@@ -634,7 +634,7 @@ void orthogonalize(const rune_orthogonalize_args& a, Scratch& ws, cudaStream_t s
     n.eps = a.eps;
     n.x = a.x;
     n.sums = ws.take<double>(a.count * n.blocks);
-    Stack x[2], g{}, h{};
+    Stack x[2]{}, g{}, h{};
     if (a.steps > 0) {
         for (int i = 0; i < (a.steps > 1 ? 2 : 1); ++i)
             x[i] = {ws.take<__half>(a.count * a.rows * ld), a.rows, a.cols, ld, a.rows * ld};

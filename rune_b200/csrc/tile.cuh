@@ -33,7 +33,9 @@ enum Kind {
     kDepthRanges,  // the same in parts: the k-blocks of all groups in equal ranges
     kBatch         // a stack of products
 };
-__host__ __device__ constexpr bool by_depth(int kind) { return kind == kDepthGroups || kind == kDepthRanges; }
+__host__ __device__ constexpr bool by_depth(int kind) {
+    return kind == kDepthGroups || kind == kDepthRanges;
+}
 
 constexpr int kBM = 128;
 constexpr int kEpiWarps = 16, kTmaWarp = 16, kMmaWarp = 17;

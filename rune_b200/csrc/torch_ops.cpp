@@ -707,7 +707,9 @@ struct GroupedFn : torch::autograd::Function<GroupedFn> {
         const bool save = act != RUNE_ACT_NONE &&
                           (inputs > g_recompute_inputs || rows * g_rows_to_inputs < met * inputs);
         LinearOut o = grouped_call(x, weight, bias, offsets, act, gated, save);
-        ctx->save_for_backward({x, weight, bias, offsets, o.z});
+        // the caller's weight and not a view of it made here, where it is read in place
+        const bool own = weight.data_ptr() != weight_.data_ptr();
+        ctx->save_for_backward({x, own ? weight : weight_, bias, offsets, o.z});
         ctx->saved_data["act"] = act;
         ctx->saved_data["gated"] = gated;
         return o.y;
@@ -718,8 +720,8 @@ struct GroupedFn : torch::autograd::Function<GroupedFn> {
     static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
         first_order_only(grads);
         const auto saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &offsets = saved[3];
-        const Tensor& z = saved[4];
+        const Tensor &x = saved[0], &bias = saved[2], &offsets = saved[3], &z = saved[4];
+        const Tensor weight = saved[1].detach().reshape({-1, x.size(1)});
         const Rows rx(x), rw(weight), dy(grads[0]);
         rune_grouped_linear_grad_args a{};
         a.rows = x.size(0), a.inputs = x.size(1), a.groups = offsets.size(0) - 1;

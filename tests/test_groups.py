@@ -837,3 +837,70 @@ def test_waits_that_give_up_in_training_steps(polls):
     finally:
         lib.rune_linear_set_wait_polls(L.DEFAULT_WAIT_POLLS)
     assert all(torch.equal(a, b) for a, b in zip(step(), want))
+
+
+def every_operator(x, w, g, index):
+    return [lambda a: ops.route(a, 2)[1], lambda a: ops.to_groups(a, g),
+            lambda a: ops.from_groups(a, g), lambda a: ops.grouped_linear(a, w, g),
+            lambda a: ops.grouped_linear(x, a[None], g),
+            lambda a: ops.grouped_gated_linear(a, w, g), lambda a: ops.orthogonalize(a)]
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_forward_mode_and_traces_are_refused(device):
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x = torch.ones(16, 16, dtype=torch.bfloat16, device=device)
+    index = torch.zeros(16, dtype=torch.int32, device=device)
+    place = torch.arange(16, dtype=torch.int32, device=device)
+    g = ops.RowGroups(torch.tensor([0, 16], dtype=torch.int32, device=device), place, place)
+    for f in every_operator(x, x[None], g, index):
+        with forward_ad.dual_level(), torch.no_grad(), pytest.raises(RuntimeError,
+                                                                     match="forward-mode"):
+            f(forward_ad.make_dual(x, torch.ones_like(x)))
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(lambda a: f(a + 1), x, check_trace=False)
+        with pytest.raises(RuntimeError, match="traced"):
+            make_fx(lambda a: f(a + 1))(x)
+        with pytest.raises((RuntimeError, ValueError)):
+            torch.func.vmap(f)(x[None])
+    with pytest.raises(RuntimeError, match="traced"):
+        make_fx(lambda i: ops.row_groups(i + 0, 1)[0])(index)
+
+
+@gpu
+def test_transforms_of_a_backward_are_refused_and_checkpoints_work():
+    from torch.autograd import forward_ad
+    from torch.utils.checkpoint import checkpoint
+
+    dt = torch.bfloat16
+    g, _ = by_sizes([20, 0, 41], 3)
+    x = normal(191, 64, 48, dtype=dt).requires_grad_(True)
+    w = normal(192, 3, 48, 48, dtype=dt, scale=0.1).requires_grad_(True)
+    for y in (ops.to_groups(x, g), ops.from_groups(x, g), ops.route(x, 2)[1],
+              ops.grouped_linear(x, w, g, activation="silu")):
+        dy = torch.ones_like(y)
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(y, x, forward_ad.make_dual(dy, dy), retain_graph=True)
+        assert bool(torch.autograd.grad(y, x, dy)[0].isfinite().all())
+
+    def block(a):
+        return ops.from_groups(ops.grouped_linear(ops.to_groups(a, g), w, g, activation="gelu"), g)
+
+    want = torch.autograd.grad(block(x).float().sum(), [x, w])
+    got = torch.autograd.grad(checkpoint(block, x, use_reentrant=False).float().sum(), [x, w])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu
+def test_weights_changed_between_the_passes_are_noticed():
+    dt = torch.bfloat16
+    g, _ = by_sizes([20, 44])
+    x = normal(193, 64, 48, dtype=dt).requires_grad_(True)
+    w = normal(194, 2, 48, 48, dtype=dt).requires_grad_(True)
+    y = ops.grouped_linear(x, w, g, activation="silu")
+    with torch.no_grad():
+        w.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.float().sum().backward()
