@@ -20,7 +20,8 @@ class Muon(torch.optim.Optimizer):
     momentum ``m <- momentum m + g`` (nesterov: of ``g + momentum m``).
 
     params: CUDA parameters of two axes, or more for stacks of matrices (float32, float16 or
-    bfloat16). Those of one shape are orthogonalised in one call.
+    bfloat16). Those of one shape are orthogonalised in one call. The momentum is float32 whatever
+    the parameters are.
     """
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5,
@@ -30,11 +31,24 @@ class Muon(torch.optim.Optimizer):
         super().__init__(params, {"lr": lr, "momentum": momentum, "nesterov": nesterov,
                                   "weight_decay": weight_decay, "steps": steps,
                                   "coefficients": tuple(coefficients), "eps": eps})
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.dim() < 2:
-                    raise ValueError("Muon takes matrices and stacks of them; give vectors to "
-                                     "another optimiser.")
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() < 2:
+                self.param_groups.pop()
+                raise ValueError("Muon takes matrices and stacks of them; give vectors to "
+                                 "another optimiser.")
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # the base class brings states to their parameters' type, which may have fewer bits
+        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
+        params = [p for group in self.param_groups for p in group["params"]]
+        for i, p in zip(ids, params):
+            if i in state_dict["state"]:
+                moment = state_dict["state"][i]["momentum"]
+                self.state[p]["momentum"] = moment.detach().to(p.device, torch.float32, copy=True)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -45,7 +59,7 @@ class Muon(torch.optim.Optimizer):
         for group in self.param_groups:
             alike = {}
             for p in group["params"]:
-                if p.grad is not None:
+                if p.grad is not None and p.numel():
                     alike.setdefault((p.shape[-2:], p.dtype, p.device), []).append(p)
             for params in alike.values():
                 self._update(params, group)
@@ -54,8 +68,9 @@ class Muon(torch.optim.Optimizer):
     def _update(self, params, group):
         for p in params:
             if "momentum" not in self.state[p]:
-                self.state[p]["momentum"] = torch.zeros_like(p.grad)
-        moments, grads = [self.state[p]["momentum"] for p in params], [p.grad for p in params]
+                self.state[p]["momentum"] = torch.zeros_like(p.grad, dtype=torch.float32)
+        moments = [self.state[p]["momentum"] for p in params]
+        grads = [p.grad.float() for p in params]
         torch._foreach_mul_(moments, group["momentum"])
         torch._foreach_add_(moments, grads)
         if group["nesterov"]:

@@ -54,6 +54,28 @@ def test_muon_takes_matrices_alone():
         Muon([torch.nn.Parameter(torch.zeros(4, 4))], lr=-1.0)
 
 
+def test_muon_refuses_vectors_added_later_and_keeps_float32_momentum_when_loaded():
+    p = torch.nn.Parameter(torch.zeros(4, 6, dtype=torch.bfloat16))
+    opt = Muon([p])
+    with pytest.raises(ValueError, match="matrices"):
+        opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(4))]})
+    assert len(opt.param_groups) == 1
+    torch.manual_seed(4)
+    opt.state[p]["momentum"] = torch.randn(4, 6)
+    other = torch.nn.Parameter(p.detach().clone())
+    loaded = Muon([other])
+    loaded.load_state_dict(opt.state_dict())
+    assert loaded.state[other]["momentum"].dtype == torch.float32
+    assert torch.equal(loaded.state[other]["momentum"], opt.state[p]["momentum"])
+    assert loaded.state[other]["momentum"] is not opt.state[p]["momentum"]
+
+
+def test_muon_skips_empty_matrices():
+    p = torch.nn.Parameter(torch.zeros(4, 0))
+    p.grad = torch.zeros(4, 0)
+    Muon([p]).step()
+
+
 # ------------------------------------------------------------------------------------ GPU
 def experts64(net, q, types, choices):
     """Energies in float64 with the given choice of experts in each block."""
@@ -182,6 +204,23 @@ def test_muon_step_is_its_formula():
     kept = params[0].detach().clone()
     opt.step()
     assert torch.equal(kept, params[0])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_muon_holds_the_momentum_of_16_bit_parameters_in_float32(dtype):
+    torch.manual_seed(5)
+    p = torch.nn.Parameter(torch.randn(48, 40, device="cuda").to(dtype))
+    opt = Muon([p], lr=0.1, momentum=0.9, nesterov=False)
+    moment = torch.zeros(48, 40, dtype=torch.float64, device="cuda")
+    for _ in range(8):
+        p.grad = torch.randn_like(p)
+        moment = 0.9 * moment + p.grad.double()
+        opt.step()
+    # three float32 roundings a step (0.9 itself among them) of values below sum |g| < 8 * 6 in size
+    kept = opt.state[p]["momentum"]
+    assert kept.dtype == torch.float32 and bool(p.isfinite().all())
+    assert float((kept.double() - moment).abs().max()) <= 8 * 3 * 2.0 ** -24 * 48
 
 
 @gpu
