@@ -80,7 +80,8 @@ k_group_maps(const __grid_constant__ MapParams p) {
     write_map(p, blockIdx.x * kMapWarps + (threadIdx.x >> 5));
 }
 
-// Number of lines of `high` rows that the groups before g fill (0), and up to g (1) or all (2).
+// Number of lines of `high` rows that the groups before g fill, up to g and all; like the tile
+// kernel's no more than offsets in order lead to, which the parts are sized for.
 struct LineCount {
     int before, with, all;
 };
@@ -92,19 +93,23 @@ __device__ __forceinline__ int group_lines(const int32_t* offsets, int64_t rows,
 __device__ __forceinline__ LineCount count_lines(const int32_t* offsets, int64_t rows, int groups,
                                                  int g, int high) {
     __shared__ int sums[2][32];
+    const int most = (int)most_lines(rows, groups, high);
     int before = 0, all = 0;
     for (int i = threadIdx.x; i < groups; i += blockDim.x) {
         const int n = group_lines(offsets, rows, i, high);
-        all += n;
-        before += i < g ? n : 0;
+        all = min(all + n, most);
+        before = min(before + (i < g ? n : 0), most);
     }
     all = (int)__reduce_add_sync(0xffffffffu, (unsigned)all);
     before = (int)__reduce_add_sync(0xffffffffu, (unsigned)before);
     if ((threadIdx.x & 31) == 0) sums[0][threadIdx.x >> 5] = before, sums[1][threadIdx.x >> 5] = all;
     __syncthreads();
     before = all = 0;
-    for (int w = 0; w < (int)blockDim.x / 32; ++w) before += sums[0][w], all += sums[1][w];
-    return {before, before + group_lines(offsets, rows, g, high), all};
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) {
+        before = min(before + sums[0][w], most);
+        all = min(all + sums[1][w], most);
+    }
+    return {before, min(before + group_lines(offsets, rows, g, high), most), all};
 }
 
 struct SumParams {
@@ -289,10 +294,6 @@ uint32_t table_bytes(int64_t groups) {
     return (uint32_t)((2 * groups + 2) * 4 + 127) / 128 * 128;
 }
 
-int64_t line_bound(int64_t rows, int64_t groups, int high) {
-    return rows / high + std::min(rows, groups);
-}
-
 // Tile and pairing of a product of rows by group, by the time of the whole product's model. Each
 // group that has rows ends inside a line of tiles.
 Plan plan_rows(int64_t rows, int64_t groups, int64_t n_cols, int kblocks, bool gate, bool act,
@@ -439,7 +440,7 @@ int run_rows(const RowProduct& g, TileParams p, bool launch_it, cudaStream_t str
             o2 = make_out_map(static_cast<T*>(p.out) + p.n, p.m_all, p.n, p.ld_out);
     }
     launch_kind<MODE, kRowGroups, T>(plan.pair, a, b, o, o2, p,
-                                     line_bound(p.m_all, g.groups, high) * p.tiles_n, fixed, sms,
+                                     most_lines(p.m_all, g.groups, high) * p.tiles_n, fixed, sms,
                                      g.device, stream);
     return high;
 }
@@ -465,7 +466,7 @@ void run_across(const RowProduct& g, TileParams p, cudaStream_t stream) {
     const CUtensorMap a = g.w.map(g.groups, g.w_mn ? 64 : kBM);
     const CUtensorMap b = make_map(g.a, 2, 16), whole = make_map(g.a, 2, kBM);
     const CUtensorMap o = p.tma_out ? make_out_map(p.out, p.m_all, p.n, p.ld_out) : a;
-    const int64_t work = line_bound(p.m_all, g.groups, 2 * kBM) * p.tiles_n;
+    const int64_t work = most_lines(p.m_all, g.groups, 2 * kBM) * p.tiles_n;
     require(work < (1LL << 31) - 1024, "too many tiles");
     launch_blocks<MODE, kRowsAcross, T, false, true>(a, b, o, whole, p, work, fixed, sms, g.device,
                                                      stream);
@@ -639,7 +640,7 @@ void backward(const rune_grouped_linear_grad_args& a, Scratch& ws, cudaStream_t 
     }
     if (a.dbias || (!plain && a.saved)) {
         const int64_t parts =
-            recompute ? line_bound(a.rows, a.groups, sum.high) * sum.each : a.rows;
+            recompute ? most_lines(a.rows, a.groups, sum.high) * sum.each : a.rows;
         if (recompute) sum.parts = ws.take<float>(parts * n_all);
         // parts or rows of a range where groups are alike: few enough that the largest group's ranges do
         // not end last, and enough to make up for a block's start

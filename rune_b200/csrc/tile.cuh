@@ -141,6 +141,11 @@ __device__ __forceinline__ int rows_across(const Tile& t) {
 // left (gated 221184 x 256 -> 2 x 512, dz: 330 us with 124 bytes spilled).
 __device__ __forceinline__ int uniform(int v) { return (int)__reduce_or_sync(0xffffffffu, (unsigned)v); }
 
+// Lines of `high` rows that groups with offsets in order can fill: each that has rows ends inside one.
+__host__ __device__ constexpr int64_t most_lines(int64_t rows, int64_t groups, int high) {
+    return rows / high + (rows < groups ? rows : groups);
+}
+
 // The tiles of one launch in the order in which a block (or pair) takes them, and the range of k of
 // each. Of groups, whose sizes only the GPU knows, a table in shared memory: rows[g], the groups'
 // first rows, and lines[g], before group g the number of lines of tiles (by rows) or of k-blocks
@@ -188,7 +193,8 @@ struct Schedule {
                 // rows, training 278 -> 270 us); of many groups, whose ranks would take longer, as
                 // they come
                 const int large =
-                    p.groups <= 256 ? (int)(3 * p.m_all / p.groups) : INT32_MAX;
+                    p.groups <= 256 ? (int)min((int64_t)INT32_MAX - 1, 3 * p.m_all / p.groups)
+                                    : INT32_MAX;
                 for (int g = threadIdx.x; g < p.groups; g += kThreads) {
                     const bool mine = rows[g + 1] - rows[g] > large;
                     int rank = large == INT32_MAX ? g : 0;
@@ -204,6 +210,9 @@ struct Schedule {
             } else {
                 if (threadIdx.x < 32) {
                     constexpr int kLine = by_depth(KIND) ? 64 : kTileRows;
+                    // no more than offsets in order lead to, which the grids and the parts
+                    // are sized for
+                    const int most = (int)most_lines(p.m_all, p.groups, kLine);
                     int before = 0;
                     for (int g0 = 0; g0 < p.groups; g0 += 32) {
                         const int g = g0 + threadIdx.x;
@@ -216,8 +225,8 @@ struct Schedule {
                             const int other = __shfl_up_sync(0xffffffffu, sum, o);
                             sum += (int)threadIdx.x >= o ? other : 0;
                         }
-                        if (g < p.groups) lines[g] = before + sum - n;
-                        before += __shfl_sync(0xffffffffu, sum, 31);
+                        if (g < p.groups) lines[g] = min(before + sum - n, most);
+                        before = min(before + __shfl_sync(0xffffffffu, sum, 31), most);
                     }
                     if (threadIdx.x == 0) lines[p.groups] = before;
                 }

@@ -492,6 +492,52 @@ def test_wrong_groups_reach_no_memory():
 
 
 @gpu
+@pytest.mark.parametrize("rows,groups,inputs,outputs", [(600, 64, 64, 96), (20000, 40, 72, 64),
+                                                        (3000, 1024, 16, 8)])
+@pytest.mark.parametrize("gated", [0, 1])
+@pytest.mark.parametrize("saved", [False, True])
+def test_offsets_out_of_order_reach_no_memory(rows, groups, inputs, outputs, gated, saved):
+    """Groups that overlap, each of all rows: more lines of tiles than offsets in order lead to. What
+    lies behind the workspace and the results stays as it was."""
+    lib = L.load_library()
+    dt, guard = torch.bfloat16, 1 << 16
+    n_all = (2 if gated else 1) * outputs
+    x, w = normal(73, rows, inputs, dtype=dt), normal(74, groups, n_all, inputs, dtype=dt)
+    bias, dy = normal(75, groups, n_all, dtype=dt), normal(76, rows, outputs, dtype=dt)
+    offsets = torch.tensor([0, rows] * (groups // 2) + [0], dtype=torch.int32, device="cuda")
+    line = (outputs + 3) // 4 * 4
+    z = normal(77, rows, (2 if gated else 1) * line, dtype=torch.float32)
+
+    def room(size):
+        return torch.full((size + guard,), 0x5A, dtype=torch.uint8, device="cuda")
+
+    def kept(t, size):
+        return bool((t[size:] == 0x5A).all())
+
+    sizes = [2 * rows * inputs, 2 * w.numel(), 2 * bias.numel(), 2 * rows * outputs]
+    dx, dw, db, y = (room(n) for n in sizes)
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    need = ctypes.c_int64(0)
+    common = dict(rows=rows, inputs=inputs, outputs=outputs, groups=groups, x_stride=inputs,
+                  weight_stride=inputs, device=0, dtype=L.RUNE_BF16,
+                  activation=L.RUNE_ACT["silu"], gated=gated, x=x.data_ptr(), weight=w.data_ptr(),
+                  bias=bias.data_ptr(), offsets=offsets.data_ptr())
+    calls = [("grouped_linear", L.GroupedLinearArgs(**common, y=y.data_ptr()), [(y, sizes[3])]),
+             ("grouped_linear_backward", L.GroupedLinearGradArgs(
+                 **common, dy_stride=outputs, dy=dy.data_ptr(), dx=dx.data_ptr(),
+                 dweight=dw.data_ptr(), dbias=db.data_ptr(), saved=z.data_ptr() if saved else None),
+              list(zip((dx, dw, db), sizes)))]
+    for name, args, results in calls:
+        assert getattr(lib, f"rune_{name}_workspace")(ctypes.byref(args), ctypes.byref(need)) == 0
+        ws = room(need.value)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), need.value
+        assert getattr(lib, f"rune_{name}")(ctypes.byref(args), stream) == 0
+        torch.cuda.synchronize()
+        assert kept(ws, need.value), name
+        assert all(kept(t, n) for t, n in results), name
+
+
+@gpu
 def test_refusals():
     dt = torch.bfloat16
     x, w = normal(81, 6, 16, dtype=dt), normal(82, 3, 8, 16, dtype=dt)
