@@ -18,7 +18,7 @@
 //
 // What bounds it (B200): wide layers the tensor cores under the power limit - 32768 x 2048 -> 4096 in
 // 64 groups 452 us, 1.2 PFLOP/s; narrow ones of many rows the epilogue - gated 221184 x 256 -> 2 x 512
-// in 8 groups 134 us forward, 270 dz with recomputed z, 98 dx (5.5 TB/s), 96 + 15 dW; small groups the
+// in 8 groups 121 us forward, 219 dz with recomputed z, 96 dx (5.6 TB/s), 94 + 16 dW; small groups the
 // weights - 8001 rows in 61 groups of 1024 -> 2 x 1408 86 us forward (5.2 TB/s), 73 dx, 88 dW (353 MB
 // written; a write alone takes 92).
 
