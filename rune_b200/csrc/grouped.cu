@@ -245,7 +245,7 @@ k_join_parts(const JoinParams p, const SumParams sum) {
     __shared__ float4 joined[kJoinThreads];
     const int tiles = p.tiles_m * p.tiles_n, g = blockIdx.x / tiles, at = blockIdx.x - g * tiles;
     if (g >= p.groups) {
-        const int64_t block = (int64_t)at * gridDim.y + blockIdx.y;
+        const int64_t block = (int64_t)(blockIdx.x - p.groups * tiles) * gridDim.y + blockIdx.y;
         join_sums<T>(sum, block * kJoinThreads + threadIdx.x);
         return;
     }

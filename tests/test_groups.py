@@ -734,6 +734,14 @@ def test_weight_gradients_over_long_groups(sizes, inputs, outputs):
 
 
 @gpu
+@pytest.mark.parametrize("count,size,inputs,outputs", [(40, 1650, 16, 128), (89, 1500, 35, 30),
+                                                       (32, 2050, 64, 1024)])
+def test_bias_gradients_of_many_long_groups(count, size, inputs, outputs):
+    """More columns of all groups than the weights' tiles have blocks for."""
+    test_weight_gradients_over_long_groups([size + 7 * i for i in range(count)], inputs, outputs)
+
+
+@gpu
 def test_offsets_beyond_32_bits():
     """Rows whose values start behind the 2^31st, spot-checked."""
     dt = torch.bfloat16
