@@ -11,8 +11,10 @@
 //                     group's matrix, since dx contracts over its rows. Or, turned round, tiles of
 //                     outputs by as many rows as there are, which wastes less at the groups' ends.
 //   dW                a product per group over its rows. What lies behind the last row must be
-//                     zeros in both operands (the next group's row may hold an infinity), so each
-//                     group has tensor maps of its own, cut to its rows: k_group_maps writes them.
+//                     zeros in both operands (the next group's row may hold an infinity), so what a
+//                     group has behind its whole blocks of 64 rows is copied to lines of its own
+//                     first (k_group_tails). Tensor maps of each group's rows, written by the GPU,
+//                     would save the copy; tests with them ended in memory faults.
 // z of an activated layer is computed again in the backward pass or read from a float32 copy that the
 // forward saved: the caller's choice, by what each costs.
 //
@@ -36,48 +38,40 @@ constexpr int64_t kMaxSize = INT32_MAX - 512;  // tile coordinates are 32-bit
 constexpr int64_t kMaxGroups = 1024;
 
 // ----------------------------------------------------------------------------- kernels
-// Maps of two matrices' rows [offsets[g], offsets[g + 1]): the whole ones with another address and
-// number of rows. A warp writes one, number `at`, from shared memory.
-struct MapParams {
-    CUtensorMap a, b;
+// The last rows of each group behind its whole blocks of 64, of two matrices: 64 lines a group, zeros
+// behind its end (those that have whole blocks alone are not written, and not read).
+struct TailParams {
     const int32_t* offsets;
     int64_t rows;
-    int groups;
-    const char *start_a, *start_b;
-    int64_t line_a, line_b;  // bytes
-    CUtensorMap* maps;       // [groups][2]; null: none wanted
+    const uint16_t* from[2];
+    uint16_t* to[2];
+    int64_t ld_from[2], cols[2], ld_to[2];
 };
-constexpr int kMapWarps = 8;
-__device__ __forceinline__ void write_map(const MapParams& p, int at) {
-    __shared__ __align__(128) uint32_t copy[kMapWarps][32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = at >> 1;
-    if (g >= p.groups) return;
-    const bool second = at & 1;
+__global__ void __launch_bounds__(256) k_group_tails(const TailParams p) {
+    follow_on();
+    const int g = blockIdx.y, which = blockIdx.z;
     const int64_t first = min((int64_t)max(p.offsets[g], 0), p.rows);
     const int64_t end = min((int64_t)max(p.offsets[g + 1], 0), p.rows);
-    if (first >= end) return;  // nothing to read: no one asks for the map
-    copy[warp][lane] = reinterpret_cast<const uint32_t*>(second ? &p.b : &p.a)[lane];
-    __syncwarp();
-    const uint32_t own = tc::smem_u32(copy[warp]);
-    if (lane == 0) {
-        const char* start = second ? p.start_b + first * p.line_b : p.start_a + first * p.line_a;
-        asm volatile("tensormap.replace.tile.global_address.shared::cta.b1024.b64 [%0], %1;"
-                     ::"r"(own), "l"(start)
-                     : "memory");
-        asm volatile("tensormap.replace.tile.global_dim.shared::cta.b1024.b32 [%0], 1, %1;"
-                     ::"r"(own), "r"((uint32_t)(end - first))
-                     : "memory");
+    const int n = first < end ? (int)((end - first) & 63) : 0;
+    if (n == 0) return;
+    const int64_t ld = p.ld_from[which], cols = p.cols[which], ld_to = p.ld_to[which];
+    const uint16_t* from = p.from[which] + (end - n) * ld;
+    uint16_t* to = p.to[which] + (int64_t)g * 64 * ld_to;
+    const unsigned pieces = (unsigned)(ld_to / 8);
+    for (unsigned i = blockIdx.x * 256 + threadIdx.x; i < 64 * pieces; i += gridDim.x * 256) {
+        const int r = (int)(i / pieces);
+        const int64_t c = (int64_t)(i - r * pieces) * 8;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < n && c + 8 <= cols) {
+            v = *reinterpret_cast<const uint4*>(from + r * ld + c);
+        } else if (r < n) {
+            uint32_t w[4] = {};
+            for (int j = 0; j < 8; ++j)
+                if (c + j < cols) w[j / 2] |= (uint32_t)from[r * ld + c + j] << (j % 2 * 16);
+            v = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        *reinterpret_cast<uint4*>(to + r * ld_to + c) = v;
     }
-    __syncwarp();
-    asm volatile(
-        "tensormap.cp_fenceproxy.global.shared::cta.tensormap::generic.release.gpu.sync.aligned"
-        " [%0], [%1], 128;" ::"l"(p.maps + at), "r"(own)
-        : "memory");
-}
-__global__ void __launch_bounds__(32 * kMapWarps)
-k_group_maps(const __grid_constant__ MapParams p) {
-    follow_on();
-    write_map(p, blockIdx.x * kMapWarps + (threadIdx.x >> 5));
 }
 
 // Number of lines of `high` rows that the groups before g fill, up to g and all; like the tile
@@ -125,19 +119,11 @@ struct SumParams {
     float* sums;             // [ranges][groups][line]
 };
 
-// The last slice of the sums' grids writes the groups' maps, which saves a launch.
-__device__ __forceinline__ bool maps_here(const MapParams& maps, int ranges) {
-    if ((int)blockIdx.z < ranges) return false;
-    write_map(maps, (blockIdx.y * gridDim.x + blockIdx.x) * kMapWarps + (threadIdx.x >> 5));
-    return true;
-}
-
 // sums (p.sums) of the columns of a range of a group's rows: kColumns a block, four rows at a time
 template <typename T>
 __global__ void __launch_bounds__(256)
-k_group_columns(const SumParams p, bool wide, const __grid_constant__ MapParams maps) {
+k_group_columns(const SumParams p, bool wide) {
     follow_on();
-    if (maps_here(maps, p.ranges)) return;
     const int64_t col = (int64_t)blockIdx.x * kColumns + (threadIdx.x & 63) * 4;
     const int count = (int)max((int64_t)0, min((int64_t)4, p.n - col)), part = threadIdx.x >> 6;
     const int g = blockIdx.y, range = blockIdx.z;
@@ -163,9 +149,8 @@ k_group_columns(const SumParams p, bool wide, const __grid_constant__ MapParams 
 // sums of a range of the parts that a group's lines of tiles left: 64 columns a block
 template <typename T>
 __global__ void __launch_bounds__(256)
-k_group_sums(const SumParams p, const __grid_constant__ MapParams maps) {
+k_group_sums(const SumParams p) {
     follow_on();
-    if (maps_here(maps, p.ranges)) return;
     __shared__ float joined[4][64];
     const int c = threadIdx.x & 63, turn = threadIdx.x >> 6;
     const int64_t col = (int64_t)blockIdx.x * 64 + c;
@@ -198,9 +183,8 @@ struct SavedParams {
 };
 template <bool GATED, typename T>
 __global__ void __launch_bounds__(256, 3)
-k_group_act_grad(const SavedParams q, const SumParams p, const __grid_constant__ MapParams maps) {
+k_group_act_grad(const SavedParams q, const SumParams p) {
     follow_on();
-    if (maps_here(maps, p.ranges)) return;
     const int g = blockIdx.y, range = blockIdx.z;
     const int64_t a = min((int64_t)max(p.offsets[g], 0), p.rows);
     const int64_t n = max((int64_t)0, min((int64_t)max(p.offsets[g + 1], 0), p.rows) - a);
@@ -385,13 +369,14 @@ struct Weights {
 template <int MODE, int KIND, typename T>
 void launch_kind(bool pair, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o,
                  const CUtensorMap& o2, const TileParams& p, int64_t work, uint32_t fixed, int sms,
-                 int device, cudaStream_t stream) {
+                 int device, cudaStream_t stream, const CUtensorMap* tail = nullptr) {
     require(work < (1LL << 31) - 1024, "too many tiles");
     if (pair)
-        launch_blocks<MODE, KIND, T, false, true>(a, b, o, o2, p, work, fixed, sms, device, stream);
+        launch_blocks<MODE, KIND, T, false, true>(a, b, o, o2, p, work, fixed, sms, device, stream,
+                                                  tail);
     else
         launch_blocks<MODE, KIND, T, false, false>(a, b, o, o2, p, work, fixed, sms, device,
-                                                   stream);
+                                                   stream, tail);
 }
 
 // Rows of A by group, each with its matrix of w (K-major, or MN-major for dx).
@@ -532,7 +517,7 @@ struct Depth {
     uint32_t fixed = 0;
     int high = 0, tiles_m = 0, tiles_n = 0;
     float* parts = nullptr;
-    MapParams maps{};
+    TailParams tails{};
 };
 
 Depth plan_weights(const rune_grouped_linear_grad_args& a, const Matrix& dz, const Matrix& x,
@@ -544,15 +529,16 @@ Depth plan_weights(const rune_grouped_linear_grad_args& a, const Matrix& dz, con
     d.high = d.plan.pair ? 2 * kBM : kBM;
     d.tiles_m = (int)((m + d.high - 1) / d.high);
     d.tiles_n = (int)((n + d.plan.bn - 1) / d.plan.bn);
-    d.maps.maps = ws.take<CUtensorMap>(2 * a.groups);
+    for (int i = 0; i < 2; ++i) {
+        const Matrix& from = i ? x : dz;
+        d.tails.from[i] = static_cast<const uint16_t*>(from.p), d.tails.ld_from[i] = from.ld;
+        d.tails.cols[i] = from.cols, d.tails.ld_to[i] = pad_line(from.cols, 2);
+        d.tails.to[i] = ws.take<uint16_t>(a.groups * 64 * d.tails.ld_to[i]);
+    }
+    d.tails.offsets = a.offsets, d.tails.rows = a.rows;
     if (d.plan.splits > 1)
         d.parts = ws.take<float>((a.groups + d.plan.splits) * d.tiles_m * d.tiles_n * d.high *
                                  d.plan.bn);
-    if (ws.sizing()) return d;
-    d.maps.a = make_map(dz, 2, 64), d.maps.b = make_map(x, 2, 64);
-    d.maps.offsets = a.offsets, d.maps.rows = a.rows, d.maps.groups = (int)a.groups;
-    d.maps.start_a = static_cast<const char*>(dz.p), d.maps.line_a = dz.ld * 2;
-    d.maps.start_b = static_cast<const char*>(x.p), d.maps.line_b = x.ld * 2;
     return d;
 }
 
@@ -562,12 +548,15 @@ bool run_weights(const rune_grouped_linear_grad_args& a, const Matrix& dz, const
                  const Depth& d, const SumParams& sum, cudaStream_t stream) {
     const int64_t m = dz.cols, n = x.cols, each = (int64_t)d.tiles_m * d.tiles_n;
     const int sms = sm_count(a.device);
-    const CUtensorMap &ma = d.maps.a, &mb = d.maps.b;
+    const CUtensorMap ma = make_map(dz, 2, 64), mb = make_map(x, 2, 64);
+    auto tail = [&](int i) {
+        return make_map({d.tails.to[i], a.groups * 64, d.tails.cols[i], d.tails.ld_to[i]}, 2, 64);
+    };
+    const CUtensorMap ta = tail(0), tb = tail(1);
     TileParams p{};
     p.m = m, p.n = n;
     p.act = RUNE_ACT_NONE;
     p.m_all = a.rows, p.groups = (int)a.groups, p.offsets = a.offsets;
-    p.group_maps = d.maps.maps;
     p.bn = d.plan.bn, p.stages = d.plan.stages, p.splits = 1;
     p.tiles_m = d.tiles_m, p.tiles_n = d.tiles_n;
     p.by_tiles = make_divisor((unsigned)each);
@@ -582,14 +571,14 @@ bool run_weights(const rune_grouped_linear_grad_args& a, const Matrix& dz, const
         p.tma_out = wide16(a.dweight, n, n);
         const CUtensorMap o =
             p.tma_out ? make_out_map3(a.dweight, m, n, n, a.groups, m * n) : ma;
-        launch_kind<kPlain, kDepthGroups, T>(d.plan.pair, ma, mb, o, o, p, each * a.groups, d.fixed,
-                                             sms, a.device, stream);
+        launch_kind<kPlain, kDepthGroups, T>(d.plan.pair, ma, mb, o, ta, p, each * a.groups, d.fixed,
+                                             sms, a.device, stream, &tb);
         return false;
     }
     p.ranges = d.plan.splits;
     p.z = d.parts, p.ld_part = d.high;
-    launch_kind<kPartial, kDepthRanges, __half>(d.plan.pair, ma, mb, ma, ma, p, p.ranges * each,
-                                                d.fixed, sms, a.device, stream);
+    launch_kind<kPartial, kDepthRanges, __half>(d.plan.pair, ma, mb, ma, ta, p, p.ranges * each,
+                                                d.fixed, sms, a.device, stream, &tb);
     // sixteen threads share the parts of a tile where these are many
     const int lanes = p.ranges >= 16 * a.groups ? 16 : 1;
     const JoinParams j{a.offsets, a.rows, m, n, (int)a.groups, d.tiles_m, d.tiles_n, d.high, p.bn,
@@ -659,7 +648,7 @@ void backward(const rune_grouped_linear_grad_args& a, Scratch& ws, cudaStream_t 
     }
     auto typed = [&](auto t) {
         using T = decltype(t);
-        const unsigned slices = sum.ranges + (a.dweight ? 1 : 0);
+        const unsigned slices = sum.ranges;
         const bool wide_dy = aligned(a.dy, 8) && a.dy_stride % 4 == 0;
         if (!plain && a.saved) {
             const SavedParams q{a.saved, a.outputs, (a.outputs + 3) / 4 * 4, dz.ld,
@@ -667,20 +656,23 @@ void backward(const rune_grouped_linear_grad_args& a, Scratch& ws, cudaStream_t 
             const dim3 grid((unsigned)((a.outputs + kColumns - 1) / kColumns), (unsigned)a.groups,
                             slices);
             if (a.gated)
-                launch(k_group_act_grad<true, T>, grid, 256, 0, 0, stream, q, sum, depth.maps);
+                launch(k_group_act_grad<true, T>, grid, 256, 0, 0, stream, q, sum);
             else
-                launch(k_group_act_grad<false, T>, grid, 256, 0, 0, stream, q, sum, depth.maps);
+                launch(k_group_act_grad<false, T>, grid, 256, 0, 0, stream, q, sum);
         } else if (a.dbias) {
             const int64_t columns = plain ? kColumns : 64;
             const dim3 grid((unsigned)((n_all + columns - 1) / columns), (unsigned)a.groups,
                             slices);
             if (plain)
-                launch(k_group_columns<T>, grid, 256, 0, 0, stream, sum, wide_dy, depth.maps);
+                launch(k_group_columns<T>, grid, 256, 0, 0, stream, sum, wide_dy);
             else
-                launch(k_group_sums<T>, grid, 256, 0, 0, stream, sum, depth.maps);
-        } else if (a.dweight) {
-            launch(k_group_maps, (unsigned)((2 * a.groups + kMapWarps - 1) / kMapWarps),
-                   32 * kMapWarps, 0, 0, stream, depth.maps);
+                launch(k_group_sums<T>, grid, 256, 0, 0, stream, sum);
+        }
+        if (a.dweight) {
+            const int64_t wide = std::max(depth.tails.ld_to[0], depth.tails.ld_to[1]) * 8;
+            const dim3 grid((unsigned)std::min<int64_t>((wide + 1023) / 1024, 256),
+                            (unsigned)a.groups, 2);
+            launch(k_group_tails, grid, 256, 0, 0, stream, depth.tails);
         }
         if (a.dx) {
             RowProduct d = g;

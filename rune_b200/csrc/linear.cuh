@@ -179,11 +179,6 @@ __device__ __forceinline__ void bulk_store3(const CUtensorMap* map, uint32_t src
                  : "memory");
 }
 
-// Tensor maps that a kernel before wrote to global memory: before this thread's first use of each.
-__device__ __forceinline__ void map_acquire(const CUtensorMap* map) {
-    asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(map) : "memory");
-}
-
 // the same tile as far as L2
 __device__ __forceinline__ void prefetch_tile(const CUtensorMap* map, int x, int y) {
     asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];"

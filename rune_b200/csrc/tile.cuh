@@ -83,7 +83,6 @@ struct TileParams {
     const int32_t* offsets;
     int64_t m_all, bias_step;
     int groups, zero_tail;  // zero_tail: rows of the output behind the last group are cleared
-    const CUtensorMap* group_maps;  // by depth: of A and B, cut to each group's rows
     int ranges;                     // kDepthRanges
     // batches, and kUpdate
     int64_t in_step, out_step;
@@ -908,7 +907,7 @@ template <int MODE, int KIND, typename T, bool FP8, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
        const __grid_constant__ CUtensorMap map_o, const __grid_constant__ CUtensorMap map_o2,
-       const TileParams p) {
+       const __grid_constant__ CUtensorMap map_t, const TileParams p) {
     using namespace tc;
     extern __shared__ __align__(1024) unsigned char smem[];
     const int b_rows = PAIR ? p.bn / 2 : p.bn;  // of B in this block's stages
@@ -984,10 +983,12 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
             int kb0, kb1;
             plan.range(w, kb0, kb1);
             const int m0 = t.row0;
-            const CUtensorMap *a_map = &map_a, *b_map = &map_b;
+            // by depth: the group's rows, and how many k-blocks of them are whole; what is left of
+            // them lies in lines of its own, zeros behind the group's end
+            int k0 = 0, whole = INT32_MAX;
             if constexpr (by_depth(KIND)) {
-                a_map = p.group_maps + 2 * t.z, b_map = a_map + 1;
-                if (one && kb0 < kb1) map_acquire(a_map), map_acquire(b_map);
+                k0 = uniform(plan.rows[t.z]);
+                whole = (uniform(plan.rows[t.z + 1]) - k0) / 64;
             }
             // first row of B here: a pair's blocks take halves of the tile, gate and up or not
             int n0 = t.nt * bw;
@@ -1000,6 +1001,9 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
                 }
                 const uint32_t bar = full0 + (uint32_t)st * 8;
                 const uint32_t a = smem_u32(smem) + (uint32_t)st * stage_bytes, b = a + kAStage;
+                const bool in = !by_depth(KIND) || kb < whole;
+                const CUtensorMap *a_map = in ? &map_a : &map_o2, *b_map = in ? &map_b : &map_t;
+                const int y = in ? k0 + kb * 64 : t.z * 64;
                 if constexpr (KIND == kRowsAcross) {
                     // this block's outputs of the matrix, and its half of the rows
                     const int f0 = t.nt * 2 * kBM + rank * kBM;
@@ -1025,14 +1029,14 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
                         mbar_expect_tx(smem_u32(&sh->full[st]), (PAIR ? 2 : 1) * stage_bytes);
                     const int x = kb * (FP8 ? 128 : 64);
                     if (p.a_mn) {
-                        load_a(a, a_map, m0, kb * 64, t.z, bar);
-                        load_a(a + kMnChunk, a_map, m0 + 64, kb * 64, t.z, bar);
+                        load_a(a, a_map, m0, y, t.z, bar);
+                        load_a(a + kMnChunk, a_map, m0 + 64, y, t.z, bar);
                     } else {
                         load_a(a, a_map, x, m0, t.z, bar);
                     }
                     if (p.b_mn) {
                         for (int i = 0; i < b_rows / 64; ++i)
-                            load_b(b + i * kMnChunk, b_map, n0 + i * 64, kb * 64, t.z, bar);
+                            load_b(b + i * kMnChunk, b_map, n0 + i * 64, y, t.z, bar);
                     } else {
                         load_b(b, b_map, x, n0, t.z, bar);
                         if (kGate && !PAIR)
@@ -1206,7 +1210,7 @@ int ring_stages(bool pair, int bn, uint32_t fixed) {
 template <int MODE, int KIND, typename T, bool FP8, bool PAIR>
 void launch_blocks(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o,
                    const CUtensorMap& o2, const TileParams& p, int64_t work, uint32_t fixed, int sms,
-                   int device, cudaStream_t stream) {
+                   int device, cudaStream_t stream, const CUtensorMap* tail = nullptr) {
     static std::atomic<uint64_t> allowed{0};  // devices whose limit is raised
     if (device >= 64 || !(allowed.load(std::memory_order_relaxed) >> device & 1)) {
         RUNE_CUDA_TRY(cudaFuncSetAttribute(k_tile<MODE, KIND, T, FP8, PAIR>,
@@ -1219,7 +1223,7 @@ void launch_blocks(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap
                                : (unsigned)std::min<int64_t>(work, sms);
     const size_t smem = (size_t)p.stages * (kAStage + (size_t)b_rows * kLineBytes) + fixed;
     launch(k_tile<MODE, KIND, T, FP8, PAIR>, grid, kThreads, smem, PAIR ? 2 : 0, stream, a, b, o,
-           o2, p);
+           o2, tail ? *tail : a, p);
 }
 
 }  // namespace

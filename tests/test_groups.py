@@ -422,6 +422,14 @@ def test_grouped_layers(sizes, behind, inputs, outputs, dtype, act, with_bias, g
 
 
 @gpu
+@pytest.mark.parametrize("dtype", NARROW, ids=str)
+@pytest.mark.parametrize("gated", [False, True])
+def test_saved_z_in_long_and_short_groups(dtype, gated):
+    """Long groups, an empty one and some of a row or two, with a saved z."""
+    test_grouped_layers([5000, 1, 0, 15, 4001, 2, 2, 2], 3, 1040, 24, dtype, "silu", True, gated)
+
+
+@gpu
 @pytest.mark.parametrize("gated", [False, True])
 def test_grouped_layers_keep_groups_apart(gated):
     """A group's infinities and NaN, and whatever rows in no group hold, stay out of the others."""
@@ -731,6 +739,29 @@ def test_weight_gradients_over_long_groups(sizes, inputs, outputs):
                "dbias")
     again = torch.autograd.grad(ops.grouped_linear(x, w, g, bias=b), [w, b], dy)
     assert torch.equal(again[0], dw) and torch.equal(again[1], db)
+
+
+@gpu
+def test_weight_gradients_keep_to_their_groups_wherever_the_operands_lie():
+    """Operands at other addresses in each pass, and groups of other sizes."""
+    gen = torch.Generator().manual_seed(7)
+    for rows, inputs, outputs, count in ((2000, 64, 283, 31), (700, 72, 520, 5), (900, 1040, 24, 8)):
+        held = []
+        for turn in range(12):
+            index = torch.randint(0, count, (rows,), generator=gen).sort().values.cuda()
+            g = ops.row_groups(index, count)
+            x, w = normal(161, rows, inputs, dtype=torch.float16).requires_grad_(True), \
+                normal(162, count, outputs, inputs, dtype=torch.float16).requires_grad_(True)
+            dy = normal(163, rows, outputs, dtype=torch.float16)
+            dx, dw = torch.autograd.grad(ops.grouped_linear(x, w, g), [x, w], dy)
+            held.append(torch.empty(100_000 + 4096 * turn, dtype=torch.uint8, device="cuda"))
+            for i in range(count):
+                part = index == i
+                d, xs = dy[part].double(), x.detach()[part].double()
+                pairs = products64(d, torch.zeros_like(d), xs, w.detach()[i], 0.0, rows)
+                within(dw[i], *rounded(pairs[1], U[torch.float16]), "dweight")
+        del held
+        torch.cuda.empty_cache()
 
 
 @gpu
