@@ -400,17 +400,18 @@ __device__ __forceinline__ void rows_loaded() {
 }
 // rows x cols (of 32 x 32, zeros beyond) from src into the buffer; there after rows_loaded()
 template <typename T>
-__device__ __forceinline__ void load_rows(const Stage& st, const T* src, int64_t ld, int rows,
-                                          int64_t cols, bool vec) {
+__device__ __forceinline__ void load_rows(const Stage& st, const T* start, const T* src, int64_t ld,
+                                          int rows, int64_t cols, bool vec) {
     if (vec) {
         const int r0 = st.lane >> 2, c = (st.lane & 3) * 8;
         const T* p = src + r0 * ld + c;
         const bool in = c < cols;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const bool some = in && r0 + 8 * i < rows;  // else zeros, and nothing is read
+            // else zeros: nothing is read, and the address is `start`, of the matrix
+            const bool some = in && r0 + 8 * i < rows;
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(st.turn(i)),
-                         "l"(some ? p + i * 8 * ld : src), "r"(some ? 16 : 0)
+                         "l"(some ? p + i * 8 * ld : start), "r"(some ? 16 : 0)
                          : "memory");
         }
     } else {
@@ -609,7 +610,7 @@ __device__ __forceinline__ void epilogue(const TileParams& p, const Tile& t, uin
     auto read_in = [&](int c) {  // residual or dy of the group
         const T* in = static_cast<const T*>(p.in);
         if constexpr (KIND == kBatch) in += t.z * p.in_step;
-        load_rows(st, in + (int64_t)row0 * p.ld_in + col0 + c, p.ld_in, rows, end - c, p.vec_in);
+        load_rows(st, in, in + (int64_t)row0 * p.ld_in + col0 + c, p.ld_in, rows, end - c, p.vec_in);
     };
     // the buffers are free again when the last copy out has read them
     auto reuse = [&] {
