@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(256) k_join_sums(const SumParams p) {
 struct JoinParams {
     const int32_t* offsets;
     int64_t rows, m, n;
-    int groups, tiles_m, tiles_n, high, bn, ranges, lanes;
+    int groups, tiles_m, tiles_n, high, bn, ranges, lanes;  // ranges: planned
     bool wide;         // rows of the output on 8 bytes
     const float* parts;
     void* out;         // [groups][m][n]
@@ -238,8 +238,9 @@ k_join_parts(const JoinParams p, const SumParams sum) {
     // the ranges in which the group's first and last k-blocks lie
     int r0 = 0, r1 = -1;
     if (lines.with > lines.before) {
-        r0 = (int)((((uint64_t)lines.before + 1) * p.ranges - 1) / (unsigned)lines.all);
-        r1 = (int)(((uint64_t)lines.with * p.ranges - 1) / (unsigned)lines.all);
+        const unsigned ranges = range_count(p.ranges, lines.all);
+        r0 = (int)range_at(lines.before, ranges, lines.all);
+        r1 = (int)range_at(lines.with - 1, ranges, lines.all);
     }
     const int each = kJoinThreads / p.lanes;
     const int item = threadIdx.x % each, lane = threadIdx.x / each;

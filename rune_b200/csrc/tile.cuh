@@ -83,7 +83,7 @@ struct TileParams {
     const int32_t* offsets;
     int64_t m_all, bias_step;
     int groups, zero_tail;  // zero_tail: rows of the output behind the last group are cleared
-    int ranges;                     // kDepthRanges
+    int ranges;                     // kDepthRanges: planned
     // batches, and kUpdate
     int64_t in_step, out_step;
     float alpha, beta;
@@ -158,7 +158,15 @@ __host__ __device__ constexpr int64_t most_lines(int64_t rows, int64_t groups, i
 //                  begins with the next range or the next group. Blocks at work at one time have
 //                  the tiles of few ranges, whose operands they share in L2 (110592 x 1024 x 256 in
 //                  8 groups, all tiles one after the other instead: 121 us, so 97). Its counter w is
-//                  k-block * tiles + tile.
+//                  k-block * tiles + tile. Where most rows are in no group there are fewer k-blocks
+//                  than the host planned ranges: range_count() of them, so that none is empty and
+//                  the join finds every part between a group's first and last written.
+__host__ __device__ constexpr unsigned range_count(int planned, unsigned kblocks) {
+    return (unsigned)planned < kblocks ? (unsigned)planned : kblocks;
+}
+__host__ __device__ constexpr unsigned range_at(unsigned x, unsigned ranges, unsigned kblocks) {
+    return (unsigned)((((uint64_t)x + 1) * ranges - 1) / kblocks);  // of k-block x
+}
 template <int KIND, bool PAIR>
 struct Schedule {
     static constexpr int kTileRows = PAIR ? 2 * kBM : kBM;
@@ -168,6 +176,7 @@ struct Schedule {
     int rank;
     unsigned unit, step;     // this block (or pair) among how many
     unsigned begin, end;     // of the counter of work
+    unsigned ranges;         // kDepthRanges
 
     __device__ __forceinline__ Schedule(const TileParams& params, int32_t* table, int r)
         : p(params), rows(table), lines(table + params.groups + 1), rank(r),
@@ -235,6 +244,7 @@ struct Schedule {
                     end = all * p.tiles_n;
                 } else {
                     end = all * tiles;
+                    ranges = range_count(p.ranges, all);
                     begin = item(unit);
                 }
             }
@@ -252,21 +262,19 @@ struct Schedule {
         return uniform(g);
     }
 
-    // kDepthRanges: the range of k-block x, the last that begins at or before it; where range r
-    // begins; and the counter at which item i begins (the end behind the last)
+    // kDepthRanges: the range of k-block x; where range r begins; and the counter at which item i
+    // begins (the end behind the last)
     __device__ __forceinline__ unsigned range_of(unsigned x) const {
-        return (unsigned)((((uint64_t)x + 1) * p.ranges - 1) / (unsigned)uniform(lines[p.groups]));
+        return range_at(x, ranges, (unsigned)uniform(lines[p.groups]));
     }
     __device__ __forceinline__ unsigned start(unsigned r) const {
-        return (unsigned)((uint64_t)(unsigned)uniform(lines[p.groups]) * r / p.ranges);
+        return (unsigned)((uint64_t)(unsigned)uniform(lines[p.groups]) * r / ranges);
     }
     __device__ __forceinline__ unsigned item(unsigned i) const {
         const unsigned tiles = p.by_tiles.by;
-        for (; i < p.ranges * tiles; i += step) {
-            const unsigned r = p.by_tiles.quotient(i), x = start(r);
-            if (x < start(r + 1)) return x * tiles + i - r * tiles;
-        }
-        return end;
+        if (i >= ranges * tiles) return end;
+        const unsigned r = p.by_tiles.quotient(i);
+        return start(r) * tiles + i - r * tiles;
     }
 
     __device__ __forceinline__ unsigned next(unsigned w) const {

@@ -989,3 +989,55 @@ def test_weights_changed_between_the_passes_are_noticed():
         w.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.float().sum().backward()
+
+
+# (rows of each group, rows in none): far fewer lines of rows in groups than blocks share among them
+MOSTLY_NONE = [([1000, 700, 0], 30000, 35, 30), ([64, 65, 200], 30000, 128, 128),
+               ([1124, 61, 802, 937], 26334, 128, 128), ([3000], 27000, 64, 64),
+               ([3327, 4611], 71454, 64, 128), ([0, 0, 130], 40000, 35, 30), ([0, 1], 30000, 64, 64),
+               ([0, 0], 30000, 128, 128)]
+
+
+@gpu
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("sizes,behind,inputs,outputs", MOSTLY_NONE)
+def test_gradients_where_most_rows_are_in_no_group(sizes, behind, inputs, outputs, gated):
+    """A padded batch, or one rank's experts: no gradient depends on what the workspace and the results
+    held before the call, or on what the rows in no group hold."""
+    lib = L.load_library()
+    dt, rows, groups = torch.bfloat16, sum(sizes) + behind, len(sizes)
+    n_all = (2 if gated else 1) * outputs
+    g, _ = by_sizes(sizes, behind)
+    pad = (inputs + 7) // 8 * 8
+    x = normal(201, rows, pad, dtype=dt)
+    w = normal(202, groups, n_all, pad, dtype=dt, scale=inputs ** -0.5)
+    dy = normal(203, rows, outputs, dtype=dt)
+    x[sum(sizes):], dy[sum(sizes):] = float("nan"), float("inf")
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    need = ctypes.c_int64(0)
+    results = []
+    for stale in (0xFF, 0x3C, 0):  # NaN, values near 0.01, zeros
+        dx, dw, db = (torch.full((n,), stale, dtype=torch.uint8, device="cuda").view(dt)
+                      for n in (2 * rows * inputs, 2 * groups * n_all * inputs, 2 * groups * n_all))
+        args = L.GroupedLinearGradArgs(
+            rows=rows, inputs=inputs, outputs=outputs, groups=groups, x_stride=pad,
+            weight_stride=pad, dy_stride=outputs, device=0, dtype=L.RUNE_BF16,
+            activation=L.RUNE_ACT["silu"] if gated else L.RUNE_ACT_NONE, gated=int(gated),
+            x=x.data_ptr(), weight=w.data_ptr(), offsets=g.offsets.data_ptr(), dy=dy.data_ptr(),
+            dx=dx.data_ptr(), dweight=dw.data_ptr(), dbias=db.data_ptr())
+        assert lib.rune_grouped_linear_backward_workspace(ctypes.byref(args), ctypes.byref(need)) == 0
+        ws = torch.full((need.value,), stale, dtype=torch.uint8, device="cuda")
+        args.workspace, args.workspace_bytes = ws.data_ptr(), need.value
+        assert lib.rune_grouped_linear_backward(ctypes.byref(args), stream) == 0
+        results.append([t.clone() for t in (dx, dw, db)])
+    for t in results[0]:
+        assert bool(t.isfinite().all())
+    for other in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(results[0], other))
+
+
+@gpu
+@pytest.mark.parametrize("act,gated", [(None, False), ("tanh", False), ("silu", True)])
+@pytest.mark.parametrize("sizes,behind,inputs,outputs", MOSTLY_NONE)
+def test_layers_where_most_rows_are_in_no_group(sizes, behind, inputs, outputs, act, gated):
+    test_grouped_layers(sizes, behind, inputs, outputs, torch.bfloat16, act, True, gated)
