@@ -63,15 +63,17 @@ class ScalarNetwork(nn.Module):
 
     gated: the blocks' first layer is ``act(x Wg^T + bg) * (x Wu^T + bu)``; ``ffn.0`` then holds
     2 * ffn rows, the gate's first. experts: the blocks are ``ExpertBlock``s of as many networks,
-    ``top_k`` of which each atom takes; 0: none. dtype: torch.bfloat16 or torch.float16, of the
+    ``top_k`` of which each atom takes (default: two, or the one that there is); 0: none. dtype: torch.bfloat16 or torch.float16, of the
     states.
     """
 
     def __init__(self, n_elements, inputs, hidden, ffn, blocks, activation="silu", gated=False,
-                 norm_eps=1.0e-8, dtype=torch.bfloat16, experts=0, top_k=2):
+                 norm_eps=1.0e-8, dtype=torch.bfloat16, experts=0, top_k=None):
         super().__init__()
         if min(n_elements, inputs, hidden, ffn) <= 0 or blocks < 0 or experts < 0:
             raise ValueError("ScalarNetwork dimensions must be positive.")
+        if top_k is None:
+            top_k = min(2, experts)
         if experts and not 1 <= top_k <= min(experts, 32):
             raise ValueError(f"top_k must be 1 to 32 and at most the {experts} experts.")
         if dtype not in (torch.bfloat16, torch.float16):

@@ -36,6 +36,13 @@ def test_dimensions_are_checked():
         ElementNetwork(2, 4, 8, dtype=torch.float32)
 
 
+@pytest.mark.parametrize("experts,top_k", [(1, 1), (2, 2), (7, 2)])
+def test_the_number_of_choices_follows_the_experts(experts, top_k):
+    assert ScalarNetwork(2, 4, 8, 16, 1, experts=experts).residual_blocks[0].top_k == top_k
+    with pytest.raises(ValueError, match="top_k"):
+        ScalarNetwork(2, 4, 8, 16, 1, experts=experts, top_k=experts + 1)
+
+
 def test_from_nep_copies_every_parameter():
     model = nep_model()
     net = ElementNetwork.from_nep(model)
