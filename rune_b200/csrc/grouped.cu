@@ -38,8 +38,8 @@ constexpr int64_t kMaxSize = INT32_MAX - 512;  // tile coordinates are 32-bit
 constexpr int64_t kMaxGroups = 1024;
 
 // ----------------------------------------------------------------------------- kernels
-// The last rows of each group behind its whole blocks of 64, of two matrices: 64 lines a group, zeros
-// behind its end (those that have whole blocks alone are not written, and not read). Memory bounds it:
+// The last rows of each group behind its whole blocks of 64, of two matrices: 64 lines a group that has
+// rows, zeros behind its end (those that have whole blocks alone are not written, and not read). Memory bounds it:
 // 61 groups of 2816 and 1024 columns 16 us, 45 MB.
 struct TailParams {
     const int32_t* offsets;
@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(256) k_group_tails(const TailParams p) {
     if (n == 0) return;
     const int64_t ld = p.ld_from[which], cols = p.cols[which], ld_to = p.ld_to[which];
     const uint16_t* from = p.from[which] + (end - n) * ld;
-    uint16_t* to = p.to[which] + (int64_t)g * 64 * ld_to;
+    uint16_t* to = p.to[which] + (int64_t)tail_place(g, (int)first) * 64 * ld_to;
     const unsigned pieces = (unsigned)(ld_to / 8);
     for (unsigned i = blockIdx.x * 256 + threadIdx.x; i < 64 * pieces; i += gridDim.x * 256) {
         const int r = (int)(i / pieces);
@@ -535,7 +535,7 @@ Depth plan_weights(const rune_grouped_linear_grad_args& a, const Matrix& dz, con
         const Matrix& from = i ? x : dz;
         d.tails.from[i] = static_cast<const uint16_t*>(from.p), d.tails.ld_from[i] = from.ld;
         d.tails.cols[i] = from.cols, d.tails.ld_to[i] = pad_line(from.cols, 2);
-        d.tails.to[i] = ws.take<uint16_t>(a.groups * 64 * d.tails.ld_to[i]);
+        d.tails.to[i] = ws.take<uint16_t>(std::min(a.groups, a.rows) * 64 * d.tails.ld_to[i]);
     }
     d.tails.offsets = a.offsets, d.tails.rows = a.rows;
     if (d.plan.splits > 1)
@@ -552,7 +552,8 @@ bool run_weights(const rune_grouped_linear_grad_args& a, const Matrix& dz, const
     const int sms = sm_count(a.device);
     const CUtensorMap ma = make_map(dz, 2, 64), mb = make_map(x, 2, 64);
     auto tail = [&](int i) {
-        return make_map({d.tails.to[i], a.groups * 64, d.tails.cols[i], d.tails.ld_to[i]}, 2, 64);
+        return make_map({d.tails.to[i], std::min(a.groups, a.rows) * 64, d.tails.cols[i],
+                         d.tails.ld_to[i]}, 2, 64);
     };
     const CUtensorMap ta = tail(0), tb = tail(1);
     TileParams p{};

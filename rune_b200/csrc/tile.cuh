@@ -145,6 +145,11 @@ __host__ __device__ constexpr int64_t most_lines(int64_t rows, int64_t groups, i
     return rows / high + (rows < groups ? rows : groups);
 }
 
+// Place of the lines that hold the last rows of group g (kDepthGroups, kDepthRanges): of groups that have
+// rows both g and the first row grow, so no two have one place, and there are no more places than
+// groups, or rows.
+__device__ __forceinline__ int tail_place(int g, int first) { return min(g, first); }
+
 // The tiles of one launch in the order in which a block (or pair) takes them, and the range of k of
 // each. Of groups, whose sizes only the GPU knows, a table in shared memory: rows[g], the groups'
 // first rows, and lines[g], before group g the number of lines of tiles (by rows) or of k-blocks
@@ -1051,7 +1056,7 @@ k_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
                 const uint32_t a = smem_u32(smem) + (uint32_t)st * stage_bytes, b = a + kAStage;
                 const bool in = !by_depth(KIND) || kb < whole;
                 const CUtensorMap *a_map = in ? &map_a : &map_o2, *b_map = in ? &map_b : &map_t;
-                const int y = in ? k0 + kb * 64 : t.z * 64;
+                const int y = in ? k0 + kb * 64 : tail_place(t.z, k0) * 64;
                 if constexpr (KIND == kRowsAcross) {
                     // this block's outputs of the matrix, and its half of the rows
                     const int f0 = t.nt * 2 * kBM + rank * kBM;

@@ -1041,3 +1041,26 @@ def test_gradients_where_most_rows_are_in_no_group(sizes, behind, inputs, output
 @pytest.mark.parametrize("sizes,behind,inputs,outputs", MOSTLY_NONE)
 def test_layers_where_most_rows_are_in_no_group(sizes, behind, inputs, outputs, act, gated):
     test_grouped_layers(sizes, behind, inputs, outputs, torch.bfloat16, act, True, gated)
+
+
+@gpu
+@pytest.mark.parametrize("sizes", [[0] * 200 + [3, 0, 70, 1] + [0] * 90 + [65],
+                                   [1] * 3 + [0] * 500 + [2, 1] + [0] * 7 + [64, 63]])
+@pytest.mark.parametrize("act,gated", [(None, False), ("silu", True)])
+def test_few_rows_among_many_groups(sizes, act, gated):
+    test_grouped_layers(sizes, 2, 136, 72, torch.bfloat16, act, True, gated)
+
+
+@gpu
+def test_scratch_of_few_rows_does_not_grow_with_the_groups():
+    """10 rows among 1024 groups of 4096 -> 4096: 64 lines of both operands for each of the ten groups
+    that may have rows, a float32 sum of each bias, and less than a MB beside."""
+    lib, need = L.load_library(), ctypes.c_int64(0)
+    rows, groups, width = 10, 1024, 4096
+    some = 1 << 20  # any aligned address: sizes alone are asked
+    args = L.GroupedLinearGradArgs(
+        rows=rows, inputs=width, outputs=width, groups=groups, x_stride=width, weight_stride=width,
+        dy_stride=width, device=0, dtype=L.RUNE_BF16, activation=L.RUNE_ACT_NONE, x=some, weight=some,
+        offsets=some, dy=some, dx=some, dweight=some, dbias=some)
+    assert lib.rune_grouped_linear_backward_workspace(ctypes.byref(args), ctypes.byref(need)) == 0
+    assert need.value <= 2 * rows * 64 * width * 2 + groups * width * 4 + (1 << 20)
