@@ -490,7 +490,8 @@ typedef struct {
     const void* dy;         /* [rows, outputs]; not read behind the last group */
     const float* saved;     /* the forward's z; NULL: recomputed from x, weight and bias */
     void* dx;               /* [rows, inputs], zeros behind the last group; or NULL */
-    void* dweight;          /* [groups, n, inputs], zeros for groups without rows; or NULL */
+    void* dweight;          /* [groups, n, inputs], zeros for groups without rows; or NULL. With it
+                               inputs and n are 2^28 at most */
     void* dbias;            /* [groups, n], or NULL */
     void* workspace;
     int64_t workspace_bytes;

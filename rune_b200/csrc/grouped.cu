@@ -535,6 +535,9 @@ Depth plan_weights(const rune_grouped_linear_grad_args& a, const Matrix& dz, con
         const Matrix& from = i ? x : dz;
         d.tails.from[i] = static_cast<const uint16_t*>(from.p), d.tails.ld_from[i] = from.ld;
         d.tails.cols[i] = from.cols, d.tails.ld_to[i] = pad_line(from.cols, 2);
+        // k_group_tails counts the pieces of 64 lines in 32 bits, and one line is a GB here
+        require(d.tails.ld_to[i] <= 1LL << 28, "inputs or outputs out of range for weight gradients: "
+                                               "2^28 at most");
         d.tails.to[i] = ws.take<uint16_t>(std::min(a.groups, a.rows) * 64 * d.tails.ld_to[i]);
     }
     d.tails.offsets = a.offsets, d.tails.rows = a.rows;

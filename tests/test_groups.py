@@ -1064,3 +1064,21 @@ def test_scratch_of_few_rows_does_not_grow_with_the_groups():
         offsets=some, dy=some, dx=some, dweight=some, dbias=some)
     assert lib.rune_grouped_linear_backward_workspace(ctypes.byref(args), ctypes.byref(need)) == 0
     assert need.value <= 2 * rows * 64 * width * 2 + groups * width * 4 + (1 << 20)
+
+
+@gpu
+@pytest.mark.parametrize("inputs,outputs,gated", [(1 << 29, 1, 0), (64, 1 << 29, 0), (64, 1 << 28, 1),
+                                                  ((1 << 28) + 1, 8, 0)])
+def test_weight_gradients_refuse_lines_that_their_counters_cannot_hold(inputs, outputs, gated):
+    """By the workspace's size, that is before anything is launched; dx alone has no such limit."""
+    lib, need, some = L.load_library(), ctypes.c_int64(0), 1 << 20
+    width = inputs
+    args = L.GroupedLinearGradArgs(
+        rows=1, inputs=inputs, outputs=outputs, groups=1, x_stride=width, weight_stride=width,
+        dy_stride=outputs, device=0, dtype=L.RUNE_BF16, activation=L.RUNE_ACT["silu"], gated=gated,
+        x=some, weight=some, offsets=some, dy=some, dx=some, dweight=some)
+    assert lib.rune_grouped_linear_backward_workspace(ctypes.byref(args), ctypes.byref(need)) \
+        == L.RUNE_ERR_INVALID
+    assert b"weight gradients" in lib.rune_last_error()
+    args.dweight = None
+    assert lib.rune_grouped_linear_backward_workspace(ctypes.byref(args), ctypes.byref(need)) == 0
