@@ -463,7 +463,8 @@ typedef struct {
     int32_t dtype;          /* RUNE_F16 or RUNE_BF16, of all matrices */
     int32_t activation;     /* RUNE_ACT_* */
     int32_t gated;          /* as in rune_linear_args */
-    const void* x;          /* [rows, inputs], sorted by group */
+    const void* x;          /* [rows, inputs], sorted by group. All rows are read, also those
+                               behind the last group, but change no result */
     const void* weight;     /* [groups, n, inputs], n = outputs or 2 outputs; rows weight_stride
                                apart throughout */
     const void* bias;       /* [groups, n] or NULL */
@@ -487,7 +488,8 @@ typedef struct {
     const void* weight;
     const void* bias;
     const int32_t* offsets;
-    const void* dy;         /* [rows, outputs]; not read behind the last group */
+    const void* dy;         /* [rows, outputs]. All rows of x and dy are read, also those behind
+                               the last group, but change no result */
     const float* saved;     /* the forward's z; NULL: recomputed from x, weight and bias */
     void* dx;               /* [rows, inputs], zeros behind the last group; or NULL */
     void* dweight;          /* [groups, n, inputs], zeros for groups without rows; or NULL. With it
