@@ -19,7 +19,7 @@
 // forward saved: the caller's choice, by what each costs.
 //
 // What bounds it (B200): wide layers the tensor cores under the power limit - 32768 x 2048 -> 4096 in
-// 64 groups 452 us, 1.2 PFLOP/s; narrow ones of many rows the epilogue - gated 221184 x 256 -> 2 x 512
+// 64 groups 520 us among other passes, 1.06 PFLOP/s (after a rest 465, 1.18); narrow ones of many rows the epilogue - gated 221184 x 256 -> 2 x 512
 // in 8 groups 135 us forward, 240 dz with recomputed z, 98 dx (5.5 TB/s), 95 + 16 dW; small groups the
 // weights - 8001 rows in 61 groups of 1024 -> 2 x 1408 86 us forward (5.2 TB/s), 73 dx, 83 dW (353 MB
 // written; a write alone takes 92).
@@ -309,10 +309,11 @@ Plan plan_rows(int64_t rows, int64_t groups, int64_t n_cols, int kblocks, bool g
 
 // Whether a product of rows by group is sooner done turned round (kRowsAcross), where the lines that
 // the groups' ends leave part empty count: contractions that hide the epilogue, groups of some rows
-// but not of very many, outputs that fill their tiles. B200, kRowGroups / kRowsAcross, us:
-//   32768 x 2048 -> 4096, 64 groups, gelu 463 / 420    16000 x 512 -> 512, 16 groups 20.5 / 18.4
-//   20000 x 4096 -> 1024, 128 groups      219 / 213    200000 x 1024 -> 256, 8 groups  96 /  98
-//   2000 x 2816 -> 1024, 61 groups         66 /  70    100 x 4096 -> 4096, 16 groups   90 /  98
+// but not of very many, outputs that fill their tiles. B200, pass after pass (under the power limit),
+// kRowGroups / kRowsAcross, us:
+//   32768 x 2048 -> 4096, 64 groups, gelu 555 / 520    16000 x 512 -> 512, 16 groups 15.0 / 12.2
+//   20000 x 4096 -> 1024, 128 groups      300 / 236    200000 x 1024 -> 256, 8 groups  96 /  97
+//   2000 x 2816 -> 1024, 61 groups       61.7 / 65.2   100 x 4096 -> 4096, 16 groups 90.7 / 92.4
 bool across_pays(int64_t rows, int64_t groups, int64_t n, int kblocks) {
     const int64_t met = std::min(rows, groups);
     return kblocks >= 8 && rows >= 96 * met && rows <= 4096 * met &&

@@ -153,7 +153,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 // ----------------------------------------------------------------------------- activations
-// For results that are rounded to 16 bits (2^-9 or 2^-12 relative): few instructions without a
+// For results that are rounded to 16 bits (2^-8 or 2^-11 relative): few instructions without a
 // branch. Values are off by 2e-6 of themselves, at |x| = 10 by 5e-6 (the exponentials' arguments
 // are float32); derivatives by as much of their terms. Exponentials below 2^-126 are 0.
 __device__ __forceinline__ float rcp_fast(float x) {

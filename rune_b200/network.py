@@ -49,6 +49,9 @@ class ExpertBlock(nn.Module):
     def forward(self, x):
         """What the block adds to the stream, of its normalised rows."""
         dtype, experts = x.dtype, self.weight_in.shape[0]
+        # The logits have 16 bits, as every layer's results here: half a step (2^-8 or 2^-11 of a
+        # logit) is within what the rounded rows and weights leave open, experts nearer than that
+        # tie and the first one wins. The softmax over the choices and its gradient are float32.
         index, weights = ops.route(ops.linear(x, self.router.weight.to(dtype)), self.top_k)
         groups = ops.row_groups(index, experts)
         layer = ops.grouped_gated_linear if self.gated else ops.grouped_linear
@@ -63,8 +66,8 @@ class ScalarNetwork(nn.Module):
 
     gated: the blocks' first layer is ``act(x Wg^T + bg) * (x Wu^T + bu)``; ``ffn.0`` then holds
     2 * ffn rows, the gate's first. experts: the blocks are ``ExpertBlock``s of as many networks,
-    ``top_k`` of which each atom takes (default: two, or the one that there is); 0: none. dtype: torch.bfloat16 or torch.float16, of the
-    states.
+    ``top_k`` of which each atom takes (default: two, or the one that there is); 0: none. dtype:
+    torch.bfloat16 or torch.float16, of the states.
     """
 
     def __init__(self, n_elements, inputs, hidden, ffn, blocks, activation="silu", gated=False,

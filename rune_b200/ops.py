@@ -52,9 +52,13 @@ RECOMPUTE_INPUTS = 1024
 
 # A grouped layer also saves z where its groups are small: where ``rows * ROWS_TO_INPUTS`` is less than
 # ``groups * inputs``, reading all groups' weights once more takes longer than z, written and read.
-# B200, training step of gated layers, recomputed / saved, us: 61 groups of 1024 -> 2 x 1408, 2000 rows
-# 284 / 232, 8001 rows 342 / 303, 32000 rows 721 / 670; 32 groups of 512 -> 2 x 512, 4096 rows 68 / 66,
-# 8192 rows 88 / 86, 16384 rows 121 / 131.
+# B200, training step of gated layers, recomputed / saved, us, for groups of like sizes (and of sizes as
+# the softmax of normal numbers):
+#   61 groups of 1024 -> 2 x 1408    2000 rows  298 /  244 (299 / 272)   8001 rows  377 /  329 (373 / 341)
+#                                   16000 rows  543 /  462 (532 / 522)  32000 rows  761 /  767 (821 / 832)
+#                                   64000 rows 1475 / 1584 (1424 / 1516)
+#   32 groups of 512 -> 2 x 512      4096 rows   92 /   88 (74 / 75)     8192 rows   81 /   82 (84 / 88)
+#                                   16384 rows  111 /  123 (115 / 131)
 ROWS_TO_INPUTS = 2
 
 # Coefficients a, b, c of the quintic a x + b x^3 + c x^5 that ``orthogonalize`` iterates: steep at
@@ -260,7 +264,7 @@ def orthogonalize(x, steps=5, coefficients=NEWTON_SCHULZ, eps=1.0e-7):
     """x [..., rows, columns] with its singular values brought near 1, in bfloat16: ``steps`` times
     ``X <- a X + (b A + c A A) X`` with ``A = X X^T``, from ``x / (norm(x) + eps)``.
 
-    For the update of a weight matrix, or of a stack of them. x: float32, float16 or bfloat16. The
+    For the update of a weight matrix, or of a stack of them (at most 65535). x: float32, float16 or bfloat16. The
     products take float16 operands and add in float32: a step rounds X, A and b A + c A A to 11
     bits. Not differentiable.
     """

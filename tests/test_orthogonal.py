@@ -197,3 +197,10 @@ def test_captured_and_replayed():
         x.copy_(normal(seed, 6, 96, 160, dtype=torch.float32))
         graph.replay()
         assert torch.equal(y, ops.orthogonalize(x))
+
+
+@gpu
+def test_the_largest_stack_and_one_more():
+    test_one_step(65535, 2, 3, torch.float32)
+    with pytest.raises(ValueError, match="65535"):
+        ops.orthogonalize(torch.zeros(65536, 2, 3, device="cuda"))
