@@ -1082,3 +1082,62 @@ def test_weight_gradients_refuse_lines_that_their_counters_cannot_hold(inputs, o
     assert b"weight gradients" in lib.rune_last_error()
     args.dweight = None
     assert lib.rune_grouped_linear_backward_workspace(ctypes.byref(args), ctypes.byref(need)) == 0
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ALL, ids=str)
+@pytest.mark.parametrize("width", [1, 33, 64, 520])
+def test_weighted_rows_to_groups_by_the_c_entry(dtype, width):
+    """rune_to_groups with weights, which no operator of ops passes: one product a value, rounded as
+    torch does, whatever lies in rows that have no place."""
+    lib = L.load_library()
+    rows, k = 70, 3
+    g = ops.row_groups(choice(211, rows, k, 9, wrong=0.3), 9)
+    x, w = normal(212, rows, width, dtype=dtype), normal(213, rows, k, dtype=torch.float32)
+    w[g.place < 0] = float("nan")
+    out = torch.full((rows * k, width), float("nan"), dtype=dtype, device="cuda")
+    code = {torch.float32: L.RUNE_F32, torch.float16: L.RUNE_F16, torch.bfloat16: L.RUNE_BF16}
+    args = L.GroupMoveArgs(rows=rows, k=k, width=width, in_stride=width, device=0, dtype=code[dtype],
+                           input=x.data_ptr(), order=g.order.data_ptr(), place=g.place.data_ptr(),
+                           weights=w.data_ptr(), out=out.data_ptr())
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert lib.rune_to_groups(ctypes.byref(args), stream) == 0
+    slot = g.order.long()
+    want = x.float()[slot.clamp(min=0) // k] * w.flatten()[slot.clamp(min=0)][:, None]
+    want = torch.where(slot[:, None] >= 0, want, torch.zeros_like(want)).to(dtype)
+    assert torch.equal(out, want)
+
+
+@gpu
+def test_a_replayed_step_whose_rows_leave_their_groups():
+    """A captured training step of 30000 rows, replayed as all but a few of them lose their group and
+    come back: the bits of the same step run at once, weights' gradients over ranges among them."""
+    dt, rows, count = torch.bfloat16, 30000, 4
+    x = normal(221, rows, 64, dtype=dt).requires_grad_(True)
+    w = normal(222, count, 96, 64, dtype=dt, scale=0.1).requires_grad_(True)
+    b = normal(223, count, 96, dtype=dt).requires_grad_(True)
+    dy = normal(224, rows, 96, dtype=dt)
+    index = choice(225, rows, 0, count)
+    whole = index.clone()
+
+    def step():
+        g = ops.row_groups(index, count)
+        y = ops.from_groups(ops.grouped_linear(ops.to_groups(x, g), w, g, bias=b,
+                                               activation="silu"), g)
+        return (y, *torch.autograd.grad(y, [x, w, b], dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for left in (rows, 1000, 130, 1, 0, 20000):
+        index.copy_(torch.where(torch.arange(rows, device="cuda") < left, whole, -1))
+        graph.replay()
+        got = [t.detach().clone() for t in out]
+        assert all(torch.equal(a, c) for a, c in zip(got, step()))
+        assert left > 0 or not any(bool(t.any()) for t in got)
+    ops.check_waits()
