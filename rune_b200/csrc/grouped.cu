@@ -19,10 +19,10 @@
 // forward saved: the caller's choice, by what each costs.
 //
 // What bounds it (B200): wide layers the tensor cores under the power limit - 32768 x 2048 -> 4096 in
-// 64 groups 520 us among other passes, 1.06 PFLOP/s (after a rest 465, 1.18); narrow ones of many rows the epilogue - gated 221184 x 256 -> 2 x 512
-// in 8 groups 135 us forward, 240 dz with recomputed z, 98 dx (5.5 TB/s), 95 + 16 dW; small groups the
-// weights - 8001 rows in 61 groups of 1024 -> 2 x 1408 86 us forward (5.2 TB/s), 73 dx, 83 dW (353 MB
-// written; a write alone takes 92).
+// 64 groups 520 us among other passes, 1.06 PFLOP/s (after a rest 465, 1.18); narrow ones of many rows
+// the epilogue - gated 221184 x 256 -> 2 x 512 in 8 groups 135 us forward, 240 dz with recomputed z, 98
+// dx (5.5 TB/s), 95 + 16 dW; small groups the weights - 8001 rows in 61 groups of 1024 -> 2 x 1408 86 us
+// forward (5.2 TB/s), 73 dx, 83 dW (353 MB written; a write alone takes 92).
 
 #include <cmath>
 
@@ -39,8 +39,8 @@ constexpr int64_t kMaxGroups = 1024;
 
 // ----------------------------------------------------------------------------- kernels
 // The last rows of each group behind its whole blocks of 64, of two matrices: 64 lines a group that has
-// rows, zeros behind its end (those that have whole blocks alone are not written, and not read). Memory bounds it:
-// 61 groups of 2816 and 1024 columns 16 us, 45 MB.
+// rows, zeros behind its end (those that have whole blocks alone are not written, and not read). Memory
+// bounds it: 61 groups of 2816 and 1024 columns 16 us, 45 MB.
 struct TailParams {
     const int32_t* offsets;
     int64_t rows;
@@ -536,7 +536,7 @@ Depth plan_weights(const rune_grouped_linear_grad_args& a, const Matrix& dz, con
         const Matrix& from = i ? x : dz;
         d.tails.from[i] = static_cast<const uint16_t*>(from.p), d.tails.ld_from[i] = from.ld;
         d.tails.cols[i] = from.cols, d.tails.ld_to[i] = pad_line(from.cols, 2);
-        // k_group_tails counts the pieces of 64 lines in 32 bits, and one line is a GB here
+        // k_group_tails counts the pieces of 64 lines in 32 bits, and one line is half a GB here
         require(d.tails.ld_to[i] <= 1LL << 28, "inputs or outputs out of range for weight gradients: "
                                                "2^28 at most");
         d.tails.to[i] = ws.take<uint16_t>(std::min(a.groups, a.rows) * 64 * d.tails.ld_to[i]);

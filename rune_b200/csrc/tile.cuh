@@ -146,8 +146,8 @@ __host__ __device__ constexpr int64_t most_lines(int64_t rows, int64_t groups, i
 }
 
 // Place of the lines that hold the last rows of group g (kDepthGroups, kDepthRanges): of groups that have
-// rows both g and the first row grow, so no two have one place, and there are no more places than
-// groups, or rows.
+// rows, with offsets in order, both g and the first row grow, so no two have one place; and there are no
+// more places than groups, or rows.
 __device__ __forceinline__ int tail_place(int g, int first) { return min(g, first); }
 
 // The tiles of one launch in the order in which a block (or pair) takes them, and the range of k of

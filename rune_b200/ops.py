@@ -264,9 +264,9 @@ def orthogonalize(x, steps=5, coefficients=NEWTON_SCHULZ, eps=1.0e-7):
     """x [..., rows, columns] with its singular values brought near 1, in bfloat16: ``steps`` times
     ``X <- a X + (b A + c A A) X`` with ``A = X X^T``, from ``x / (norm(x) + eps)``.
 
-    For the update of a weight matrix, or of a stack of them (at most 65535). x: float32, float16 or bfloat16. The
-    products take float16 operands and add in float32: a step rounds X, A and b A + c A A to 11
-    bits. Not differentiable.
+    For the update of a weight matrix, or of a stack of them (at most 65535). x: float32, float16 or
+    bfloat16. The products take float16 operands and add in float32: a step rounds X, A and
+    b A + c A A to 11 bits. Not differentiable.
     """
     a, b, c = coefficients
     return (_BINDING or _native()).orthogonalize(x, steps, a, b, c, eps)
